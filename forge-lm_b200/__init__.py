@@ -24,10 +24,12 @@ import numpy as np
 from . import _native as N
 from ._native import ArgumentError, InvalidDataError, NativeError
 from .dotnet_random import DotNetRandom
+from .serving import QuantKvCache, W4Linear, logit_controls
 
 __all__ = ["ModelConfig", "B200Backend", "Sampler", "DotNetRandom", "ArgumentError", "NativeError",
            "InvalidDataError", "param_names", "param_shapes", "init_params", "device_count", "library_path",
-           "read_forgemodel_header", "write_forgemodel", "BpeTokenizer"]
+           "read_forgemodel_header", "write_forgemodel", "BpeTokenizer", "QuantKvCache",
+           "W4Linear", "logit_controls"]
 
 
 def library_path() -> str:

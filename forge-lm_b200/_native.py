@@ -23,6 +23,13 @@ FB2_INVALID_DATA = -7
 FB2_WEIGHTS_FP32 = 0
 FB2_WEIGHTS_BF16 = 1
 
+FB2_F32 = 0
+FB2_BF16 = 1
+FB2_F16 = 2
+
+FB2_KVQ_INT8 = 0
+FB2_KVQ_INT4 = 1
+
 FB2_RNG_SEEDS = 0
 FB2_RNG_SESSION = 1
 FB2_RNG_UNIFORMS = 2
@@ -38,6 +45,8 @@ EXPORTED = [
     "fb2_forgemodel_read_header", "fb2_model_load_forgemodel", "fb2_forgemodel_write",
     "fb2_tokenizer_load", "fb2_tokenizer_destroy", "fb2_tokenizer_info", "fb2_tokenizer_encode",
     "fb2_tokenizer_decode",
+    "fb2_kvq_sizes", "fb2_kvq_write", "fb2_kvq_read", "fb2_kvq_attend_workspace", "fb2_kvq_attend",
+    "fb2_w4_sizes", "fb2_w4_pack", "fb2_w4_matvec_workspace", "fb2_w4_matvec", "fb2_logit_controls",
 ]
 TEST_EXPORTED = ["fb2_test_expf", "fb2_test_expf_hash", "fb2_test_dotnet_random", "fb2_test_mk_trace",
                  "fb2_test_gemm_tc", "fb2_test_sha256", "fb2_test_mk_withhold", "fb2_test_fail_alloc", "fb2_test_mk_geometry"]
@@ -130,6 +139,18 @@ def load(path: str | None = None):
     L.fb2_tokenizer_info.argtypes = [vp, C.POINTER(i32), C.POINTER(i32)]
     L.fb2_tokenizer_encode.argtypes = [vp, vp, i64, vp, i64, C.POINTER(i64)]
     L.fb2_tokenizer_decode.argtypes = [vp, vp, i64, vp, i64, C.POINTER(i64)]
+    # the serving operators' structs are passed as packed bytes (serving.py)
+    st, i64p = C.c_char_p, C.POINTER(i64)
+    L.fb2_kvq_sizes.argtypes = [st, i64p, i64p]
+    L.fb2_kvq_write.argtypes = [st, i32, vp, vp, i32, i64, i64, i64, i64, vp, vp]
+    L.fb2_kvq_read.argtypes = [st, i32, vp, vp, vp, i32, vp]
+    L.fb2_kvq_attend_workspace.argtypes = [st, st, i64p]
+    L.fb2_kvq_attend.argtypes = [st, st, vp]
+    L.fb2_w4_sizes.argtypes = [st, i64p, i64p]
+    L.fb2_w4_pack.argtypes = [st, vp, i32, i64, vp]
+    L.fb2_w4_matvec_workspace.argtypes = [st, i32, i32, i64p]
+    L.fb2_w4_matvec.argtypes = [st, i32, vp, i64, vp, i64, i32, vp, i64, vp]
+    L.fb2_logit_controls.argtypes = [st, vp]
     for name in EXPORTED + TEST_EXPORTED:
         fn = getattr(L, name)
         if fn.restype is C.c_int:  # default

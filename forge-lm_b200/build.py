@@ -4,7 +4,8 @@ Steps:
   1. gen_expf_fixups (host gcc) -> csrc/generated/expf_fixups.inc: the inputs
      where the host libm expf differs from the correctly rounded exponential
      (the on-device sampler reproduces the host expf bit for bit).
-  2. nvcc -gencode arch=compute_100a,code=sm_100a -> libforge_b200.so.
+  2. nvcc -gencode arch=compute_100a,code=sm_100a: one object per .cu file
+     (in csrc/generated/), linked to libforge_b200.so.
 No fast-math: the sampler's division and exponentials must round as IEEE.
 """
 from __future__ import annotations
@@ -15,10 +16,12 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 GEN = os.path.join(CSRC, "generated")
+OBJ = GEN  # the objects lie with the other generated files
 LIB = os.path.join(HERE, "libforge_b200.so")
 ROOT = os.path.dirname(HERE)
 
@@ -101,6 +104,25 @@ def read_stamp(lib: str = LIB) -> dict:
         return {}
 
 
+def _compile(unit: str, flags: list[str], force: bool, verbose: bool) -> str:
+    """One translation unit's object file, compiled again where the unit or a
+    file it included the last time (nvcc's dependency list) is newer."""
+    obj = os.path.join(OBJ, os.path.basename(unit) + ".o")
+    deps = obj + ".d"
+    try:
+        with open(deps) as f:
+            listed = f.read().replace("\\\n", " ").split(":", 1)[1].split()
+        stale = _newer(obj, [unit] + [d for d in listed if d.startswith(ROOT)])
+    except (OSError, IndexError):
+        stale = True
+    if force or stale:
+        cmd = [_nvcc(), *flags, "-c", "-MD", "-MF", deps, "-o", obj, unit]
+        if verbose:
+            print(" ".join(cmd))
+        subprocess.run(cmd, check=True)
+    return obj
+
+
 def build(verbose: bool = False, force: bool = False) -> str:
     gen_fixups(verbose)
     sources = _sources()
@@ -108,10 +130,11 @@ def build(verbose: bool = False, force: bool = False) -> str:
     same_flags = read_stamp().get("flags") == flags
     if not force and same_flags and not _newer(LIB, sources):
         return LIB
-    cmd = [_nvcc(), *flags, "-shared", "-o", LIB + ".tmp", os.path.join(CSRC, "forge_b200.cu")]
-    if verbose:
-        print(" ".join(cmd))
-    subprocess.run(cmd, check=True)
+    os.makedirs(OBJ, exist_ok=True)
+    units = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith(".cu")]
+    with ThreadPoolExecutor(len(units)) as pool:  # each runs an nvcc of its own
+        objects = list(pool.map(lambda u: _compile(u, flags, force or not same_flags, verbose), units))
+    subprocess.run([_nvcc(), *flags, "-shared", "-o", LIB + ".tmp", *objects], check=True)
     os.replace(LIB + ".tmp", LIB)
     with open(stamp_path(), "w") as f:
         json.dump({"flags": flags, "sources_sha256": source_fingerprint(flags, sources)}, f)

@@ -246,6 +246,184 @@ int32_t fb2_sample_logits(fb2_session* s, int32_t n, const float* logits, const 
 int32_t fb2_forward_last_logits_noalloc(fb2_model* m, int32_t device_slot, int32_t n_tokens,
                                         const int32_t* device_tokens, float* device_logits, void* cuda_stream);
 
+/* ---- serving operators ---------------------------------------------------------
+ * Device-side operators for a host that runs its own decode step (drafting
+ * and verifying several tokens at once, compressed weights and caches).  No
+ * counterpart in the reference, whose decode has fp32 weights, no cache and
+ * one token a step.  Conventions of this block:
+ *   - every pointer named device_* is device memory of the calling thread's
+ *     current CUDA device; cuda_stream is a cudaStream_t of that device
+ *     (NULL: the legacy default stream).  Work is enqueued and the call
+ *     returns without waiting; nothing is allocated and nothing is kept
+ *     between calls;
+ *   - strides count elements; the innermost dimension is contiguous;
+ *   - sizes that are zero make the call a no-op;
+ *   - the host checks shapes, types, alignment and sizes.  Values in device
+ *     memory (slots, page ids, lengths, token ids) are checked by the kernels,
+ *     which skip what is out of range as said at each function. */
+typedef enum { FB2_F32 = 0, FB2_BF16 = 1, FB2_F16 = 2 } fb2_dtype;
+
+/* A paged, quantised K/V cache of one layer in the caller's buffers.
+ *   device_codes: bytes [n_pages][n_kv_heads][2: K, V][page_size][row bytes],
+ *                 16-byte aligned;
+ *   device_meta:  uint32 [n_pages][n_kv_heads][2][page_size], 16-byte aligned.
+ * page_size is a power of two in 8..1024, head_dim a multiple of 16 in 16..256,
+ * n_pages * page_size at most 2^31 - 1.  A slot is page * page_size + offset.
+ *   FB2_KVQ_INT8: row bytes = head_dim; byte = code + 128, code in -127..127;
+ *     meta = bits of the fp32 scale; value = code * scale.
+ *     scale = max|x| / 127, code = round(x * (127 / max|x|)) to nearest even.
+ *   FB2_KVQ_INT4: row bytes = head_dim / 2; dimension 2i is the low nibble of
+ *     byte i, 2i + 1 the high one; meta = bf16 bits scale | minimum << 16;
+ *     value = minimum + scale * code.
+ *     minimum = bf16(min x), scale = bf16((max x - min x) / 15),
+ *     code = round((x - minimum) * (1 / scale)) clamped to 0..15.
+ * Each K or V row of one head has its own meta word.  A row with a non-finite
+ * element (or, for int4, a range or minimum that bf16 cannot hold) is stored
+ * as NaN: whoever reads or attends it sees NaN.  A row whose max|x| (int8) or
+ * scale (int4) is below 1e-35 gets scale 0 and codes 0. */
+typedef enum { FB2_KVQ_INT8 = 0, FB2_KVQ_INT4 = 1 } fb2_kvq_format;
+typedef struct {
+    void* device_codes;
+    void* device_meta;
+    int32_t n_pages;
+    int32_t page_size;
+    int32_t n_kv_heads;
+    int32_t head_dim;
+    int32_t format; /* fb2_kvq_format */
+    int32_t reserved;
+} fb2_kvq_cache;
+
+/* Bytes of the two buffers for these sizes (the pointers are not looked at). */
+int32_t fb2_kvq_sizes(const fb2_kvq_cache* c, int64_t* code_bytes, int64_t* meta_bytes);
+
+/* Quantises n_rows rows of K and V into the cache: row r of every head goes
+ * to slot device_slots[r].  K of row r, head h starts at
+ * device_k + r * k_row_stride + h * k_head_stride.  A slot outside the cache
+ * (negative, say) skips its row; slots of one call are distinct. */
+int32_t fb2_kvq_write(const fb2_kvq_cache* c, int32_t n_rows, const void* device_k, const void* device_v, int32_t dtype,
+                      int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride,
+                      const int32_t* device_slots, void* cuda_stream);
+
+/* Reads n_rows slots back: device_k and device_v [n_rows][n_kv_heads][head_dim]
+ * dense.  A slot outside the cache reads as zeros. */
+int32_t fb2_kvq_read(const fb2_kvq_cache* c, int32_t n_rows, const int32_t* device_slots, void* device_k, void* device_v,
+                     int32_t dtype, void* cuda_stream);
+
+/* Attention of new tokens over the cache.  Sequence b has prefix_lens[b]
+ * cached tokens and the T_b = row_starts[b+1] - row_starts[b] rows of q from
+ * row_starts[b] on; its row i is the token at position prefix_lens[b] + i,
+ * whose K and V the cache holds already (fb2_kvq_write first).  Position p of
+ * sequence b is in page page_table[b * table_stride + p / page_size].
+ * Row i sees every position below prefix_lens[b], and position
+ * prefix_lens[b] + j, j < T_b, where its mask says so: bit j of the row's
+ * mask words (bit j % 32 of word j / 32) for a drafted tree, j <= i where
+ * device_mask is NULL.
+ *   out[r][h] = sum_p softmax_p(scale * q[r][h] . k[p][g]) v[p][g],
+ *   lse[r][h] = log sum_p exp(scale * q . k),  g = h / (n_heads / n_kv_heads).
+ * A row that sees nothing gives out = 0 and lse = -inf.  Positions whose page
+ * id is outside the cache, or that lie past max_pages * page_size or past
+ * max_len, are not seen.  Rows past max_nodes of a sequence and rows outside
+ * every sequence are not written. */
+typedef struct {
+    const void* device_q;  /* [n_rows][n_heads][head_dim], strides below */
+    void* device_out;      /* [n_rows][n_heads][head_dim] dense, q's type */
+    float* device_lse;     /* [n_rows][n_heads], or NULL */
+    const int32_t* device_page_table;  /* [n_seqs][max_pages], rows table_stride apart */
+    const int32_t* device_prefix_lens; /* [n_seqs] */
+    const int32_t* device_row_starts;  /* [n_seqs + 1], or NULL: one row per sequence */
+    const uint32_t* device_mask;       /* [n_rows][mask_words], or NULL */
+    void* device_workspace;            /* fb2_kvq_attend_workspace bytes, 16-byte aligned */
+    int64_t workspace_bytes;
+    int64_t q_row_stride;
+    int64_t q_head_stride;
+    int64_t table_stride;
+    int32_t n_seqs;
+    int32_t n_rows;
+    int32_t n_heads;
+    int32_t dtype;      /* fb2_dtype of q and out */
+    int32_t max_pages;
+    int32_t max_nodes;  /* host bound of T_b */
+    int32_t max_len;    /* host bound of prefix_lens[b] + T_b; 0: max_pages * page_size */
+    int32_t mask_words; /* at least ceil(max_nodes / 32) with a mask */
+    float scale;        /* finite */
+    int32_t reserved;
+} fb2_kvq_attention;
+int32_t fb2_kvq_attend_workspace(const fb2_kvq_cache* c, const fb2_kvq_attention* a, int64_t* bytes);
+int32_t fb2_kvq_attend(const fb2_kvq_cache* c, const fb2_kvq_attention* a, void* cuda_stream);
+
+/* A linear layer y = x W + bias whose W [in][out] is held in 4-bit codes:
+ * W[i][o] = minimum + scale * code, the pair for each output and group of
+ * `group` (32, 64 or 128) consecutive inputs.  Blocks of 16 outputs x 64
+ * inputs, padded up:
+ *   device_codes: uint32 [ceil(out/16)][ceil(in/64)][32][4], 16-byte aligned;
+ *     nibble p (bits 4p..) of word j of lane 4g + t is output 8 (p & 1) + g
+ *     and input 16 t + 4 j + (p & 2) + (p >> 2) of its block;
+ *   device_meta:  uint32 [ceil(out/16)][ceil(in/group)][16], 16-byte aligned:
+ *     bf16 bits scale | minimum << 16.
+ * Padding may hold anything. */
+typedef struct {
+    const void* device_codes;
+    const void* device_meta;
+    const float* device_bias; /* [out], or NULL */
+    int32_t in_features;
+    int32_t out_features;
+    int32_t group;
+    int32_t reserved;
+} fb2_w4_linear;
+int32_t fb2_w4_sizes(const fb2_w4_linear* w, int64_t* code_bytes, int64_t* meta_bytes);
+
+/* Packs W [in][out] (dtype; row stride w_row_stride elements): per group
+ * minimum = bf16(min w), scale = bf16((max w - min w) / 15),
+ * code = round((w - minimum) * (1 / scale)) clamped to 0..15; a scale below
+ * 1e-35 gives scale 0 and codes 0, a group with a non-finite weight NaN.
+ * codes and meta are written (the struct's bias is not looked at). */
+int32_t fb2_w4_pack(const fb2_w4_linear* w, const void* device_w, int32_t dtype, int64_t w_row_stride, void* cuda_stream);
+
+/* y[n_rows][out] = x[n_rows][in] W + bias, products exact and sums in fp32,
+ * rounded once to dtype.  Rows of x and y are x_row_stride / y_row_stride
+ * elements apart.  A row of x with a non-finite element gives a non-finite
+ * row of y.  device_workspace: fb2_w4_matvec_workspace bytes, 16-byte aligned. */
+int32_t fb2_w4_matvec_workspace(const fb2_w4_linear* w, int32_t n_rows, int32_t dtype, int64_t* bytes);
+int32_t fb2_w4_matvec(const fb2_w4_linear* w, int32_t n_rows, const void* device_x, int64_t x_row_stride, void* device_y,
+                      int64_t y_row_stride, int32_t dtype, void* device_workspace, int64_t workspace_bytes,
+                      void* cuda_stream);
+
+/* Controls on logit rows, in this order, in fp32 and rounded once to dtype:
+ *   c = how often id v is among the row's tokens (ids outside the vocabulary
+ *       count nowhere);
+ *   c > 0: l = l < 0 ? l * repetition : l / repetition (Sampler.cs:111-129),
+ *          l = l - presence - frequency * c;
+ *   l = l + bias of v (listed at most once per row; of several the last counts);
+ *   l = -inf where the row's grammar mask does not allow v (bit v % 32 of word
+ *       v / 32; 1 allows), whatever l was.
+ * A row whose mask allows nothing is all -inf.  Each control is left out where
+ * its pointer is NULL.  device_out may be device_logits. */
+typedef struct {
+    const void* device_logits; /* [n_rows][vocab], rows logits_row_stride apart */
+    void* device_out;          /* rows out_row_stride apart, same type */
+    const int32_t* device_tokens;       /* the rows' windows back to back */
+    const int32_t* device_token_starts; /* [n_rows + 1] */
+    const float* device_repetition;     /* [n_rows] */
+    const float* device_presence;       /* [n_rows] */
+    const float* device_frequency;      /* [n_rows] */
+    const int32_t* device_bias_ids;
+    const float* device_bias_values;
+    const int32_t* device_bias_starts;  /* [n_rows + 1] */
+    const uint32_t* device_allowed;     /* [n_masks][mask_words] */
+    const int32_t* device_mask_rows;    /* [n_rows] mask of each row, outside 0..n_masks-1: none; NULL: mask r */
+    int64_t logits_row_stride;
+    int64_t out_row_stride;
+    int64_t n_tokens;  /* entries of device_tokens: starts beyond it are cut to it */
+    int64_t n_biases;  /* entries of the bias lists, likewise */
+    int32_t n_rows;
+    int32_t vocab;
+    int32_t dtype;
+    int32_t n_masks;
+    int32_t mask_words; /* at least ceil(vocab / 32) with masks */
+    int32_t reserved;
+} fb2_logit_control;
+int32_t fb2_logit_controls(const fb2_logit_control* c, void* cuda_stream);
+
 /* ---- synthetic weights -------------------------------------------------------
  * Host-only: fills params[i] (caller-allocated fp32 arrays of the sizes listed
  * at fb2_model_create) with the weights `new GptModel(config, backend,

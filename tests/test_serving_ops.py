@@ -1,0 +1,808 @@
+"""The serving operators (quantised K/V cache, attention over it, 4-bit linear
+layers, logit controls) against plain 64-bit implementations, at the sizes and
+masks where they can go wrong, and their refusals."""
+from __future__ import annotations
+
+import math
+import random
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+gpu = pytest.mark.gpu
+DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def within(got, want, tol):
+    """Whether every value is the rounding, in its own type, of something at
+    most tol from want (fp64): rounding is monotonic, so it lies between the
+    roundings of the ends."""
+    got, want = got.cpu(), want.cpu()
+    low, high = (want - tol).to(got.dtype), (want + tol).to(got.dtype)
+    return bool(((got >= low) & (got <= high)).all())
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def normal(g, *shape, dtype=torch.float32):
+    return torch.randn(shape, device="cuda", generator=g).to(dtype)
+
+
+def decode(cache):
+    """fp64 (k, v) [slots, kv heads, head_dim] that the buffers stand for."""
+    codes, meta = cache.codes.cpu().numpy(), cache.meta.cpu().numpy()
+    if cache.fmt == "int8":
+        scale = meta.view(np.float32).astype(np.float64)
+        x = (codes.astype(np.float64) - 128) * scale[..., None]
+    else:
+        code = np.stack([codes & 15, codes >> 4], -1).reshape(codes.shape[:-1] + (-1,)).astype(np.float64)
+        scale = (meta << 16).view(np.float32).astype(np.float64)
+        least = (meta & -65536).view(np.float32).astype(np.float64)
+        x = least[..., None] + scale[..., None] * code
+    both = torch.from_numpy(x).permute(2, 0, 3, 1, 4).flatten(1, 2)  # [2][pages*size][heads][dim]
+    return both[0], both[1]
+
+
+def filled(pkg, g, pages, page, heads, dim, fmt):
+    cache = pkg.QuantKvCache.empty(pages, page, heads, dim, fmt)
+    slots = torch.arange(pages * page, dtype=torch.int32, device="cuda")
+    cache.write(normal(g, pages * page, heads, dim), normal(g, pages * page, heads, dim), slots)
+    return cache
+
+
+# ---- the cache ------------------------------------------------------------------
+
+def check_rows(fmt, x, codes, meta):
+    """One side's stored rows against the formats' definition in 64 bits:
+    x fp64 [rows, heads, dim], codes and meta as stored."""
+    if fmt == "int8":
+        scale = meta.view(np.float32).astype(np.float64)
+        top = np.abs(x).max(-1)
+        # one fp32 division
+        assert (np.abs(scale - top / 127) <= 2.0 ** -23 * top / 127).all()
+        want = 127 * x / top[..., None]
+        # the factor and the product are rounded once each: below 2 * 127 * 2^-24 off a code
+        assert (np.abs(codes.astype(np.float64) - 128 - want) <= 0.5 + 2e-5).all()
+    else:
+        scale = (meta << 16).view(np.float32).astype(np.float64)
+        least = (meta & -65536).view(np.float32).astype(np.float64)
+        low, span = x.min(-1), x.max(-1) - x.min(-1)
+        assert (np.abs(least - low) <= 2.0 ** -8 * np.abs(low)).all()
+        assert (np.abs(scale - span / 15) <= 2.0 ** -8 * span / 15).all()
+        code = np.stack([codes & 15, codes >> 4], -1).reshape(x.shape).astype(np.float64)
+        want = np.clip((x - least[..., None]) / scale[..., None], 0, 15)
+        assert (np.abs(code - want) <= 0.5 + 2e-5).all()
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("rows,heads,dim,page", [(1, 1, 16, 8), (3, 12, 64, 16), (37, 5, 80, 32), (130, 8, 128, 64),
+                                                  (17, 2, 256, 1024), (9, 3, 48, 8)])
+def test_write_stores_the_rows_and_nothing_else(pkg, fmt, dtype, rows, heads, dim, page):
+    g = gen(rows + dim)
+    pages = -(-2 * rows // page) + 1
+    cache = pkg.QuantKvCache.empty(pages, page, heads, dim, fmt)
+    cache.codes.random_(0, 256, generator=g)
+    cache.meta.random_(0, 1 << 30, generator=g)
+    before = cache.codes.clone(), cache.meta.clone()
+    slots = torch.randperm(pages * page, device="cuda", generator=g)[:rows].to(torch.int32)
+    k, v = normal(g, rows, heads, dim, dtype=DTYPES[dtype]), 3 * normal(g, rows, heads, dim, dtype=DTYPES[dtype])
+    cache.write(k, v, slots)
+    at = slots.long()
+    codes = cache.codes.permute(2, 0, 3, 1, 4).flatten(1, 2)
+    meta = cache.meta.permute(2, 0, 3, 1).flatten(1, 2)
+    for kind, x in enumerate((k, v)):
+        check_rows(fmt, x.double().cpu().numpy(), codes[kind][at].cpu().numpy(), meta[kind][at].cpu().numpy())
+    others = torch.ones(pages * page, dtype=torch.bool, device="cuda")
+    others[at] = False
+    assert torch.equal(codes[:, others], before[0].permute(2, 0, 3, 1, 4).flatten(1, 2)[:, others])
+    assert torch.equal(meta[:, others], before[1].permute(2, 0, 3, 1).flatten(1, 2)[:, others])
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("rows,heads,dim,page", [(1, 1, 16, 8), (5, 12, 64, 16), (131, 5, 80, 32), (40, 8, 128, 64),
+                                                  (17, 2, 256, 1024)])
+def test_read_gives_the_stored_values(pkg, fmt, dtype, rows, heads, dim, page):
+    g = gen(7)
+    pages = -(-rows // page) + 2
+    cache = filled(pkg, g, pages, page, heads, dim, fmt)
+    slots = torch.randint(0, pages * page, (rows,), device="cuda", generator=g).to(torch.int32)
+    slots[rows // 2] = -1 if rows > 1 else slots[0]
+    if rows > 4:
+        slots[3] = pages * page
+    k, v = cache.read(slots, DTYPES[dtype])
+    wk, wv = decode(cache)
+    for got, want in ((k, wk), (v, wv)):
+        want = want[slots.long().cpu().clamp(0, pages * page - 1)]
+        want[(slots.cpu() < 0) | (slots.cpu() >= pages * page)] = 0
+        # one fp32 rounding, then the type's
+        assert got.dtype == DTYPES[dtype] and torch.equal(got.cpu(), want.float().to(DTYPES[dtype]))
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+def test_write_of_strided_unaligned_and_skipped_rows(pkg, fmt):
+    g = gen(3)
+    heads, dim, rows = 4, 32, 21
+    cache = pkg.QuantKvCache.empty(4, 16, heads, dim, fmt)
+    dense = pkg.QuantKvCache.empty(4, 16, heads, dim, fmt)
+    base = normal(g, rows, 3 * heads * dim + 1)
+    k = base[:, 1:1 + heads * dim].unflatten(1, (heads, dim))                    # not 16-byte aligned
+    v = base[:, 1 + heads * dim:1 + 2 * heads * dim].unflatten(1, (dim, heads)).transpose(1, 2)  # wrong last stride
+    slots = torch.arange(rows, dtype=torch.int32, device="cuda") * 3
+    slots[4], slots[9], slots[20] = -1, 64, 2 ** 31 - 1
+    with pytest.raises(pkg.ArgumentError):
+        cache.write(k, v, slots)
+    v = base[:, :heads * dim].unflatten(1, (heads, dim)).flip(0)
+    cache.write(k, v, slots)
+    keep = (slots >= 0) & (slots < 64)
+    dense.write(k.contiguous()[keep], v.contiguous()[keep], slots[keep].contiguous())
+    assert torch.equal(cache.codes, dense.codes) and torch.equal(cache.meta, dense.meta)
+    one = normal(g, 1, 1, dim).expand(rows, heads, dim)  # one row for every head and token
+    cache.write(one, one, slots)
+    k2, _ = cache.read(slots[:1].contiguous())
+    assert torch.equal(k2[0, 0], k2[0, 3])
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+@pytest.mark.parametrize("dim", [16, 80, 128])
+def test_write_of_special_rows(pkg, fmt, dim):
+    inf, nan = math.inf, math.nan
+    rows = torch.randn((9, dim), generator=torch.Generator().manual_seed(1))
+    rows[0] = 0.0
+    rows[1] = 2.5                  # a constant
+    rows[2, dim - 1] = inf
+    rows[3, 3] = -inf
+    rows[4, 0] = nan
+    rows[5] *= 1e-40               # below every scale that can be held
+    rows[6] *= 1e30
+    rows[7] = -0.0
+    rows[8] = nan
+    x = rows[:, None].cuda()
+    cache = pkg.QuantKvCache.empty(2, 8, 1, dim, fmt)
+    slots = torch.arange(9, dtype=torch.int32, device="cuda")
+    cache.write(x, x.flip(2).contiguous(), slots)
+    k, v = (t[:, 0].double().cpu() for t in cache.read(slots))
+    for t in (k, v):
+        assert (t[0] == 0).all() and (t[7] == 0).all()
+        assert (t[1] == 2.5).all()
+        assert t[2].isnan().all() and t[3].isnan().all() and t[4].isnan().all() and t[8].isnan().all()
+        assert (t[5].abs() <= 1e-35).all()
+    span = rows[6].double().max() - rows[6].double().min()
+    step = rows[6].double().abs().max() / 127 if fmt == "int8" else span / 15
+    # half a step, and for int4 the bf16 roundings of scale (15 codes) and minimum
+    more = 0 if fmt == "int8" else (15 * step + rows[6].double().abs().max()) * 2.0 ** -8
+    assert ((k[6] - rows[6].double()).abs() <= 0.501 * step + more).all()
+
+
+# ---- attention --------------------------------------------------------------------
+
+def plain_attention(cache, q, table, prefix, starts, bits, scale, max_len=None):
+    """fp64 (out, lse) by the definition; bits: per row the set of drafted
+    tokens it sees, or None for the causal order."""
+    k, v = decode(cache)
+    q = q.double().cpu()
+    rows, heads, dim = q.shape
+    out = torch.zeros((rows, heads, dim), dtype=torch.float64)
+    lse = torch.full((rows, heads), -math.inf, dtype=torch.float64)
+    share = heads // cache.n_kv_heads
+    table = table.cpu()
+    cap = table.shape[1] * cache.page_size
+    for b in range(len(prefix)):
+        for r in range(starts[b], starts[b + 1]):
+            i = r - starts[b]
+            seen = list(range(prefix[b])) + [prefix[b] + j for j in range(starts[b + 1] - starts[b])
+                                             if (j <= i if bits is None else j in bits[r])]
+            seen = [p for p in seen if p < cap and (max_len is None or p < max_len)]
+            pages = [int(table[b, p // cache.page_size]) for p in seen]
+            slots = [pg * cache.page_size + p % cache.page_size for pg, p in zip(pages, seen)
+                     if 0 <= pg < cache.n_pages]
+            if not slots:
+                continue
+            for h in range(heads):
+                s = (k[slots, h // share] @ q[r, h]) * scale
+                lse[r, h] = torch.logsumexp(s, 0)
+                out[r, h] = torch.softmax(s, 0) @ v[slots, h // share]
+    return out, lse
+
+
+def check_attention(dtype, got, want, big, scores):
+    """big: largest |v|; scores: largest |score|.  fp32: a score is off by a few
+    roundings of its size (sums of up to 256 products, the scale's and the
+    exponential's), which moves out by that times the values' spread; every
+    product and sum after it by 2^-24 and the accumulations by less than
+    2^-20 of the largest value.  The type's rounding comes on top."""
+    out, lse = got
+    tol = (8 * 2.0 ** -23 * (scores + 4) + 2.0 ** -20) * big
+    if dtype != "fp32":
+        tol += 2.0 ** -11 * big  # probabilities may be carried in 11 bits
+    assert torch.isfinite(out).all()
+    assert within(out, want[0], tol), float((out.double().cpu() - want[0]).abs().max())
+    empty = want[1] == -math.inf
+    assert torch.equal(lse.cpu() == -math.inf, empty)
+    assert (out.cpu()[empty] == 0).all()
+    off = (lse.double().cpu() - want[1])[~empty].abs()
+    assert off.numel() == 0 or float(off.max()) <= 8 * 2.0 ** -23 * (scores + 16)
+
+
+def attention_case(pkg, seed, fmt, dtype, prefix, nodes, heads, kv_heads, dim, page, tree, spare=3, scale=None,
+                   wide_table=0, max_len=None):
+    g, rnd = gen(seed), random.Random(seed)
+    lens = [p + t for p, t in zip(prefix, nodes)]
+    need = [-(-n // page) for n in lens]
+    pages = sum(need) + spare
+    cache = filled(pkg, g, pages, page, kv_heads, dim, fmt)
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(seed)).tolist()
+    table = torch.full((len(lens), max(need + [1]) + wide_table), -1, dtype=torch.int32)
+    used = torch.zeros(pages * page, dtype=torch.bool)
+    at = 0
+    for b, n in enumerate(need):
+        mine = order[at:at + n]
+        table[b, :n] = torch.tensor(mine, dtype=torch.int32)
+        for p in range(lens[b]):
+            used[mine[p // page] * page + p % page] = True
+        at += n
+    # what no row sees must not count: NaN scales and other codes there
+    hidden = ~used.view(pages, page).cuda()
+    meta = cache.meta.permute(0, 3, 1, 2)
+    meta[hidden] = torch.tensor(0x7FC07FC0, dtype=torch.int32, device="cuda")
+    cache.codes.permute(0, 3, 1, 2, 4)[hidden] = 255
+    clean = pkg.QuantKvCache(cache.codes, cache.meta, dim, fmt)
+    starts = [0]
+    for t in nodes:
+        starts.append(starts[-1] + t)
+    q = (2 * normal(g, starts[-1], heads, dim)).to(DTYPES[dtype])
+    bits = mask = None
+    if tree:
+        words = (max(nodes) + 31) // 32
+        bits, flat = [], []
+        for b, t in enumerate(nodes):
+            seen = []
+            for i in range(t):
+                up = seen[rnd.randrange(i)] if i and rnd.random() < 0.9 else set()
+                seen.append(up | {i})
+            if t > 2:
+                seen[t - 1] = set()  # sees nothing drafted, not even itself
+            bits += seen
+        for s in bits:
+            flat.append([sum(1 << (j - 32 * w) for j in s if 32 * w <= j < 32 * w + 32) for w in range(words)])
+        mask = torch.tensor(flat, dtype=torch.int64).reshape(-1, words).to(torch.int32).cuda()
+    got = clean.attend(q, table.cuda(), torch.tensor(prefix, dtype=torch.int32, device="cuda"),
+                       starts=torch.tensor(starts, dtype=torch.int32, device="cuda"), mask=mask, scale=scale,
+                       max_nodes=max(nodes), max_len=max_len)
+    s = scale if scale is not None else 1 / math.sqrt(dim)
+    want = plain_attention(clean, q, table, prefix, starts, bits, s, max_len)
+    k, v = cache.read(torch.arange(pages * page, dtype=torch.int32, device="cuda")[used.cuda()])
+    top = float(v.abs().max()) if v.numel() else 1.0
+    scores = float(q.float().norm(dim=2).max() * k.norm(dim=2).max() * abs(s)) if k.numel() else 1.0
+    check_attention(dtype, got, want, top, scores)
+    return got
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(1, 1, 16, 8), (12, 12, 64, 16), (8, 1, 64, 32), (14, 2, 80, 8),
+                                                      (32, 8, 128, 64), (4, 4, 256, 16), (15, 5, 32, 1024),
+                                                      (3, 1, 112, 16), (17, 1, 192, 8)])
+def test_attention_of_single_tokens(pkg, fmt, dtype, heads, kv_heads, dim, page):
+    prefix = [0, 1, 7, 15, 16, 31, 32, 33, 63, 64, 100, 257]
+    attention_case(pkg, dim, fmt, dtype, prefix, [1] * len(prefix), heads, kv_heads, dim, page, tree=False)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(2, 2, 16, 8), (12, 12, 64, 16), (8, 2, 128, 32), (7, 1, 64, 64),
+                                                      (5, 5, 80, 8), (4, 1, 256, 16)])
+def test_attention_of_drafted_trees(pkg, fmt, dtype, heads, kv_heads, dim, page):
+    attention_case(pkg, dim + 1, fmt, dtype, [0, 5, 64, 200, 31, 0], [9, 64, 1, 33, 17, 3], heads, kv_heads, dim, page,
+                   tree=True)
+
+
+@gpu
+@pytest.mark.parametrize("fmt,dtype", [("int8", "fp32"), ("int4", "bf16"), ("int8", "bf16"), ("int4", "fp32")])
+def test_attention_of_long_rows_in_causal_order(pkg, fmt, dtype):
+    attention_case(pkg, 11, fmt, dtype, [0, 130, 3], [75, 1, 130], 6, 2, 64, 16, tree=False)
+
+
+@gpu
+@pytest.mark.parametrize("fmt,dtype", [("int8", "fp32"), ("int4", "fp16"), ("int8", "bf16")])
+@pytest.mark.parametrize("nodes", [1, 40])
+def test_attention_over_long_caches(pkg, fmt, dtype, nodes):
+    """Lengths at which one sequence is split over many blocks."""
+    attention_case(pkg, 5, fmt, dtype, [9000, 2047, 4500], [nodes, max(1, nodes // 3), nodes], 4, 2, 64, 32,
+                   tree=nodes > 1, wide_table=700)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_attention_with_more_mask_words_than_one(pkg, dtype):
+    attention_case(pkg, 21, "int8", dtype, [70, 0], [100, 129], 4, 4, 64, 16, tree=True)
+
+
+@gpu
+def test_attention_rows_that_see_nothing(pkg):
+    g = gen(1)
+    cache = filled(pkg, g, 4, 16, 2, 64, "int8")
+    q = normal(g, 3, 4, 64)
+    table = torch.tensor([[0, 1], [-1, -1], [7, 3]], dtype=torch.int32, device="cuda")
+    prefix = torch.tensor([0, 20, 16], dtype=torch.int32, device="cuda")
+    starts = torch.arange(4, dtype=torch.int32, device="cuda")
+    mask = torch.zeros((3, 1), dtype=torch.int32, device="cuda")
+    out, lse = cache.attend(q, table, prefix, starts=starts, mask=mask, max_nodes=1)
+    # row 0: an empty mask and no prefix; row 1: no pages; row 2: its prefix's page is not in the cache
+    assert (out == 0).all() and (lse == -math.inf).all()
+    mask[2] = 1
+    out, lse = cache.attend(q, table, prefix, starts=starts, mask=mask, max_nodes=1)
+    _, v = cache.read(torch.tensor([48], dtype=torch.int32, device="cuda"))
+    assert (out[:2] == 0).all()
+    want = v[0].repeat_interleave(2, 0)
+    assert ((out[2] - want).abs() <= 2.0 ** -21 * want.abs().max()).all() and torch.isfinite(lse[2]).all()
+
+
+@gpu
+def test_attention_of_masked_and_seen_nan(pkg):
+    """A NaN row of the cache reaches the rows that see it and no others."""
+    g = gen(2)
+    heads, dim = 2, 64
+    for fmt in ("int8", "int4"):
+        for dtype in (torch.float32, torch.bfloat16):
+            for kind in (0, 1):
+                cache = filled(pkg, g, 4, 16, heads, dim, fmt)
+                table = torch.tensor([[2, 0, 1]], dtype=torch.int32, device="cuda")
+                x = normal(g, 1, heads, dim)
+                bad = x.clone()
+                bad[:, 1] = math.nan
+                cache.write(bad if kind == 0 else x, bad if kind == 1 else x,
+                            torch.tensor([2 * 16 + 11], dtype=torch.int32, device="cuda"))
+                mask = torch.tensor([[1], [0b10], [0b101]], dtype=torch.int32, device="cuda")
+                out, _ = cache.attend(normal(g, 3, heads, dim, dtype=dtype), table,
+                                      torch.tensor([10], dtype=torch.int32, device="cuda"),
+                                      starts=torch.tensor([0, 3], dtype=torch.int32, device="cuda"), mask=mask, max_nodes=3)
+                assert torch.isfinite(out[[0, 2]]).all() and torch.isfinite(out[1, 0]).all()
+                assert out[1, 1].isnan().all()
+
+
+@gpu
+@pytest.mark.parametrize("size", [1e-30, 1e-6, 1e4, 1e30])
+def test_attention_of_large_and_small_values(pkg, size):
+    g = gen(4)
+    cache = pkg.QuantKvCache.empty(8, 16, 2, 64, "int8")
+    slots = torch.arange(128, dtype=torch.int32, device="cuda")
+    spread = torch.logspace(-3, 0, 128, device="cuda")[:, None, None]
+    cache.write(normal(g, 128, 2, 64) / size, normal(g, 128, 2, 64) * size * spread, slots)
+    table = torch.arange(8, dtype=torch.int32, device="cuda")[None]
+    q = normal(g, 1, 4, 64) * size
+    prefix = torch.tensor([121], dtype=torch.int32, device="cuda")
+    got = cache.attend(q, table, prefix)
+    want = plain_attention(cache, q, table, [121], [0, 1], None, 0.125)
+    k, v = decode(cache)
+    check_attention("fp32", (got[0] / size, got[1]), (want[0] / size, want[1]), float(v.abs().max()) / size,
+                    float(q.double().norm(dim=2).max().cpu() * k.norm(dim=2).max()) / 8)
+
+
+@gpu
+def test_attention_of_strided_queries_on_another_stream(pkg):
+    g = gen(6)
+    heads, dim = 6, 64
+    cache = filled(pkg, g, 12, 16, 2, dim, "int8")
+    table = torch.randperm(12, device="cuda", generator=g)[None].to(torch.int32)
+    qkv = normal(g, 5, heads * dim * 3 + 3)
+    q = qkv[:, 3:3 + heads * dim].unflatten(1, (heads, dim))
+    prefix = torch.tensor([150], dtype=torch.int32, device="cuda")
+    starts = torch.tensor([0, 5], dtype=torch.int32, device="cuda")
+    want = cache.attend(q.contiguous(), table, prefix, starts=starts, max_nodes=5)
+    turned = q.transpose(0, 1).contiguous().transpose(0, 1)  # heads outermost
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = cache.attend(q, table, prefix, starts=starts, max_nodes=5)
+        other = cache.attend(turned, table.expand(1, 12), prefix, starts=starts, max_nodes=5, max_len=155)
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    assert ((other[0] - want[0]).abs() <= 2.0 ** -20 * want[0].abs().max()).all()
+    again = cache.attend(q.contiguous(), table, prefix, starts=starts, max_nodes=5)
+    assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])  # the same bits each time
+
+
+@gpu
+def test_attention_bounds_that_cut(pkg):
+    """max_len and the page table's width cut what is seen; max_nodes which rows are written."""
+    attention_case(pkg, 31, "int8", "fp32", [100, 40], [1, 1], 4, 2, 64, 16, tree=False, max_len=77)
+    g = gen(8)
+    cache = filled(pkg, g, 8, 16, 2, 64, "int8")
+    table = torch.arange(3, dtype=torch.int32, device="cuda")[None]
+    q = normal(g, 1, 4, 64)
+    got = cache.attend(q, table, torch.tensor([500], dtype=torch.int32, device="cuda"))
+    want = plain_attention(cache, q, table, [500], [0, 1], None, 0.125)
+    check_attention("fp32", got, want, 5.0, 20.0)
+    low = cache.attend(q, table, torch.tensor([-5], dtype=torch.int32, device="cuda"))
+    none = cache.attend(q, table, torch.tensor([0], dtype=torch.int32, device="cuda"))
+    assert torch.equal(low[0], none[0])
+
+
+@gpu
+def test_cache_past_32_bit_offsets(pkg):
+    """5 GB of codes: byte and row offsets past 2^32."""
+    pages, page, dim = 10000, 1024, 256
+    codes = torch.empty((pages, 1, 2, page, dim), dtype=torch.uint8, device="cuda")
+    meta = torch.zeros((pages, 1, 2, page), dtype=torch.int32, device="cuda")
+    cache = pkg.QuantKvCache(codes, meta, dim, "int8")
+    g = gen(9)
+    slots = torch.arange((pages - 1) * page - 40, (pages - 1) * page + 60, dtype=torch.int32, device="cuda")
+    k, v = normal(g, 100, 1, dim), normal(g, 100, 1, dim)
+    small = pkg.QuantKvCache.empty(2, page, 1, dim)
+    cache.write(k, v, slots)
+    small.write(k, v, torch.arange(page - 40, page + 60, dtype=torch.int32, device="cuda"))
+    for a, b in zip(cache.read(slots), small.read(torch.arange(page - 40, page + 60, dtype=torch.int32, device="cuda"))):
+        assert torch.equal(a, b)
+    codes[pages - 2, :, :, :page - 40] = 128
+    small.codes[0, :, :, :page - 40] = 128
+    q = normal(g, 1, 2, dim)
+    prefix = torch.tensor([page + 59], dtype=torch.int32, device="cuda")
+    got = cache.attend(q, torch.tensor([[pages - 2, pages - 1]], dtype=torch.int32, device="cuda"), prefix)
+    want = small.attend(q, torch.tensor([[0, 1]], dtype=torch.int32, device="cuda"), prefix)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# ---- 4-bit linear layers --------------------------------------------------------------
+
+def unpack(linear):
+    """fp64 W [in][out] that the packed buffers stand for."""
+    k, n, group = linear.in_features, linear.out_features, linear.group
+    codes, meta = linear.codes.cpu().numpy(), linear.meta.cpu().numpy()
+    w = np.empty((k, n))
+    i, o = np.meshgrid(np.arange(k), np.arange(n), indexing="ij")
+    lane = 4 * (o % 8) + i % 64 // 16
+    nibble = (o % 16) // 8 + (i & 2) + 4 * (i & 1)
+    code = (codes[o // 16, i // 64, lane, i % 16 // 4] >> (4 * nibble)) & 15
+    m = meta[o // 16, i // group, o % 16]
+    return (m & -65536).view(np.float32).astype(np.float64) + (m << 16).view(np.float32).astype(np.float64) * code
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("k,n,group", [(64, 16, 64), (100, 77, 32), (32, 1, 32), (1, 40, 128), (300, 130, 128), (256, 64, 64)])
+def test_pack_of_weights(pkg, dtype, k, n, group):
+    g = gen(k)
+    w = (0.02 * normal(g, k, n)).to(DTYPES[dtype])
+    w[0, 0] = 0.5
+    linear = pkg.W4Linear.pack(w, group)
+    got, want = unpack(linear), w.double().cpu().numpy()
+    for a in range(0, k, group):
+        part = want[a:a + group]
+        span = part.max(0) - part.min(0)
+        # half a step, plus the bf16 roundings of scale (over 15 codes) and minimum
+        most = span / 15 * (0.5 + 1e-3) + 2.0 ** -8 * (span + np.abs(part.min(0)))
+        assert (np.abs(got[a:a + group] - part) <= most).all()
+
+
+@gpu
+def test_pack_of_special_weights(pkg):
+    w = torch.randn((64, 20), generator=torch.Generator().manual_seed(5)).cuda()
+    w[:, 3] = 0.25
+    w[7, 5] = math.nan
+    w[9, 6] = math.inf
+    w[:, 8] = 1e-40
+    wide = torch.zeros((64, 33), device="cuda")
+    wide[:, 5:25] = w
+    linear = pkg.W4Linear.pack(wide[:, 5:25], 32)
+    got = unpack(linear)
+    assert (got[:, 3] == 0.25).all() and np.isnan(got[:32, 5]).all() and np.isnan(got[:32, 6]).all()
+    assert np.isfinite(got[32:, 5]).all() and (np.abs(got[:, 8]) < 1e-35).all()
+    y = linear(torch.randn((3, 64), device="cuda"))
+    assert y[:, [5, 6]].isnan().all() and torch.isfinite(y[:, [i for i in range(20) if i not in (5, 6)]]).all()
+
+
+def random_linear(pkg, g, k, n, group, bias):
+    blocks, groups = -(-n // 16), -(-k // group)
+    codes = torch.randint(-2 ** 31, 2 ** 31, (blocks, -(-k // 64), 32, 4), device="cuda", generator=g).to(torch.int32)
+    scale = 0.01 + 0.02 * torch.rand((blocks, groups, 16), device="cuda", generator=g)
+    least = -7.0 * scale + 0.02 * torch.randn((blocks, groups, 16), device="cuda", generator=g)
+    pair = torch.stack((scale, least), -1).to(torch.bfloat16).view(torch.int32).squeeze(-1).contiguous()
+    # padded outputs' scales are not looked at
+    pad = torch.arange(blocks * 16, device="cuda").view(blocks, 1, 16) >= n
+    pair[pad.expand_as(pair)] = 0x7FC07FC0
+    return pkg.W4Linear(codes, pair, k, n, group, bias=normal(g, n) if bias else None)
+
+
+def check_product(pkg, dtype, rows, k, n, group, bias=True, strided=False):
+    g = gen(rows * 7 + k + n)
+    linear = random_linear(pkg, g, k, n, group, bias)
+    x = normal(g, rows, k + (5 if strided else 0), dtype=DTYPES[dtype])
+    if strided:
+        x = x[:, 5:]
+    y = linear(x)
+    w, xd = unpack(linear), x.double().cpu().numpy()
+    want = xd @ w + (linear.bias.double().cpu().numpy() if bias else 0)
+    # fp32 sums of code * x and of x: their terms' sizes bound the roundings
+    # (pairwise over at least 16, at most k / 16 + 16 in a row)
+    m = linear.meta.cpu().numpy()
+    step = (m << 16).view(np.float32).astype(np.float64)[:, :, :].transpose(0, 2, 1).reshape(-1, m.shape[1])[:n]
+    low = np.abs((m & -65536).view(np.float32).astype(np.float64)).transpose(0, 2, 1).reshape(-1, m.shape[1])[:n]
+    grp = np.arange(k) // group
+    size = np.abs(xd) @ (15 * step + low)[:, grp].T + np.abs(want)
+    tol = 2.0 ** -24 * (k / 16 + 16) ** 0.5 * 4 * size
+    assert y.dtype == DTYPES[dtype] and within(y, torch.from_numpy(want), torch.from_numpy(tol))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("rows,k,n", [(1, 64, 16), (1, 768, 2304), (1, 1, 1), (2, 100, 77), (3, 300, 130), (8, 1000, 33),
+                                       (5, 2000, 50), (9, 192, 100), (17, 640, 48), (33, 96, 200), (64, 1024, 70),
+                                       (100, 130, 40), (1, 5000, 16)])
+def test_products_with_4_bit_weights(pkg, dtype, group, rows, k, n):
+    check_product(pkg, dtype, rows, k, n, group)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("rows,k,n", [(1, 333, 64), (7, 128, 48), (40, 515, 19)])
+def test_products_of_unaligned_rows(pkg, dtype, rows, k, n):
+    check_product(pkg, dtype, rows, k, n, 64, bias=False, strided=True)
+
+
+@gpu
+def test_products_of_special_rows_and_shapes(pkg):
+    g = gen(12)
+    linear = random_linear(pkg, g, 200, 40, 32, True)
+    x = normal(g, 6, 200)
+    want = linear(x)
+    x[1, 7], x[2, 199], x[4] = math.inf, math.nan, 0.0
+    got = linear(x)
+    assert torch.equal(got[[0, 3, 5]], want[[0, 3, 5]]) and not torch.isfinite(got[[1, 2]]).any()
+    assert torch.equal(got[4], linear.bias)
+    assert linear(x[:0]).shape == (0, 40)
+    assert torch.equal(linear(x.view(2, 3, 200)).nan_to_num(), got.view(2, 3, 40).nan_to_num())
+    assert torch.equal(linear(x[0]), got[0])
+    assert torch.equal(linear(x[[0, 3]]), linear(x[[0, 3]]))  # the same bits each time
+    plain = pkg.W4Linear(linear.codes, linear.meta, 200, 40, 32)
+    small, large = plain(x[[0, 3]] * 2.0 ** -80), plain(x[[0, 3]] * 2.0 ** 80)
+    base = plain(x[[0, 3]])
+    assert torch.equal(small * 2.0 ** 80, base) and torch.equal(large * 2.0 ** -80, base)
+
+
+# ---- logit controls -----------------------------------------------------------------------
+
+def plain_controls(logits, windows=None, rep=None, pres=None, freq=None, biases=None, allowed=None, mask_rows=None):
+    out = logits.double().cpu().clone()
+    rows, vocab = out.shape
+    for r in range(rows):
+        if windows is not None:
+            for t in set(windows[r]):
+                if not 0 <= t < vocab:
+                    continue
+                x = float(out[r, t])
+                if rep is not None:
+                    x = x * float(rep[r]) if x < 0 else x / float(rep[r])
+                x -= (float(pres[r]) if pres is not None else 0) + (float(freq[r]) if freq is not None else 0) * windows[r].count(t)
+                out[r, t] = x
+        if biases is not None:
+            for t, b in dict(biases[r]).items():
+                if 0 <= t < vocab:
+                    out[r, t] += b
+        if allowed is not None:
+            m = r if mask_rows is None else mask_rows[r]
+            if 0 <= m < len(allowed):
+                bits = (allowed[m].cpu().long()[:, None] >> torch.arange(32)) & 1
+                out[r, bits.flatten()[:vocab] == 0] = -math.inf
+    return out
+
+
+def lists(rows, kind):
+    flat = [x for r in rows for x in r]
+    starts = np.concatenate([[0], np.cumsum([len(r) for r in rows])])
+    return torch.tensor(flat, dtype=kind, device="cuda"), torch.tensor(starts, dtype=torch.int32, device="cuda")
+
+
+def check_controls(got, want):
+    # four fp32 operations on values below `size`, then the type's rounding
+    assert torch.equal(torch.isfinite(got.cpu()), torch.isfinite(want))
+    fine = torch.isfinite(want)
+    assert (got.cpu()[~fine] == -math.inf).all()
+    assert within(got.cpu()[fine], want[fine], 2.0 ** -22 * (want[fine].abs() + 40))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (1, 16384), (3, 1003), (2, 4096), (4, 4097), (2, 131071), (5, 33)])
+def test_controls_on_logits(pkg, dtype, rows, vocab):
+    rnd = random.Random(vocab)
+    g = gen(vocab)
+    logits = (5 * normal(g, rows, vocab)).to(DTYPES[dtype])
+    windows = [[rnd.randrange(-2, min(vocab + 3, 300)) for _ in range(rnd.randrange(0, 700))] + [vocab - 1, vocab, 2 ** 31 - 1]
+               for _ in range(rows)]
+    windows[0] = windows[0] * 2
+    if rows > 2:
+        windows[2] = []
+    biases = [[(rnd.randrange(-1, vocab + 1), rnd.uniform(-3, 3)) for _ in range(rnd.randrange(0, 50))] for _ in range(rows)]
+    biases[0] = biases[0] + [(0, 1.5), (0, -2.5)]  # the last of an id's biases counts
+    biases = [[(t, float(np.float32(b))) for t, b in r] for r in biases]
+    tokens, token_starts = lists(windows, torch.int32)
+    ids, bias_starts = lists([[t for t, _ in r] for r in biases], torch.int32)
+    values, _ = lists([[b for _, b in r] for r in biases], torch.float32)
+    rep = (1 + torch.rand(rows, device="cuda", generator=g))
+    pres, freq = torch.rand(rows, device="cuda", generator=g), torch.rand(rows, device="cuda", generator=g) - 0.5
+    allowed = torch.randint(-2 ** 31, 2 ** 31, (3, (vocab + 31) // 32 + 1), device="cuda", generator=g).to(torch.int32)
+    allowed[1] = 0
+    which = [rnd.randrange(-1, 4) for _ in range(rows)]
+    mask_rows = torch.tensor(which, dtype=torch.int32, device="cuda")
+    every = dict(tokens=tokens, token_starts=token_starts, repetition=rep, presence=pres, frequency=freq, bias_ids=ids,
+                 bias_values=values, bias_starts=bias_starts, allowed=allowed, mask_rows=mask_rows)
+    want = plain_controls(logits, windows, rep, pres, freq, biases, allowed, which)
+    got = pkg.logit_controls(logits, **every)
+    assert got.dtype == logits.dtype and got.data_ptr() != logits.data_ptr()
+    check_controls(got, want)
+    # rows apart and unaligned, in place
+    wide = torch.zeros((rows, vocab + 3), dtype=logits.dtype, device="cuda")
+    wide[:, 1:1 + vocab] = logits
+    view = wide[:, 1:1 + vocab]
+    assert pkg.logit_controls(view, out=view, **every) is view
+    assert torch.equal(view, got) and (wide[:, 0] == 0).all() and (wide[:, 1 + vocab:] == 0).all()
+    # each control alone
+    check_controls(pkg.logit_controls(logits, tokens=tokens, token_starts=token_starts, repetition=rep),
+                   plain_controls(logits, windows, rep))
+    check_controls(pkg.logit_controls(logits, tokens=tokens, token_starts=token_starts, frequency=freq),
+                   plain_controls(logits, windows, freq=freq))
+    check_controls(pkg.logit_controls(logits, bias_ids=ids, bias_values=values, bias_starts=bias_starts),
+                   plain_controls(logits, biases=biases))
+    check_controls(pkg.logit_controls(logits, allowed=allowed, mask_rows=mask_rows),
+                   plain_controls(logits, allowed=allowed, mask_rows=which))
+    assert torch.equal(pkg.logit_controls(logits), logits)
+
+
+@gpu
+def test_controls_on_special_logits(pkg):
+    logits = torch.tensor([[math.inf, -math.inf, math.nan, 1.0, torch.finfo(torch.float32).min]], device="cuda")
+    allowed = torch.tensor([[0b11000]], dtype=torch.int32, device="cuda")
+    got = pkg.logit_controls(logits, allowed=allowed)
+    assert (got[0, :3] == -math.inf).all() and torch.equal(got[0, 3:], logits[0, 3:])  # masked whatever they were
+    tokens = torch.tensor([0, 1, 4], dtype=torch.int32, device="cuda")
+    starts = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    got = pkg.logit_controls(logits, tokens=tokens, token_starts=starts, repetition=torch.tensor([2.0], device="cuda"))
+    assert got[0, 0] == math.inf and got[0, 1] == -math.inf and got[0, 2].isnan() and got[0, 4] == -math.inf
+
+
+@gpu
+def test_controls_of_long_windows(pkg):
+    """More tokens in a window than a block has threads many times over; one id thousands of times."""
+    g = gen(14)
+    vocab = 50000
+    logits = normal(g, 2, vocab)
+    windows = [torch.randint(0, vocab, (40000,), generator=torch.Generator().manual_seed(1)).tolist(), [77] * 30000]
+    tokens, starts = lists(windows, torch.int32)
+    freq = torch.tensor([0.25, 0.125], device="cuda")
+    got = pkg.logit_controls(logits, tokens=tokens, token_starts=starts, frequency=freq).double().cpu()
+    count = torch.stack([torch.bincount(torch.tensor(w), minlength=vocab) for w in windows]).double()
+    want = logits.double().cpu() - freq.double().cpu()[:, None] * count
+    assert ((got - want).abs() <= 2.0 ** -22 * (want.abs() + 10)).all()
+
+
+# ---- refusals -------------------------------------------------------------------------------
+
+@gpu
+def test_refusals_on_the_device(pkg):
+    E = pkg.ArgumentError
+    cache = pkg.QuantKvCache.empty(4, 16, 2, 64)
+    slots = torch.zeros(3, dtype=torch.int32, device="cuda")
+    k = torch.zeros((3, 2, 64), device="cuda")
+    for bad in (dict(page_size=12), dict(page_size=4), dict(page_size=2048), dict(head_dim=24), dict(head_dim=272),
+                dict(fmt="fp8")):
+        with pytest.raises(E):
+            pkg.QuantKvCache.empty(**{**dict(n_pages=2, page_size=16, n_kv_heads=2, head_dim=64), **bad})
+    for args in ((k[:2], k, slots), (k, k.half(), slots), (k.cpu(), k, slots), (k, k, slots.long()), (k, k, slots.cpu()),
+                 (k.double(), k.double(), slots), (k[:, :1], k, slots), (k[..., :32], k, slots)):
+        with pytest.raises(E):
+            cache.write(*args)
+    with pytest.raises(E):
+        cache.read(slots, torch.float64)
+    with pytest.raises(E):
+        cache.read(slots.view(3, 1).expand(3, 2))
+    table = torch.zeros((3, 2), dtype=torch.int32, device="cuda")
+    prefix, starts = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.arange(4, dtype=torch.int32, device="cuda")
+    good = dict(q=torch.zeros((3, 4, 64), device="cuda"), page_table=table, prefix_lens=prefix)
+    cache.attend(**good)
+    for bad in (dict(q=good["q"][:, :3]), dict(q=good["q"][..., :32]), dict(q=good["q"].double()), dict(q=good["q"][:2]),
+                dict(page_table=table.long()), dict(page_table=table.t()), dict(prefix_lens=prefix[:2]),
+                dict(prefix_lens=prefix.float()), dict(starts=starts[:3]), dict(max_nodes=2),
+                dict(mask=torch.zeros((3, 0), dtype=torch.int32, device="cuda")), dict(scale=math.nan), dict(scale=math.inf),
+                dict(starts=starts, max_nodes=40, mask=torch.zeros((3, 1), dtype=torch.int32, device="cuda")),
+                dict(starts=starts, max_nodes=0), dict(max_len=-1)):
+        with pytest.raises(E):
+            cache.attend(**{**good, **bad})
+    w = torch.zeros((64, 32), device="cuda")
+    linear = pkg.W4Linear.pack(w, 32)
+    for call in (lambda: pkg.W4Linear.pack(w, 16), lambda: pkg.W4Linear.pack(w.double()), lambda: pkg.W4Linear.pack(w.t()),
+                 lambda: linear(torch.zeros((2, 63), device="cuda")), lambda: linear(torch.zeros((2, 64))),
+                 lambda: linear(torch.zeros((2, 64), device="cuda", dtype=torch.float64)),
+                 lambda: linear(torch.zeros((64, 2), device="cuda").t()),
+                 lambda: pkg.W4Linear(linear.codes, linear.meta, 64, 48, 32),
+                 lambda: pkg.W4Linear(linear.codes, linear.meta, 64, 32, 32, bias=torch.zeros(31, device="cuda"))):
+        with pytest.raises(E):
+            call()
+    logits = torch.zeros((2, 100), device="cuda")
+    t32 = torch.zeros(4, dtype=torch.int32, device="cuda")
+    s3 = torch.tensor([0, 2, 4], dtype=torch.int32, device="cuda")
+    row = torch.ones(2, device="cuda")
+    for bad in (dict(tokens=t32), dict(repetition=row), dict(tokens=t32, token_starts=s3[:2]),
+                dict(tokens=t32.long(), token_starts=s3), dict(tokens=t32, token_starts=s3, repetition=row[:1]),
+                dict(bias_ids=t32, bias_starts=s3), dict(bias_ids=t32, bias_values=row, bias_starts=s3),
+                dict(allowed=torch.zeros((2, 3), dtype=torch.int32, device="cuda")),
+                dict(allowed=torch.zeros((1, 4), dtype=torch.int32, device="cuda")), dict(mask_rows=t32[:2]),
+                dict(out=torch.zeros((2, 99), device="cuda")), dict(out=logits.half())):
+        with pytest.raises(E):
+            pkg.logit_controls(logits, **bad)
+    with pytest.raises(E):
+        pkg.logit_controls(logits.t())
+    with pytest.raises(E):
+        pkg.logit_controls(logits.double())
+
+
+def test_refusals_of_the_c_entries(pkg):
+    """What the C entry points refuse before any device work."""
+    import ctypes as C
+    import struct
+    from forge_lm_b200 import _native as N
+    L = N.load()
+    cache = struct.Struct("=QQ6i")
+    a, b = C.c_int64(), C.c_int64()
+    assert L.fb2_kvq_sizes(cache.pack(0, 0, 10, 16, 3, 64, 0, 0), C.byref(a), C.byref(b)) == N.FB2_OK
+    assert (a.value, b.value) == (10 * 16 * 3 * 2 * 64, 10 * 16 * 3 * 2 * 4)
+    assert L.fb2_kvq_sizes(cache.pack(0, 0, 10, 16, 3, 64, 1, 0), C.byref(a), C.byref(b)) == N.FB2_OK
+    assert a.value == 10 * 16 * 3 * 2 * 32
+    for bad in ((-1, 16, 3, 64, 0), (10, 17, 3, 64, 0), (10, 16, 0, 64, 0), (10, 16, 3, 8, 0), (10, 16, 3, 64, 2),
+                (2 ** 31 - 1, 16, 3, 64, 0)):
+        assert L.fb2_kvq_sizes(cache.pack(0, 0, *bad, 0), C.byref(a), C.byref(b)) == N.FB2_INVALID_ARG
+    assert L.fb2_kvq_sizes(None, C.byref(a), C.byref(b)) == N.FB2_INVALID_ARG
+    ok = cache.pack(4096, 4096, 10, 16, 3, 64, 0, 0)
+    args = (1, 1, 1, 1)
+    assert L.fb2_kvq_write(ok, 1, None, None, 0, *args, None, None) == N.FB2_INVALID_ARG
+    assert L.fb2_kvq_write(ok, -1, 4096, 4096, 0, *args, 4096, None) == N.FB2_INVALID_ARG
+    assert L.fb2_kvq_write(ok, 1, 4096, 4096, 7, *args, 4096, None) == N.FB2_INVALID_ARG
+    assert L.fb2_kvq_write(ok, 1, 4098, 4096, 0, *args, 4096, None) == N.FB2_INVALID_ARG
+    assert L.fb2_kvq_write(ok, 0, None, None, 0, *args, None, None) == N.FB2_OK
+    assert L.fb2_kvq_write(cache.pack(4097, 4096, 10, 16, 3, 64, 0, 0), 1, 4096, 4096, 0, *args, 4096, None) == N.FB2_INVALID_ARG
+    assert L.fb2_kvq_read(ok, 1, 4096, 4100, 4096, 0, None) == N.FB2_INVALID_ARG
+    assert L.fb2_kvq_read(ok, 0, None, None, None, 0, None) == N.FB2_OK
+    att = struct.Struct("=8Q4q8ifi")
+    base = [4096] * 3 + [4096, 4096, 0, 0, 0] + [0, 64, 64, 4] + [2, 2, 6, 0, 4, 1, 0, 0] + [0.125, 0]
+    assert L.fb2_kvq_attend_workspace(ok, att.pack(*base), C.byref(a)) == N.FB2_OK and a.value >= 0
+    for where, value in ((12, -1), (13, 3), (14, 7), (14, 0), (15, 3), (16, -1), (17, 0), (17, 2), (18, -1), (11, 3),
+                         (20, math.nan)):
+        bad = list(base)
+        bad[where] = value
+        assert L.fb2_kvq_attend_workspace(ok, att.pack(*bad), C.byref(a)) == N.FB2_INVALID_ARG, where
+        assert L.fb2_kvq_attend(ok, att.pack(*bad), None) == N.FB2_INVALID_ARG, where
+    assert b"" != L.fb2_last_error()
+    lin = struct.Struct("=QQQ4i")
+    assert L.fb2_w4_sizes(lin.pack(0, 0, 0, 100, 33, 32, 0), C.byref(a), C.byref(b)) == N.FB2_OK
+    assert (a.value, b.value) == (3 * 2 * 512, 3 * 4 * 64)
+    for bad in ((0, 33, 32), (100, 0, 32), (100, 33, 48), (2 ** 31 - 1, 33, 32)):
+        assert L.fb2_w4_sizes(lin.pack(0, 0, 0, *bad, 0), C.byref(a), C.byref(b)) == N.FB2_INVALID_ARG
+    w = lin.pack(4096, 4096, 0, 100, 33, 32, 0)
+    assert L.fb2_w4_pack(w, 4096, 0, 32, None) == N.FB2_INVALID_ARG
+    assert L.fb2_w4_pack(w, None, 0, 33, None) == N.FB2_INVALID_ARG
+    assert L.fb2_w4_matvec(w, 2, 4096, 100, 4096, 32, 0, None, 0, None) == N.FB2_INVALID_ARG
+    assert L.fb2_w4_matvec(w, -1, 4096, 100, 4096, 33, 0, None, 0, None) == N.FB2_INVALID_ARG
+    assert L.fb2_w4_matvec(w, 0, None, 0, None, 0, 0, None, 0, None) == N.FB2_OK
+    con = struct.Struct("=12Q4q6i")
+    base = [4096, 4096] + [0] * 10 + [100, 100, 0, 0] + [2, 100, 0, 0, 0, 0]
+    for where, value in ((0, 0), (1, 0), (0, 4097), (13, 99), (2, 4096), (7, 4096), (10, 4096), (16, -1),
+                         (16, 70000), (17, -1), (18, 5)):
+        bad = list(base)
+        bad[where] = value
+        assert L.fb2_logit_controls(con.pack(*bad), None) == N.FB2_INVALID_ARG, where
+    assert L.fb2_logit_controls(None, None) == N.FB2_INVALID_ARG
+    base[16] = 0
+    assert L.fb2_logit_controls(con.pack(*base), None) == N.FB2_OK
