@@ -11,6 +11,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cstring>
+
 #include "common.cuh"
 
 namespace fb2 {
@@ -71,127 +73,195 @@ FB2_DEV void load8(const T* p, float (&x)[8]) {
         for (int i = 0; i < 8; i++) x[i] = Dense<T>::get(p[i]);
     }
 }
-template <class T>
-FB2_DEV void store8(T* p, const float (&x)[8]) {
-    constexpr int N = sizeof(T) / 2;
-    uint4 w[N];
-    T* t = reinterpret_cast<T*>(w);
-#pragma unroll
-    for (int i = 0; i < 8; i++) t[i] = Dense<T>::put(x[i]);
-#pragma unroll
-    for (int i = 0; i < N; i++) reinterpret_cast<uint4*>(p)[i] = w[i];
-}
+// A row is shared by `width` neighbouring lanes of a warp (a power of two); a
+// lane holds NP pieces of 16 bytes, piece j at index part + width * j, so that
+// every load and store of a row is one run of bytes.  16 values per lane: the
+// reductions over the row, the divisions and the addresses are paid once for
+// them.
+constexpr int KVQ_THREADS = 128;
 
-// 8 codes (8 bytes of int8, 4 bytes of int4) and the row's meta word -> values.
-FB2_DEV void kvq_decode8(uint2 c, float scale, float (&x)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const uint32_t byte = ((i < 4 ? c.x : c.y) >> (8 * (i & 3))) & 0xffu;
-        x[i] = (float)((int)byte - 128) * scale;
+template <class T>
+struct KvqPiece {
+    static constexpr int N = 16 / sizeof(T);  // values
+    static constexpr int NP = 16 / N;         // per lane
+};
+
+// The code bytes of a piece: N bytes (int8) or N / 2 (int4).
+template <int FMT, int N>
+FB2_DEV void kvq_store_codes(unsigned char* row, int piece, const uint32_t* w) {
+    if constexpr (FMT == KVQ_INT8) {
+        if constexpr (N == 8)
+            *reinterpret_cast<uint2*>(row + piece * 8) = make_uint2(w[0], w[1]);
+        else
+            *reinterpret_cast<uint32_t*>(row + piece * 4) = w[0];
+    } else {
+        if constexpr (N == 8)
+            *reinterpret_cast<uint32_t*>(row + piece * 4) = w[0];
+        else
+            *reinterpret_cast<unsigned short*>(row + piece * 2) = (unsigned short)w[0];
     }
 }
-FB2_DEV void kvq_decode8(uint32_t c, float scale, float least, float (&x)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = fmaf((float)((c >> (4 * i)) & 15u), scale, least);
+template <int FMT, int N>
+FB2_DEV void kvq_load_codes(const unsigned char* row, int piece, uint32_t* w) {
+    if constexpr (FMT == KVQ_INT8) {
+        if constexpr (N == 8) {
+            const uint2 v = __ldcs(reinterpret_cast<const uint2*>(row + piece * 8));
+            w[0] = v.x, w[1] = v.y;
+        } else {
+            w[0] = __ldcs(reinterpret_cast<const uint32_t*>(row + piece * 4));
+        }
+    } else {
+        if constexpr (N == 8)
+            w[0] = __ldcs(reinterpret_cast<const uint32_t*>(row + piece * 4));
+        else
+            w[0] = __ldcs(reinterpret_cast<const unsigned short*>(row + piece * 2));
+    }
 }
 
-// A row's lanes are `width` (a power of two, >= head_dim / 8) neighbours of a
-// warp, 8 values each; blockIdx.y: K or V.
-constexpr int KVQ_THREADS = 256;
+FB2_DEV float min_nan(float a, float b) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+FB2_DEV float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
 
+// rint(x) for |x| < 2^22 as the low bits of 1.5 2^23 + x
+constexpr float kRint = 12582912.0f;
+constexpr uint32_t kRintBits = 0x4b400000u;
+
+// blockIdx: rows, K/V head, K or V.
 template <class T, int FMT, bool VEC>
 __global__ void __launch_bounds__(KVQ_THREADS)
     k_kvq_write(KvqView c, int n_rows, const T* __restrict__ k, const T* __restrict__ v, long long k_row, long long k_head,
                 long long v_row, long long v_head, const int* __restrict__ slots, int width) {
-    const int kind = blockIdx.y;
-    const long long item = ((long long)blockIdx.x * KVQ_THREADS + threadIdx.x) / width;
-    const int part = threadIdx.x & (width - 1);
-    const int row = (int)(item / c.heads), head = (int)(item - (long long)row * c.heads);
+    constexpr int N = KvqPiece<T>::N, NP = KvqPiece<T>::NP;
+    const int kind = blockIdx.z, head = blockIdx.y;
+    const int row = blockIdx.x * (KVQ_THREADS / width) + threadIdx.x / width, part = threadIdx.x & (width - 1);
     // lanes of a row agree on `live`; the shuffles below run with the whole warp
     const int slot = row < n_rows ? __ldg(slots + row) : -1;
     const bool live = (uint32_t)slot < (uint32_t)c.n_slots;
-    const bool mine = live && part * 8 < c.hd;
-    float x[8];
-    if (mine) {
-        const T* p = kind ? v + row * v_row + head * v_head : k + row * k_row + head * k_head;
-        load8<T, VEC>(p + part * 8, x);
+    const T* p = kind ? v + row * v_row + head * v_head : k + row * k_row + head * k_head;
+    float x[NP][N];
+    bool mine[NP];
+#pragma unroll
+    for (int j = 0; j < NP; j++) {
+        const int piece = part + width * j;
+        mine[j] = live && piece * N < c.hd;
+        if constexpr (VEC) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (mine[j]) w = __ldcs(reinterpret_cast<const uint4*>(p) + piece);
+            T t[N];
+            memcpy(t, &w, 16);
+#pragma unroll
+            for (int i = 0; i < N; i++) x[j][i] = Dense<T>::get(t[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) x[j][i] = mine[j] ? Dense<T>::get(p[piece * N + i]) : 0.f;
+        }
     }
+    const size_t at = live ? c.row(slot, head, kind) : 0;
+    unsigned char* to = c.codes + at * c.row_bytes;
     if constexpr (FMT == KVQ_INT8) {
         // max|x| through the bits: NaN > inf > finite
         uint32_t top = 0;
-        if (mine)
 #pragma unroll
-            for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+        for (int j = 0; j < NP; j++)
+#pragma unroll
+            for (int i = 0; i < N; i++) top = max(top, __float_as_uint(x[j][i]) & 0x7fffffffu);
         for (int o = width / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
         const bool finite = top < 0x7f800000u;
         const float amax = __uint_as_float(top);
         const bool some = finite && amax >= kKvqTiny;
         const float inv = some ? 127.0f / amax : 0.0f;
-        if (!mine) return;
-        uint32_t w[2] = {0u, 0u};
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int code = some ? (int)fminf(fmaxf(rintf(x[i] * inv), -127.0f), 127.0f) : 0;
-            w[i >> 2] |= (uint32_t)(code + 128) << (8 * (i & 3));
+        for (int j = 0; j < NP; j++) {
+            if (!mine[j]) continue;
+            uint32_t w[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                // |x inv| <= 127 (1 + 2^-23): it rounds to 127 at most; NaN rows hold code 0
+                const float f = finite ? x[j][i] * inv : 0.f;
+                w[i / 4] += (__float_as_uint(f + kRint) - kRintBits + 128u) << (8 * (i % 4));
+            }
+            kvq_store_codes<FMT, N>(to, part + width * j, w);
         }
-        const size_t at = c.row(slot, head, kind);
-        *reinterpret_cast<uint2*>(c.codes + at * c.row_bytes + part * 8) = make_uint2(w[0], w[1]);
-        if (part == 0)
-            c.meta[at] = finite ? __float_as_uint(some ? amax / 127.0f : 0.0f) : 0x7fc00000u;
+        if (part == 0 && live) c.meta[at] = finite ? __float_as_uint(some ? amax / 127.0f : 0.0f) : 0x7fc00000u;
     } else {
         const float inf = __uint_as_float(0x7f800000u);
-        float lo = inf, hi = -inf;
-        if (mine)
+        float lo = inf, hi = -inf;  // NaN stays
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const bool nan = x[i] != x[i];
-                lo = fminf(lo, nan ? -inf : x[i]);
-                hi = fmaxf(hi, nan ? inf : x[i]);
-            }
+        for (int j = 0; j < NP; j++)
+            if (mine[j])
+#pragma unroll
+                for (int i = 0; i < N; i++) lo = min_nan(lo, x[j][i]), hi = max_nan(hi, x[j][i]);
         for (int o = width / 2; o > 0; o >>= 1) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         }
-        if (!mine) return;
-        uint32_t scale_b = float_to_bf16_bits((hi - lo) / 15.0f);
-        const uint32_t least_b = float_to_bf16_bits(lo);
-        const float least = bf16_bits_to_float(least_b);
-        float scale = bf16_bits_to_float(scale_b);
+        const uint32_t scale_b = float_to_bf16_bits((hi - lo) / 15.0f), least_b = float_to_bf16_bits(lo);
+        const float least = bf16_bits_to_float(least_b), scale = bf16_bits_to_float(scale_b);
         const bool finite = scale < inf && fabsf(least) < inf;  // false for NaN
         const bool some = finite && scale >= kKvqTiny;
         const float inv = some ? 1.0f / scale : 0.0f;
-        uint32_t w = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int code = some ? (int)fminf(fmaxf(rintf((x[i] - least) * inv), 0.0f), 15.0f) : 0;
-            w |= (uint32_t)code << (4 * i);
+        for (int j = 0; j < NP; j++) {
+            if (!mine[j]) continue;
+            uint32_t w = 0;
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const float f = some ? fminf(fmaxf((x[j][i] - least) * inv, 0.0f), 15.0f) : 0.f;
+                w += (__float_as_uint(f + kRint) - kRintBits) << (4 * i);
+            }
+            kvq_store_codes<FMT, N>(to, part + width * j, &w);
         }
-        const size_t at = c.row(slot, head, kind);
-        *reinterpret_cast<uint32_t*>(c.codes + at * c.row_bytes + part * 4) = w;
-        if (part == 0) c.meta[at] = finite ? ((some ? scale_b : 0u) | (least_b << 16)) : 0x7fc07fc0u;
+        if (part == 0 && live) c.meta[at] = finite ? ((some ? scale_b : 0u) | (least_b << 16)) : 0x7fc07fc0u;
     }
 }
 
 template <class T, int FMT>
 __global__ void __launch_bounds__(KVQ_THREADS)
     k_kvq_read(KvqView c, int n_rows, const int* __restrict__ slots, T* __restrict__ k, T* __restrict__ v, int width) {
-    const int kind = blockIdx.y;
-    const long long item = ((long long)blockIdx.x * KVQ_THREADS + threadIdx.x) / width;
-    const int part = threadIdx.x & (width - 1);
-    const int row = (int)(item / c.heads), head = (int)(item - (long long)row * c.heads);
-    if (row >= n_rows || part * 8 >= c.hd) return;
+    constexpr int N = KvqPiece<T>::N, NP = KvqPiece<T>::NP;
+    const int kind = blockIdx.z, head = blockIdx.y;
+    const int row = blockIdx.x * (KVQ_THREADS / width) + threadIdx.x / width, part = threadIdx.x & (width - 1);
+    if (row >= n_rows) return;
     const int slot = __ldg(slots + row);
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if ((uint32_t)slot < (uint32_t)c.n_slots) {
+    const bool live = (uint32_t)slot < (uint32_t)c.n_slots;
+    uint32_t w[NP][2], m = 0;
+#pragma unroll
+    for (int j = 0; j < NP; j++) w[j][0] = w[j][1] = 0;
+    if (live) {
         const size_t at = c.row(slot, head, kind);
-        const uint32_t m = c.meta[at];
-        if constexpr (FMT == KVQ_INT8)
-            kvq_decode8(*reinterpret_cast<const uint2*>(c.codes + at * c.row_bytes + part * 8), __uint_as_float(m), x);
-        else
-            kvq_decode8(*reinterpret_cast<const uint32_t*>(c.codes + at * c.row_bytes + part * 4),
-                        bf16_bits_to_float(m & 0xffffu), __uint_as_float(m & 0xffff0000u), x);
+        m = __ldg(c.meta + at);
+#pragma unroll
+        for (int j = 0; j < NP; j++)
+            if ((part + width * j) * N < c.hd) kvq_load_codes<FMT, N>(c.codes + at * c.row_bytes, part + width * j, w[j]);
     }
-    store8((kind ? v : k) + (size_t)item * c.hd + part * 8, x);
+    uint4* to = reinterpret_cast<uint4*>((kind ? v : k) + ((size_t)row * c.heads + head) * c.hd);
+#pragma unroll
+    for (int j = 0; j < NP; j++) {
+        if ((part + width * j) * N >= c.hd) continue;
+        T t[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            float x;
+            if constexpr (FMT == KVQ_INT8) {
+                const float code = __uint_as_float(kRintBits + ((w[j][i / 4] >> (8 * (i % 4))) & 0xffu)) - (kRint + 128.0f);
+                x = live ? code * __uint_as_float(m) : 0.f;
+            } else {
+                const float code = __uint_as_float(kRintBits + ((w[j][0] >> (4 * i)) & 15u)) - kRint;
+                x = fmaf(code, bf16_bits_to_float(m & 0xffffu), __uint_as_float(m & 0xffff0000u));
+            }
+            t[i] = Dense<T>::put(x);
+        }
+        uint4 o;
+        memcpy(&o, t, 16);
+        __stcs(to + part + width * j, o);
+    }
 }
 
 }  // namespace fb2

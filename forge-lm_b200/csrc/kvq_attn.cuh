@@ -3,8 +3,14 @@
 //
 // out = sum_p softmax_p(scale q.k_p) v_p over the positions a row sees, in one
 // pass: the running maximum m, l = sum exp(s - m) and o = sum exp(s - m) v,
-// rescaled when m grows; parts merge by the same rule.
+// rescaled when m grows; parts merge by the same rule.  With codes c and the
+// row's scale a and (int4) minimum b, k = a c + b:
+//   q.k = a (q.c) + b sum(q),    sum_p w_p v_p = sum_p (w_p a_p) c_p + sum_p w_p b_p,
+// so both products run on the codes themselves, which fp16 holds exactly, and
+// the scales are applied to scores and probabilities.
 #pragma once
+#include <type_traits>
+
 #include "kvq.cuh"
 
 namespace fb2 {
@@ -18,8 +24,11 @@ struct KvqAttnArgs {
     const int* prefix;
     const int* starts;       // null: one row per sequence
     const uint32_t* mask;    // null: causal
+    float* part_o;           // [n_rows][n_heads][splits][hd], and
+    float2* part_ml;         // (m, l) of each, where splits > 1
     long long q_row, q_head, table_stride;
-    int n_seqs, n_rows, n_heads, max_pages, max_nodes, max_len, mask_words;
+    int n_seqs, n_rows, n_heads, share, max_nodes, max_len, mask_words, dtype;
+    int splits, chunk, row_blocks;
     float scale;
     FB2_DEV void rows_of(int b, int& first, int& count) const {
         first = starts ? __ldg(starts + b) : b;
@@ -28,72 +37,551 @@ struct KvqAttnArgs {
         first = max(first, 0);
         count = min(min(last, n_rows) - first, max_nodes);
     }
-    FB2_DEV int slot(int b, int p) const {  // -1: not in the cache
-        const int page = __ldg(table + b * table_stride + (p >> c.page_shift));
-        if ((uint32_t)page >= (uint32_t)(c.n_slots >> c.page_shift)) return -1;
-        return (page << c.page_shift) | (p & ((1 << c.page_shift) - 1));
+    FB2_DEV float load_q(long long row, int head, int d) const {
+        const long long at = row * q_row + head * q_head + d;
+        if (dtype == 0) return __ldg(static_cast<const float*>(q) + at);
+        if (dtype == 1) return __bfloat162float(static_cast<const __nv_bfloat16*>(q)[at]);
+        return __half2float(static_cast<const __half*>(q)[at]);
+    }
+    FB2_DEV void store_out(size_t at, float v) const {
+        if (dtype == 0)
+            static_cast<float*>(out)[at] = v;
+        else if (dtype == 1)
+            static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
+        else
+            static_cast<__half*>(out)[at] = __float2half_rn(v);
     }
 };
 
-// One warp per (row, head).
-template <class T, int FMT>
-__global__ void __launch_bounds__(128) k_kvq_attend(KvqAttnArgs a) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int b = blockIdx.z, i = blockIdx.y, h = blockIdx.x * 4 + warp;
+namespace kva {
+
+FB2_DEV void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+FB2_DEV uint32_t transpose8x8(uint32_t a) {
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+FB2_DEV uint32_t h2_sub(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+FB2_DEV uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+FB2_DEV uint32_t h2_pack(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+FB2_DEV float2 h2_floats(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+
+// fp16 pairs of codes.  0x6400 | b is 1024 + b (b < 1024), exactly.
+// int8 bytes 0,1 (2,3 with `high`) of w as code = byte - 128.
+template <bool HIGH>
+FB2_DEV uint32_t codes8(uint32_t w) {
+    return h2_sub(__byte_perm(w, 0x64646464u, HIGH ? 0x4342 : 0x4140), 0x64806480u);
+}
+// Nibbles I and I + 4 of w as codes - 8 (a nibble at bits 4..7 of its half
+// is 16 c in the sum: times 1/16, minus 72).  Around 8 they nearly cancel in
+// the sums, so that the probabilities' roundings do too; the minimum that
+// goes with them is b + 8 a.
+template <int I>
+FB2_DEV uint32_t codes4(uint32_t w) {
+    const uint32_t v = I < 2 ? w : w >> 8;
+    if constexpr (I % 2 == 0) return h2_sub((v & 0x000f000fu) | 0x64006400u, 0x64086408u);
+    return h2_fma((v & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);
+}
+
+// b + 8 a of an int4 row's meta word
+FB2_DEV float centre(uint32_t w) { return fmaf(8.0f, bf16_bits_to_float(w & 0xffffu), __uint_as_float(w & 0xffff0000u)); }
+
+FB2_DEV float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+}  // namespace kva
+
+// A CTA of 4 warps takes one chunk of one sequence's positions for one K/V
+// head and a block of 8 NT rows (the rows of its tokens and of the query
+// heads that share the K/V head).  Each warp works on its own tiles of 16 MT
+// positions from global memory to registers, with no barrier until the end:
+//   S^T[position][row] = K codes (A, 16 positions) x q (B, 8 rows),
+//   O^T[dim][row]     += V codes^T (A, 16 dims) x P^T (B, 16 positions x 8 rows),
+// the same column = row layout for both accumulators, so maxima and rescaling
+// need no exchange between the two; P's 8 x 8 blocks are transposed by
+// movmatrix.  Dimensions and positions are assigned to fragments so that a
+// lane's K and V codes are consecutive bytes (K: 16 dims of a position; V: HD/8
+// dims of 2 positions); q's fragments are built in that order once.
+// q is scaled by a power of two to just below 2^13 and split in two fp16
+// terms (one for 16-bit types, whose values fit); P is scaled to just below
+// 2^14 together with the largest V scale so far, and split likewise.  Sums
+// over a tile start at zero and are added to the running fp32 sums.
+constexpr int KVA_WARPS = 4;
+
+template <int HD, int FMT, int NT, bool SPLIT>
+struct KvaShape {
+    static constexpr int MT = HD > 128 ? 1 : 2;       // 16-position groups of a tile
+    static constexpr int TT = 16 * MT;                // positions of a tile
+    static constexpr int KCH = HD / 64;               // 16-dim chunks of K per lane and position
+    static constexpr int KW = FMT == KVQ_INT8 ? 4 : 2;  // words of a chunk
+    static constexpr int VD = HD / 8;                 // dims of V per lane and position
+    static constexpr int VW = FMT == KVQ_INT8 ? VD / 4 : VD / 8;
+    static constexpr int STEPS = HD / 16;
+    static constexpr int PARTS = SPLIT ? 2 : 1;
+    static constexpr int ROWS = 8 * NT;
+    static constexpr int Q_BYTES = PARTS * NT * STEPS * 32 * 8;
+    static constexpr int O_STRIDE = HD + 8;
+    static constexpr int O_BYTES = KVA_WARPS * ROWS * O_STRIDE * 4;
+    static constexpr int SMEM = (Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES) + ROWS * 8 + KVA_WARPS * ROWS * 8;
+};
+
+template <int HD, int FMT, int NT, bool SPLIT>
+__global__ void __launch_bounds__(KVA_WARPS * 32) k_kvq_attend(KvqAttnArgs a) {
+    using namespace kva;
+    using S = KvaShape<HD, FMT, NT, SPLIT>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int kBig = S::Q_BYTES > S::O_BYTES ? S::Q_BYTES : S::O_BYTES;
+    __half* sq = reinterpret_cast<__half*>(smem);
+    float* so = reinterpret_cast<float*>(smem);
+    float2* srow = reinterpret_cast<float2*>(smem + kBig);                        // (score factor, factor * sum q)
+    float2* sml = reinterpret_cast<float2*>(smem + kBig + S::ROWS * 8);           // [warp][row] (m, l)
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int b = blockIdx.y;
+    const int rb = blockIdx.x % a.row_blocks, rest = blockIdx.x / a.row_blocks;
+    const int split = rest % a.splits, head = rest / a.splits;
     int first, count;
     a.rows_of(b, first, count);
-    if (i >= count || h >= a.n_heads) return;
-    const int row = first + i, g = h / (a.n_heads / a.c.heads);
+    const int row0 = rb * S::ROWS, n_rows = min(S::ROWS, count * a.share - row0);
+    if (n_rows <= 0) return;
     const int prefix = max(__ldg(a.prefix + b), 0);
     const int len = (int)min((long long)prefix + count, (long long)a.max_len);
-    float q[8], o[8], x[8];
-    const bool mine = lane * 8 < a.c.hd;
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-        q[j] = 0.f;
-        o[j] = 0.f;
+    const int c0 = split * a.chunk, c1 = min(len, c0 + a.chunk);
+    // row r of the block: token (row0 + r) / share of the sequence, query head
+    // head * share + (row0 + r) % share
+    if (c0 >= c1 && a.splits > 1) {  // nothing here: the merge has to know
+        for (int r = tid; r < n_rows; r += KVA_WARPS * 32) {
+            const int node = (row0 + r) / a.share, h = head * a.share + (row0 + r) - node * a.share;
+            a.part_ml[((size_t)(first + node) * a.n_heads + h) * a.splits + split] = make_float2(-INFINITY, 0.f);
+        }
+        return;
     }
-    if (mine) load8<T, false>((const T*)a.q + row * a.q_row + h * a.q_head + lane * 8, q);
-    float m = -INFINITY, l = 0.f;
-    auto values = [&](size_t at) {
-        const uint32_t w = a.c.meta[at];
-        if constexpr (FMT == KVQ_INT8)
-            kvq_decode8(*reinterpret_cast<const uint2*>(a.c.codes + at * a.c.row_bytes + lane * 8), __uint_as_float(w), x);
-        else
-            kvq_decode8(*reinterpret_cast<const uint32_t*>(a.c.codes + at * a.c.row_bytes + lane * 4),
-                        bf16_bits_to_float(w & 0xffffu), __uint_as_float(w & 0xffff0000u), x);
+
+    // ---- the tile loop's addresses -------------------------------------------
+    const int ps = 1 << a.c.page_shift, rbytes = a.c.row_bytes, hd = a.c.hd;
+    const int n_pages = a.c.n_slots >> a.c.page_shift;
+    const int tiles = (c1 - c0 + S::TT - 1) / S::TT;
+    constexpr int GR = 2 * S::MT;        // 8-position groups of a tile, each in one page
+    constexpr int AHEAD = 32 / GR;       // tiles whose page ids a warp holds, one per lane
+    const int* table = a.table + b * a.table_stride;
+    int ids = -1;
+    auto load_ids = [&](int tile) {      // of tiles tile, tile + WARPS, ..
+        const int pos = c0 + (tile + (lane / GR) * KVA_WARPS) * S::TT + (lane % GR) * 8;
+        ids = -1;
+        if (pos < c1) {
+            const int id = __ldg(table + (pos >> a.c.page_shift));
+            if ((uint32_t)id < (uint32_t)n_pages) ids = id;
+        }
     };
-    for (int p = 0; p < len; p++) {
-        const int j = p - prefix;
-        if (j >= 0) {
-            const bool see = a.mask ? (__ldg(a.mask + (size_t)row * a.mask_words + (j >> 5)) >> (j & 31)) & 1 : j <= i;
-            if (!see) continue;
+    // index of the K row of the group's first position; < 0: none
+    auto group_row = [&](int id, int pos) -> long long {
+        return id < 0 ? -1 : (((((long long)id * a.c.heads + head) * 2) << a.c.page_shift) | (pos & (ps - 1)));
+    };
+    uint32_t kr[GR][S::KCH][S::KW], vr[GR][2][S::VW], km[GR], vm[GR];
+    auto load_words = [&](const unsigned char* p, uint32_t* w, auto n) {
+        constexpr int N = decltype(n)::value;
+        if constexpr (N == 1) {
+            w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+        } else if constexpr (N == 2) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+            w[0] = v.x, w[1] = v.y;
+        } else {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
         }
-        const int slot = a.slot(b, p);
-        if (slot < 0) continue;
-        float s = 0.f;
-        if (mine) {
-            values(a.c.row(slot, g, 0));
+    };
+    auto load_k = [&](int tile, int slot) {
 #pragma unroll
-            for (int d = 0; d < 8; d++) s = fmaf(q[d], x[d], s);
+        for (int j = 0; j < GR; j++) {
+            const int pos = c0 + tile * S::TT + j * 8;
+            const long long row = group_row(__shfl_sync(0xffffffffu, ids, slot * GR + j), pos);
+            const bool live = row >= 0 && pos + g < c1;
+            const unsigned char* p = a.c.codes + (row + g) * rbytes;
+            km[j] = live ? __ldg(a.c.meta + row + g) : 0u;
+#pragma unroll
+            for (int cc = 0; cc < S::KCH; cc++) {
+                const int chunk = t + 4 * cc;
+#pragma unroll
+                for (int i = 0; i < S::KW; i++) kr[j][cc][i] = 0;
+                if (live && chunk * 16 < hd)
+                    load_words(p + chunk * (S::KW * 4), kr[j][cc], std::integral_constant<int, S::KW>{});
+            }
         }
-        s = warp_sum(s) * a.scale;
-        const float n = fmaxf(m, s), f = __expf(m - n), e = expf(s - n);
-        m = n;
-        l = l * f + e;
-        if (mine) {
-            values(a.c.row(slot, g, 1));
+    };
+    auto load_v = [&](int tile, int slot) {
 #pragma unroll
-            for (int d = 0; d < 8; d++) o[d] = fmaf(o[d], f, e * x[d]);
+        for (int j = 0; j < GR; j++) {
+            const int pos = c0 + tile * S::TT + j * 8;
+            long long row = group_row(__shfl_sync(0xffffffffu, ids, slot * GR + j), pos);
+            const bool any = row >= 0;
+            row += ps;  // the V rows lie one page behind the K rows
+            vm[j] = any && pos + g < c1 ? __ldg(a.c.meta + row + g) : 0u;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const bool live = any && pos + 2 * t + e < c1;
+                const unsigned char* p = a.c.codes + (row + 2 * t + e) * rbytes + g * (S::VW * 4);
+                constexpr int PIECE = S::VW > S::KW ? S::KW : S::VW;  // at most 16 dims at once
+#pragma unroll
+                for (int i = 0; i < S::VW; i++) vr[j][e][i] = 0;
+#pragma unroll
+                for (int i = 0; i < S::VW; i += PIECE)
+                    if (live && g * S::VD + i * (S::VD / S::VW) < hd)
+                        load_words(p + 4 * i, vr[j][e] + i, std::integral_constant<int, PIECE>{});
+            }
+        }
+    };
+    int held = 0;  // tiles of `ids` used up
+    if (warp < tiles) {
+        load_ids(warp);
+        load_k(warp, 0);
+        load_v(warp, 0);
+    }
+
+    // ---- q's fragments (while the first tile is on its way) --------------------
+    for (int r = warp; r < S::ROWS; r += KVA_WARPS) {
+        float x[HD / 32], top = 0.f, sum = 0.f;
+        const int node = (row0 + r) / a.share, h = head * a.share + (row0 + r) - node * a.share;
+#pragma unroll
+        for (int i = 0; i < HD / 32; i++) {
+            const int d = lane + 32 * i;
+            x[i] = r < n_rows && d < hd ? a.load_q(first + node, h, d) : 0.f;
+            top = fmaxf(top, fabsf(x[i]));
+        }
+        top = warp_max(top);
+        // a power of two that brings max|q| just below 2^13; NaN or inf stay in x
+        const int e = top > 0.f && top < INFINITY ? ilogbf(top) : 0;
+#pragma unroll
+        for (int i = 0; i < HD / 32; i++) {
+            const int d = lane + 32 * i, c = d >> 4, w = d & 15;
+            x[i] = scalbnf(x[i], 12 - e);
+            sum += x[i];
+            int step, reg, half;
+            if constexpr (FMT == KVQ_INT8) {
+                step = w >> 2, reg = (w >> 1) & 1, half = w & 1;
+            } else {
+                step = 2 * (w >> 3) + ((w >> 1) & 1), reg = w & 1, half = (w >> 2) & 1;
+            }
+            step += 4 * (c >> 2);
+            const __half hi = __float2half_rn(x[i]);
+            const int at = (((r >> 3) * S::STEPS + step) * 32 + 4 * (r & 7) + (c & 3)) * 4 + 2 * reg + half;
+            sq[at] = hi;
+            if constexpr (SPLIT) sq[at + NT * S::STEPS * 128] = __float2half_rn(x[i] - __half2float(hi));
+        }
+        sum = warp_sum(sum);
+        const float f = scalbnf(a.scale * 1.44269504088896341f, e - 12);
+        if (lane == 0) srow[r] = make_float2(f, sum * f);
+    }
+    __syncthreads();
+
+    // ---- the pass over the positions --------------------------------------------
+    float o[S::VD / 2][NT][4], m[NT][2], l[NT][2], z[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) m[n][i] = -INFINITY, l[n][i] = 0.f, z[n][i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < S::VD / 2; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) o[i][n][c] = 0.f;
+    }
+    float2 rowf[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) rowf[n][i] = srow[8 * n + 2 * t + i];
+    // exponent field of the largest V scale so far (o is in units of
+    // 2^(vexp - 126 - 14)); 20: small enough for every scale, 2^(140 - 20) is finite
+    uint32_t vexp = 20;
+
+    for (int tile = warp; tile < tiles; tile += KVA_WARPS) {
+        const int pos0 = c0 + tile * S::TT;
+        // every position seen by every row?
+        bool full = pos0 + S::TT <= min(prefix, c1);
+#pragma unroll
+        for (int j = 0; j < GR; j++) full &= __shfl_sync(0xffffffffu, ids, held * GR + j) >= 0;
+        uint32_t live = 0;  // groups with a page
+        if (!full)
+#pragma unroll
+            for (int j = 0; j < GR; j++) live |= (uint32_t)(__shfl_sync(0xffffffffu, ids, held * GR + j) >= 0) << j;
+
+        float s[S::MT][NT][4];
+#pragma unroll
+        for (int i = 0; i < S::MT; i++)
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) s[i][n][c] = 0.f;
+#pragma unroll
+        for (int st = 0; st < S::STEPS; st++) {
+            uint2 qf[NT][S::PARTS];
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int p = 0; p < S::PARTS; p++)
+                    qf[n][p] = reinterpret_cast<const uint2*>(sq)[((p * NT + n) * S::STEPS + st) * 32 + lane];
+#pragma unroll
+            for (int i = 0; i < S::MT; i++) {
+                uint32_t f[2][2];
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    if constexpr (FMT == KVQ_INT8) {
+                        const uint32_t w = kr[2 * i + j][st / 4][st % 4];
+                        f[j][0] = codes8<false>(w);
+                        f[j][1] = codes8<true>(w);
+                    } else {
+                        const uint32_t w = kr[2 * i + j][st / 4][(st % 4) / 2];
+                        f[j][0] = st % 2 ? codes4<2>(w) : codes4<0>(w);
+                        f[j][1] = st % 2 ? codes4<3>(w) : codes4<1>(w);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int p = 0; p < S::PARTS; p++)
+                        mma_f16(s[i][n], f[0][0], f[1][0], f[0][1], f[1][1], qf[n][p].x, qf[n][p].y);
+            }
+        }
+        // scores in units of log2
+#pragma unroll
+        for (int i = 0; i < S::MT; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const uint32_t w = km[2 * i + (c >> 1)];
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    const float2 f = rowf[n][c & 1];
+                    if constexpr (FMT == KVQ_INT8)
+                        s[i][n][c] *= __uint_as_float(w) * f.x;
+                    else
+                        s[i][n][c] = fmaf(s[i][n][c], bf16_bits_to_float(w & 0xffffu) * f.x, centre(w) * f.y);
+                }
+            }
+        if (!full) {
+#pragma unroll
+            for (int i = 0; i < S::MT; i++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const int j = 2 * i + (c >> 1), pos = pos0 + 8 * j + g, node = pos - prefix;
+                    const bool there = ((live >> j) & 1) && pos < c1;
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const int r = 8 * n + 2 * t + (c & 1);
+                        bool see = there && r < n_rows;
+                        if (see && node >= 0) {
+                            const int mine = (row0 + r) / a.share;
+                            see = a.mask ? (__ldg(a.mask + (size_t)(first + mine) * a.mask_words + (node >> 5)) >> (node & 31)) & 1
+                                         : node <= mine;
+                        }
+                        if (!see) s[i][n][c] = -INFINITY;
+                    }
+                }
+        }
+        // the next tile's K goes out: its registers are free
+        const int next = tile + KVA_WARPS;
+        if (next < tiles) {
+            if (++held == AHEAD) {
+                held = 0;
+                load_ids(next);
+            }
+            load_k(next, held);
+        }
+        // V's scales: the largest finite one sets the unit of o
+        uint32_t vtop = 0;
+#pragma unroll
+        for (int j = 0; j < GR; j++) {
+            const uint32_t bits = (FMT == KVQ_INT8 ? vm[j] : vm[j] << 16) & 0x7fffffffu;
+            if (bits < 0x7f800000u) vtop = max(vtop, bits);
+        }
+        vtop = max(__reduce_max_sync(0xffffffffu, vtop) >> 23, vexp);
+        float grow = __uint_as_float((127u - min(vtop - vexp, 126u)) << 23);  // 2^(old - new); below 2^-126 all the same
+        vexp = vtop;
+        const float unit = __uint_as_float((127u + 140u - vexp) << 23);  // 2^(140 - vexp), vexp >= 20 keeps it finite
+        // softmax; alpha rescales what there is
+        float alpha[NT][2];
+        uint32_t pb[S::MT][NT][S::PARTS][2];
+        float vs[GR], vl[GR];
+#pragma unroll
+        for (int j = 0; j < GR; j++) {
+            vs[j] = (FMT == KVQ_INT8 ? __uint_as_float(vm[j]) : bf16_bits_to_float(vm[j] & 0xffffu)) * unit;
+            vl[j] = FMT == KVQ_INT8 ? 0.f : centre(vm[j]);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            float top[2];
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                top[c] = fmaxf(s[0][n][c], s[0][n][c + 2]);
+                if constexpr (S::MT == 2) top[c] = fmaxf(top[c], fmaxf(s[1][n][c], s[1][n][c + 2]));
+#pragma unroll
+                for (int x = 4; x < 32; x *= 2) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], x));
+                top[c] = fmaxf(top[c], m[n][c]);
+                const float base = top[c] == -INFINITY ? 0.f : top[c];
+                alpha[n][c] = exp2_fast(m[n][c] - base);
+                m[n][c] = top[c];
+                top[c] = base;
+                l[n][c] *= alpha[n][c];
+                z[n][c] *= alpha[n][c];
+            }
+#pragma unroll
+            for (int i = 0; i < S::MT; i++) {
+                float w[4];
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const int j = 2 * i + (c >> 1);
+                    const float p = exp2_fast(s[i][n][c] - top[c & 1]);
+                    l[n][c & 1] += p;
+                    // what a row does not see has weight 0 even where V is NaN
+                    const bool see = full || s[i][n][c] != -INFINITY;
+                    w[c] = see ? p * vs[j] : 0.f;
+                    if (FMT == KVQ_INT4 && see) z[n][c & 1] = fmaf(p, vl[j], z[n][c & 1]);
+                }
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const uint32_t hi = h2_pack(w[2 * j], w[2 * j + 1]);
+                    pb[i][n][0][j] = transpose8x8(hi);
+                    if constexpr (SPLIT) {
+                        const float2 f = h2_floats(hi);
+                        pb[i][n][1][j] = transpose8x8(h2_pack(w[2 * j] - f.x, w[2 * j + 1] - f.y));
+                    }
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 2; c++) alpha[n][c] *= grow;
+        }
+        // O^T += V^T P^T, two rows of 8 dims (dims 2 i, 2 i + 1 of each lane) at a time
+#pragma unroll
+        for (int i = 0; i < S::VD / 2; i++) {
+            float acc[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) acc[n][c] = 0.f;
+#pragma unroll
+            for (int k = 0; k < S::MT; k++) {
+                uint32_t f[2][2];  // [dim][positions 2t,2t+1 | +8]
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int gr = 2 * k + j;
+                    if constexpr (FMT == KVQ_INT8) {
+                        const uint32_t x = __byte_perm(vr[gr][0][i / 2], vr[gr][1][i / 2], i % 2 ? 0x7362 : 0x5140);
+                        f[0][j] = codes8<false>(x);
+                        f[1][j] = codes8<true>(x);
+                    } else {
+                        const uint32_t x = __byte_perm(vr[gr][0][i / 4], vr[gr][1][i / 4], (i % 4) / 2 ? 0x7632 : 0x5410);
+                        f[0][j] = i % 2 ? codes4<2>(x) : codes4<0>(x);
+                        f[1][j] = i % 2 ? codes4<3>(x) : codes4<1>(x);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int p = 0; p < S::PARTS; p++)
+                        mma_f16(acc[n], f[0][0], f[1][0], f[0][1], f[1][1], pb[k][n][p][0], pb[k][n][p][1]);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) o[i][n][c] = fmaf(o[i][n][c], alpha[n][c & 1], acc[n][c]);
+        }
+        if (next < tiles) load_v(next, held);
+    }
+
+    // ---- merge the warps ------------------------------------------------------------
+    const float back = __uint_as_float((vexp + 127u - 140u) << 23);  // 2^(vexp - 140)
+    __syncthreads();  // q's fragments are done with
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+#pragma unroll
+            for (int x = 4; x < 32; x *= 2) {
+                l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], x);
+                z[n][c] += __shfl_xor_sync(0xffffffffu, z[n][c], x);
+            }
+            const int r = 8 * n + 2 * t + c;
+            if (g == 0) sml[warp * S::ROWS + r] = make_float2(m[n][c], l[n][c]);
+            float* to = so + (warp * S::ROWS + r) * S::O_STRIDE + g * S::VD;
+#pragma unroll
+            for (int i = 0; i < S::VD / 2; i++)
+                *reinterpret_cast<float2*>(to + 2 * i) =
+                    make_float2(fmaf(o[i][n][c], back, z[n][c]), fmaf(o[i][n][c + 2], back, z[n][c]));
+        }
+    __syncthreads();
+    for (int at = tid; at < n_rows * hd; at += KVA_WARPS * 32) {
+        const int r = at / hd, d = at - r * hd;
+        float top = -INFINITY, sum = 0.f, x = 0.f;
+#pragma unroll
+        for (int w = 0; w < KVA_WARPS; w++) top = fmaxf(top, sml[w * S::ROWS + r].x);
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < KVA_WARPS; w++) {
+            const float2 ml = sml[w * S::ROWS + r];
+            const float f = exp2_fast(ml.x - base);
+            sum = fmaf(ml.y, f, sum);
+            x = fmaf(so[(w * S::ROWS + r) * S::O_STRIDE + d], f, x);
+        }
+        const int node = (row0 + r) / a.share, h = head * a.share + (row0 + r) - node * a.share;
+        const size_t item = (size_t)(first + node) * a.n_heads + h;
+        if (a.splits == 1) {
+            a.store_out(item * hd + d, sum == 0.f ? 0.f : x / sum);  // 0: nothing seen (NaN stays)
+            if (d == 0 && a.lse) a.lse[item] = 0.693147180559945309f * (top + log2f(sum));
+        } else {
+            a.part_o[(item * a.splits + split) * hd + d] = x;
+            if (d == 0) a.part_ml[item * a.splits + split] = make_float2(top, sum);
         }
     }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    if (mine) {
+}
+
+// One warp per (row, head): the chunks' parts by their maxima.
+__global__ void __launch_bounds__(128) k_kvq_attend_merge(KvqAttnArgs a) {
+    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.y;
+    int first, count;
+    a.rows_of(b, first, count);
+    const int at = blockIdx.x * 4 + warp;
+    if (at >= count * a.n_heads) return;
+    const size_t item = (size_t)first * a.n_heads + at;
+    const float2* ml = a.part_ml + item * a.splits;
+    const float* part = a.part_o + item * a.splits * a.c.hd;
+    float top = -INFINITY;
+    for (int s = lane; s < a.splits; s += 32) top = fmaxf(top, __ldcg(ml + s).x);
+    top = warp_max(top);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.splits; s++) {
+        const float2 w = __ldcg(ml + s);
+        if (w.y == 0.f) continue;  // nothing seen there, maybe no part written
+        const float f = kva::exp2_fast(w.x - base);
+        sum = fmaf(w.y, f, sum);
 #pragma unroll
-        for (int d = 0; d < 8; d++) o[d] *= inv;
-        store8((T*)a.out + ((size_t)row * a.n_heads + h) * a.c.hd + lane * 8, o);
+        for (int i = 0; i < 8; i++) {
+            const int d = lane + 32 * i;
+            if (d < a.c.hd) x[i] = fmaf(__ldcg(part + (size_t)s * a.c.hd + d), f, x[i]);
+        }
     }
-    if (a.lse && lane == 0) a.lse[(size_t)row * a.n_heads + h] = m + logf(l);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int d = lane + 32 * i;
+        if (d < a.c.hd) a.store_out(item * a.c.hd + d, sum == 0.f ? 0.f : x[i] / sum);
+    }
+    if (a.lse && lane == 0) a.lse[item] = 0.693147180559945309f * (top + log2f(sum));
 }
 
 }  // namespace fb2

@@ -2,9 +2,12 @@
 // cache, attention over it, 4-bit linear layers, logit controls.  Checks of
 // arguments and launches; the kernels are in kvq.cuh, kvq_attn.cuh, w4.cuh
 // and logit_controls.cuh.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdint>
+#include <mutex>
+#include <set>
 
 #include "capi.cuh"
 #include "kvq.cuh"
@@ -42,6 +45,18 @@ void with_type(int dtype, F&& f) {
 
 void launched() { CK(cudaGetLastError()); }
 
+// Dynamic shared memory above 48 KB, once per kernel and device.
+void opt_in_smem(const void* kernel, int bytes) {
+    static std::mutex lock;
+    static std::set<std::pair<const void*, int>> done;
+    int device = 0;
+    CK(cudaGetDevice(&device));
+    std::lock_guard<std::mutex> hold(lock);
+    if (done.count({kernel, device})) return;
+    CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.insert({kernel, device});
+}
+
 void check_cache_sizes(const fb2_kvq_cache* c) {
     need(c, "cache is NULL");
     need(c->format == FB2_KVQ_INT8 || c->format == FB2_KVQ_INT4, "format must be FB2_KVQ_INT8 or FB2_KVQ_INT4");
@@ -67,21 +82,18 @@ KvqView view_of(const fb2_kvq_cache* c) {
     return v;
 }
 
-// lanes of a row at 8 values each, a power of two
+// lanes of a row at 16 values each, a power of two
 int row_lanes(int hd) {
-    int w = 2;
-    while (w * 8 < hd) w *= 2;
+    int w = 1;
+    while (w * 16 < hd) w *= 2;
     return w;
 }
-unsigned row_blocks(int64_t n_rows, int heads, int width) {
-    const int64_t blocks = (n_rows * heads * width + KVQ_THREADS - 1) / KVQ_THREADS;
-    need(blocks <= INT32_MAX, "too many rows for one call");
-    return (unsigned)blocks;
+dim3 row_grid(int n_rows, int heads, int width) {
+    const int per = KVQ_THREADS / width;
+    return dim3((unsigned)(((int64_t)n_rows + per - 1) / per), heads, 2);
 }
 
 }  // namespace
-
-extern "C" {
 
 int32_t fb2_kvq_sizes(const fb2_kvq_cache* c, int64_t* code_bytes, int64_t* meta_bytes) {
     return guarded([&] {
@@ -104,7 +116,7 @@ int32_t fb2_kvq_write(const fb2_kvq_cache* c, int32_t n_rows, const void* k, con
         const size_t es = size_of(dtype);
         need(aligned(k, es) && aligned(v, es) && aligned(slots, 4), "a tensor is not aligned to its element size");
         const int width = row_lanes(view.hd);
-        const dim3 grid(row_blocks(n_rows, view.heads, width), 2);
+        const dim3 grid = row_grid(n_rows, view.heads, width);
         const bool vec = aligned(k, 16) && aligned(v, 16) && k_row * es % 16 == 0 && k_head * es % 16 == 0 &&
                          v_row * es % 16 == 0 && v_head * es % 16 == 0;
         with_type(dtype, [&](auto t) {
@@ -129,7 +141,7 @@ int32_t fb2_kvq_read(const fb2_kvq_cache* c, int32_t n_rows, const int32_t* slot
         need(aligned(k, 16) && aligned(v, 16), "k and v must be 16-byte aligned");
         need(aligned(slots, 4), "slots is not aligned to its element size");
         const int width = row_lanes(view.hd);
-        const dim3 grid(row_blocks(n_rows, view.heads, width), 2);
+        const dim3 grid = row_grid(n_rows, view.heads, width);
         with_type(dtype, [&](auto t) {
             using T = decltype(t);
             auto kernel = view.row_bytes == view.hd ? k_kvq_read<T, KVQ_INT8> : k_kvq_read<T, KVQ_INT4>;
@@ -141,6 +153,21 @@ int32_t fb2_kvq_read(const fb2_kvq_cache* c, int32_t n_rows, const int32_t* slot
 
 // ---- attention ---------------------------------------------------------------
 namespace {
+// Chunks of positions: enough blocks to fill the device a few times over,
+// none shorter than a round of the four warps' tiles and none so long that
+// one long sequence among short ones runs alone.
+void plan_attention(KvqAttnArgs& k) {
+    const int64_t rows = (int64_t)k.max_nodes * k.share;
+    const int block = rows > 8 ? 16 : 8;
+    k.row_blocks = (int)((rows + block - 1) / block);
+    const int64_t units = (int64_t)k.n_seqs * k.c.heads * k.row_blocks;
+    const int64_t want = 148 * 8;
+    int64_t chunk = k.max_len * units / want;
+    chunk = std::min<int64_t>(std::max<int64_t>((chunk + 127) / 128 * 128, 128), 2048);
+    k.chunk = (int)chunk;
+    k.splits = std::max(1, (int)((k.max_len + chunk - 1) / chunk));
+}
+
 KvqAttnArgs attn_args(const fb2_kvq_cache* c, const fb2_kvq_attention* a) {
     need(a, "attention arguments are NULL");
     KvqAttnArgs k{};
@@ -172,20 +199,54 @@ KvqAttnArgs attn_args(const fb2_kvq_cache* c, const fb2_kvq_attention* a) {
     k.n_seqs = a->n_seqs;
     k.n_rows = a->n_rows;
     k.n_heads = a->n_heads;
-    k.max_pages = a->max_pages;
+    k.share = a->n_heads / c->n_kv_heads;
+    k.dtype = a->dtype;
     k.max_nodes = a->max_nodes;
     k.max_len = a->max_len && a->max_len < cap ? a->max_len : (int)cap;
     k.mask_words = a->mask_words;
     k.scale = a->scale;
+    plan_attention(k);
     return k;
+}
+
+int64_t attn_workspace(const KvqAttnArgs& k) {
+    if (k.splits == 1) return 0;
+    const int64_t parts = (int64_t)k.n_rows * k.n_heads * k.splits;
+    return (parts * 8 + 15) / 16 * 16 + parts * k.c.hd * 4;
+}
+
+template <int HD, int FMT, int NT, bool SPLIT>
+void launch_attend(const KvqAttnArgs& k, cudaStream_t stream) {
+    using S = KvaShape<HD, FMT, NT, SPLIT>;
+    auto kernel = k_kvq_attend<HD, FMT, NT, SPLIT>;
+    if (S::SMEM > 48 * 1024) opt_in_smem((const void*)kernel, S::SMEM);
+    const int64_t blocks = (int64_t)k.row_blocks * k.splits * k.c.heads;
+    need(blocks <= INT32_MAX, "too many rows for one call");
+    kernel<<<dim3((unsigned)blocks, k.n_seqs), KVA_WARPS * 32, S::SMEM, stream>>>(k);
+}
+template <int HD, int FMT>
+void launch_attend(const KvqAttnArgs& k, cudaStream_t stream) {
+    const bool wide = (int64_t)k.max_nodes * k.share > 8, split = k.dtype == FB2_F32;
+    if (wide)
+        split ? launch_attend<HD, FMT, 2, true>(k, stream) : launch_attend<HD, FMT, 2, false>(k, stream);
+    else
+        split ? launch_attend<HD, FMT, 1, true>(k, stream) : launch_attend<HD, FMT, 1, false>(k, stream);
+}
+template <int FMT>
+void launch_attend(const KvqAttnArgs& k, cudaStream_t stream) {
+    if (k.c.hd <= 64)
+        launch_attend<64, FMT>(k, stream);
+    else if (k.c.hd <= 128)
+        launch_attend<128, FMT>(k, stream);
+    else
+        launch_attend<256, FMT>(k, stream);
 }
 }  // namespace
 
 int32_t fb2_kvq_attend_workspace(const fb2_kvq_cache* c, const fb2_kvq_attention* a, int64_t* bytes) {
     return guarded([&] {
         need(bytes, "bytes is NULL");
-        attn_args(c, a);
-        *bytes = 0;
+        *bytes = attn_workspace(attn_args(c, a));
     });
 }
 
@@ -193,18 +254,30 @@ int32_t fb2_kvq_attend(const fb2_kvq_cache* c, const fb2_kvq_attention* a, void*
     return guarded([&] {
         const KvqAttnArgs k = attn_args(c, a);
         if (a->n_seqs == 0 || a->n_rows == 0) return;
-        need(k.q && k.out && k.prefix && (k.table || k.max_pages == 0), "NULL argument");
+        need(k.q && k.out && k.prefix && (k.table || a->max_pages == 0), "NULL argument");
         const size_t es = size_of(a->dtype);
         need(aligned(k.q, es) && aligned(k.lse, 4) && aligned(k.table, 4) && aligned(k.prefix, 4) && aligned(k.starts, 4) &&
                  aligned(k.mask, 4),
              "a tensor is not aligned to its element size");
         need(aligned(k.out, 16), "out must be 16-byte aligned");
-        const dim3 grid((k.n_heads + 3) / 4, k.max_nodes, k.n_seqs);
-        with_type(a->dtype, [&](auto t) {
-            using T = decltype(t);
-            auto kernel = k.c.row_bytes == k.c.hd ? k_kvq_attend<T, KVQ_INT8> : k_kvq_attend<T, KVQ_INT4>;
-            kernel<<<grid, 128, 0, (cudaStream_t)stream>>>(k);
-        });
+        KvqAttnArgs args = k;
+        const int64_t bytes = attn_workspace(k);
+        if (bytes) {
+            need(a->device_workspace && a->workspace_bytes >= bytes, "the workspace is too small");
+            need(aligned(a->device_workspace, 16), "the workspace must be 16-byte aligned");
+            const int64_t parts = (int64_t)k.n_rows * k.n_heads * k.splits;
+            args.part_ml = static_cast<float2*>(a->device_workspace);
+            args.part_o = reinterpret_cast<float*>(static_cast<char*>(a->device_workspace) + (parts * 8 + 15) / 16 * 16);
+        }
+        if (c->format == FB2_KVQ_INT8)
+            launch_attend<KVQ_INT8>(args, (cudaStream_t)stream);
+        else
+            launch_attend<KVQ_INT4>(args, (cudaStream_t)stream);
+        launched();
+        if (bytes) {
+            const int64_t blocks = ((int64_t)k.max_nodes * k.n_heads + 3) / 4;
+            launch_pdl(k_kvq_attend_merge, dim3((unsigned)blocks, k.n_seqs), dim3(128), 0, (cudaStream_t)stream, args);
+        }
         launched();
     });
 }
@@ -263,13 +336,129 @@ int32_t fb2_w4_pack(const fb2_w4_linear* w, const void* dense, int32_t dtype, in
     });
 }
 
+namespace {
+// Few rows take the 8-bit tiles (up to 4 tiles of 8 columns, one column for a
+// digit), more the 16-bit ones (one column, three for fp32).
+int w4_digits_of(int dtype) { return dtype == FB2_F32 ? 4 : 3; }
+int w4_parts(int dtype) { return dtype == FB2_F32 ? 3 : 1; }
+struct W4Shape {
+    bool narrow;
+    int tiles;   // of 8 columns: all (narrow), of a chunk (wide)
+    int per;     // rows of a chunk
+    int chunks;
+};
+W4Shape w4_shape(int rows, int dtype) {
+    const int64_t digits = (int64_t)rows * w4_digits_of(dtype), cols = (int64_t)rows * w4_parts(dtype);
+    if (digits <= 32) return {true, (int)((digits + 7) / 8), rows, 1};
+    const int tiles = cols <= 16 ? 2 : 4, per = tiles * 8 / w4_parts(dtype);
+    return {false, tiles, per, (rows + per - 1) / per};
+}
+
+// Blocks of 16 outputs per warp, and CTAs per cluster (which share the inputs).
+// More blocks per warp spread the columns' cost (16384 x 16384, one bf16 row:
+// 37.7 us with 1, 34.3 with 2, 31.9 with 4) where enough CTAs are left (4096 x
+// 4096: 7.6, 7.4, 8.7 us).  A cluster's sums cost 1 to 3 us, which pays only
+// where less than half of the SMs have a CTA (16384 x 64: 10.5 us alone, 6.6
+// by 4; 4096 x 4096: 7.4 alone, 7.7 by 2; 32 rows, 8192 x 2048: 62 alone, 25
+// by 4, 33 by 8).
+struct W4Plan {
+    int rt, ranks;
+};
+W4Plan w4_plan(const W4View& v, const W4Shape& shape) {
+    const int blocks = (v.N + 15) / 16, units = (v.k64 + 1) / 2;
+    W4Plan p{1, 1};
+    if (shape.narrow) {
+        p.rt = blocks >= 512 ? 4 : blocks >= 128 ? 2 : 1;
+        if (shape.tiles > 1) p.rt = std::min(p.rt, shape.tiles > 2 ? 1 : 2);  // registers
+        const int ctas = (blocks + p.rt - 1) / p.rt;
+        while (p.ranks < 8 && ctas * p.ranks * 2 <= 148 && p.ranks * 4 * W4_WARPS <= units) p.ranks *= 2;
+    } else {
+        const int ctas = (blocks + W4_WARPS - 1) / W4_WARPS;
+        while (p.ranks < 4 && (int64_t)ctas * shape.chunks * p.ranks * 2 <= 148 && p.ranks * 4 <= units) p.ranks *= 2;
+    }
+    return p;
+}
+struct W4Workspace {
+    int64_t columns, sums;
+};
+W4Workspace w4_workspace(const W4View& v, const W4Shape& s) {
+    const int64_t units = (int64_t)(v.k64 + 1) / 2 * s.chunks;
+    if (s.narrow) return {units * s.tiles * W4_COL, 0};
+    return {units * s.tiles * 2048, units * (128 >> v.group_shift) * s.tiles * 32};
+}
+// x in fixed point is made by the product itself where each warp has one or
+// two units of inputs, else by a launch before it (768 x 2304 fp32: 3.3 and 4.1
+// us; 1024 x 4096 bf16: 3.7 and 5.0; 4096 x 4096 fp16: 9.3 and 6.8; 16384 x
+// 16384 bf16: 44 and 32)
+bool w4_direct(const W4View& v, int rows, int dtype) { return rows * w4_digits_of(dtype) <= 8 && v.k64 <= 32; }
+
+template <class K, class... A>
+void launch_cluster(K kernel, dim3 grid, int threads, int smem, int ranks, bool early, cudaStream_t stream, A... args) {
+    if (smem > 48 * 1024) opt_in_smem((const void*)kernel, smem);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = early ? 2 : 1;
+    CK(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+template <class T, int RT, int NT, bool DIRECT>
+void launch_narrow(const W4View& v, int ranks, const T* x, int64_t x_row, const unsigned char* columns, int rows, T* y,
+                   int64_t y_row, int vec, cudaStream_t stream) {
+    const unsigned grid = ((v.N + 15) / 16 + RT - 1) / RT * ranks;
+    launch_cluster(k_w4_narrow<T, RT, NT, DIRECT>, dim3(grid), W4_WARPS * 32, W4Narrow<RT, NT, DIRECT>::SMEM, ranks, !DIRECT, stream,
+                   v, x, (long long)x_row, columns, rows, y, (long long)y_row, vec);
+}
+template <class T, int NT, bool DIRECT, class... A>
+void launch_narrow(const W4View& v, const W4Plan& p, A... args) {
+    if constexpr (NT == 1)
+        if (p.rt == 4) return launch_narrow<T, 4, NT, DIRECT>(v, p.ranks, args...);
+    if constexpr (NT <= 2)
+        if (p.rt == 2) return launch_narrow<T, 2, NT, DIRECT>(v, p.ranks, args...);
+    launch_narrow<T, 1, NT, DIRECT>(v, p.ranks, args...);
+}
+template <class T, int NT, int GS>
+void launch_wide(const W4View& v, const W4Shape& s, int ranks, const uint4* columns, const float* sums, int rows, T* y,
+                 int64_t y_row, cudaStream_t stream) {
+    launch_cluster(k_w4_wide<T, NT, GS>, dim3((unsigned)(((v.N + 15) / 16 + W4_WARPS - 1) / W4_WARPS * ranks), s.chunks),
+                   W4_WARPS * 32, W4Wide<NT>::SMEM, ranks, true, stream, v, columns, sums, rows, s.per, y, (long long)y_row);
+}
+template <class T, int NT, class... A>
+void launch_wide(const W4View& v, const W4Shape& s, A... args) {
+    if (v.group_shift == 5)
+        launch_wide<T, NT, 5>(v, s, args...);
+    else if (v.group_shift == 6)
+        launch_wide<T, NT, 6>(v, s, args...);
+    else
+        launch_wide<T, NT, 7>(v, s, args...);
+}
+template <class T, class... A>
+void launch_wide(const W4View& v, const W4Shape& s, const W4Plan& p, A... args) {
+    if (s.tiles == 2)
+        launch_wide<T, 2>(v, s, p.ranks, args...);
+    else
+        launch_wide<T, 4>(v, s, p.ranks, args...);
+}
+}  // namespace
+
 int32_t fb2_w4_matvec_workspace(const fb2_w4_linear* w, int32_t n_rows, int32_t dtype, int64_t* bytes) {
     return guarded([&] {
-        w4_view(w);
+        const W4View v = w4_view(w);
         check_dtype(dtype);
         need(n_rows >= 0, "n_rows must not be negative");
         need(bytes, "bytes is NULL");
         *bytes = 0;
+        if (n_rows == 0 || w4_direct(v, n_rows, dtype)) return;
+        const W4Workspace ws = w4_workspace(v, w4_shape(n_rows, dtype));
+        *bytes = ws.columns + ws.sums;
     });
 }
 
@@ -285,12 +474,47 @@ int32_t fb2_w4_matvec(const fb2_w4_linear* w, int32_t n_rows, const void* x, int
         const size_t es = size_of(dtype);
         need(aligned(x, es) && aligned(y, es) && aligned(v.bias, 4), "a tensor is not aligned to its element size");
         need(n_rows == 1 || y_row >= v.N, "y_row_stride must be at least out_features");
-        need(n_rows <= 65535, "n_rows must be at most 65535");
+        int64_t bytes = 0;
+        fb2_w4_matvec_workspace(w, n_rows, dtype, &bytes);
+        need(bytes == 0 || (workspace && workspace_bytes >= bytes), "the workspace is too small");
+        need(aligned(workspace, 16), "the workspace must be 16-byte aligned");
+        const int vec = aligned(x, 16) && (n_rows == 1 || x_row * es % 16 == 0);
+        const cudaStream_t st = (cudaStream_t)stream;
         with_type(dtype, [&](auto t) {
             using T = decltype(t);
-            k_w4_matvec<T><<<dim3((v.N + 3) / 4, n_rows), 128, 0, (cudaStream_t)stream>>>(v, (const T*)x, x_row, (T*)y, y_row);
+            const W4Shape shape = w4_shape(n_rows, dtype);
+            const W4Plan plan = w4_plan(v, shape);
+            const T* xt = (const T*)x;
+            T* yt = (T*)y;
+            if (bytes == 0) {
+                launch_narrow<T, 1, true>(v, plan, xt, x_row, (const unsigned char*)nullptr, n_rows, yt, y_row, vec, st);
+                return;
+            }
+            const W4Workspace ws = w4_workspace(v, shape);
+            unsigned char* columns = static_cast<unsigned char*>(workspace);
+            float* sums = reinterpret_cast<float*>(columns + ws.columns);
+            const int units = (v.k64 + 1) / 2;
+            const int64_t blocks = ((int64_t)units * shape.tiles * shape.chunks + 3) / 4;
+            need(blocks <= INT32_MAX && shape.chunks <= 65535, "too many rows for one call");
+            if (!shape.narrow) {
+                k_w4_columns<T><<<(unsigned)blocks, 128, 0, st>>>(xt, x_row, n_rows, shape.per, v.K, units, shape.tiles, shape.chunks,
+                                                                 v.group_shift, (uint4*)columns, sums, vec);
+                launched();
+                launch_wide<T>(v, shape, plan, (const uint4*)columns, (const float*)sums, n_rows, yt, y_row, st);
+                return;
+            }
+            k_w4_digits<T><<<(unsigned)blocks, 128, 0, st>>>(xt, x_row, n_rows, v.K, units, shape.tiles, v.group_shift, columns, vec);
+            launched();
+            const unsigned char* cols = columns;
+            if (shape.tiles == 1)
+                launch_narrow<T, 1, false>(v, plan, xt, x_row, cols, n_rows, yt, y_row, vec, st);
+            else if (shape.tiles == 2)
+                launch_narrow<T, 2, false>(v, plan, xt, x_row, cols, n_rows, yt, y_row, vec, st);
+            else if (shape.tiles == 3)
+                launch_narrow<T, 3, false>(v, plan, xt, x_row, cols, n_rows, yt, y_row, vec, st);
+            else
+                launch_narrow<T, 4, false>(v, plan, xt, x_row, cols, n_rows, yt, y_row, vec, st);
         });
-        launched();
     });
 }
 
@@ -322,13 +546,17 @@ int32_t fb2_logit_controls(const fb2_logit_control* c, void* stream) {
                       c->device_presence, c->device_frequency, c->device_bias_ids, c->device_bias_values,
                       c->device_bias_starts, c->device_allowed, c->device_mask_rows, c->logits_row_stride,
                       c->out_row_stride, c->n_tokens, c->n_biases, c->n_rows, c->vocab, c->n_masks, c->mask_words};
-        const dim3 grid((c->vocab + CTL_CHUNK - 1) / CTL_CHUNK, c->n_rows);
+        // long rows: few chunks, as each looks through the row's lists; few rows:
+        // enough chunks to give every SM some
+        int chunk = 16384;
+        while (chunk > 512 && (int64_t)((c->vocab + chunk - 1) / chunk) * c->n_rows < 148 * 3) chunk /= 2;
+        const dim3 grid((c->vocab + chunk - 1) / chunk, c->n_rows);
+        const int smem = chunk * 4 + chunk / 8;
         with_type(c->dtype, [&](auto t) {
             using T = decltype(t);
-            k_logit_controls<T><<<grid, CTL_THREADS, 0, (cudaStream_t)stream>>>(a);
+            if (smem > 48 * 1024) opt_in_smem((const void*)k_logit_controls<T>, smem);
+            k_logit_controls<T><<<grid, CTL_THREADS, smem, (cudaStream_t)stream>>>(a, chunk);
         });
         launched();
     });
 }
-
-}  // extern "C"

@@ -27,47 +27,76 @@ _CONTROL = struct.Struct("=12Q4q6i")
 
 _torch = None
 _codes: dict = {}
+_stream = _device = None
 
 
 def _t():
     """torch, imported at the first use: the rest of the package does without it."""
-    global _torch
+    global _torch, _stream, _device
     if _torch is None:
         import torch
         _codes.update({torch.float32: N.FB2_F32, torch.bfloat16: N.FB2_BF16, torch.float16: N.FB2_F16})
+        # the handle itself: a Stream object costs more than a small kernel
+        _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda index: torch.cuda.current_stream(index).cuda_stream)
+        _device = torch.cuda.current_device
         _torch = torch
     return _torch
 
 
+def _refuse(message: str):
+    raise ArgumentError(N.FB2_INVALID_ARG, message)
+
+
 def _need(ok: bool, message: str) -> None:
     if not ok:
-        raise ArgumentError(N.FB2_INVALID_ARG, message)
+        _refuse(message)
 
 
 def _code(dtype) -> int:
     code = _codes.get(dtype)
     if code is None:
-        raise ArgumentError(N.FB2_INVALID_ARG, f"dtype must be float32, bfloat16 or float16, not {dtype}")
+        _refuse(f"dtype must be float32, bfloat16 or float16, not {dtype}")
     return code
 
 
-def _plain(t, name: str, dtype, device) -> int:
-    """Address of a contiguous tensor of `dtype` on `device`; 0 for None."""
+def _plain(t, name: str, dtype, index: int) -> int:
+    """Address of a contiguous tensor of `dtype` on CUDA device `index`; 0 for None."""
     if t is None:
         return 0
-    if t.dtype is not dtype or t.device != device or not t.is_contiguous():
-        raise ArgumentError(N.FB2_INVALID_ARG, f"{name} must be a contiguous {dtype} tensor on {device}")
+    if t.dtype is not dtype or t.get_device() != index or not t.is_contiguous():
+        _refuse(f"{name} must be a contiguous {dtype} tensor on cuda:{index}")
     return t.data_ptr()
 
 
-def _run(device, fn, *args) -> None:
-    """fn(*args, stream) on `device`'s current stream."""
-    torch = _torch
-    if torch.cuda.current_device() == device.index:
-        N.check(fn(*args, torch.cuda.current_stream().cuda_stream))
+def _run(index: int, fn, *args) -> None:
+    """fn(*args, stream) on device `index`'s current stream."""
+    if _device() == index:
+        status = fn(*args, _stream(index))
     else:
-        with torch.cuda.device(device):
-            N.check(fn(*args, torch.cuda.current_stream().cuda_stream))
+        with _torch.cuda.device(index):
+            status = fn(*args, _stream(index))
+    if status:
+        N.check(status)
+
+
+class _Workspace:
+    """Scratch memory of a handle, one buffer for each stream that uses it:
+    calls of one stream run one after the other.  A call that is captured in a
+    graph gets a buffer of the graph's own, as its replays run elsewhere."""
+
+    def __init__(self):
+        self.buffers: dict = {}
+
+    def address(self, index: int, size: int) -> int:
+        if _torch.cuda.is_current_stream_capturing():
+            return _torch.empty(size, dtype=_torch.uint8, device=f"cuda:{index}").data_ptr()
+        stream = _stream(index)
+        held = self.buffers.get(stream)
+        if held is None or held[1] < size:
+            buffer = _torch.empty(size, dtype=_torch.uint8, device=f"cuda:{index}")
+            held = self.buffers[stream] = (buffer, size, buffer.data_ptr())
+        return held[2]
 
 
 class QuantKvCache:
@@ -89,9 +118,9 @@ class QuantKvCache:
               "codes must be a CUDA uint8 tensor [pages, kv heads, 2, page size, row bytes]")
         _need(head_dim == codes.shape[4] * (1 if fmt == "int8" else 2), f"row bytes do not fit head_dim {head_dim}")
         _need(tuple(meta.shape) == tuple(codes.shape[:4]), "meta must be [pages, kv heads, 2, page size]")
-        self.device = codes.device
-        p_codes = _plain(codes, "codes", torch.uint8, self.device)
-        p_meta = _plain(meta, "meta", torch.int32, self.device)
+        self.device, self._index = codes.device, codes.get_device()
+        p_codes = _plain(codes, "codes", torch.uint8, self._index)
+        p_meta = _plain(meta, "meta", torch.int32, self._index)
         self.codes, self.meta = codes, meta
         self.n_pages, self.n_kv_heads, _, self.page_size, _ = codes.shape
         self.head_dim, self.fmt = int(head_dim), fmt
@@ -99,8 +128,12 @@ class QuantKvCache:
         self._desc = _CACHE.pack(p_codes, p_meta, self.n_pages, self.page_size, self.n_kv_heads, self.head_dim,
                                  _FORMATS[fmt], 0)
         size = C.c_int64()
-        self._lib = N.load()
-        N.check(self._lib.fb2_kvq_sizes(self._desc, C.byref(size), C.byref(C.c_int64())))
+        L = N.load()
+        N.check(L.fb2_kvq_sizes(self._desc, C.byref(size), C.byref(C.c_int64())))
+        self._write, self._read, self._attend = L.fb2_kvq_write, L.fb2_kvq_read, L.fb2_kvq_attend
+        self._attend_workspace = L.fb2_kvq_attend_workspace
+        self._workspace, self._sizes = _Workspace(), {}
+        self._scale = 1.0 / math.sqrt(self.head_dim)
 
     @classmethod
     def empty(cls, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, fmt: str = "int8",
@@ -115,34 +148,35 @@ class QuantKvCache:
         return cls(codes, meta, head_dim, fmt)
 
     def _rows(self, t, name: str, rows: int, heads: int):
-        if t.dim() != 3 or t.shape[0] != rows or t.shape[1] != heads or t.shape[2] != self.head_dim:
-            raise ArgumentError(N.FB2_INVALID_ARG, f"{name} must be [{rows}, {heads}, {self.head_dim}]")
+        if tuple(t.shape) != (rows, heads, self.head_dim):
+            _refuse(f"{name} must be [{rows}, {heads}, {self.head_dim}]")
         stride = t.stride()
-        if stride[2] != 1 or t.device != self.device:
-            raise ArgumentError(N.FB2_INVALID_ARG, f"{name} must be on {self.device} with a contiguous last dimension")
+        if stride[2] != 1 or t.get_device() != self._index:
+            _refuse(f"{name} must be on {self.device} with a contiguous last dimension")
         return stride
 
     def write(self, k, v, slots) -> None:
         """Quantises rows k, v [rows, kv heads, head_dim] (any row and head
         strides) into the slots (int32, one per row, distinct; a negative one
         skips its row)."""
-        torch = _torch
-        rows = slots.numel()
-        ks, vs = self._rows(k, "k", rows, self.n_kv_heads), self._rows(v, "v", rows, self.n_kv_heads)
-        _need(v.dtype is k.dtype, "k and v must have the same dtype")
-        _run(self.device, self._lib.fb2_kvq_write, self._desc, rows, k.data_ptr(), v.data_ptr(), _code(k.dtype), ks[0],
-             ks[1], vs[0], vs[1], _plain(slots, "slots", torch.int32, self.device))
+        rows, heads = slots.numel(), self.n_kv_heads
+        ks, vs = self._rows(k, "k", rows, heads), self._rows(v, "v", rows, heads)
+        dtype = k.dtype
+        if v.dtype is not dtype:
+            _refuse("k and v must have the same dtype")
+        _run(self._index, self._write, self._desc, rows, k.data_ptr(), v.data_ptr(), _code(dtype), ks[0], ks[1], vs[0], vs[1],
+             _plain(slots, "slots", _torch.int32, self._index))
 
     def read(self, slots, dtype=None):
         """(k, v) [rows, kv heads, head_dim] of the slots as `dtype` (default
         float32); a slot outside the cache reads as zeros."""
-        torch = _torch
-        dtype = dtype or torch.float32
-        code = _code(dtype)
-        both = torch.empty((2, slots.numel(), self.n_kv_heads, self.head_dim), dtype=dtype, device=self.device)
-        k, v = both.unbind(0)
-        _run(self.device, self._lib.fb2_kvq_read, self._desc, slots.numel(),
-             _plain(slots, "slots", torch.int32, self.device), k.data_ptr(), v.data_ptr(), code)
+        dtype = dtype or _torch.float32
+        code, rows = _code(dtype), slots.numel()
+        where = _plain(slots, "slots", _torch.int32, self._index)
+        shape = (rows, self.n_kv_heads, self.head_dim)
+        k = _torch.empty(shape, dtype=dtype, device=self.device)
+        v = _torch.empty(shape, dtype=dtype, device=self.device)
+        _run(self._index, self._read, self._desc, rows, where, k.data_ptr(), v.data_ptr(), code)
         return k, v
 
     def attend(self, q, page_table, prefix_lens, starts=None, mask=None, scale: float | None = None,
@@ -160,22 +194,24 @@ class QuantKvCache:
         table's width): the tighter, the better the work is split.  out has
         q's dtype, lse [rows, heads] is float32; a row that sees nothing
         gives zeros and -inf."""
-        torch = _torch
-        device = self.device
+        torch, index = _torch, self._index
         _need(q.dim() == 3, "q must be [rows, heads, head_dim]")
-        rows, heads, _ = q.shape
+        rows, heads, dim = q.shape
         qs = self._rows(q, "q", rows, heads)
-        code = _code(q.dtype)
-        _need(page_table.dim() == 2 and page_table.dtype is torch.int32 and page_table.device == device and
-              (page_table.stride(1) == 1 or page_table.shape[1] <= 1),
-              f"page_table must be an int32 tensor [sequences, pages] on {device} with contiguous rows")
+        dtype = q.dtype
+        code, i32 = _code(dtype), torch.int32
+        if page_table.dim() != 2 or page_table.dtype is not i32 or page_table.get_device() != index:
+            _refuse(f"page_table must be an int32 tensor [sequences, pages] on {self.device}")
         seqs, pages = page_table.shape
-        _need(prefix_lens.numel() == seqs, "prefix_lens must have one entry per sequence")
+        row, step = page_table.stride()
+        if step != 1 and pages > 1:
+            _refuse("page_table must have contiguous rows")
+        if prefix_lens.numel() != seqs:
+            _refuse("prefix_lens must have one entry per sequence")
         words = 0
         if mask is not None:
-            _need(mask.dim() == 2 and mask.shape[0] == rows, "mask must be [rows, words]")
+            _need(mask.dim() == 2 and mask.shape[0] == rows and mask.shape[1] > 0, "mask must be [rows, words]")
             words = mask.shape[1]
-            _need(words > 0, "mask must have words")
         if starts is None:
             _need(max_nodes is None or max_nodes == 1, "starts is needed for more than one row per sequence")
             max_nodes = 1
@@ -183,21 +219,27 @@ class QuantKvCache:
             _need(starts.numel() == seqs + 1, "starts must have one entry more than there are sequences")
             if max_nodes is None:
                 max_nodes = max(rows, 1)
-        out = torch.empty((rows, heads, self.head_dim), dtype=q.dtype, device=device)
-        lse = torch.empty((rows, heads), dtype=torch.float32, device=device)
+        p_prefix = _plain(prefix_lens, "prefix_lens", i32, index)
+        p_starts, p_mask = _plain(starts, "starts", i32, index), _plain(mask, "mask", i32, index)
+        out = torch.empty((rows, heads, dim), dtype=dtype, device=self.device)
+        lse = torch.empty((rows, heads), dtype=torch.float32, device=self.device)
         if rows == 0:
             return out, lse
-        fields = [q.data_ptr(), out.data_ptr(), lse.data_ptr(), page_table.data_ptr(),
-                  _plain(prefix_lens, "prefix_lens", torch.int32, device),
-                  _plain(starts, "starts", torch.int32, device), _plain(mask, "mask", torch.int32, device), 0, 0, qs[0],
-                  qs[1], max(page_table.stride(0), pages), seqs, rows, heads, code, pages, max_nodes, max_len or 0, words,
-                  1.0 / math.sqrt(self.head_dim) if scale is None else scale, 0]
-        size = C.c_int64()
-        N.check(self._lib.fb2_kvq_attend_workspace(self._desc, _ATTENTION.pack(*fields), C.byref(size)))
-        if size.value:
-            workspace = torch.empty(size.value, dtype=torch.uint8, device=device)
-            fields[7], fields[8] = workspace.data_ptr(), size.value
-        _run(device, self._lib.fb2_kvq_attend, self._desc, _ATTENTION.pack(*fields))
+        sizes = (seqs, rows, heads, code, pages, max_nodes, max_len or 0, words,
+                 self._scale if scale is None else scale, 0)
+        head = (q.data_ptr(), out.data_ptr(), lse.data_ptr(), page_table.data_ptr(), p_prefix, p_starts, p_mask)
+        strides = (qs[0], qs[1], row if row > pages else pages)
+        # the workspace's size goes by these numbers alone
+        bound = (seqs, rows, heads, pages, max_nodes, max_len)
+        size = self._sizes.get(bound)
+        if size is None:
+            got = C.c_int64()
+            N.check(self._attend_workspace(self._desc, _ATTENTION.pack(*head, 0, 0, *strides, *sizes), C.byref(got)))
+            if len(self._sizes) >= 1024:
+                self._sizes.clear()
+            size = self._sizes[bound] = got.value
+        work = self._workspace.address(index, size) if size else 0
+        _run(index, self._attend, self._desc, _ATTENTION.pack(*head, work, size, *strides, *sizes))
         return out, lse
 
 
@@ -213,19 +255,22 @@ class W4Linear:
 
     def __init__(self, codes, meta, in_features: int, out_features: int, group: int, bias=None):
         torch = _t()
-        self.device = codes.device
         _need(codes.is_cuda, "codes must be a CUDA tensor")
-        p_codes, p_meta = _plain(codes, "codes", torch.int32, self.device), _plain(meta, "meta", torch.int32, self.device)
-        p_bias = _plain(bias, "bias", torch.float32, self.device)
+        self.device, self._index = codes.device, codes.get_device()
+        p_codes = _plain(codes, "codes", torch.int32, self._index)
+        p_meta = _plain(meta, "meta", torch.int32, self._index)
+        p_bias = _plain(bias, "bias", torch.float32, self._index)
         _need(bias is None or bias.numel() == out_features, "bias must have out_features entries")
         self.codes, self.meta, self.bias = codes, meta, bias
         self.in_features, self.out_features, self.group = int(in_features), int(out_features), int(group)
         self._desc = _LINEAR.pack(p_codes, p_meta, p_bias, self.in_features, self.out_features, self.group, 0)
-        self._lib = N.load()
+        L = N.load()
         n_codes, n_meta = C.c_int64(), C.c_int64()
-        N.check(self._lib.fb2_w4_sizes(self._desc, C.byref(n_codes), C.byref(n_meta)))
+        N.check(L.fb2_w4_sizes(self._desc, C.byref(n_codes), C.byref(n_meta)))
         _need(codes.numel() * 4 == n_codes.value and meta.numel() * 4 == n_meta.value,
               f"codes and meta must have {n_codes.value} and {n_meta.value} bytes")
+        self._matvec, self._matvec_workspace = L.fb2_w4_matvec, L.fb2_w4_matvec_workspace
+        self._workspace, self._sizes = _Workspace(), {}
 
     @classmethod
     def pack(cls, w, group: int = 64, bias=None) -> "W4Linear":
@@ -239,26 +284,33 @@ class W4Linear:
         codes = torch.zeros((blocks, -(-k // 64), 32, 4), dtype=torch.int32, device=w.device)
         meta = torch.zeros((blocks, -(-k // group), 16), dtype=torch.int32, device=w.device)
         self = cls(codes, meta, k, n, group, bias)
-        _run(w.device, self._lib.fb2_w4_pack, self._desc, w.data_ptr(), _code(w.dtype), max(w.stride(0), n))
+        _run(self._index, N.load().fb2_w4_pack, self._desc, w.data_ptr(), _code(w.dtype), max(w.stride(0), n))
         return self
 
     def __call__(self, x):
         """x [..., in] -> [..., out] in x's dtype; sums in fp32."""
-        torch = _torch
-        k, n = self.in_features, self.out_features
-        _need(x.dim() >= 1 and x.shape[-1] == k and x.device == self.device, f"x must be [..., {k}] on {self.device}")
-        code = _code(x.dtype)
-        flat = x if x.dim() == 2 else x.reshape(-1, k)
-        _need(flat.stride(1) == 1 or k == 1, "x must have a contiguous last dimension")
+        k, n, index, shape = self.in_features, self.out_features, self._index, x.shape
+        if len(shape) == 0 or shape[-1] != k or x.get_device() != index:
+            _refuse(f"x must be [..., {k}] on {self.device}")
+        dtype = x.dtype
+        code = _code(dtype)
+        flat = x if len(shape) == 2 else x.reshape(-1, k)
+        row, step = flat.stride()
+        if step != 1 and k != 1:
+            _refuse("x must have a contiguous last dimension")
         rows = flat.shape[0]
-        y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=self.device)
+        y = _torch.empty((*shape[:-1], n), dtype=dtype, device=self.device)
         if rows == 0:
             return y
-        size = C.c_int64()
-        N.check(self._lib.fb2_w4_matvec_workspace(self._desc, rows, code, C.byref(size)))
-        workspace = torch.empty(size.value, dtype=torch.uint8, device=self.device) if size.value else None
-        _run(self.device, self._lib.fb2_w4_matvec, self._desc, rows, flat.data_ptr(), flat.stride(0), y.data_ptr(), n, code,
-             workspace.data_ptr() if size.value else None, size.value)
+        size = self._sizes.get((rows, code))
+        if size is None:
+            got = C.c_int64()
+            N.check(self._matvec_workspace(self._desc, rows, code, C.byref(got)))
+            if len(self._sizes) >= 1024:
+                self._sizes.clear()
+            size = self._sizes[(rows, code)] = got.value
+        work = self._workspace.address(index, size) if size else None
+        _run(index, self._matvec, self._desc, rows, flat.data_ptr(), row, y.data_ptr(), n, code, work, size)
         return y
 
 
@@ -277,16 +329,21 @@ def logit_controls(logits, *, tokens=None, token_starts=None, repetition=None, p
     does not allow becomes -inf.  Computed in fp32; the result has the logits'
     dtype and goes to `out` (which may be `logits`) or a new tensor."""
     torch = _t()
-    device = logits.device
-    _need(logits.dim() == 2 and logits.is_cuda and (logits.stride(1) == 1 or logits.shape[1] <= 1),
-          "logits must be a CUDA tensor [rows, vocab] with contiguous rows")
+    if logits.dim() != 2 or not logits.is_cuda:
+        _refuse("logits must be a CUDA tensor [rows, vocab]")
     rows, vocab = logits.shape
-    code = _code(logits.dtype)
+    row, step = logits.stride()
+    index, dtype = logits.get_device(), logits.dtype
+    code = _code(dtype)
+    if step != 1 and vocab > 1:
+        _refuse("logits must have contiguous rows")
     if out is None:
-        out = torch.empty((rows, vocab), dtype=logits.dtype, device=device)
+        out = torch.empty((rows, vocab), dtype=dtype, device=logits.device)
+        out_row = vocab
     else:
-        _need(out.shape == logits.shape and out.dtype is logits.dtype and out.device == device and
+        _need(out.shape == logits.shape and out.dtype is dtype and out.get_device() == index and
               (out.stride(1) == 1 or vocab <= 1), "out must have the logits' shape, dtype, device and contiguous rows")
+        out_row = out.stride(0)
     i32, f32 = torch.int32, torch.float32
     _need((tokens is None) == (token_starts is None), "tokens and token_starts go together")
     _need(tokens is not None or (repetition is None and presence is None and frequency is None),
@@ -310,13 +367,13 @@ def logit_controls(logits, *, tokens=None, token_starts=None, repetition=None, p
     else:
         _need(mask_rows is None, "mask_rows needs allowed")
     args = _CONTROL.pack(
-        logits.data_ptr(), out.data_ptr(), _plain(tokens, "tokens", i32, device),
-        _plain(token_starts, "token_starts", i32, device), _plain(repetition, "repetition", f32, device),
-        _plain(presence, "presence", f32, device), _plain(frequency, "frequency", f32, device),
-        _plain(bias_ids, "bias_ids", i32, device), _plain(bias_values, "bias_values", f32, device),
-        _plain(bias_starts, "bias_starts", i32, device), _plain(allowed, "allowed", i32, device),
-        _plain(mask_rows, "mask_rows", i32, device), logits.stride(0), out.stride(0),
+        logits.data_ptr(), out.data_ptr(), _plain(tokens, "tokens", i32, index),
+        _plain(token_starts, "token_starts", i32, index), _plain(repetition, "repetition", f32, index),
+        _plain(presence, "presence", f32, index), _plain(frequency, "frequency", f32, index),
+        _plain(bias_ids, "bias_ids", i32, index), _plain(bias_values, "bias_values", f32, index),
+        _plain(bias_starts, "bias_starts", i32, index), _plain(allowed, "allowed", i32, index),
+        _plain(mask_rows, "mask_rows", i32, index), row, out_row,
         tokens.numel() if tokens is not None else 0, n_biases, rows, vocab, code, n_masks, words, 0)
     if rows and vocab:
-        _run(device, N.load().fb2_logit_controls, args)
+        _run(index, N.load().fb2_logit_controls, args)
     return out
