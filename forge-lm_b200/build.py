@@ -6,6 +6,8 @@ Steps:
      (the on-device sampler reproduces the host expf bit for bit).
   2. nvcc -gencode arch=compute_100a,code=sm_100a: one object per .cu file
      (in csrc/generated/), linked to libforge_b200.so.
+  3. g++ csrc/serving_binding.cpp -> _serving.so, the serving operators' calls
+     on torch tensors.
 No fast-math: the sampler's division and exponentials must round as IEEE.
 """
 from __future__ import annotations
@@ -16,6 +18,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -23,6 +26,7 @@ CSRC = os.path.join(HERE, "csrc")
 GEN = os.path.join(CSRC, "generated")
 OBJ = GEN  # the objects lie with the other generated files
 LIB = os.path.join(HERE, "libforge_b200.so")
+BINDING = os.path.join(HERE, "_serving.so")
 ROOT = os.path.dirname(HERE)
 
 NVCC_FLAGS = [
@@ -123,12 +127,39 @@ def _compile(unit: str, flags: list[str], force: bool, verbose: bool) -> str:
     return obj
 
 
+def _binding_command(out: str) -> list[str]:
+    """g++ for the Python extension _serving: torch's headers, the library
+    beside it (found through the extension's own folder)."""
+    import torch
+    from torch.utils import cpp_extension
+
+    includes = cpp_extension.include_paths() + [sysconfig.get_paths()["include"], "/usr/local/cuda/include"]
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    return ["g++", "-O2", "-std=c++20", "-shared", "-fPIC", "-fvisibility=hidden", "-w",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-isystem{i}" for i in includes],
+            os.path.join(CSRC, "serving_binding.cpp"), "-o", out, f"-L{HERE}", "-l:libforge_b200.so", f"-L{libs}",
+            "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN"]
+
+
+def build_binding(verbose: bool = False, force: bool = False) -> str:
+    """The extension module, compiled again where its source or the C header is newer."""
+    sources = [os.path.join(CSRC, "serving_binding.cpp"), os.path.join(ROOT, "include", "forge_b200.h")]
+    if force or _newer(BINDING, sources):
+        cmd = _binding_command(BINDING + ".tmp")
+        if verbose:
+            print(" ".join(cmd))
+        subprocess.run(cmd, check=True)
+        os.replace(BINDING + ".tmp", BINDING)
+    return BINDING
+
+
 def build(verbose: bool = False, force: bool = False) -> str:
     gen_fixups(verbose)
     sources = _sources()
     flags = _flags()
     same_flags = read_stamp().get("flags") == flags
     if not force and same_flags and not _newer(LIB, sources):
+        build_binding(verbose)
         return LIB
     os.makedirs(OBJ, exist_ok=True)
     units = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith(".cu")]
@@ -138,6 +169,7 @@ def build(verbose: bool = False, force: bool = False) -> str:
     os.replace(LIB + ".tmp", LIB)
     with open(stamp_path(), "w") as f:
         json.dump({"flags": flags, "sources_sha256": source_fingerprint(flags, sources)}, f)
+    build_binding(verbose, force)
     return LIB
 
 

@@ -60,6 +60,23 @@ FB2_DEV void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint3
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// a fresh sum
+FB2_DEV void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+FB2_DEV void mma_u8s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// a sum that starts at z0 in the even columns, z1 in the odd ones
+FB2_DEV void mma_u8s8_first(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int z0, int z1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(z0), "r"(z1));
+}
 FB2_DEV uint32_t transpose8x8(uint32_t a) {
     uint32_t d;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -120,10 +137,16 @@ FB2_DEV float exp2_fast(float x) {
 // movmatrix.  Dimensions and positions are assigned to fragments so that a
 // lane's K and V codes are consecutive bytes (K: 16 dims of a position; V: HD/8
 // dims of 2 positions); q's fragments are built in that order once.
-// q is scaled by a power of two to just below 2^13 and split in two fp16
-// terms (one for 16-bit types, whose values fit); P is scaled to just below
-// 2^14 together with the largest V scale so far, and split likewise.  Sums
-// over a tile start at zero and are added to the running fp32 sums.
+//
+// Scores take 8-bit integer tiles (16 positions x 32 dims, exact sums): the
+// codes are bytes as they lie in memory (int4: one or two logical operations
+// per four), and q is in fixed point, rint(q 2^(22 - e)) for max|q| < 2^e of
+// its row, in three digits of 8 bits, which is exact to 2^-23 of max|q|.  The
+// codes' offset (128, 8) is taken off where the sums start.
+// Values take fp16 tiles: what a probability adds can be of any size, so P
+// stays in floating point, scaled to just below 2^14 together with the
+// largest V scale so far (one fp16 term for the 16-bit types, two for fp32,
+// whose sums over a tile start at zero and are added to the running ones).
 constexpr int KVA_WARPS = 4;
 
 template <int HD, int FMT, int NT, bool SPLIT>
@@ -134,13 +157,13 @@ struct KvaShape {
     static constexpr int KW = FMT == KVQ_INT8 ? 4 : 2;  // words of a chunk
     static constexpr int VD = HD / 8;                 // dims of V per lane and position
     static constexpr int VW = FMT == KVQ_INT8 ? VD / 4 : VD / 8;
-    static constexpr int STEPS = HD / 16;
-    static constexpr int PARTS = SPLIT ? 2 : 1;
+    static constexpr int STEPS = HD / 32;             // of 32 dims
+    static constexpr int PARTS = SPLIT ? 2 : 1;       // terms of P
     static constexpr int ROWS = 8 * NT;
-    static constexpr int Q_BYTES = PARTS * NT * STEPS * 32 * 8;
+    static constexpr int Q_BYTES = NT * 3 * STEPS * 32 * 8;
     static constexpr int O_STRIDE = HD + 8;
     static constexpr int O_BYTES = KVA_WARPS * ROWS * O_STRIDE * 4;
-    static constexpr int SMEM = (Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES) + ROWS * 8 + KVA_WARPS * ROWS * 8;
+    static constexpr int SMEM = (Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES) + ROWS * 8 + ROWS * 16 + KVA_WARPS * ROWS * 8;
 };
 
 template <int HD, int FMT, int NT, bool SPLIT>
@@ -149,10 +172,11 @@ __global__ void __launch_bounds__(KVA_WARPS * 32) k_kvq_attend(KvqAttnArgs a) {
     using S = KvaShape<HD, FMT, NT, SPLIT>;
     extern __shared__ __align__(16) unsigned char smem[];
     constexpr int kBig = S::Q_BYTES > S::O_BYTES ? S::Q_BYTES : S::O_BYTES;
-    __half* sq = reinterpret_cast<__half*>(smem);
+    unsigned char* sq = smem;  // [row tile][digit][step][lane] 8 bytes
     float* so = reinterpret_cast<float*>(smem);
     float2* srow = reinterpret_cast<float2*>(smem + kBig);                        // (score factor, factor * sum q)
-    float2* sml = reinterpret_cast<float2*>(smem + kBig + S::ROWS * 8);           // [warp][row] (m, l)
+    int4* szero = reinterpret_cast<int4*>(smem + kBig + S::ROWS * 8);             // where each digit's sums start
+    float2* sml = reinterpret_cast<float2*>(smem + kBig + S::ROWS * 24);          // [warp][row] (m, l)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int b = blockIdx.y;
     const int rb = blockIdx.x % a.row_blocks, rest = blockIdx.x / a.row_blocks;
@@ -176,24 +200,27 @@ __global__ void __launch_bounds__(KVA_WARPS * 32) k_kvq_attend(KvqAttnArgs a) {
 
     // ---- the tile loop's addresses -------------------------------------------
     const int ps = 1 << a.c.page_shift, rbytes = a.c.row_bytes, hd = a.c.hd;
-    const int n_pages = a.c.n_slots >> a.c.page_shift;
+    const uint32_t n_pages = a.c.n_slots >> a.c.page_shift;
     const int tiles = (c1 - c0 + S::TT - 1) / S::TT;
     constexpr int GR = 2 * S::MT;        // 8-position groups of a tile, each in one page
-    constexpr int AHEAD = 32 / GR;       // tiles whose page ids a warp holds, one per lane
+    constexpr int AHEAD = 32 / GR;       // tiles whose groups a warp holds, one per lane
+    constexpr uint32_t NONE = 0xffffffffu;
     const int* table = a.table + b * a.table_stride;
-    int ids = -1;
+    // index of a group among all groups of 8 K or V rows (V's lie ps / 8 after K's)
+    uint32_t ids = NONE;
     auto load_ids = [&](int tile) {      // of tiles tile, tile + WARPS, ..
         const int pos = c0 + (tile + (lane / GR) * KVA_WARPS) * S::TT + (lane % GR) * 8;
-        ids = -1;
+        ids = NONE;
         if (pos < c1) {
-            const int id = __ldg(table + (pos >> a.c.page_shift));
-            if ((uint32_t)id < (uint32_t)n_pages) ids = id;
+            const uint32_t page = __ldg(table + (pos >> a.c.page_shift));
+            if (page < n_pages) ids = (((page * a.c.heads + head) * 2) << (a.c.page_shift - 3)) + ((pos & (ps - 1)) >> 3);
         }
     };
-    // index of the K row of the group's first position; < 0: none
-    auto group_row = [&](int id, int pos) -> long long {
-        return id < 0 ? -1 : (((((long long)id * a.c.heads + head) * 2) << a.c.page_shift) | (pos & (ps - 1)));
-    };
+    const uint32_t gbytes = 8 * rbytes;
+    const unsigned char* k_codes = a.c.codes + g * rbytes + t * (S::KW * 4);
+    const unsigned char* v_codes = a.c.codes + (ps + 2 * t) * rbytes + g * (S::VW * 4);
+    const uint32_t* k_meta = a.c.meta + g;
+    const uint32_t* v_meta = a.c.meta + ps + g;
     uint32_t kr[GR][S::KCH][S::KW], vr[GR][2][S::VW], km[GR], vm[GR];
     auto load_words = [&](const unsigned char* p, uint32_t* w, auto n) {
         constexpr int N = decltype(n)::value;
@@ -207,86 +234,118 @@ __global__ void __launch_bounds__(KVA_WARPS * 32) k_kvq_attend(KvqAttnArgs a) {
             w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
         }
     };
-    auto load_k = [&](int tile, int slot) {
+    constexpr int PIECE = S::VW > S::KW ? S::KW : S::VW;  // words of V at once, at most 16 dims
+    // whether all of a tile is there and a lane's pieces are all in the row
+    auto whole = [&](int tile, int slot) {
+        bool w = hd == HD && c0 + (tile + 1) * S::TT <= c1;
+#pragma unroll
+        for (int j = 0; j < GR; j++) w &= __shfl_sync(0xffffffffu, ids, slot * GR + j) != NONE;
+        return w;
+    };
+    auto load_k = [&](int tile, int slot, bool all) {
 #pragma unroll
         for (int j = 0; j < GR; j++) {
-            const int pos = c0 + tile * S::TT + j * 8;
-            const long long row = group_row(__shfl_sync(0xffffffffu, ids, slot * GR + j), pos);
-            const bool live = row >= 0 && pos + g < c1;
-            const unsigned char* p = a.c.codes + (row + g) * rbytes;
-            km[j] = live ? __ldg(a.c.meta + row + g) : 0u;
+            const uint32_t grp = __shfl_sync(0xffffffffu, ids, slot * GR + j);
+            const unsigned char* p = k_codes + (uint64_t)grp * gbytes;
+            if (all) {
+                km[j] = __ldg(k_meta + (uint64_t)grp * 8);
 #pragma unroll
-            for (int cc = 0; cc < S::KCH; cc++) {
-                const int chunk = t + 4 * cc;
+                for (int cc = 0; cc < S::KCH; cc++) load_words(p + cc * (S::KW * 16), kr[j][cc], std::integral_constant<int, S::KW>{});
+            } else {
+                const bool live = grp != NONE && c0 + tile * S::TT + j * 8 + g < c1;
+                km[j] = live ? __ldg(k_meta + (uint64_t)grp * 8) : 0u;
 #pragma unroll
-                for (int i = 0; i < S::KW; i++) kr[j][cc][i] = 0;
-                if (live && chunk * 16 < hd)
-                    load_words(p + chunk * (S::KW * 4), kr[j][cc], std::integral_constant<int, S::KW>{});
+                for (int cc = 0; cc < S::KCH; cc++) {
+#pragma unroll
+                    for (int i = 0; i < S::KW; i++) kr[j][cc][i] = 0;
+                    if (live && (t + 4 * cc) * 16 < hd) load_words(p + cc * (S::KW * 16), kr[j][cc], std::integral_constant<int, S::KW>{});
+                }
             }
         }
     };
-    auto load_v = [&](int tile, int slot) {
+    auto load_v = [&](int tile, int slot, bool all) {
 #pragma unroll
         for (int j = 0; j < GR; j++) {
-            const int pos = c0 + tile * S::TT + j * 8;
-            long long row = group_row(__shfl_sync(0xffffffffu, ids, slot * GR + j), pos);
-            const bool any = row >= 0;
-            row += ps;  // the V rows lie one page behind the K rows
-            vm[j] = any && pos + g < c1 ? __ldg(a.c.meta + row + g) : 0u;
+            const uint32_t grp = __shfl_sync(0xffffffffu, ids, slot * GR + j);
+            const unsigned char* p = v_codes + (uint64_t)grp * gbytes;
+            if (all) {
+                vm[j] = __ldg(v_meta + (uint64_t)grp * 8);
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const bool live = any && pos + 2 * t + e < c1;
-                const unsigned char* p = a.c.codes + (row + 2 * t + e) * rbytes + g * (S::VW * 4);
-                constexpr int PIECE = S::VW > S::KW ? S::KW : S::VW;  // at most 16 dims at once
+                for (int e = 0; e < 2; e++)
 #pragma unroll
-                for (int i = 0; i < S::VW; i++) vr[j][e][i] = 0;
+                    for (int i = 0; i < S::VW; i += PIECE)
+                        load_words(p + e * rbytes + 4 * i, vr[j][e] + i, std::integral_constant<int, PIECE>{});
+            } else {
+                const int pos = c0 + tile * S::TT + j * 8;
+                vm[j] = grp != NONE && pos + g < c1 ? __ldg(v_meta + (uint64_t)grp * 8) : 0u;
 #pragma unroll
-                for (int i = 0; i < S::VW; i += PIECE)
-                    if (live && g * S::VD + i * (S::VD / S::VW) < hd)
-                        load_words(p + 4 * i, vr[j][e] + i, std::integral_constant<int, PIECE>{});
+                for (int e = 0; e < 2; e++) {
+                    const bool live = grp != NONE && pos + 2 * t + e < c1;
+#pragma unroll
+                    for (int i = 0; i < S::VW; i++) vr[j][e][i] = 0;
+#pragma unroll
+                    for (int i = 0; i < S::VW; i += PIECE)
+                        if (live && g * S::VD + i * (S::VD / S::VW) < hd)
+                            load_words(p + e * rbytes + 4 * i, vr[j][e] + i, std::integral_constant<int, PIECE>{});
+                }
             }
         }
     };
     int held = 0;  // tiles of `ids` used up
     if (warp < tiles) {
         load_ids(warp);
-        load_k(warp, 0);
-        load_v(warp, 0);
+        const bool all = whole(warp, 0);
+        load_k(warp, 0, all);
+        load_v(warp, 0, all);
     }
 
     // ---- q's fragments (while the first tile is on its way) --------------------
+    // integer sums start at the bits of 1.5 2^23 (less the codes' offset): below
+    // 2^22 in size, they are then the bits of 1.5 2^23 + sum
+    constexpr int ZERO = 0x4b400000;
+    constexpr float ZERO_F = 12582912.0f;
     for (int r = warp; r < S::ROWS; r += KVA_WARPS) {
         float x[HD / 32], top = 0.f, sum = 0.f;
+        int digits[3] = {0, 0, 0};
         const int node = (row0 + r) / a.share, h = head * a.share + (row0 + r) - node * a.share;
 #pragma unroll
         for (int i = 0; i < HD / 32; i++) {
             const int d = lane + 32 * i;
             x[i] = r < n_rows && d < hd ? a.load_q(first + node, h, d) : 0.f;
-            top = fmaxf(top, fabsf(x[i]));
+            top = max_nan(top, fabsf(x[i]));
         }
-        top = warp_max(top);
-        // a power of two that brings max|q| just below 2^13; NaN or inf stay in x
-        const int e = top > 0.f && top < INFINITY ? ilogbf(top) : 0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const bool finite = top < INFINITY;
+        const int e = finite && top > 0.f ? ilogbf(top) + 1 : 0;  // max|q| < 2^e
 #pragma unroll
         for (int i = 0; i < HD / 32; i++) {
             const int d = lane + 32 * i, c = d >> 4, w = d & 15;
-            x[i] = scalbnf(x[i], 12 - e);
+            x[i] = finite ? rintf(scalbnf(x[i], 22 - e)) : 0.f;
             sum += x[i];
-            int step, reg, half;
-            if constexpr (FMT == KVQ_INT8) {
-                step = w >> 2, reg = (w >> 1) & 1, half = w & 1;
-            } else {
-                step = 2 * (w >> 3) + ((w >> 1) & 1), reg = w & 1, half = (w >> 2) & 1;
+            // digits of q + 128 (1 + 2^8 + 2^16), each less 128
+            const uint32_t q = (uint32_t)(int)x[i] + 0x808080u;
+            int step = 2 * (c >> 2) + (w >> 3), reg, byte;
+            if constexpr (FMT == KVQ_INT8)
+                reg = (w >> 2) & 1, byte = w & 3;
+            else
+                reg = w & 1, byte = (w >> 1) & 3;
+#pragma unroll
+            for (int k = 0; k < 3; k++) {
+                const int digit = (int)((q >> (8 * k)) & 0xffu) - 128;
+                digits[k] += digit;
+                sq[((((r >> 3) * 3 + k) * S::STEPS + step) * 32 + 4 * (r & 7) + (c & 3)) * 8 + 4 * reg + byte] = (unsigned char)digit;
             }
-            step += 4 * (c >> 2);
-            const __half hi = __float2half_rn(x[i]);
-            const int at = (((r >> 3) * S::STEPS + step) * 32 + 4 * (r & 7) + (c & 3)) * 4 + 2 * reg + half;
-            sq[at] = hi;
-            if constexpr (SPLIT) sq[at + NT * S::STEPS * 128] = __float2half_rn(x[i] - __half2float(hi));
         }
         sum = warp_sum(sum);
-        const float f = scalbnf(a.scale * 1.44269504088896341f, e - 12);
-        if (lane == 0) srow[r] = make_float2(f, sum * f);
+#pragma unroll
+        for (int k = 0; k < 3; k++) digits[k] = __reduce_add_sync(0xffffffffu, digits[k]);
+        if (lane == 0) {
+            const float f = finite ? scalbnf(a.scale * 1.44269504088896341f, e - 22) : NAN;
+            constexpr int off = FMT == KVQ_INT8 ? 128 : 8;
+            srow[r] = make_float2(f, sum * f);
+            szero[r] = make_int4(ZERO - off * digits[0], ZERO - off * digits[1], ZERO - off * digits[2], 0);
+        }
     }
     __syncthreads();
 
@@ -306,57 +365,61 @@ __global__ void __launch_bounds__(KVA_WARPS * 32) k_kvq_attend(KvqAttnArgs a) {
     for (int n = 0; n < NT; n++)
 #pragma unroll
         for (int i = 0; i < 2; i++) rowf[n][i] = srow[8 * n + 2 * t + i];
+    int zero[NT][2][3];
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int4 v = szero[8 * n + 2 * t + i];
+            zero[n][i][0] = v.x, zero[n][i][1] = v.y, zero[n][i][2] = v.z;
+        }
     // exponent field of the largest V scale so far (o is in units of
     // 2^(vexp - 126 - 14)); 20: small enough for every scale, 2^(140 - 20) is finite
     uint32_t vexp = 20;
 
     for (int tile = warp; tile < tiles; tile += KVA_WARPS) {
         const int pos0 = c0 + tile * S::TT;
-        // every position seen by every row?
-        bool full = pos0 + S::TT <= min(prefix, c1);
-#pragma unroll
-        for (int j = 0; j < GR; j++) full &= __shfl_sync(0xffffffffu, ids, held * GR + j) >= 0;
         uint32_t live = 0;  // groups with a page
-        if (!full)
 #pragma unroll
-            for (int j = 0; j < GR; j++) live |= (uint32_t)(__shfl_sync(0xffffffffu, ids, held * GR + j) >= 0) << j;
+        for (int j = 0; j < GR; j++) live |= (uint32_t)(__shfl_sync(0xffffffffu, ids, held * GR + j) != NONE) << j;
+        // every position seen by every row?
+        const bool full = pos0 + S::TT <= min(prefix, c1) && live == (1u << GR) - 1;
 
         float s[S::MT][NT][4];
 #pragma unroll
-        for (int i = 0; i < S::MT; i++)
+        for (int i = 0; i < S::MT; i++) {
+            int acc[NT][3][4];
 #pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) s[i][n][c] = 0.f;
-#pragma unroll
-        for (int st = 0; st < S::STEPS; st++) {
-            uint2 qf[NT][S::PARTS];
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int p = 0; p < S::PARTS; p++)
-                    qf[n][p] = reinterpret_cast<const uint2*>(sq)[((p * NT + n) * S::STEPS + st) * 32 + lane];
-#pragma unroll
-            for (int i = 0; i < S::MT; i++) {
-                uint32_t f[2][2];
+            for (int st = 0; st < S::STEPS; st++) {
+                uint32_t f[4];  // positions g | g + 8, first | second four dims
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
                     if constexpr (FMT == KVQ_INT8) {
-                        const uint32_t w = kr[2 * i + j][st / 4][st % 4];
-                        f[j][0] = codes8<false>(w);
-                        f[j][1] = codes8<true>(w);
+                        f[j] = kr[2 * i + j][st / 2][2 * (st % 2)];
+                        f[2 + j] = kr[2 * i + j][st / 2][2 * (st % 2) + 1];
                     } else {
-                        const uint32_t w = kr[2 * i + j][st / 4][(st % 4) / 2];
-                        f[j][0] = st % 2 ? codes4<2>(w) : codes4<0>(w);
-                        f[j][1] = st % 2 ? codes4<3>(w) : codes4<1>(w);
+                        const uint32_t w = kr[2 * i + j][st / 2][st % 2];
+                        f[j] = w & 0x0f0f0f0fu;
+                        f[2 + j] = (w >> 4) & 0x0f0f0f0fu;
                     }
                 }
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int p = 0; p < S::PARTS; p++)
-                        mma_f16(s[i][n], f[0][0], f[1][0], f[0][1], f[1][1], qf[n][p].x, qf[n][p].y);
+                    for (int k = 0; k < 3; k++) {
+                        const uint2 qf = reinterpret_cast<const uint2*>(sq)[((n * 3 + k) * S::STEPS + st) * 32 + lane];
+                        if (st == 0)
+                            mma_u8s8_first(acc[n][k], f, qf.x, qf.y, zero[n][0][k], zero[n][1][k]);
+                        else
+                            mma_u8s8(acc[n][k], f, qf.x, qf.y);
+                    }
             }
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    s[i][n][c] = fmaf(fmaf(__int_as_float(acc[n][2][c]) - ZERO_F, 256.f, __int_as_float(acc[n][1][c]) - ZERO_F), 256.f,
+                                      __int_as_float(acc[n][0][c]) - ZERO_F);
         }
         // scores in units of log2
 #pragma unroll
@@ -395,12 +458,14 @@ __global__ void __launch_bounds__(KVA_WARPS * 32) k_kvq_attend(KvqAttnArgs a) {
         }
         // the next tile's K goes out: its registers are free
         const int next = tile + KVA_WARPS;
+        bool all = false;
         if (next < tiles) {
             if (++held == AHEAD) {
                 held = 0;
                 load_ids(next);
             }
-            load_k(next, held);
+            all = whole(next, held);
+            load_k(next, held, all);
         }
         // V's scales: the largest finite one sets the unit of o
         uint32_t vtop = 0;
@@ -465,14 +530,22 @@ __global__ void __launch_bounds__(KVA_WARPS * 32) k_kvq_attend(KvqAttnArgs a) {
 #pragma unroll
             for (int c = 0; c < 2; c++) alpha[n][c] *= grow;
         }
+        if constexpr (!SPLIT) {  // the running sums are the tiles' accumulators
+            bool same = true;
+#pragma unroll
+            for (int n = 0; n < NT; n++) same &= alpha[n][0] == 1.f && alpha[n][1] == 1.f;
+            if (!__all_sync(0xffffffffu, same))
+#pragma unroll
+                for (int i = 0; i < S::VD / 2; i++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) o[i][n][c] *= alpha[n][c & 1];
+        }
         // O^T += V^T P^T, two rows of 8 dims (dims 2 i, 2 i + 1 of each lane) at a time
 #pragma unroll
         for (int i = 0; i < S::VD / 2; i++) {
             float acc[NT][4];
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) acc[n][c] = 0.f;
 #pragma unroll
             for (int k = 0; k < S::MT; k++) {
                 uint32_t f[2][2];  // [dim][positions 2t,2t+1 | +8]
@@ -492,15 +565,22 @@ __global__ void __launch_bounds__(KVA_WARPS * 32) k_kvq_attend(KvqAttnArgs a) {
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int p = 0; p < S::PARTS; p++)
-                        mma_f16(acc[n], f[0][0], f[1][0], f[0][1], f[1][1], pb[k][n][p][0], pb[k][n][p][1]);
+                    for (int p = 0; p < S::PARTS; p++) {
+                        if (!SPLIT)
+                            mma_f16(o[i][n], f[0][0], f[1][0], f[0][1], f[1][1], pb[k][n][p][0], pb[k][n][p][1]);
+                        else if (k == 0 && p == 0)
+                            mma_f16_first(acc[n], f[0][0], f[1][0], f[0][1], f[1][1], pb[k][n][p][0], pb[k][n][p][1]);
+                        else
+                            mma_f16(acc[n], f[0][0], f[1][0], f[0][1], f[1][1], pb[k][n][p][0], pb[k][n][p][1]);
+                    }
             }
+            if constexpr (SPLIT)
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+                for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int c = 0; c < 4; c++) o[i][n][c] = fmaf(o[i][n][c], alpha[n][c & 1], acc[n][c]);
+                    for (int c = 0; c < 4; c++) o[i][n][c] = fmaf(o[i][n][c], alpha[n][c & 1], acc[n][c]);
         }
-        if (next < tiles) load_v(next, held);
+        if (next < tiles) load_v(next, held, all);
     }
 
     // ---- merge the warps ------------------------------------------------------------

@@ -186,6 +186,8 @@ KvqAttnArgs attn_args(const fb2_kvq_cache* c, const fb2_kvq_attention* a) {
     need(a->table_stride >= a->max_pages, "table_stride must be at least max_pages");
     const int64_t cap = (int64_t)a->max_pages * c->page_size;
     need(cap <= INT32_MAX, "max_pages * page_size must be at most 2^31 - 1");
+    // groups of 8 rows are counted in 32 bits (a cache of that size has over 270 GB)
+    need((int64_t)c->n_pages * c->page_size / 8 * 2 * c->n_kv_heads < UINT32_MAX, "the cache is too large");
     k.q = a->device_q;
     k.out = a->device_out;
     k.lse = a->device_lse;
