@@ -38,6 +38,38 @@ struct KvqView {
 FB2_DEV float bf16_bits_to_float(uint32_t b) { return __uint_as_float(b << 16); }
 FB2_DEV uint32_t float_to_bf16_bits(float f) { return (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(f)); }
 
+// Copies from global to shared memory that wait nowhere (cp.async), and reads
+// of shared memory by its 32-bit addresses.  `live` false: zeros are written.
+FB2_DEV void copy16(uint32_t to, const void* from, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
+}
+FB2_DEV void copy16(uint32_t to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+FB2_DEV void copy8(uint32_t to, const void* from, bool live) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(live ? 8 : 0) : "memory");
+}
+FB2_DEV void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+FB2_DEV void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+FB2_DEV uint4 lds4(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+FB2_DEV float2 lds2(uint32_t at) {
+    float2 v;
+    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at));
+    return v;
+}
+FB2_DEV uint32_t lds(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
+    return v;
+}
+
 // Element types of dense tensors: 8 consecutive values <-> fp32.
 template <class T>
 struct Dense;

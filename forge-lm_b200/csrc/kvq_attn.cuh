@@ -28,7 +28,7 @@ struct KvqAttnArgs {
     float2* part_ml;         // (m, l) of each, where splits > 1
     long long q_row, q_head, table_stride;
     int n_seqs, n_rows, n_heads, share, max_nodes, max_len, mask_words, dtype;
-    int splits, chunk, row_blocks;
+    int splits, chunk, row_blocks, warps;
     float scale;
     FB2_DEV void rows_of(int b, int& first, int& count) const {
         first = starts ? __ldg(starts + b) : b;
@@ -71,11 +71,11 @@ FB2_DEV void mma_u8s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// a sum that starts at z0 in the even columns, z1 in the odd ones
-FB2_DEV void mma_u8s8_first(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int z0, int z1) {
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+// a sum that starts at z
+FB2_DEV void mma_u8s8_first(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const int (&z)[4]) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
         : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(z0), "r"(z1));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(z[0]), "r"(z[1]), "r"(z[2]), "r"(z[3]));
 }
 FB2_DEV uint32_t transpose8x8(uint32_t a) {
     uint32_t d;
@@ -126,7 +126,7 @@ FB2_DEV float exp2_fast(float x) {
 
 }  // namespace kva
 
-// A CTA of 4 warps takes one chunk of one sequence's positions for one K/V
+// A CTA takes one chunk of one sequence's positions for one K/V
 // head and a block of 8 NT rows (the rows of its tokens and of the query
 // heads that share the K/V head).  Each warp works on its own tiles of 16 MT
 // positions from global memory to registers, with no barrier until the end:
@@ -144,15 +144,13 @@ FB2_DEV float exp2_fast(float x) {
 // its row, in three digits of 8 bits, which is exact to 2^-23 of max|q|.  The
 // codes' offset (128, 8) is taken off where the sums start.
 // Values take fp16 tiles: what a probability adds can be of any size, so P
-// stays in floating point, scaled to just below 2^14 together with the
-// largest V scale so far (one fp16 term for the 16-bit types, two for fp32,
+// stays in floating point, scaled together with the V scales (one fp16 term for the 16-bit types, two for fp32,
 // whose sums over a tile start at zero and are added to the running ones).
-constexpr int KVA_WARPS = 4;
-
-template <int HD, int FMT, int NT, bool SPLIT>
+template <int HD, int FMT, int NT, bool SPLIT, int WARPS>
 struct KvaShape {
     static constexpr int MT = HD > 128 ? 1 : 2;       // 16-position groups of a tile
     static constexpr int TT = 16 * MT;                // positions of a tile
+    static constexpr int RB = FMT == KVQ_INT8 ? HD : HD / 2;  // bytes of a row in shared memory
     static constexpr int KCH = HD / 64;               // 16-dim chunks of K per lane and position
     static constexpr int KW = FMT == KVQ_INT8 ? 4 : 2;  // words of a chunk
     static constexpr int VD = HD / 8;                 // dims of V per lane and position
@@ -160,23 +158,38 @@ struct KvaShape {
     static constexpr int STEPS = HD / 32;             // of 32 dims
     static constexpr int PARTS = SPLIT ? 2 : 1;       // terms of P
     static constexpr int ROWS = 8 * NT;
+    // a warp's ring: two tiles of K rows, V rows (by groups of 8 positions) and
+    // meta words
+    static constexpr int GROUP = 16 * RB, META = TT / 8 * GROUP, SLOT = META + 2 * TT * 4, DEPTH = 2;
+    static constexpr int RING = WARPS * DEPTH * SLOT;
     static constexpr int Q_BYTES = NT * 3 * STEPS * 32 * 8;
     static constexpr int O_STRIDE = HD + 8;
-    static constexpr int O_BYTES = KVA_WARPS * ROWS * O_STRIDE * 4;
-    static constexpr int SMEM = (Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES) + ROWS * 8 + ROWS * 16 + KVA_WARPS * ROWS * 8;
+    static constexpr int O_BYTES = WARPS * ROWS * O_STRIDE * 4;
+    static constexpr int BIG = RING > O_BYTES ? RING : O_BYTES;  // the merge takes the rings' place
+    static constexpr int SMEM = BIG + Q_BYTES + ROWS * 8 + ROWS * 16 + WARPS * ROWS * 8;
+    // CTAs per SM that the registers are kept to (shared memory allows them)
+    static constexpr int RESIDENT = WARPS == 8 ? 1 : NT == 1 ? (HD == 64 || (HD == 128 && FMT == KVQ_INT4) ? 4 : HD == 128 ? 3 : 2) : 2;
+    // Where 16-byte unit u of 8 rows lies: moved within its 128-byte line so
+    // that the K reads (8 neighbouring rows, a run of each) and the V reads
+    // (every second row, another run) both spread over the banks.
+    static FB2_DEV uint32_t place(uint32_t u) {
+        if constexpr (RB == 32) return u ^ (((u >> 3) & 1) << 1);
+        if constexpr (RB == 64) return u ^ (((u >> 3) & 3) << 1);
+        const uint32_t row = u / (RB / 16);
+        return u ^ ((((row >> 1) & 3) << 1) ^ ((row & 1) << 2));
+    }
 };
 
-template <int HD, int FMT, int NT, bool SPLIT>
-__global__ void __launch_bounds__(KVA_WARPS * 32) k_kvq_attend(KvqAttnArgs a) {
+template <int HD, int FMT, int NT, bool SPLIT, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, KvaShape<HD, FMT, NT, SPLIT, WARPS>::RESIDENT) k_kvq_attend(KvqAttnArgs a) {
     using namespace kva;
-    using S = KvaShape<HD, FMT, NT, SPLIT>;
+    using S = KvaShape<HD, FMT, NT, SPLIT, WARPS>;
     extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int kBig = S::Q_BYTES > S::O_BYTES ? S::Q_BYTES : S::O_BYTES;
-    unsigned char* sq = smem;  // [row tile][digit][step][lane] 8 bytes
     float* so = reinterpret_cast<float*>(smem);
-    float2* srow = reinterpret_cast<float2*>(smem + kBig);                        // (score factor, factor * sum q)
-    int4* szero = reinterpret_cast<int4*>(smem + kBig + S::ROWS * 8);             // where each digit's sums start
-    float2* sml = reinterpret_cast<float2*>(smem + kBig + S::ROWS * 24);          // [warp][row] (m, l)
+    unsigned char* sq = smem + S::BIG;                                  // [row tile][digit][two steps][lane] 16 bytes
+    float4* szero = reinterpret_cast<float4*>(sq + S::Q_BYTES);         // what to take off each digit's sums
+    float2* srow = reinterpret_cast<float2*>(sq + S::Q_BYTES + S::ROWS * 16);  // (score factor, factor * sum q)
+    float2* sml = srow + S::ROWS;                                       // [warp][row] (m, l)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int b = blockIdx.y;
     const int rb = blockIdx.x % a.row_blocks, rest = blockIdx.x / a.row_blocks;
@@ -191,7 +204,7 @@ __global__ void __launch_bounds__(KVA_WARPS * 32) k_kvq_attend(KvqAttnArgs a) {
     // row r of the block: token (row0 + r) / share of the sequence, query head
     // head * share + (row0 + r) % share
     if (c0 >= c1 && a.splits > 1) {  // nothing here: the merge has to know
-        for (int r = tid; r < n_rows; r += KVA_WARPS * 32) {
+        for (int r = tid; r < n_rows; r += WARPS * 32) {
             const int node = (row0 + r) / a.share, h = head * a.share + (row0 + r) - node * a.share;
             a.part_ml[((size_t)(first + node) * a.n_heads + h) * a.splits + split] = make_float2(-INFINITY, 0.f);
         }
@@ -204,107 +217,100 @@ __global__ void __launch_bounds__(KVA_WARPS * 32) k_kvq_attend(KvqAttnArgs a) {
     const int tiles = (c1 - c0 + S::TT - 1) / S::TT;
     constexpr int GR = 2 * S::MT;        // 8-position groups of a tile, each in one page
     constexpr int AHEAD = 32 / GR;       // tiles whose groups a warp holds, one per lane
-    constexpr uint32_t NONE = 0xffffffffu;
     const int* table = a.table + b * a.table_stride;
     // index of a group among all groups of 8 K or V rows (V's lie ps / 8 after K's)
-    uint32_t ids = NONE;
+    uint32_t ids = 0, valid = 0;         // one group per lane; which of them have a page
     auto load_ids = [&](int tile) {      // of tiles tile, tile + WARPS, ..
-        const int pos = c0 + (tile + (lane / GR) * KVA_WARPS) * S::TT + (lane % GR) * 8;
-        ids = NONE;
-        if (pos < c1) {
-            const uint32_t page = __ldg(table + (pos >> a.c.page_shift));
-            if (page < n_pages) ids = (((page * a.c.heads + head) * 2) << (a.c.page_shift - 3)) + ((pos & (ps - 1)) >> 3);
-        }
+        const int pos = c0 + (tile + (lane / GR) * WARPS) * S::TT + (lane % GR) * 8;
+        const uint32_t page = pos < c1 ? (uint32_t)__ldg(table + (pos >> a.c.page_shift)) : n_pages;
+        valid = __ballot_sync(0xffffffffu, page < n_pages);
+        ids = page < n_pages ? (((page * a.c.heads + head) * 2) << (a.c.page_shift - 3)) + ((pos & (ps - 1)) >> 3) : 0;
     };
-    const uint32_t gbytes = 8 * rbytes;
-    const unsigned char* k_codes = a.c.codes + g * rbytes + t * (S::KW * 4);
-    const unsigned char* v_codes = a.c.codes + (ps + 2 * t) * rbytes + g * (S::VW * 4);
-    const uint32_t* k_meta = a.c.meta + g;
-    const uint32_t* v_meta = a.c.meta + ps + g;
-    uint32_t kr[GR][S::KCH][S::KW], vr[GR][2][S::VW], km[GR], vm[GR];
-    auto load_words = [&](const unsigned char* p, uint32_t* w, auto n) {
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * S::DEPTH * S::SLOT;
+    constexpr int UNITS = S::RB / 2, COPIES = (2 * UNITS + 31) / 32;  // 16-byte units of 8 rows; a lane's of a group
+    const unsigned char* copy_from[COPIES];
+    uint32_t copy_to[COPIES];
+#pragma unroll
+    for (int i = 0; i < COPIES; i++) {
+        const uint32_t u = 32 * i + lane, kind = u / UNITS, at = u % UNITS;
+        copy_from[i] = a.c.codes + kind * (ps * S::RB) + at * 16;
+        copy_to[i] = kind * (8 * S::RB) + S::place(at) * 16;
+    }
+    const uint32_t* meta_from = a.c.meta + ((lane >> 1) & 1) * ps + (lane & 1) * 4;
+    const uint32_t meta_to = S::META + ((lane >> 1) & 1) * (S::TT * 4) + (lane >> 2) * 32 + (lane & 1) * 16;
+    // Starts the copies of a tile; returns which of its groups have a page (the
+    // others are zeros).  Positions past c1 bring whatever the page holds there.
+    auto fetch = [&](int held, uint32_t to) {
+        const uint32_t live = (valid >> (held * GR)) & ((1u << GR) - 1);
+        const uint32_t mine = __shfl_sync(0xffffffffu, ids, (held * GR + (lane >> 2)) & 31);
+        const bool all = hd == HD && live == (1u << GR) - 1;
+#pragma unroll
+        for (int j = 0; j < GR; j++) {
+            const uint64_t skip = (uint64_t)__shfl_sync(0xffffffffu, ids, held * GR + j) * (uint32_t)(8 * rbytes);
+            const bool there = (live >> j) & 1;
+            if (all) {
+#pragma unroll
+                for (int i = 0; i < COPIES; i++) copy16(to + copy_to[i] + j * S::GROUP, copy_from[i] + skip);
+            } else if (hd == HD) {
+#pragma unroll
+                for (int i = 0; i < COPIES; i++) copy16(to + copy_to[i] + j * S::GROUP, copy_from[i] + skip, there);
+            } else {
+                // rows shorter than in shared memory: 8 bytes at a time
+                const int per = rbytes / 8;
+                for (int i = lane; i < 16 * per; i += 32) {
+                    const int row = i / per, at = i - row * per, kind = row >> 3;
+                    const uint32_t byte = (row & 7) * S::RB + at * 8;
+                    copy8(to + j * S::GROUP + kind * (8 * S::RB) + S::place(byte >> 4) * 16 + (byte & 8),
+                          a.c.codes + skip + kind * (ps * rbytes) + (row & 7) * rbytes + at * 8, there);
+                }
+            }
+        }
+        if (lane < 4 * GR) {  // group lane / 4: K's and V's 8 words, 4 at a time
+            copy16(to + meta_to, meta_from + (uint64_t)mine * 8, (live >> (lane >> 2)) & 1);
+        }
+        return live;
+    };
+    // a lane's reads in the first group: K chunks of position g, V of positions 2 t, 2 t + 1
+    uint32_t k_at[S::KCH], v_at[2][S::VW > 4 ? 2 : 1];
+#pragma unroll
+    for (int cc = 0; cc < S::KCH; cc++) {
+        const uint32_t byte = g * S::RB + (t + 4 * cc) * (S::KW * 4);
+        k_at[cc] = S::place(byte >> 4) * 16 + (byte & 15);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int i = 0; i < (S::VW > 4 ? 2 : 1); i++) {
+            const uint32_t byte = (2 * t + e) * S::RB + g * (S::VW * 4) + 16 * i;
+            v_at[e][i] = 8 * S::RB + S::place(byte >> 4) * 16 + (byte & 15);
+        }
+    auto read_words = [&](uint32_t at, uint32_t* w, auto n) {
         constexpr int N = decltype(n)::value;
         if constexpr (N == 1) {
-            w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+            w[0] = lds(at);
         } else if constexpr (N == 2) {
-            const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-            w[0] = v.x, w[1] = v.y;
+            const float2 v = lds2(at);
+            w[0] = __float_as_uint(v.x), w[1] = __float_as_uint(v.y);
         } else {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+            const uint4 v = lds4(at);
             w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
         }
     };
-    constexpr int PIECE = S::VW > S::KW ? S::KW : S::VW;  // words of V at once, at most 16 dims
-    // whether all of a tile is there and a lane's pieces are all in the row
-    auto whole = [&](int tile, int slot) {
-        bool w = hd == HD && c0 + (tile + 1) * S::TT <= c1;
-#pragma unroll
-        for (int j = 0; j < GR; j++) w &= __shfl_sync(0xffffffffu, ids, slot * GR + j) != NONE;
-        return w;
-    };
-    auto load_k = [&](int tile, int slot, bool all) {
-#pragma unroll
-        for (int j = 0; j < GR; j++) {
-            const uint32_t grp = __shfl_sync(0xffffffffu, ids, slot * GR + j);
-            const unsigned char* p = k_codes + (uint64_t)grp * gbytes;
-            if (all) {
-                km[j] = __ldg(k_meta + (uint64_t)grp * 8);
-#pragma unroll
-                for (int cc = 0; cc < S::KCH; cc++) load_words(p + cc * (S::KW * 16), kr[j][cc], std::integral_constant<int, S::KW>{});
-            } else {
-                const bool live = grp != NONE && c0 + tile * S::TT + j * 8 + g < c1;
-                km[j] = live ? __ldg(k_meta + (uint64_t)grp * 8) : 0u;
-#pragma unroll
-                for (int cc = 0; cc < S::KCH; cc++) {
-#pragma unroll
-                    for (int i = 0; i < S::KW; i++) kr[j][cc][i] = 0;
-                    if (live && (t + 4 * cc) * 16 < hd) load_words(p + cc * (S::KW * 16), kr[j][cc], std::integral_constant<int, S::KW>{});
-                }
-            }
-        }
-    };
-    auto load_v = [&](int tile, int slot, bool all) {
-#pragma unroll
-        for (int j = 0; j < GR; j++) {
-            const uint32_t grp = __shfl_sync(0xffffffffu, ids, slot * GR + j);
-            const unsigned char* p = v_codes + (uint64_t)grp * gbytes;
-            if (all) {
-                vm[j] = __ldg(v_meta + (uint64_t)grp * 8);
-#pragma unroll
-                for (int e = 0; e < 2; e++)
-#pragma unroll
-                    for (int i = 0; i < S::VW; i += PIECE)
-                        load_words(p + e * rbytes + 4 * i, vr[j][e] + i, std::integral_constant<int, PIECE>{});
-            } else {
-                const int pos = c0 + tile * S::TT + j * 8;
-                vm[j] = grp != NONE && pos + g < c1 ? __ldg(v_meta + (uint64_t)grp * 8) : 0u;
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const bool live = grp != NONE && pos + 2 * t + e < c1;
-#pragma unroll
-                    for (int i = 0; i < S::VW; i++) vr[j][e][i] = 0;
-#pragma unroll
-                    for (int i = 0; i < S::VW; i += PIECE)
-                        if (live && g * S::VD + i * (S::VD / S::VW) < hd)
-                            load_words(p + e * rbytes + 4 * i, vr[j][e] + i, std::integral_constant<int, PIECE>{});
-                }
-            }
-        }
-    };
     int held = 0;  // tiles of `ids` used up
+    uint32_t live_next = 0;
     if (warp < tiles) {
         load_ids(warp);
-        const bool all = whole(warp, 0);
-        load_k(warp, 0, all);
-        load_v(warp, 0, all);
+        live_next = fetch(0, ring);
     }
+    copies_commit();
 
     // ---- q's fragments (while the first tile is on its way) --------------------
-    // integer sums start at the bits of 1.5 2^23 (less the codes' offset): below
-    // 2^22 in size, they are then the bits of 1.5 2^23 + sum
-    constexpr int ZERO = 0x4b400000;
-    constexpr float ZERO_F = 12582912.0f;
-    for (int r = warp; r < S::ROWS; r += KVA_WARPS) {
+    // Integer sums start at the bits of 1.5 2^23: up to 2^22 in size, they are
+    // then the bits of 1.5 2^23 + sum (over 256 dims and bytes they are larger
+    // and converted).
+    constexpr bool BITS = !(HD == 256 && FMT == KVQ_INT8);
+    constexpr int START = BITS ? (int)kRintBits : 0;
+    for (int r = warp; r < S::ROWS; r += WARPS) {
         float x[HD / 32], top = 0.f, sum = 0.f;
         int digits[3] = {0, 0, 0};
         const int node = (row0 + r) / a.share, h = head * a.share + (row0 + r) - node * a.share;
@@ -317,11 +323,13 @@ __global__ void __launch_bounds__(KVA_WARPS * 32) k_kvq_attend(KvqAttnArgs a) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
         const bool finite = top < INFINITY;
-        const int e = finite && top > 0.f ? ilogbf(top) + 1 : 0;  // max|q| < 2^e
+        // max|q| < 2^e; below 2^-95 only what no score keeps is lost
+        const int e = finite ? max((int)(__float_as_uint(top) >> 23) - 126, -95) : 0;
+        const float up = __uint_as_float((uint32_t)(127 + 22 - e) << 23);
 #pragma unroll
         for (int i = 0; i < HD / 32; i++) {
             const int d = lane + 32 * i, c = d >> 4, w = d & 15;
-            x[i] = finite ? rintf(scalbnf(x[i], 22 - e)) : 0.f;
+            x[i] = finite ? rintf(x[i] * up) : 0.f;
             sum += x[i];
             // digits of q + 128 (1 + 2^8 + 2^16), each less 128
             const uint32_t q = (uint32_t)(int)x[i] + 0x808080u;
@@ -334,27 +342,29 @@ __global__ void __launch_bounds__(KVA_WARPS * 32) k_kvq_attend(KvqAttnArgs a) {
             for (int k = 0; k < 3; k++) {
                 const int digit = (int)((q >> (8 * k)) & 0xffu) - 128;
                 digits[k] += digit;
-                sq[((((r >> 3) * 3 + k) * S::STEPS + step) * 32 + 4 * (r & 7) + (c & 3)) * 8 + 4 * reg + byte] = (unsigned char)digit;
+                sq[((((r >> 3) * 3 + k) * (S::STEPS / 2) + step / 2) * 32 + 4 * (r & 7) + (c & 3)) * 16 + 8 * (step & 1) + 4 * reg + byte] =
+                    (unsigned char)digit;
             }
         }
         sum = warp_sum(sum);
 #pragma unroll
         for (int k = 0; k < 3; k++) digits[k] = __reduce_add_sync(0xffffffffu, digits[k]);
         if (lane == 0) {
-            const float f = finite ? scalbnf(a.scale * 1.44269504088896341f, e - 22) : NAN;
+            const float f = finite ? a.scale * 1.44269504088896341f * __uint_as_float((uint32_t)(127 - 22 + e) << 23) : NAN;
             constexpr int off = FMT == KVQ_INT8 ? 128 : 8;
             srow[r] = make_float2(f, sum * f);
-            szero[r] = make_int4(ZERO - off * digits[0], ZERO - off * digits[1], ZERO - off * digits[2], 0);
+            constexpr float start = BITS ? kRint : 0.f;
+            szero[r] = make_float4(start + (float)(off * digits[0]), start + (float)(off * digits[1]), start + (float)(off * digits[2]), 0.f);
         }
     }
     __syncthreads();
 
     // ---- the pass over the positions --------------------------------------------
-    float o[S::VD / 2][NT][4], m[NT][2], l[NT][2], z[NT][2];
+    float o[S::VD / 2][NT][4], base[NT][2], limit[NT][2], l[NT][2], z[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) m[n][i] = -INFINITY, l[n][i] = 0.f, z[n][i] = 0.f;
+        for (int i = 0; i < 2; i++) base[n][i] = 0.f, limit[n][i] = -INFINITY, l[n][i] = 0.f, z[n][i] = 0.f;
 #pragma unroll
         for (int i = 0; i < S::VD / 2; i++)
 #pragma unroll
@@ -365,61 +375,100 @@ __global__ void __launch_bounds__(KVA_WARPS * 32) k_kvq_attend(KvqAttnArgs a) {
     for (int n = 0; n < NT; n++)
 #pragma unroll
         for (int i = 0; i < 2; i++) rowf[n][i] = srow[8 * n + 2 * t + i];
-    int zero[NT][2][3];
+    float zero[NT][2][3];
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const int4 v = szero[8 * n + 2 * t + i];
+            const float4 v = szero[8 * n + 2 * t + i];
             zero[n][i][0] = v.x, zero[n][i][1] = v.y, zero[n][i][2] = v.z;
         }
-    // exponent field of the largest V scale so far (o is in units of
-    // 2^(vexp - 126 - 14)); 20: small enough for every scale, 2^(140 - 20) is finite
+    // Probabilities are exp2(s - base), base the largest score at the last time
+    // that one exceeded base + kLag (limit; -inf: nothing seen yet), and
+    // weights are probability * V scale * unit: unit brings the largest scale
+    // to 2^7..2^8 at such a time and may lag behind until kLagV.  Both are below
+    // 65504 then.  vexp: that scale's exponent field (20: small enough for
+    // every scale); o is in units of 2^(vexp - 134).
+    constexpr float kLag = 6.f, kLagV = 900.f;
     uint32_t vexp = 20;
+    float unit = __uint_as_float((127u + 134u - 20u) << 23);
+    const uint32_t q_at = (uint32_t)__cvta_generic_to_shared(sq) + lane * 16;
 
-    for (int tile = warp; tile < tiles; tile += KVA_WARPS) {
+    int slot = 0;
+    for (int tile = warp; tile < tiles; tile += WARPS) {
         const int pos0 = c0 + tile * S::TT;
-        uint32_t live = 0;  // groups with a page
-#pragma unroll
-        for (int j = 0; j < GR; j++) live |= (uint32_t)(__shfl_sync(0xffffffffu, ids, held * GR + j) != NONE) << j;
+        const uint32_t live = live_next, at = ring + slot * S::SLOT;  // live: groups with a page
+        slot ^= 1;
+        __syncwarp();  // every lane is done with the slot that is filled now
+        if (tile + WARPS < tiles) {
+            if (++held == AHEAD) {
+                held = 0;
+                load_ids(tile + WARPS);
+            }
+            live_next = fetch(held, ring + slot * S::SLOT);
+        }
+        copies_commit();
+        copies_wait<1>();
+        __syncwarp();
         // every position seen by every row?
         const bool full = pos0 + S::TT <= min(prefix, c1) && live == (1u << GR) - 1;
+        uint32_t km[GR], vm[GR];
+#pragma unroll
+        for (int j = 0; j < GR; j++) {
+            km[j] = lds(at + S::META + (8 * j + g) * 4);
+            vm[j] = lds(at + S::META + (S::TT + 8 * j + g) * 4);
+            if (!full) vm[j] = pos0 + 8 * j + g < c1 ? vm[j] : 0;
+        }
 
+        const int start[4] = {START, START, START, START};
         float s[S::MT][NT][4];
 #pragma unroll
         for (int i = 0; i < S::MT; i++) {
             int acc[NT][3][4];
+            uint32_t kr[2][S::KCH][S::KW];
 #pragma unroll
-            for (int st = 0; st < S::STEPS; st++) {
-                uint32_t f[4];  // positions g | g + 8, first | second four dims
+            for (int j = 0; j < 2; j++)
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    if constexpr (FMT == KVQ_INT8) {
-                        f[j] = kr[2 * i + j][st / 2][2 * (st % 2)];
-                        f[2 + j] = kr[2 * i + j][st / 2][2 * (st % 2) + 1];
-                    } else {
-                        const uint32_t w = kr[2 * i + j][st / 2][st % 2];
-                        f[j] = w & 0x0f0f0f0fu;
-                        f[2 + j] = (w >> 4) & 0x0f0f0f0fu;
+                for (int cc = 0; cc < S::KCH; cc++)
+                    read_words(at + (2 * i + j) * S::GROUP + k_at[cc], kr[j][cc], std::integral_constant<int, S::KW>{});
+#pragma unroll
+            for (int st = 0; st < S::STEPS; st += 2) {
+                uint32_t f[2][4];  // positions g | g + 8, first | second four dims
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        if constexpr (FMT == KVQ_INT8) {
+                            f[e][j] = kr[j][st / 2][2 * e];
+                            f[e][2 + j] = kr[j][st / 2][2 * e + 1];
+                        } else {
+                            const uint32_t w = kr[j][st / 2][e];
+                            f[e][j] = w & 0x0f0f0f0fu;
+                            f[e][2 + j] = (w >> 4) & 0x0f0f0f0fu;
+                        }
                     }
-                }
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
                     for (int k = 0; k < 3; k++) {
-                        const uint2 qf = reinterpret_cast<const uint2*>(sq)[((n * 3 + k) * S::STEPS + st) * 32 + lane];
+                        const uint4 qf = lds4(q_at + ((n * 3 + k) * (S::STEPS / 2) + st / 2) * 512);
                         if (st == 0)
-                            mma_u8s8_first(acc[n][k], f, qf.x, qf.y, zero[n][0][k], zero[n][1][k]);
+                            mma_u8s8_first(acc[n][k], f[0], qf.x, qf.y, start);
                         else
-                            mma_u8s8(acc[n][k], f, qf.x, qf.y);
+                            mma_u8s8(acc[n][k], f[0], qf.x, qf.y);
+                        mma_u8s8(acc[n][k], f[1], qf.z, qf.w);
                     }
             }
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int c = 0; c < 4; c++)
-                    s[i][n][c] = fmaf(fmaf(__int_as_float(acc[n][2][c]) - ZERO_F, 256.f, __int_as_float(acc[n][1][c]) - ZERO_F), 256.f,
-                                      __int_as_float(acc[n][0][c]) - ZERO_F);
+                for (int c = 0; c < 4; c++) {
+                    float d[3];
+#pragma unroll
+                    for (int k = 0; k < 3; k++)
+                        d[k] = (BITS ? __int_as_float(acc[n][k][c]) : (float)acc[n][k][c]) - zero[n][c & 1][k];
+                    s[i][n][c] = fmaf(fmaf(d[2], 256.f, d[1]), 256.f, d[0]);
+                }
         }
         // scores in units of log2
 #pragma unroll
@@ -456,66 +505,83 @@ __global__ void __launch_bounds__(KVA_WARPS * 32) k_kvq_attend(KvqAttnArgs a) {
                     }
                 }
         }
-        // the next tile's K goes out: its registers are free
-        const int next = tile + KVA_WARPS;
-        bool all = false;
-        if (next < tiles) {
-            if (++held == AHEAD) {
-                held = 0;
-                load_ids(next);
-            }
-            all = whole(next, held);
-            load_k(next, held, all);
-        }
-        // V's scales: the largest finite one sets the unit of o
-        uint32_t vtop = 0;
+        float top[NT][2], vs[GR], vl[GR], vmax = 0.f;
+        bool over = false;
 #pragma unroll
-        for (int j = 0; j < GR; j++) {
-            const uint32_t bits = (FMT == KVQ_INT8 ? vm[j] : vm[j] << 16) & 0x7fffffffu;
-            if (bits < 0x7f800000u) vtop = max(vtop, bits);
-        }
-        vtop = max(__reduce_max_sync(0xffffffffu, vtop) >> 23, vexp);
-        float grow = __uint_as_float((127u - min(vtop - vexp, 126u)) << 23);  // 2^(old - new); below 2^-126 all the same
-        vexp = vtop;
-        const float unit = __uint_as_float((127u + 140u - vexp) << 23);  // 2^(140 - vexp), vexp >= 20 keeps it finite
-        // softmax; alpha rescales what there is
-        float alpha[NT][2];
-        uint32_t pb[S::MT][NT][S::PARTS][2];
-        float vs[GR], vl[GR];
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                top[n][c] = fmaxf(s[0][n][c], s[0][n][c + 2]);
+                if constexpr (S::MT == 2) top[n][c] = fmaxf(top[n][c], fmaxf(s[1][n][c], s[1][n][c + 2]));
+                over |= top[n][c] > limit[n][c];
+            }
 #pragma unroll
         for (int j = 0; j < GR; j++) {
             vs[j] = (FMT == KVQ_INT8 ? __uint_as_float(vm[j]) : bf16_bits_to_float(vm[j] & 0xffffu)) * unit;
             vl[j] = FMT == KVQ_INT8 ? 0.f : centre(vm[j]);
+            vmax = fmaxf(vmax, fabsf(vs[j]));
         }
+        if (__any_sync(0xffffffffu, over || vmax >= kLagV)) {
+            // new references: this tile's largest score and V scale (finite ones)
+            uint32_t vtop = 0;
+#pragma unroll
+            for (int j = 0; j < GR; j++) {
+                const uint32_t bits = (FMT == KVQ_INT8 ? vm[j] : vm[j] << 16) & 0x7fffffffu;
+                if (bits < 0x7f800000u) vtop = max(vtop, bits);
+            }
+            vtop = max(__reduce_max_sync(0xffffffffu, vtop) >> 23, vexp);
+            const float grow = __uint_as_float((127u - min(vtop - vexp, 126u)) << 23);  // old / new unit of o
+            vexp = vtop;
+            const float next = __uint_as_float((127u + 134u - vexp) << 23);
+#pragma unroll
+            for (int j = 0; j < GR; j++)
+                vs[j] = (FMT == KVQ_INT8 ? __uint_as_float(vm[j]) : bf16_bits_to_float(vm[j] & 0xffffu)) * next;
+            unit = next;
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                float alpha[2];
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+#pragma unroll
+                    for (int x = 4; x < 32; x *= 2) top[n][c] = fmaxf(top[n][c], __shfl_xor_sync(0xffffffffu, top[n][c], x));
+                    const bool seen = limit[n][c] != -INFINITY;
+                    const float to = seen ? fmaxf(base[n][c], top[n][c]) : top[n][c];
+                    alpha[c] = seen ? exp2_fast(base[n][c] - to) : 1.f;  // nothing summed yet
+                    if (to != -INFINITY) base[n][c] = to, limit[n][c] = to + kLag;
+                    l[n][c] *= alpha[c];
+                    z[n][c] *= alpha[c];
+                    alpha[c] *= grow;
+                }
+#pragma unroll
+                for (int i = 0; i < S::VD / 2; i++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) o[i][n][c] *= alpha[c & 1];
+            }
+        }
+        uint32_t pb[S::MT][NT][S::PARTS][2];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            float top[2];
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-                top[c] = fmaxf(s[0][n][c], s[0][n][c + 2]);
-                if constexpr (S::MT == 2) top[c] = fmaxf(top[c], fmaxf(s[1][n][c], s[1][n][c + 2]));
-#pragma unroll
-                for (int x = 4; x < 32; x *= 2) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], x));
-                top[c] = fmaxf(top[c], m[n][c]);
-                const float base = top[c] == -INFINITY ? 0.f : top[c];
-                alpha[n][c] = exp2_fast(m[n][c] - base);
-                m[n][c] = top[c];
-                top[c] = base;
-                l[n][c] *= alpha[n][c];
-                z[n][c] *= alpha[n][c];
-            }
 #pragma unroll
             for (int i = 0; i < S::MT; i++) {
                 float w[4];
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     const int j = 2 * i + (c >> 1);
-                    const float p = exp2_fast(s[i][n][c] - top[c & 1]);
+                    const float p = exp2_fast(s[i][n][c] - base[n][c & 1]);
                     l[n][c & 1] += p;
-                    // what a row does not see has weight 0 even where V is NaN
-                    const bool see = full || s[i][n][c] != -INFINITY;
-                    w[c] = see ? p * vs[j] : 0.f;
-                    if (FMT == KVQ_INT4 && see) z[n][c & 1] = fmaf(p, vl[j], z[n][c & 1]);
+                    w[c] = p * vs[j];
+                    s[i][n][c] = p;
+                }
+                if (full) {
+                    if constexpr (FMT == KVQ_INT4)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) z[n][c & 1] = fmaf(s[i][n][c], vl[2 * i + (c >> 1)], z[n][c & 1]);
+                } else {  // what a row does not see has weight 0 even where V is NaN
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        if (FMT == KVQ_INT4 && s[i][n][c] != 0.f) z[n][c & 1] = fmaf(s[i][n][c], vl[2 * i + (c >> 1)], z[n][c & 1]);
+                        if (s[i][n][c] == 0.f) w[c] = 0.f;
+                    }
                 }
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
@@ -527,21 +593,15 @@ __global__ void __launch_bounds__(KVA_WARPS * 32) k_kvq_attend(KvqAttnArgs a) {
                     }
                 }
             }
-#pragma unroll
-            for (int c = 0; c < 2; c++) alpha[n][c] *= grow;
         }
-        if constexpr (!SPLIT) {  // the running sums are the tiles' accumulators
-            bool same = true;
+        uint32_t vr[GR][2][S::VW];
 #pragma unroll
-            for (int n = 0; n < NT; n++) same &= alpha[n][0] == 1.f && alpha[n][1] == 1.f;
-            if (!__all_sync(0xffffffffu, same))
+        for (int j = 0; j < GR; j++)
 #pragma unroll
-                for (int i = 0; i < S::VD / 2; i++)
+            for (int e = 0; e < 2; e++)
 #pragma unroll
-                    for (int n = 0; n < NT; n++)
-#pragma unroll
-                        for (int c = 0; c < 4; c++) o[i][n][c] *= alpha[n][c & 1];
-        }
+                for (int i = 0; i < S::VW; i += 4)
+                    read_words(at + j * S::GROUP + v_at[e][i / 4], vr[j][e] + i, std::integral_constant<int, (S::VW > 4 ? 4 : S::VW)>{});
         // O^T += V^T P^T, two rows of 8 dims (dims 2 i, 2 i + 1 of each lane) at a time
 #pragma unroll
         for (int i = 0; i < S::VD / 2; i++) {
@@ -578,14 +638,14 @@ __global__ void __launch_bounds__(KVA_WARPS * 32) k_kvq_attend(KvqAttnArgs a) {
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int c = 0; c < 4; c++) o[i][n][c] = fmaf(o[i][n][c], alpha[n][c & 1], acc[n][c]);
+                    for (int c = 0; c < 4; c++) o[i][n][c] += acc[n][c];
         }
-        if (next < tiles) load_v(next, held, all);
     }
 
     // ---- merge the warps ------------------------------------------------------------
-    const float back = __uint_as_float((vexp + 127u - 140u) << 23);  // 2^(vexp - 140)
-    __syncthreads();  // q's fragments are done with
+    const float back = __uint_as_float((vexp + 127u - 134u) << 23);  // 2^(vexp - 134)
+    copies_wait<0>();
+    __syncthreads();  // the rings are done with
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -596,7 +656,7 @@ __global__ void __launch_bounds__(KVA_WARPS * 32) k_kvq_attend(KvqAttnArgs a) {
                 z[n][c] += __shfl_xor_sync(0xffffffffu, z[n][c], x);
             }
             const int r = 8 * n + 2 * t + c;
-            if (g == 0) sml[warp * S::ROWS + r] = make_float2(m[n][c], l[n][c]);
+            if (g == 0) sml[warp * S::ROWS + r] = make_float2(limit[n][c] == -INFINITY ? -INFINITY : base[n][c], l[n][c]);
             float* to = so + (warp * S::ROWS + r) * S::O_STRIDE + g * S::VD;
 #pragma unroll
             for (int i = 0; i < S::VD / 2; i++)
@@ -604,14 +664,14 @@ __global__ void __launch_bounds__(KVA_WARPS * 32) k_kvq_attend(KvqAttnArgs a) {
                     make_float2(fmaf(o[i][n][c], back, z[n][c]), fmaf(o[i][n][c + 2], back, z[n][c]));
         }
     __syncthreads();
-    for (int at = tid; at < n_rows * hd; at += KVA_WARPS * 32) {
+    for (int at = tid; at < n_rows * hd; at += WARPS * 32) {
         const int r = at / hd, d = at - r * hd;
         float top = -INFINITY, sum = 0.f, x = 0.f;
 #pragma unroll
-        for (int w = 0; w < KVA_WARPS; w++) top = fmaxf(top, sml[w * S::ROWS + r].x);
+        for (int w = 0; w < WARPS; w++) top = fmaxf(top, sml[w * S::ROWS + r].x);
         const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-        for (int w = 0; w < KVA_WARPS; w++) {
+        for (int w = 0; w < WARPS; w++) {
             const float2 ml = sml[w * S::ROWS + r];
             const float f = exp2_fast(ml.x - base);
             sum = fmaf(ml.y, f, sum);

@@ -161,11 +161,13 @@ void plan_attention(KvqAttnArgs& k) {
     const int block = rows > 8 ? 16 : 8;
     k.row_blocks = (int)((rows + block - 1) / block);
     const int64_t units = (int64_t)k.n_seqs * k.c.heads * k.row_blocks;
-    const int64_t want = 148 * 8;
-    int64_t chunk = k.max_len * units / want;
-    chunk = std::min<int64_t>(std::max<int64_t>((chunk + 127) / 128 * 128, 128), 2048);
+    int64_t chunk = k.max_len * units / (148 * 6);
+    chunk = std::min<int64_t>(std::max<int64_t>((chunk + 127) / 128 * 128, 1024), 4096);
+    if (const char* e = getenv("FB2_KVA_CHUNK")) chunk = atoi(e);
     k.chunk = (int)chunk;
     k.splits = std::max(1, (int)((k.max_len + chunk - 1) / chunk));
+    k.warps = block == 8 && units * k.splits <= 148 ? 8 : 4;
+    if (const char* e = getenv("FB2_KVA_WARPS")) k.warps = atoi(e);
 }
 
 KvqAttnArgs attn_args(const fb2_kvq_cache* c, const fb2_kvq_attention* a) {
@@ -217,22 +219,24 @@ int64_t attn_workspace(const KvqAttnArgs& k) {
     return (parts * 8 + 15) / 16 * 16 + parts * k.c.hd * 4;
 }
 
-template <int HD, int FMT, int NT, bool SPLIT>
+template <int HD, int FMT, int NT, bool SPLIT, int WARPS>
 void launch_attend(const KvqAttnArgs& k, cudaStream_t stream) {
-    using S = KvaShape<HD, FMT, NT, SPLIT>;
-    auto kernel = k_kvq_attend<HD, FMT, NT, SPLIT>;
+    using S = KvaShape<HD, FMT, NT, SPLIT, WARPS>;
+    auto kernel = k_kvq_attend<HD, FMT, NT, SPLIT, WARPS>;
     if (S::SMEM > 48 * 1024) opt_in_smem((const void*)kernel, S::SMEM);
     const int64_t blocks = (int64_t)k.row_blocks * k.splits * k.c.heads;
     need(blocks <= INT32_MAX, "too many rows for one call");
-    kernel<<<dim3((unsigned)blocks, k.n_seqs), KVA_WARPS * 32, S::SMEM, stream>>>(k);
+    kernel<<<dim3((unsigned)blocks, k.n_seqs), WARPS * 32, S::SMEM, stream>>>(k);
 }
 template <int HD, int FMT>
 void launch_attend(const KvqAttnArgs& k, cudaStream_t stream) {
-    const bool wide = (int64_t)k.max_nodes * k.share > 8, split = k.dtype == FB2_F32;
-    if (wide)
-        split ? launch_attend<HD, FMT, 2, true>(k, stream) : launch_attend<HD, FMT, 2, false>(k, stream);
+    const bool split = k.dtype == FB2_F32;
+    if ((int64_t)k.max_nodes * k.share > 8)
+        split ? launch_attend<HD, FMT, 2, true, 4>(k, stream) : launch_attend<HD, FMT, 2, false, 4>(k, stream);
+    else if (k.warps == 8)
+        split ? launch_attend<HD, FMT, 1, true, 8>(k, stream) : launch_attend<HD, FMT, 1, false, 8>(k, stream);
     else
-        split ? launch_attend<HD, FMT, 1, true>(k, stream) : launch_attend<HD, FMT, 1, false>(k, stream);
+        split ? launch_attend<HD, FMT, 1, true, 4>(k, stream) : launch_attend<HD, FMT, 1, false, 4>(k, stream);
 }
 template <int FMT>
 void launch_attend(const KvqAttnArgs& k, cudaStream_t stream) {

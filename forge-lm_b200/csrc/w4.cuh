@@ -226,29 +226,6 @@ FB2_DEV void column(const T* __restrict__ x, long long x_row, int row, int part,
     for (int i = 0; i < 8; i++) f[i] = Form<T>::pair(v + 2 * i, part);
 }
 
-FB2_DEV void copy16(uint32_t to, const void* from, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
-}
-FB2_DEV void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-FB2_DEV void copies_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-FB2_DEV uint4 lds4(uint32_t at) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
-    return v;
-}
-FB2_DEV float2 lds2(uint32_t at) {
-    float2 v;
-    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at));
-    return v;
-}
-FB2_DEV uint32_t lds(uint32_t at) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
-    return v;
-}
 FB2_DEV void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -553,7 +530,7 @@ __global__ void __launch_bounds__(W4_WARPS * 32, 2)
 #pragma unroll
         for (int i = 0; i < NT * W4_COL / 16; i += 32)
             if (i + lane < NT * W4_COL / 16)
-                w4::copy16(ring + to * S::SLOT + RT * w4::UNIT + (i + lane) * 16, from + (i + lane) * 16, true);
+                copy16(ring + to * S::SLOT + RT * w4::UNIT + (i + lane) * 16, from + (i + lane) * 16, true);
     };
     // the first units' codes before the columns are there
 #pragma unroll
@@ -562,14 +539,14 @@ __global__ void __launch_bounds__(W4_WARPS * 32, 2)
 #pragma unroll
     for (int i = 0; i < S::DEPTH - 1; i++) {
         fetch_x(u + i * stride, i);
-        w4::copies_commit();
+        copies_commit();
     }
     ahead = u + (S::DEPTH - 1) * stride, fill = S::DEPTH - 1;
     for (; u < units; u += stride) {
         __syncwarp();  // every lane is done with the slot that is filled next
         fetch_codes(ahead, fill);
         fetch_x(ahead, fill);
-        w4::copies_commit();
+        copies_commit();
         ahead += stride;
         fill = fill + 1 == S::DEPTH ? 0 : fill + 1;
         uint32_t xf[NT][8];
@@ -580,17 +557,17 @@ __global__ void __launch_bounds__(W4_WARPS * 32, 2)
             w4_digits<T>(x, x_row, row, g - row * D, row < rows, u * 128, w.K, vec, w.group_shift, xf[0], own_weight, own_sum);
             weight[0] = make_float2(__shfl_sync(0xffffffffu, own_weight, 8 * t), __shfl_sync(0xffffffffu, own_weight, 8 * t + 4));
         }
-        w4::copies_wait<S::DEPTH - 1>();
+        copies_wait<S::DEPTH - 1>();
         __syncwarp();
         const uint32_t at = ring + slot * S::SLOT, xat = at + RT * w4::UNIT;
         slot = slot + 1 == S::DEPTH ? 0 : slot + 1;
         if constexpr (!DIRECT)
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                const uint4 a = w4::lds4(xat + n * W4_COL + lane * 16), b = w4::lds4(xat + n * W4_COL + 512 + lane * 16);
+                const uint4 a = lds4(xat + n * W4_COL + lane * 16), b = lds4(xat + n * W4_COL + 512 + lane * 16);
                 xf[n][0] = a.x, xf[n][1] = a.y, xf[n][2] = a.z, xf[n][3] = a.w;
                 xf[n][4] = b.x, xf[n][5] = b.y, xf[n][6] = b.z, xf[n][7] = b.w;
-                weight[n] = w4::lds2(xat + n * W4_COL + 1024 + 8 * t);
+                weight[n] = lds2(xat + n * W4_COL + 1024 + 8 * t);
             }
         // integer sums start at the bits of 1.5 2^23: below 2^22 in size, they
         // are then the bits of 1.5 2^23 + sum
@@ -618,14 +595,14 @@ __global__ void __launch_bounds__(W4_WARPS * 32, 2)
                     xs[n].x = __shfl_sync(0xffffffffu, own_sum[grp], 8 * t);
                     xs[n].y = __shfl_sync(0xffffffffu, own_sum[grp], 8 * t + 4);
                 } else {
-                    xs[n] = w4::lds2(xat + n * W4_COL + 1056 + grp * 32 + 8 * t);
+                    xs[n] = lds2(xat + n * W4_COL + 1056 + grp * 32 + 8 * t);
                 }
             }
 #pragma unroll
             for (int r = 0; r < RT; r++)
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
-                    const uint32_t m = w4::lds(at + r * w4::UNIT + 1024 + grp * 64 + (half * 8 + g) * 4);
+                    const uint32_t m = lds(at + r * w4::UNIT + 1024 + grp * 64 + (half * 8 + g) * 4);
                     const float s = bf16_bits_to_float(m & 0xffffu), low = __uint_as_float(m & 0xffff0000u);
 #pragma unroll
                     for (int n = 0; n < NT; n++)
@@ -642,7 +619,7 @@ __global__ void __launch_bounds__(W4_WARPS * 32, 2)
         for (int b = 0; b < 2; b++) {
             uint4 word[RT];
 #pragma unroll
-            for (int r = 0; r < RT; r++) word[r] = w4::lds4(at + r * w4::UNIT + b * 512 + lane * 16);
+            for (int r = 0; r < RT; r++) word[r] = lds4(at + r * w4::UNIT + b * 512 + lane * 16);
             if (w.group_shift == 5) {
 #pragma unroll
                 for (int r = 0; r < RT; r++) {
@@ -671,7 +648,7 @@ __global__ void __launch_bounds__(W4_WARPS * 32, 2)
             }
         }
     }
-    w4::copies_wait<0>();
+    copies_wait<0>();
     __syncthreads();  // the rings are done with
     float* red = reinterpret_cast<float*>(w4_smem);  // [warp][OUT][COLS], then the CTA's sums
 #pragma unroll
@@ -732,9 +709,9 @@ __global__ void __launch_bounds__(W4_WARPS * 32, 2)
         const uint32_t to = smem + st * S::STAGE;
         const uint4* from = columns + cu * (S::X / 16);
 #pragma unroll
-        for (int i = 0; i < S::X / 16; i += W4_WARPS * 32) w4::copy16(to + (i + threadIdx.x) * 16, from + i + threadIdx.x, true);
+        for (int i = 0; i < S::X / 16; i += W4_WARPS * 32) copy16(to + (i + threadIdx.x) * 16, from + i + threadIdx.x, true);
         if (threadIdx.x < GROUPS * NT * 2)
-            w4::copy16(to + S::X + threadIdx.x * 16, sums + cu * (GROUPS * NT * 8) + threadIdx.x * 4, true);
+            copy16(to + S::X + threadIdx.x * 16, sums + cu * (GROUPS * NT * 8) + threadIdx.x * 4, true);
     };
 
     float sum[NT][4];
@@ -749,17 +726,17 @@ __global__ void __launch_bounds__(W4_WARPS * 32, 2)
 #pragma unroll
     for (int i = 0; i < S::DEPTH - 1; i++) {
         fetch_x(rank + i * ranks, i);
-        w4::copies_commit();
+        copies_commit();
     }
     int slot = 0;
     for (int u = rank; u < units; u += ranks) {
-        w4::copies_wait<S::DEPTH - 2>();
+        copies_wait<S::DEPTH - 2>();
         __syncthreads();  // the unit is there for all, and all are done with the stage that is filled next
         {
             const int ahead = u + (S::DEPTH - 1) * ranks, st = slot == 0 ? S::DEPTH - 1 : slot - 1;
             fetch_codes(ahead, st);
             fetch_x(ahead, st);
-            w4::copies_commit();
+            copies_commit();
         }
         const uint32_t xat = smem + slot * S::STAGE, sat = xat + S::X, cat = sat + S::SUMS + warp * w4::UNIT;
         slot = slot + 1 == S::DEPTH ? 0 : slot + 1;
@@ -768,14 +745,14 @@ __global__ void __launch_bounds__(W4_WARPS * 32, 2)
             float xs[NT][4];
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                const float2 v = w4::lds2(sat + (grp * NT * 8 + n * 8 + 2 * t) * 4);
+                const float2 v = lds2(sat + (grp * NT * 8 + n * 8 + 2 * t) * 4);
                 xs[n][0] = v.x, xs[n][1] = v.y;
             }
             w4::close_group<T, NT>(cat + 1024, grp, g, acc, xs, sum);
         };
 #pragma unroll
         for (int b = 0; b < 2; b++) {
-            const uint4 words = w4::lds4(cat + b * 512 + lane * 16);
+            const uint4 words = lds4(cat + b * 512 + lane * 16);
             uint32_t word[4] = {words.x, words.y, words.z, words.w};
             if constexpr (GS == 5) {
                 w4::by_group(word[0], word[1]);
@@ -789,7 +766,7 @@ __global__ void __launch_bounds__(W4_WARPS * 32, 2)
                 F::codes(word[GS == 5 ? 2 + h : 2 * h + 1], f[1]);
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    const uint4 v = w4::lds4(xat + ((b * NT + n) * 2 + h) * 512 + lane * 16);
+                    const uint4 v = lds4(xat + ((b * NT + n) * 2 + h) * 512 + lane * 16);
                     if (GS == 5 || (h == 0 && (b == 0 || GS == 6)))
                         w4::mma_first<F::BF16>(acc[n], f[0], v.x, v.y);
                     else
@@ -802,7 +779,7 @@ __global__ void __launch_bounds__(W4_WARPS * 32, 2)
         }
         if constexpr (GS == 7) close(0);
     }
-    w4::copies_wait<0>();
+    copies_wait<0>();
     __syncthreads();
     float* own = reinterpret_cast<float*>(w4_smem);
 #pragma unroll
