@@ -28,7 +28,7 @@ struct KvqAttnArgs {
     float2* part_ml;         // (m, l) of each, where splits > 1
     long long q_row, q_head, table_stride;
     int n_seqs, n_rows, n_heads, share, max_nodes, max_len, mask_words, dtype;
-    int splits, chunk, row_blocks, warps;
+    int splits, chunk, row_blocks, block_rows, warps;  // block_rows 8, 16: k_kvq_attend; 128: k_kvq_attend_tc
     float scale;
     FB2_DEV void rows_of(int b, int& first, int& count) const {
         first = starts ? __ldg(starts + b) : b;
@@ -704,23 +704,43 @@ __global__ void __launch_bounds__(128) k_kvq_attend_merge(KvqAttnArgs a) {
     for (int s = lane; s < a.splits; s += 32) top = fmaxf(top, __ldcg(ml + s).x);
     top = warp_max(top);
     const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.splits; s++) {
-        const float2 w = __ldcg(ml + s);
-        if (w.y == 0.f) continue;  // nothing seen there, maybe no part written
-        const float f = kva::exp2_fast(w.x - base);
-        sum = fmaf(w.y, f, sum);
+    const int hd = a.c.hd, d0 = 4 * lane;  // a lane's dims: d0 .. d0 + 3, and 128 further
+    float sum = 0.f, x[2][4] = {};
+    for (int s0 = 0; s0 < a.splits; s0 += 32) {
+        const float2 w = s0 + lane < a.splits ? __ldcg(ml + s0 + lane) : make_float2(-INFINITY, 0.f);
+        const float scale = kva::exp2_fast(w.x - base);
+        sum = fmaf(w.y, scale, sum);
+        // parts in which nothing was seen may not have been written
+        uint32_t there = __ballot_sync(0xffffffffu, w.y != 0.f);
+        while (there) {
+            float4 v[4][2];
+            float f[4];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int d = lane + 32 * i;
-            if (d < a.c.hd) x[i] = fmaf(__ldcg(part + (size_t)s * a.c.hd + d), f, x[i]);
+            for (int u = 0; u < 4; u++) {  // four parts' loads before their sums
+                const int s = there ? __ffs(there) - 1 : 0;
+                f[u] = there ? __shfl_sync(0xffffffffu, scale, s) : 0.f;
+                const float4* p = reinterpret_cast<const float4*>(part + (size_t)(s0 + s) * hd + d0);
+                v[u][0] = there && d0 < hd ? __ldcg(p) : make_float4(0.f, 0.f, 0.f, 0.f);
+                v[u][1] = there && d0 + 128 < hd ? __ldcg(p + 32) : make_float4(0.f, 0.f, 0.f, 0.f);
+                there &= there - 1;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    x[i][0] = fmaf(v[u][i].x, f[u], x[i][0]);
+                    x[i][1] = fmaf(v[u][i].y, f[u], x[i][1]);
+                    x[i][2] = fmaf(v[u][i].z, f[u], x[i][2]);
+                    x[i][3] = fmaf(v[u][i].w, f[u], x[i][3]);
+                }
         }
     }
+    sum = warp_sum(sum);
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int d = lane + 32 * i;
-        if (d < a.c.hd) a.store_out(item * a.c.hd + d, sum == 0.f ? 0.f : x[i] / sum);
-    }
+    for (int i = 0; i < 2; i++)
+        if (d0 + 128 * i < hd)
+#pragma unroll
+            for (int e = 0; e < 4; e++) a.store_out(item * hd + d0 + 128 * i + e, sum == 0.f ? 0.f : x[i][e] / sum);
     if (a.lse && lane == 0) a.lse[item] = 0.693147180559945309f * (top + log2f(sum));
 }
 

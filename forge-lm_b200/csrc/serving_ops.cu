@@ -12,6 +12,7 @@
 #include "capi.cuh"
 #include "kvq.cuh"
 #include "kvq_attn.cuh"
+#include "kvq_attn_tc.cuh"
 #include "logit_controls.cuh"
 #include "w4.cuh"
 
@@ -153,21 +154,22 @@ int32_t fb2_kvq_read(const fb2_kvq_cache* c, int32_t n_rows, const int32_t* slot
 
 // ---- attention ---------------------------------------------------------------
 namespace {
-// Chunks of positions: enough blocks to fill the device a few times over,
-// none shorter than a round of the four warps' tiles and none so long that
-// one long sequence among short ones runs alone.
+// Rows to a block, and chunks of positions: enough blocks to fill the device a
+// few times over, and none so long that one long sequence among short ones
+// runs alone.
 void plan_attention(KvqAttnArgs& k) {
     const int64_t rows = (int64_t)k.max_nodes * k.share;
-    const int block = rows > 8 ? 16 : 8;
-    k.row_blocks = (int)((rows + block - 1) / block);
+    const char* e = getenv("FB2_KVA_TC");
+    const bool tc = k.dtype != FB2_F32 && k.c.hd <= 128 && rows > (e ? atoi(e) : 16);
+    k.block_rows = tc ? KVT_ROWS : rows > 8 ? 16 : 8;
+    k.row_blocks = (int)((rows + k.block_rows - 1) / k.block_rows);
     const int64_t units = (int64_t)k.n_seqs * k.c.heads * k.row_blocks;
-    int64_t chunk = k.max_len * units / (148 * 6);
-    chunk = std::min<int64_t>(std::max<int64_t>((chunk + 127) / 128 * 128, 1024), 4096);
+    int64_t chunk = k.max_len * units / (148 * (tc ? 3 : 6));
+    chunk = std::min<int64_t>(std::max<int64_t>((chunk + 127) / 128 * 128, 1024), tc ? 8192 : 4096);
     if (const char* e = getenv("FB2_KVA_CHUNK")) chunk = atoi(e);
     k.chunk = (int)chunk;
     k.splits = std::max(1, (int)((k.max_len + chunk - 1) / chunk));
-    k.warps = block == 8 && units * k.splits <= 148 ? 8 : 4;
-    if (const char* e = getenv("FB2_KVA_WARPS")) k.warps = atoi(e);
+    k.warps = k.block_rows == 8 && units * k.splits <= 148 ? 8 : 4;
 }
 
 KvqAttnArgs attn_args(const fb2_kvq_cache* c, const fb2_kvq_attention* a) {
@@ -231,15 +233,31 @@ void launch_attend(const KvqAttnArgs& k, cudaStream_t stream) {
 template <int HD, int FMT>
 void launch_attend(const KvqAttnArgs& k, cudaStream_t stream) {
     const bool split = k.dtype == FB2_F32;
-    if ((int64_t)k.max_nodes * k.share > 8)
+    if (k.block_rows == 16)
         split ? launch_attend<HD, FMT, 2, true, 4>(k, stream) : launch_attend<HD, FMT, 2, false, 4>(k, stream);
     else if (k.warps == 8)
         split ? launch_attend<HD, FMT, 1, true, 8>(k, stream) : launch_attend<HD, FMT, 1, false, 8>(k, stream);
     else
         split ? launch_attend<HD, FMT, 1, true, 4>(k, stream) : launch_attend<HD, FMT, 1, false, 4>(k, stream);
 }
+template <int HD, int FMT>
+void launch_attend_tc(const KvqAttnArgs& k, cudaStream_t stream) {
+    auto kernel = k_kvq_attend_tc<HD, FMT>;
+    constexpr int smem = KvtShape<HD, FMT>::SMEM;
+    opt_in_smem((const void*)kernel, smem);
+    const int64_t blocks = (int64_t)k.row_blocks * k.splits * k.c.heads;
+    need(blocks <= INT32_MAX, "too many rows for one call");
+    kernel<<<dim3((unsigned)blocks, k.n_seqs), KVT_LAUNCH, smem, stream>>>(k);
+}
 template <int FMT>
 void launch_attend(const KvqAttnArgs& k, cudaStream_t stream) {
+    if (k.block_rows == KVT_ROWS) {
+        if (k.c.hd <= 64)
+            launch_attend_tc<64, FMT>(k, stream);
+        else
+            launch_attend_tc<128, FMT>(k, stream);
+        return;
+    }
     if (k.c.hd <= 64)
         launch_attend<64, FMT>(k, stream);
     else if (k.c.hd <= 128)
