@@ -438,25 +438,29 @@ __global__ void __launch_bounds__(KVT_LAUNCH, 1) k_kvq_attend_tc(KvqAttnArgs a) 
         tc::fence_before();
         if (!__syncthreads_and(ok)) break;
         if (t + 1 < ntiles) load_meta(t + 2);  // (positions past c1 give 0)
-        float s[KVT_COLS];
         const bool full = p0 + KVT_KEYS <= min(prefix, c1) && live == 0xffffu;
         const float vtop = __uint_as_float(max(max(s_vtop[t & 1][0], s_vtop[t & 1][1]), max(s_vtop[t & 1][2], s_vtop[t & 1][3])));
         bool over = vtop * unit >= kLagV;
-        uint32_t see = 0xffffffffu;
-        if (busy) {
-            kvt::ld(tmem + lanes + 128u * (t & 1) + KVT_COLS * part, s);
+        // the row's scores of columns c .. c + 15 of its part (without f); they
+        // are read twice, as registers are short
+        auto scores = [&](int c, float (&s)[16]) {
+            kvt::ld(tmem + lanes + 128u * (t & 1) + KVT_COLS * part + c, s);
+            const float* ks = &s_k[t & 1][0][KVT_COLS * part + c];
             kvt::wait_ld();
 #pragma unroll
-            for (int j = 0; j < KVT_COLS; j += 4) {
-                const float4 k4 = *reinterpret_cast<const float4*>(&s_k[t & 1][0][KVT_COLS * part + j]);
+            for (int j = 0; j < 16; j += 4) {
+                const float4 k4 = *reinterpret_cast<const float4*>(ks + j);
                 if constexpr (FMT == KVQ_INT8) {
                     s[j] *= k4.x, s[j + 1] *= k4.y, s[j + 2] *= k4.z, s[j + 3] *= k4.w;
                 } else {
-                    const float4 c4 = *reinterpret_cast<const float4*>(&s_k[t & 1][1][KVT_COLS * part + j]);
+                    const float4 c4 = *reinterpret_cast<const float4*>(ks + KVT_KEYS + j);
                     s[j] = fmaf(s[j], k4.x, c4.x * qsum), s[j + 1] = fmaf(s[j + 1], k4.y, c4.y * qsum);
                     s[j + 2] = fmaf(s[j + 2], k4.z, c4.z * qsum), s[j + 3] = fmaf(s[j + 3], k4.w, c4.w * qsum);
                 }
             }
+        };
+        uint32_t see = 0xffffffffu;
+        if (busy) {
             if (!full) {
                 // bit i: position at0 + i is there and seen by the row
                 const int at0 = p0 + KVT_COLS * part, n0 = at0 - prefix;
@@ -472,13 +476,24 @@ __global__ void __launch_bounds__(KVT_LAUNCH, 1) k_kvq_attend_tc(KvqAttnArgs a) 
                     const int low = n0 & ~31;
                     see &= n0 < 0 ? (word(0) << (-n0)) | ((1u << (-n0)) - 1) : __funnelshift_r(word(low), word(low + 32), n0 & 31);
                 }
-#pragma unroll
-                for (int j = 0; j < KVT_COLS; j++)
-                    if (!((see >> j) & 1)) s[j] = -INFINITY;
             }
-            float top[4] = {s[0], s[1], s[2], s[3]};  // four chains
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four chains
+            auto largest = [&](auto all) {
 #pragma unroll
-            for (int j = 4; j < KVT_COLS; j++) top[j & 3] = fmaxf(top[j & 3], s[j]);
+                for (int c = 0; c < KVT_COLS; c += 16) {
+                    float s[16];
+                    scores(c, s);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        if constexpr (!decltype(all)::value) s[j] = (see >> (c + j)) & 1 ? s[j] : -INFINITY;
+                        top[j & 3] = fmaxf(top[j & 3], s[j]);
+                    }
+                }
+            };
+            if (full)
+                largest(std::true_type{});
+            else
+                largest(std::false_type{});
             const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
             s_red[part][r] = most;
             over |= most * f > limit;
@@ -517,32 +532,37 @@ __global__ void __launch_bounds__(KVT_LAUNCH, 1) k_kvq_attend_tc(KvqAttnArgs a) 
             // weights of 8 columns at a time; `all`: the row sees every one
             auto weights = [&](auto all) {
 #pragma unroll
-                for (int j = 0; j < KVT_COLS; j += 8) {
-                    float w[8];
+                for (int c = 0; c < KVT_COLS; c += 16) {
+                    float s[16];
+                    scores(c, s);
 #pragma unroll
-                    for (int i = 0; i < 8; i += 4) {
-                        const float4 v4 = *reinterpret_cast<const float4*>(&s_v[t & 1][0][KVT_COLS * part + j + i]);
-                        const float vs[4] = {v4.x, v4.y, v4.z, v4.w};
-                        float vc[4] = {0.f, 0.f, 0.f, 0.f};
-                        if constexpr (FMT == KVQ_INT4) {
-                            const float4 c4 = *reinterpret_cast<const float4*>(&s_v[t & 1][1][KVT_COLS * part + j + i]);
-                            vc[0] = c4.x, vc[1] = c4.y, vc[2] = c4.z, vc[3] = c4.w;
-                        }
+                    for (int j = 0; j < 16; j += 8) {
+                        float w[8];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int at = j + i + e;
-                            float p = kva::exp2_fast(fmaf(s[at], f, -base)), v = vs[e] * unit;
-                            if constexpr (!decltype(all)::value) {  // nothing of what it does not see, NaN or not
-                                const bool seen = (see >> at) & 1;
-                                p = seen ? p : 0.f, v = seen ? v : 0.f, vc[e] = seen ? vc[e] : 0.f;
+                        for (int i = 0; i < 8; i += 4) {
+                            const float* to = &s_v[t & 1][0][KVT_COLS * part + c + j + i];
+                            const float4 v4 = *reinterpret_cast<const float4*>(to);
+                            const float vs[4] = {v4.x, v4.y, v4.z, v4.w};
+                            float vc[4] = {0.f, 0.f, 0.f, 0.f};
+                            if constexpr (FMT == KVQ_INT4) {
+                                const float4 c4 = *reinterpret_cast<const float4*>(to + KVT_KEYS);
+                                vc[0] = c4.x, vc[1] = c4.y, vc[2] = c4.z, vc[3] = c4.w;
                             }
-                            w[i + e] = p * v;
-                            l[e] += p;
-                            if constexpr (FMT == KVQ_INT4) z[e] = fmaf(p, vc[e], z[e]);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                float p = kva::exp2_fast(fmaf(s[j + i + e], f, -base)), v = vs[e] * unit;
+                                if constexpr (!decltype(all)::value) {  // nothing of what it does not see, NaN or not
+                                    const bool seen = (see >> (c + j + i + e)) & 1;
+                                    p = seen ? p : 0.f, v = seen ? v : 0.f, vc[e] = seen ? vc[e] : 0.f;
+                                }
+                                w[i + e] = p * v;
+                                l[e] += p;
+                                if constexpr (FMT == KVQ_INT4) z[e] = fmaf(p, vc[e], z[e]);
+                            }
                         }
+                        kvt::st4(P + kvt::place(r, (KVT_COLS * part + c + j) / 8),
+                                 make_uint4(kva::h2_pack(w[0], w[1]), kva::h2_pack(w[2], w[3]), kva::h2_pack(w[4], w[5]), kva::h2_pack(w[6], w[7])));
                     }
-                    kvt::st4(P + kvt::place(r, (KVT_COLS * part + j) / 8),
-                             make_uint4(kva::h2_pack(w[0], w[1]), kva::h2_pack(w[2], w[3]), kva::h2_pack(w[4], w[5]), kva::h2_pack(w[6], w[7])));
                 }
             };
             if (full)

@@ -154,19 +154,22 @@ int32_t fb2_kvq_read(const fb2_kvq_cache* c, int32_t n_rows, const int32_t* slot
 
 // ---- attention ---------------------------------------------------------------
 namespace {
-// Rows to a block, and chunks of positions: enough blocks to fill the device a
-// few times over, and none so long that one long sequence among short ones
-// runs alone.
+// Rows to a block, and chunks of positions.
 void plan_attention(KvqAttnArgs& k) {
     const int64_t rows = (int64_t)k.max_nodes * k.share;
-    const char* e = getenv("FB2_KVA_TC");
-    const bool tc = k.dtype != FB2_F32 && k.c.hd <= 128 && rows > (e ? atoi(e) : 16);
+    const bool tc = k.dtype != FB2_F32 && k.c.hd <= 128 && rows > 32;
     k.block_rows = tc ? KVT_ROWS : rows > 8 ? 16 : 8;
     k.row_blocks = (int)((rows + k.block_rows - 1) / k.block_rows);
     const int64_t units = (int64_t)k.n_seqs * k.c.heads * k.row_blocks;
-    int64_t chunk = k.max_len * units / (148 * (tc ? 3 : 6));
-    chunk = std::min<int64_t>(std::max<int64_t>((chunk + 127) / 128 * 128, 1024), tc ? 8192 : 4096);
-    if (const char* e = getenv("FB2_KVA_CHUNK")) chunk = atoi(e);
+    // CTAs for a few waves, counted as if all sequences were of max_len
+    int64_t chunk = k.max_len * units / (tc ? 512 : 888), least = 512;
+    if (!tc) {
+        if (k.block_rows == 8 && k.max_len <= 1024) least = 1024;
+        if (k.block_rows == 16 && k.max_len <= 1024 && units <= 16) least = 256;
+        least = std::max<int64_t>(least, k.max_len / 64);
+    }
+    chunk = std::min<int64_t>(std::max(chunk, least), std::max<int64_t>(tc ? 8192 : 4096, k.max_len / 64));
+    chunk = (chunk + 127) / 128 * 128;
     k.chunk = (int)chunk;
     k.splits = std::max(1, (int)((k.max_len + chunk - 1) / chunk));
     k.warps = k.block_rows == 8 && units * k.splits <= 148 ? 8 : 4;
