@@ -1,7 +1,6 @@
 // logit_controls.cuh — penalties for repeated tokens, biases and grammar masks
 // on logit rows (include/forge_b200.h, fb2_logit_controls, has the formula).
 #pragma once
-#include <cstring>
 #include <type_traits>
 
 #include "kvq.cuh"
@@ -23,170 +22,171 @@ struct ControlArgs {
     int n_rows, vocab, n_masks, mask_words;
 };
 
-constexpr int CTL_THREADS = 256;
+// A CTA takes a row, or, of few rows, a slice of one.  It gathers what the
+// row's window and bias list name in a hash table in shared memory (how often
+// the window has the id, which bias is its last), copies the slice, or -inf
+// where the mask does not allow an entry, sixteen bytes at a time, and then
+// writes the entries that the lists name: few beside the vocabulary, so that
+// the copies bound it.
+constexpr int CTL_THREADS = 512, CTL_VECS = 4;
+// List entries a thread, and the table's slots at most: at most three quarters
+// of them are taken.
+constexpr int CTL_IDS = 12, CTL_SLOTS = CTL_THREADS * CTL_IDS / 3 * 4;
 
-// A CTA takes `chunk` vocabulary entries (a multiple of 32) of one row.  The
-// ids that the row's window or bias list names are few: they get a bit each,
-// and a word in a table that only they initialise (how often the window has
-// the id, and which bias is its last).  Then one pass over the chunk: entries
-// without a bit are copied or masked as they are, sixteen bytes at a time,
-// the others computed in fp32.
-// Table words: bias index + 1 in the high half, count in the low half; lists
-// too long for 16 bits use two words, half as many entries at a time.
+// blockIdx: slice of `slice` entries (a multiple of 32), row; `slots` (a power
+// of two): the table's, two words each.
 template <class T>
-struct ControlRow {
-    const ControlArgs& a;
-    const uint32_t* allowed;  // null: everything
-    float rep, pres, freq;
-    const float* biases;      // of the row's list
-    FB2_DEV float value(float x, uint32_t count, uint32_t bias) const {
+__global__ void __launch_bounds__(CTL_THREADS, 2) k_logit_controls(ControlArgs a, int slice, int slots, bool copies) {
+    extern __shared__ uint32_t ctl_smem[];
+    const int tid = threadIdx.x, row = blockIdx.y, v0 = blockIdx.x * slice, len = min(slice, a.vocab - v0);
+    long long t0 = 0, b0 = 0, nt = 0, nb = 0;
+    if (a.tokens) {
+        t0 = max(__ldg(a.token_starts + row), 0);
+        nt = max(0ll, min((long long)__ldg(a.token_starts + row + 1), a.n_tokens) - t0);
+    }
+    if (a.bias_ids) {
+        b0 = max(__ldg(a.bias_starts + row), 0);
+        nb = max(0ll, min((long long)__ldg(a.bias_starts + row + 1), a.n_biases) - b0);
+    }
+    const float rep = a.repetition ? __ldg(a.repetition + row) : 1.f;
+    const float pres = a.presence ? __ldg(a.presence + row) : 0.f, freq = a.frequency ? __ldg(a.frequency + row) : 0.f;
+    const uint32_t* words = nullptr;  // the row's mask; null: everything is allowed
+    if (a.allowed) {
+        const int mask = a.mask_rows ? __ldg(a.mask_rows + row) : row;
+        if ((unsigned)mask < (unsigned)a.n_masks) words = a.allowed + (size_t)mask * a.mask_words + (v0 >> 5);
+    }
+    const T* in = (const T*)a.logits + row * a.in_row + v0;
+    T* out = (T*)a.out + row * a.out_row + v0;
+    auto allows = [&](int i) { return !words || ((__ldg(words + (i >> 5)) >> (i & 31)) & 1); };
+    auto clear = [&](int n) {
+        for (int i = tid; i < n / 4; i += CTL_THREADS) reinterpret_cast<uint4*>(ctl_smem)[i] = make_uint4(0, 0, 0, 0);
+    };
+    // entry i of the slice, named `count` times in the window, `bias`: 1 + the
+    // index of its last bias
+    auto change = [&](int i, float x, uint32_t count, uint32_t bias) {
         if (count) {
             if (a.repetition) x = x < 0.f ? x * rep : x / rep;
             x = x - pres - freq * (float)count;
         }
-        if (bias) x += __ldg(biases + bias - 1);
-        return x;
-    }
-};
-
-// 32 bits of a bit string from bit `at` on; words past `last` are not read.
-FB2_DEV uint32_t bits_from(const uint32_t* w, int at, int last) {
-    const int i = at >> 5;
-    return __funnelshift_r(w[i], i < last ? w[i + 1] : 0u, at & 31);
-}
-
-template <class T>
-__global__ void __launch_bounds__(CTL_THREADS, 3) k_logit_controls(ControlArgs a, int chunk) {
-    extern __shared__ uint32_t ctl_smem[];
-    uint32_t* table = ctl_smem;          // [chunk]
-    uint32_t* bits = ctl_smem + chunk;   // [chunk / 32]
-    const int tid = threadIdx.x, row = blockIdx.y;
-    const int c0 = blockIdx.x * chunk, c1 = min(c0 + chunk, a.vocab);
-
-    long long t0 = 0, t1 = 0, b0 = 0, b1 = 0;
-    if (a.tokens) {
-        t0 = max(__ldg(a.token_starts + row), 0);
-        t1 = min((long long)__ldg(a.token_starts + row + 1), a.n_tokens);
-    }
-    if (a.bias_ids) {
-        b0 = max(__ldg(a.bias_starts + row), 0);
-        b1 = min((long long)__ldg(a.bias_starts + row + 1), a.n_biases);
-    }
-    ControlRow<T> r{a, nullptr, 1.f, 0.f, 0.f, a.bias_values + b0};
-    if (a.repetition) r.rep = __ldg(a.repetition + row);
-    if (a.presence) r.pres = __ldg(a.presence + row);
-    if (a.frequency) r.freq = __ldg(a.frequency + row);
-    if (a.allowed) {
-        const int mask = a.mask_rows ? __ldg(a.mask_rows + row) : row;
-        if ((unsigned)mask < (unsigned)a.n_masks) r.allowed = a.allowed + (size_t)mask * a.mask_words;
-    }
-    const T* in = (const T*)a.logits + row * a.in_row;
-    T* out = (T*)a.out + row * a.out_row;
-
-    const bool shared_word = t1 - t0 <= 0xffff && b1 - b0 <= 0xfffe;
-    const int cap = shared_word ? chunk : chunk / 2;  // chunk is a multiple of 64
-    for (int v0 = c0; v0 < c1; v0 += cap) {
-        const int n = min(cap, c1 - v0);
-        uint32_t* bias_table = shared_word ? table : table + cap;
-        for (int i = tid; i < cap / 32; i += CTL_THREADS) bits[i] = 0;
-        __syncthreads();
-        auto touch = [&](int id) {
-            const uint32_t at = (uint32_t)id - (uint32_t)v0;
-            if (at < (uint32_t)n) {
-                atomicOr(bits + (at >> 5), 1u << (at & 31));
-                table[at] = 0;
-                if (!shared_word) bias_table[at] = 0;
-            }
-        };
-#pragma unroll 4
-        for (long long i = t0 + tid; i < t1; i += CTL_THREADS) touch(__ldg(a.tokens + i));
-        for (long long i = b0 + tid; i < b1; i += CTL_THREADS) touch(__ldg(a.bias_ids + i));
-        __syncthreads();
-        for (long long i = b0 + tid; i < b1; i += CTL_THREADS) {
-            const uint32_t at = (uint32_t)__ldg(a.bias_ids + i) - (uint32_t)v0;
-            if (at < (uint32_t)n) atomicMax(bias_table + at, (uint32_t)(i - b0 + 1) << (shared_word ? 16 : 0));
+        if (bias) x += __ldg(a.bias_values + b0 + bias - 1);
+        out[i] = Dense<T>::put(x);
+    };
+    auto copy = [&]() {
+        constexpr int PER = 16 / sizeof(T);
+        auto one = [&](int i) { out[i] = allows(i) ? in[i] : Dense<T>::put(-INFINITY); };
+        const uint32_t in_at = (uint32_t)reinterpret_cast<uintptr_t>(in) & 15, out_at = (uint32_t)reinterpret_cast<uintptr_t>(out) & 15;
+        if (in_at != out_at) {  // of different alignment: one entry at a time
+            for (int i = tid; i < len; i += CTL_THREADS) one(i);
+            return;
         }
-        __syncthreads();
-#pragma unroll 4
-        for (long long i = t0 + tid; i < t1; i += CTL_THREADS) {
-            const uint32_t at = (uint32_t)__ldg(a.tokens + i) - (uint32_t)v0;
-            if (at < (uint32_t)n) atomicAdd(table + at, 1u);
-        }
-        __syncthreads();
-
-        auto touched = [&](float x, int at) {
-            const uint32_t w = table[at];
-            return shared_word ? r.value(x, w & 0xffffu, w >> 16) : r.value(x, w, bias_table[at]);
-        };
-        auto one = [&](int at) {
-            const int v = v0 + at;
-            if (r.allowed && !((__ldg(r.allowed + (v >> 5)) >> (v & 31)) & 1)) {
-                out[v] = Dense<T>::put(-INFINITY);
-            } else if ((bits[at >> 5] >> (at & 31)) & 1) {
-                out[v] = Dense<T>::put(touched(Dense<T>::get(in[v]), at));
-            } else {
-                out[v] = in[v];
-            }
-        };
-        constexpr int PER = 16 / sizeof(T);  // entries of 16 bytes
-        const uint32_t in_at = (uint32_t)reinterpret_cast<uintptr_t>(in + v0) & 15, out_at = (uint32_t)reinterpret_cast<uintptr_t>(out + v0) & 15;
-        if (in_at != out_at) {  // in and out of different alignment: one entry at a time
-            for (int i = tid; i < n; i += CTL_THREADS) one(i);
-        } else {
-            const int head = min(n, (int)((16 - in_at) & 15) / (int)sizeof(T)), vecs = (n - head) / PER;
-            if (tid < head) one(tid);
-            if (head + vecs * PER + tid < n) one(head + vecs * PER + tid);
-            const uint4* from = reinterpret_cast<const uint4*>(in + v0 + head);
-            uint4* to = reinterpret_cast<uint4*>(out + v0 + head);
-            constexpr int U = 4;  // loads in flight
-            for (int i0 = tid; i0 < vecs; i0 += CTL_THREADS * U) {
-                uint4 x[U];
-                uint32_t ok[U];
+        const int head = min(len, (int)((16 - in_at) & 15) / (int)sizeof(T)), vecs = (len - head) / PER;
+        const int n_words = a.mask_words - (v0 >> 5);
+        const uint4* from = reinterpret_cast<const uint4*>(in + head);
+        uint4* to = reinterpret_cast<uint4*>(out + head);
+        if (tid < head) one(tid);
+        if (head + vecs * PER + tid < len) one(head + vecs * PER + tid);
+        for (int i0 = tid; i0 < vecs; i0 += CTL_THREADS * CTL_VECS) {
+            uint4 x[CTL_VECS];
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const int i = i0 + u * CTL_THREADS;
-                    if (i < vecs) {
-                        x[u] = __ldcs(from + i);
-                        ok[u] = r.allowed ? bits_from(r.allowed, v0 + head + i * PER, a.mask_words - 1) : 0xffffffffu;
-                    }
-                }
+            for (int u = 0; u < CTL_VECS; u++)
+                if (i0 + u * CTL_THREADS < vecs) x[u] = from[i0 + u * CTL_THREADS];
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const int i = i0 + u * CTL_THREADS, at = head + i * PER;
-                    if (i >= vecs) break;
-                    uint32_t hit = bits_from(bits, at, cap / 32 - 1) & ((1u << PER) - 1);
-                    uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-                    if (hit &= ok[u]) {
-#pragma unroll
-                        for (int e = 0; e < PER; e++)
-                            if ((hit >> e) & 1) {
-                                if constexpr (sizeof(T) == 4) {
-                                    w[e] = __float_as_uint(touched(__uint_as_float(w[e]), at + e));
-                                } else {
-                                    const unsigned short h = (unsigned short)(w[e / 2] >> (16 * (e & 1)));
-                                    T v;
-                                    memcpy(&v, &h, 2);
-                                    v = Dense<T>::put(touched(Dense<T>::get(v), at + e));
-                                    unsigned short z;
-                                    memcpy(&z, &v, 2);
-                                    w[e / 2] = __byte_perm(w[e / 2], z, e & 1 ? 0x5410 : 0x3254);
-                                }
-                            }
-                    }
+            for (int u = 0; u < CTL_VECS; u++) {
+                const int i = i0 + u * CTL_THREADS;
+                if (i >= vecs) break;
+                uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+                if (words) {
+                    const int e0 = head + i * PER, at = e0 >> 5;  // PER bits from e0 on
+                    const uint32_t ok = __funnelshift_r(__ldg(words + at), at + 1 < n_words ? __ldg(words + at + 1) : 0u, e0 & 31);
 #pragma unroll
                     for (int e = 0; e < PER; e++) {
                         constexpr uint32_t NEG = std::is_same<T, __half>::value ? 0xfc00u : 0xff80u;
                         if constexpr (sizeof(T) == 4) {
-                            if (!((ok[u] >> e) & 1)) w[e] = 0xff800000u;
+                            if (!((ok >> e) & 1)) w[e] = 0xff800000u;
                         } else {
-                            if (!((ok[u] >> e) & 1)) w[e / 2] = e & 1 ? (w[e / 2] & 0xffffu) | NEG << 16 : (w[e / 2] & 0xffff0000u) | NEG;
+                            if (!((ok >> e) & 1)) w[e / 2] = e & 1 ? (w[e / 2] & 0xffffu) | NEG << 16 : (w[e / 2] & 0xffff0000u) | NEG;
                         }
                     }
-                    __stcs(to + i, make_uint4(w[0], w[1], w[2], w[3]));
                 }
+                to[i] = make_uint4(w[0], w[1], w[2], w[3]);
             }
         }
-        __syncthreads();  // the table is written again
+    };
+
+    if (nt + nb <= min(slots / 4 * 3, CTL_THREADS * CTL_IDS)) {
+        // key: 1 + entry of the slice, 0 if free; value: bias << 16 | count.
+        // The thread that takes a slot writes its entry.
+        uint32_t *keys = ctl_smem, *values = ctl_smem + slots;
+        const int n = (int)(nt + nb), nbias = (int)nb, shift = 32 - __popc(slots - 1);
+        int at[CTL_IDS];
+        uint32_t mine = 0;
+        if (n) {
+#pragma unroll
+            for (int u = 0; u < CTL_IDS; u++) {
+                const int j = u * CTL_THREADS + tid;
+                at[u] = -1;
+                if (u * CTL_THREADS < n && j < n) at[u] = __ldg(j < nbias ? a.bias_ids + b0 + j : a.tokens + t0 + (j - nbias));
+            }
+            clear(2 * slots);
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < CTL_IDS; u++) {
+                if (u * CTL_THREADS >= n) break;
+                const int e = (uint32_t)at[u] < (uint32_t)a.vocab ? at[u] - v0 : -1;
+                at[u] = -1;
+                if ((uint32_t)e >= (uint32_t)len) continue;
+                uint32_t s = ((uint32_t)e * 0x9e3779b1u) >> shift;
+                for (;;) {
+                    const uint32_t was = atomicCAS(keys + s, 0u, (uint32_t)e + 1u);
+                    if (was == 0u) mine |= 1u << u;
+                    if (was == 0u || was == (uint32_t)e + 1u) break;
+                    s = (s + 1) & (slots - 1);
+                }
+                at[u] = (int)s;
+                if (u * CTL_THREADS + tid < nbias) atomicMax(values + s, (uint32_t)(u * CTL_THREADS + tid + 1) << 16);
+            }
+            if (nbias) __syncthreads();  // counts are added to finished indexes of biases
+#pragma unroll
+            for (int u = 0; u < CTL_IDS; u++)
+                if (u * CTL_THREADS < n && at[u] >= 0 && u * CTL_THREADS + tid >= nbias) atomicAdd(values + at[u], 1u);
+        }
+        T x[CTL_IDS];  // in place the copies write the same logits
+#pragma unroll
+        for (int u = 0; u < CTL_IDS; u++)
+            if ((mine >> u) & 1) {
+                const int e = (int)keys[at[u]] - 1;
+                if (allows(e))
+                    x[u] = in[e];
+                else
+                    mine &= ~(1u << u);
+            }
+        if (copies) copy();
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < CTL_IDS; u++)
+            if ((mine >> u) & 1) change((int)keys[at[u]] - 1, Dense<T>::get(x[u]), values[at[u]] & 0xffffu, values[at[u]] >> 16);
+        return;
+    }
+    // longer lists: ranges of ids, two words for each
+    if (copies) copy();
+    uint32_t *counts = ctl_smem, *biases = ctl_smem + slots;
+    for (int e0 = 0; e0 < len; e0 += slots) {
+        const int range = min(slots, len - e0), base = v0 + e0;
+        __syncthreads();
+        clear(2 * slots);
+        __syncthreads();
+        for (long long i = tid; i < nb; i += CTL_THREADS) {
+            const int e = __ldg(a.bias_ids + b0 + i) - base;
+            if ((uint32_t)e < (uint32_t)range) atomicMax(biases + e, (uint32_t)i + 1u);
+        }
+#pragma unroll 4
+        for (long long i = tid; i < nt; i += CTL_THREADS) {
+            const int e = __ldg(a.tokens + t0 + i) - base;
+            if ((uint32_t)e < (uint32_t)range) atomicAdd(counts + e, 1u);
+        }
+        __syncthreads();
+        for (int i = tid; i < range; i += CTL_THREADS)
+            if ((counts[i] | biases[i]) && allows(e0 + i)) change(e0 + i, Dense<T>::get(in[e0 + i]), counts[i], biases[i]);
     }
 }
 

@@ -573,16 +573,20 @@ int32_t fb2_logit_controls(const fb2_logit_control* c, void* stream) {
                       c->device_presence, c->device_frequency, c->device_bias_ids, c->device_bias_values,
                       c->device_bias_starts, c->device_allowed, c->device_mask_rows, c->logits_row_stride,
                       c->out_row_stride, c->n_tokens, c->n_biases, c->n_rows, c->vocab, c->n_masks, c->mask_words};
-        // long rows: few chunks, as each looks through the row's lists; few rows:
-        // enough chunks to give every SM some
-        int chunk = 16384;
-        while (chunk > 512 && (int64_t)((c->vocab + chunk - 1) / chunk) * c->n_rows < 148 * 3) chunk /= 2;
-        const dim3 grid((c->vocab + chunk - 1) / chunk, c->n_rows);
-        const int smem = chunk * 4 + chunk / 8;
+        const bool copies = c->device_allowed || c->device_out != c->device_logits || c->out_row_stride != c->logits_row_stride;
+        // room for the average list in half the table; a row whose list is longer
+        // than three quarters of it goes through ranges of ids
+        const int64_t average = (c->n_tokens + c->n_biases + c->n_rows - 1) / c->n_rows;
+        int slots = 1024;
+        while (slots < CTL_SLOTS && slots / 2 < average) slots *= 2;
+        // two CTAs on each SM, of at least 2048 entries each
+        const int slices = std::max(1, std::min(2 * 148 / std::max(c->n_rows, 1), c->vocab / 2048));
+        const int slice = ((c->vocab + slices - 1) / slices + 31) / 32 * 32;
         with_type(c->dtype, [&](auto t) {
             using T = decltype(t);
-            if (smem > 48 * 1024) opt_in_smem((const void*)k_logit_controls<T>, smem);
-            k_logit_controls<T><<<grid, CTL_THREADS, smem, (cudaStream_t)stream>>>(a, chunk);
+            if (slots * 8 > 48 * 1024) opt_in_smem((const void*)k_logit_controls<T>, slots * 8);
+            k_logit_controls<T><<<dim3((c->vocab + slice - 1) / slice, c->n_rows), CTL_THREADS, slots * 8, (cudaStream_t)stream>>>(
+                a, slice, slots, copies);
         });
         launched();
     });
