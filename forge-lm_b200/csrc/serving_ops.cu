@@ -574,11 +574,9 @@ int32_t fb2_logit_controls(const fb2_logit_control* c, void* stream) {
                       c->device_bias_starts, c->device_allowed, c->device_mask_rows, c->logits_row_stride,
                       c->out_row_stride, c->n_tokens, c->n_biases, c->n_rows, c->vocab, c->n_masks, c->mask_words};
         const bool copies = c->device_allowed || c->device_out != c->device_logits || c->out_row_stride != c->logits_row_stride;
-        // room for the average list in half the table; a row whose list is longer
-        // than three quarters of it goes through ranges of ids
-        const int64_t average = (c->n_tokens + c->n_biases + c->n_rows - 1) / c->n_rows;
+        // a table with half of its slots free for a row that has all of the lists
         int slots = 1024;
-        while (slots < CTL_SLOTS && slots / 2 < average) slots *= 2;
+        while (slots < CTL_SLOTS && slots / 2 < c->n_tokens + c->n_biases) slots *= 2;
         // two CTAs on each SM, of at least 2048 entries each
         const int slices = std::max(1, std::min(2 * 148 / std::max(c->n_rows, 1), c->vocab / 2048));
         const int slice = ((c->vocab + slices - 1) / slices + 31) / 32 * 32;

@@ -689,6 +689,154 @@ def test_controls_of_long_windows(pkg):
     assert ((got - want).abs() <= 2.0 ** -22 * (want.abs() + 10)).all()
 
 
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "fp16"])
+@pytest.mark.parametrize("ids", [511, 768, 769, 4096, 6143, 6145, 9000])
+def test_controls_of_lists_of_many_different_ids(pkg, dtype, ids):
+    """One row's lists alone are long: what it keeps of them outgrows one size after another."""
+    rnd = random.Random(ids)
+    vocab = 20001
+    logits = (3 * normal(gen(ids), 3, vocab)).to(DTYPES[dtype])
+    windows = [[5, 5, 20000], rnd.sample(range(vocab), ids - 200) + [19999] * 40, []]
+    some = rnd.sample(range(vocab), 159)
+    biases = [[], [(t, float(np.float32(rnd.uniform(-2, 2)))) for t in some + some[:1]], [(7, 1.25)]]
+    tokens, token_starts = lists(windows, torch.int32)
+    bias_ids, bias_starts = lists([[t for t, _ in r] for r in biases], torch.int32)
+    values, _ = lists([[b for _, b in r] for r in biases], torch.float32)
+    rep, pres = torch.tensor([1.5, 1.25, 2.0], device="cuda"), torch.tensor([0.5, -0.25, 1.0], device="cuda")
+    freq = torch.tensor([0.125, 0.0625, 1.0], device="cuda")
+    every = dict(tokens=tokens, token_starts=token_starts, repetition=rep, presence=pres, frequency=freq,
+                 bias_ids=bias_ids, bias_values=values, bias_starts=bias_starts)
+    got = pkg.logit_controls(logits, **every)
+    check_controls(got, plain_controls(logits, windows, rep, pres, freq, biases))
+    pkg.logit_controls(logits, out=logits, **every)
+    assert torch.equal(logits, got)
+
+
+# ---- together -------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_operators_in_a_graph(pkg, dtype):
+    """Captured once, replayed with other contents of the same tensors."""
+    g = gen(77)
+    cache = filled(pkg, g, 12, 16, 2, 64, "int8")
+    linear = random_linear(pkg, g, 512, 96, 64, True)
+    table = torch.arange(12, dtype=torch.int32, device="cuda").view(2, 6)
+    prefix, starts = _i32([40, 90]), _i32([0, 3, 5])
+    slots, mask = _i32([40, 41, 42, 186, 187]), _i32([[1], [3], [5], [1], [3]])
+    tokens, token_starts = _i32([1, 2, 2, 7, 9]), _i32([0, 3, 4, 4, 5, 5])
+    rep = torch.full((5,), 1.5, device="cuda")
+
+    def step(k, v, q):
+        cache.write(k, v, slots)
+        out, lse = cache.attend(q, table, prefix, starts=starts, mask=mask, max_nodes=3, max_len=96)
+        y = linear(out.reshape(5, 512))
+        return out, lse, y, pkg.logit_controls(y, tokens=tokens, token_starts=token_starts, repetition=rep)
+
+    def inputs():
+        return [normal(g, 5, h, 64).to(DTYPES[dtype]) for h in (2, 2, 8)]
+
+    held = inputs()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*held)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(*held)
+    for _ in range(3):
+        for t, new in zip(held, inputs()):
+            t.copy_(new)
+        want = [t.clone() for t in step(*held)]
+        for t in outs:
+            t.zero_()
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+@gpu
+@pytest.mark.parametrize("fmt,dtype", [("int8", "fp32"), ("int4", "fp32"), ("int8", "bf16"), ("int4", "fp16")])
+@pytest.mark.parametrize("scale", [0.0, -0.07, 1e-6])
+def test_attention_with_any_scale(pkg, fmt, dtype, scale):
+    """No weighting, the smallest scores first, and nearly none; few rows and many."""
+    attention_case(pkg, 91, fmt, dtype, [70, 0, 33], [1, 1, 1], 4, 2, 64, 16, False, scale=scale)
+    attention_case(pkg, 92, fmt, dtype, [150, 9], [20, 40], 4, 1, 64, 16, True, scale=scale)
+    attention_case(pkg, 93, fmt, dtype, [150, 9], [20, 40], 4, 2, 80, 16, True, scale=scale)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("dim,share", [(48, 6), (80, 3), (128, 8)])
+def test_attention_of_many_unaligned_rows(pkg, fmt, dtype, dim, share):
+    """The same rows at an odd element and in one piece: the same values."""
+    g = gen(dim)
+    cache = filled(pkg, g, 40, 16, 2, dim, fmt)
+    table = torch.randperm(40, generator=torch.Generator().manual_seed(3)).to(torch.int32).cuda().view(2, 20)
+    rows, heads = 33, 2 * share
+    flat = normal(g, rows * heads * dim + 1).to(DTYPES[dtype])
+    q = flat[1:].view(rows, heads, dim)
+    args = (table, _i32([281, 130]))
+    kw = dict(starts=_i32([0, 20, 33]), max_nodes=20)
+    out, lse = cache.attend(q, *args, **kw)
+    again, lse2 = cache.attend(q.clone(), *args, **kw)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+    bits = [set(range(i + 1)) for t in (20, 13) for i in range(t)]
+    want = plain_attention(cache, q, table.cpu(), [281, 130], [0, 20, 33], bits, 1 / math.sqrt(dim))
+    k, v = cache.read(torch.arange(640, dtype=torch.int32, device="cuda"))
+    check_attention(dtype, (out, lse), want, float(v.abs().max()),
+                    float(q.float().norm(dim=2).max() * k.norm(dim=2).max()) / math.sqrt(dim))
+
+
+@gpu
+@pytest.mark.parametrize("cache", ["int8", "int4"])
+def test_example_of_a_decoder(pkg, cache):
+    """Drafted generation gives greedy tokens: each is the largest controlled
+    logit of a run of the whole text in one piece, up to the difference that
+    a stored code one step off makes (a score moves by 1 / 127 or 1 / 15 of
+    its key's range at most where sums of another order round another way)."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "quantised_decode.py")
+    spec = importlib.util.spec_from_file_location("quantised_decode", path)
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    cfg = pkg.ModelConfig(512, 128, 128, 3, 4)
+    params = pkg.init_params(cfg, 5)
+    prompts = [[1, 2, 3, 1, 2, 3, 1, 2], [7], [9, 8] * 20]
+    words = torch.full((1, 16), -1, dtype=torch.int32, device="cuda")
+    words[0, 1], words[0, 15] = 0, 0  # neither 32..63 nor 480..511
+
+    def model():
+        return ex.QuantisedGpt(cfg, params, 3, cache, dtype=torch.float32)
+
+    out, steps = ex.generate(model(), prompts, 24, draft=4, repetition=0.8, allowed=words)
+    assert [len(t) for t in out] == [24] * 3 and 1 <= steps <= 24
+    once, single = ex.generate(model(), prompts, 24, draft=0, repetition=0.8, allowed=words)
+    assert single == 24 and steps < 24  # a repetition "penalty" below one repeats itself: drafts are kept
+    text = [p + t for p, t in zip(prompts, out)]
+    whole = model()
+    starts, slots = [0], []
+    for s, t in enumerate(text):
+        starts.append(starts[-1] + len(t))
+        slots += whole.slots(s, range(len(t)))
+    logits = whole.logits([x for t in text for x in t], [i for t in text for i in range(len(t))], slots, [0, 0, 0],
+                          starts, max_nodes=max(map(len, text)))
+    step = 1 / 127 if cache == "int8" else 1 / 15
+    for s, (p, t) in enumerate(zip(prompts, text)):
+        for i in range(len(p), len(t)):
+            assert not (32 <= t[i] < 64 or t[i] >= 480)
+            row = logits[starts[s] + i - 1:starts[s] + i]
+            want = plain_controls(row, [t[:i]], [0.8], allowed=words, mask_rows=[0])[0]
+            assert float(want[t[i]]) >= float(want.max()) - step * float(row.abs().max())
+
+
 # ---- refusals -------------------------------------------------------------------------------
 
 @gpu
