@@ -8,6 +8,8 @@
 // All in fp32 with IEEE division and rounding to nearest even; the codes use
 // the rounded scale and minimum, so the stored row is the best one for them.
 #pragma once
+#include <type_traits>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -89,6 +91,40 @@ struct Dense<__half> {
     static FB2_DEV __half put(float v) { return __float2half_rn(v); }
 };
 
+// 16 bytes <-> their values, two at a time for the 16-bit types.
+template <class T>
+FB2_DEV void unpack16(const uint4& w, float* x) {
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) {
+            x[i] = __uint_as_float(v[i]);
+        } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            x[2 * i] = __uint_as_float(v[i] << 16), x[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+        } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[i]));
+            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        }
+    }
+}
+template <class T>
+FB2_DEV uint4 pack16(const float* x) {
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) {
+            v[i] = __float_as_uint(x[i]);
+        } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+            memcpy(&v[i], &h, 4);
+        } else {
+            const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+            memcpy(&v[i], &h, 4);
+        }
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
 // 8 values from p (VEC: p is 16-byte aligned).
 template <class T, bool VEC>
 FB2_DEV void load8(const T* p, float (&x)[8]) {
@@ -105,7 +141,7 @@ FB2_DEV void load8(const T* p, float (&x)[8]) {
         for (int i = 0; i < 8; i++) x[i] = Dense<T>::get(p[i]);
     }
 }
-// A row is shared by `width` neighbouring lanes of a warp (a power of two); a
+// A row is shared by `width` = 1 << `shift` neighbouring lanes of a warp; a
 // lane holds NP pieces of 16 bytes, piece j at index part + width * j, so that
 // every load and store of a row is one run of bytes.  16 values per lane: the
 // reductions over the row, the divisions and the addresses are paid once for
@@ -161,6 +197,17 @@ FB2_DEV float max_nan(float a, float b) {
     return d;
 }
 
+FB2_DEV float min3_nan(float a, float b, float c) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+FB2_DEV float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // rint(x) for |x| < 2^22 as the low bits of 1.5 2^23 + x
 constexpr float kRint = 12582912.0f;
 constexpr uint32_t kRintBits = 0x4b400000u;
@@ -169,10 +216,11 @@ constexpr uint32_t kRintBits = 0x4b400000u;
 template <class T, int FMT, bool VEC>
 __global__ void __launch_bounds__(KVQ_THREADS)
     k_kvq_write(KvqView c, int n_rows, const T* __restrict__ k, const T* __restrict__ v, long long k_row, long long k_head,
-                long long v_row, long long v_head, const int* __restrict__ slots, int width) {
+                long long v_row, long long v_head, const int* __restrict__ slots, int shift) {
     constexpr int N = KvqPiece<T>::N, NP = KvqPiece<T>::NP;
     const int kind = blockIdx.z, head = blockIdx.y;
-    const int row = blockIdx.x * (KVQ_THREADS / width) + threadIdx.x / width, part = threadIdx.x & (width - 1);
+    const int width = 1 << shift;
+    const int row = blockIdx.x * (KVQ_THREADS >> shift) + (threadIdx.x >> shift), part = threadIdx.x & (width - 1);
     // lanes of a row agree on `live`; the shuffles below run with the whole warp
     const int slot = row < n_rows ? __ldg(slots + row) : -1;
     const bool live = (uint32_t)slot < (uint32_t)c.n_slots;
@@ -186,10 +234,7 @@ __global__ void __launch_bounds__(KVQ_THREADS)
         if constexpr (VEC) {
             uint4 w = make_uint4(0, 0, 0, 0);
             if (mine[j]) w = __ldcs(reinterpret_cast<const uint4*>(p) + piece);
-            T t[N];
-            memcpy(t, &w, 16);
-#pragma unroll
-            for (int i = 0; i < N; i++) x[j][i] = Dense<T>::get(t[i]);
+            unpack16<T>(w, x[j]);
         } else {
 #pragma unroll
             for (int i = 0; i < N; i++) x[j][i] = mine[j] ? Dense<T>::get(p[piece * N + i]) : 0.f;
@@ -198,26 +243,27 @@ __global__ void __launch_bounds__(KVQ_THREADS)
     const size_t at = live ? c.row(slot, head, kind) : 0;
     unsigned char* to = c.codes + at * c.row_bytes;
     if constexpr (FMT == KVQ_INT8) {
-        // max|x| through the bits: NaN > inf > finite
-        uint32_t top = 0;
+        float amax = 0.f;  // NaN stays
 #pragma unroll
         for (int j = 0; j < NP; j++)
 #pragma unroll
-            for (int i = 0; i < N; i++) top = max(top, __float_as_uint(x[j][i]) & 0x7fffffffu);
-        for (int o = width / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const bool finite = top < 0x7f800000u;
-        const float amax = __uint_as_float(top);
+            for (int i = 0; i < N; i += 2) amax = max3_nan(amax, fabsf(x[j][i]), fabsf(x[j][i + 1]));
+        for (int o = width / 2; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        const bool finite = amax < INFINITY;  // false for NaN
         const bool some = finite && amax >= kKvqTiny;
         const float inv = some ? 127.0f / amax : 0.0f;
 #pragma unroll
         for (int j = 0; j < NP; j++) {
             if (!mine[j]) continue;
-            uint32_t w[2] = {0, 0};
+            // |x inv| <= 127 (1 + 2^-23): it rounds to 127 at most; NaN rows hold code 0
+            uint32_t w[2];
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                // |x inv| <= 127 (1 + 2^-23): it rounds to 127 at most; NaN rows hold code 0
-                const float f = finite ? x[j][i] * inv : 0.f;
-                w[i / 4] += (__float_as_uint(f + kRint) - kRintBits + 128u) << (8 * (i % 4));
+            for (int i = 0; i < N; i += 4) {
+                uint32_t q[4];
+#pragma unroll
+                for (int l = 0; l < 4; l++) q[l] = __float_as_uint(x[j][i + l] * inv + (kRint + 128.0f));
+                const uint32_t four = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+                w[i / 4] = finite ? four : 0x80808080u;
             }
             kvq_store_codes<FMT, N>(to, part + width * j, w);
         }
@@ -229,7 +275,7 @@ __global__ void __launch_bounds__(KVQ_THREADS)
         for (int j = 0; j < NP; j++)
             if (mine[j])
 #pragma unroll
-                for (int i = 0; i < N; i++) lo = min_nan(lo, x[j][i]), hi = max_nan(hi, x[j][i]);
+                for (int i = 0; i < N; i += 2) lo = min3_nan(lo, x[j][i], x[j][i + 1]), hi = max3_nan(hi, x[j][i], x[j][i + 1]);
         for (int o = width / 2; o > 0; o >>= 1) {
             lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
             hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
@@ -238,16 +284,18 @@ __global__ void __launch_bounds__(KVQ_THREADS)
         const float least = bf16_bits_to_float(least_b), scale = bf16_bits_to_float(scale_b);
         const bool finite = scale < inf && fabsf(least) < inf;  // false for NaN
         const bool some = finite && scale >= kKvqTiny;
-        const float inv = some ? 1.0f / scale : 0.0f;
+        const float inv = some ? 1.0f / scale * (1.0f / 15.0f) : 0.0f;
 #pragma unroll
         for (int j = 0; j < NP; j++) {
             if (!mine[j]) continue;
-            uint32_t w = 0;
+            uint32_t w = 0;  // the sum of the shifted bits less that of kRint's
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const float f = some ? fminf(fmaxf((x[j][i] - least) * inv, 0.0f), 15.0f) : 0.f;
-                w += (__float_as_uint(f + kRint) - kRintBits) << (4 * i);
+                // in 0..1 (NaN, and inf 0: 0): the minimum and scale are rounded, a value may lie outside
+                const float f = __saturatef((x[j][i] - least) * inv);
+                w += __float_as_uint(fmaf(f, 15.0f, kRint)) << (4 * i);
             }
+            w -= N == 8 ? kRintBits * 0x11111111u : kRintBits * 0x1111u;
             kvq_store_codes<FMT, N>(to, part + width * j, &w);
         }
         if (part == 0 && live) c.meta[at] = finite ? ((some ? scale_b : 0u) | (least_b << 16)) : 0x7fc07fc0u;
@@ -256,10 +304,11 @@ __global__ void __launch_bounds__(KVQ_THREADS)
 
 template <class T, int FMT>
 __global__ void __launch_bounds__(KVQ_THREADS)
-    k_kvq_read(KvqView c, int n_rows, const int* __restrict__ slots, T* __restrict__ k, T* __restrict__ v, int width) {
+    k_kvq_read(KvqView c, int n_rows, const int* __restrict__ slots, T* __restrict__ k, T* __restrict__ v, int shift) {
     constexpr int N = KvqPiece<T>::N, NP = KvqPiece<T>::NP;
     const int kind = blockIdx.z, head = blockIdx.y;
-    const int row = blockIdx.x * (KVQ_THREADS / width) + threadIdx.x / width, part = threadIdx.x & (width - 1);
+    const int width = 1 << shift;
+    const int row = blockIdx.x * (KVQ_THREADS >> shift) + (threadIdx.x >> shift), part = threadIdx.x & (width - 1);
     if (row >= n_rows) return;
     const int slot = __ldg(slots + row);
     const bool live = (uint32_t)slot < (uint32_t)c.n_slots;
@@ -273,25 +322,25 @@ __global__ void __launch_bounds__(KVQ_THREADS)
         for (int j = 0; j < NP; j++)
             if ((part + width * j) * N < c.hd) kvq_load_codes<FMT, N>(c.codes + at * c.row_bytes, part + width * j, w[j]);
     }
+    const float scale = bf16_bits_to_float(m & 0xffffu), scale16 = scale * 0.0625f, least = __uint_as_float(m & 0xffff0000u);
     uint4* to = reinterpret_cast<uint4*>((kind ? v : k) + ((size_t)row * c.heads + head) * c.hd);
 #pragma unroll
     for (int j = 0; j < NP; j++) {
         if ((part + width * j) * N >= c.hd) continue;
-        T t[N];
+        float x[N];
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            float x;
             if constexpr (FMT == KVQ_INT8) {
-                const float code = __uint_as_float(kRintBits + ((w[j][i / 4] >> (8 * (i % 4))) & 0xffu)) - (kRint + 128.0f);
-                x = live ? code * __uint_as_float(m) : 0.f;
+                const float code = __uint_as_float(__byte_perm(w[j][i / 4], kRintBits, 0x7650 + i % 4)) - (kRint + 128.0f);
+                x[i] = code * __uint_as_float(m);
             } else {
-                const float code = __uint_as_float(kRintBits + ((w[j][0] >> (4 * i)) & 15u)) - kRint;
-                x = fmaf(code, bf16_bits_to_float(m & 0xffffu), __uint_as_float(m & 0xffff0000u));
+                // a byte's high nibble stays in place: 16 code, with scale / 16 (a power of two: exact)
+                const uint32_t byte = w[j][0] >> (8 * (i / 2)), nibble = i & 1 ? 0xf0u : 0xfu;
+                const float code = __uint_as_float((byte & nibble) | kRintBits) - kRint;
+                x[i] = fmaf(code, i & 1 ? scale16 : scale, least);
             }
-            t[i] = Dense<T>::put(x);
         }
-        uint4 o;
-        memcpy(&o, t, 16);
+        const uint4 o = live ? pack16<T>(x) : make_uint4(0, 0, 0, 0);
         __stcs(to + part + width * j, o);
     }
 }

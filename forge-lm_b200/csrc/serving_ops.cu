@@ -84,13 +84,13 @@ KvqView view_of(const fb2_kvq_cache* c) {
 }
 
 // lanes of a row at 16 values each, a power of two
-int row_lanes(int hd) {
-    int w = 1;
-    while (w * 16 < hd) w *= 2;
-    return w;
+int row_shift(int hd) {
+    int s = 0;
+    while ((16 << s) < hd) s++;
+    return s;
 }
-dim3 row_grid(int n_rows, int heads, int width) {
-    const int per = KVQ_THREADS / width;
+dim3 row_grid(int n_rows, int heads, int shift) {
+    const int per = KVQ_THREADS >> shift;
     return dim3((unsigned)(((int64_t)n_rows + per - 1) / per), heads, 2);
 }
 
@@ -116,8 +116,8 @@ int32_t fb2_kvq_write(const fb2_kvq_cache* c, int32_t n_rows, const void* k, con
         need(k && v && slots, "NULL argument");
         const size_t es = size_of(dtype);
         need(aligned(k, es) && aligned(v, es) && aligned(slots, 4), "a tensor is not aligned to its element size");
-        const int width = row_lanes(view.hd);
-        const dim3 grid = row_grid(n_rows, view.heads, width);
+        const int shift = row_shift(view.hd);
+        const dim3 grid = row_grid(n_rows, view.heads, shift);
         const bool vec = aligned(k, 16) && aligned(v, 16) && k_row * es % 16 == 0 && k_head * es % 16 == 0 &&
                          v_row * es % 16 == 0 && v_head * es % 16 == 0;
         with_type(dtype, [&](auto t) {
@@ -125,7 +125,7 @@ int32_t fb2_kvq_write(const fb2_kvq_cache* c, int32_t n_rows, const void* k, con
             auto kernel = view.row_bytes == view.hd ? (vec ? k_kvq_write<T, KVQ_INT8, true> : k_kvq_write<T, KVQ_INT8, false>)
                                                     : (vec ? k_kvq_write<T, KVQ_INT4, true> : k_kvq_write<T, KVQ_INT4, false>);
             kernel<<<grid, KVQ_THREADS, 0, (cudaStream_t)stream>>>(view, n_rows, (const T*)k, (const T*)v, k_row, k_head,
-                                                                  v_row, v_head, slots, width);
+                                                                  v_row, v_head, slots, shift);
         });
         launched();
     });
@@ -141,12 +141,12 @@ int32_t fb2_kvq_read(const fb2_kvq_cache* c, int32_t n_rows, const int32_t* slot
         need(k && v && slots, "NULL argument");
         need(aligned(k, 16) && aligned(v, 16), "k and v must be 16-byte aligned");
         need(aligned(slots, 4), "slots is not aligned to its element size");
-        const int width = row_lanes(view.hd);
-        const dim3 grid = row_grid(n_rows, view.heads, width);
+        const int shift = row_shift(view.hd);
+        const dim3 grid = row_grid(n_rows, view.heads, shift);
         with_type(dtype, [&](auto t) {
             using T = decltype(t);
             auto kernel = view.row_bytes == view.hd ? k_kvq_read<T, KVQ_INT8> : k_kvq_read<T, KVQ_INT4>;
-            kernel<<<grid, KVQ_THREADS, 0, (cudaStream_t)stream>>>(view, n_rows, slots, (T*)k, (T*)v, width);
+            kernel<<<grid, KVQ_THREADS, 0, (cudaStream_t)stream>>>(view, n_rows, slots, (T*)k, (T*)v, shift);
         });
         launched();
     });
