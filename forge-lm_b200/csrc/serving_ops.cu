@@ -83,10 +83,10 @@ KvqView view_of(const fb2_kvq_cache* c) {
     return v;
 }
 
-// lanes of a row at 16 values each, a power of two
+// log2 of the lanes of a row at 32 values each
 int row_shift(int hd) {
     int s = 0;
-    while ((16 << s) < hd) s++;
+    while ((32 << s) < hd) s++;
     return s;
 }
 dim3 row_grid(int n_rows, int heads, int shift) {
