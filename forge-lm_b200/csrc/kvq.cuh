@@ -4,7 +4,8 @@
 // itself, so a write touches nothing but its own bytes and meta word:
 //   int8: scale = max|x| / 127, code = rint(x * (127 / max|x|)), byte = code + 128;
 //   int4: min = bf16(min x), scale = bf16((max x - min x) / 15),
-//         code = clamp(rint((x - min) * (1 / scale)), 0, 15).
+//         code = clamp(rint((x - min) / scale), 0, 15), the quotient as a product
+//         with the reciprocal: 2^-20 off at most.
 // All in fp32 with IEEE division and rounding to nearest even; the codes use
 // the rounded scale and minimum, so the stored row is the best one for them.
 #pragma once

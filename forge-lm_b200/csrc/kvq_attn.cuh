@@ -129,7 +129,9 @@ FB2_DEV float exp2_fast(float x) {
 // A CTA takes one chunk of one sequence's positions for one K/V
 // head and a block of 8 NT rows (the rows of its tokens and of the query
 // heads that share the K/V head).  Each warp works on its own tiles of 16 MT
-// positions from global memory to registers, with no barrier until the end:
+// positions through its own ring in shared memory (two tiles ahead by cp.async;
+// straight to registers: 472 us for what the ring took to 268), with no barrier
+// until the end:
 //   S^T[position][row] = K codes (A, 16 positions) x q (B, 8 rows),
 //   O^T[dim][row]     += V codes^T (A, 16 dims) x P^T (B, 16 positions x 8 rows),
 // the same column = row layout for both accumulators, so maxima and rescaling
@@ -144,8 +146,15 @@ FB2_DEV float exp2_fast(float x) {
 // its row, in three digits of 8 bits, which is exact to 2^-23 of max|q|.  The
 // codes' offset (128, 8) is taken off where the sums start.
 // Values take fp16 tiles: what a probability adds can be of any size, so P
-// stays in floating point, scaled together with the V scales (one fp16 term for the 16-bit types, two for fp32,
-// whose sums over a tile start at zero and are added to the running ones).
+// stays in floating point, scaled together with the V scales (one fp16 term for
+// the 16-bit types, whose results have no more bits; two for fp32, whose sums
+// over a tile start at zero and are added to the running ones).
+//
+// What bounds it: with many long sequences the instructions that make operands
+// of the codes and probabilities of the scores (16 sequences of 40 to 65 K int4
+// positions, 32 heads on 8 of 128, fp16: 254 us, 3.6 TB/s; 32 sequences of up to
+// 1023 int8 positions, 12 heads of 64, fp32: 14.5 us, 2.0 TB/s); with few the
+// chain from a launch over the page table to the merge (one of 576: 7.4 us).
 template <int HD, int FMT, int NT, bool SPLIT, int WARPS>
 struct KvaShape {
     static constexpr int MT = HD > 128 ? 1 : 2;       // 16-position groups of a tile

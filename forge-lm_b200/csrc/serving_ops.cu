@@ -154,14 +154,31 @@ int32_t fb2_kvq_read(const fb2_kvq_cache* c, int32_t n_rows, const int32_t* slot
 
 // ---- attention ---------------------------------------------------------------
 namespace {
-// Rows to a block, and chunks of positions.
+// Rows to a block, chunks of positions, warps.  Measured (us):
+// - Blocks of 128 rows on tcgen05 tiles where a K/V head has more than 32 rows,
+//   else blocks of 8 or 16 on mma.sync tiles.  4 sequences of 8192 int8
+//   positions, 8 K/V heads, bf16, head_dim 64 and 128: 32 rows 44 and 65 in
+//   blocks of 16, 53 and 70 on tcgen05 tiles; 64 rows 73 and 111, 60 and 80.
+// - Chunks of a size that gives some 888 CTAs (512 of the larger kind): 16
+//   sequences of 40 to 65 K positions take 292 with chunks of 1024, 254 with
+//   4096, 275 with 8192; 4 trees over 9 to 33 K, 263 with 2048, 257 with 4096,
+//   450 with 16384.  Each chunk costs its start and its part of the merge: at
+//   least 512 positions, and at most 64 chunks (one row over 60000 positions:
+//   51, 29, 23, 23 with 256, 512, 1024, 2048).
+// - A cache of up to 1024 positions is one chunk for blocks of 8 rows (12 heads
+//   over 576: 7.4; 8.5 with 512, 8.0 with 256), and cut finer for a few blocks
+//   of 16, which take longer per position (4 blocks over 1000: 19.5 with 256,
+//   25.4 with 512; 128 blocks: 34 and 25).
+// - 8 warps to a block of 8 rows where no SM gets two CTAs (60000 positions:
+//   22.8, 26.5 with 4; 12 heads over 576: 7.4 and 8.7), else 4 (384 CTAs of up
+//   to 1023 positions: 14.6, 22.1 with 8).
 void plan_attention(KvqAttnArgs& k) {
     const int64_t rows = (int64_t)k.max_nodes * k.share;
     const bool tc = k.dtype != FB2_F32 && k.c.hd <= 128 && rows > 32;
     k.block_rows = tc ? KVT_ROWS : rows > 8 ? 16 : 8;
     k.row_blocks = (int)((rows + k.block_rows - 1) / k.block_rows);
     const int64_t units = (int64_t)k.n_seqs * k.c.heads * k.row_blocks;
-    // CTAs for a few waves, counted as if all sequences were of max_len
+    // counted as if all sequences were of max_len
     int64_t chunk = k.max_len * units / (tc ? 512 : 888), least = 512;
     if (!tc) {
         if (k.block_rows == 8 && k.max_len <= 1024) least = 1024;

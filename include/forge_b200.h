@@ -276,7 +276,8 @@ typedef enum { FB2_F32 = 0, FB2_BF16 = 1, FB2_F16 = 2 } fb2_dtype;
  *     byte i, 2i + 1 the high one; meta = bf16 bits scale | minimum << 16;
  *     value = minimum + scale * code.
  *     minimum = bf16(min x), scale = bf16((max x - min x) / 15),
- *     code = round((x - minimum) * (1 / scale)) clamped to 0..15.
+ *     code = round((x - minimum) / scale) clamped to 0..15, the quotient in
+ *     fp32 to within 1e-5.
  * Each K or V row of one head has its own meta word.  A row with a non-finite
  * element (or, for int4, a range or minimum that bf16 cannot hold) is stored
  * as NaN: whoever reads or attends it sees NaN.  A row whose max|x| (int8) or
@@ -323,7 +324,10 @@ int32_t fb2_kvq_read(const fb2_kvq_cache* c, int32_t n_rows, const int32_t* devi
  * A row that sees nothing gives out = 0 and lse = -inf.  Positions whose page
  * id is outside the cache, or that lie past max_pages * page_size or past
  * max_len, are not seen.  Rows past max_nodes of a sequence and rows outside
- * every sequence are not written. */
+ * every sequence are not written.  K and V are exact; for q, fp32 values are
+ * brought to a fixed point of 23 bits below the row's largest, and the
+ * probabilities of 16-bit types are carried in fp16.  Waits inside a kernel are
+ * bounded (about a second); rows of a block whose wait ran out are NaN. */
 typedef struct {
     const void* device_q;  /* [n_rows][n_heads][head_dim], strides below */
     void* device_out;      /* [n_rows][n_heads][head_dim] dense, q's type */
@@ -379,8 +383,10 @@ int32_t fb2_w4_sizes(const fb2_w4_linear* w, int64_t* code_bytes, int64_t* meta_
  * codes and meta are written (the struct's bias is not looked at). */
 int32_t fb2_w4_pack(const fb2_w4_linear* w, const void* device_w, int32_t dtype, int64_t w_row_stride, void* cuda_stream);
 
-/* y[n_rows][out] = x[n_rows][in] W + bias, products exact and sums in fp32,
- * rounded once to dtype.  Rows of x and y are x_row_stride / y_row_stride
+/* y[n_rows][out] = x[n_rows][in] W + bias, sums in fp32, rounded once to dtype.
+ * Products are exact for many rows; for few (up to 32 / 3 rows of a 16-bit type,
+ * 8 of fp32) x is first brought to a fixed point of 23 (31) bits below its
+ * largest |x| in each run of 128 inputs.  Rows of x and y are x_row_stride / y_row_stride
  * elements apart.  A row of x with a non-finite element gives a non-finite
  * row of y.  device_workspace: fb2_w4_matvec_workspace bytes, 16-byte aligned. */
 int32_t fb2_w4_matvec_workspace(const fb2_w4_linear* w, int32_t n_rows, int32_t dtype, int64_t* bytes);
