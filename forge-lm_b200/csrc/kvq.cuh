@@ -4,8 +4,7 @@
 // itself, so a write touches nothing but its own bytes and meta word:
 //   int8: scale = max|x| / 127, code = rint(x * (127 / max|x|)), byte = code + 128;
 //   int4: min = bf16(min x), scale = bf16((max x - min x) / 15),
-//         code = clamp(rint((x - min) / scale), 0, 15), the quotient as a product
-//         with the reciprocal: 2^-20 off at most.
+//         code = clamp(rint((x - min) * (1 / scale)), 0, 15).
 // All in fp32 with IEEE division and rounding to nearest even; the codes use
 // the rounded scale and minimum, so the stored row is the best one for them.
 #pragma once
@@ -147,7 +146,7 @@ FB2_DEV void load8(const T* p, float (&x)[8]) {
 // every load and store of a row is one run of bytes.  32 values per lane: the
 // reductions over the row, the divisions and the addresses are paid once for
 // them.  Memory bounds both kernels where there are rows enough.  32785 rows x 8
-// heads x 128 in bf16 written as int4 and read back (304 MB): 65.6 us, 4.6 TB/s
+// heads x 128 in bf16 written as int4 and read back (304 MB): 67.9 us, 4.5 TB/s
 // (16 values a lane: 75.1), the instructions of the write still showing; 131072
 // rows of int8 read back as bf16 (814 MB): 138 us, 5.9 TB/s.  Few rows take as
 // long as a launch and a chain of loads, 4.2 us with the read back (16 values: 3.9).
@@ -260,13 +259,14 @@ __global__ void __launch_bounds__(KVQ_THREADS)
 #pragma unroll
         for (int j = 0; j < NP; j++) {
             if (!mine[j]) continue;
-            // |x inv| <= 127 (1 + 2^-23): it rounds to 127 at most; NaN rows hold code 0
+            // |x inv| <= 127 (1 + 2^-23): it rounds to 127 at most; NaN rows hold code 0.
+            // The product is rounded by itself, as the formula says.
             uint32_t w[2];
 #pragma unroll
             for (int i = 0; i < N; i += 4) {
                 uint32_t q[4];
 #pragma unroll
-                for (int l = 0; l < 4; l++) q[l] = __float_as_uint(x[j][i + l] * inv + (kRint + 128.0f));
+                for (int l = 0; l < 4; l++) q[l] = __float_as_uint(__fmul_rn(x[j][i + l], inv) + (kRint + 128.0f));
                 const uint32_t four = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
                 w[i / 4] = finite ? four : 0x80808080u;
             }
@@ -289,16 +289,20 @@ __global__ void __launch_bounds__(KVQ_THREADS)
         const float least = bf16_bits_to_float(least_b), scale = bf16_bits_to_float(scale_b);
         const bool finite = scale < inf && fabsf(least) < inf;  // false for NaN
         const bool some = finite && scale >= kKvqTiny;
-        const float inv = some ? 1.0f / scale * (1.0f / 15.0f) : 0.0f;
+        const float inv = some ? 1.0f / scale : 0.0f;
+        // The minimum and scale are rounded, so that a code may lie outside 0..15,
+        // but hardly ever does: the row's ends show it (rounding is monotonic).
+        const bool inside = finite && (lo - least) * inv >= -0.5f && (hi - least) * inv < 15.5f;
+        const bool all_inside = __all_sync(0xffffffffu, inside);
 #pragma unroll
         for (int j = 0; j < NP; j++) {
             if (!mine[j]) continue;
             uint32_t w = 0;  // the sum of the shifted bits less that of kRint's
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                // in 0..1 (NaN, and inf 0: 0): the minimum and scale are rounded, a value may lie outside
-                const float f = __saturatef((x[j][i] - least) * inv);
-                w += __float_as_uint(fmaf(f, 15.0f, kRint)) << (4 * i);
+                float f = __fmul_rn(x[j][i] - least, inv);  // rounded as the formula says: not one step with the sum
+                if (!all_inside) f = fminf(fmaxf(f, 0.0f), 15.0f);  // NaN (inf 0): 0
+                w += __float_as_uint(f + kRint) << (4 * i);
             }
             w -= N == 8 ? kRintBits * 0x11111111u : kRintBits * 0x1111u;
             kvq_store_codes<FMT, N>(to, part + width * j, &w);

@@ -276,8 +276,8 @@ typedef enum { FB2_F32 = 0, FB2_BF16 = 1, FB2_F16 = 2 } fb2_dtype;
  *     byte i, 2i + 1 the high one; meta = bf16 bits scale | minimum << 16;
  *     value = minimum + scale * code.
  *     minimum = bf16(min x), scale = bf16((max x - min x) / 15),
- *     code = round((x - minimum) / scale) clamped to 0..15, the quotient in
- *     fp32 to within 1e-5.
+ *     code = round((x - minimum) * (1 / scale)) clamped to 0..15, each step of
+ *     it rounded to fp32 (values of 16-bit types often lie halfway).
  * Each K or V row of one head has its own meta word.  A row with a non-finite
  * element (or, for int4, a range or minimum that bf16 cannot hold) is stored
  * as NaN: whoever reads or attends it sees NaN.  A row whose max|x| (int8) or

@@ -107,6 +107,33 @@ def test_write_stores_the_rows_and_nothing_else(pkg, fmt, dtype, rows, heads, di
 @gpu
 @pytest.mark.parametrize("fmt", ["int8", "int4"])
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("dim", [64, 128, 208])
+def test_written_codes_are_those_of_the_formula_in_fp32(pkg, fmt, dtype, dim):
+    """Bit for bit, where values lie halfway between two codes too: multiples of
+    a power of two, as values of 16-bit types are."""
+    g = gen(dim)
+    rows = 64
+    x = normal(g, rows, 2, dim)
+    x[::2] = torch.round(x[::2] * 8) / 8
+    x[1::4] += 300  # a minimum that is rounded by more than a code
+    x = x.to(DTYPES[dtype])
+    cache = pkg.QuantKvCache.empty(4, 16, 2, dim, fmt)
+    cache.write(x, x, torch.arange(rows, dtype=torch.int32, device="cuda"))
+    f = x.float().cpu()
+    codes = cache.codes.permute(2, 0, 3, 1, 4).flatten(1, 2).cpu()
+    if fmt == "int8":
+        want = torch.round(f * torch.div(torch.tensor(127.0), f.abs().amax(-1, keepdim=True))) + 128  # number / tensor is two roundings
+    else:
+        low, high = f.amin(-1, keepdim=True), f.amax(-1, keepdim=True)
+        scale, least = ((high - low) / 15).bfloat16().float(), low.bfloat16().float()
+        want = torch.round((f - least) * (1 / scale)).clamp(0, 15)
+        codes = torch.stack([codes & 15, codes >> 4], -1).flatten(-2)
+    assert torch.equal(codes[0].float(), want) and torch.equal(codes[1].float(), want)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("rows,heads,dim,page", [(1, 1, 16, 8), (5, 12, 64, 16), (131, 5, 80, 32), (40, 8, 128, 64),
                                                   (17, 2, 256, 1024)])
 def test_read_gives_the_stored_values(pkg, fmt, dtype, rows, heads, dim, page):
