@@ -324,6 +324,7 @@ template <class T>
 __global__ void __launch_bounds__(128)
     k_w4_columns(const T* __restrict__ x, long long x_row, int rows, int per, int K, int units, int tiles, int chunks,
                  int group_shift, uint4* __restrict__ to, float* __restrict__ sums, int vec) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the product fetches its first codes meanwhile
     const long long at = ((long long)blockIdx.x * 128 + threadIdx.x) >> 5;  // (chunk, unit, tile)
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     if (at >= (long long)chunks * units * tiles) return;
@@ -464,6 +465,7 @@ template <class T>
 __global__ void __launch_bounds__(128)
     k_w4_digits(const T* __restrict__ x, long long x_row, int rows, int K, int units, int tiles, int group_shift,
                 unsigned char* __restrict__ to, int vec) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the product fetches its first codes meanwhile
     const long long at = ((long long)blockIdx.x * 128 + threadIdx.x) >> 5;
     if (at >= (long long)units * tiles) return;
     constexpr int D = sizeof(T) == 4 ? 4 : 3;
