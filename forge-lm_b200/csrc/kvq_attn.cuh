@@ -203,6 +203,7 @@ __global__ void __launch_bounds__(WARPS * 32, KvaShape<HD, FMT, NT, SPLIT, WARPS
     const int b = blockIdx.y;
     const int rb = blockIdx.x % a.row_blocks, rest = blockIdx.x / a.row_blocks;
     const int split = rest % a.splits, head = rest / a.splits;
+    if (a.splits > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge's launch
     int first, count;
     a.rows_of(b, first, count);
     const int row0 = rb * S::ROWS, n_rows = min(S::ROWS, count * a.share - row0);
@@ -264,13 +265,15 @@ __global__ void __launch_bounds__(WARPS * 32, KvaShape<HD, FMT, NT, SPLIT, WARPS
 #pragma unroll
                 for (int i = 0; i < COPIES; i++) copy16(to + copy_to[i] + j * S::GROUP, copy_from[i] + skip, there);
             } else {
-                // rows shorter than in shared memory: 8 bytes at a time
-                const int per = rbytes / 8;
-                for (int i = lane; i < 16 * per; i += 32) {
-                    const int row = i / per, at = i - row * per, kind = row >> 3;
-                    const uint32_t byte = (row & 7) * S::RB + at * 8;
-                    copy8(to + j * S::GROUP + kind * (8 * S::RB) + S::place(byte >> 4) * 16 + (byte & 8),
-                          a.c.codes + skip + kind * (ps * rbytes) + (row & 7) * rbytes + at * 8, there);
+                // rows shorter than in shared memory: two lanes to a row
+                const int row = lane >> 1, kind = row >> 3, r = row & 7;
+                const unsigned char* from = a.c.codes + skip + kind * (ps * rbytes) + r * rbytes;
+                const uint32_t base = to + j * S::GROUP + kind * (8 * S::RB);
+                if ((rbytes & 15) == 0) {
+                    for (int u = lane & 1; u < rbytes / 16; u += 2) copy16(base + S::place(r * (S::RB / 16) + u) * 16, from + u * 16, there);
+                } else {
+                    for (int u = lane & 1; u < rbytes / 8; u += 2)
+                        copy8(base + S::place(r * (S::RB / 16) + (u >> 1)) * 16 + (u & 1) * 8, from + u * 8, there);
                 }
             }
         }

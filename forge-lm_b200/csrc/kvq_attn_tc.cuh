@@ -155,6 +155,7 @@ __global__ void __launch_bounds__(KVT_LAUNCH, 1) k_kvq_attend_tc(KvqAttnArgs a) 
     const int b = blockIdx.y;
     const int rb = blockIdx.x % a.row_blocks, rest = blockIdx.x / a.row_blocks;
     const int split = rest % a.splits, head = rest / a.splits;
+    if (a.splits > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge's launch
     int first, count;
     a.rows_of(b, first, count);
     const int row0 = rb * KVT_ROWS, n_rows = min(KVT_ROWS, count * a.share - row0);
