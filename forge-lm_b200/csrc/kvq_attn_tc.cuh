@@ -9,7 +9,7 @@
 // 3.2 us a tile of 128 positions, of which the 16384 exponentials take 1.1 at
 // their pipe's rate and the rest is the four steps below, one after another.
 // 4 trees of 23 to 64 tokens over 9 to 33 K int8 positions, 32 heads on 8 of
-// 128, bf16: 257 us, 195 TFLOP/s (450 on mma.sync tiles).
+// 128, bf16: 255 us, 197 TFLOP/s (450 on mma.sync tiles).
 //
 // 512 threads of a CTA take one chunk of a sequence's positions, one K/V head
 // and 128 rows; row r is TMEM lane r; warps w, w + 4, w + 8, w + 12 read lane

@@ -432,8 +432,8 @@ W4Workspace w4_workspace(const W4View& v, const W4Shape& s) {
 }
 // x in fixed point is made by the product itself where each warp has one or
 // two units of inputs, else by a launch before it (768 x 2304 fp32: 3.3 and 4.1
-// us; 1024 x 4096 bf16: 3.7 and 5.0; 4096 x 4096 fp16: 9.3 and 6.8; 16384 x
-// 16384 bf16: 44 and 32)
+// us; 1024 x 4096 bf16: 3.7 and 5.0; 4096 x 4096 fp16: 9.3 and 5.8; 16384 x
+// 16384 bf16: 44 and 29)
 bool w4_direct(const W4View& v, int rows, int dtype) { return rows * w4_digits_of(dtype) <= 8 && v.k64 <= 32; }
 
 template <class K, class... A>
