@@ -152,9 +152,9 @@ FB2_DEV float exp2_fast(float x) {
 //
 // What bounds it: with many long sequences the instructions that make operands
 // of the codes and probabilities of the scores (16 sequences of 40 to 65 K int4
-// positions, 32 heads on 8 of 128, fp16: 254 us, 3.6 TB/s; 32 sequences of up to
-// 1023 int8 positions, 12 heads of 64, fp32: 14.5 us, 2.0 TB/s); with few the
-// chain from a launch over the page table to the merge (one of 576: 7.4 us).
+// positions, 32 heads on 8 of 128, fp16: 256 us, 3.6 TB/s; 32 sequences of up to
+// 1023 int8 positions, 12 heads of 64, fp32: 14.7 us, 1.9 TB/s); with few the
+// chain from a launch over the page table to the merge (one of 576: 7.3 us).
 template <int HD, int FMT, int NT, bool SPLIT, int WARPS>
 struct KvaShape {
     static constexpr int MT = HD > 128 ? 1 : 2;       // 16-position groups of a tile
@@ -203,7 +203,6 @@ __global__ void __launch_bounds__(WARPS * 32, KvaShape<HD, FMT, NT, SPLIT, WARPS
     const int b = blockIdx.y;
     const int rb = blockIdx.x % a.row_blocks, rest = blockIdx.x / a.row_blocks;
     const int split = rest % a.splits, head = rest / a.splits;
-    if (a.splits > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge's launch
     int first, count;
     a.rows_of(b, first, count);
     const int row0 = rb * S::ROWS, n_rows = min(S::ROWS, count * a.share - row0);
@@ -270,8 +269,10 @@ __global__ void __launch_bounds__(WARPS * 32, KvaShape<HD, FMT, NT, SPLIT, WARPS
                 const unsigned char* from = a.c.codes + skip + kind * (ps * rbytes) + r * rbytes;
                 const uint32_t base = to + j * S::GROUP + kind * (8 * S::RB);
                 if ((rbytes & 15) == 0) {
+#pragma unroll 1
                     for (int u = lane & 1; u < rbytes / 16; u += 2) copy16(base + S::place(r * (S::RB / 16) + u) * 16, from + u * 16, there);
                 } else {
+#pragma unroll 1
                     for (int u = lane & 1; u < rbytes / 8; u += 2)
                         copy8(base + S::place(r * (S::RB / 16) + (u >> 1)) * 16 + (u & 1) * 8, from + u * 8, there);
                 }
