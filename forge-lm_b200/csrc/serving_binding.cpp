@@ -260,7 +260,7 @@ PyObject* cache_attend(PyObject*, PyObject* const* args, Py_ssize_t count) {
         a.max_pages = small(pages, "pages");
         a.q_row_stride = q.stride(0);
         a.q_head_stride = q.stride(1);
-        a.table_stride = std::max<int64_t>(table.stride(0), pages);
+        a.table_stride = seqs > 1 ? table.stride(0) : pages;  // one row may have any stride
         a.device_q = q.data_ptr();
         a.device_page_table = data<int32_t>(&table);
         a.device_prefix_lens = data<int32_t>(prefix);

@@ -207,7 +207,7 @@ KvqAttnArgs attn_args(const fb2_kvq_cache* c, const fb2_kvq_attention* a) {
          "without row_starts there is one row per sequence and max_nodes is 1");
     need(std::isfinite(a->scale), "scale must be finite");
     need(!a->device_mask || (int64_t)a->mask_words * 32 >= a->max_nodes, "mask_words must cover max_nodes");
-    need(a->table_stride >= a->max_pages, "table_stride must be at least max_pages");
+    need(a->table_stride == 0 || a->table_stride >= a->max_pages, "table_stride must be 0 or at least max_pages");
     const int64_t cap = (int64_t)a->max_pages * c->page_size;
     need(cap <= INT32_MAX, "max_pages * page_size must be at most 2^31 - 1");
     // groups of 8 rows are counted in 32 bits (a cache of that size has over 270 GB)

@@ -96,7 +96,8 @@ class QuantKvCache:
 
         Sequence b's rows are q[starts[b]:starts[b+1]] (starts None: one row
         per sequence); its row i is the token at position prefix_lens[b] + i,
-        already written to the cache, whose pages page_table[b] lists.  A row
+        already written to the cache, whose pages page_table[b] lists (an
+        expanded table gives all sequences the same pages).  A row
         sees every position before prefix_lens[b] and, of its sequence's own
         rows, those whose bit its mask words [rows, words] int32 set (mask
         None: itself and the earlier ones).  scale defaults to

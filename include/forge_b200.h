@@ -332,7 +332,7 @@ typedef struct {
     const void* device_q;  /* [n_rows][n_heads][head_dim], strides below */
     void* device_out;      /* [n_rows][n_heads][head_dim] dense, q's type */
     float* device_lse;     /* [n_rows][n_heads], or NULL */
-    const int32_t* device_page_table;  /* [n_seqs][max_pages], rows table_stride apart */
+    const int32_t* device_page_table;  /* [n_seqs][max_pages], rows table_stride apart (0: all sequences share one row) */
     const int32_t* device_prefix_lens; /* [n_seqs] */
     const int32_t* device_row_starts;  /* [n_seqs + 1], or NULL: one row per sequence */
     const uint32_t* device_mask;       /* [n_rows][mask_words], or NULL */

@@ -443,6 +443,42 @@ def test_attention_of_strided_queries_on_another_stream(pkg):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("nodes", [1, 12])
+def test_attention_of_sequences_that_share_a_page_table(pkg, dtype, nodes):
+    """A table expanded over the sequences, or with rows apart: the values of a dense copy."""
+    g = gen(41)
+    cache = filled(pkg, g, 24, 16, 2, 64, "int8")
+    q = normal(g, 3 * nodes, 8, 64, dtype=DTYPES[dtype])
+    prefix, starts = _i32([150, 0, 77]), _i32([0, nodes, 2 * nodes, 3 * nodes])
+    row = torch.randperm(24, generator=torch.Generator().manual_seed(4))[:11].to(torch.int32).cuda()
+    wide = torch.randint(0, 24, (3, 20), device="cuda", generator=g).to(torch.int32)
+    for table in (row[None].expand(3, 11), row[:1, None].expand(3, 1), wide[:, 3:14]):
+        want = cache.attend(q, table.contiguous(), prefix, starts=starts, max_nodes=nodes)
+        got = cache.attend(q, table, prefix, starts=starts, max_nodes=nodes)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    # one sequence's row may have any stride; rows that overlap in part are refused
+    one = cache.attend(q[:nodes], row.as_strided((1, 11), (3, 1)), prefix[:1], starts=starts[:2], max_nodes=nodes)
+    want = cache.attend(q[:nodes], row[None].contiguous(), prefix[:1], starts=starts[:2], max_nodes=nodes)
+    assert torch.equal(one[0], want[0])
+    with pytest.raises(pkg.ArgumentError):
+        cache.attend(q, row.as_strided((3, 7), (2, 1)), prefix, starts=starts, max_nodes=nodes)
+
+
+def test_stride_of_a_shared_page_table(pkg):
+    """The C entry takes a row stride of 0 as it is and refuses rows that overlap in part."""
+    import ctypes as C
+    import struct
+    from forge_lm_b200 import _native as N
+    L, size = N.load(), C.c_int64()
+    cache = struct.Struct("=QQ6i").pack(4096, 4096, 10, 16, 3, 64, 0, 0)
+    for stride, status in ((0, N.FB2_OK), (4, N.FB2_OK), (9, N.FB2_OK), (1, N.FB2_INVALID_ARG), (3, N.FB2_INVALID_ARG),
+                           (-4, N.FB2_INVALID_ARG)):
+        a = struct.Struct("=8Q4q8ifi").pack(*[4096] * 5, 0, 0, 0, 0, 64, 64, stride, 2, 2, 6, 0, 4, 1, 0, 0, 0.125, 0)
+        assert L.fb2_kvq_attend_workspace(cache, a, C.byref(size)) == status, stride
+
+
+@gpu
 def test_attention_bounds_that_cut(pkg):
     """max_len and the page table's width cut what is seen; max_nodes which rows are written."""
     attention_case(pkg, 31, "int8", "fp32", [100, 40], [1, 1], 4, 2, 64, 16, tree=False, max_len=77)
