@@ -325,7 +325,8 @@ PyObject* linear_pack(PyObject*, PyObject* const* args, Py_ssize_t count) {
              "w must be a CUDA tensor [in, out] with contiguous rows");
         const int32_t code = code_of(w.scalar_type());
         OnDevice on(h.index);
-        status(fb2_w4_pack(&h.w, w.data_ptr(), code, std::max<int64_t>(w.stride(0), w.size(1)), on.stream()));
+        const int64_t row = w.size(0) > 1 ? w.stride(0) : w.size(1);  // one row may have any stride
+        status(fb2_w4_pack(&h.w, w.data_ptr(), code, row, on.stream()));
         Py_RETURN_NONE;
     });
 }

@@ -367,7 +367,7 @@ int32_t fb2_w4_pack(const fb2_w4_linear* w, const void* dense, int32_t dtype, in
         check_dtype(dtype);
         need(dense, "w is NULL");
         need(aligned(dense, size_of(dtype)), "w is not aligned to its element size");
-        need(w_row >= v.N, "w_row_stride must be at least out_features");
+        need(w_row == 0 || w_row >= v.N, "w_row_stride must be 0 or at least out_features");
         const int64_t units = (int64_t)((v.N + 15) / 16) * v.groups * 8;
         need((units + 127) / 128 <= INT32_MAX, "the layer is too large for one call");
         with_type(dtype, [&](auto t) {

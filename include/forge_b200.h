@@ -376,7 +376,8 @@ typedef struct {
 } fb2_w4_linear;
 int32_t fb2_w4_sizes(const fb2_w4_linear* w, int64_t* code_bytes, int64_t* meta_bytes);
 
-/* Packs W [in][out] (dtype; row stride w_row_stride elements): per group
+/* Packs W [in][out] (dtype; row stride w_row_stride elements, 0: every input
+ * has the same row): per group
  * minimum = bf16(min w), scale = bf16((max w - min w) / 15),
  * code = round((w - minimum) * (1 / scale)) clamped to 0..15; a scale below
  * 1e-35 gives scale 0 and codes 0, a group with a non-finite weight NaN.

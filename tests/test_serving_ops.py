@@ -567,6 +567,30 @@ def test_pack_of_special_weights(pkg):
     assert y[:, [5, 6]].isnan().all() and torch.isfinite(y[:, [i for i in range(20) if i not in (5, 6)]]).all()
 
 
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_pack_of_broadcast_and_single_rows(pkg, dtype):
+    """W with every row the same (stride 0) or one row of any stride: as its dense copy."""
+    g = gen(43)
+    row = normal(g, 1, 50, dtype=DTYPES[dtype])
+    for w in (row.expand(100, 50), row[0].as_strided((1, 50), (3, 1)), normal(g, 70, 1, dtype=DTYPES[dtype])[:1].expand(70, 1)):
+        got, want = pkg.W4Linear.pack(w, 32), pkg.W4Linear.pack(w.contiguous(), 32)
+        assert torch.equal(got.codes, want.codes) and torch.equal(got.meta, want.meta)
+    with pytest.raises(pkg.ArgumentError):
+        pkg.W4Linear.pack(normal(g, 90, dtype=DTYPES[dtype]).as_strided((20, 50), (2, 1)), 32)
+
+
+def test_stride_of_weights_to_pack(pkg):
+    """The C entry refuses rows that overlap in part."""
+    import struct
+    from forge_lm_b200 import _native as N
+    L = N.load()
+    w = struct.Struct("=QQQ4i").pack(4096, 4096, 0, 100, 33, 32, 0)
+    for stride in (1, 32, -33):
+        assert L.fb2_w4_pack(w, 4096, 0, stride, None) == N.FB2_INVALID_ARG
+        assert b"w_row_stride" in L.fb2_last_error()
+
+
 def random_linear(pkg, g, k, n, group, bias):
     blocks, groups = -(-n // 16), -(-k // group)
     codes = torch.randint(-2 ** 31, 2 ** 31, (blocks, -(-k // 64), 32, 4), device="cuda", generator=g).to(torch.int32)
