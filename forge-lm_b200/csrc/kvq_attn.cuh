@@ -373,11 +373,21 @@ __global__ void __launch_bounds__(WARPS * 32, KvaShape<HD, FMT, NT, SPLIT, WARPS
     __syncthreads();
 
     // ---- the pass over the positions --------------------------------------------
-    float o[S::VD / 2][NT][4], base[NT][2], limit[NT][2], l[NT][2], z[NT][2];
+    // A row's probabilities are exp2(s - base), at most 1: base is kLag above the
+    // largest score at the last time that one exceeded base.  Its weights are
+    // probability * V scale, and unit, a power of two, brings the largest that the
+    // row had so far to 2^2..2^3 at times.  Those times are when base moves and
+    // when V scale * unit, the most that a weight can be, reaches kMost; so fp16
+    // holds every weight, with at least 16 bits below the row's largest, whatever
+    // other rows or masked positions have.  o is in units of 1 / unit.
+    constexpr float kLag = 9.f, kMost = 32768.f, kNone = -3.402823466e38f;  // kNone: nothing seen yet
+    constexpr uint32_t kUnit = 241;  // exponent field of the largest unit
+    float vlim = kMost * __uint_as_float((254u - kUnit) << 23);  // kMost / the lane's largest unit
+    float o[S::VD / 2][NT][4], base[NT][2], unit[NT][2], l[NT][2], z[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) base[n][i] = 0.f, limit[n][i] = -INFINITY, l[n][i] = 0.f, z[n][i] = 0.f;
+        for (int i = 0; i < 2; i++) base[n][i] = kNone, unit[n][i] = __uint_as_float(kUnit << 23), l[n][i] = 0.f, z[n][i] = 0.f;
 #pragma unroll
         for (int i = 0; i < S::VD / 2; i++)
 #pragma unroll
@@ -396,15 +406,6 @@ __global__ void __launch_bounds__(WARPS * 32, KvaShape<HD, FMT, NT, SPLIT, WARPS
             const float4 v = szero[8 * n + 2 * t + i];
             zero[n][i][0] = v.x, zero[n][i][1] = v.y, zero[n][i][2] = v.z;
         }
-    // Probabilities are exp2(s - base), base the largest score at the last time
-    // that one exceeded base + kLag (limit; -inf: nothing seen yet), and
-    // weights are probability * V scale * unit: unit brings the largest scale
-    // to 2^7..2^8 at such a time and may lag behind until kLagV.  Both are below
-    // 65504 then.  vexp: that scale's exponent field (20: small enough for
-    // every scale); o is in units of 2^(vexp - 134).
-    constexpr float kLag = 6.f, kLagV = 900.f;
-    uint32_t vexp = 20;
-    float unit = __uint_as_float((127u + 134u - 20u) << 23);
     const uint32_t q_at = (uint32_t)__cvta_generic_to_shared(sq) + lane * 16;
 
     int slot = 0;
@@ -521,59 +522,58 @@ __global__ void __launch_bounds__(WARPS * 32, KvaShape<HD, FMT, NT, SPLIT, WARPS
         float top[NT][2], vs[GR], vl[GR], vmax = 0.f;
         bool over = false;
 #pragma unroll
+        for (int j = 0; j < GR; j++) {
+            vs[j] = FMT == KVQ_INT8 ? __uint_as_float(vm[j]) : bf16_bits_to_float(vm[j] & 0xffffu);
+            vl[j] = FMT == KVQ_INT8 ? 0.f : centre(vm[j]);
+            vmax = fmaxf(vmax, fabsf(vs[j]));
+        }
+#pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 top[n][c] = fmaxf(s[0][n][c], s[0][n][c + 2]);
                 if constexpr (S::MT == 2) top[n][c] = fmaxf(top[n][c], fmaxf(s[1][n][c], s[1][n][c + 2]));
-                over |= top[n][c] > limit[n][c];
+                over |= top[n][c] > base[n][c];
             }
-#pragma unroll
-        for (int j = 0; j < GR; j++) {
-            vs[j] = (FMT == KVQ_INT8 ? __uint_as_float(vm[j]) : bf16_bits_to_float(vm[j] & 0xffffu)) * unit;
-            vl[j] = FMT == KVQ_INT8 ? 0.f : centre(vm[j]);
-            vmax = fmaxf(vmax, fabsf(vs[j]));
-        }
-        if (__any_sync(0xffffffffu, over || vmax >= kLagV)) {
-            // new references: this tile's largest score and V scale (finite ones)
-            uint32_t vtop = 0;
-#pragma unroll
-            for (int j = 0; j < GR; j++) {
-                const uint32_t bits = (FMT == KVQ_INT8 ? vm[j] : vm[j] << 16) & 0x7fffffffu;
-                if (bits < 0x7f800000u) vtop = max(vtop, bits);
-            }
-            vtop = max(__reduce_max_sync(0xffffffffu, vtop) >> 23, vexp);
-            const float grow = __uint_as_float((127u - min(vtop - vexp, 126u)) << 23);  // old / new unit of o
-            vexp = vtop;
-            const float next = __uint_as_float((127u + 134u - vexp) << 23);
-#pragma unroll
-            for (int j = 0; j < GR; j++)
-                vs[j] = (FMT == KVQ_INT8 ? __uint_as_float(vm[j]) : bf16_bits_to_float(vm[j] & 0xffffu)) * next;
-            unit = next;
+        over |= vmax >= vlim;
+        if (__any_sync(0xffffffffu, over)) {
+            uint32_t high = 0;
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                float alpha[2];
+                float beta[2];
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
 #pragma unroll
                     for (int x = 4; x < 32; x *= 2) top[n][c] = fmaxf(top[n][c], __shfl_xor_sync(0xffffffffu, top[n][c], x));
-                    const bool seen = limit[n][c] != -INFINITY;
-                    const float to = seen ? fmaxf(base[n][c], top[n][c]) : top[n][c];
-                    alpha[c] = seen ? exp2_fast(base[n][c] - to) : 1.f;  // nothing summed yet
-                    if (to != -INFINITY) base[n][c] = to, limit[n][c] = to + kLag;
-                    l[n][c] *= alpha[c];
-                    z[n][c] *= alpha[c];
-                    alpha[c] *= grow;
+                    const bool rise = top[n][c] > base[n][c];
+                    const float to = rise ? top[n][c] + kLag : base[n][c], by = rise ? to - base[n][c] : 0.f;
+                    base[n][c] = to;
+                    l[n][c] *= exp2_fast(-by);
+                    z[n][c] *= exp2_fast(-by);
+                    // unit grows as the old weights shrink, up to what the tile's largest weight allows
+                    float most = 0.f;  // (NaN: not counted)
+#pragma unroll
+                    for (int i = 0; i < S::MT; i++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) most = fmaxf(most, fabsf(exp2_fast(s[i][n][c + 2 * e] - to) * vs[2 * i + e]));
+#pragma unroll
+                    for (int x = 4; x < 32; x *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
+                    const uint32_t field = __float_as_uint(unit[n][c]) >> 23, grow = min((uint32_t)fminf(by, 300.f), kUnit - field);
+                    const uint32_t next = min(field + grow, 256u - (__float_as_uint(most) >> 23));
+                    unit[n][c] = __uint_as_float(next << 23);
+                    high = max(high, next);
+                    beta[c] = exp2_fast((float)(int)(next - field) - by);
                 }
 #pragma unroll
                 for (int i = 0; i < S::VD / 2; i++)
 #pragma unroll
-                    for (int c = 0; c < 4; c++) o[i][n][c] *= alpha[c & 1];
+                    for (int c = 0; c < 4; c++) o[i][n][c] *= beta[c & 1];
             }
+            vlim = kMost * __uint_as_float((254u - high) << 23);
         }
         uint32_t pb[S::MT][NT][S::PARTS][2];
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
+        for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int i = 0; i < S::MT; i++) {
                 float w[4];
@@ -582,7 +582,7 @@ __global__ void __launch_bounds__(WARPS * 32, KvaShape<HD, FMT, NT, SPLIT, WARPS
                     const int j = 2 * i + (c >> 1);
                     const float p = exp2_fast(s[i][n][c] - base[n][c & 1]);
                     l[n][c & 1] += p;
-                    w[c] = p * vs[j];
+                    w[c] = p * (vs[j] * unit[n][c & 1]);
                     s[i][n][c] = p;
                 }
                 if (full) {
@@ -606,7 +606,6 @@ __global__ void __launch_bounds__(WARPS * 32, KvaShape<HD, FMT, NT, SPLIT, WARPS
                     }
                 }
             }
-        }
         uint32_t vr[GR][2][S::VW];
 #pragma unroll
         for (int j = 0; j < GR; j++)
@@ -656,7 +655,6 @@ __global__ void __launch_bounds__(WARPS * 32, KvaShape<HD, FMT, NT, SPLIT, WARPS
     }
 
     // ---- merge the warps ------------------------------------------------------------
-    const float back = __uint_as_float((vexp + 127u - 134u) << 23);  // 2^(vexp - 134)
     copies_wait<0>();
     __syncthreads();  // the rings are done with
 #pragma unroll
@@ -669,7 +667,8 @@ __global__ void __launch_bounds__(WARPS * 32, KvaShape<HD, FMT, NT, SPLIT, WARPS
                 z[n][c] += __shfl_xor_sync(0xffffffffu, z[n][c], x);
             }
             const int r = 8 * n + 2 * t + c;
-            if (g == 0) sml[warp * S::ROWS + r] = make_float2(limit[n][c] == -INFINITY ? -INFINITY : base[n][c], l[n][c]);
+            if (g == 0) sml[warp * S::ROWS + r] = make_float2(base[n][c] == kNone ? -INFINITY : base[n][c], l[n][c]);
+            const float back = __uint_as_float((254u << 23) - __float_as_uint(unit[n][c]));  // 1 / unit
             float* to = so + (warp * S::ROWS + r) * S::O_STRIDE + g * S::VD;
 #pragma unroll
             for (int i = 0; i < S::VD / 2; i++)

@@ -19,12 +19,13 @@
 // operands of 128-byte rows, [64 dims][position], 128-byte swizzled: K-major
 // for S = Q K^T and, with the positions as the contraction, MN-major for O = P V.
 // q is scaled by a power of two to just below 2^13 (exact: the 16-bit types'
-// values fit fp16 then); P carries the V scales and a power of two, with the
+// values fit fp16 then); P carries the V scales and the row's power of two, with the
 // references that lag of kvq_attn.cuh, so that O stays in TMEM and is rescaled
 // only when one of them moves.  Iteration t:
 //   1. wait for S(t); K(t+1) becomes an operand, S(t+1) goes to the other tile;
-//   2. scores, their largest; where it is over a row's limit, rescale;
-//   3. wait for O(t-1); probabilities into P(t), V(t) becomes an operand, O(t).
+//   2. scores, their largest; wait for O(t-1); where a row's references have to
+//      move, the largest weight, and rescale;
+//   3. weights into P(t), V(t) becomes an operand, O(t).
 // One more warp issues the MMAs (which takes as long as the tensor cores need)
 // and looks up the pages of later tiles.
 // Every mbarrier wait is bounded; on expiry the CTA stops, drains its MMAs
@@ -310,7 +311,11 @@ __global__ void __launch_bounds__(KVT_LAUNCH, 1) k_kvq_attend_tc(KvqAttnArgs a) 
                 issue_s(t + 1);
                 put_ids(t + 3, page_of(t + 3));  // of tiles up to t + 2 the others may still read
             }
-            if (__syncthreads_or(0) && s_abort) break;
+            if (__syncthreads_or(0)) {
+                if (s_abort) break;
+                __syncthreads();  // the rows' largest scores are read
+                __syncthreads();  // their largest weights
+            }
             __syncthreads();  // P(t), V(t)
             if (lane == 0) {
                 tc::fence_after();
@@ -415,10 +420,10 @@ __global__ void __launch_bounds__(KVT_LAUNCH, 1) k_kvq_attend_tc(KvqAttnArgs a) 
 
     // ---- the tiles -----------------------------------------------------------------------
     constexpr int OD = HD / KVT_PARTS;  // dims of O that a thread rescales and writes
-    constexpr float kLag = 6.f, kLagV = 900.f;  // as in k_kvq_attend
-    float base = 0.f, limit = -INFINITY, l[4] = {0.f, 0.f, 0.f, 0.f}, z[4] = {0.f, 0.f, 0.f, 0.f};
-    uint32_t vexp = 20;
-    float unit = __uint_as_float((127u + 134u - 20u) << 23);
+    constexpr float kLag = 9.f, kMost = 32768.f, kNone = -3.402823466e38f;  // as in k_kvq_attend
+    constexpr uint32_t kUnit = 241;
+    float base = kNone, l[4] = {0.f, 0.f, 0.f, 0.f}, z[4] = {0.f, 0.f, 0.f, 0.f};
+    float unit = __uint_as_float(kUnit << 23);
     const bool busy = 32 * quarter < n_rows;  // warps whose rows are all past the end only keep step
     const uint32_t o_at = tmem + lanes + S::O_COL + part * OD;
     bool ok = true;
@@ -444,7 +449,7 @@ __global__ void __launch_bounds__(KVT_LAUNCH, 1) k_kvq_attend_tc(KvqAttnArgs a) 
         if (t + 1 < ntiles) load_meta(t + 2);  // (positions past c1 give 0)
         const bool full = p0 + KVT_KEYS <= min(prefix, c1) && live == 0xffffu;
         const float vtop = __uint_as_float(max(max(s_vtop[t & 1][0], s_vtop[t & 1][1]), max(s_vtop[t & 1][2], s_vtop[t & 1][3])));
-        bool over = vtop * unit >= kLagV;
+        bool over = false;
         // the row's scores of columns c .. c + 15 of its part (without f); they
         // are read twice, as registers are short
         auto scores = [&](int c, float (&s)[16]) {
@@ -500,32 +505,47 @@ __global__ void __launch_bounds__(KVT_LAUNCH, 1) k_kvq_attend_tc(KvqAttnArgs a) 
                 largest(std::false_type{});
             const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
             s_red[part][r] = most;
-            over |= most * f > limit;
+            over = most * f > base || vtop * unit >= kMost;
         }
         if (t > 0) ok = tc::bar_wait(&bar_o, (uint32_t)((t - 1) & 1), &s_abort);  // P, V and O are free
         if (__syncthreads_or(over || !ok)) {
             if (s_abort) break;
             tc::fence_after();
-            const uint32_t to_exp = max(__float_as_uint(vtop) >> 23, vexp);
-            const float grow = __uint_as_float((127u - min(to_exp - vexp, 126u)) << 23);  // old / new unit of o
-            vexp = to_exp;
-            unit = __uint_as_float((127u + 134u - vexp) << 23);
+            // f > 0: the largest product is the largest score
+            const float top = fmaxf(fmaxf(s_red[0][r], s_red[1][r]), fmaxf(s_red[2][r], s_red[3][r])) * f;
+            __syncthreads();
+            const bool rise = top > base;
+            const float to = rise ? top + kLag : base, by = rise ? to - base : 0.f;
+            base = to;
             if (busy) {
-                // f > 0: the largest product is the largest score
-                const float top = fmaxf(fmaxf(s_red[0][r], s_red[1][r]), fmaxf(s_red[2][r], s_red[3][r])) * f;
-                const bool seen = limit != -INFINITY;
-                const float to = seen ? fmaxf(base, top) : top;
-                float alpha = seen ? kva::exp2_fast(base - to) : 1.f;  // nothing summed yet
-                if (to > -INFINITY) base = to, limit = to + kLag;
+                float most = 0.f;  // (NaN: not counted)
 #pragma unroll
-                for (int i = 0; i < 4; i++) l[i] *= alpha, z[i] *= alpha;
+                for (int c = 0; c < KVT_COLS; c += 16) {
+                    float s[16];
+                    scores(c, s);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        const float w = fabsf(kva::exp2_fast(fmaf(s[j], f, -base)) * s_v[t & 1][0][KVT_COLS * part + c + j]);
+                        most = fmaxf(most, (see >> (c + j)) & 1 ? w : 0.f);
+                    }
+                }
+                s_red[part][r] = most;
+            }
+            __syncthreads();
+            if (busy) {
+                const float most = fmaxf(fmaxf(s_red[0][r], s_red[1][r]), fmaxf(s_red[2][r], s_red[3][r]));
+                const uint32_t field = __float_as_uint(unit) >> 23, grow = min((uint32_t)fminf(by, 300.f), kUnit - field);
+                const uint32_t next = min(field + grow, 256u - (__float_as_uint(most) >> 23));
+                unit = __uint_as_float(next << 23);
+#pragma unroll
+                for (int i = 0; i < 4; i++) l[i] *= kva::exp2_fast(-by), z[i] *= kva::exp2_fast(-by);
                 if (t > 0) {
+                    const float beta = kva::exp2_fast((float)(int)(next - field) - by);
                     float v[OD];
                     kvt::ld(o_at, v);
                     kvt::wait_ld();
-                    alpha *= grow;
 #pragma unroll
-                    for (int i = 0; i < OD; i++) v[i] *= alpha;
+                    for (int i = 0; i < OD; i++) v[i] *= beta;
                     kvt::st(o_at, v);
                     kvt::wait_st();
                 }
@@ -594,7 +614,7 @@ __global__ void __launch_bounds__(KVT_LAUNCH, 1) k_kvq_attend_tc(KvqAttnArgs a) 
         }
     }
     copies_wait<0>();
-    const float back = __uint_as_float((vexp + 127u - 134u) << 23);
+    const float back = __uint_as_float((254u << 23) - __float_as_uint(unit));  // 1 / unit
     const bool gave_up = s_abort;
     s_sum[0][part][r] = (l[0] + l[1]) + (l[2] + l[3]);
     s_sum[1][part][r] = (z[0] + z[1]) + (z[2] + z[3]);
@@ -605,7 +625,7 @@ __global__ void __launch_bounds__(KVT_LAUNCH, 1) k_kvq_attend_tc(KvqAttnArgs a) 
     if (gave_up) ls = NAN;
     if (mine && part == 0) {
         if (a.splits > 1)
-            a.part_ml[item * a.splits + split] = make_float2(limit == -INFINITY ? -INFINITY : base, ls);
+            a.part_ml[item * a.splits + split] = make_float2(base == kNone ? -INFINITY : base, ls);
         else if (a.lse)
             a.lse[item] = 0.693147180559945309f * ((ls == 0.f ? -INFINITY : base) + log2f(ls));
     }

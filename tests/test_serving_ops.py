@@ -417,6 +417,115 @@ def test_attention_of_large_and_small_values(pkg, size):
                     float(q.double().norm(dim=2).max().cpu() * k.norm(dim=2).max()) / 8)
 
 
+def plain_of_one_sequence(cache, q, slots, prefix, bits, scale):
+    """fp64 (out, lse) of one sequence's rows by the definition, its positions in
+    `slots`, and for each row and head sum_p softmax_p max|v_p|; bits as for
+    plain_attention."""
+    k, v = (x[slots.long().cpu()].repeat_interleave(q.shape[1] // cache.n_kv_heads, 1) for x in decode(cache))
+    rows, total = q.shape[0], len(slots)
+    sees = torch.zeros((rows, total), dtype=torch.bool)
+    sees[:, :prefix] = True
+    for r in range(rows):
+        sees[r, [prefix + j for j in (range(r + 1) if bits is None else bits[r])]] = True
+    s = torch.einsum("rhd,phd->rhp", q.double().cpu(), k) * scale
+    s[~sees[:, None].expand_as(s)] = -math.inf
+    p = torch.softmax(s, 2)
+    return ((torch.einsum("rhp,phd->rhd", p, v), torch.logsumexp(s, 2)),
+            torch.einsum("rhp,ph->rh", p, v.abs().amax(2)))
+
+
+def check_own_size(fmt, dtype, got, want, own, scores, rows):
+    """As check_attention, for each row by what the row itself weighs: the
+    weights' errors are relative to the row's largest weight, whatever other
+    rows or masked positions hold.  int4 values are summed in two parts (the
+    row's middle and codes - 8), each up to about as large as the values."""
+    tol = 8 * 2.0 ** -23 * (scores + 4) + 2.0 ** -20
+    if dtype != "fp32":
+        tol += 2.0 ** -11
+    tol *= 2 if fmt == "int4" else 1
+    out, lse = got
+    assert torch.isfinite(out[rows]).all()
+    assert within(out[rows], want[0][rows], tol * own[rows][:, :, None]), \
+        float(((out.double().cpu() - want[0]).abs() / own[:, :, None])[rows].max())
+    assert float((lse.double().cpu() - want[1])[rows].abs().max()) <= 8 * 2.0 ** -23 * (scores + 16)
+
+
+def large_value_case(pkg, fmt, dtype, nodes, dim, big, far, late):
+    """One V row 2^big times the others: a drafted node that some rows do not
+    see (far 0), or a cached position that all see with a score about `far`
+    below the others (at the end or the start of the prefix)."""
+    g = gen(51)
+    prefix, heads = 300, 4
+    cache = pkg.QuantKvCache.empty(24, 16, 2, dim, fmt)
+    order = torch.randperm(24, generator=torch.Generator().manual_seed(6)).to(torch.int32)
+    total = prefix + nodes
+    k, v = normal(g, total, 2, dim), normal(g, total, 2, dim)
+    q = (2 * normal(g, nodes, heads, dim)).to(DTYPES[dtype])
+    scale = 1 / math.sqrt(dim)
+    k[:, :, 0] = 0
+    q[:, :, 0] = 8
+    which = prefix + 1 if not far else prefix - 3 if late else 2
+    if far:
+        k[which, :, 0] = -far / 8 / scale
+    v[which] *= 2.0 ** big
+    slots = torch.tensor([int(order[p // 16]) * 16 + p % 16 for p in range(total)], dtype=torch.int32, device="cuda")
+    cache.write(k, v, slots)
+    bits = [{0, i} | ({1} if i % 2 else set()) for i in range(nodes)]
+    words = (nodes + 31) // 32
+    flat = [[sum(1 << (j - 32 * w) for j in s if 32 * w <= j < 32 * w + 32) for w in range(words)] for s in bits]
+    mask = torch.tensor(flat, dtype=torch.int64).to(torch.int32).cuda()
+    got = cache.attend(q, order[None].cuda(), _i32([prefix]), starts=_i32([0, nodes]), mask=mask, max_nodes=nodes)
+    want, own = plain_of_one_sequence(cache, q, slots, prefix, bits, scale)
+    ks, _ = decode(cache)
+    scores = float(q.double().cpu().norm(dim=2).max() * ks.norm(dim=2).max() * scale)
+    # what fp16 cannot hold is no result to compare
+    rows = torch.tensor([i for i in range(nodes) if far or i % 2 == 0 or dtype != "fp16"])
+    check_own_size(fmt, dtype, got, want, own, scores, rows)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("nodes,dim", [(4, 64), (40, 64), (34, 128), (8, 256)])
+@pytest.mark.parametrize("big", [20, 40, 100])
+def test_attention_beside_large_masked_values(pkg, fmt, dtype, nodes, dim, big):
+    """What a row does not see does not cost it bits, however large."""
+    large_value_case(pkg, fmt, dtype, nodes, dim, big, 0, False)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("nodes,dim", [(4, 64), (40, 64), (34, 128), (8, 256)])
+@pytest.mark.parametrize("late", [False, True])
+def test_attention_with_large_values_of_no_weight(pkg, fmt, dtype, nodes, dim, late):
+    """Nor does what it sees with a score 100 below its others, first or last."""
+    large_value_case(pkg, fmt, dtype, nodes, dim, 60, 100, late)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("nodes", [2, 40])
+@pytest.mark.parametrize("step", [12, -12])
+def test_attention_over_values_that_grow(pkg, fmt, dtype, nodes, step):
+    """V rows 2^12 larger (or smaller) every 128 positions, all of them seen."""
+    g = gen(52)
+    prefix, dim = 900, 64
+    total = prefix + nodes
+    cache = pkg.QuantKvCache.empty(60, 16, 2, dim, fmt)
+    order = torch.randperm(60, generator=torch.Generator().manual_seed(7)).to(torch.int32)
+    v = normal(g, total, 2, dim) * 2.0 ** (step * (torch.arange(total, device="cuda") // 128).float())[:, None, None]
+    slots = torch.tensor([int(order[p // 16]) * 16 + p % 16 for p in range(total)], dtype=torch.int32, device="cuda")
+    cache.write(normal(g, total, 2, dim), v, slots)
+    q = (2 * normal(g, nodes, 4, dim)).to(DTYPES[dtype])
+    got = cache.attend(q, order[None].cuda(), _i32([prefix]), starts=_i32([0, nodes]), max_nodes=nodes)
+    want, own = plain_of_one_sequence(cache, q, slots, prefix, None, 0.125)
+    ks, _ = decode(cache)
+    scores = float(q.double().cpu().norm(dim=2).max() * ks.norm(dim=2).max() * 0.125)
+    check_own_size(fmt, dtype, got, want, own, scores, torch.arange(nodes))
+
+
 @gpu
 def test_attention_of_strided_queries_on_another_stream(pkg):
     g = gen(6)
