@@ -152,8 +152,8 @@ FB2_DEV float exp2_fast(float x) {
 //
 // What bounds it: with many long sequences the instructions that make operands
 // of the codes and probabilities of the scores (16 sequences of 40 to 65 K int4
-// positions, 32 heads on 8 of 128, fp16: 256 us, 3.6 TB/s; 32 sequences of up to
-// 1023 int8 positions, 12 heads of 64, fp32: 14.7 us, 1.9 TB/s); with few the
+// positions, 32 heads on 8 of 128, fp16: 257 us, 3.6 TB/s; 32 sequences of up to
+// 1023 int8 positions, 12 heads of 64, fp32: 15.0 us, 1.9 TB/s); with few the
 // chain from a launch over the page table to the merge (one of 576: 7.3 us).
 template <int HD, int FMT, int NT, bool SPLIT, int WARPS>
 struct KvaShape {
@@ -379,7 +379,10 @@ __global__ void __launch_bounds__(WARPS * 32, KvaShape<HD, FMT, NT, SPLIT, WARPS
     // row had so far to 2^2..2^3 at times.  Those times are when base moves and
     // when V scale * unit, the most that a weight can be, reaches kMost; so fp16
     // holds every weight, with at least 16 bits below the row's largest, whatever
-    // other rows or masked positions have.  o is in units of 1 / unit.
+    // other rows or masked positions have.  (One unit for all rows, by the tile's
+    // largest V scale: 255.9 us for 257.4 on the long sequences, 66.7 for 69.0 over 32
+    // of 1000 to 9000, 12 heads of 64 in bf16; but a V row 2^20 times the others,
+    // seen or not, left the others' weights 4 bits.)  o is in units of 1 / unit.
     constexpr float kLag = 9.f, kMost = 32768.f, kNone = -3.402823466e38f;  // kNone: nothing seen yet
     constexpr uint32_t kUnit = 241;  // exponent field of the largest unit
     float vlim = kMost * __uint_as_float((254u - kUnit) << 23);  // kMost / the lane's largest unit

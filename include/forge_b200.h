@@ -325,8 +325,9 @@ int32_t fb2_kvq_read(const fb2_kvq_cache* c, int32_t n_rows, const int32_t* devi
  * id is outside the cache, or that lie past max_pages * page_size or past
  * max_len, are not seen.  Rows past max_nodes of a sequence and rows outside
  * every sequence are not written.  K and V are exact; for q, fp32 values are
- * brought to a fixed point of 23 bits below the row's largest, and the
- * probabilities of 16-bit types are carried in fp16.  Waits inside a kernel are
+ * brought to a fixed point of 23 bits below the row's largest, and what a row
+ * weighs V with is carried in fp16 (for fp32 in two such terms) relative to the
+ * row's own largest weight.  Waits inside a kernel are
  * bounded (about a second); rows of a block whose wait ran out are NaN. */
 typedef struct {
     const void* device_q;  /* [n_rows][n_heads][head_dim], strides below */
