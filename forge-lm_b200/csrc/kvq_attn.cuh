@@ -580,24 +580,19 @@ __global__ void __launch_bounds__(WARPS * 32, KvaShape<HD, FMT, NT, SPLIT, WARPS
 #pragma unroll
             for (int i = 0; i < S::MT; i++) {
                 float w[4];
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
+                auto weigh = [&](int c, bool none) {
                     const int j = 2 * i + (c >> 1);
                     const float p = exp2_fast(s[i][n][c] - base[n][c & 1]);
                     l[n][c & 1] += p;
-                    w[c] = p * (vs[j] * unit[n][c & 1]);
-                    s[i][n][c] = p;
-                }
+                    if (FMT == KVQ_INT4 && !none) z[n][c & 1] = fmaf(p, vl[j], z[n][c & 1]);
+                    w[c] = none ? 0.f : p * (vs[j] * unit[n][c & 1]);
+                };
                 if (full) {
-                    if constexpr (FMT == KVQ_INT4)
 #pragma unroll
-                        for (int c = 0; c < 4; c++) z[n][c & 1] = fmaf(s[i][n][c], vl[2 * i + (c >> 1)], z[n][c & 1]);
+                    for (int c = 0; c < 4; c++) weigh(c, false);
                 } else {  // what a row does not see has weight 0 even where V is NaN
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        if (FMT == KVQ_INT4 && s[i][n][c] != 0.f) z[n][c & 1] = fmaf(s[i][n][c], vl[2 * i + (c >> 1)], z[n][c & 1]);
-                        if (s[i][n][c] == 0.f) w[c] = 0.f;
-                    }
+                    for (int c = 0; c < 4; c++) weigh(c, s[i][n][c] == -INFINITY);
                 }
 #pragma unroll
                 for (int j = 0; j < 2; j++) {

@@ -400,6 +400,28 @@ def test_attention_of_masked_and_seen_nan(pkg):
 
 
 @gpu
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("nodes", [1, 40])
+@pytest.mark.parametrize("at", [3, 70, 300, 303])
+def test_attention_of_seen_nan_with_no_weight(pkg, fmt, dtype, nodes, at):
+    """A NaN V row that a row sees reaches it however small its probability, in a whole
+    tile of positions (3, 70) as in the last one (300, 303)."""
+    g = gen(53)
+    prefix, dim = 304, 64
+    cache = filled(pkg, g, 24, 16, 2, dim, fmt)
+    k, v = torch.zeros((1, 2, dim), device="cuda"), torch.full((1, 2, dim), math.nan, device="cuda")
+    k[..., 0] = -400.0  # a score some 400 below the others
+    v[:, 0] = 1.0       # the first head's row is not NaN
+    cache.write(k, v, _i32([at]))
+    q = normal(g, nodes, 4, dim, dtype=DTYPES[dtype])
+    q[..., 0] = 8
+    out, lse = cache.attend(q, torch.arange(24, dtype=torch.int32, device="cuda")[None], _i32([prefix]),
+                            starts=_i32([0, nodes]), max_nodes=nodes)
+    assert torch.isfinite(out[:, :2]).all() and out[:, 2:].isnan().all() and torch.isfinite(lse).all()
+
+
+@gpu
 @pytest.mark.parametrize("size", [1e-30, 1e-6, 1e4, 1e30])
 def test_attention_of_large_and_small_values(pkg, size):
     g = gen(4)
