@@ -238,17 +238,18 @@ PyObject* cache_attend(PyObject*, PyObject* const* args, Py_ssize_t count) {
         need(prefix && prefix->numel() == seqs, "prefix_lens must have one entry per sequence");
         const at::Tensor* starts = plain(args[4], "starts", at::kInt, h.index);
         const at::Tensor* mask = plain(args[5], "mask", at::kInt, h.index);
-        int64_t nodes = args[7] == Py_None ? -1 : integer(args[7], "max_nodes");
-        if (starts) {
-            need(starts->numel() == seqs + 1, "starts must have one entry more than there are sequences");
-            if (args[7] == Py_None) nodes = std::max<int64_t>(rows, 1);
-        } else {
-            need(args[7] == Py_None || nodes == 1, "starts is needed for more than one row per sequence");
-            nodes = 1;
-        }
         if (mask) {
             need(mask->dim() == 2 && mask->size(0) == rows && mask->size(1) > 0, "mask must be [rows, words]");
             a.mask_words = small(mask->size(1), "mask words");
+        }
+        int64_t nodes = args[7] == Py_None ? -1 : integer(args[7], "max_nodes");
+        if (starts) {
+            need(starts->numel() == seqs + 1, "starts must have one entry more than there are sequences");
+            // a sequence has no more rows than the call, nor than its mask has bits
+            if (args[7] == Py_None) nodes = std::max<int64_t>(mask ? std::min(rows, 32 * mask->size(1)) : rows, 1);
+        } else {
+            need(args[7] == Py_None || nodes == 1, "starts is needed for more than one row per sequence");
+            nodes = 1;
         }
         a.scale = args[6] == Py_None ? (float)(1.0 / std::sqrt((double)h.c.head_dim)) : (float)PyFloat_AsDouble(args[6]);
         if (args[6] != Py_None && PyErr_Occurred()) throw Raised{};

@@ -202,7 +202,7 @@ KvqAttnArgs attn_args(const fb2_kvq_cache* c, const fb2_kvq_attention* a) {
     need(a->n_heads >= 1 && a->n_heads % c->n_kv_heads == 0, "n_heads must be a positive multiple of n_kv_heads");
     need(a->n_heads <= 65535, "n_heads must be at most 65535");
     need(a->max_pages >= 0 && a->max_len >= 0, "max_pages and max_len must not be negative");
-    need(a->max_nodes >= 1 && a->max_nodes <= 65535, "max_nodes must be in 1..65535");
+    need(a->max_nodes >= 1 && (int64_t)a->max_nodes * a->n_heads <= INT32_MAX - 1024, "max_nodes must be in 1..2^31 / n_heads");
     need(a->device_row_starts || (a->n_rows == a->n_seqs && a->max_nodes == 1),
          "without row_starts there is one row per sequence and max_nodes is 1");
     need(std::isfinite(a->scale), "scale must be finite");

@@ -102,8 +102,10 @@ class QuantKvCache:
         rows, those whose bit its mask words [rows, words] int32 set (mask
         None: itself and the earlier ones).  scale defaults to
         1 / sqrt(head_dim).  max_nodes and max_len are host bounds of a
-        sequence's rows and of prefix + rows (default: all rows, the page
-        table's width): the tighter, the better the work is split.  out has
+        sequence's rows and of prefix + rows (default: all rows, or as many as
+        the mask has bits; the page table's width): the tighter, the better the
+        work is split, and several sequences without max_nodes are planned as
+        if each had all of the rows.  out has
         q's dtype, lse [rows, heads] is float32; a row that sees nothing
         gives zeros and -inf."""
         return self._calls.cache_attend(self._handle, q, page_table, prefix_lens, starts, mask, scale, max_nodes, max_len)

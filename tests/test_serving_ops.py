@@ -610,6 +610,29 @@ def test_stride_of_a_shared_page_table(pkg):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_attention_without_max_nodes(pkg, dtype):
+    """Several trees whose mask has fewer bits than the call has rows; more rows than 2^16."""
+    g, rnd = gen(61), random.Random(61)
+    cache = filled(pkg, g, 24, 16, 2, 64, "int8")
+    table = torch.arange(24, dtype=torch.int32, device="cuda").view(3, 8)
+    q = normal(g, 60, 4, 64, dtype=DTYPES[dtype])
+    mask = _i32([[rnd.randrange(1 << (i % 20 + 1)) | 1 << i % 20] for i in range(60)])
+    args = (q, table, _i32([90, 0, 31]))
+    kw = dict(starts=_i32([0, 20, 40, 60]), mask=mask)
+    got, want = cache.attend(*args, **kw), cache.attend(*args, **kw, max_nodes=20)
+    assert ((got[0].double() - want[0].double()).abs() <= (2.0 ** -20 if dtype == "fp32" else 2.0 ** -7) * 5).all()
+    assert ((got[1] - want[1]).abs() <= 8 * 2.0 ** -23 * 40).all()
+    rows = 70000  # with the page table's width, each sees at most 16 positions
+    q = normal(g, rows, 2, 64, dtype=DTYPES[dtype])
+    args = (q, table[:2, :1].contiguous(), _i32([3, 11]))
+    kw = dict(starts=_i32([0, rows // 2, rows]))
+    got, want = cache.attend(*args, **kw), cache.attend(*args, **kw, max_nodes=rows // 2)
+    assert ((got[0].double() - want[0].double()).abs() <= (2.0 ** -20 if dtype == "fp32" else 2.0 ** -7) * 5).all()
+    assert torch.isfinite(got[1]).all()
+
+
+@gpu
 def test_attention_bounds_that_cut(pkg):
     """max_len and the page table's width cut what is seen; max_nodes which rows are written."""
     attention_case(pkg, 31, "int8", "fp32", [100, 40], [1, 1], 4, 2, 64, 16, tree=False, max_len=77)
