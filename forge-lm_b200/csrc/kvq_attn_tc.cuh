@@ -154,6 +154,7 @@ __global__ void __launch_bounds__(KVT_LAUNCH, 1) k_kvq_attend_tc(KvqAttnArgs a) 
     const bool worker = warp < KVT_THREADS / 32;
 
     const int b = blockIdx.y;
+    if (b >= a.n_seqs) return a.fill_rest();
     const int rb = blockIdx.x % a.row_blocks, rest = blockIdx.x / a.row_blocks;
     const int split = rest % a.splits, head = rest / a.splits;
     if (a.splits > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge's launch

@@ -276,6 +276,9 @@ PyObject* cache_attend(PyObject*, PyObject* const* args, Py_ssize_t count) {
         a.device_lse = static_cast<float*>(lse.data_ptr());
         a.device_workspace = size ? work.data_ptr() : nullptr;
         a.workspace_bytes = size;
+        // fresh memory: rows of no sequence are filled by the call, or here where it has no room for that
+        a.fill_rest = starts && seqs > 0 && seqs <= 65534;
+        if (starts && !a.fill_rest) out.zero_(), lse.fill_(-INFINITY);
         status(fb2_kvq_attend(&h.c, &a, on.stream()));
         return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(lse)));
     });

@@ -198,7 +198,7 @@ KvqAttnArgs attn_args(const fb2_kvq_cache* c, const fb2_kvq_attention* a) {
     k.c = view_of(c);
     check_dtype(a->dtype);
     need(a->n_seqs >= 0 && a->n_rows >= 0, "n_seqs and n_rows must not be negative");
-    need(a->n_seqs <= 65535, "n_seqs must be at most 65535");
+    need(a->n_seqs <= (a->fill_rest ? 65534 : 65535), "n_seqs must be at most 65535, 65534 with fill_rest");
     need(a->n_heads >= 1 && a->n_heads % c->n_kv_heads == 0, "n_heads must be a positive multiple of n_kv_heads");
     need(a->n_heads <= 65535, "n_heads must be at most 65535");
     need(a->max_pages >= 0 && a->max_len >= 0, "max_pages and max_len must not be negative");
@@ -231,6 +231,7 @@ KvqAttnArgs attn_args(const fb2_kvq_cache* c, const fb2_kvq_attention* a) {
     k.max_len = a->max_len && a->max_len < cap ? a->max_len : (int)cap;
     k.mask_words = a->mask_words;
     k.scale = a->scale;
+    k.fill = a->fill_rest != 0 && a->device_row_starts;
     plan_attention(k);
     return k;
 }
@@ -248,7 +249,7 @@ void launch_attend(const KvqAttnArgs& k, cudaStream_t stream) {
     if (S::SMEM > 48 * 1024) opt_in_smem((const void*)kernel, S::SMEM);
     const int64_t blocks = (int64_t)k.row_blocks * k.splits * k.c.heads;
     need(blocks <= INT32_MAX, "too many rows for one call");
-    kernel<<<dim3((unsigned)blocks, k.n_seqs), WARPS * 32, S::SMEM, stream>>>(k);
+    kernel<<<dim3((unsigned)blocks, k.n_seqs + k.fill), WARPS * 32, S::SMEM, stream>>>(k);
 }
 template <int HD, int FMT>
 void launch_attend(const KvqAttnArgs& k, cudaStream_t stream) {
@@ -267,7 +268,7 @@ void launch_attend_tc(const KvqAttnArgs& k, cudaStream_t stream) {
     opt_in_smem((const void*)kernel, smem);
     const int64_t blocks = (int64_t)k.row_blocks * k.splits * k.c.heads;
     need(blocks <= INT32_MAX, "too many rows for one call");
-    kernel<<<dim3((unsigned)blocks, k.n_seqs), KVT_LAUNCH, smem, stream>>>(k);
+    kernel<<<dim3((unsigned)blocks, k.n_seqs + k.fill), KVT_LAUNCH, smem, stream>>>(k);
 }
 template <int FMT>
 void launch_attend(const KvqAttnArgs& k, cudaStream_t stream) {

@@ -106,8 +106,8 @@ class QuantKvCache:
         the mask has bits; the page table's width): the tighter, the better the
         work is split, and several sequences without max_nodes are planned as
         if each had all of the rows.  out has
-        q's dtype, lse [rows, heads] is float32; a row that sees nothing
-        gives zeros and -inf."""
+        q's dtype, lse [rows, heads] is float32; a row that sees nothing, is
+        in no sequence or lies past max_nodes of its own gives zeros and -inf."""
         return self._calls.cache_attend(self._handle, q, page_table, prefix_lens, starts, mask, scale, max_nodes, max_len)
 
 

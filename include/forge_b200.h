@@ -324,7 +324,8 @@ int32_t fb2_kvq_read(const fb2_kvq_cache* c, int32_t n_rows, const int32_t* devi
  * A row that sees nothing gives out = 0 and lse = -inf.  Positions whose page
  * id is outside the cache, or that lie past max_pages * page_size or past
  * max_len, are not seen.  Rows past max_nodes of a sequence and rows outside
- * every sequence are not written.  K and V are exact; for q, fp32 values are
+ * every sequence (before the first or after the last) are not
+ * written, or with fill_rest are given out = 0 and lse = -inf.  K and V are exact; for q, fp32 values are
  * brought to a fixed point of 23 bits below the row's largest, and what a row
  * weighs V with is carried in fp16 (for fp32 in two such terms) relative to the
  * row's own largest weight.  Waits inside a kernel are
@@ -351,7 +352,7 @@ typedef struct {
     int32_t max_len;    /* host bound of prefix_lens[b] + T_b; 0: max_pages * page_size */
     int32_t mask_words; /* at least ceil(max_nodes / 32) with a mask */
     float scale;        /* finite */
-    int32_t reserved;
+    int32_t fill_rest;  /* not 0: rows that belong to no sequence are written too */
 } fb2_kvq_attention;
 int32_t fb2_kvq_attend_workspace(const fb2_kvq_cache* c, const fb2_kvq_attention* a, int64_t* bytes);
 int32_t fb2_kvq_attend(const fb2_kvq_cache* c, const fb2_kvq_attention* a, void* cuda_stream);

@@ -633,6 +633,56 @@ def test_attention_without_max_nodes(pkg, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("heads", [2, 8])
+@pytest.mark.parametrize("pages", [8, 300])
+def test_attention_rows_outside_every_sequence(pkg, dtype, heads, pages):
+    """They, and rows past max_nodes, give zeros and -inf from Python; the C call leaves
+    them alone unless it is asked to fill them."""
+    import ctypes as C
+    import struct
+    from forge_lm_b200 import _native as N
+    g = gen(62)
+    cache = filled(pkg, g, 24, 16, 2, 64, "int8")
+    table = torch.full((3, pages), -1, dtype=torch.int32, device="cuda")  # a wide one: several blocks and their merge
+    table[:, :8] = torch.arange(24, dtype=torch.int32, device="cuda").view(3, 8)
+    q = normal(g, 50, heads, 64, dtype=DTYPES[dtype])
+    prefix, starts = _i32([90, 0, 31]), _i32([3, 10, 30, 44])
+    rest = torch.ones(50, dtype=torch.bool, device="cuda")
+    for a, b in ((3, 10), (10, 22), (30, 42)):
+        rest[a:b] = False
+
+    def poison():
+        for shape, kind in ((q.shape, q.dtype), (q.shape[:2], torch.float32)):
+            x = torch.full(shape, 7.0, dtype=kind, device="cuda")
+            del x  # what the call gets next
+
+    poison()
+    out, lse = cache.attend(q, table, prefix, starts=starts, max_nodes=12)
+    assert (out[rest] == 0).all() and (lse[rest] == -math.inf).all()
+    assert (out[~rest] != 0).any(-1).all() and torch.isfinite(lse[~rest]).all()
+    out2, lse2 = cache.attend(q, table, prefix, starts=_i32([3, 3, 50, 50]), max_nodes=12)  # sequences without rows
+    assert (out2[:3] == 0).all() and (out2[15:] == 0).all() and torch.isfinite(lse2[3:15]).all() and (lse2[15:] == -math.inf).all()
+    for kw in (dict(), dict(max_nodes=5)):  # no sequence at all
+        poison()
+        none, no_lse = cache.attend(q, table[:0], prefix[:0], starts=starts[:1], **kw)
+        assert (none == 0).all() and (no_lse == -math.inf).all()
+    L, size = N.load(), C.c_int64()
+    c = struct.Struct("=QQ6i").pack(cache.codes.data_ptr(), cache.meta.data_ptr(), 24, 16, 2, 64, 0, 0)
+    for fill in (0, 1):
+        got, got_lse = torch.full_like(out, 7.0), torch.full_like(lse, 7.0)
+        work = torch.empty(1 << 22, dtype=torch.uint8, device="cuda")
+        a = struct.Struct("=8Q4q8ifi").pack(
+            q.data_ptr(), got.data_ptr(), got_lse.data_ptr(), table.data_ptr(), prefix.data_ptr(), starts.data_ptr(), 0,
+            work.data_ptr(), work.numel(), heads * 64, 64, pages, 3, 50, heads, 0 if dtype == "fp32" else 1, pages, 12, 0, 0, 0.125, fill)
+        assert L.fb2_kvq_attend_workspace(c, a, C.byref(size)) == N.FB2_OK and size.value <= work.numel()
+        assert L.fb2_kvq_attend(c, a, torch.cuda.current_stream().cuda_stream) == N.FB2_OK
+        torch.cuda.synchronize()
+        assert torch.equal(got[~rest], out[~rest]) and torch.equal(got_lse[~rest], lse[~rest])
+        assert (got[rest] == (0 if fill else 7)).all() and (got_lse[rest] == (-math.inf if fill else 7)).all()
+
+
+@gpu
 def test_attention_bounds_that_cut(pkg):
     """max_len and the page table's width cut what is seen; max_nodes which rows are written."""
     attention_case(pkg, 31, "int8", "fp32", [100, 40], [1, 1], 4, 2, 64, 16, tree=False, max_len=77)
