@@ -31,12 +31,11 @@ struct KvqAttnArgs {
     int fill;                // 1: a row of blocks for fill_rest
     int splits, chunk, row_blocks, block_rows, warps;  // block_rows 8, 16: k_kvq_attend; 128: k_kvq_attend_tc
     float scale;
+    // a malformed list must not reach past the tensors: each start is cut to them
+    FB2_DEV int start_of(int b) const { return starts ? min(max(__ldg(starts + b), 0), n_rows) : b; }
     FB2_DEV void rows_of(int b, int& first, int& count) const {
-        first = starts ? __ldg(starts + b) : b;
-        const int last = starts ? __ldg(starts + b + 1) : b + 1;
-        // a malformed list must not reach past the tensors
-        first = max(first, 0);
-        count = min(min(last, n_rows) - first, max_nodes);
+        first = start_of(b);
+        count = min(max(start_of(b + 1) - first, 0), max_nodes);
     }
     // Zeros and -inf for the rows that lie past those that their sequence may have,
     // before the first sequence or after the last: the work of a row of blocks of its
@@ -54,8 +53,8 @@ struct KvqAttnArgs {
         for (int b = blockIdx.x; b < n_seqs; b += gridDim.x) {
             int first, count;
             rows_of(b, first, count);
-            if (b == 0) fill_rows(0, min(first, n_rows));
-            fill_rows(min(first + max(count, 0), n_rows), b + 1 < n_seqs ? min(__ldg(starts + b + 1), n_rows) : n_rows);
+            if (b == 0) fill_rows(0, first);
+            fill_rows(first + count, b + 1 < n_seqs ? start_of(b + 1) : n_rows);
         }
     }
     FB2_DEV float load_q(long long row, int head, int d) const {

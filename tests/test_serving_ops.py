@@ -683,6 +683,23 @@ def test_attention_rows_outside_every_sequence(pkg, dtype, heads, pages):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("heads", [2, 8])
+def test_attention_of_malformed_starts(pkg, dtype, heads):
+    """Row starts at the ends of 32 bits reach nothing outside the tensors, and the
+    rows that they do name are right."""
+    g = gen(63)
+    cache = filled(pkg, g, 24, 16, 2, 64, "int8")
+    table = torch.arange(24, dtype=torch.int32, device="cuda").view(3, 8)
+    q = normal(g, 50, heads, 64, dtype=DTYPES[dtype])
+    got = cache.attend(q, table, _i32([90, 70, 31]), starts=_i32([5, -2 ** 31, 2 ** 31 - 1, 50]), max_nodes=50)
+    want = cache.attend(q, table, _i32([90, 70, 31]), starts=_i32([0, 0, 50, 50]), max_nodes=50)
+    assert torch.equal(got[0][5:], want[0][5:]) and torch.equal(got[1][5:], want[1][5:])
+    got = cache.attend(q, table, _i32([90, 70, 31]), starts=_i32([2 ** 31 - 1, -2 ** 31, -2 ** 31, -2 ** 31]), max_nodes=50)
+    assert (got[0] == 0).all() and (got[1] == -math.inf).all()
+
+
+@gpu
 def test_attention_bounds_that_cut(pkg):
     """max_len and the page table's width cut what is seen; max_nodes which rows are written."""
     attention_case(pkg, 31, "int8", "fp32", [100, 40], [1, 1], 4, 2, 64, 16, tree=False, max_len=77)
