@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(WARPS * 32, KvaShape<HD, FMT, NT, SPLIT, WARPS
     if (n_rows <= 0) return;
     const int prefix = max(__ldg(a.prefix + b), 0);
     const int len = (int)min((long long)prefix + count, (long long)a.max_len);
-    const int c0 = split * a.chunk, c1 = min(len, c0 + a.chunk);
+    const int c0 = split * a.chunk, c1 = len - c0 > a.chunk ? c0 + a.chunk : len;
     // row r of the block: token (row0 + r) / share of the sequence, query head
     // head * share + (row0 + r) % share
     if (c0 >= c1 && a.splits > 1) {  // nothing here: the merge has to know

@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(KVT_LAUNCH, 1) k_kvq_attend_tc(KvqAttnArgs a) 
     if (n_rows <= 0) return;
     const int prefix = max(__ldg(a.prefix + b), 0);
     const int len = (int)min((long long)prefix + count, (long long)a.max_len);
-    const int c0 = split * a.chunk, c1 = min(len, c0 + a.chunk);
+    const int c0 = split * a.chunk, c1 = len - c0 > a.chunk ? c0 + a.chunk : len;
     const int r = 32 * quarter + lane, node = (row0 + r) / a.share, h = head * a.share + (row0 + r) - node * a.share;
     const bool mine = worker && r < n_rows;
     const size_t item = (size_t)(first + node) * a.n_heads + h;

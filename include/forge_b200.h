@@ -349,7 +349,7 @@ typedef struct {
     int32_t dtype;      /* fb2_dtype of q and out */
     int32_t max_pages;
     int32_t max_nodes;  /* host bound of T_b */
-    int32_t max_len;    /* host bound of prefix_lens[b] + T_b; 0: max_pages * page_size */
+    int32_t max_len;    /* host bound of prefix_lens[b] + T_b, up to 2^31 - 65536; 0: max_pages * page_size */
     int32_t mask_words; /* at least ceil(max_nodes / 32) with a mask */
     float scale;        /* finite */
     int32_t fill_rest;  /* not 0: rows that belong to no sequence are written too */

@@ -700,6 +700,41 @@ def test_attention_of_malformed_starts(pkg, dtype, heads):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,heads", [("fp32", 1), ("bf16", 1), ("bf16", 40)])
+def test_attention_over_two_billion_positions(pkg, dtype, heads):
+    """As many positions as are counted, most of them in one page: what counts is the last page."""
+    g = gen(64)
+    pages, page, dim = (2 ** 31 - 65536) // 1024, 1024, 16
+    cache = filled(pkg, g, 2, page, 1, dim, "int4")
+    k = normal(g, page, 1, dim)
+    k[..., 0] = 30.0
+    v = normal(g, page, 1, dim)
+    cache.write(k, v, torch.arange(page, 2 * page, dtype=torch.int32, device="cuda"))
+    table = torch.zeros((1, pages), dtype=torch.int32, device="cuda")
+    table[0, -1] = 1
+    q = normal(g, 1, heads, dim, dtype=DTYPES[dtype])
+    q[..., 0] = 12  # scores some 80 above the other page's: together they weigh 2^31 exp(-80)
+    got = cache.attend(q, table, _i32([pages * page - 1]))
+    want = plain_attention(cache, q, torch.tensor([[1]]), [page - 1], [0, 1], None, 0.25)
+    _, vs = decode(cache)
+    ks, _ = decode(cache)
+    check_attention(dtype, got, want, float(vs.abs().max()), float(q.double().cpu().norm(dim=2).max() * ks.norm(dim=2).max() * 0.25))
+
+
+def test_longest_page_table(pkg):
+    """The host refuses more positions than the kernels count, by the table's width or by max_len."""
+    import ctypes as C
+    import struct
+    from forge_lm_b200 import _native as N
+    L, size = N.load(), C.c_int64()
+    cache = struct.Struct("=QQ6i").pack(4096, 4096, 10, 1024, 3, 64, 0, 0)
+    for pages, max_len, status in ((2097088, 0, N.FB2_OK), (2097089, 0, N.FB2_INVALID_ARG), (2097089, 1000, N.FB2_OK),
+                                   (2097151, 2 ** 31 - 65536, N.FB2_OK), (2097151, 2 ** 31 - 65535, N.FB2_INVALID_ARG)):
+        a = struct.Struct("=8Q4q8ifi").pack(*[4096] * 5, 0, 0, 0, 0, 64, 64, pages, 2, 2, 6, 0, pages, 1, max_len, 0, 0.125, 0)
+        assert L.fb2_kvq_attend_workspace(cache, a, C.byref(size)) == status, (pages, max_len)
+
+
+@gpu
 def test_attention_bounds_that_cut(pkg):
     """max_len and the page table's width cut what is seen; max_nodes which rows are written."""
     attention_case(pkg, 31, "int8", "fp32", [100, 40], [1, 1], 4, 2, 64, 16, tree=False, max_len=77)
