@@ -398,7 +398,7 @@ W4Shape w4_shape(int rows, int dtype) {
     const int64_t digits = (int64_t)rows * w4_digits_of(dtype), cols = (int64_t)rows * w4_parts(dtype);
     if (digits <= 32) return {true, (int)((digits + 7) / 8), rows, 1};
     const int tiles = cols <= 16 ? 2 : 4, per = tiles * 8 / w4_parts(dtype);
-    return {false, tiles, per, (rows + per - 1) / per};
+    return {false, tiles, per, (int)(((int64_t)rows + per - 1) / per)};
 }
 
 // Blocks of 16 outputs per warp, and CTAs per cluster (which share the inputs).
@@ -437,7 +437,7 @@ W4Workspace w4_workspace(const W4View& v, const W4Shape& s) {
 // two units of inputs, else by a launch before it (768 x 2304 fp32: 3.3 and 4.1
 // us; 1024 x 4096 bf16: 3.7 and 5.0; 4096 x 4096 fp16: 9.3 and 5.8; 16384 x
 // 16384 bf16: 44 and 29)
-bool w4_direct(const W4View& v, int rows, int dtype) { return rows * w4_digits_of(dtype) <= 8 && v.k64 <= 32; }
+bool w4_direct(const W4View& v, int64_t rows, int dtype) { return rows * w4_digits_of(dtype) <= 8 && v.k64 <= 32; }
 
 template <class K, class... A>
 void launch_cluster(K kernel, dim3 grid, int threads, int smem, int ranks, bool early, cudaStream_t stream, A... args) {

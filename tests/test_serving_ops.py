@@ -916,6 +916,22 @@ def test_products_of_special_rows_and_shapes(pkg):
     assert torch.equal(small * 2.0 ** 80, base) and torch.equal(large * 2.0 ** -80, base)
 
 
+def test_more_rows_than_a_product_takes(pkg):
+    """Sizes are computed in 64 bits: no number of rows is taken for a few."""
+    import ctypes as C
+    import struct
+    from forge_lm_b200 import _native as N
+    L, size = N.load(), C.c_int64()
+    w = struct.Struct("=QQQ4i").pack(4096, 4096, 0, 1, 1, 32, 0)
+    for dtype in (0, 1, 2):
+        last = 0
+        for rows in (100, 10 ** 6, 2 ** 29, 2 ** 30, 715827883, 1431655766, 2 ** 31 - 1):
+            assert L.fb2_w4_matvec_workspace(w, rows, dtype, C.byref(size)) == N.FB2_OK
+            assert (size.value > last) if rows < 2 ** 29 else size.value >= rows * 2048 // 16
+            last = size.value
+            assert L.fb2_w4_matvec(w, rows, 4096, 1, 4096, 1, dtype, None, 0, None) == N.FB2_INVALID_ARG
+
+
 # ---- logit controls -----------------------------------------------------------------------
 
 def plain_controls(logits, windows=None, rep=None, pres=None, freq=None, biases=None, allowed=None, mask_rows=None):
