@@ -90,6 +90,7 @@ int row_shift(int hd) {
     return s;
 }
 dim3 row_grid(int n_rows, int heads, int shift) {
+    need(n_rows <= INT32_MAX - KVQ_THREADS, "n_rows must be at most 2^31 - 129");  // rows are counted in 32 bits
     const int per = KVQ_THREADS >> shift;
     return dim3((unsigned)(((int64_t)n_rows + per - 1) / per), heads, 2);
 }

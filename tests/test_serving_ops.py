@@ -210,6 +210,17 @@ def test_write_of_special_rows(pkg, fmt, dim):
     assert ((k[6] - rows[6].double()).abs() <= 0.501 * step + more).all()
 
 
+def test_more_rows_than_the_cache_takes(pkg):
+    """The last blocks' row numbers stay within 32 bits."""
+    import struct
+    from forge_lm_b200 import _native as N
+    L = N.load()
+    c = struct.Struct("=QQ6i").pack(4096, 4096, 10, 16, 3, 64, 0, 0)
+    for rows in (2 ** 31 - 128, 2 ** 31 - 1):
+        assert L.fb2_kvq_write(c, rows, 4096, 4096, 0, 192, 64, 192, 64, 4096, None) == N.FB2_INVALID_ARG
+        assert L.fb2_kvq_read(c, rows, 4096, 4096, 4096, 0, None) == N.FB2_INVALID_ARG
+
+
 # ---- attention --------------------------------------------------------------------
 
 def plain_attention(cache, q, table, prefix, starts, bits, scale, max_len=None):
