@@ -229,7 +229,7 @@ KvqAttnArgs attn_args(const fb2_kvq_cache* c, const fb2_kvq_attention* a) {
     k.share = a->n_heads / c->n_kv_heads;
     k.dtype = a->dtype;
     k.max_nodes = a->max_nodes;
-    k.max_len = a->max_len && a->max_len < cap ? a->max_len : (int)cap;
+    k.max_len = c->n_pages == 0 ? 0 : a->max_len && a->max_len < cap ? a->max_len : (int)cap;  // no pages: no buffers to address
     // positions are counted in 32 bits, some thousands past the last one
     need(k.max_len <= INT32_MAX - 65535, "max_len (0: max_pages * page_size) must be at most 2^31 - 65536");
     k.mask_words = a->mask_words;

@@ -746,6 +746,27 @@ def test_longest_page_table(pkg):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,heads", [("fp32", 2), ("bf16", 80)])
+def test_cache_without_pages(pkg, dtype, heads):
+    """Its buffers are empty: nothing is written, zeros are read, no row sees anything."""
+    cache = pkg.QuantKvCache.empty(0, 16, 2, 64)
+    k = torch.ones((3, 2, 64), device="cuda")
+    cache.write(k, k, _i32([0, 1, -1]))
+    assert all((t == 0).all() for t in cache.read(_i32([0, 1, -1])))
+    q = torch.ones((3, heads, 64), dtype=DTYPES[dtype], device="cuda")
+    for table in (torch.zeros((3, 40), dtype=torch.int32, device="cuda"), torch.zeros((3, 0), dtype=torch.int32, device="cuda")):
+        out, lse = cache.attend(q, table, _i32([600, 0, 5]))
+        assert (out == 0).all() and (lse == -math.inf).all()
+    from forge_lm_b200 import _native as N
+    import ctypes as C
+    import struct
+    size = C.c_int64()
+    a = struct.Struct("=8Q4q8ifi").pack(*[4096] * 5, 0, 0, 0, 0, 64, 64, 4000, 2, 2, 6, 0, 4000, 1, 0, 0, 0.125, 0)
+    assert N.load().fb2_kvq_attend_workspace(struct.Struct("=QQ6i").pack(0, 0, 0, 16, 3, 64, 0, 0), a, C.byref(size)) == N.FB2_OK
+    assert size.value == 0  # nothing to split
+
+
+@gpu
 def test_attention_bounds_that_cut(pkg):
     """max_len and the page table's width cut what is seen; max_nodes which rows are written."""
     attention_case(pkg, 31, "int8", "fp32", [100, 40], [1, 1], 4, 2, 64, 16, tree=False, max_len=77)
