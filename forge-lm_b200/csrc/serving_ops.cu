@@ -567,6 +567,22 @@ int32_t fb2_w4_matvec(const fb2_w4_linear* w, int32_t n_rows, const void* x, int
 }
 
 // ---- logit controls --------------------------------------------------------------
+namespace {
+// Whether a row of logits shares entries with a row of out that is not its own in place.
+bool rows_collide(const fb2_logit_control* c, int64_t size) {
+    const int64_t from = (int64_t)(intptr_t)c->device_logits, to = (int64_t)(intptr_t)c->device_out, row = c->vocab * size;
+    const int64_t si = c->n_rows > 1 ? c->logits_row_stride * size : 0, so = c->n_rows > 1 ? c->out_row_stride * size : row;
+    const int64_t last = c->n_rows - 1;
+    if (from + last * si + row <= to || to + last * so + row <= from || (from == to && (si == so || last == 0))) return false;
+    for (int64_t r = 0; r <= last; r++) {
+        const int64_t at = from + r * si - to;  // out's rows lie at q * so, so >= row
+        for (int64_t q = std::max<int64_t>(0, at / so - 1); q <= std::min(last, at / so + 1); q++)
+            if (at < q * so + row && q * so < at + row) return true;
+    }
+    return false;
+}
+}  // namespace
+
 int32_t fb2_logit_controls(const fb2_logit_control* c, void* stream) {
     return guarded([&] {
         need(c, "controls are NULL");
@@ -580,6 +596,7 @@ int32_t fb2_logit_controls(const fb2_logit_control* c, void* stream) {
         need(aligned(c->device_logits, es) && aligned(c->device_out, es), "a tensor is not aligned to its element size");
         need(c->n_rows == 1 || (c->out_row_stride >= c->vocab && c->logits_row_stride >= 0),
              "out_row_stride must be at least vocab");
+        need(!rows_collide(c, (int64_t)es), "out must be the logits, row for row, or not overlap them");
         need(!c->device_tokens || (c->device_token_starts && c->n_tokens >= 0), "tokens need token_starts and n_tokens");
         need(!c->device_bias_ids || (c->device_bias_values && c->device_bias_starts && c->n_biases >= 0),
              "bias_ids need bias_values, bias_starts and n_biases");

@@ -159,6 +159,7 @@ def logit_controls(logits, *, tokens=None, token_starts=None, repetition=None, p
     window holds c > 0 times: l * repetition where l < 0, else l / repetition;
     then - presence - frequency * c.  Then the bias is added and what the mask
     does not allow becomes -inf.  Computed in fp32; the result has the logits'
-    dtype and goes to `out` (which may be `logits`) or a new tensor."""
+    dtype and goes to `out` (which may be `logits`, but not overlap it in any
+    other way) or a new tensor."""
     return (_calls or _load()).controls(logits, tokens, token_starts, repetition, presence, frequency, bias_ids, bias_values,
                                         bias_starts, allowed, mask_rows, out)

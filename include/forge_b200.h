@@ -406,7 +406,8 @@ int32_t fb2_w4_matvec(const fb2_w4_linear* w, int32_t n_rows, const void* device
  *   l = -inf where the row's grammar mask does not allow v (bit v % 32 of word
  *       v / 32; 1 allows), whatever l was.
  * A row whose mask allows nothing is all -inf.  Each control is left out where
- * its pointer is NULL.  device_out may be device_logits. */
+ * its pointer is NULL.  device_out may be device_logits with the same row stride;
+ * otherwise its rows share nothing with the logits'. */
 typedef struct {
     const void* device_logits; /* [n_rows][vocab], rows logits_row_stride apart */
     void* device_out;          /* rows out_row_stride apart, same type */

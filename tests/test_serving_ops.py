@@ -1104,6 +1104,38 @@ def test_controls_of_lists_of_many_different_ids(pkg, dtype, ids):
     assert torch.equal(logits, got)
 
 
+def test_controls_refuse_rows_that_overlap(pkg):
+    """out in place of the logits, beside them or between them, but not across them."""
+    import struct
+    from forge_lm_b200 import _native as N
+    L, con = N.load(), struct.Struct("=12Q4q6i")
+
+    def status(logits, out, in_row, out_row, rows, vocab=100):
+        s = L.fb2_logit_controls(con.pack(logits, out, *[0] * 10, in_row, out_row, 0, 0, rows, vocab, 0, 0, 0, 0), None)
+        return s == N.FB2_INVALID_ARG and b"overlap" in L.fb2_last_error()
+
+    at = 1 << 20
+    for logits, out, in_row, out_row, rows in ((at, at, 100, 120, 3), (at, at, 0, 100, 3), (at, at + 4, 100, 100, 1),
+                                               (at, at + 4, 120, 120, 3), (at, at + 400, 100, 100, 3), (at + 400, at, 100, 100, 3),
+                                               (at, at + 440, 220, 200, 9), (at, at + 396, 300, 300, 2), (at + 1000, at, 0, 200, 4)):
+        assert status(logits, out, in_row, out_row, rows)
+
+
+@gpu
+def test_controls_between_rows_of_the_logits(pkg):
+    g = gen(71)
+    both = normal(g, 5, 300)
+    keep = both[:, :100].clone()
+    allowed = torch.randint(-2 ** 31, 2 ** 31, (5, 4), device="cuda", generator=g).to(torch.int32)
+    want = pkg.logit_controls(keep, allowed=allowed)
+    pkg.logit_controls(both[:, :100], allowed=allowed, out=both[:, 100:200])
+    assert torch.equal(both[:, 100:200], want) and torch.equal(both[:, :100], keep)
+    pkg.logit_controls(both[:, :100], allowed=allowed, out=both[:, :100])
+    assert torch.equal(both[:, :100], want)
+    with pytest.raises(pkg.ArgumentError):
+        pkg.logit_controls(both[:, :100], out=both[:, 50:150])
+
+
 # ---- together -------------------------------------------------------------------------------
 
 @gpu
