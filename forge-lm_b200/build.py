@@ -32,7 +32,7 @@ ROOT = os.path.dirname(HERE)
 NVCC_FLAGS = [
     "-O3", "-std=c++17", "-lineinfo",
     "-gencode", "arch=compute_100a,code=sm_100a",
-    "-Xcompiler", "-fPIC,-O3",
+    "-Xcompiler", "-fPIC,-O3,-fvisibility=hidden",
     "--expt-relaxed-constexpr",
     "-Xptxas", "-warn-spills",
 ]
@@ -78,7 +78,7 @@ def _flags() -> list[str]:
 
 def _sources() -> list[str]:
     sources = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh", ".hpp"))]
-    sources.append(os.path.join(ROOT, "include", "forge_b200.h"))
+    sources += [os.path.join(ROOT, "include", h) for h in ("forge_b200.h", "forge_b200_testing.h")]
     sources.append(os.path.join(GEN, "expf_fixups.inc"))
     return sorted(sources)
 

@@ -26,6 +26,7 @@
 #include <vector>
 
 #include "../../include/forge_b200.h"
+#include "../../include/forge_b200_testing.h"
 #include "capi.cuh"
 #include "dotnet_random.hpp"
 #include "kernels.cuh"

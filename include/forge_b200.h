@@ -33,6 +33,9 @@
 #ifdef __cplusplus
 extern "C" {
 #endif
+#ifdef __GNUC__
+#pragma GCC visibility push(default) /* the library exports these and hides the rest */
+#endif
 
 #define FB2_ABI_VERSION 1
 
@@ -493,6 +496,9 @@ int32_t fb2_tokenizer_encode(const fb2_tokenizer* t, const uint8_t* bytes, int64
 int32_t fb2_tokenizer_decode(const fb2_tokenizer* t, const int32_t* ids, int64_t n_ids, uint8_t* bytes,
                              int64_t capacity, int64_t* n_bytes);
 
+#ifdef __GNUC__
+#pragma GCC visibility pop
+#endif
 #ifdef __cplusplus
 }
 #endif

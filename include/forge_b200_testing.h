@@ -14,6 +14,9 @@
 #ifdef __cplusplus
 extern "C" {
 #endif
+#ifdef __GNUC__
+#pragma GCC visibility push(default) /* the library exports these and hides the rest */
+#endif
 
 /* y[i] = device exponential of x[i] (host arrays, n > 0). */
 int32_t fb2_test_expf(const float* x, float* y, int64_t n);
@@ -62,6 +65,9 @@ int32_t fb2_test_sha256(const void* data, int64_t n, uint8_t* out32);
  * FB2_UNSUPPORTED when the tensor-core path is unavailable. */
 int32_t fb2_test_gemm_tc(int32_t M, int32_t N, int32_t K, const float* A, const float* W, float* out);
 
+#ifdef __GNUC__
+#pragma GCC visibility pop
+#endif
 #ifdef __cplusplus
 }
 #endif

@@ -33,6 +33,21 @@ def test_library_exports_every_declared_symbol(pkg):
     assert set(N.EXPORTED) | set(N.TEST_EXPORTED) >= declared
 
 
+def test_library_exports_nothing_else(pkg):
+    """A function of the host program (a `fail` or `ck` of its own, say) replaces
+    none of the library's: what is exported is the C interface and instances
+    of the standard library's templates."""
+    import shutil
+    import subprocess
+    if shutil.which("nm") is None:
+        pytest.skip("needs nm")
+    out = subprocess.run(["nm", "-D", "--defined-only", "-C", pkg.library_path()], check=True, capture_output=True, text=True)
+    names = [line.split(None, 2)[2] for line in out.stdout.splitlines()]
+    declared = _declared_symbols()
+    other = [n for n in names if n not in declared and "std::" not in n]
+    assert not other, other[:10]
+
+
 def test_version_and_errors_without_device(pkg):
     from forge_lm_b200 import _native as N
     L = N.load()
