@@ -7,12 +7,13 @@ Steps:
   2. nvcc -gencode arch=compute_100a,code=sm_100a: one object per .cu file
      (in csrc/generated/), linked to libforge_b200.so.
   3. g++ csrc/serving_binding.cpp -> _serving.so, the serving operators' calls
-     on torch tensors.
+     on torch tensors, where torch is installed.
 No fast-math: the sampler's division and exponentials must round as IEEE.
 """
 from __future__ import annotations
 
 import hashlib
+import importlib.util
 import json
 import os
 import shutil
@@ -141,8 +142,12 @@ def _binding_command(out: str) -> list[str]:
             "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN"]
 
 
-def build_binding(verbose: bool = False, force: bool = False) -> str:
-    """The extension module, compiled again where its source or the C header is newer."""
+def build_binding(verbose: bool = False, force: bool = False) -> str | None:
+    """The extension module, compiled again where its source or the C header is
+    newer.  None without torch: the C library does not need it."""
+    if importlib.util.find_spec("torch") is None:
+        print("torch is not installed: the serving operators' Python calls (_serving.so) are not built")
+        return None
     sources = [os.path.join(CSRC, "serving_binding.cpp"), os.path.join(ROOT, "include", "forge_b200.h")]
     if force or _newer(BINDING, sources):
         cmd = _binding_command(BINDING + ".tmp")
