@@ -13,6 +13,7 @@ No fast-math: the sampler's division and exponentials must round as IEEE.
 from __future__ import annotations
 
 import hashlib
+import importlib.metadata
 import importlib.util
 import json
 import os
@@ -144,17 +145,21 @@ def _binding_command(out: str) -> list[str]:
 
 def build_binding(verbose: bool = False, force: bool = False) -> str | None:
     """The extension module, compiled again where its source or the C header is
-    newer.  None without torch: the C library does not need it."""
+    newer or it was built for another torch or Python (the JSON beside it says
+    for which).  None without torch: the C library does not need it."""
     if importlib.util.find_spec("torch") is None:
         print("torch is not installed: the serving operators' Python calls (_serving.so) are not built")
         return None
     sources = [os.path.join(CSRC, "serving_binding.cpp"), os.path.join(ROOT, "include", "forge_b200.h")]
-    if force or _newer(BINDING, sources):
+    made_for = {"torch": importlib.metadata.version("torch"), "python": sysconfig.get_config_var("EXT_SUFFIX")}
+    if force or _newer(BINDING, sources) or read_stamp(BINDING) != made_for:
         cmd = _binding_command(BINDING + ".tmp")
         if verbose:
             print(" ".join(cmd))
         subprocess.run(cmd, check=True)
         os.replace(BINDING + ".tmp", BINDING)
+        with open(stamp_path(BINDING), "w") as f:
+            json.dump(made_for, f)
     return BINDING
 
 

@@ -11,7 +11,9 @@ are compiled (csrc/serving_binding.cpp).
 """
 from __future__ import annotations
 
+import importlib.metadata
 import importlib.util
+import json
 import os
 
 from . import _native as N
@@ -34,6 +36,13 @@ def _load():
         N.load()
         if not os.path.exists(_PATH):
             raise OSError(f"_serving.so not built at {_PATH}; run __graft_entry__.build()")
+        try:  # what it was built for (build.py)
+            with open(_PATH + ".flags") as f:
+                built = json.load(f)["torch"]
+        except (OSError, ValueError, KeyError):
+            built = None
+        if built != importlib.metadata.version("torch"):
+            raise OSError(f"_serving.so was built for torch {built}, not the installed one; run __graft_entry__.build()")
         spec = importlib.util.spec_from_file_location("_serving", _PATH)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)

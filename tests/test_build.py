@@ -1,6 +1,7 @@
 """The build of the Python extension beside the C library (build.py)."""
 from __future__ import annotations
 
+import importlib.metadata
 import importlib.util
 import os
 
@@ -38,3 +39,29 @@ def test_the_library_builds_without_torch(build, monkeypatch):
     assert build.build_binding() is None
     assert build.build() == build.LIB
     assert build.ran == [] and not os.path.exists(build.BINDING)
+
+
+def test_the_extension_is_built_again_for_another_torch(build, monkeypatch):
+    pytest.importorskip("torch")
+    assert build.build_binding() == build.BINDING and len(build.ran) == 1
+    assert build.build_binding() == build.BINDING and len(build.ran) == 1  # up to date
+    real = importlib.metadata.version
+    monkeypatch.setattr(importlib.metadata, "version", lambda name: "0.0.1" if name == "torch" else real(name))
+    build.build_binding()
+    assert len(build.ran) == 2
+    build.build_binding()
+    assert len(build.ran) == 2
+    os.remove(build.stamp_path(build.BINDING))  # one whose torch is not known
+    build.build_binding()
+    assert len(build.ran) == 3
+
+
+def test_an_extension_for_another_torch_is_not_loaded(pkg, monkeypatch):
+    pytest.importorskip("torch")
+    from forge_lm_b200 import serving
+    monkeypatch.setattr(serving, "_calls", None)
+    assert serving._load() is not None
+    monkeypatch.setattr(serving, "_calls", None)
+    monkeypatch.setattr(importlib.metadata, "version", lambda name: "0.0.1")
+    with pytest.raises(OSError, match="another|installed"):
+        serving._load()
