@@ -40,8 +40,8 @@ def _load():
             with open(_PATH + ".flags") as f:
                 built = json.load(f)["torch"]
         except (OSError, ValueError, KeyError):
-            built = None
-        if built != importlib.metadata.version("torch"):
+            built = None  # not known
+        if built not in (None, importlib.metadata.version("torch")):
             raise OSError(f"_serving.so was built for torch {built}, not the installed one; run __graft_entry__.build()")
         spec = importlib.util.spec_from_file_location("_serving", _PATH)
         module = importlib.util.module_from_spec(spec)

@@ -65,3 +65,13 @@ def test_an_extension_for_another_torch_is_not_loaded(pkg, monkeypatch):
     monkeypatch.setattr(importlib.metadata, "version", lambda name: "0.0.1")
     with pytest.raises(OSError, match="another|installed"):
         serving._load()
+
+
+def test_an_extension_without_its_record_is_loaded(pkg, monkeypatch, tmp_path):
+    pytest.importorskip("torch")
+    from forge_lm_b200 import serving
+    lone = tmp_path / "_serving.so"
+    lone.symlink_to(serving._PATH)
+    monkeypatch.setattr(serving, "_PATH", str(lone))
+    monkeypatch.setattr(serving, "_calls", None)
+    assert serving._load() is not None
