@@ -140,11 +140,29 @@ H& handle(PyObject* o) {
 
 // ---- the cache -------------------------------------------------------------------
 
+// A buffer that a handle holds: still of the size and kind that it was made with?
+// (resize_, set_ or .data may have changed the tensor since.)
+void check_held(const at::Tensor& t, at::ScalarType type, int64_t bytes, int index, const char* name) {
+    if (t.scalar_type() != type || !t.is_cuda() || t.get_device() != index || !t.is_contiguous() ||
+        t.numel() * (int64_t)t.element_size() != bytes)
+        refuse(std::string(name) + " was given another size, type, layout or device since the object was made");
+}
+
 struct Cache {
     static constexpr const char* kName = "forge_b200.cache";
     at::Tensor codes, meta;
     fb2_kvq_cache c{};
+    int64_t code_bytes = 0, meta_bytes = 0;
     int index = 0;
+    // the cache with the buffers where they are now
+    fb2_kvq_cache now() const {
+        check_held(codes, at::kByte, code_bytes, index, "codes");
+        check_held(meta, at::kInt, meta_bytes, index, "meta");
+        fb2_kvq_cache n = c;
+        n.device_codes = codes.data_ptr();
+        n.device_meta = meta.data_ptr();
+        return n;
+    }
 };
 
 PyObject* cache_new(PyObject*, PyObject* const* args, Py_ssize_t count) {
@@ -162,14 +180,11 @@ PyObject* cache_new(PyObject*, PyObject* const* args, Py_ssize_t count) {
         const int64_t dim = integer(args[2], "head_dim");
         h->c.format = (int32_t)integer(args[3], "format");
         need(dim == h->codes.size(4) * (h->c.format == FB2_KVQ_INT8 ? 1 : 2), "row bytes do not fit head_dim");
-        h->c.device_codes = h->codes.data_ptr();
-        h->c.device_meta = h->meta.data_ptr();
         h->c.n_pages = small(h->codes.size(0), "pages");
         h->c.n_kv_heads = small(h->codes.size(1), "kv heads");
         h->c.page_size = small(h->codes.size(3), "page size");
         h->c.head_dim = small(dim, "head_dim");
-        int64_t a, b;
-        status(fb2_kvq_sizes(&h->c, &a, &b));
+        status(fb2_kvq_sizes(&h->c, &h->code_bytes, &h->meta_bytes));
         return capsule(std::move(h));
     });
 }
@@ -195,8 +210,9 @@ PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t count) {
         const at::Tensor &k = rows_of(h, args[1], "k", rows, h.c.n_kv_heads), &v = rows_of(h, args[2], "v", rows, h.c.n_kv_heads);
         need(k.scalar_type() == v.scalar_type(), "k and v must have the same dtype");
         const int32_t code = code_of(k.scalar_type());
+        const fb2_kvq_cache c = h.now();
         OnDevice on(h.index);
-        status(fb2_kvq_write(&h.c, small(rows, "rows"), k.data_ptr(), v.data_ptr(), code, k.stride(0), k.stride(1), v.stride(0),
+        status(fb2_kvq_write(&c, small(rows, "rows"), k.data_ptr(), v.data_ptr(), code, k.stride(0), k.stride(1), v.stride(0),
                              v.stride(1), data<int32_t>(slots), on.stream()));
         Py_RETURN_NONE;
     });
@@ -211,10 +227,11 @@ PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t count) {
         need(args[2] == Py_None || THPDtype_Check(args[2]), "dtype must be a torch dtype");
         const at::ScalarType type = args[2] == Py_None ? at::kFloat : reinterpret_cast<THPDtype*>(args[2])->scalar_type;
         const int32_t code = code_of(type);
+        const fb2_kvq_cache c = h.now();
         OnDevice on(h.index);
         const int64_t shape[3] = {slots->numel(), h.c.n_kv_heads, h.c.head_dim};
         at::Tensor k = empty(shape, type, h.index), v = empty(shape, type, h.index);
-        status(fb2_kvq_read(&h.c, small(shape[0], "rows"), data<int32_t>(slots), k.data_ptr(), v.data_ptr(), code, on.stream()));
+        status(fb2_kvq_read(&c, small(shape[0], "rows"), data<int32_t>(slots), k.data_ptr(), v.data_ptr(), code, on.stream()));
         return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(k)), THPVariable_Wrap(std::move(v)));
     });
 }
@@ -267,9 +284,10 @@ PyObject* cache_attend(PyObject*, PyObject* const* args, Py_ssize_t count) {
         a.device_prefix_lens = data<int32_t>(prefix);
         a.device_row_starts = data<int32_t>(starts);
         a.device_mask = data<uint32_t>(mask);
+        const fb2_kvq_cache c = h.now();
         OnDevice on(h.index);
         int64_t size = 0;
-        status(fb2_kvq_attend_workspace(&h.c, &a, &size));
+        status(fb2_kvq_attend_workspace(&c, &a, &size));
         at::Tensor out = empty({rows, heads, h.c.head_dim}, q.scalar_type(), h.index), lse = empty({rows, heads}, at::kFloat, h.index), work;
         if (size) work = empty({size}, at::kByte, h.index);
         a.device_out = out.data_ptr();
@@ -279,7 +297,7 @@ PyObject* cache_attend(PyObject*, PyObject* const* args, Py_ssize_t count) {
         // fresh memory: rows of no sequence are filled by the call, or here where it has no room for that
         a.fill_rest = starts && seqs > 0 && seqs <= 65534;
         if (starts && !a.fill_rest) out.zero_(), lse.fill_(-INFINITY);
-        status(fb2_kvq_attend(&h.c, &a, on.stream()));
+        status(fb2_kvq_attend(&c, &a, on.stream()));
         return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(lse)));
     });
 }
@@ -290,7 +308,20 @@ struct Linear {
     static constexpr const char* kName = "forge_b200.linear";
     at::Tensor codes, meta, bias;
     fb2_w4_linear w{};
+    int64_t code_bytes = 0, meta_bytes = 0;
     int index = 0;
+    fb2_w4_linear now() const {
+        check_held(codes, at::kInt, code_bytes, index, "codes");
+        check_held(meta, at::kInt, meta_bytes, index, "meta");
+        fb2_w4_linear n = w;
+        n.device_codes = codes.data_ptr();
+        n.device_meta = meta.data_ptr();
+        if (bias.defined()) {
+            check_held(bias, at::kFloat, (int64_t)w.out_features * 4, index, "bias");
+            n.device_bias = static_cast<const float*>(bias.data_ptr());
+        }
+        return n;
+    }
 };
 
 PyObject* linear_new(PyObject*, PyObject* const* args, Py_ssize_t count) {
@@ -308,13 +339,9 @@ PyObject* linear_new(PyObject*, PyObject* const* args, Py_ssize_t count) {
         h->w.out_features = small(integer(args[4], "out_features"), "out_features");
         h->w.group = small(integer(args[5], "group"), "group");
         need(!h->bias.defined() || h->bias.numel() == h->w.out_features, "bias must have out_features entries");
-        int64_t a, b;
-        status(fb2_w4_sizes(&h->w, &a, &b));
-        if (h->codes.numel() * 4 != a || h->meta.numel() * 4 != b)
-            refuse("codes and meta must have " + std::to_string(a) + " and " + std::to_string(b) + " bytes");
-        h->w.device_codes = h->codes.data_ptr();
-        h->w.device_meta = h->meta.data_ptr();
-        h->w.device_bias = h->bias.defined() ? static_cast<const float*>(h->bias.data_ptr()) : nullptr;
+        status(fb2_w4_sizes(&h->w, &h->code_bytes, &h->meta_bytes));
+        if (h->codes.numel() * 4 != h->code_bytes || h->meta.numel() * 4 != h->meta_bytes)
+            refuse("codes and meta must have " + std::to_string(h->code_bytes) + " and " + std::to_string(h->meta_bytes) + " bytes");
         return capsule(std::move(h));
     });
 }
@@ -328,9 +355,10 @@ PyObject* linear_pack(PyObject*, PyObject* const* args, Py_ssize_t count) {
                  (w.stride(1) == 1 || w.size(1) == 1),
              "w must be a CUDA tensor [in, out] with contiguous rows");
         const int32_t code = code_of(w.scalar_type());
+        const fb2_w4_linear l = h.now();
         OnDevice on(h.index);
         const int64_t row = w.size(0) > 1 ? w.stride(0) : w.size(1);  // one row may have any stride
-        status(fb2_w4_pack(&h.w, w.data_ptr(), code, row, on.stream()));
+        status(fb2_w4_pack(&l, w.data_ptr(), code, row, on.stream()));
         Py_RETURN_NONE;
     });
 }
@@ -350,13 +378,14 @@ PyObject* linear_call(PyObject*, PyObject* const* args, Py_ssize_t count) {
         need(flat.stride(1) == 1 || k == 1, "x must have a contiguous last dimension");
         c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
         shape.back() = n;
+        const fb2_w4_linear l = h.now();
         OnDevice on(h.index);
         at::Tensor y = empty(shape, x.scalar_type(), h.index), work;
         const int32_t rows = small(flat.size(0), "rows");
         int64_t size = 0;
-        status(fb2_w4_matvec_workspace(&h.w, rows, code, &size));
+        status(fb2_w4_matvec_workspace(&l, rows, code, &size));
         if (size) work = empty({size}, at::kByte, h.index);
-        status(fb2_w4_matvec(&h.w, rows, flat.data_ptr(), flat.stride(0), y.data_ptr(), n, code, size ? work.data_ptr() : nullptr,
+        status(fb2_w4_matvec(&l, rows, flat.data_ptr(), flat.stride(0), y.data_ptr(), n, code, size ? work.data_ptr() : nullptr,
                              size, on.stream()));
         return THPVariable_Wrap(std::move(y));
     });

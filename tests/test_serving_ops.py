@@ -1260,6 +1260,41 @@ def test_example_of_a_decoder(pkg, cache):
             assert float(want[t[i]]) >= float(want.max()) - step * float(row.abs().max())
 
 
+@gpu
+def test_buffers_that_are_replaced(pkg):
+    """Calls use the held tensors' memory as it is at the call; ones of another size are refused."""
+    g = gen(81)
+    cache = filled(pkg, g, 4, 16, 2, 64, "int8")
+    slots = torch.arange(64, dtype=torch.int32, device="cuda")
+    k, v = cache.read(slots)
+    codes, meta = cache.codes, cache.meta
+    old = codes.data_ptr()
+    codes.data, meta.data = codes.clone(), meta.clone()
+    codes.data[0], meta.data[0] = 128, 0
+    assert codes.data_ptr() != old
+    k2, v2 = cache.read(slots)
+    assert (k2[:16] == 0).all() and torch.equal(k2[16:], k[16:]) and torch.equal(v2[16:], v[16:])
+    linear = random_linear(pkg, g, 128, 48, 64, True)
+    x = normal(g, 2, 128)
+    y = linear(x)
+    linear.codes.data = torch.zeros_like(linear.codes)
+    linear.meta.data = torch.zeros_like(linear.meta)
+    assert torch.equal(linear(x), linear.bias.expand(2, 48))
+    linear.bias.data = linear.bias + 1
+    assert torch.equal(linear(x), linear.bias.expand(2, 48)) and not torch.equal(y, linear(x))
+    for tensor, change in ((codes, lambda: codes.resize_(1, 2, 2, 16, 64)), (meta, lambda: meta.set_(torch.zeros(3, dtype=torch.int32, device="cuda"))),
+                           (linear.bias, lambda: linear.bias.resize_(47)), (linear.codes, lambda: setattr(linear.codes, "data", linear.codes[:1]))):
+        keep = tensor.data
+        change()
+        with pytest.raises(pkg.ArgumentError):
+            cache.read(slots) if tensor is codes or tensor is meta else linear(x)
+        with pytest.raises(pkg.ArgumentError):
+            cache.write(k, v, slots) if tensor is codes or tensor is meta else linear(x)
+        tensor.data = keep.clone()
+        if tensor is codes:
+            codes.resize_(4, 2, 2, 16, 64)
+
+
 # ---- refusals -------------------------------------------------------------------------------
 
 @gpu
