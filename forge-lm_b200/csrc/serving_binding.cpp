@@ -45,6 +45,11 @@ void status(int32_t s) {
     throw Raised{};
 }
 
+// Tells autograd and whoever else counts versions that a call changed t.
+void changed(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // Python errors for what `f` throws
 template <class F>
 PyObject* guarded(F&& f) {
@@ -214,6 +219,7 @@ PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t count) {
         OnDevice on(h.index);
         status(fb2_kvq_write(&c, small(rows, "rows"), k.data_ptr(), v.data_ptr(), code, k.stride(0), k.stride(1), v.stride(0),
                              v.stride(1), data<int32_t>(slots), on.stream()));
+        changed(h.codes), changed(h.meta);
         Py_RETURN_NONE;
     });
 }
@@ -359,6 +365,7 @@ PyObject* linear_pack(PyObject*, PyObject* const* args, Py_ssize_t count) {
         OnDevice on(h.index);
         const int64_t row = w.size(0) > 1 ? w.stride(0) : w.size(1);  // one row may have any stride
         status(fb2_w4_pack(&l, w.data_ptr(), code, row, on.stream()));
+        changed(h.codes), changed(h.meta);
         Py_RETURN_NONE;
     });
 }
@@ -460,6 +467,7 @@ PyObject* controls(PyObject*, PyObject* const* args, Py_ssize_t count) {
         c.vocab = small(vocab, "vocab");
         if (rows && vocab) status(fb2_logit_controls(&c, on.stream()));
         if (fresh.defined()) return THPVariable_Wrap(std::move(fresh));
+        changed(*out);
         return Py_NewRef(args[11]);
     });
 }

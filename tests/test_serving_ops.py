@@ -1295,6 +1295,34 @@ def test_buffers_that_are_replaced(pkg):
             codes.resize_(4, 2, 2, 16, 64)
 
 
+@gpu
+def test_changed_tensors_are_counted(pkg):
+    """What a call writes into has a new version: autograd refuses to use a stale value."""
+    cache = pkg.QuantKvCache.empty(2, 16, 1, 32)
+    k = torch.ones((1, 1, 32), device="cuda")
+    before = cache.codes._version, cache.meta._version
+    cache.write(k, k, _i32([3]))
+    assert cache.codes._version > before[0] and cache.meta._version > before[1]
+    before = cache.codes._version
+    cache.read(_i32([3]))
+    assert cache.codes._version == before
+    logits = torch.randn((2, 64), device="cuda")
+    weight = torch.ones((2, 64), device="cuda", requires_grad=True)
+    loss = (weight * logits).sum()  # keeps logits for weight's gradient
+    before = logits._version
+    pkg.logit_controls(logits, allowed=torch.zeros((2, 2), dtype=torch.int32, device="cuda"), out=logits)
+    assert logits._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():  # has no versions
+        out = torch.zeros((2, 64), device="cuda")
+        assert pkg.logit_controls(torch.ones((2, 64), device="cuda"), out=out) is out and (out == 1).all()
+        other = pkg.QuantKvCache.empty(2, 16, 1, 32)
+        other.write(k, k, _i32([3]))
+    other.write(k, k, _i32([4]))
+    assert all((t == 1).all() for t in other.read(_i32([3, 4])))
+
+
 # ---- refusals -------------------------------------------------------------------------------
 
 @gpu
