@@ -70,7 +70,10 @@ PyObject* guarded(F&& f) {
 
 const at::Tensor& tensor(PyObject* o, const char* name) {
     if (!THPVariable_Check(o)) refuse(std::string(name) + " must be a tensor");
-    return THPVariable_Unpack(o);
+    const at::Tensor& t = THPVariable_Unpack(o);
+    // its memory holds the values with the other sign
+    if (t.is_neg()) refuse(std::string(name) + " must not be a negated view (resolve_neg() makes a tensor of it)");
+    return t;
 }
 int32_t code_of(at::ScalarType t) {
     switch (t) {

@@ -1326,6 +1326,28 @@ def test_changed_tensors_are_counted(pkg):
 # ---- refusals -------------------------------------------------------------------------------
 
 @gpu
+def test_negated_views_are_refused(pkg):
+    """Their memory holds the values with the other sign."""
+    g = gen(82)
+    cache = pkg.QuantKvCache.empty(2, 16, 1, 32)
+    k, slots = normal(g, 1, 1, 32), _i32([3])
+    neg = torch._neg_view(k)
+    assert neg.is_neg() and torch.equal(neg, -k)
+    w = normal(g, 32, 16)
+    linear = pkg.W4Linear.pack(w, 32)
+    logits = normal(g, 1, 32)
+    for call in (lambda: cache.write(neg, k, slots), lambda: cache.write(k, neg, slots),
+                 lambda: cache.attend(neg, _i32([[0, 1]]), _i32([4])), lambda: linear(neg),
+                 lambda: pkg.W4Linear.pack(torch._neg_view(w), 32), lambda: pkg.logit_controls(torch._neg_view(logits)),
+                 lambda: pkg.logit_controls(logits, out=torch._neg_view(logits.clone()))):
+        with pytest.raises(pkg.ArgumentError, match="negated"):
+            call()
+    cache.write(neg.resolve_neg(), k, slots)
+    got, _ = cache.read(slots)
+    assert ((got + k).abs() <= k.abs().max() / 250).all()
+
+
+@gpu
 def test_refusals_on_the_device(pkg):
     E = pkg.ArgumentError
     cache = pkg.QuantKvCache.empty(4, 16, 2, 64)
