@@ -49,7 +49,8 @@ EXPORTED = [
     "fb2_w4_sizes", "fb2_w4_pack", "fb2_w4_matvec_workspace", "fb2_w4_matvec", "fb2_logit_controls",
 ]
 TEST_EXPORTED = ["fb2_test_expf", "fb2_test_expf_hash", "fb2_test_dotnet_random", "fb2_test_mk_trace",
-                 "fb2_test_gemm_tc", "fb2_test_sha256", "fb2_test_mk_withhold", "fb2_test_fail_alloc", "fb2_test_mk_geometry"]
+                 "fb2_test_gemm_tc", "fb2_test_sha256", "fb2_test_mk_withhold", "fb2_test_fail_alloc", "fb2_test_mk_geometry",
+                 "fb2_test_kvq_withhold"]
 
 
 class ModelDesc(C.Structure):
@@ -128,6 +129,7 @@ def load(path: str | None = None):
     L.fb2_test_gemm_tc.argtypes = [i32, i32, i32, vp, vp, vp]
     L.fb2_test_sha256.argtypes = [vp, i64, vp]
     L.fb2_test_mk_withhold.argtypes = [vp, i32, i64]
+    L.fb2_test_kvq_withhold.argtypes = [i32, i64]
     L.fb2_test_fail_alloc.argtypes = [i64, C.POINTER(i64)]
     L.fb2_test_mk_geometry.argtypes = [vp, C.POINTER(i32), C.POINTER(i32), C.POINTER(i32), C.POINTER(i32)]
     L.fb2_forgemodel_read_header.argtypes = [C.c_char_p, C.POINTER(ModelDesc), C.c_char_p, i32]

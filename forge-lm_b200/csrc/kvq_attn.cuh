@@ -31,6 +31,8 @@ struct KvqAttnArgs {
     int fill;                // 1: a row of blocks for fill_rest
     int splits, chunk, row_blocks, block_rows, warps;  // block_rows 8, 16: k_kvq_attend; 128: k_kvq_attend_tc
     float scale;
+    int withhold;            // test hook: block 0 does not announce the end of this tile's O; -1: every block does
+    unsigned long long wait_ns;  // limit of k_kvq_attend_tc's waits
     // a malformed list must not reach past the tensors: each start is cut to them
     FB2_DEV int start_of(int b) const { return starts ? min(max(__ldg(starts + b), 0), n_rows) : b; }
     FB2_DEV void rows_of(int b, int& first, int& count) const {

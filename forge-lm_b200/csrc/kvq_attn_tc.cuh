@@ -28,8 +28,8 @@
 //   3. weights into P(t), V(t) becomes an operand, O(t).
 // One more warp issues the MMAs (which takes as long as the tensor cores need)
 // and looks up the pages of later tiles.
-// Every mbarrier wait is bounded; on expiry the CTA stops, drains its MMAs
-// (bounded), frees its TMEM and writes NaN for its rows.
+// Every mbarrier wait is bounded (2 s); on expiry the CTA stops, drains its MMAs
+// (bounded as well), frees its TMEM and writes NaN for its rows.
 #pragma once
 #include "kvq_attn.cuh"
 #include "tc.cuh"
@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(KVT_LAUNCH, 1) k_kvq_attend_tc(KvqAttnArgs a) 
 #pragma unroll
                 for (int kk = 0; kk < KVT_KEYS / 16; kk++)
                     kvt::mma(tmem + S::O_COL, p_desc + kvt::step_k(kk), v_desc + kvt::step_mn(kk), kvt::idesc(HD, true), t > 0 || kk != 0);
-                tc::mma_commit(&bar_o);
+                if (t != a.withhold || (blockIdx.x | blockIdx.y)) tc::mma_commit(&bar_o);
             }
             __syncwarp();
         }
@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(KVT_LAUNCH, 1) k_kvq_attend_tc(KvqAttnArgs a) 
         } else {
             copies_wait<0>();
         }
-        ok = tc::bar_wait(&bar_s, (uint32_t)(t & 1), &s_abort);
+        ok = tc::bar_wait(&bar_s, (uint32_t)(t & 1), &s_abort, a.wait_ns);
         tc::fence_after();
         const uint32_t live = s_live[t & 3];
         if (t + 1 < ntiles) {
@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(KVT_LAUNCH, 1) k_kvq_attend_tc(KvqAttnArgs a) 
             s_red[part][r] = most;
             over = most * f > base || vtop * unit >= kMost;
         }
-        if (t > 0) ok = tc::bar_wait(&bar_o, (uint32_t)((t - 1) & 1), &s_abort);  // P, V and O are free
+        if (t > 0) ok = tc::bar_wait(&bar_o, (uint32_t)((t - 1) & 1), &s_abort, a.wait_ns);  // P, V and O are free
         if (__syncthreads_or(over || !ok)) {
             if (s_abort) break;
             tc::fence_after();
@@ -607,7 +607,7 @@ __global__ void __launch_bounds__(KVT_LAUNCH, 1) k_kvq_attend_tc(KvqAttnArgs a) 
     }
     float o[OD];
     if (t == ntiles) {
-        ok = tc::bar_wait(&bar_o, (uint32_t)((ntiles - 1) & 1), &s_abort);
+        ok = tc::bar_wait(&bar_o, (uint32_t)((ntiles - 1) & 1), &s_abort, a.wait_ns);
         if (__syncthreads_and(ok)) {
             tc::fence_after();
             kvt::ld(o_at, o);

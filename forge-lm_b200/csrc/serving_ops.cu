@@ -3,12 +3,14 @@
 // arguments and launches; the kernels are in kvq.cuh, kvq_attn.cuh, w4.cuh
 // and logit_controls.cuh.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cmath>
 #include <cstdint>
 #include <mutex>
 #include <set>
 
+#include "../../include/forge_b200_testing.h"
 #include "capi.cuh"
 #include "kvq.cuh"
 #include "kvq_attn.cuh"
@@ -298,6 +300,19 @@ int32_t fb2_kvq_attend_workspace(const fb2_kvq_cache* c, const fb2_kvq_attention
     });
 }
 
+// test hook: what the next launch on tcgen05 tiles withholds
+namespace {
+std::atomic<int> g_withhold_tile{-1};
+std::atomic<int64_t> g_withhold_wait_ns{0};
+}  // namespace
+int32_t fb2_test_kvq_withhold(int32_t tile, int64_t wait_ns) {
+    return guarded([&] {
+        need(tile >= 0 && wait_ns > 0 && wait_ns <= (int64_t)kTcTimeoutNs, "bad hook arguments");
+        g_withhold_wait_ns = wait_ns;
+        g_withhold_tile = tile;
+    });
+}
+
 int32_t fb2_kvq_attend(const fb2_kvq_cache* c, const fb2_kvq_attention* a, void* stream) {
     return guarded([&] {
         const KvqAttnArgs k = attn_args(c, a);
@@ -317,6 +332,8 @@ int32_t fb2_kvq_attend(const fb2_kvq_cache* c, const fb2_kvq_attention* a, void*
             args.part_ml = static_cast<float2*>(a->device_workspace);
             args.part_o = reinterpret_cast<float*>(static_cast<char*>(a->device_workspace) + (parts * 8 + 15) / 16 * 16);
         }
+        args.withhold = k.block_rows == KVT_ROWS ? g_withhold_tile.exchange(-1) : -1;
+        args.wait_ns = args.withhold < 0 ? kTcTimeoutNs : (unsigned long long)g_withhold_wait_ns.load();
         if (c->format == FB2_KVQ_INT8)
             launch_attend<KVQ_INT8>(args, (cudaStream_t)stream);
         else

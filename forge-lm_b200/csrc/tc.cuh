@@ -35,12 +35,12 @@ FB2_DEV bool bar_try(uint64_t* b, uint32_t parity) {
     return ok != 0;
 }
 // Bounded wait for phase `parity` of barrier b; false on expiry or abort.
-FB2_DEV bool bar_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag) {
+FB2_DEV bool bar_wait(uint64_t* b, uint32_t parity, volatile int* abort_flag, unsigned long long limit_ns = kTcTimeoutNs) {
     if (bar_try(b, parity)) return true;
     const unsigned long long t0 = now_ns();
     while (!bar_try(b, parity)) {
         if (*abort_flag) return false;
-        if (now_ns() - t0 > kTcTimeoutNs) {
+        if (now_ns() - t0 > limit_ns) {
             *abort_flag = 1;
             return false;
         }

@@ -332,7 +332,8 @@ int32_t fb2_kvq_read(const fb2_kvq_cache* c, int32_t n_rows, const int32_t* devi
  * brought to a fixed point of 23 bits below the row's largest, and what a row
  * weighs V with is carried in fp16 (for fp32 in two such terms) relative to the
  * row's own largest weight.  Waits inside a kernel are
- * bounded (about a second); rows of a block whose wait ran out are NaN. */
+ * bounded (2 s each, and 2 s more for what is in flight then); rows of a block
+ * whose wait ran out are NaN. */
 typedef struct {
     const void* device_q;  /* [n_rows][n_heads][head_dim], strides below */
     void* device_out;      /* [n_rows][n_heads][head_dim] dense, q's type */

@@ -45,6 +45,14 @@ int32_t fb2_test_mk_trace(struct fb2_session* s, uint64_t* out, int64_t capacity
  * stays usable. */
 int32_t fb2_test_mk_withhold(struct fb2_session* s, int32_t cta, int64_t wait_ns);
 
+/* The same for attention over the quantised cache: in the next fb2_kvq_attend
+ * that runs on tcgen05 tiles (16-bit types, more than 32 rows of a K/V head),
+ * the first block does not announce the end of its MMAs of tile `tile` (of 128
+ * positions), and every wait of the launch gives up after wait_ns (<= 2 s).
+ * The block leaves together and its rows are NaN; a chunk without that tile
+ * is unaffected, and so is the next call. */
+int32_t fb2_test_kvq_withhold(int32_t tile, int64_t wait_ns);
+
 /* Geometry of the session's persistent decode kernel on its first device:
  * CTAs, cluster size and attention CTAs of the head-cluster layout (0 when
  * it uses column strips), and ring stages at one row. */

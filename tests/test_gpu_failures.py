@@ -100,3 +100,41 @@ def test_allocation_failure_on_the_second_device_copy(pkg, O):
         got = be.forward_last(list(range(1, 30)))
     want = O.forward_last(ocfg, params, list(range(1, 30)))
     assert float(np.max(np.abs(got - want) / np.maximum(1.0, np.abs(want)))) <= 1e-3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,dim", [("int8", 64), ("int4", 128)])
+@pytest.mark.parametrize("prefix,max_len,tile", [(300, 512, 0), (300, 512, 1), (300, 512, 2), (1500, 40000, 0), (1500, 40000, 3)])
+def test_attention_whose_wait_runs_out(pkg, fmt, dim, prefix, max_len, tile):
+    """A block of the tcgen05 attention whose MMAs are not announced gives NaN rows
+    after its limit, for the first tile, one between and the last, with one chunk of
+    positions and with several; other blocks and the next call are right."""
+    torch = pytest.importorskip("torch")
+    from forge_lm_b200 import _native as N
+    L = N.load()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    pages = -(-max_len // 64)
+    cache = pkg.QuantKvCache.empty(pages, 64, 2, dim, fmt)
+    total = min(max_len, 2048)
+    k = torch.randn((total, 2, dim), device="cuda", generator=g)
+    cache.write(k, k.flip(0), torch.arange(total, dtype=torch.int32, device="cuda"))
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    q = torch.randn((40, 4, dim), device="cuda", generator=g).bfloat16()
+    args = (q, table, torch.tensor([prefix], dtype=torch.int32, device="cuda"))
+    kw = dict(starts=torch.tensor([0, 40], dtype=torch.int32, device="cuda"), max_nodes=40, max_len=max_len)
+    want = cache.attend(*args, **kw)
+    assert torch.isfinite(want[0]).all()
+    N.check(L.fb2_test_kvq_withhold(tile, 20_000_000))
+    out, lse = cache.attend(*args, **kw)
+    # block 0: the first K/V head's rows (heads 0 and 1)
+    assert out[:, :2].isnan().all() and lse[:, :2].isnan().all()
+    assert torch.equal(out[:, 2:], want[0][:, 2:]) and torch.equal(lse[:, 2:], want[1][:, 2:])
+    again = cache.attend(*args, **kw)
+    assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
+
+
+def test_withhold_hook_checks_its_arguments(pkg):
+    from forge_lm_b200 import _native as N
+    L = N.load()
+    for tile, wait in ((-1, 1000), (0, 0), (0, 3_000_000_000)):
+        assert L.fb2_test_kvq_withhold(tile, wait) == N.FB2_INVALID_ARG
