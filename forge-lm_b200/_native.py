@@ -141,7 +141,7 @@ def load(path: str | None = None):
     L.fb2_tokenizer_info.argtypes = [vp, C.POINTER(i32), C.POINTER(i32)]
     L.fb2_tokenizer_encode.argtypes = [vp, vp, i64, vp, i64, C.POINTER(i64)]
     L.fb2_tokenizer_decode.argtypes = [vp, vp, i64, vp, i64, C.POINTER(i64)]
-    # the serving operators' structs are passed as packed bytes (serving.py)
+    # the serving operators' structs are passed as packed bytes (Python programs call them through _serving.so)
     st, i64p = C.c_char_p, C.POINTER(i64)
     L.fb2_kvq_sizes.argtypes = [st, i64p, i64p]
     L.fb2_kvq_write.argtypes = [st, i32, vp, vp, i32, i64, i64, i64, i64, vp, vp]

@@ -125,21 +125,16 @@ FB2_DEV uint4 pack16(const float* x) {
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// 8 values from p (VEC: p is 16-byte aligned).
-template <class T, bool VEC>
+// 8 values from p, 16-byte aligned.
+template <class T>
 FB2_DEV void load8(const T* p, float (&x)[8]) {
-    if constexpr (VEC) {
-        constexpr int N = sizeof(T) / 2;  // 16-byte pieces of 8 values
-        uint4 w[N];
+    constexpr int N = sizeof(T) / 2;  // 16-byte pieces of 8 values
+    uint4 w[N];
 #pragma unroll
-        for (int i = 0; i < N; i++) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-        const T* t = reinterpret_cast<const T*>(w);
+    for (int i = 0; i < N; i++) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    const T* t = reinterpret_cast<const T*>(w);
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = Dense<T>::get(t[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = Dense<T>::get(p[i]);
-    }
+    for (int i = 0; i < 8; i++) x[i] = Dense<T>::get(t[i]);
 }
 // A row is shared by `width` = 1 << `shift` neighbouring lanes of a warp; a
 // lane holds NP pieces of 16 bytes, piece j at index part + width * j, so that

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(128)
 // the rows of x its columns, so a block's 512 bytes (one 16-byte load per
 // lane) go through the tensor cores once for 8 columns.  The codes enter as
 // fp16 or bf16 values that one shift and one logical operation make of four
-// bits; a group's sum and the sum of its x (the same product with ones) then
+// bits; a group's sum and the sum of its x (k_w4_columns adds it up) then
 // give scale * sum(code x) + minimum * sum(x) in fp32:
 //   bf16 x: 128 + code (bit pattern 0x4300 | code);
 //   fp16 x: 1 + code / 16 (0x3c00 | code << 6);
@@ -122,7 +122,6 @@ template <>
 struct Form<__nv_bfloat16> {
     static constexpr bool BF16 = true;
     static constexpr int PARTS = 1;
-    static constexpr uint32_t ONES = 0x3f803f80u;
     static FB2_DEV void codes(uint32_t w, uint32_t (&f)[4]) {
 #pragma unroll
         for (int i = 0; i < 4; i++) f[i] = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
@@ -139,7 +138,6 @@ template <>
 struct Form<__half> {
     static constexpr bool BF16 = false;
     static constexpr int PARTS = 1;
-    static constexpr uint32_t ONES = 0x3c003c00u;
     static FB2_DEV void codes(uint32_t w, uint32_t (&f)[4]) {
         f[0] = ((w << 6) & 0x03c003c0u) | 0x3c003c00u;
         f[1] = ((w << 2) & 0x03c003c0u) | 0x3c003c00u;
@@ -161,7 +159,6 @@ template <>
 struct Form<float> {
     static constexpr bool BF16 = true;
     static constexpr int PARTS = 3;
-    static constexpr uint32_t ONES = 0x3f803f80u;
     static FB2_DEV void codes(uint32_t w, uint32_t (&f)[4]) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -404,10 +401,10 @@ FB2_DEV void w4_digits(const T* __restrict__ x, long long x_row, int row, int di
         const T* p = x + row * x_row + k;
         if (live && vec && k + 16 <= K) {
             float a[8];
-            load8<T, true>(p, a);
+            load8<T>(p, a);
 #pragma unroll
             for (int i = 0; i < 8; i++) v[16 * b + i] = a[i];
-            load8<T, true>(p + 8, a);
+            load8<T>(p + 8, a);
 #pragma unroll
             for (int i = 0; i < 8; i++) v[16 * b + 8 + i] = a[i];
         } else {
