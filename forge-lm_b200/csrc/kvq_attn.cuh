@@ -563,6 +563,8 @@ __global__ void __launch_bounds__(WARPS * 32, KvaShape<HD, FMT, NT, SPLIT, WARPS
             }
         over |= vmax >= vlim;
         if (__any_sync(0xffffffffu, over)) {
+            // a row's own scores and the tile's V decide, not the rows beside it
+            vmax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vmax)));
             uint32_t high = 0;
 #pragma unroll
             for (int n = 0; n < NT; n++) {
@@ -585,7 +587,7 @@ __global__ void __launch_bounds__(WARPS * 32, KvaShape<HD, FMT, NT, SPLIT, WARPS
 #pragma unroll
                     for (int x = 4; x < 32; x *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
                     const uint32_t field = __float_as_uint(unit[n][c]) >> 23, grow = min((uint32_t)fminf(by, 300.f), kUnit - field);
-                    const uint32_t next = min(field + grow, 256u - (__float_as_uint(most) >> 23));
+                    const uint32_t next = rise || vmax * unit[n][c] >= kMost ? min(field + grow, 256u - (__float_as_uint(most) >> 23)) : field;
                     unit[n][c] = __uint_as_float(next << 23);
                     high = max(high, next);
                     beta[c] = exp2_fast((float)(int)(next - field) - by);

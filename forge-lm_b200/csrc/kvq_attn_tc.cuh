@@ -536,7 +536,7 @@ __global__ void __launch_bounds__(KVT_LAUNCH, 1) k_kvq_attend_tc(KvqAttnArgs a) 
             if (busy) {
                 const float most = fmaxf(fmaxf(s_red[0][r], s_red[1][r]), fmaxf(s_red[2][r], s_red[3][r]));
                 const uint32_t field = __float_as_uint(unit) >> 23, grow = min((uint32_t)fminf(by, 300.f), kUnit - field);
-                const uint32_t next = min(field + grow, 256u - (__float_as_uint(most) >> 23));
+                const uint32_t next = rise || vtop * unit >= kMost ? min(field + grow, 256u - (__float_as_uint(most) >> 23)) : field;
                 unit = __uint_as_float(next << 23);
 #pragma unroll
                 for (int i = 0; i < 4; i++) l[i] *= kva::exp2_fast(-by), z[i] *= kva::exp2_fast(-by);

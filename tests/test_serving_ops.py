@@ -767,6 +767,32 @@ def test_cache_without_pages(pkg, dtype, heads):
 
 
 @gpu
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+@pytest.mark.parametrize("dtype,power", [("fp32", 90), ("bf16", 90), ("fp16", 10)])
+@pytest.mark.parametrize("nodes", [2, 30])
+def test_attention_of_large_and_small_queries(pkg, fmt, dtype, power, nodes):
+    """q times a power of two with a scale that takes it back: the same bits; rows of q
+    that are not finite give NaN and leave the others alone."""
+    g = gen(65)
+    cache = filled(pkg, g, 24, 16, 2, 64, fmt)
+    table = torch.arange(24, dtype=torch.int32, device="cuda")[None]
+    q = normal(g, nodes, 4, 64, dtype=DTYPES[dtype])
+    if dtype == "fp16":  # where 2^-10 does not make subnormal numbers of them
+        q = torch.where(q.abs() < 2.0 ** -3, torch.zeros_like(q), q)
+    kw = dict(starts=_i32([0, nodes]), max_nodes=nodes)
+    want = cache.attend(q, table, _i32([200]), scale=0.125, **kw)
+    for p in (power, -power):
+        got = cache.attend(q * 2.0 ** p, table, _i32([200]), scale=0.125 * 2.0 ** -p, **kw)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    q[1, 2, 7], q[0, 0, 63] = math.inf, math.nan
+    got = cache.attend(q, table, _i32([200]), scale=0.125, **kw)
+    bad = torch.zeros((nodes, 4), dtype=torch.bool, device="cuda")
+    bad[1, 2] = bad[0, 0] = True
+    assert got[0][bad].isnan().all() and got[1][bad].isnan().all()
+    assert torch.equal(got[0][~bad], want[0][~bad]) and torch.equal(got[1][~bad], want[1][~bad])
+
+
+@gpu
 def test_attention_bounds_that_cut(pkg):
     """max_len and the page table's width cut what is seen; max_nodes which rows are written."""
     attention_case(pkg, 31, "int8", "fp32", [100, 40], [1, 1], 4, 2, 64, 16, tree=False, max_len=77)
@@ -926,6 +952,14 @@ def test_products_with_4_bit_weights(pkg, dtype, group, rows, k, n):
 @pytest.mark.parametrize("rows,k,n", [(1, 333, 64), (7, 128, 48), (40, 515, 19)])
 def test_products_of_unaligned_rows(pkg, dtype, rows, k, n):
     check_product(pkg, dtype, rows, k, n, 64, bias=False, strided=True)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("rows,k,n,group", [(129, 200, 50, 32), (513, 320, 77, 64), (2050, 130, 33, 128)])
+def test_products_of_a_prompt(pkg, dtype, rows, k, n, group):
+    """Hundreds of rows: many chunks of columns, the last of them not full."""
+    check_product(pkg, dtype, rows, k, n, group)
 
 
 @gpu
@@ -1177,6 +1211,40 @@ def test_operators_in_a_graph(pkg, dtype):
             t.zero_()
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+@pytest.mark.parametrize("dtype,nodes", [("fp32", 3), ("bf16", 3), ("bf16", 40), ("fp16", 40)])
+def test_split_attention_in_a_graph(pkg, fmt, dtype, nodes):
+    """Chunks, their merge and the tcgen05 blocks captured once; replayed over another
+    prefix, other pages and other rows."""
+    g = gen(78)
+    cache = filled(pkg, g, 200, 16, 2, 64, fmt)
+    held = [normal(g, 2 * nodes, 4, 64, dtype=DTYPES[dtype]), _i32([1500, 700]),
+            torch.randperm(200, generator=torch.Generator().manual_seed(9))[:200].to(torch.int32).cuda().view(2, 100)]
+    starts = _i32([0, nodes, 2 * nodes])
+
+    def step(q, prefix, table):
+        return cache.attend(q, table, prefix, starts=starts, max_nodes=nodes, max_len=1600)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*held)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(*held)
+    for lens in ([1500, 700], [3, 1555], [640, 0]):
+        held[0].copy_(normal(g, 2 * nodes, 4, 64, dtype=DTYPES[dtype]))
+        held[1].copy_(_i32(lens))
+        held[2].copy_(held[2].flip(1).clone())
+        want = [t.clone() for t in step(*held)]
+        for t in outs:
+            t.zero_()
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want)) and torch.isfinite(want[1]).all()
 
 
 def _i32(x):
