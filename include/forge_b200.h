@@ -356,7 +356,7 @@ typedef struct {
     int32_t max_len;    /* host bound of prefix_lens[b] + T_b, up to 2^31 - 65536; 0: max_pages * page_size */
     int32_t mask_words; /* at least ceil(max_nodes / 32) with a mask */
     float scale;        /* finite */
-    int32_t fill_rest;  /* not 0: rows that belong to no sequence are written too */
+    int32_t fill_rest;  /* not 0: rows that belong to no sequence are written too (n_seqs up to 65534) */
 } fb2_kvq_attention;
 int32_t fb2_kvq_attend_workspace(const fb2_kvq_cache* c, const fb2_kvq_attention* a, int64_t* bytes);
 int32_t fb2_kvq_attend(const fb2_kvq_cache* c, const fb2_kvq_attention* a, void* cuda_stream);
@@ -395,7 +395,8 @@ int32_t fb2_w4_pack(const fb2_w4_linear* w, const void* device_w, int32_t dtype,
  * 8 of fp32) x is first brought to a fixed point of 23 (31) bits below its
  * largest |x| in each run of 128 inputs.  Rows of x and y are x_row_stride / y_row_stride
  * elements apart.  A row of x with a non-finite element gives a non-finite
- * row of y.  device_workspace: fb2_w4_matvec_workspace bytes, 16-byte aligned. */
+ * row of y, and so may one of bf16 whose values reach 2^114 (group sums of
+ * 143 |x| have to be finite).  device_workspace: fb2_w4_matvec_workspace bytes, 16-byte aligned. */
 int32_t fb2_w4_matvec_workspace(const fb2_w4_linear* w, int32_t n_rows, int32_t dtype, int64_t* bytes);
 int32_t fb2_w4_matvec(const fb2_w4_linear* w, int32_t n_rows, const void* device_x, int64_t x_row_stride, void* device_y,
                       int64_t y_row_stride, int32_t dtype, void* device_workspace, int64_t workspace_bytes,
