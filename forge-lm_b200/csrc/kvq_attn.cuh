@@ -261,13 +261,16 @@ __global__ void __launch_bounds__(WARPS * 32, KvaShape<HD, FMT, NT, SPLIT, WARPS
         ids = page < n_pages ? (((page * a.c.heads + head) * 2) << (a.c.page_shift - 3)) + ((pos & (ps - 1)) >> 3) : 0;
     };
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * S::DEPTH * S::SLOT;
-    constexpr int UNITS = S::RB / 2, COPIES = (2 * UNITS + 31) / 32;  // 16-byte units of 8 rows; a lane's of a group
+    // 16-byte units of 8 rows; a lane's of a group: of K, then as many of V, or (16
+    // units) the lower lanes of K and the others of V
+    constexpr int UNITS = S::RB / 2, KINDS = UNITS >= 32 ? 2 : 1, COPIES = 2 * UNITS / 32 / KINDS;
     const unsigned char* copy_from[COPIES];
     uint32_t copy_to[COPIES];
+    const uint32_t v_from = ps * S::RB;  // where V lies after K
 #pragma unroll
     for (int i = 0; i < COPIES; i++) {
         const uint32_t u = 32 * i + lane, kind = u / UNITS, at = u % UNITS;
-        copy_from[i] = a.c.codes + kind * (ps * S::RB) + at * 16;
+        copy_from[i] = a.c.codes + kind * v_from + at * 16;
         copy_to[i] = kind * (8 * S::RB) + S::place(at) * 16;
     }
     const uint32_t* meta_from = a.c.meta + ((lane >> 1) & 1) * ps + (lane & 1) * 4;
@@ -284,10 +287,13 @@ __global__ void __launch_bounds__(WARPS * 32, KvaShape<HD, FMT, NT, SPLIT, WARPS
             const bool there = (live >> j) & 1;
             if (all) {
 #pragma unroll
-                for (int i = 0; i < COPIES; i++) copy16(to + copy_to[i] + j * S::GROUP, copy_from[i] + skip);
+                for (int i = 0; i < COPIES * KINDS; i++)
+                    copy16(to + copy_to[i % COPIES] + j * S::GROUP + i / COPIES * (8 * S::RB), copy_from[i % COPIES] + skip + i / COPIES * v_from);
             } else if (hd == HD) {
 #pragma unroll
-                for (int i = 0; i < COPIES; i++) copy16(to + copy_to[i] + j * S::GROUP, copy_from[i] + skip, there);
+                for (int i = 0; i < COPIES * KINDS; i++)
+                    copy16(to + copy_to[i % COPIES] + j * S::GROUP + i / COPIES * (8 * S::RB), copy_from[i % COPIES] + skip + i / COPIES * v_from,
+                           there);
             } else {
                 // rows shorter than in shared memory: two lanes to a row
                 const int row = lane >> 1, kind = row >> 3, r = row & 7;
