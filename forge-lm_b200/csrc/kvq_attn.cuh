@@ -171,14 +171,14 @@ FB2_DEV float exp2_fast(float x) {
 // stays in floating point, scaled together with the V scales: one fp16 term for
 // the 16-bit types, whose results have no more bits (a second one brings the error
 // of fp16 against 64 bits from 2.8e-4 to 2.1e-4, its rounding alone, and takes 279
-// us for 258 on the long sequences below, 15.3 for 14.4 on the short ones); two for
+// us for 258 on the long sequences below, 15.3 for 14.4 on the short ones in fp16); two for
 // fp32, whose sums over a tile start at zero and are added to the running ones.
 //
 // What bounds it: with many long sequences the instructions that make operands
 // of the codes and probabilities of the scores (16 sequences of 40 to 65 K int4
-// positions, 32 heads on 8 of 128, fp16: 257 us, 3.6 TB/s; 32 sequences of up to
-// 1023 int8 positions, 12 heads of 64, fp32: 15.0 us, 1.9 TB/s); with few the
-// chain from a launch over the page table to the merge (one of 576: 7.3 us).
+// positions, 32 heads on 8 of 128, fp16: 259 us, 3.5 TB/s; 32 sequences of up to
+// 1023 int8 positions, 12 heads of 64, fp32: 15.1 us, 1.9 TB/s); with few the
+// chain from a launch over the page table to the merge (one of 576: 7.6 us).
 template <int HD, int FMT, int NT, bool SPLIT, int WARPS>
 struct KvaShape {
     static constexpr int MT = HD > 128 ? 1 : 2;       // 16-position groups of a tile
@@ -411,9 +411,9 @@ __global__ void __launch_bounds__(WARPS * 32, KvaShape<HD, FMT, NT, SPLIT, WARPS
     // when V scale * unit, the most that a weight can be, reaches kMost; so fp16
     // holds every weight, with at least 16 bits below the row's largest, whatever
     // other rows or masked positions have.  (One unit for all rows, by the tile's
-    // largest V scale: 255.9 us for 257.4 on the long sequences, 66.7 for 69.0 over 32
-    // of 1000 to 9000, 12 heads of 64 in bf16; but a V row 2^20 times the others,
-    // seen or not, left the others' weights 4 bits.)  o is in units of 1 / unit.
+    // largest V scale: 256 us for 259 on the long sequences, 14.4 for 15.1 on the short
+    // ones; but a V row 2^20 times the others, seen or not, left the others' weights
+    // 4 bits.)  o is in units of 1 / unit.
     constexpr float kLag = 9.f, kMost = 32768.f, kNone = -3.402823466e38f;  // kNone: nothing seen yet
     constexpr uint32_t kUnit = 241;  // exponent field of the largest unit
     float vlim = kMost * __uint_as_float((254u - kUnit) << 23);  // kMost / the lane's largest unit

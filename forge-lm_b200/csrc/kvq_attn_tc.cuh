@@ -9,7 +9,7 @@
 // a tile, 0.5 us at 16 a clock) comes in the steps below, one after another: some
 // 3.2 us a tile of 128 positions, in which neither the tensor pipe nor the issue
 // slots are busy.  4 trees of 23 to 64 tokens over 9 to 33 K int8 positions, 32 heads on 8 of
-// 128, bf16: 255 us, 197 TFLOP/s (450 on mma.sync tiles).
+// 128, bf16: 254 us, 198 TFLOP/s (450 on mma.sync tiles).
 //
 // 512 threads of a CTA take one chunk of a sequence's positions, one K/V head
 // and 128 rows; row r is TMEM lane r; warps w, w + 4, w + 8, w + 12 read lane
@@ -536,7 +536,7 @@ __global__ void __launch_bounds__(KVT_LAUNCH, 1) k_kvq_attend_tc(KvqAttnArgs a) 
             if (busy) {
                 const float most = fmaxf(fmaxf(s_red[0][r], s_red[1][r]), fmaxf(s_red[2][r], s_red[3][r]));
                 const uint32_t field = __float_as_uint(unit) >> 23, grow = min((uint32_t)fminf(by, 300.f), kUnit - field);
-                const uint32_t next = rise || vtop * unit >= kMost ? min(field + grow, 256u - (__float_as_uint(most) >> 23)) : field;
+                const uint32_t next = by > 0.f || vtop * unit >= kMost ? min(field + grow, 256u - (__float_as_uint(most) >> 23)) : field;
                 unit = __uint_as_float(next << 23);
 #pragma unroll
                 for (int i = 0; i < 4; i++) l[i] *= kva::exp2_fast(-by), z[i] *= kva::exp2_fast(-by);
