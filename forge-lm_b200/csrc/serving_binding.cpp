@@ -17,6 +17,8 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -48,6 +50,18 @@ void status(int32_t s) {
 // Tells autograd and whoever else counts versions that a call changed t.
 void changed(const at::Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+bool needs_gradient(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+// A result of `from`: no gradient is computed, and a backward pass that comes
+// to it says so instead of stopping there.
+PyObject* result(at::Tensor t, const at::Tensor& from, const char* call) {
+    if (needs_gradient(from)) {
+        const auto node = std::make_shared<torch::autograd::Error>(std::string(call) + " computes no gradient",
+                                                                   torch::autograd::collect_next_edges(from));
+        torch::autograd::set_history(t, node);
+    }
+    return THPVariable_Wrap(std::move(t));
 }
 
 // Python errors for what `f` throws
@@ -307,7 +321,7 @@ PyObject* cache_attend(PyObject*, PyObject* const* args, Py_ssize_t count) {
         a.fill_rest = starts && seqs > 0 && seqs <= 65534;
         if (starts && !a.fill_rest) out.zero_(), lse.fill_(-INFINITY);
         status(fb2_kvq_attend(&c, &a, on.stream()));
-        return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(lse)));
+        return Py_BuildValue("(NN)", result(std::move(out), q, "QuantKvCache.attend"), result(std::move(lse), q, "QuantKvCache.attend"));
     });
 }
 
@@ -397,7 +411,7 @@ PyObject* linear_call(PyObject*, PyObject* const* args, Py_ssize_t count) {
         if (size) work = empty({size}, at::kByte, h.index);
         status(fb2_w4_matvec(&l, rows, flat.data_ptr(), flat.stride(0), y.data_ptr(), n, code, size ? work.data_ptr() : nullptr,
                              size, on.stream()));
-        return THPVariable_Wrap(std::move(y));
+        return result(std::move(y), x, "W4Linear");
     });
 }
 
@@ -444,6 +458,7 @@ PyObject* controls(PyObject*, PyObject* const* args, Py_ssize_t count) {
         OnDevice on(index);
         at::Tensor fresh;
         const at::Tensor* out = args[11] == Py_None ? nullptr : &tensor(args[11], "out");
+        need(!out || !(needs_gradient(logits) || needs_gradient(*out)), "out= goes without gradients: detach() or no_grad()");
         if (out)
             need(out->sizes() == logits.sizes() && out->scalar_type() == logits.scalar_type() && out->is_cuda() &&
                      out->get_device() == index && (out->stride(1) == 1 || vocab <= 1),
@@ -469,7 +484,7 @@ PyObject* controls(PyObject*, PyObject* const* args, Py_ssize_t count) {
         c.n_rows = small(rows, "rows");
         c.vocab = small(vocab, "vocab");
         if (rows && vocab) status(fb2_logit_controls(&c, on.stream()));
-        if (fresh.defined()) return THPVariable_Wrap(std::move(fresh));
+        if (fresh.defined()) return result(std::move(fresh), logits, "logit_controls");
         changed(*out);
         return Py_NewRef(args[11]);
     });

@@ -5,7 +5,9 @@ and penalties, biases and grammar masks on logits.
 
 Every call runs the library's kernels on torch's current stream of the
 tensors' device and returns without waiting.  Results and workspaces come from
-torch's allocator.  Nothing here records gradients.  Wrong shapes, types or
+torch's allocator.  Nothing here computes gradients: a backward pass that comes
+to the result of an input that requires one raises (out= refuses such inputs;
+what is written to a cache or packed is its values).  Wrong shapes, types or
 devices raise ArgumentError before anything is launched.  The checks and calls
 are compiled (csrc/serving_binding.cpp).
 """

@@ -1364,6 +1364,38 @@ def test_buffers_that_are_replaced(pkg):
 
 
 @gpu
+def test_gradients_are_not_cut_in_silence(pkg):
+    """A backward pass through a result of an input that requires a gradient raises."""
+    g = gen(83)
+    cache = filled(pkg, g, 4, 16, 2, 64, "int8")
+    linear = random_linear(pkg, g, 64, 48, 64, True)
+    x, q, logits = normal(g, 2, 64), normal(g, 1, 4, 64), normal(g, 2, 32)
+    calls = ((x, lambda t: linear(t)), (x, lambda t: linear(t.view(1, 2, 64))), (logits, lambda t: pkg.logit_controls(t)),
+             (q, lambda t: cache.attend(t, _i32([[0, 1]]), _i32([20]))[0]), (q, lambda t: cache.attend(t, _i32([[0, 1]]), _i32([20]))[1]))
+    for value, call in calls:
+        plain = call(value)
+        assert not plain.requires_grad
+        tracked = value.clone().requires_grad_()
+        with torch.no_grad():
+            assert not call(tracked).requires_grad
+        got = call(tracked)
+        assert torch.equal(got, plain)
+        other = torch.ones((), device="cuda", requires_grad=True)
+        with pytest.raises(RuntimeError, match="computes no gradient"):
+            (got.sum() * other).backward()
+        assert tracked.grad is None
+    tracked = logits.clone().requires_grad_()
+    with pytest.raises(pkg.ArgumentError):
+        pkg.logit_controls(tracked, out=torch.empty_like(logits))
+    with torch.no_grad():
+        pkg.logit_controls(tracked, out=torch.empty_like(logits))
+    # values are stored and packed whether they require a gradient or not
+    k = normal(g, 1, 2, 64).requires_grad_()
+    cache.write(k, k, _i32([5]))
+    pkg.W4Linear.pack(torch.nn.Parameter(normal(g, 64, 16)), 32)
+
+
+@gpu
 def test_changed_tensors_are_counted(pkg):
     """What a call writes into has a new version: autograd refuses to use a stale value."""
     cache = pkg.QuantKvCache.empty(2, 16, 1, 32)
