@@ -24,12 +24,13 @@ import numpy as np
 from . import _native as N
 from ._native import ArgumentError, InvalidDataError, NativeError
 from .dotnet_random import DotNetRandom
-from .serving import QuantKvCache, W4Linear, logit_controls
+from .serving import (PageTable, QuantKvCache, W4Linear, W8Linear, logit_controls, quantise_rows, residual_norm,
+                      verify_drafts)
 
 __all__ = ["ModelConfig", "B200Backend", "Sampler", "DotNetRandom", "ArgumentError", "NativeError",
            "InvalidDataError", "param_names", "param_shapes", "init_params", "device_count", "library_path",
            "read_forgemodel_header", "write_forgemodel", "BpeTokenizer", "QuantKvCache",
-           "W4Linear", "logit_controls"]
+           "W4Linear", "logit_controls", "PageTable", "W8Linear", "quantise_rows", "residual_norm", "verify_drafts"]
 
 
 def library_path() -> str:

@@ -53,16 +53,20 @@ void changed(const at::Tensor& t) {
 }
 
 bool needs_gradient(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
-// A result of `from`: no gradient is computed, and a backward pass that comes
-// to it says so instead of stopping there.
-PyObject* result(at::Tensor t, const at::Tensor& from, const char* call) {
-    if (needs_gradient(from)) {
+// A result of `from` (null: not given): no gradient is computed, and a backward
+// pass that comes to it says so instead of stopping there.
+PyObject* result(at::Tensor t, std::initializer_list<const at::Tensor*> from, const char* call) {
+    torch::autograd::variable_list inputs;
+    for (const at::Tensor* i : from)
+        if (i && needs_gradient(*i)) inputs.push_back(*i);
+    if (!inputs.empty()) {
         const auto node = std::make_shared<torch::autograd::Error>(std::string(call) + " computes no gradient",
-                                                                   torch::autograd::collect_next_edges(from));
+                                                                   torch::autograd::collect_next_edges(inputs));
         torch::autograd::set_history(t, node);
     }
     return THPVariable_Wrap(std::move(t));
 }
+PyObject* result(at::Tensor t, const at::Tensor& from, const char* call) { return result(std::move(t), {&from}, call); }
 
 // Python errors for what `f` throws
 template <class F>
@@ -104,6 +108,10 @@ const at::Tensor* plain(PyObject* o, const char* name, at::ScalarType type, int 
     if (t.scalar_type() != type || !t.is_cuda() || t.get_device() != index || !t.is_contiguous())
         refuse(std::string(name) + " must be a contiguous " + c10::toString(type) + " tensor on cuda:" + std::to_string(index));
     return &t;
+}
+const at::Tensor* given(const at::Tensor* t, const char* name) {
+    if (!t) refuse(std::string(name) + " must be a tensor");
+    return t;
 }
 template <class T>
 T* data(const at::Tensor* t) {
@@ -490,6 +498,358 @@ PyObject* controls(PyObject*, PyObject* const* args, Py_ssize_t count) {
     });
 }
 
+// ---- pages of sequences ---------------------------------------------------------------
+
+struct Pages {
+    static constexpr const char* kName = "forge_b200.pages";
+    at::Tensor table, lens, free, n_free;
+    fb2_pages p{};
+    int index = 0;
+    fb2_pages now() const {
+        check_held(table, at::kInt, 4ll * p.n_seqs * p.max_pages, index, "table");
+        check_held(lens, at::kInt, 4ll * p.n_seqs, index, "lens");
+        check_held(free, at::kInt, 4ll * p.n_pages, index, "free");
+        check_held(n_free, at::kInt, 4, index, "n_free");
+        fb2_pages n = p;
+        n.device_table = static_cast<int32_t*>(table.data_ptr());
+        n.device_lens = static_cast<int32_t*>(lens.data_ptr());
+        n.device_free = static_cast<int32_t*>(free.data_ptr());
+        n.device_n_free = static_cast<int32_t*>(n_free.data_ptr());
+        return n;
+    }
+};
+
+PyObject* pages_new(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    ARGS(5)  // table, lens, free, n_free, page_size
+    return guarded([&] {
+        auto h = std::make_unique<Pages>();
+        h->table = tensor(args[0], "table");
+        need(h->table.is_cuda() && h->table.dim() == 2, "table must be a CUDA int32 tensor [sequences, pages]");
+        h->index = h->table.get_device();
+        plain(args[0], "table", at::kInt, h->index);
+        h->lens = *given(plain(args[1], "lens", at::kInt, h->index), "lens");
+        h->free = *given(plain(args[2], "free", at::kInt, h->index), "free");
+        h->n_free = *given(plain(args[3], "n_free", at::kInt, h->index), "n_free");
+        need(h->lens.numel() == h->table.size(0), "lens must have one entry per sequence");
+        need(h->n_free.numel() == 1, "n_free must have one entry");
+        h->p.n_seqs = small(h->table.size(0), "sequences");
+        h->p.max_pages = small(h->table.size(1), "pages of a sequence");
+        h->p.n_pages = small(h->free.numel(), "pages");
+        h->p.page_size = small(integer(args[4], "page_size"), "page_size");
+        h->p.table_stride = h->p.max_pages;
+        const fb2_pages p = h->now();
+        status(fb2_pages_check(&p));
+        return capsule(std::move(h));
+    });
+}
+
+PyObject* pages_extend(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    ARGS(3)  // handle, counts, max_rows
+    return guarded([&]() -> PyObject* {
+        const Pages& h = handle<Pages>(args[0]);
+        const at::Tensor* counts = given(plain(args[1], "counts", at::kInt, h.index), "counts");
+        need(counts->numel() == h.p.n_seqs, "counts must have one entry per sequence");
+        const int32_t rows = small(integer(args[2], "max_rows"), "max_rows");
+        need(rows >= 0, "max_rows must not be negative");
+        const fb2_pages p = h.now();
+        OnDevice on(h.index);
+        at::Tensor starts = empty({(int64_t)p.n_seqs + 1}, at::kInt, h.index), prefix = empty({p.n_seqs}, at::kInt, h.index);
+        at::Tensor slots = empty({rows}, at::kInt, h.index), positions = empty({rows}, at::kInt, h.index);
+        status(fb2_pages_extend(&p, data<int32_t>(counts), rows, data<int32_t>(&starts), data<int32_t>(&prefix), data<int32_t>(&slots),
+                                data<int32_t>(&positions), on.stream()));
+        changed(h.table), changed(h.lens), changed(h.n_free);
+        return Py_BuildValue("(NNNN)", THPVariable_Wrap(std::move(starts)), THPVariable_Wrap(std::move(prefix)),
+                             THPVariable_Wrap(std::move(slots)), THPVariable_Wrap(std::move(positions)));
+    });
+}
+
+PyObject* pages_truncate(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    ARGS(2)  // handle, lens
+    return guarded([&]() -> PyObject* {
+        const Pages& h = handle<Pages>(args[0]);
+        const at::Tensor* lens = given(plain(args[1], "lens", at::kInt, h.index), "lens");
+        need(lens->numel() == h.p.n_seqs, "lens must have one entry per sequence");
+        const fb2_pages p = h.now();
+        OnDevice on(h.index);
+        status(fb2_pages_truncate(&p, data<int32_t>(lens), on.stream()));
+        changed(h.table), changed(h.lens), changed(h.free), changed(h.n_free);
+        Py_RETURN_NONE;
+    });
+}
+
+// ---- residual stream and norms -----------------------------------------------------------
+
+// A tensor [rows, dim] on a device with contiguous rows, of one of two types
+const at::Tensor& matrix(PyObject* o, const char* name, int64_t rows, int64_t dim, int index) {
+    const at::Tensor& t = tensor(o, name);
+    if (t.dim() != 2 || t.size(0) != rows || t.size(1) != dim || !t.is_cuda() || t.get_device() != index || (t.stride(1) != 1 && dim > 1))
+        refuse(std::string(name) + " must be [" + std::to_string(rows) + ", " + std::to_string(dim) + "] on cuda:" + std::to_string(index) +
+               " with contiguous rows");
+    return t;
+}
+// rows of codes that begin on 16 bytes
+at::Tensor empty_codes(int64_t rows, int64_t dim, int index) {
+    return empty({rows, (dim + 15) / 16 * 16}, at::kChar, index).narrow(1, 0, dim);
+}
+
+PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    // h, x, weight, bias, post_weight, post_bias, gate, scale, kind, eps, quantise, dtype
+    ARGS(12)
+    return guarded([&]() -> PyObject* {
+        const at::Tensor& x = tensor(args[1], "x");
+        need(x.dim() == 2 && x.is_cuda(), "x must be a CUDA tensor [rows, dim]");
+        const int index = x.get_device();
+        const int64_t rows = x.size(0), dim = x.size(1);
+        matrix(args[1], "x", rows, dim, index);
+        const at::Tensor* h = args[0] == Py_None ? nullptr : &matrix(args[0], "h", rows, dim, index);
+        fb2_norm n{};
+        at::ScalarType type = h ? h->scalar_type() : x.scalar_type();
+        if (args[11] != Py_None) {
+            need(THPDtype_Check(args[11]), "dtype must be a torch dtype");
+            const at::ScalarType asked = reinterpret_cast<THPDtype*>(args[11])->scalar_type;
+            need(!h || asked == type, "dtype must be h's");
+            type = asked;
+        }
+        n.dtype = code_of(type);
+        n.stream_dtype = code_of(x.scalar_type());
+        need(n.stream_dtype == n.dtype || n.stream_dtype == FB2_F32, "x must have the result's dtype or be float32");
+        const char* names[4] = {"weight", "bias", "post_weight", "post_bias"};
+        const at::Tensor* w[4];
+        for (int i = 0; i < 4; i++) {
+            w[i] = plain(args[2 + i], names[i], at::kFloat, index);
+            if (w[i] && w[i]->numel() != dim) refuse(std::string(names[i]) + " must have one entry per column");
+        }
+        need(w[0], "weight must be a tensor");
+        const at::Tensor* gate = args[6] == Py_None ? nullptr : &tensor(args[6], "gate");
+        if (gate) {
+            need(h && gate->scalar_type() == type, "gate goes with h and has its dtype");
+            if (gate->dim() == 1) {
+                need(gate->size(0) == dim && gate->is_cuda() && gate->get_device() == index && (gate->stride(0) == 1 || dim <= 1),
+                     "gate must be [dim] or [rows, dim] on x's device with contiguous rows");
+            } else {
+                matrix(args[6], "gate", rows, dim, index);
+                n.gate_row_stride = gate->stride(0);
+            }
+        }
+        n.scale = (float)PyFloat_AsDouble(args[7]);
+        if (PyErr_Occurred()) throw Raised{};
+        n.kind = (int32_t)integer(args[8], "kind");
+        n.eps = (float)PyFloat_AsDouble(args[9]);
+        if (PyErr_Occurred()) throw Raised{};
+        const int quantise = PyObject_IsTrue(args[10]);
+        if (quantise < 0) throw Raised{};
+        OnDevice on(index);
+        at::Tensor sum, y, codes, scales;
+        if (h) sum = empty({rows, dim}, x.scalar_type(), index);
+        if (quantise)
+            codes = empty_codes(rows, dim, index), scales = empty({rows}, at::kFloat, index);
+        else
+            y = empty({rows, dim}, type, index);
+        n.device_h = data<void>(h);
+        n.device_x = x.data_ptr();
+        n.device_gate = data<void>(gate);
+        n.device_weight = data<float>(w[0]);
+        n.device_bias = data<float>(w[1]);
+        n.device_post_weight = data<float>(w[2]);
+        n.device_post_bias = data<float>(w[3]);
+        n.device_sum = h ? sum.data_ptr() : nullptr;
+        n.device_y = quantise ? nullptr : y.data_ptr();
+        n.device_codes = quantise ? codes.data_ptr() : nullptr;
+        n.device_scales = quantise ? static_cast<float*>(scales.data_ptr()) : nullptr;
+        n.h_row_stride = h ? h->stride(0) : 0;
+        n.x_row_stride = x.stride(0);
+        n.sum_row_stride = n.y_row_stride = dim;
+        n.code_row_stride = (dim + 15) / 16 * 16;
+        n.n_rows = small(rows, "rows");
+        n.dim = small(dim, "dim");
+        if (rows) status(fb2_residual_norm(&n, on.stream()));
+        const auto from = {h, &x, gate, w[0], w[1], w[2], w[3]};
+        const char* call = "residual_norm";
+        PyObject* first = h ? result(std::move(sum), {h, &x, gate, w[2], w[3]}, call) : Py_NewRef(args[1]);
+        if (!quantise) return Py_BuildValue("(NN)", first, result(std::move(y), from, call));
+        return Py_BuildValue("(NNN)", first, THPVariable_Wrap(std::move(codes)), result(std::move(scales), from, call));
+    });
+}
+
+// ---- 8-bit linear layers ------------------------------------------------------------------
+
+struct Linear8 {
+    static constexpr const char* kName = "forge_b200.linear8";
+    at::Tensor codes, scales, bias;
+    fb2_w8_linear w{};
+    int index = 0;
+    fb2_w8_linear now() const {
+        if (codes.scalar_type() != at::kChar || !codes.is_cuda() || codes.get_device() != index || codes.dim() != 2 ||
+            codes.size(0) != w.out_features || codes.size(1) != w.in_features || codes.stride(0) != w.code_row_stride ||
+            (codes.stride(1) != 1 && w.in_features > 1))
+            refuse("codes was given another size, type, layout or device since the object was made");
+        check_held(scales, at::kFloat, 4ll * w.out_features, index, "scales");
+        fb2_w8_linear n = w;
+        n.device_codes = codes.data_ptr();
+        n.device_scales = static_cast<const float*>(scales.data_ptr());
+        if (bias.defined()) {
+            check_held(bias, at::kFloat, 4ll * w.out_features, index, "bias");
+            n.device_bias = static_cast<const float*>(bias.data_ptr());
+        }
+        return n;
+    }
+};
+
+PyObject* linear8_new(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    ARGS(3)  // codes, scales, bias
+    return guarded([&] {
+        auto h = std::make_unique<Linear8>();
+        h->codes = tensor(args[0], "codes");
+        need(h->codes.is_cuda() && h->codes.dim() == 2 && h->codes.scalar_type() == at::kChar &&
+                 (h->codes.stride(1) == 1 || h->codes.size(1) == 1),
+             "codes must be a CUDA int8 tensor [out, in] with contiguous rows");
+        h->index = h->codes.get_device();
+        h->scales = *given(plain(args[1], "scales", at::kFloat, h->index), "scales");
+        if (const at::Tensor* b = plain(args[2], "bias", at::kFloat, h->index)) h->bias = *b;
+        h->w.out_features = small(h->codes.size(0), "out_features");
+        h->w.in_features = small(h->codes.size(1), "in_features");
+        h->w.code_row_stride = h->codes.stride(0);
+        need(h->scales.numel() == h->w.out_features, "scales must have one entry per output");
+        need(!h->bias.defined() || h->bias.numel() == h->w.out_features, "bias must have one entry per output");
+        const fb2_w8_linear w = h->now();
+        status(fb2_w8_check(&w));
+        return capsule(std::move(h));
+    });
+}
+
+PyObject* linear8_pack(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    ARGS(2)  // handle, w
+    return guarded([&]() -> PyObject* {
+        const Linear8& h = handle<Linear8>(args[0]);
+        const at::Tensor& w = tensor(args[1], "w");
+        need(w.dim() == 2 && w.is_cuda() && w.get_device() == h.index && w.size(0) == h.w.in_features && w.size(1) == h.w.out_features &&
+                 (w.stride(1) == 1 || w.size(1) == 1),
+             "w must be a CUDA tensor [in, out] with contiguous rows");
+        const int32_t code = code_of(w.scalar_type());
+        const fb2_w8_linear l = h.now();
+        OnDevice on(h.index);
+        const int64_t row = w.size(0) > 1 ? w.stride(0) : w.size(1);  // one row may have any stride
+        status(fb2_w8_pack(&l, w.data_ptr(), code, row, on.stream()));
+        changed(h.codes), changed(h.scales);
+        Py_RETURN_NONE;
+    });
+}
+
+// codes and scales of the rows of x
+void quantised(const at::Tensor& x, int64_t rows, int64_t dim, int index, at::Tensor& codes, at::Tensor& scales, void* stream) {
+    const int32_t code = code_of(x.scalar_type());
+    codes = empty_codes(rows, dim, index), scales = empty({rows}, at::kFloat, index);
+    if (rows)
+        status(fb2_quantise_rows(small(rows, "rows"), small(dim, "columns"), x.data_ptr(), code, x.stride(0), codes.data_ptr(), codes.stride(0),
+                                 static_cast<float*>(scales.data_ptr()), stream));
+}
+
+PyObject* quantise_rows(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    ARGS(1)  // x
+    return guarded([&]() -> PyObject* {
+        const at::Tensor& x = tensor(args[0], "x");
+        need(x.dim() == 2 && x.is_cuda() && x.size(1) > 0, "x must be a CUDA tensor [rows, columns]");
+        matrix(args[0], "x", x.size(0), x.size(1), x.get_device());
+        OnDevice on(x.get_device());
+        at::Tensor codes, scales;
+        quantised(x, x.size(0), x.size(1), on.index, codes, scales, on.stream());
+        return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(codes)), result(std::move(scales), x, "quantise_rows"));
+    });
+}
+
+PyObject* linear8_call(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    ARGS(4)  // handle, x, scales, dtype
+    return guarded([&]() -> PyObject* {
+        const Linear8& h = handle<Linear8>(args[0]);
+        const at::Tensor& x = tensor(args[1], "x");
+        const int64_t k = h.w.in_features, n = h.w.out_features;
+        if (x.dim() == 0 || x.size(-1) != k || !x.is_cuda() || x.get_device() != h.index)
+            refuse("x must be [..., " + std::to_string(k) + "] on cuda:" + std::to_string(h.index));
+        const bool coded = x.scalar_type() == at::kChar;
+        need(coded == (args[2] != Py_None), "codes (int8) go with scales, values without");
+        need(args[3] == Py_None || THPDtype_Check(args[3]), "dtype must be a torch dtype");
+        const at::ScalarType type = args[3] != Py_None ? reinterpret_cast<THPDtype*>(args[3])->scalar_type : coded ? at::kFloat : x.scalar_type();
+        const int32_t code = code_of(type);
+        at::Tensor other;
+        if (x.dim() != 2) other = x.reshape({-1, k});
+        const at::Tensor& flat = x.dim() == 2 ? x : other;
+        need(flat.stride(1) == 1 || k == 1, "x must have a contiguous last dimension");
+        const int64_t rows = flat.size(0);
+        const at::Tensor* given_scales = coded ? given(plain(args[2], "scales", at::kFloat, h.index), "scales") : nullptr;
+        need(!coded || given_scales->numel() == rows, "scales must have one entry per row");
+        c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
+        shape.back() = n;
+        const fb2_w8_linear l = h.now();
+        OnDevice on(h.index);
+        at::Tensor codes, scales;
+        if (!coded)
+            quantised(flat, rows, k, h.index, codes, scales, on.stream());
+        else if (reinterpret_cast<uintptr_t>(flat.data_ptr()) % 16 || (rows > 1 && (flat.stride(0) % 16 || flat.stride(0) < k)))
+            codes = empty_codes(rows, k, h.index).copy_(flat);  // the kernels' copies begin on 16 bytes
+        const at::Tensor& c = codes.defined() ? codes : flat;
+        at::Tensor y = empty(shape, type, h.index);
+        status(fb2_w8_matmul(&l, small(rows, "rows"), c.data_ptr(), c.stride(0),
+                             static_cast<const float*>((coded ? *given_scales : scales).data_ptr()), y.data_ptr(), n, code, on.stream()));
+        return result(std::move(y), {&x, given_scales, &h.scales, h.bias.defined() ? &h.bias : nullptr}, "W8Linear");
+    });
+}
+
+// ---- verification of drafts ----------------------------------------------------------------
+
+PyObject* verify(PyObject*, PyObject* const* args, Py_ssize_t count) {
+    // logits, drafts, uniforms, starts, parents, draft_probs, temperature, max_nodes
+    ARGS(8)
+    return guarded([&]() -> PyObject* {
+        const at::Tensor& logits = tensor(args[0], "logits");
+        need(logits.dim() == 2 && logits.is_cuda() && logits.size(1) > 0, "logits must be a CUDA tensor [rows, vocab]");
+        const int64_t rows = logits.size(0), vocab = logits.size(1);
+        const int index = logits.get_device();
+        matrix(args[0], "logits", rows, vocab, index);
+        fb2_verify v{};
+        v.dtype = code_of(logits.scalar_type());
+        const at::Tensor* drafts = given(plain(args[1], "drafts", at::kInt, index), "drafts");
+        const at::Tensor* uniforms = given(plain(args[2], "uniforms", at::kDouble, index), "uniforms");
+        const at::Tensor* starts = plain(args[3], "starts", at::kInt, index);
+        const at::Tensor* parents = plain(args[4], "parents", at::kInt, index);
+        const at::Tensor* probs = args[5] == Py_None ? nullptr : &matrix(args[5], "draft_probs", rows, vocab, index);
+        const at::Tensor* temperature = plain(args[6], "temperature", at::kFloat, index);
+        need(drafts->numel() == rows && uniforms->numel() == rows && (!parents || parents->numel() == rows),
+             "drafts, uniforms and parents must have one entry per row");
+        need(!starts || starts->numel() >= 1, "starts must have one entry more than there are sequences");
+        const int64_t seqs = starts ? starts->numel() - 1 : rows;
+        need(!temperature || temperature->numel() == seqs, "temperature must have one entry per sequence");
+        need(!probs || probs->scalar_type() == at::kFloat, "draft_probs must be float32");
+        need(!probs || !parents, "draft_probs go with chains: one draft to a node, no parents");
+        int64_t nodes = args[7] == Py_None ? std::max<int64_t>(1, std::min<int64_t>(starts ? rows : 1, 1024)) : integer(args[7], "max_nodes");
+        need(nodes >= 1 && nodes <= 1024, "max_nodes must be in 1..1024");
+        need(args[7] != Py_None || !starts || rows <= 1024, "max_nodes is needed for more than 1024 rows");
+        v.device_logits = logits.data_ptr();
+        v.device_draft_probs = data<float>(probs);
+        v.device_drafts = data<int32_t>(drafts);
+        v.device_row_starts = data<int32_t>(starts);
+        v.device_parents = data<int32_t>(parents);
+        v.device_uniforms = data<double>(uniforms);
+        v.device_temperature = data<float>(temperature);
+        v.logits_row_stride = logits.stride(0);
+        v.probs_row_stride = probs ? probs->stride(0) : 0;
+        v.n_seqs = small(seqs, "sequences");
+        v.n_rows = small(rows, "rows");
+        v.vocab = small(vocab, "vocab");
+        v.max_nodes = (int32_t)nodes;
+        OnDevice on(index);
+        at::Tensor tokens = empty({seqs, nodes}, at::kInt, index), path = empty({seqs, nodes}, at::kInt, index),
+                   counts = empty({seqs}, at::kInt, index), work;
+        status(fb2_verify_workspace(&v, &v.workspace_bytes));
+        if (v.workspace_bytes) work = empty({v.workspace_bytes}, at::kByte, index);
+        v.device_workspace = v.workspace_bytes ? work.data_ptr() : nullptr;
+        v.device_tokens = data<int32_t>(&tokens);
+        v.device_nodes = data<int32_t>(&path);
+        v.device_counts = data<int32_t>(&counts);
+        status(fb2_verify_drafts(&v, on.stream()));
+        return Py_BuildValue("(NNN)", THPVariable_Wrap(std::move(tokens)), THPVariable_Wrap(std::move(path)), THPVariable_Wrap(std::move(counts)));
+    });
+}
+
 PyObject* setup(PyObject*, PyObject* const* args, Py_ssize_t count) {
     ARGS(2)  // ArgumentError, check
     Py_XSETREF(g_argument_error, Py_NewRef(args[0]));
@@ -498,8 +858,11 @@ PyObject* setup(PyObject*, PyObject* const* args, Py_ssize_t count) {
 }
 
 #define METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
-PyMethodDef kMethods[] = {METHOD(setup),      METHOD(cache_new),   METHOD(cache_write), METHOD(cache_read), METHOD(cache_attend),
-                          METHOD(linear_new), METHOD(linear_pack), METHOD(linear_call), METHOD(controls),   {nullptr, nullptr, 0, nullptr}};
+PyMethodDef kMethods[] = {METHOD(setup),       METHOD(cache_new),    METHOD(cache_write),    METHOD(cache_read),
+                          METHOD(cache_attend), METHOD(linear_new),   METHOD(linear_pack),    METHOD(linear_call),
+                          METHOD(controls),    METHOD(pages_new),    METHOD(pages_extend),   METHOD(pages_truncate),
+                          METHOD(norm),        METHOD(linear8_new),  METHOD(linear8_pack),   METHOD(linear8_call),
+                          METHOD(quantise_rows), METHOD(verify),     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_serving", "The serving operators on torch tensors (see serving.py).", -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,430 @@
+// w8.cuh — linear layers in 8-bit integers on tcgen05 tiles: weights with a scale
+// for each output, rows of x with a scale each (include/forge_b200.h,
+// fb2_w8_matmul, has the formula).
+//
+// y = (codes of x . codes of W) * scale of W * scale of x + bias: the products and
+// their sums are exact in 32-bit integers, in tensor memory, whatever the order
+// (127 * 127 * in_features < 2^31), so that splitting the inputs over CTAs changes
+// no bit; only the epilogue rounds.  Both operands are K-major rows of bytes, TMA
+// boxes of 128 bytes x rows, 128-byte swizzled.
+//
+// k_w8_few: up to 128 rows of x to a tile, as the N side of the tiles, the weights
+// as the M side: each weight is read once.  A cluster shares a tile's inputs where
+// there are fewer tiles than SMs.
+// k_w8_many: 128 rows of x by 256 outputs, one CTA on each SM.
+// Every wait is bounded (2 s); on expiry a CTA stops, waits (bounded) for its
+// copies and MMAs in flight, frees its tensor memory, and its rows of y are NaN.
+#pragma once
+#include <type_traits>
+
+#include "norm.cuh"
+#include "pages.cuh"
+#include "tc.cuh"
+
+namespace fb2 {
+
+constexpr int W8_K = 128;  // bytes of a stage's rows
+constexpr int W8_THREADS = 192, W8_TILE = 128 * W8_K;
+
+struct W8Args {
+    const float *x_scales, *w_scales, *bias;
+    void* y;
+    long long y_row;
+    int rows, in, out;
+    bool vec;       // rows of y begin on 16 bytes
+    int withhold;   // test hook: the k block of block 0 whose copy is left out; -1: none
+    unsigned long long wait_ns;
+};
+
+namespace w8 {
+
+// A, B signed 8-bit, D 32-bit integers, both operands K-major.
+constexpr uint32_t idesc(int M, int N) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+FB2_DEV void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+    asm volatile(
+        "{ .reg .pred p; setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, {%5, %5, %5, %5}, p; }" ::"r"(d),
+        "l"(a), "l"(b), "r"(id), "r"(accumulate), "r"(0u)
+        : "memory");
+}
+FB2_DEV void ld16(uint32_t at, int (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(at));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+FB2_DEV void arrive(uint64_t* b) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_addr(b)) : "memory"); }
+FB2_DEV int peek(uint32_t at, int rank) {
+    uint32_t r;
+    int v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(r) : "memory");
+    return v;
+}
+FB2_DEV float value(int sum, float w_scale, float x_scale, float bias) {
+    return fmaf((float)sum * w_scale, x_scale, bias);
+}
+
+}  // namespace w8
+
+template <int BN>
+struct W8Few {
+    static constexpr int STAGE = W8_TILE + BN * W8_K;
+    static constexpr int STAGES = (200 * 1024) / STAGE > 8 ? 8 : (200 * 1024) / STAGE;
+    static constexpr int PART = BN * 128 * 4;  // sums of a tile
+    static constexpr int SMEM = (STAGES * STAGE > PART ? STAGES * STAGE : PART) + 1024;
+    static constexpr uint32_t COLS = BN < 32 ? 32 : BN;
+};
+
+// blockIdx.x: tile of 128 outputs and, fastest, the CTA's rank in the cluster that
+// shares its inputs; blockIdx.y: tile of BN rows of x.
+template <class T, int BN>
+__global__ void __launch_bounds__(W8_THREADS, 1)
+    k_w8_few(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, W8Args a, int ranks) {
+    using S = W8Few<BN>;
+    extern __shared__ unsigned char w8_raw[];
+    __shared__ __align__(8) uint64_t full[S::STAGES], empty[S::STAGES], done;
+    __shared__ uint32_t tmem_base;
+    __shared__ volatile int s_abort;
+    unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(w8_raw) + 1023) & ~(uintptr_t)1023);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = blockIdx.x % ranks, o0 = blockIdx.x / ranks * 128, r0 = blockIdx.y * BN;
+    const int blocks = (a.in + W8_K - 1) / W8_K;
+    const int k0 = (int)((long long)blocks * rank / ranks), nk = (int)((long long)blocks * (rank + 1) / ranks) - k0;
+    if (tid == 0) {
+        s_abort = 0;
+        for (int i = 0; i < S::STAGES; i++) {
+            tc::bar_init(&full[i], 1);
+            tc::bar_init(&empty[i], 1);
+        }
+        tc::bar_init(&done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_addr(&tmem_base)), "r"(S::COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = tmem_base;
+    pdl_wait();
+
+    if (warp == 0 && lane == 0) {
+        int i = 0;
+        for (; i < nk; i++) {
+            const int st = i % S::STAGES;
+            if (i >= S::STAGES && !tc::bar_wait(&empty[st], (i / S::STAGES - 1) & 1, &s_abort, a.wait_ns)) break;
+            unsigned char* at = sm + st * S::STAGE;
+            const bool leave = i == a.withhold && blockIdx.x == 0 && blockIdx.y == 0;
+            tc::bar_expect_tx(&full[st], S::STAGE);
+            tc::tma_load_2d(at, &map_w, (k0 + i) * W8_K, o0, &full[st]);
+            if (leave) break;  // the rest never comes
+            tc::tma_load_2d(at + W8_TILE, &map_x, (k0 + i) * W8_K, r0, &full[st]);
+        }
+    } else if (warp == 1 && lane == 0) {
+        for (int i = 0; i < nk; i++) {
+            const int st = i % S::STAGES;
+            if (!tc::bar_wait(&full[st], (i / S::STAGES) & 1, &s_abort, a.wait_ns)) break;
+            tc::fence_after();
+            const uint32_t at = tc::smem_addr(sm + st * S::STAGE);
+            const uint64_t w = tc::sw128_desc(at, 16, 1024), x = tc::sw128_desc(at + W8_TILE, 16, 1024);
+#pragma unroll
+            for (int k = 0; k < W8_K / 32; k++) w8::mma(tmem, w + 2 * k, x + 2 * k, w8::idesc(128, BN), (i | k) != 0);
+            tc::mma_commit(&empty[st]);
+        }
+        tc::mma_commit(&done);
+    }
+    __syncwarp();
+    // all MMAs have completed, with all copies that they read; after an abort the
+    // copies in flight land before the ring is used again
+    bool ok = tc::bar_try(&done, 0);
+    if (!ok) {
+        const unsigned long long t0 = tc::now_ns();
+        while (!(ok = tc::bar_try(&done, 0)) && tc::now_ns() - t0 < 2 * kTcTimeoutNs) {
+        }
+        if (!ok) s_abort = 1;
+    }
+    __syncthreads();
+    tc::fence_after();
+    const bool failed = s_abort != 0;
+    const int quarter = warp & 3;
+    const float nan = __uint_as_float(0x7fc00000u);
+    T* y = static_cast<T*>(a.y);
+    if (failed) {
+        // a copy of a stage that never filled may still land: nothing is written there
+        if (tid == 0) {
+            const unsigned long long t0 = tc::now_ns();
+            for (int st = 0; st < S::STAGES && st < nk; st++) {
+                const int last = st + (nk - 1 - st) / S::STAGES * S::STAGES;
+                while (!tc::bar_try(&full[st], (last / S::STAGES) & 1) && tc::now_ns() - t0 < a.wait_ns) {
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (ranks == 1) {
+        if (warp < 4) {
+            const int o = o0 + 32 * quarter + lane;
+            const float ws = o < a.out ? __ldg(a.w_scales + o) : 0.f, bias = a.bias && o < a.out ? __ldg(a.bias + o) : 0.f;
+#pragma unroll 1
+            for (int c = 0; c < BN; c += 16) {
+                if (r0 + c >= a.rows) break;
+                int v[16];
+                w8::ld16(tmem + ((uint32_t)(32 * quarter) << 16) + c, v);
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int r = r0 + c + i;
+                    if (r < a.rows && o < a.out)
+                        y[r * a.y_row + o] = Dense<T>::put(failed ? nan : w8::value(v[i], ws, __ldg(a.x_scales + r), bias));
+                }
+            }
+        }
+    } else {
+        int* part = reinterpret_cast<int*>(sm);  // [BN][128]
+        __shared__ int s_failed;
+        if (tid == 0) s_failed = failed;
+        if (warp < 4) {
+#pragma unroll 1
+            for (int c = 0; c < BN; c += 16) {
+                int v[16];
+                w8::ld16(tmem + ((uint32_t)(32 * quarter) << 16) + c, v);
+#pragma unroll
+                for (int i = 0; i < 16; i++) part[(c + i) * 128 + 32 * quarter + lane] = v[i];
+            }
+        }
+        pg::cluster_sync();
+        // each CTA sums and writes some of the rows
+        if (warp < 4) {
+            bool bad = false;
+            for (int k = 0; k < ranks; k++) bad |= w8::peek(tc::smem_addr(&s_failed), k) != 0;
+            const int o = o0 + 32 * quarter + lane;
+            const float ws = o < a.out ? __ldg(a.w_scales + o) : 0.f, bias = a.bias && o < a.out ? __ldg(a.bias + o) : 0.f;
+            for (int c = rank; c < BN && r0 + c < a.rows; c += ranks) {
+                int sum = 0;
+                for (int k = 0; k < ranks; k++) sum += w8::peek(tc::smem_addr(part + c * 128 + 32 * quarter + lane), k);
+                const int r = r0 + c;
+                if (o < a.out) y[r * a.y_row + o] = Dense<T>::put(bad ? nan : w8::value(sum, ws, __ldg(a.x_scales + r), bias));
+            }
+        }
+        pg::cluster_sync();  // the others' shared memory stays until it is read
+    }
+    tc::fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc::fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");
+    }
+}
+
+// ---- many rows -------------------------------------------------------------------------
+constexpr int W8M_N = 256, W8M_STAGE = W8_TILE + W8M_N * W8_K, W8M_STAGES = 4;
+constexpr int W8M_SMEM = W8M_STAGES * W8M_STAGE + 1024;
+constexpr int W8M_GROUP = 16;  // tiles of rows that are walked together: what runs at a time shares operands in L2
+
+// One CTA on each SM walks the tiles.  Warp 0 copies, warp 1 issues the MMAs into
+// one of two accumulators, warps 2..5 bring the other one out: lane r of quarter q
+// is row 32 q + r of the tile, its columns are outputs.
+template <class T>
+__global__ void __launch_bounds__(W8_THREADS, 1)
+    k_w8_many(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, W8Args a) {
+    extern __shared__ unsigned char w8_raw[];
+    __shared__ __align__(8) uint64_t full[W8M_STAGES], empty[W8M_STAGES], ready[2], taken[2], drain;
+    __shared__ uint32_t tmem_base;
+    __shared__ volatile int s_abort;
+    __shared__ __align__(16) float s_scale[2][W8M_N], s_bias[2][W8M_N];
+    unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(w8_raw) + 1023) & ~(uintptr_t)1023);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tiles_r = (a.rows + 127) / 128, tiles_o = (a.out + W8M_N - 1) / W8M_N;
+    const int tiles = tiles_r * tiles_o;
+    const int nk = (a.in + W8_K - 1) / W8_K;
+    // groups of W8M_GROUP tiles of rows, through all outputs
+    auto place = [&](int t, int& r0, int& o0) {
+        const int group = t / (W8M_GROUP * tiles_o), within = t - group * W8M_GROUP * tiles_o;
+        const int high = min(W8M_GROUP, tiles_r - group * W8M_GROUP);
+        r0 = (group * W8M_GROUP + within % high) * 128;
+        o0 = within / high * W8M_N;
+    };
+    if (tid == 0) {
+        s_abort = 0;
+        for (int i = 0; i < W8M_STAGES; i++) {
+            tc::bar_init(&full[i], 1);
+            tc::bar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            tc::bar_init(&ready[i], 1);
+            tc::bar_init(&taken[i], 4);
+        }
+        tc::bar_init(&drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_addr(&tmem_base)), "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = tmem_base;
+    pdl_wait();
+
+    if (warp == 0 && lane == 0) {
+        uint32_t it = 0;
+        bool stop = false;
+        for (int t = blockIdx.x; t < tiles && !stop; t += gridDim.x) {
+            int r0, o0;
+            place(t, r0, o0);
+            for (int i = 0; i < nk; i++, it++) {
+                const int st = it % W8M_STAGES;
+                if (it >= W8M_STAGES && !tc::bar_wait(&empty[st], (it / W8M_STAGES - 1) & 1, &s_abort, a.wait_ns)) {
+                    stop = true;
+                    break;
+                }
+                unsigned char* at = sm + st * W8M_STAGE;
+                tc::bar_expect_tx(&full[st], W8M_STAGE);
+                tc::tma_load_2d(at, &map_x, i * W8_K, r0, &full[st]);
+                if (blockIdx.x == 0 && (int)it == a.withhold) {
+                    stop = true;
+                    break;
+                }
+                tc::tma_load_2d(at + W8_TILE, &map_w, i * W8_K, o0, &full[st]);
+            }
+        }
+        // copies still landing (after an abort): each stage's latest fill
+        if (s_abort || stop) {
+            const unsigned long long t0 = tc::now_ns();
+            for (uint32_t j = it > W8M_STAGES ? it - W8M_STAGES : 0; j < it; j++)
+                while (!tc::bar_try(&full[j % W8M_STAGES], (j / W8M_STAGES) & 1) && tc::now_ns() - t0 < kTcTimeoutNs) {
+                }
+        }
+    } else if (warp == 1 && lane == 0) {
+        uint32_t it = 0, local = 0;
+        bool stop = false;
+        for (int t = blockIdx.x; t < tiles && !stop; t += gridDim.x, local++) {
+            const uint32_t acc = local & 1;
+            if (local >= 2 && !tc::bar_wait(&taken[acc], (local / 2 - 1) & 1, &s_abort, a.wait_ns)) break;
+            tc::fence_after();
+            for (int i = 0; i < nk; i++, it++) {
+                const int st = it % W8M_STAGES;
+                if (!tc::bar_wait(&full[st], (it / W8M_STAGES) & 1, &s_abort, a.wait_ns)) {
+                    stop = true;
+                    break;
+                }
+                tc::fence_after();
+                const uint32_t at = tc::smem_addr(sm + st * W8M_STAGE);
+                const uint64_t x = tc::sw128_desc(at, 16, 1024), w = tc::sw128_desc(at + W8_TILE, 16, 1024);
+#pragma unroll
+                for (int k = 0; k < W8_K / 32; k++)
+                    w8::mma(tmem + acc * W8M_N, x + 2 * k, w + 2 * k, w8::idesc(128, W8M_N), (i | k) != 0);
+                tc::mma_commit(&empty[st]);
+            }
+            if (!stop) tc::mma_commit(&ready[acc]);
+        }
+        // every MMA issued completes before the accumulators are freed
+        tc::mma_commit(&drain);
+        const unsigned long long t0 = tc::now_ns();
+        while (!tc::bar_try(&drain, 0) && tc::now_ns() - t0 < kTcTimeoutNs) {
+        }
+    } else if (warp >= 2) {
+        const int quarter = warp & 3, thread = tid - 64;
+        const float nan = __uint_as_float(0x7fc00000u);
+        T* y = static_cast<T*>(a.y);
+        uint32_t local = 0;
+        bool failed = false;  // from the first tile that never came on: the rest is NaN
+        for (int t = blockIdx.x; t < tiles; t += gridDim.x, local++) {
+            const uint32_t acc = local & 1;
+            int r0, o0;
+            place(t, r0, o0);
+            // the four warps fill the tile's scales; the one before last may still be read
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            for (int i = thread; i < W8M_N; i += 128) {
+                const int o = o0 + i;
+                s_scale[acc][i] = o < a.out ? __ldg(a.w_scales + o) : 0.f;
+                s_bias[acc][i] = a.bias && o < a.out ? __ldg(a.bias + o) : 0.f;
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            const bool ok = !failed && tc::bar_wait(&ready[acc], (local / 2) & 1, &s_abort, 2 * a.wait_ns);
+            failed = !__all_sync(0xffffffffu, ok);
+            tc::fence_after();
+            const int r = r0 + 32 * quarter + lane;
+            const float xs = r < a.rows ? __ldg(a.x_scales + r) : 0.f;
+            T* to = y + r * a.y_row + o0;
+#pragma unroll 1
+            for (int c = 0; c < W8M_N; c += 16) {
+                int v[16];
+                w8::ld16(tmem + acc * W8M_N + ((uint32_t)(32 * quarter) << 16) + c, v);
+                if (r >= a.rows || o0 + c >= a.out) continue;
+                float f[16];
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const float4 s4 = *reinterpret_cast<const float4*>(&s_scale[acc][c + i]);
+                    const float4 b4 = *reinterpret_cast<const float4*>(&s_bias[acc][c + i]);
+                    f[i] = w8::value(v[i], s4.x, xs, b4.x), f[i + 1] = w8::value(v[i + 1], s4.y, xs, b4.y);
+                    f[i + 2] = w8::value(v[i + 2], s4.z, xs, b4.z), f[i + 3] = w8::value(v[i + 3], s4.w, xs, b4.w);
+                }
+                if (failed) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) f[i] = nan;
+                }
+                if (a.vec && o0 + c + 16 <= a.out) {
+                    constexpr int N = 16 / sizeof(T);
+#pragma unroll
+                    for (int i = 0; i < 16; i += N) *reinterpret_cast<uint4*>(to + c + i) = pack16<T>(f + i);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if (o0 + c + i < a.out) to[c + i] = Dense<T>::put(f[i]);
+                }
+            }
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) w8::arrive(&taken[acc]);
+        }
+    }
+    __syncwarp();
+    tc::fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc::fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// W [in][out] as codes [out][in] with a scale for each output: a warp's lanes take 32
+// neighbouring outputs, 8 warps the inputs in turns; codes go through shared memory,
+// so that both sides are read and written in runs.
+constexpr int W8P_THREADS = 256;
+template <class T>
+__global__ void __launch_bounds__(W8P_THREADS) k_w8_pack(const T* w, long long w_row, int in, int out, signed char* codes, long long code_row,
+                                                         float* scales) {
+    __shared__ uint32_t s_top[8][32];
+    __shared__ signed char s_code[32][128 + 4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, o0 = blockIdx.x * 32, o = o0 + lane;
+    uint32_t top = 0;
+    if (o < out)
+        for (int i = warp; i < in; i += 8) top = max(top, __float_as_uint(Dense<T>::get(w[i * w_row + o])) & 0x7fffffffu);
+    s_top[warp][lane] = top;
+    __syncthreads();
+    for (int k = 0; k < 8; k++) top = max(top, s_top[k][lane]);
+    float inv, scale;
+    nrm::code_scale(top, inv, scale);
+    if (warp == 0 && o < out) scales[o] = scale;
+    for (int i0 = 0; i0 < in; i0 += 128) {
+        __syncthreads();
+        for (int i = warp; i < 128; i += 8)
+            s_code[lane][i] = o < out && i0 + i < in ? (signed char)nrm::code(Dense<T>::get(w[(i0 + i) * w_row + o]), inv) : 0;
+        __syncthreads();
+        for (int k = threadIdx.x; k < 32 * 128; k += W8P_THREADS) {
+            const int to = o0 + k / 128, i = i0 + k % 128;
+            if (to < out && i < in) codes[to * code_row + i] = s_code[k / 128][k % 128];
+        }
+    }
+}
+
+}  // namespace fb2

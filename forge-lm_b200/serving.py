@@ -1,7 +1,8 @@
 """Serving operators on torch CUDA tensors (include/forge_b200.h, "serving
-operators"): a paged K/V cache that is quantised as it is written, attention
-of single tokens or drafted trees over it, linear layers with 4-bit weights,
-and penalties, biases and grammar masks on logits.
+operators"): pages of sequences, a paged K/V cache that is quantised as it is
+written, attention of single tokens or drafted trees over it, the residual stream
+with its norms, linear layers with 4-bit weights or in 8-bit integers, penalties,
+biases and grammar masks on logits, and the verification of drafted tokens.
 
 Every call runs the library's kernels on torch's current stream of the
 tensors' device and returns without waiting.  Results and workspaces come from
@@ -21,8 +22,9 @@ import os
 from . import _native as N
 from ._native import ArgumentError
 
-__all__ = ["QuantKvCache", "W4Linear", "logit_controls"]
+__all__ = ["QuantKvCache", "W4Linear", "logit_controls", "PageTable", "W8Linear", "quantise_rows", "residual_norm", "verify_drafts"]
 
+_NORMS = {"layer": N.FB2_NORM_LAYER, "rms": N.FB2_NORM_RMS}
 _FORMATS = {"int8": N.FB2_KVQ_INT8, "int4": N.FB2_KVQ_INT4}
 _PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_serving.so")
 _calls = None
@@ -174,3 +176,133 @@ def logit_controls(logits, *, tokens=None, token_starts=None, repetition=None, p
     other way) or a new tensor."""
     return (_calls or _load()).controls(logits, tokens, token_starts, repetition, presence, frequency, bias_ids, bias_values,
                                         bias_starts, allowed, mask_rows, out)
+
+
+class PageTable:
+    """Pages of a cache for a number of sequences, kept on the device:
+
+      table  int32 [sequences, pages]  the pages of each, -1 behind them
+      lens   int32 [sequences]         tokens of each
+      free   int32 [all pages]         free pages, the first n_free entries
+      n_free int32 [1]
+
+    (QuantKvCache.attend's page_table is `table`.)  A page belongs to one
+    sequence or to the list.  The object holds the buffers; `empty` makes new
+    ones."""
+
+    def __init__(self, table, lens, free, n_free, page_size: int):
+        self._calls = _load()
+        self._handle = self._calls.pages_new(table, lens, free, n_free, page_size)
+        self.table, self.lens, self.free, self.n_free = table, lens, free, n_free
+        self.page_size, self.device = int(page_size), table.device
+        self.n_seqs, self.max_pages = table.shape
+
+    @classmethod
+    def empty(cls, n_seqs: int, max_pages: int, n_pages: int, page_size: int, device="cuda") -> "PageTable":
+        """Sequences without tokens and all pages free (page 0 is taken first)."""
+        import torch
+
+        def ints(shape, value):
+            return torch.full(shape, value, dtype=torch.int32, device=device)
+
+        free = torch.arange(n_pages - 1, -1, -1, dtype=torch.int32, device=device)
+        return cls(ints((n_seqs, max_pages), -1), ints((n_seqs,), 0), free, ints((1,), n_pages), page_size)
+
+    def extend(self, counts, max_rows: int):
+        """(starts, prefix_lens, slots, positions) for counts [sequences] int32
+        more tokens of each sequence.
+
+        Sequence b's rows are starts[b]:starts[b+1] of slots and positions
+        [max_rows], its length before is prefix_lens[b]; rows behind the last
+        have slot -1 and position 0.  These are what QuantKvCache.write and
+        .attend take.  Sequences are served in their order: one whose tokens
+        would not fit its row of the table (or whose count is negative) asks
+        for nothing; of the others one is served if the tokens asked for up to
+        it are at most max_rows and, where it needs pages, the pages asked for
+        at most the free ones.  What is not served stays as it is and has no
+        rows."""
+        return self._calls.pages_extend(self._handle, counts, max_rows)
+
+    def truncate(self, lens) -> None:
+        """Shortens the sequences to lens [sequences] int32 tokens (one that is
+        not longer stays as it is); pages that they no longer need are free."""
+        self._calls.pages_truncate(self._handle, lens)
+
+
+def residual_norm(h, x, weight, bias=None, *, post_weight=None, post_bias=None, gate=None, scale: float = 1.0, kind: str = "layer",
+                  eps: float = 1e-5, quantise: bool = False, dtype=None):
+    """(s, y) with s = x + scale * gate * post(h) and y = norm(s), over rows
+    [rows, dim] with contiguous last dimension; with quantise (s, codes, scales),
+    y's rows as quantise_rows makes them.
+
+    kind "layer": (v - mean) / sqrt(variance + eps) * weight + bias, "rms":
+    v / sqrt(mean of squares + eps) * weight + bias; weights and biases are
+    float32 [dim].  post_weight norms h first; gate [dim] or [rows, dim] has h's
+    dtype.  x, the stream, has h's dtype or is float32.  h None: s is x, and y
+    has x's dtype or `dtype`.  Computed in fp32, y from s before s is rounded; s
+    has x's dtype, y has h's."""
+    _need(kind in _NORMS, "kind must be 'layer' or 'rms'")
+    return (_calls or _load()).norm(h, x, weight, bias, post_weight, post_bias, gate, scale, _NORMS[kind], eps, quantise, dtype)
+
+
+def quantise_rows(x):
+    """(codes int8 [rows, columns], scales float32 [rows]) of x [rows, columns]:
+    scale = max|x| / 127, code = round(x * (127 / max|x|)).  Rows of codes begin on
+    16 bytes.  A row with a non-finite element has scale NaN."""
+    return (_calls or _load()).quantise_rows(x)
+
+
+class W8Linear:
+    """y = x W + bias in 8-bit integers: codes int8 [out, in] (rows a multiple of
+    16 bytes apart) with a float32 scale for each output, W[i][o] =
+    codes[o][i] * scales[o], and rows of x as quantise_rows makes them.  Sums of
+    products are exact; scales and bias are applied in fp32."""
+
+    def __init__(self, codes, scales, bias=None):
+        self._calls = _load()
+        self._handle = self._calls.linear8_new(codes, scales, bias)
+        self.codes, self.scales, self.bias, self.device = codes, scales, bias, codes.device
+        self.out_features, self.in_features = codes.shape
+
+    @classmethod
+    def pack(cls, w, bias=None) -> "W8Linear":
+        """Quantises W [in, out] (the layout of the model's projections)."""
+        import torch
+        _need(w.dim() == 2 and w.is_cuda, "w must be a CUDA tensor [in, out]")
+        k, n = w.shape
+        codes = torch.zeros((n, -(-k // 16) * 16), dtype=torch.int8, device=w.device)[:, :k]
+        self = cls(codes, torch.zeros(n, dtype=torch.float32, device=w.device), bias)
+        self._calls.linear8_pack(self._handle, w)
+        return self
+
+    def __call__(self, x, scales=None, dtype=None):
+        """x [..., in] -> [..., out] in x's dtype (or `dtype`), its rows quantised
+        first; or codes int8 x [..., in] with scales, one per row, -> `dtype`
+        (default float32).  Codes whose rows do not begin on 16 bytes are copied
+        first."""
+        return self._calls.linear8_call(self._handle, x, scales, dtype)
+
+
+def verify_drafts(logits, drafts, uniforms, *, starts=None, parents=None, draft_probs=None, temperature=None, max_nodes: int | None = None):
+    """(tokens, nodes, counts): which drafted tokens the target accepts, and the
+    token that follows them.
+
+    Sequence b's rows are starts[b]:starts[b+1] (None: one each): its last token,
+    then drafts [rows] int32 below it.  parents [rows] int32 counts a row's parent
+    from the sequence's first (earlier) row; None: a chain.  logits [rows, vocab]
+    are what the target says follows each row, p = softmax(logits / temperature[b])
+    (float32; None: 1; 0: all of it on the largest logit).  From the first row on,
+    drafts c below a row are tried in order, each with uniforms[c] (float64 in
+    [0, 1)).  With draft_probs [rows, vocab] float32 (chains): accepted where
+    uniforms[c] * q(c) < p(c), and what may follow a rejected one is max(p - q, 0).
+    Without: accepted where uniforms[c] * (1 - p of siblings rejected) < p(c), and
+    what may follow is p without the rejected ones.  The last token is the lowest id
+    at which the running sum of that passes uniforms[starts[b]] times its total.
+
+    counts [sequences] int32: tokens gained, accepted ones and the last; tokens
+    [sequences, max_nodes] int32: these; nodes [sequences, max_nodes] int32: the
+    row, counted from the sequence's first, that each of them follows, so the rows
+    that stay in the cache; -1 behind them.  max_nodes (up to 1024) is a host bound
+    of a sequence's rows; later ones are not looked at.  A row of logits with a NaN, a +inf
+    or nothing above -inf accepts nothing and draws -1."""
+    return (_calls or _load()).verify(logits, drafts, uniforms, starts, parents, draft_probs, temperature, max_nodes)

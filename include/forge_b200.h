@@ -439,6 +439,162 @@ typedef struct {
 } fb2_logit_control;
 int32_t fb2_logit_controls(const fb2_logit_control* c, void* cuda_stream);
 
+/* Pages of sequences: the caller's page table, lengths and list of free pages.
+ * Sequence b has lens[b] tokens in the first ceil(lens[b] / page_size) pages of
+ * its row of the table; entries behind them are -1.  The free pages are
+ * free[0 .. n_free - 1].  A page belongs to one sequence or to the list. */
+typedef struct {
+    int32_t* device_table;  /* [n_seqs][max_pages], rows table_stride apart */
+    int32_t* device_lens;   /* [n_seqs] */
+    int32_t* device_free;   /* [n_pages] */
+    int32_t* device_n_free; /* [1] */
+    int64_t table_stride;
+    int32_t n_seqs;    /* up to 16384 */
+    int32_t max_pages; /* of a sequence */
+    int32_t n_pages;   /* of the cache */
+    int32_t page_size; /* a power of two in 8..1024 */
+} fb2_pages;
+int32_t fb2_pages_check(const fb2_pages* p); /* whether the calls below take it */
+
+/* Room for counts[b] more tokens of every sequence b.  Sequences are served in
+ * their order.  One whose length or count is negative, or whose tokens would not
+ * fit max_pages, asks for nothing.  Of the others sequence b is served where the
+ * tokens that sequences 0..b ask for are at most max_rows and, if it needs pages,
+ * the pages that they ask for at most n_free.  What is not served keeps its
+ * length and has no rows.  Rows of the call are the served tokens in order:
+ *   starts[b] .. starts[b + 1] - 1 are sequence b's, prefix_lens[b] its length
+ *   before (fb2_kvq_attend's row_starts and prefix_lens);
+ *   slots[r] = page * page_size + offset (fb2_kvq_write's), positions[r] the
+ *   token's position; behind the last row, up to max_rows: -1 and 0.
+ * New pages are taken from the end of the list, in the order of sequences and
+ * positions, and entered into the table; lens and n_free are brought up to date.
+ * A page id on the list that is outside the cache gives slots of -1. */
+int32_t fb2_pages_extend(const fb2_pages* p, const int32_t* device_counts, int32_t max_rows, int32_t* device_starts,
+                         int32_t* device_prefix_lens, int32_t* device_slots, int32_t* device_positions, void* cuda_stream);
+
+/* Shortens every sequence b to lens[b] tokens (below 0: 0; a sequence that is not
+ * longer stays as it is).  Pages that it no longer needs go to the end of the list,
+ * the first of them last: an extend that asks for them again gets the same ones.
+ * Their table entries become -1.  device_lens here may not be the pages' own. */
+int32_t fb2_pages_truncate(const fb2_pages* p, const int32_t* device_lens, void* cuda_stream);
+
+/* A block's output h onto the residual stream x, and the norm before what follows:
+ *   s = x + scale * gate * post(h),   y = norm(s),
+ * post(h) = h without post_weight, gate 1 where NULL, each norm
+ *   FB2_NORM_LAYER: (v - mean) / sqrt(variance + eps) * weight + bias,
+ *   FB2_NORM_RMS:   v / sqrt(mean of v^2 + eps) * weight + bias,
+ * the biases 0 where NULL.  Without h: s = x, which is not written.  In fp32 from
+ * the inputs on (y is the norm of s before s is rounded); sum has x's type, y h's.
+ * The result is y, or codes and scales as fb2_quantise_rows makes them of y before
+ * it is rounded.  Squares of differences from the mean have to be finite in fp32.
+ * sum, y, codes and scales share nothing with the inputs. */
+typedef enum { FB2_NORM_LAYER = 0, FB2_NORM_RMS = 1 } fb2_norm_kind;
+typedef struct {
+    const void* device_h;            /* [n_rows][dim], or NULL */
+    const void* device_x;            /* [n_rows][dim] */
+    const void* device_gate;         /* [n_rows][dim] (gate_row_stride 0: one row for all), h's type, or NULL */
+    const float* device_weight;      /* [dim] */
+    const float* device_bias;        /* [dim], or NULL */
+    const float* device_post_weight; /* [dim], or NULL */
+    const float* device_post_bias;   /* [dim], or NULL */
+    void* device_sum;                /* [n_rows][dim] */
+    void* device_y;                  /* [n_rows][dim], or NULL */
+    void* device_codes;              /* int8 [n_rows][dim], rows on 16 bytes, or NULL */
+    float* device_scales;            /* [n_rows], with codes */
+    int64_t h_row_stride;
+    int64_t x_row_stride;
+    int64_t gate_row_stride;
+    int64_t sum_row_stride;
+    int64_t y_row_stride;
+    int64_t code_row_stride;
+    int32_t n_rows;
+    int32_t dim;          /* up to 32768 */
+    int32_t dtype;        /* of h, gate and y */
+    int32_t stream_dtype; /* of x and sum: dtype or FB2_F32 */
+    int32_t kind;         /* fb2_norm_kind */
+    float scale;
+    float eps;
+    int32_t reserved;
+} fb2_norm;
+int32_t fb2_residual_norm(const fb2_norm* n, void* cuda_stream);
+
+/* Rows as 8-bit codes: scale = max|x| / 127, code = round(x * (127 / max|x|)) to
+ * nearest even, each step rounded to fp32.  A row with a non-finite element has
+ * codes 0 and scale NaN, one whose max|x| is below 1e-35 codes 0 and scale 0.
+ * Rows of codes are code_row_stride bytes apart, a multiple of 16, and begin on 16
+ * bytes; bytes behind dim are not written. */
+int32_t fb2_quantise_rows(int32_t n_rows, int32_t dim, const void* device_x, int32_t dtype, int64_t x_row_stride, void* device_codes,
+                          int64_t code_row_stride, float* device_scales, void* cuda_stream);
+
+/* A linear layer with 8-bit weights and a scale for each output:
+ *   codes int8 [out][in], rows code_row_stride bytes apart (a multiple of 16),
+ *   16-byte aligned; W[i][o] = code * scale[o].  Codes of -128 are as good as others.
+ * What lies behind in_features in a row is not read as a value. */
+typedef struct {
+    const void* device_codes;
+    const float* device_scales; /* [out] */
+    const float* device_bias;   /* [out], or NULL */
+    int64_t code_row_stride;
+    int32_t in_features;  /* up to 131072 */
+    int32_t out_features;
+} fb2_w8_linear;
+int32_t fb2_w8_check(const fb2_w8_linear* w); /* whether the calls below take it */
+/* Packs W [in][out] (dtype; w_row_stride as in fb2_w4_pack): each output's column as
+ * a row of fb2_quantise_rows.  codes and scales are written, bias is not looked at. */
+int32_t fb2_w8_pack(const fb2_w8_linear* w, const void* device_w, int32_t dtype, int64_t w_row_stride, void* cuda_stream);
+/* y[r][o] = (sum_i codes[r][i] * W codes[o][i]) * W scale[o] * scales[r] + bias[o]: the sum
+ * is exact, the products with the scales and the bias are fp32, rounded once to dtype.
+ * codes int8 [n_rows][in] as fb2_quantise_rows writes them.  Waits inside a kernel are
+ * bounded as in fb2_kvq_attend. */
+int32_t fb2_w8_matmul(const fb2_w8_linear* w, int32_t n_rows, const void* device_codes, int64_t code_row_stride, const float* device_scales,
+                      void* device_y, int64_t y_row_stride, int32_t dtype, void* cuda_stream);
+
+/* Drafted tokens against the target's probabilities.  Rows row_starts[b] ..
+ * row_starts[b + 1] - 1 (ascending) are sequence b's nodes: the first its last
+ * token, the others drafts below it, node i below node parents[i] < i (counted from the
+ * sequence's first; NULL: a chain, i - 1).  logits[r] is what the target says follows
+ * node r, p = softmax(logits / temperature[b]).  From the first node on, a node's
+ * drafts c are tried in the order of rows:
+ *   draft_probs NULL: accepted where uniforms[c] * (1 - m) < p(drafts[c]), m the p of its
+ *     siblings that were rejected (a token that was rejected there counts as 0);
+ *   else (chains): accepted where uniforms[c] * q(drafts[c]) < p(drafts[c]), q = draft_probs[c],
+ *     the probabilities that c was drawn from.
+ * An accepted draft is the next node.  Where none is, the last token is drawn from what
+ * may follow: p without the rejected tokens, or max(p - q, 0) of the rejected draft
+ * (where nothing of it is left: p).  It is the lowest id at which the running sum passes
+ * uniforms[row_starts[b]] times the total.  So each token is distributed as p, for uniforms
+ * in [0, 1) and drafts drawn from q, or chosen without regard to the uniforms.
+ * temperature <= 0 (or NaN): p is 1 at the lowest id of the largest logit.  -inf logits have
+ * p = 0; a row with a NaN, a +inf or nothing above -inf accepts nothing, and its draw is -1.
+ * Sums and exponentials are fp64.
+ *   counts[b]: tokens that sequence b gains, accepted ones and the last (0: no rows);
+ *   tokens[b][0 .. counts[b] - 1]: these; nodes[b][j]: the node that tokens[b][j] follows (nodes
+ *   that stay in the cache); -1 behind them.  Nodes past max_nodes are not looked at. */
+typedef struct {
+    const void* device_logits;        /* [n_rows][vocab], rows logits_row_stride apart */
+    const float* device_draft_probs;  /* [n_rows][vocab], rows probs_row_stride apart, or NULL */
+    const int32_t* device_drafts;     /* [n_rows]; a sequence's first is not looked at */
+    const int32_t* device_row_starts; /* [n_seqs + 1], or NULL: one row per sequence */
+    const int32_t* device_parents;    /* [n_rows], or NULL; a sequence's first is not looked at */
+    const double* device_uniforms;    /* [n_rows] */
+    const float* device_temperature;  /* [n_seqs], or NULL: 1 */
+    int32_t* device_tokens;           /* [n_seqs][max_nodes] */
+    int32_t* device_nodes;            /* [n_seqs][max_nodes] */
+    int32_t* device_counts;           /* [n_seqs] */
+    void* device_workspace;           /* fb2_verify_workspace bytes, 16-byte aligned */
+    int64_t workspace_bytes;
+    int64_t logits_row_stride;
+    int64_t probs_row_stride;
+    int32_t n_seqs;
+    int32_t n_rows;
+    int32_t vocab;
+    int32_t dtype;     /* of the logits */
+    int32_t max_nodes; /* 1..1024: host bound of a sequence's rows */
+    int32_t reserved;
+} fb2_verify;
+int32_t fb2_verify_workspace(const fb2_verify* v, int64_t* bytes);
+int32_t fb2_verify_drafts(const fb2_verify* v, void* cuda_stream);
+
 /* ---- synthetic weights -------------------------------------------------------
  * Host-only: fills params[i] (caller-allocated fp32 arrays of the sizes listed
  * at fb2_model_create) with the weights `new GptModel(config, backend,

@@ -53,6 +53,12 @@ int32_t fb2_test_mk_withhold(struct fb2_session* s, int32_t cta, int64_t wait_ns
  * is unaffected, and so is the next call. */
 int32_t fb2_test_kvq_withhold(int32_t tile, int64_t wait_ns);
 
+/* The next fb2_w8_matmul on tcgen05 tiles leaves out the copy of x's (few rows) or
+ * W's (many) block `block` of inputs in its first block, whose waits end after
+ * wait_ns (up to 2 s): that block's rows (and, of many, those of its later tiles)
+ * are NaN, the call returns, the next call is unaffected. */
+int32_t fb2_test_w8_withhold(int32_t block, int64_t wait_ns);
+
 /* Geometry of the session's persistent decode kernel on its first device:
  * CTAs, cluster size and attention CTAs of the head-cluster layout (0 when
  * it uses column strips), and ring stages at one row. */

@@ -1,0 +1,671 @@
+"""The serving operators around attention and 4-bit layers (pages of sequences,
+residual stream and norms, 8-bit linear layers, verification of drafts) against
+plain implementations in whole numbers or 64 bits, at the sizes and values where
+they can go wrong, and their refusals."""
+from __future__ import annotations
+
+import itertools
+import math
+import random
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+gpu = pytest.mark.gpu
+DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def within(got, want, tol):
+    """Whether every value is the rounding, in its own type, of something at
+    most tol from want (fp64): rounding is monotonic, so it lies between the
+    roundings of the ends."""
+    got, want = got.cpu(), want.cpu()
+    tol = tol.cpu() if torch.is_tensor(tol) else tol
+    low, high = (want - tol).to(got.dtype), (want + tol).to(got.dtype)
+    return bool(((got >= low) & (got <= high)).all())
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def normal(g, *shape, dtype=torch.float32):
+    return torch.randn(shape, device="cuda", generator=g).to(dtype)
+
+
+def ints(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+# ---- pages of sequences ------------------------------------------------------------
+
+class Pages:
+    """The rules in Python lists."""
+
+    def __init__(self, seqs, width, pages, page):
+        self.page, self.width = page, width
+        self.table = [[-1] * width for _ in range(seqs)]
+        self.lens = [0] * seqs
+        self.free = list(range(pages - 1, -1, -1))
+
+    def need(self, n):
+        return -(-n // self.page)
+
+    def extend(self, counts, most):
+        starts, prefix, slots, positions = [0], list(self.lens), [], []
+        asked = wanted = 0
+        had = len(self.free)
+        for b, count in enumerate(counts):
+            n = self.lens[b]
+            if count < 0 or n < 0 or n + count > self.width * self.page:
+                count = 0
+            need = self.need(n + count) - self.need(n) if count else 0
+            asked, wanted = asked + count, wanted + need
+            if asked <= most and (need == 0 or wanted <= had):
+                for i in range(need):
+                    self.table[b][self.need(n) + i] = self.free.pop()
+                for p in range(n, n + count):
+                    slots.append(self.table[b][p // self.page] * self.page + p % self.page)
+                    positions.append(p)
+                self.lens[b] = n + count
+            starts.append(len(slots))
+        return starts, prefix, slots + [-1] * (most - len(slots)), positions + [0] * (most - len(positions))
+
+    def truncate(self, lens):
+        dropped = []
+        for b, want in enumerate(lens):
+            want = max(want, 0)
+            if want < self.lens[b]:
+                for i in range(self.need(want), self.need(self.lens[b])):
+                    dropped.append(self.table[b][i])
+                    self.table[b][i] = -1
+                self.lens[b] = want
+        self.free += dropped[::-1]
+
+    def same(self, pages):
+        n = int(pages.n_free)
+        return (n == len(self.free) and pages.free[:n].tolist() == self.free and pages.lens.tolist() == self.lens
+                and pages.table.tolist() == self.table)
+
+
+@gpu
+@pytest.mark.parametrize("seqs,width,pages,page,most", [(1, 1, 1, 8, 8), (1, 40, 50, 16, 300), (3, 7, 12, 8, 40), (33, 5, 100, 16, 200),
+                                                         (1024, 3, 2000, 8, 9000), (1500, 2, 900, 32, 4000), (16384, 1, 9000, 8, 30000)])
+def test_pages_come_and_go(pkg, seqs, width, pages, page, most):
+    rng = random.Random(seqs)
+    own, want = pkg.PageTable.empty(seqs, width, pages, page), Pages(seqs, width, pages, page)
+    assert want.same(own)
+    for step in range(6):
+        counts = [rng.choice([0, 1, 1, 2, page, rng.randint(0, width * page)]) for _ in range(seqs)]
+        if step == 3:
+            counts = [-c if i % 5 == 2 else c for i, c in enumerate(counts)]  # refused one by one
+        got = own.extend(ints(counts), most)
+        for g, w in zip(got, want.extend(counts, most)):
+            assert g.dtype == torch.int32 and g.tolist() == w
+        assert want.same(own)
+        to = [rng.choice([n, n + 3, n - 1, n // 2, 0, -1]) for n in want.lens]
+        own.truncate(ints(to))
+        want.truncate(to)
+        assert want.same(own)
+
+
+@gpu
+def test_pages_that_were_dropped_come_back(pkg):
+    own = pkg.PageTable.empty(4, 8, 20, 8)
+    own.extend(ints([5, 17, 0, 30]), 64)
+    before = [t.clone() for t in (own.table, own.lens, own.free[:int(own.n_free)])]
+    first = own.extend(ints([9, 1, 8, 12]), 64)
+    own.truncate(first[1])
+    assert all(torch.equal(a, b) for a, b in zip(before, (own.table, own.lens, own.free[:int(own.n_free)])))
+    again = own.extend(ints([9, 1, 8, 12]), 64)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@gpu
+def test_pages_without_room(pkg):
+    own = pkg.PageTable.empty(3, 4, 5, 8)
+    # 3 pages, then 3 of the 2 that are left, then none
+    starts, prefix, slots, positions = own.extend(ints([20, 17, 0]), 100)
+    assert starts.tolist() == [0, 20, 20, 20] and own.lens.tolist() == [20, 0, 0] and int(own.n_free) == 2
+    assert slots[20:].eq(-1).all() and positions[20:].eq(0).all()
+    # a sequence that needs no page is served behind one that gets none
+    starts, *_ = own.extend(ints([0, 32, 0]), 100)
+    assert starts.tolist() == [0, 0, 0, 0]
+    starts, *_ = own.extend(ints([4, 0, 8]), 100)
+    assert starts.tolist() == [0, 4, 4, 12] and own.lens.tolist() == [24, 0, 8]
+    # rows: the second would pass them, the third with it
+    own.truncate(ints([0, 0, 0]))
+    starts, *_ = own.extend(ints([3, 6, 2]), 8)
+    assert starts.tolist() == [0, 3, 3, 3]
+    starts, _, slots, _ = own.extend(ints([0, 0, 0]), 0)
+    assert starts.tolist() == [0, 0, 0, 0] and slots.numel() == 0
+    # 33 tokens do not fit 4 pages of 8, whatever the others ask
+    starts, *_ = own.extend(ints([0, 33, 8]), 100)
+    assert starts.tolist() == [0, 0, 0, 8]
+
+
+@gpu
+def test_pages_of_malformed_state(pkg):
+    """Lengths, lists and counts that no sequence of calls makes: nothing outside the buffers is touched."""
+    own = pkg.PageTable.empty(4, 4, 6, 8)
+    own.lens.copy_(ints([-3, 2 ** 31 - 1, 33, 5]))
+    own.table[3, 0] = 5
+    own.free.copy_(ints([0, 9, -7, 2 ** 31 - 1, 1, 5]))
+    own.n_free.fill_(2 ** 31 - 1)  # read as 6
+    starts, prefix, slots, _ = own.extend(ints([2 ** 31 - 1, 1, 1, 20]), 50)
+    assert starts.tolist() == [0, 0, 0, 0, 20] and prefix.tolist() == [-3, 2 ** 31 - 1, 33, 5]
+    # pages 5 (its own), 5, 1 and what no page is
+    assert slots[:20].tolist() == [45, 46, 47] + list(range(40, 48)) + list(range(8, 16)) + [-1]
+    own.n_free.fill_(6)
+    own.truncate(ints([0, 0, 0, 0]))
+    assert own.lens.tolist() == [0 if n == 25 else n for n in (-3, 2 ** 31 - 1, 33, 25)]
+    assert int(own.n_free) == 6 and own.table[3].tolist() == [-1] * 4
+    own.n_free.fill_(-5)
+    starts, *_ = own.extend(ints([0, 0, 0, 1]), 8)
+    assert starts.tolist() == [0] * 5
+
+
+# ---- residual stream and norms ---------------------------------------------------------
+
+def plain_norm(v, w, b, kind, eps):
+    if kind == "layer":
+        v = v - v.mean(1, keepdim=True)
+    out = v / torch.sqrt((v * v).mean(1, keepdim=True) + eps) * w.double()
+    return out if b is None else out + b.double()
+
+
+def norm_case(g, rows, dim, dtype, stream, post, gate, bias=True, strided=False):
+    def make(n, t):
+        wide = normal(g, n, dim + (5 if strided else 0)).to(t)
+        return wide[:, 3:3 + dim] if strided else wide
+    c = dict(h=make(rows, dtype), x=2 * make(rows, stream) + 0.5, weight=1 + 0.2 * normal(g, dim),
+             bias=0.2 * normal(g, dim) if bias else None)
+    if post:
+        c.update(post_weight=1 + 0.2 * normal(g, dim), post_bias=0.2 * normal(g, dim) if bias else None)
+    if gate:
+        c["gate"] = make(rows, dtype) if gate == "rows" else normal(g, dim).to(dtype)
+    return c
+
+
+def plain_residual_norm(c, scale, kind, eps):
+    h = c["h"].double()
+    if c.get("post_weight") is not None:
+        h = plain_norm(h, c["post_weight"], c["post_bias"], kind, eps)
+    if c.get("gate") is not None:
+        h = h * c["gate"].double()
+    s = c["x"].double() + scale * h
+    return s, plain_norm(s, c["weight"], c["bias"], kind, eps)
+
+
+# A row's sums of up to 32768 terms: at most 32 in a thread, 5 steps over lanes, 32 warps, so
+# fewer than 80 roundings on one path: 2^-24 * 80 < 2^-17 relative in a mean or variance.
+SUMS = 2.0 ** -17
+
+
+def check_norm(c, got, scale, kind, eps):
+    s, y = plain_residual_norm(c, scale, kind, eps)
+    # post(h): a relative SUMS of its size (values of some units), then three roundings
+    big = s.abs().amax(1, keepdim=True).clamp(min=1) + 8
+    off = 2.0 ** -22 * big + (SUMS * 8 if c.get("post_weight") is not None else 0)
+    assert got[0].dtype == c["x"].dtype and within(got[0], s, off)
+    # y: an error of s as itself, in its mean and in its variance, over the row's spread; sums as said
+    v = s - s.mean(1, keepdim=True) if kind == "layer" else s
+    spread = torch.sqrt((v * v).mean(1, keepdim=True) + eps)
+    off = (4 * off / spread + 2 * SUMS * (1 + v.abs() / spread + s.abs().mean(1, keepdim=True) / spread)) * 2 + 2.0 ** -22
+    assert within(got[1], y, off * (1 + v.abs() / spread))
+
+
+@gpu
+@pytest.mark.parametrize("dtype,stream", [("fp32", "fp32"), ("bf16", "bf16"), ("bf16", "fp32"), ("fp16", "fp16"), ("fp16", "fp32")])
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("rows,dim", [(1, 768), (5, 64), (3, 1), (7, 257), (9, 1000), (2, 1025), (4, 4096), (3, 5001), (2, 16384), (2, 32767)])
+def test_residual_and_norm(pkg, dtype, stream, kind, rows, dim):
+    g = gen(rows * dim)
+    for post, gate, strided in ((False, None, False), (True, "rows", False), (True, "all", True), (False, "rows", True)):
+        c = norm_case(g, rows, dim, DTYPES[dtype], DTYPES[stream], post, gate, bias=kind == "layer", strided=strided)
+        got = pkg.residual_norm(c["h"], c["x"], c["weight"], c["bias"], post_weight=c.get("post_weight"),
+                                post_bias=c.get("post_bias"), gate=c.get("gate"), scale=0.7, kind=kind, eps=1e-5)
+        assert got[1].dtype == DTYPES[dtype]
+        check_norm(c, got, 0.7, kind, 1e-5)
+
+
+@gpu
+@pytest.mark.parametrize("stream", ["fp32", "bf16"])
+def test_norm_alone(pkg, stream):
+    g = gen(1)
+    c = norm_case(g, 6, 333, torch.bfloat16, DTYPES[stream], False, None)
+    c["h"] = torch.zeros_like(c["h"])
+    got = pkg.residual_norm(None, c["x"], c["weight"], c["bias"], dtype=torch.bfloat16)
+    assert got[0] is c["x"] and got[1].dtype == torch.bfloat16
+    check_norm(c, got, 1.0, "layer", 1e-5)
+    assert pkg.residual_norm(None, c["x"], c["weight"])[1].dtype == DTYPES[stream]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("rows,dim", [(1, 768), (11, 33), (4, 1024), (5, 4099)])
+def test_norm_into_codes(pkg, dtype, kind, rows, dim):
+    """The codes stand for y to half a step of its row, and the error that y itself may have."""
+    g = gen(dim)
+    c = norm_case(g, rows, dim, DTYPES[dtype], torch.float32, True, "rows")
+    args = dict(post_weight=c["post_weight"], post_bias=c["post_bias"], gate=c["gate"], scale=1.3, kind=kind)
+    s, codes, scales = pkg.residual_norm(c["h"], c["x"], c["weight"], c["bias"], quantise=True, **args)
+    dense = pkg.residual_norm(c["h"], c["x"], c["weight"], c["bias"], **args)
+    assert torch.equal(s, dense[0]) and codes.dtype == torch.int8 and scales.dtype == torch.float32
+    assert codes.shape == (rows, dim) and codes.stride(0) % 16 == 0
+    _, y = plain_residual_norm(c, 1.3, kind, 1e-5)
+    top = y.abs().amax(1)
+    assert ((scales.double() - top / 127).abs() <= 1e-4 * top / 127).all()
+    step = scales.double()[:, None]
+    assert ((codes.double() * step - y).abs() <= 0.5 * step * (1 + 1e-4) + 1e-4 * (1 + y.abs())).all()
+    if dtype == "fp32":  # y in hand: the codes are its own
+        again, its = pkg.quantise_rows(dense[1])
+        assert torch.equal(again, codes) and torch.equal(its, scales)
+
+
+@gpu
+def test_norm_of_special_rows(pkg):
+    x = torch.randn((6, 100), generator=torch.Generator().manual_seed(2))
+    x[1] = 3.0                    # no variance
+    x[2, 5] = math.nan
+    x[3, 7] = math.inf
+    x[4] = 0.0
+    x = x.cuda()
+    h = torch.zeros_like(x)
+    w, b = torch.ones(100, device="cuda"), torch.full((100,), 0.25, device="cuda")
+    for kind in ("layer", "rms"):
+        s, y = pkg.residual_norm(h, x, w, b, kind=kind)
+        assert torch.equal(s.nan_to_num(9), x.nan_to_num(9)) and y[2].isnan().all() and y[0].isfinite().all() and y[5].isfinite().all()
+        assert not y[3].isfinite().all() and y[4].eq(0.25).all()
+        assert y[1].sub(0.25 if kind == "layer" else 1.25).abs().max() < 1e-5
+        _, codes, scales = pkg.residual_norm(h, x, w, b, kind=kind, quantise=True)
+        assert scales[2].isnan() and scales[3].isnan() and codes[2].eq(0).all() and scales[[0, 1, 4, 5]].isfinite().all()
+
+
+# ---- rows as codes, 8-bit products ---------------------------------------------------------
+
+def plain_codes(x):
+    """The formula, with its roundings to fp32."""
+    x = x.float().cpu()
+    top = x.abs().amax(-1, keepdim=True)
+    live = top >= 1e-35
+    inv = torch.div(torch.tensor(127.0), torch.where(live, top, 1.0))
+    codes = torch.where(live, torch.round(x * inv), 0.0)
+    return codes, torch.where(live, top / torch.tensor(127.0), 0.0).squeeze(-1)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("rows,dim", [(1, 1), (3, 16), (5, 77), (2, 768), (9, 2056), (2, 40001)])
+def test_rows_as_codes(pkg, dtype, rows, dim):
+    g = gen(dim)
+    x = normal(g, rows, dim)
+    x[::2] = torch.round(x[::2] * 8) / 8  # many values halfway
+    for x in (x.to(DTYPES[dtype]), normal(g, rows, dim + 3, dtype=DTYPES[dtype])[:, 1:1 + dim]):
+        codes, scales = pkg.quantise_rows(x)
+        want, its = plain_codes(x)
+        assert torch.equal(codes.cpu().float(), want) and torch.equal(scales.cpu(), its)
+        assert codes.data_ptr() % 16 == 0 and (rows == 1 or codes.stride(0) % 16 == 0)
+
+
+@gpu
+def test_codes_of_special_rows(pkg):
+    x = torch.randn((7, 50), generator=torch.Generator().manual_seed(3))
+    x[0] = 0.0
+    x[1, 4], x[2, 49], x[3, 0] = math.nan, math.inf, -math.inf
+    x[4] *= 1e-38
+    x[5] *= 1e37
+    codes, scales = pkg.quantise_rows(x.cuda())
+    codes, scales = codes.cpu(), scales.cpu()
+    assert scales[1:4].isnan().all() and codes[:5].eq(0).all() and scales[0] == 0 and scales[4] == 0
+    for r in (5, 6):
+        want, its = plain_codes(x[r:r + 1])
+        assert torch.equal(codes[r:r + 1].float(), want) and scales[r] == its[0]
+
+
+def w8_case(pkg, g, k, n, bias=True, pad=0):
+    codes = torch.full((n, -(-k // 16) * 16 + pad), 99, dtype=torch.int8, device="cuda")[:, :k]  # what is behind a row does not count
+    codes.copy_(torch.randint(-128, 128, (n, k), device="cuda", generator=g))
+    return pkg.W8Linear(codes, torch.rand(n, device="cuda", generator=g) + 0.1, normal(g, n) if bias else None)
+
+
+def check_w8(linear, codes, scales, got):
+    """Exact sums; a fp32 rounding of the sum, two products and an addition."""
+    sums = codes.double().cpu() @ linear.codes.double().cpu().T
+    part = sums * linear.scales.double().cpu() * scales.double().cpu()[:, None]
+    bias = 0.0 if linear.bias is None else linear.bias.double().cpu()
+    assert within(got, part + bias, 2.0 ** -24 * (3 * part.abs() + (part + bias).abs()) * 1.01)
+
+
+ROWS = [1, 2, 5, 8, 9, 16, 17, 32, 33, 64, 65, 128, 129, 200, 300]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("k,n", [(1, 1), (16, 7), (100, 130), (128, 128), (768, 257), (1000, 33), (2064, 400)])
+def test_products_of_codes(pkg, dtype, k, n):
+    g = gen(k + n)
+    linear = w8_case(pkg, g, k, n, bias=n % 2 == 1, pad=16 * (k % 3))
+    for rows in ROWS:
+        x = torch.randint(-128, 128, (rows, -(-k // 16) * 16 + 16), device="cuda", generator=g).to(torch.int8)[:, :k]
+        scales = torch.rand(rows, device="cuda", generator=g) + 0.1
+        y = linear(x, scales=scales, dtype=DTYPES[dtype])
+        assert y.shape == (rows, n) and y.dtype == DTYPES[dtype]
+        check_w8(linear, x, scales, y)
+
+
+@gpu
+@pytest.mark.parametrize("rows,k,n", [(1, 131072, 40), (3, 40000, 300), (20, 16384, 128), (1, 8192, 9000), (700, 520, 1100),
+                                      (1500, 4096, 520), (4100, 256, 700)])
+def test_products_of_codes_at_length(pkg, rows, k, n):
+    g = gen(k + n)
+    linear = w8_case(pkg, g, k, n)
+    linear.codes[: n // 2].fill_(-128)  # the largest sums there are
+    x = torch.randint(-128, 128, (rows, k), device="cuda", generator=g).to(torch.int8)
+    x[0] = 127
+    scales = torch.rand(rows, device="cuda", generator=g) + 0.1
+    check_w8(linear, x, scales, linear(x, scales=scales))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("rows,k,n", [(1, 768, 2304), (1, 77, 50), (4, 1000, 60), (13, 512, 1000), (150, 640, 96), (1, 8200, 64)])
+def test_products_of_values(pkg, dtype, rows, k, n):
+    g = gen(k)
+    linear = w8_case(pkg, g, k, n)
+    x = normal(g, rows, k + 2, dtype=DTYPES[dtype])
+    for x in (x[:, 1:1 + k], x[:, :k].contiguous()):
+        y = linear(x)
+        assert y.dtype == DTYPES[dtype]
+        codes, scales = plain_codes(x)
+        check_w8(linear, codes, scales, y)
+        assert torch.equal(y, linear(*pkg.quantise_rows(x), dtype=DTYPES[dtype]))
+    assert torch.equal(linear(x.view(1, rows, 1, k))[0, :, 0], y)
+    assert linear(x, dtype=torch.float32).dtype == torch.float32
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 3, 140])
+def test_products_of_special_rows(pkg, rows):
+    g = gen(9)
+    linear = w8_case(pkg, g, 300, 150)
+    x = normal(g, rows, 300)
+    x[rows // 2, 17] = math.nan
+    y = linear(x)
+    assert y[rows // 2].isnan().all()
+    keep = [r for r in range(rows) if r != rows // 2]
+    assert y[keep].isfinite().all()
+    assert torch.equal(linear(torch.zeros_like(x)), linear.bias.expand(rows, 150))
+    assert linear(x[:0]).shape == (0, 150)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("k,n", [(64, 16), (100, 77), (1, 40), (300, 130), (513, 32)])
+def test_pack_of_8_bit_weights(pkg, dtype, k, n):
+    g = gen(n)
+    for w in (normal(g, k, n, dtype=DTYPES[dtype]), normal(g, k, n + 3, dtype=DTYPES[dtype])[:, 2:2 + n], normal(g, 1, n, dtype=DTYPES[dtype]).expand(k, n)):
+        linear = pkg.W8Linear.pack(w)
+        codes, scales = plain_codes(w.T)
+        assert torch.equal(linear.codes.cpu().float(), codes) and torch.equal(linear.scales.cpu(), scales)
+        assert linear.in_features == k and linear.out_features == n
+    w[0, n // 2:] = math.inf
+    y = pkg.W8Linear.pack(w.clone())(torch.ones((2, k), device="cuda"))
+    assert y[:, n // 2:].isnan().all() and y[:, :n // 2].isfinite().all()
+
+
+# ---- verification of drafts -----------------------------------------------------------------
+
+def plain_verify(logits, drafts, uniforms, starts, parents=None, probs=None, heat=None, wide=None):
+    """The rules in fp64, one row after another."""
+    logits, uniforms = logits.double().cpu(), uniforms.cpu()
+    probs = None if probs is None else probs.double().cpu()
+    tokens, nodes, counts = [], [], []
+    for b in range(len(starts) - 1):
+        a, n = starts[b], min(starts[b + 1] - starts[b], wide)
+        t = 1.0 if heat is None else float(heat[b])
+        if n == 0:
+            tokens.append([-1] * wide), nodes.append([-1] * wide), counts.append(0)
+            continue
+
+        def target(i):
+            x = logits[a + i]
+            if x.isnan().any() or x.max() == math.inf or x.max() == -math.inf:
+                return None
+            if t > 0:
+                e = torch.exp((x - x.max()) / t)
+                return torch.where(x == -math.inf, 0.0, e / e.sum()) if math.isinf(t) is False else (x > -math.inf).double() / (x > -math.inf).sum()
+            return torch.zeros_like(x).index_fill_(0, (x == x.max()).nonzero()[0], 1.0)
+
+        at, said, path = 0, [], [0]
+        while True:
+            p = target(at)
+            left, gone = (p, set())
+            taken = None
+            for i in range(at + 1, n):
+                if (i - 1 if parents is None else parents[a + i]) != at or p is None:
+                    continue
+                x, u = int(drafts[a + i]), float(uniforms[a + i])
+                here = float(left[x]) if 0 <= x < len(left) else 0.0
+                if probs is not None:
+                    q = float(probs[a + i, x]) if 0 <= x < len(p) else math.nan
+                    if u * q < float(p[x] if 0 <= x < len(p) else 0):
+                        taken = i
+                        break
+                    left = (p - probs[a + i]).clamp(min=0)
+                    left = p if float(left.sum()) == 0 else left
+                else:
+                    if u * float(left.sum()) < here:
+                        taken = i
+                        break
+                    if 0 <= x < len(left):
+                        left = left.clone()
+                        left[x] = 0
+            if taken is None:
+                break
+            said.append(int(drafts[a + taken]))
+            path.append(taken)
+            at = taken
+        if p is None:
+            said.append(-1)
+        else:
+            left = p if float(left.sum()) == 0 else left
+            run = torch.cumsum(left, 0)
+            past = (run > float(uniforms[a]) * float(run[-1])).nonzero()
+            said.append(int(past[0]) if len(past) else int(left.nonzero()[-1]))
+        tokens.append(said + [-1] * (wide - len(said)))
+        nodes.append(path + [-1] * (wide - len(path)))
+        counts.append(len(said))
+    return tokens, nodes, counts
+
+
+def check_verify(pkg, logits, drafts, uniforms, starts, parents=None, probs=None, heat=None, wide=None, **more):
+    wide = wide or max(1, max(b - a for a, b in zip(starts, starts[1:])))
+    got = pkg.verify_drafts(logits, drafts, uniforms, starts=ints(starts), parents=None if parents is None else ints(parents),
+                            draft_probs=probs, temperature=None if heat is None else torch.tensor(heat, device="cuda"),
+                            max_nodes=wide, **more)
+    want = plain_verify(logits, drafts.tolist(), uniforms, starts, parents, probs,
+                        None if heat is None else torch.tensor(heat).tolist(), wide)
+    for g, w in zip(got, want):
+        assert g.dtype == torch.int32 and g.tolist() == w
+    return got
+
+
+def verify_case(g, rng, nodes, vocab, dtype, tree, peak=8.0):
+    rows = sum(nodes)
+    logits = normal(g, rows, vocab)
+    logits += peak * (torch.rand((rows, vocab), device="cuda", generator=g) < 4 / vocab)
+    starts, parents = [0], []
+    for n in nodes:
+        parents += [rng.randrange(i) if i and tree else i - 1 for i in range(n)]
+        starts.append(starts[-1] + n)
+    first = [s for s, n in zip(starts, nodes) for _ in range(n)]
+    above = [max(f + p, 0) for f, p in zip(first, parents)]
+    logits = logits.to(dtype)
+    best = logits.float().topk(min(vocab, 3), 1).indices
+    drafts = ints([int(best[a, rng.randrange(best.shape[1])]) for a in above])
+    uniforms = torch.rand(rows, device="cuda", generator=g, dtype=torch.float64)
+    return logits, drafts, uniforms, starts, parents, above
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("vocab", [1, 2, 17, 1000, 4099, 16384, 50257])
+def test_verification_of_trees(pkg, dtype, vocab):
+    g, rng = gen(vocab), random.Random(vocab)
+    for turn in range(4):
+        nodes = [1, 2, 9, rng.randint(1, 40), 0, 5]
+        logits, drafts, uniforms, starts, parents, _ = verify_case(g, rng, nodes, vocab, DTYPES[dtype], True)
+        check_verify(pkg, logits, drafts, uniforms, starts, parents, heat=[0.7, 1.0, 0.0, 1.3, 1.0, 0.8])
+        check_verify(pkg, logits, drafts, uniforms, starts)  # as chains
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("vocab", [1, 2, 17, 1000, 4099, 16384, 50257])
+def test_verification_of_drawn_chains(pkg, dtype, vocab):
+    g, rng = gen(vocab), random.Random(vocab)
+    for turn in range(4):
+        nodes = [3, 1, 6, 2, 12]
+        logits, _, uniforms, starts, _, above = verify_case(g, rng, nodes, vocab, DTYPES[dtype], False)
+        probs = torch.softmax(logits.float()[above] + normal(g, len(above), vocab), 1)
+        drafts = torch.multinomial(probs, 1, generator=g).squeeze(1).to(torch.int32)
+        check_verify(pkg, logits, drafts, uniforms, starts, probs=probs, heat=[1.0, 0.9, 0.0, 1.2, 0.8])
+        wide = torch.zeros((len(above), vocab + 5), device="cuda")  # rows that begin anywhere
+        wide[:, 3:3 + vocab] = probs
+        logits2 = torch.zeros((len(above), vocab + 3), device="cuda", dtype=DTYPES[dtype])
+        logits2[:, 1:1 + vocab] = logits
+        check_verify(pkg, logits2[:, 1:1 + vocab], drafts, uniforms, starts, probs=wide[:, 3:3 + vocab])
+
+
+@gpu
+def test_verification_of_one_row_each(pkg):
+    g = gen(4)
+    logits = normal(g, 300, 5000, dtype=torch.bfloat16)
+    uniforms = torch.rand(300, device="cuda", generator=g, dtype=torch.float64)
+    drafts = torch.zeros(300, dtype=torch.int32, device="cuda")
+    tokens, nodes, counts = pkg.verify_drafts(logits, drafts, uniforms)
+    want = plain_verify(logits, drafts.tolist(), uniforms, list(range(301)), wide=1)
+    assert tokens.tolist() == want[0] and nodes.eq(0).all() and counts.eq(1).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_verification_next_to_borders(pkg, dtype):
+    """Draws just inside both ends of tokens' intervals, the narrowest of them 2^-30 of the widest.
+    Uniforms and running sums up to total < 2.1 are fp64: 8 of each are off by less than 2^-49 total together, so
+    that a draw as far inside is the token's (2^-30 * 1e-9 inside would round to the end itself)."""
+    vocab = 64
+    powers = [0, 3, 1, 2, 5, 4, 8, 30]
+    x = torch.full((1, vocab), -math.inf)
+    for i, k in enumerate(powers):
+        x[0, 5 * i + 1] = -k * math.log(2.0)
+    heat = 1.0
+    weights = [math.exp(float(x[0, 5 * i + 1].to(DTYPES[dtype]).double())) for i in range(len(powers))]
+    total = math.fsum(weights)
+    draws, want, run = [], [], 0.0
+    for i, w in enumerate(weights):
+        inside = max(w * 1e-9, 2.0 ** -49 * total)
+        for u in ((run + inside) / total, (run + w - inside) / total):
+            draws.append(u), want.append(5 * i + 1)
+        run += w
+    rows = len(draws)
+    logits = x.to(DTYPES[dtype]).cuda().expand(rows, vocab).contiguous()
+    uniforms = torch.tensor(draws, dtype=torch.float64, device="cuda")
+    tokens, _, _ = pkg.verify_drafts(logits, torch.zeros(rows, dtype=torch.int32, device="cuda"), uniforms,
+                                     temperature=torch.full((rows,), heat, device="cuda"))
+    assert tokens[:, 0].tolist() == want
+    # the ends of the uniforms, and what is none
+    ends = torch.tensor([0.0, 1 - 2.0 ** -53, 1.0, -1.0, math.nan], dtype=torch.float64, device="cuda")
+    tokens, _, _ = pkg.verify_drafts(logits[:5], torch.zeros(5, dtype=torch.int32, device="cuda"), ends)
+    assert tokens[:, 0].tolist() == [1, 36, 36, 1, 36]
+
+
+@gpu
+def test_verification_of_rows_without_probabilities(pkg):
+    g = gen(6)
+    logits = normal(g, 12, 3000)
+    logits[1] = -math.inf
+    logits[3, 7] = math.nan
+    logits[5, 2999] = math.inf
+    logits[7] = -math.inf
+    logits[7, 11] = -5.0       # one that is left
+    logits[9, ::2] = -math.inf
+    drafts = logits.nan_to_num(0).argmax(1).to(torch.int32)
+    drafts[0] = -1
+    drafts = drafts.roll(1)
+    uniforms = torch.rand(12, device="cuda", generator=g, dtype=torch.float64)
+    for heat in ([1.0] * 6, [0.0] * 6, [-1.0] * 6, [math.inf] * 6, [1e-30] * 6):
+        check_verify(pkg, logits, drafts, uniforms, list(range(0, 13, 2)), heat=heat)
+        check_verify(pkg, logits, drafts, uniforms * 0, [0, 4, 8, 12], heat=heat[:3])
+
+
+@gpu
+def test_verification_of_same_and_unknown_drafts(pkg):
+    """Siblings with the same token, tokens outside the vocabulary, parents that are none."""
+    g = gen(8)
+    vocab = 40
+    logits = normal(g, 14, vocab)
+    top = int(logits[0].argmax())
+    drafts = ints([0, top, top, 999, -5, vocab, top, 3, 3, 4, 5, 6, 7, 2 ** 31 - 1])
+    parents = [0] * 14
+    for u in (0.0, 0.3, 0.6, 0.999999):
+        uniforms = torch.full((14,), u, device="cuda", dtype=torch.float64)
+        check_verify(pkg, logits, drafts, uniforms, [0, 14], parents, heat=[1.0])
+    odd = [5, 7, -1, 2 ** 31 - 1, 4, 0, 99, 0, 0, 9, 1, 0, 2, 0]
+    uniforms = torch.rand(14, device="cuda", generator=g, dtype=torch.float64)
+    seen = [p if 0 <= p < i else -1 for i, p in enumerate(odd)]
+    want = plain_verify(logits, drafts.tolist(), uniforms, [0, 14], seen, wide=14)
+    got = pkg.verify_drafts(logits, drafts, uniforms, starts=ints([0, 14]), parents=ints(odd))
+    assert [t.tolist() for t in got] == list(want)
+    # every token of the vocabulary rejected, one after another
+    logits = torch.zeros((vocab + 1, vocab), device="cuda")
+    drafts = ints([0] + list(range(vocab)))
+    uniforms = torch.full((vocab + 1,), 2.0, device="cuda", dtype=torch.float64)
+    got = pkg.verify_drafts(logits, drafts, uniforms, starts=ints([0, vocab + 1]), parents=ints([0] * (vocab + 1)))
+    assert got[2].tolist() == [1] and got[0][0, 0] == vocab - 1
+
+
+@gpu
+def test_verification_cuts_nodes(pkg):
+    g, rng = gen(5), random.Random(5)
+    logits, drafts, uniforms, starts, parents, _ = verify_case(g, rng, [20, 3, 1024], 300, torch.float32, True, peak=2.0)
+    check_verify(pkg, logits, drafts, uniforms, starts, parents, wide=6)
+    check_verify(pkg, logits, drafts, uniforms, starts, parents)
+
+
+@gpu
+def test_verification_of_malformed_starts(pkg):
+    """Starts that descend or lie outside: nothing outside the tensors is touched; sequences in order come out right."""
+    g, rng = gen(5), random.Random(5)
+    logits, drafts, uniforms, _, _, _ = verify_case(g, rng, [4, 4], 500, torch.float32, False)
+    for starts in ([0, 4, 4, 8], [-7, 4, 100, 300], [8, 0, 8], [5, 3, 8], [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1]):
+        tokens, nodes, counts = pkg.verify_drafts(logits, drafts, uniforms, starts=ints(starts), max_nodes=8)
+        assert counts.ge(0).all() and counts.le(8).all()
+    want = plain_verify(logits, drafts.tolist(), uniforms, [0, 4, 8, 8], wide=8)
+    tokens, nodes, counts = pkg.verify_drafts(logits, drafts, uniforms, starts=ints([-7, 4, 100, 300]), max_nodes=8)
+    assert tokens.tolist() == want[0] and counts.tolist() == want[2]
+
+
+@gpu
+@pytest.mark.parametrize("drawn", [False, True])
+def test_accepted_tokens_are_distributed_as_the_target(pkg, drawn):
+    """The first token of many sequences against p: 40000 of them, so that a count's deviation is
+    sqrt(n p (1 - p)) and 6 of them hold for all 12 tokens but once in some 10^8 runs."""
+    g = gen(11)
+    n, vocab = 40000, 12
+    one, other = normal(g, vocab), normal(g, vocab)
+    p, q = torch.softmax(one.double(), 0), torch.softmax(other, 0)
+    logits = one.expand(2 * n, vocab).contiguous()
+    starts = torch.arange(0, 2 * n + 1, 2, dtype=torch.int32, device="cuda")
+    uniforms = torch.rand(2 * n, device="cuda", generator=g, dtype=torch.float64)
+    drafts = torch.multinomial(q, 2 * n, replacement=True, generator=g).to(torch.int32)
+    probs = q.expand(2 * n, vocab).contiguous() if drawn else None
+    if not drawn:
+        drafts = torch.full_like(drafts, 3)
+    tokens, _, _ = pkg.verify_drafts(logits, drafts, uniforms, starts=starts, draft_probs=probs, max_nodes=2)
+    counts = torch.bincount(tokens[:, 0].long(), minlength=vocab).double()
+    assert ((counts - n * p).abs() <= 6 * torch.sqrt(n * p * (1 - p))).all()
