@@ -368,7 +368,7 @@ int32_t fb2_verify_drafts(const fb2_verify* v, void* stream) {
         with_type(v->dtype, [&](auto t) {
             using T = decltype(t);
             if (a.n_rows) launch_cluster(k_verify_rows<T>, dim3(a.n_rows * a.ranks), VF_THREADS, 0, a.ranks, false, stream, a);
-            launch_cluster(k_verify_walk<T>, dim3(a.n_seqs * a.ranks), VF_THREADS, 0, a.ranks, true, stream, a);
+            launch_cluster(k_verify_walk<T>, dim3(a.n_seqs * a.ranks), VW_THREADS, 0, a.ranks, a.n_rows > 0, stream, a);
         });
     });
 }

@@ -11,8 +11,12 @@
 // looked through.
 //
 // Which id a draw gives hangs on running sums over a whole row: in 32 bits they
-// are off by some 1e-7 of the total, wider than most tokens of a large vocabulary,
-// so exponentials and sums are in 64 bits here.
+// are off by some 1e-6 of the total, wider than most tokens of a large vocabulary,
+// so the weights of the draw's row and their sums are in 64 bits.  Whether a draft is
+// accepted hangs on one comparison, which a sum from 32-bit exponentials decides
+// but for one uniform in some 2^16; where it does not, that row is summed in 64 bits
+// first.  So every decision is that of fp64, and all rows but one of a sequence are
+// read at the cost of 32-bit exponentials.
 #pragma once
 #include "kvq.cuh"
 #include "pages.cuh"
@@ -20,9 +24,19 @@
 namespace fb2 {
 
 constexpr int VF_THREADS = 256, VF_WARPS = VF_THREADS / 32, VF_NODES = 1024, VF_RANKS = 8;
+constexpr int VW_THREADS = 512, VW_WARPS = VW_THREADS / 32;
+constexpr int VW_BATCH = 8;                 // loads of a lane that are in flight at once
+constexpr int VW_RUN = 32 * VW_BATCH;       // ids of a warp's batch
+constexpr int VW_PARTS = 16;                // of a warp's ids, each with its own sum
+// How far a sum of k_verify_rows may be off, relative.  An exponent (l - top) * log2(e) / T
+// has three roundings, and the exponents' mean under p is at most log2(vocab) <= 31: 31 *
+// 3 * 2^-24 * ln 2; ex2.approx 2^-22; a sum of 8 in fp32, the rest in fp64: 2^-21.
+// Together below 2^-17.  Twice that, for the products it enters.
+constexpr double VF_OFF = 1.0 / 65536;
+constexpr float VF_COLD = 1e-30f;  // a T below is not divided by in 32 bits: all its tests go by 64
 
 struct VerifyRow {
-    double sum;  // of exp((l - top) / T); not positive and finite where the row has no probabilities
+    double sum;  // of exp((l - top) / T), to VF_OFF; not positive and finite where the row has no probabilities
     float top;
     int best;  // the lowest id of the largest logit (T <= 0)
 };
@@ -72,9 +86,63 @@ FB2_DEV double warp_sum(double v) {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-// exp((l - top) / T) with cold = 1 / T; 0 for l = -inf, whatever T is
-FB2_DEV double weight(float l, float top, double cold) {
-    return l == -INFINITY ? 0.0 : exp(((double)l - (double)top) * cold);
+FB2_DEV float ex2(float x) {
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 2^(i / 256), i = 0..255: what the exponentials in 64 bits are looked up in.
+FB2_DEV void fill_powers(double* powers) {
+    for (int i = threadIdx.x; i < 256; i += blockDim.x) powers[i] = exp2((double)i / 256);
+}
+// exp((l - top) / T) with cold = 256 log2(e) / T, by a table and a polynomial (P. T. P.
+// Tang, Table-driven implementation of the exponential function, ACM TOMS 15, 1989):
+// 2^(n / 256) from the table and the exponent, exp(t), |t| <= ln 2 / 512, from its
+// series to t^4 (t^5 / 120 < 2^-54).  l <= top; 0 where it falls below 2^-1000.
+FB2_DEV double weight(float l, float top, double cold, const double* powers) {
+    double x = ((double)l - (double)top) * cold;
+    if (!(x > -256000.0)) x = -256000.0;  // (-inf too)
+    const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the nearest whole number
+    const double high = x + magic;
+    const int n = __double2loint(high);
+    const double t = (x - (high - magic)) * 2.70760617406228636e-3;  // ln 2 / 256
+    double e = fma(t, 1.0 / 24, 1.0 / 6);
+    e = fma(e, t, 0.5);
+    e = fma(e, t, 1.0);
+    const double p = powers[n & 255];
+    e = fma(e * t, p, p);
+    if (n <= -256000) return 0.0;
+    return __hiloint2double(__double2hiint(e) + ((n >> 8) << 20), __double2loint(e));
+}
+// The first k in 0..n-1 whose running sum over `part`, from `passed` on, passes the
+// target, else the last with a positive part (-1: none); `passed` becomes the sum
+// before it.  By the lanes of a warp.
+template <class F>
+FB2_DEV int pick(F part, int n, double target, double& passed) {
+    const int lane = threadIdx.x & 31, per = (n + 31) / 32, k0 = min(lane * per, n), k1 = min(k0 + per, n);
+    double sum = 0.0;
+    for (int k = k0; k < k1; k++) sum += fmax(part(k), 0.0);
+    double up = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const double v = __shfl_up_sync(0xffffffffu, up, o);
+        if (lane >= o) up += v;
+    }
+    const uint32_t over = __ballot_sync(0xffffffffu, sum > 0.0 && passed + up > target), any = __ballot_sync(0xffffffffu, sum > 0.0);
+    if (!any) return -1;
+    const int chosen = over ? __ffs(over) - 1 : 31 - __clz(any);
+    int at = -1;
+    double before = passed + (up - sum), run = before;
+    if (lane == chosen)
+        for (int k = k0; k < k1; k++) {
+            const double v = part(k);
+            if (!(v > 0.0)) continue;
+            at = k, before = run;
+            run += v;
+            if (run > target) break;
+        }
+    passed = __shfl_sync(0xffffffffu, before, chosen);
+    return __shfl_sync(0xffffffffu, at, chosen);
 }
 // The sequence of a row: the last b with starts[b] <= row, by all lanes.
 FB2_DEV int owner(const int* starts, int n, int row) {
@@ -98,6 +166,7 @@ __global__ void __launch_bounds__(VF_THREADS) k_verify_rows(VerifyArgs a) {
     __shared__ double s_sum[VF_WARPS], c_sum;
     __shared__ float s_top[VF_WARPS], c_top;
     __shared__ int s_best[VF_WARPS], c_best;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the walk's launch; it waits for this grid's end
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int ranks = a.ranks, rank = blockIdx.x % ranks, row = blockIdx.x / ranks;
     const int b = a.starts ? vf::owner(a.starts, a.n_seqs, row) : row;
@@ -109,52 +178,64 @@ __global__ void __launch_bounds__(VF_THREADS) k_verify_rows(VerifyArgs a) {
     }
     const float heat = a.heat(b);
     const bool greedy = !(heat > 0.f);
-    const double cold = greedy ? 0.0 : 1.0 / (double)heat;
+    // (not 0 for T = inf: -inf times it is -inf)
+    const float cold = fmaxf(1.44269504088896341f / (greedy ? 1.f : fmaxf(heat, VF_COLD)), 1e-44f);
     const T* p = (const T*)a.logits + row * a.logits_row;
     constexpr int N = 16 / sizeof(T);
     // ids before the first 16-byte boundary, pieces of 16 bytes, the rest
     const int head = min(a.vocab, (int)(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T)));
     const int pieces = (a.vocab - head) / N, per = (pieces + ranks - 1) / ranks;
     const int p0 = min(rank * per, pieces), p1 = min(p0 + per, pieces);
-    float top = -INFINITY;
+    float top = -3.402823466e38f;  // (finite: -inf less this is -inf)
     double sum = 0.0;
-    int best = INT_MAX;
-    auto take = [&](const float* v, int n, int id) {
-        float most = v[0];
-        for (int i = 1; i < n; i++) most = fmaxf(most, v[i]);
-        if (greedy) {
-            for (int i = 0; i < n; i++)
-                if (v[i] > top) top = v[i], best = id + i;
-        } else if (most > top) {
-            sum *= vf::weight(top, most, cold);
-            top = most;
+    int best = -1;
+    auto raise = [&](float to) {
+        if (to > top) {
+            sum *= (double)vf::ex2((top - to) * cold);
+            top = to;
         }
-        for (int i = 0; i < n; i++) sum += vf::weight(v[i], top, cold);
     };
-    if (rank == 0 && tid < head) {
-        const float v = Dense<T>::get(p[tid]);
-        take(&v, 1, tid);
+    auto term = [&](float v) { return vf::ex2((v - top) * cold); };  // NaN for NaN, and for all where one is inf
+    const uint4* body = reinterpret_cast<const uint4*>(p + head);
+    constexpr int M = 4;  // loads in flight
+    for (int i0 = p0 + tid; i0 < p1; i0 += M * VF_THREADS) {
+        uint4 w[M];
+#pragma unroll
+        for (int m = 0; m < M; m++) w[m] = i0 + m * VF_THREADS < p1 ? __ldg(body + i0 + m * VF_THREADS) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int m = 0; m < M; m++) {
+            const int i = i0 + m * VF_THREADS;
+            if (i >= p1) break;
+            float v[N];
+            unpack16<T>(w[m], v);
+            float most = v[0];
+#pragma unroll
+            for (int j = 1; j < N; j++) most = fmaxf(most, v[j]);
+            if (greedy && (most > top || (most == top && best < 0)))
+#pragma unroll
+                for (int j = N - 1; j >= 0; j--)
+                    if (v[j] == most) best = head + i * N + j;
+            raise(most);
+            float part = 0.f;
+#pragma unroll
+            for (int j = 0; j < N; j++) part += term(v[j]);
+            sum += (double)part;
+        }
     }
-    for (int i = p0 + tid; i < p1; i += VF_THREADS) {
-        float v[N];
-        unpack16<T>(__ldg(reinterpret_cast<const uint4*>(p + head) + i), v);
-        take(v, N, head + i * N);
-    }
-    if (rank == ranks - 1 && head + pieces * N + tid < a.vocab) {
-        const int id = head + pieces * N + tid;
-        const float v = Dense<T>::get(p[id]);
-        take(&v, 1, id);
-    }
-    // (top, sum, best) of the warp, the CTA, the cluster
+    // (top, sum, best) with another part's
     auto join = [&](float t2, double s2, int b2) {
         const float t = fmaxf(top, t2);
-        if (!greedy)
-            sum = sum * vf::weight(top, t, cold) + s2 * vf::weight(t2, t, cold);
-        else
-            sum += s2;
-        best = top > t2 ? best : t2 > top ? b2 : min(best, b2);
+        sum = sum * (double)vf::ex2((top - t) * cold) + s2 * (double)vf::ex2((t2 - t) * cold);
+        if (best < 0 || (b2 >= 0 && (t2 > top || (t2 == top && b2 < best)))) best = b2;
         top = t;
     };
+    auto edge = [&](int id) {
+        const float v = Dense<T>::get(p[id]);
+        const bool more = v > -3.402823466e38f;
+        join(more ? v : -3.402823466e38f, v == -INFINITY ? 0.0 : v == v && v < INFINITY ? 1.0 : (double)NAN, v > -INFINITY ? id : -1);
+    };
+    if (rank == 0 && tid < head) edge(tid);
+    if (rank == ranks - 1 && head + pieces * N + tid < a.vocab) edge(head + pieces * N + tid);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         const float t2 = __shfl_xor_sync(0xffffffffu, top, o);
@@ -177,175 +258,228 @@ __global__ void __launch_bounds__(VF_THREADS) k_verify_rows(VerifyArgs a) {
 
 // A cluster to a sequence; its CTAs share the draw's row.
 template <class T>
-__global__ void __launch_bounds__(VF_THREADS) k_verify_walk(VerifyArgs a) {
+__global__ void __launch_bounds__(VW_THREADS, 1) k_verify_walk(VerifyArgs a) {
     __shared__ double s_mass[VF_NODES], s_limit[VF_NODES], s_total[VF_NODES];
     __shared__ int s_parent[VF_NODES], s_token[VF_NODES], s_gone[VF_NODES];
-    __shared__ double s_warp[VF_WARPS], c_sum;
-    __shared__ int s_at, s_count, s_gone_n, s_rejected;
-    pdl_wait();
+    __shared__ double s_powers[256], s_part[VW_WARPS * VW_PARTS], s_warp[VW_WARPS], c_sum[2];
+    __shared__ double s_lost;
+    __shared__ int s_at, s_count, s_gone_n, s_rejected, s_next, s_ask;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int ranks = a.ranks, rank = blockIdx.x % ranks, b = blockIdx.x / ranks;
+    vf::fill_powers(s_powers);
     int first, last;
     a.rows_of(b, first, last);
     const int n = last - first;
     int* tokens = a.tokens + (long long)b * a.max_nodes;
     int* nodes = a.nodes + (long long)b * a.max_nodes;
+    const float heat = a.heat(b);
+    const bool greedy = !(heat > 0.f);
+    const double cold = greedy ? 0.0 : 256 * 1.4426950408889634074 / (double)heat;
+    const T* logits = (const T*)a.logits;
+    pdl_wait();  // the rows' sums, and the outputs' memory
     if (rank == 0)
-        for (int i = tid; i < a.max_nodes; i += VF_THREADS) tokens[i] = nodes[i] = -1;
+        for (int i = tid; i < a.max_nodes; i += VW_THREADS) tokens[i] = nodes[i] = -1;
     if (n == 0) {  // the whole cluster
         if (rank == 0 && tid == 0) a.counts[b] = 0;
         return;
     }
-    const float heat = a.heat(b);
-    const bool greedy = !(heat > 0.f);
-    const double cold = greedy ? 0.0 : 1.0 / (double)heat;
-    const T* logits = (const T*)a.logits;
+    __syncthreads();  // the table
     // a draft's weight at its parent, and what it is held against
-    for (int i = 1 + tid; i < n; i += VF_THREADS) {
+    for (int i = 1 + tid; i < n; i += VW_THREADS) {
         int parent = a.parents ? __ldg(a.parents + first + i) : i - 1;
         const int token = __ldg(a.drafts + first + i);
         double mass = 0.0, total = 1.0, limit = __ldg(a.uniforms + first + i);
         if (parent < 0 || parent >= i) {
             parent = -1;
         } else {
-            const VerifyRow r = a.rows[first + parent];
             const bool known = (unsigned)token < (unsigned)a.vocab;
+            const float l = known ? Dense<T>::get(logits[(first + parent) * a.logits_row + token]) : -INFINITY;
+            const double q = a.probs && known ? (double)a.probs[(first + i) * a.probs_row + token] : NAN;
+            const VerifyRow r = a.rows[first + parent];
             if (!vf::proper(r.sum))
                 mass = NAN;  // nothing is accepted
             else if (greedy)
                 mass = token == r.best;
-            else if (known)
-                mass = vf::weight(Dense<T>::get(logits[(first + parent) * a.logits_row + token]), r.top, cold);
+            else
+                mass = vf::weight(l, r.top, cold, s_powers);
             if (!greedy) total = r.sum;
-            if (a.probs) limit = known ? limit * (double)a.probs[(first + i) * a.probs_row + token] * total : NAN;
+            if (a.probs) limit *= q;
         }
         s_parent[i] = parent, s_token[i] = token;
         s_mass[i] = mass, s_limit[i] = limit, s_total[i] = total;
     }
+    if (tid == 0) s_at = 0, s_count = 1, s_gone_n = 0, s_rejected = -1, s_next = 1, s_lost = 0.0;
+    if (tid == 0 && rank == 0) nodes[0] = 0;
     __syncthreads();
-    if (tid == 0) {
-        int at = 0, count = 1, gone_n = 0, rejected = -1;
-        double gone = 0.0;
-        if (rank == 0) nodes[0] = 0;
-        for (int i = 1; i < n; i++) {
-            if (s_parent[i] != at) continue;
-            double mass = s_mass[i];
-            for (int k = 0; k < gone_n; k++)
-                if (s_gone[k] == s_token[i]) mass = 0.0;  // as a sibling that was rejected
-            if ((a.probs ? s_limit[i] : s_limit[i] * (s_total[i] - gone)) < mass) {
-                if (rank == 0) nodes[count] = i, tokens[count - 1] = s_token[i];
-                at = i, count++;
-                gone = 0.0, gone_n = 0, rejected = -1;
-            } else {
-                gone += mass;
-                s_gone[gone_n++] = s_token[i];
-                rejected = i;
-            }
-        }
-        s_at = at, s_count = count, s_gone_n = gone_n, s_rejected = rejected;
-    }
-    __syncthreads();
-    const int count = s_count, gone_n = a.probs ? 0 : s_gone_n;
-    const VerifyRow r = a.rows[first + s_at];
-    if (greedy || !vf::proper(r.sum)) {  // the whole cluster
-        if (rank == 0 && tid == 0) {
-            tokens[count - 1] = vf::proper(r.sum) ? r.best : -1;
-            a.counts[b] = count;
-        }
-        return;
-    }
-    const T* p = logits + (first + s_at) * a.logits_row;
-    const float* q = a.probs && s_rejected >= 0 ? a.probs + (first + s_rejected) * a.probs_row : nullptr;
-    unsigned long long filter = 0;  // ids that may be among the rejected ones, by their low bits
-    for (int k = 0; k < gone_n; k++) filter |= 1ull << (s_gone[k] & 63);
-    bool all = false;  // no rejection counts
-    auto mass = [&](int id) {
-        const double e = vf::weight(Dense<T>::get(p[id]), r.top, cold);
-        if (all) return e;
-        if (q) return fmax(e / r.sum - (double)q[id], 0.0);
+
+    // ---- sums over a row, in parts in the order of ids: a CTA's, a warp's, a batch's
+    const int share = ((a.vocab + ranks - 1) / ranks + VW_THREADS - 1) / VW_THREADS * VW_THREADS, each = share / VW_WARPS;
+    const int w0 = min(a.vocab, rank * share + warp * each), w1 = min(a.vocab, w0 + each);
+    const int run = ((each + VW_PARTS - 1) / VW_PARTS + VW_RUN - 1) / VW_RUN * VW_RUN;  // ids of a part
+    const T* p = nullptr;
+    const float* q = nullptr;  // the rejected draft's probabilities
+    float top = 0.f;
+    double scale = 1.0;                  // with q: 1 / the row's sum
+    int gone_n = 0;                      // rejected tokens that count as nothing
+    unsigned long long filter = 0;       // their low bits
+    auto weigh = [&](int id, float l, float qv) {
+        const double e = vf::weight(l, top, cold, s_powers);
+        if (q) return fmax(e * scale - (double)qv, 0.0);
         if ((filter >> (id & 63)) & 1)
             for (int k = 0; k < gone_n; k++)
                 if (s_gone[k] == id) return 0.0;
         return e;
     };
-    // parts of the row, in order: a CTA's, a warp's
-    const int share = ((a.vocab + ranks - 1) / ranks + VF_THREADS - 1) / VF_THREADS * VF_THREADS, each = share / VF_WARPS;
-    const int w0 = min(a.vocab, rank * share + warp * each), w1 = min(a.vocab, w0 + each);
-    double total;
-    for (int turn = 0;; turn++) {
-        double sum = 0.0;
-        for (int id = w0 + lane; id < w1; id += 32) sum += mass(id);
-        sum = vf::warp_sum(sum);
-        if (lane == 0) s_warp[warp] = sum;
+    // weights of VW_BATCH ids from `id` on, `step` apart, up to `end`
+    auto batch = [&](int id, int step, int end, double (&m)[VW_BATCH]) {
+        float l[VW_BATCH], qv[VW_BATCH];
+#pragma unroll
+        for (int j = 0; j < VW_BATCH; j++) {
+            const int at = id + j * step;
+            l[j] = at < end ? Dense<T>::get(p[at]) : -INFINITY;
+            qv[j] = q && at < end ? __ldg(q + at) : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < VW_BATCH; j++) m[j] = id + j * step < end ? weigh(id + j * step, l[j], qv[j]) : 0.0;
+    };
+    int turn = 0;
+    auto sum_row = [&]() {
+        double all = 0.0;
+        for (int k = 0, p0 = w0; k < VW_PARTS; k++, p0 += run) {
+            double sum = 0.0;
+            const int p1 = min(w1, p0 + run);
+            for (int id = p0; id < p1; id += VW_RUN) {
+                double m[VW_BATCH];
+                batch(id + lane, 32, p1, m);
+#pragma unroll
+                for (int j = 0; j < VW_BATCH; j++) sum += m[j];
+            }
+            if (p0 < w1) sum = vf::warp_sum(sum);
+            if (lane == 0) s_part[warp * VW_PARTS + k] = sum;
+            all += sum;
+        }
+        if (lane == 0) s_warp[warp] = all;
         __syncthreads();
+        double* c = &c_sum[turn & 1];  // the other one may still be read
+        turn++;
         if (tid == 0) {
-            sum = 0.0;
-            for (int w = 0; w < VF_WARPS; w++) sum += s_warp[w];
-            c_sum = sum;
+            double s = 0.0;
+            for (int w = 0; w < VW_WARPS; w++) s += s_warp[w];
+            *c = s;
         }
         pg::cluster_sync();
-        total = 0.0;
-        for (int k = 0; k < ranks; k++) total += vf::peek(&c_sum, k);
-        if (total > 0.0 || turn) break;
-        all = true;  // nothing is left: rounding alone leaves the draft's row there
-        pg::cluster_sync();
+        double total = 0.0;
+        for (int k = 0; k < ranks; k++) total += vf::peek(c, k);
+        return total;
+    };
+
+    // ---- the walk: one thread, until it ends or a test needs its row's sum in 64 bits
+    int known = -1;  // the node whose sum is known
+    double exact = 0.0;
+    for (;;) {
+        if (tid == 0) {
+            int at = s_at, count = s_count, gn = s_gone_n, rejected = s_rejected, i = s_next, ask = -1;
+            double gone = s_lost;  // the rejected siblings' weight
+            for (; i < n; i++) {
+                if (s_parent[i] != at) continue;
+                double mass = s_mass[i];
+                bool again = false;  // a sibling with this token was rejected
+                for (int k = 0; k < gn; k++) again |= s_gone[k] == s_token[i];
+                if (again) mass = 0.0;
+                const double total = known == at ? exact : s_total[i], weighed = a.probs ? total : total - gone;
+                const double held = s_limit[i] * weighed;
+                if (!greedy && known != at && mass > 0.0 &&
+                    (fabs(held - mass) <= VF_OFF * fabs(s_limit[i]) * total || heat < VF_COLD)) {
+                    ask = at;
+                    break;
+                }
+                if (held < mass) {
+                    if (rank == 0) nodes[count] = i, tokens[count - 1] = s_token[i];
+                    at = i, count++;
+                    gone = 0.0, gn = 0, rejected = -1;
+                } else {
+                    if (!again) gone += mass, s_gone[gn++] = s_token[i];
+                    rejected = i;
+                }
+            }
+            s_at = at, s_count = count, s_gone_n = gn, s_rejected = rejected, s_next = i, s_lost = gone, s_ask = ask;
+        }
+        __syncthreads();
+        const int node = s_at, ask = s_ask;
+        const VerifyRow r = a.rows[first + node];
+        p = logits + (first + node) * a.logits_row;
+        top = r.top;
+        if (ask < 0) {
+            if (greedy || !vf::proper(r.sum)) {  // the whole cluster
+                if (rank == 0 && tid == 0) {
+                    tokens[s_count - 1] = vf::proper(r.sum) ? r.best : -1;
+                    a.counts[b] = s_count;
+                }
+                // what others have of this CTA's sums they have read: nothing was summed, or a barrier follows
+                if (turn) pg::cluster_sync();
+                return;
+            }
+            if (!(a.probs && s_rejected >= 0) || known == node) break;
+        }
+        exact = sum_row();
+        known = node;
+        if (ask < 0) break;
+    }
+
+    // ---- the draw
+    const int count = s_count;
+    if (a.probs) {
+        if (s_rejected >= 0) q = a.probs + (first + s_rejected) * a.probs_row, scale = 1.0 / exact;
+    } else {
+        gone_n = s_gone_n;
+        for (int k = 0; k < gone_n; k++) filter |= 1ull << (s_gone[k] & 63);
+    }
+    double total = sum_row();
+    if (!(total > 0.0)) {  // nothing is left: the row as if nothing had been rejected
+        q = nullptr, filter = 0;
+        total = sum_row();
     }
     const double target = __ldg(a.uniforms + first) * total;
-    // the first part whose running sum passes the target, else the last that has any
-    auto part_of = [&](auto part, int parts, double& passed) {
-        double run = passed;
-        int pick = 0;
-        for (int k = 0; k < parts; k++) {
-            const double v = part(k);
-            if (!(v > 0.0)) continue;
-            pick = k, passed = run;
-            run += v;
-            if (run > target) break;
-        }
-        return pick;
-    };
-    double passed = 0.0;
-    const int cta = part_of([&](int k) { return vf::peek(&c_sum, k); }, ranks, passed);
-    if (cta == rank) {
-        const int w = part_of([&](int k) { return s_warp[k]; }, VF_WARPS, passed);
-        if (w == warp) {
-            // a lane's ids are neighbours: sums over the lanes, then through the lane's own
-            const int run = (w1 - w0 + 31) / 32, l0 = min(w1, w0 + lane * run), l1 = min(w1, l0 + run);
-            double sum = 0.0;
-            int some = -1;  // the lane's last id that has any
-            for (int id = l0; id < l1; id++) {
-                const double v = mass(id);
-                sum += v;
-                if (v > 0.0) some = id;
-            }
-            double up = sum;
+    const double* sums = &c_sum[(turn - 1) & 1];
+    if (warp == 0) {
+        double passed = 0.0;
+        const int cta = vf::pick([&](int k) { return vf::peek(sums, k); }, ranks, target, passed);
+        if (cta == rank) {
+            const int part = vf::pick([&](int k) { return s_part[k]; }, VW_WARPS * VW_PARTS, target, passed);
+            // ids of the part: a lane's are neighbours
+            const int c0 = rank * share + part / VW_PARTS * each;
+            const int p0 = c0 + part % VW_PARTS * run, p1 = min(min(a.vocab, c0 + each), p0 + run);
+            int token = -1;
+            for (int id = p0; id < p1; id += VW_RUN) {
+                double m[VW_BATCH], sum = 0.0;
+                batch(id + lane * VW_BATCH, 1, p1, m);
 #pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const double v = __shfl_up_sync(0xffffffffu, up, o);
-                if (lane >= o) up += v;
-            }
-            const uint32_t over = __ballot_sync(0xffffffffu, some >= 0 && passed + up > target);
-            const uint32_t any = __ballot_sync(0xffffffffu, some >= 0);
-            const int chosen = over ? __ffs(over) - 1 : any ? 31 - __clz(any) : -1;
-            if (lane == chosen) {
-                int token = some;
-                if (over) {
-                    double at = passed + up - sum;
-                    for (int id = l0; id < l1; id++) {
-                        const double v = mass(id);
-                        if (!(v > 0.0)) continue;
-                        at += v;
-                        if (at > target) {
-                            token = id;
-                            break;
-                        }
-                    }
+                for (int j = 0; j < VW_BATCH; j++) sum += m[j];
+                double up = sum;
+#pragma unroll
+                for (int o = 1; o < 32; o *= 2) {
+                    const double v = __shfl_up_sync(0xffffffffu, up, o);
+                    if (lane >= o) up += v;
                 }
+                const uint32_t over = __ballot_sync(0xffffffffu, sum > 0.0 && passed + up > target), any = __ballot_sync(0xffffffffu, sum > 0.0);
+                if (any) {
+                    const int chosen = over ? __ffs(over) - 1 : 31 - __clz(any);
+                    int mine = -1;
+                    double at = passed + (up - sum);
+#pragma unroll
+                    for (int j = 0; j < VW_BATCH; j++)
+                        if (m[j] > 0.0 && (mine < 0 || !(at > target))) mine = id + lane * VW_BATCH + j, at += m[j];
+                    token = __shfl_sync(0xffffffffu, mine, chosen);
+                }
+                if (over) break;
+                passed += __shfl_sync(0xffffffffu, up, 31);
+            }
+            if (lane == 0) {
                 tokens[count - 1] = token;
+                a.counts[b] = count;
             }
         }
     }
-    if (rank == 0 && tid == 0) a.counts[b] = count;
     pg::cluster_sync();  // the others' sums stay until they are read
 }
 
