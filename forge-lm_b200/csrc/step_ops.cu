@@ -77,10 +77,17 @@ int32_t fb2_pages_extend(const fb2_pages* p, const int32_t* counts, int32_t max_
         need(starts && (v.n_seqs == 0 || (counts && prefix_lens)) && (max_rows == 0 || (slots && positions)), "NULL argument");
         need(aligned(counts, 4) && aligned(starts, 4) && aligned(prefix_lens, 4) && aligned(slots, 4) && aligned(positions, 4),
              "a tensor is not aligned to its element size");
+        const bool vec = aligned(slots, 16) && aligned(positions, 16);
+        auto launch = [&](auto kernel, int threads, int ranks) {
+            launch_cluster(kernel, dim3(ranks), threads, 12 * v.n_seqs, ranks, false, stream, v, counts, max_rows, starts, prefix_lens, slots,
+                           positions, vec);
+        };
         int ranks = 1;
-        while (ranks < 8 && max_rows > 2 * PG_THREADS * ranks) ranks *= 2;
-        launch_cluster(k_pages_extend, dim3(ranks), PG_THREADS, 12 * v.n_seqs, ranks, false, stream, v, counts, max_rows, starts, prefix_lens,
-                       slots, positions);
+        while (ranks < 8 && max_rows > 1024 * PG_RUN * ranks) ranks *= 2;
+        if (v.n_seqs <= 256 && max_rows <= 256 * PG_RUN)
+            launch(k_pages_extend<256>, 256, 1);
+        else
+            launch(k_pages_extend<1024>, 1024, ranks);
     });
 }
 
@@ -90,7 +97,10 @@ int32_t fb2_pages_truncate(const fb2_pages* p, const int32_t* lens, void* stream
         if (v.n_seqs == 0) return;
         need(lens, "NULL argument");
         need(aligned(lens, 4), "a tensor is not aligned to its element size");
-        launch_cluster(k_pages_truncate, dim3(1), PG_THREADS, 8 * v.n_seqs, 1, false, stream, v, lens);
+        if (v.n_seqs <= 256)
+            launch_cluster(k_pages_truncate<256>, dim3(1), 256, 8 * v.n_seqs, 1, false, stream, v, lens);
+        else
+            launch_cluster(k_pages_truncate<1024>, dim3(1), 1024, 8 * v.n_seqs, 1, false, stream, v, lens);
     });
 }
 
@@ -338,9 +348,17 @@ VerifyArgs verify_args(const fb2_verify* v) {
     a.n_rows = v->n_rows;
     a.vocab = v->vocab;
     a.max_nodes = v->max_nodes;
-    a.ranks = 1;
-    while (a.ranks < VF_RANKS && a.vocab > 2048 * a.ranks) a.ranks *= 2;
     return a;
+}
+// CTAs to a row: of at least 2048 ids each where rows leave SMs free, else of 16384
+// and up to 8 on each SM (161 rows x 131071 bf16, all of a call: 53 us with 4, 57 with
+// 2, 64 with 1; 289 x 50257 fp16: 35 with 2, 37 with 4, 41 with 8).
+int verify_ranks(int vocab, int rows) {
+    int ranks = 1;
+    while (ranks < VF_RANKS && vocab > 2048 * ranks &&
+           ((int64_t)rows * ranks * 2 <= 2 * 148 || (vocab > 16384 * ranks && (int64_t)rows * ranks * 2 <= 8 * 148)))
+        ranks *= 2;
+    return ranks;
 }
 }  // namespace
 
@@ -367,7 +385,9 @@ int32_t fb2_verify_drafts(const fb2_verify* v, void* stream) {
         a.rows = static_cast<VerifyRow*>(v->device_workspace);
         with_type(v->dtype, [&](auto t) {
             using T = decltype(t);
+            a.ranks = verify_ranks(a.vocab, a.n_rows);
             if (a.n_rows) launch_cluster(k_verify_rows<T>, dim3(a.n_rows * a.ranks), VF_THREADS, 0, a.ranks, false, stream, a);
+            a.ranks = verify_ranks(a.vocab, a.n_seqs);
             launch_cluster(k_verify_walk<T>, dim3(a.n_seqs * a.ranks), VW_THREADS, 0, a.ranks, a.n_rows > 0, stream, a);
         });
     });

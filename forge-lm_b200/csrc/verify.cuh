@@ -25,7 +25,7 @@ namespace fb2 {
 
 constexpr int VF_THREADS = 256, VF_WARPS = VF_THREADS / 32, VF_NODES = 1024, VF_RANKS = 8;
 constexpr int VW_THREADS = 512, VW_WARPS = VW_THREADS / 32;
-constexpr int VW_BATCH = 8;                 // loads of a lane that are in flight at once
+constexpr int VW_BATCH = 4;                 // loads of a lane that are in flight at once
 constexpr int VW_RUN = 32 * VW_BATCH;       // ids of a warp's batch
 constexpr int VW_PARTS = 16;                // of a warp's ids, each with its own sum
 // How far a sum of k_verify_rows may be off, relative.  An exponent (l - top) * log2(e) / T
@@ -49,7 +49,7 @@ struct VerifyArgs {
     int *tokens, *nodes, *counts;
     VerifyRow* rows;
     long long logits_row, probs_row;
-    int n_seqs, n_rows, vocab, max_nodes, ranks;  // ranks: CTAs of a cluster
+    int n_seqs, n_rows, vocab, max_nodes, ranks;  // ranks: CTAs of a cluster, a power of two
     // the rows of sequence b
     FB2_DEV void rows_of(int b, int& first, int& last) const {
         if (!starts) {
@@ -88,32 +88,58 @@ FB2_DEV double warp_sum(double v) {
 }
 FB2_DEV float ex2(float x) {
     float y;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// 2^(i / 256), i = 0..255: what the exponentials in 64 bits are looked up in.
-FB2_DEV void fill_powers(double* powers) {
-    for (int i = threadIdx.x; i < 256; i += blockDim.x) powers[i] = exp2((double)i / 256);
+FB2_DEV float2 add2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return reinterpret_cast<float2&>(r);
 }
-// exp((l - top) / T) with cold = 256 log2(e) / T, by a table and a polynomial (P. T. P.
-// Tang, Table-driven implementation of the exponential function, ACM TOMS 15, 1989):
-// 2^(n / 256) from the table and the exponent, exp(t), |t| <= ln 2 / 512, from its
-// series to t^4 (t^5 / 120 < 2^-54).  l <= top; 0 where it falls below 2^-1000.
-FB2_DEV double weight(float l, float top, double cold, const double* powers) {
-    double x = ((double)l - (double)top) * cold;
-    if (!(x > -256000.0)) x = -256000.0;  // (-inf too)
-    const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the nearest whole number
-    const double high = x + magic;
-    const int n = __double2loint(high);
-    const double t = (x - (high - magic)) * 2.70760617406228636e-3;  // ln 2 / 256
-    double e = fma(t, 1.0 / 24, 1.0 / 6);
-    e = fma(e, t, 0.5);
-    e = fma(e, t, 1.0);
-    const double p = powers[n & 255];
-    e = fma(e * t, p, p);
-    if (n <= -256000) return 0.0;
-    return __hiloint2double(__double2hiint(e) + ((n >> 8) << 20), __double2loint(e));
+FB2_DEV float2 mul2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return reinterpret_cast<float2&>(r);
 }
+// 2^(i / 1024), i = 0..1023: what the exponentials in 64 bits are looked up in;
+// products of two factors, so that a thread calls exp2 once or not at all.
+FB2_DEV void fill_powers(double* powers, double* factors) {
+    const int i = threadIdx.x;
+    if (i < 64) factors[i] = exp2(i < 32 ? (double)i / 1024 : (double)(i - 32) / 32);
+    __syncthreads();
+    for (int k = i; k < 1024; k += blockDim.x) powers[k] = factors[k & 31] * factors[32 + (k >> 5)];
+}
+// fp32 as fp64, without a conversion (which go at the rate of fp64 arithmetic): 0 and
+// what is smaller than 2^-126 become some 2^-127, infinities 2^128.
+FB2_DEV double widen(float v) {
+    const int bits = __float_as_int(v);
+    return __hiloint2double(((bits >> 3) & 0x8fffffff) + 0x38000000, bits << 29);
+}
+// exp((l - top) / T), l <= top, by a table and a polynomial (P. T. P. Tang,
+// Table-driven implementation of the exponential function, ACM TOMS 15, 1989):
+// 2^(n / 1024) from the table and the exponent, exp(t), |t| <= ln 2 / 2048, from its
+// series to t^3 (t^4 / 24 < 2^-50).  0 where it falls below 2^-1000.
+struct Heat {
+    double cold;  // 1024 log2(e) / T
+    float near;   // log2(e) / T, not 0
+    double top;
+    float top32;
+    FB2_DEV double weight(float l, const double* powers) const {
+        const bool none = (l - top32) * near < -1000.f;  // (-inf too)
+        const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the nearest whole number
+        const double d = widen(l) - top, high = fma(d, cold, magic), t = fma(d, cold, magic - high);
+        const int n = __double2loint(high);
+        constexpr double u = 6.7690154351557159e-4;  // ln 2 / 1024
+        double e = fma(t, u * u * u / 6, u * u / 2);
+        e = fma(e, t, u);
+        double p = powers[n & 1023];
+        p = __hiloint2double(__double2hiint(p) + ((n >> 10) << 20), __double2loint(p));
+        e = fma(e * t, p, p);
+        return none ? 0.0 : e;  // (no branch: weights of neighbours overlap)
+    }
+};
+// v where it is positive, else 0
+FB2_DEV double positive(double v) { return __double2hiint(v) < 0 ? 0.0 : v; }
 // The first k in 0..n-1 whose running sum over `part`, from `passed` on, passes the
 // target, else the last with a positive part (-1: none); `passed` becomes the sum
 // before it.  By the lanes of a warp.
@@ -195,7 +221,17 @@ __global__ void __launch_bounds__(VF_THREADS) k_verify_rows(VerifyArgs a) {
             top = to;
         }
     };
-    auto term = [&](float v) { return vf::ex2((v - top) * cold); };  // NaN for NaN, and for all where one is inf
+    // sum of exp2((v - top) * cold) of a piece (NaN for NaN, and for all where one is inf), two values to an instruction
+    auto terms = [&](const float (&v)[16 / sizeof(T)]) {
+        const float2 up = make_float2(-top, -top), by = make_float2(cold, cold);
+        float2 part = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+            const float2 x = vf::mul2(vf::add2(make_float2(v[j], v[j + 1]), up), by);
+            part = vf::add2(part, make_float2(vf::ex2(x.x), vf::ex2(x.y)));
+        }
+        return part.x + part.y;
+    };
     const uint4* body = reinterpret_cast<const uint4*>(p + head);
     constexpr int M = 4;  // loads in flight
     for (int i0 = p0 + tid; i0 < p1; i0 += M * VF_THREADS) {
@@ -216,57 +252,61 @@ __global__ void __launch_bounds__(VF_THREADS) k_verify_rows(VerifyArgs a) {
                 for (int j = N - 1; j >= 0; j--)
                     if (v[j] == most) best = head + i * N + j;
             raise(most);
-            float part = 0.f;
-#pragma unroll
-            for (int j = 0; j < N; j++) part += term(v[j]);
-            sum += (double)part;
+            sum += (double)terms(v);
         }
     }
-    // (top, sum, best) with another part's
-    auto join = [&](float t2, double s2, int b2) {
-        const float t = fmaxf(top, t2);
-        sum = sum * (double)vf::ex2((top - t) * cold) + s2 * (double)vf::ex2((t2 - t) * cold);
-        if (best < 0 || (b2 >= 0 && (t2 > top || (t2 == top && b2 < best)))) best = b2;
-        top = t;
-    };
     auto edge = [&](int id) {
         const float v = Dense<T>::get(p[id]);
-        const bool more = v > -3.402823466e38f;
-        join(more ? v : -3.402823466e38f, v == -INFINITY ? 0.0 : v == v && v < INFINITY ? 1.0 : (double)NAN, v > -INFINITY ? id : -1);
+        if (v > top || (v == top && (best < 0 || id < best))) best = id;
+        raise(v);
+        sum += (double)vf::ex2((v - top) * cold);
     };
     if (rank == 0 && tid < head) edge(tid);
     if (rank == ranks - 1 && head + pieces * N + tid < a.vocab) edge(head + pieces * N + tid);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float t2 = __shfl_xor_sync(0xffffffffu, top, o);
-        const double s2 = __shfl_xor_sync(0xffffffffu, sum, o);
-        join(t2, s2, __shfl_xor_sync(0xffffffffu, best, o));
-    }
+    // the lanes' parts: in every lane the largest, the sum below it, the first id that has it
+    auto join = [&]() {
+        const float most = warp_max(top);
+        if (greedy) best = (int)__reduce_min_sync(0xffffffffu, top == most ? (uint32_t)best : 0xffffffffu);  // -1: none
+        sum = vf::warp_sum(sum * (double)vf::ex2((top - most) * cold));
+        top = most;
+    };
+    auto none = [&]() { top = -3.402823466e38f, sum = 0.0, best = -1; };
+    join();
     if (lane == 0) s_top[warp] = top, s_sum[warp] = sum, s_best[warp] = best;
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < VF_WARPS; w++) join(s_top[w], s_sum[w], s_best[w]);
-        c_top = top, c_sum = sum, c_best = best;
+    if (warp == 0) {  // the warps' parts, then the cluster's
+        if (lane < VF_WARPS)
+            top = s_top[lane], sum = s_sum[lane], best = s_best[lane];
+        else
+            none();
+        join();
+        if (lane == 0) c_top = top, c_sum = sum, c_best = best;
     }
     if (ranks > 1) pg::cluster_sync();
-    if (rank == 0 && tid == 0) {
-        for (int r = 1; r < ranks; r++) join(vf::peek(&c_top, r), vf::peek(&c_sum, r), vf::peek(&c_best, r));
-        a.rows[row] = {sum, top, best};
+    if (rank == 0 && warp == 0) {
+        if (ranks > 1) {
+            if (lane < ranks)
+                top = vf::peek(&c_top, lane), sum = vf::peek(&c_sum, lane), best = vf::peek(&c_best, lane);
+            else
+                none();
+            join();
+        }
+        if (lane == 0) a.rows[row] = {sum, top, best};
     }
     if (ranks > 1) pg::cluster_sync();  // the others' shared memory stays until it is read
 }
 
 // A cluster to a sequence; its CTAs share the draw's row.
 template <class T>
-__global__ void __launch_bounds__(VW_THREADS, 1) k_verify_walk(VerifyArgs a) {
+__global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
     __shared__ double s_mass[VF_NODES], s_limit[VF_NODES], s_total[VF_NODES];
     __shared__ int s_parent[VF_NODES], s_token[VF_NODES], s_gone[VF_NODES];
-    __shared__ double s_powers[256], s_part[VW_WARPS * VW_PARTS], s_warp[VW_WARPS], c_sum[2];
+    __shared__ double s_powers[1024], s_factors[64], s_part[VW_WARPS * VW_PARTS], s_warp[VW_WARPS], c_sum[2];
     __shared__ double s_lost;
     __shared__ int s_at, s_count, s_gone_n, s_rejected, s_next, s_ask;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int ranks = a.ranks, rank = blockIdx.x % ranks, b = blockIdx.x / ranks;
-    vf::fill_powers(s_powers);
+    vf::fill_powers(s_powers, s_factors);
     int first, last;
     a.rows_of(b, first, last);
     const int n = last - first;
@@ -274,7 +314,9 @@ __global__ void __launch_bounds__(VW_THREADS, 1) k_verify_walk(VerifyArgs a) {
     int* nodes = a.nodes + (long long)b * a.max_nodes;
     const float heat = a.heat(b);
     const bool greedy = !(heat > 0.f);
-    const double cold = greedy ? 0.0 : 256 * 1.4426950408889634074 / (double)heat;
+    vf::Heat at_heat;
+    at_heat.cold = greedy ? 0.0 : 1024 * 1.4426950408889634074 / (double)heat;
+    at_heat.near = fmaxf((float)(at_heat.cold / 1024), 1e-44f);
     const T* logits = (const T*)a.logits;
     pdl_wait();  // the rows' sums, and the outputs' memory
     if (rank == 0)
@@ -300,8 +342,11 @@ __global__ void __launch_bounds__(VW_THREADS, 1) k_verify_walk(VerifyArgs a) {
                 mass = NAN;  // nothing is accepted
             else if (greedy)
                 mass = token == r.best;
-            else
-                mass = vf::weight(l, r.top, cold, s_powers);
+            else {
+                vf::Heat h = at_heat;
+                h.top32 = r.top, h.top = vf::widen(r.top);
+                mass = h.weight(l, s_powers);
+            }
             if (!greedy) total = r.sum;
             if (a.probs) limit *= q;
         }
@@ -310,6 +355,7 @@ __global__ void __launch_bounds__(VW_THREADS, 1) k_verify_walk(VerifyArgs a) {
     }
     if (tid == 0) s_at = 0, s_count = 1, s_gone_n = 0, s_rejected = -1, s_next = 1, s_lost = 0.0;
     if (tid == 0 && rank == 0) nodes[0] = 0;
+    for (int i = tid; i < VW_WARPS * VW_PARTS; i += VW_THREADS) s_part[i] = 0.0;  // parts behind the row's end stay so
     __syncthreads();
 
     // ---- sums over a row, in parts in the order of ids: a CTA's, a warp's, a batch's
@@ -318,141 +364,142 @@ __global__ void __launch_bounds__(VW_THREADS, 1) k_verify_walk(VerifyArgs a) {
     const int run = ((each + VW_PARTS - 1) / VW_PARTS + VW_RUN - 1) / VW_RUN * VW_RUN;  // ids of a part
     const T* p = nullptr;
     const float* q = nullptr;  // the rejected draft's probabilities
-    float top = 0.f;
     double scale = 1.0;                  // with q: 1 / the row's sum
+    const double* sums = nullptr;        // of the CTAs
     int gone_n = 0;                      // rejected tokens that count as nothing
     unsigned long long filter = 0;       // their low bits
-    auto weigh = [&](int id, float l, float qv) {
-        const double e = vf::weight(l, top, cold, s_powers);
-        if (q) return fmax(e * scale - (double)qv, 0.0);
-        if ((filter >> (id & 63)) & 1)
-            for (int k = 0; k < gone_n; k++)
-                if (s_gone[k] == id) return 0.0;
-        return e;
-    };
-    // weights of VW_BATCH ids from `id` on, `step` apart, up to `end`
-    auto batch = [&](int id, int step, int end, double (&m)[VW_BATCH]) {
-        float l[VW_BATCH], qv[VW_BATCH];
+    // weights of VW_BATCH ids from `id` on, STEP apart, up to `end`
+    auto batch = [&](int id, int end, double (&m)[VW_BATCH], auto step) {
+        constexpr int N = VW_BATCH, STEP = decltype(step)::value;
+        float l[N], qv[N];
 #pragma unroll
-        for (int j = 0; j < VW_BATCH; j++) {
-            const int at = id + j * step;
-            l[j] = at < end ? Dense<T>::get(p[at]) : -INFINITY;
-            qv[j] = q && at < end ? __ldg(q + at) : 0.f;
+        for (int j = 0; j < N; j++) l[j] = id + STEP * j < end ? Dense<T>::get(p[id + STEP * j]) : -INFINITY;
+        if (q) {
+#pragma unroll
+            for (int j = 0; j < N; j++) qv[j] = id + STEP * j < end ? __ldg(q + id + STEP * j) : 0.f;
         }
 #pragma unroll
-        for (int j = 0; j < VW_BATCH; j++) m[j] = id + j * step < end ? weigh(id + j * step, l[j], qv[j]) : 0.0;
-    };
-    int turn = 0;
-    auto sum_row = [&]() {
-        double all = 0.0;
-        for (int k = 0, p0 = w0; k < VW_PARTS; k++, p0 += run) {
-            double sum = 0.0;
-            const int p1 = min(w1, p0 + run);
-            for (int id = p0; id < p1; id += VW_RUN) {
-                double m[VW_BATCH];
-                batch(id + lane, 32, p1, m);
+        for (int j = 0; j < N; j++) m[j] = at_heat.weight(l[j], s_powers);
+        if (q) {
 #pragma unroll
-                for (int j = 0; j < VW_BATCH; j++) sum += m[j];
-            }
-            if (p0 < w1) sum = vf::warp_sum(sum);
-            if (lane == 0) s_part[warp * VW_PARTS + k] = sum;
-            all += sum;
+            for (int j = 0; j < N; j++) m[j] = vf::positive(fma(m[j], scale, -vf::widen(qv[j])));
         }
-        if (lane == 0) s_warp[warp] = all;
-        __syncthreads();
-        double* c = &c_sum[turn & 1];  // the other one may still be read
-        turn++;
-        if (tid == 0) {
-            double s = 0.0;
-            for (int w = 0; w < VW_WARPS; w++) s += s_warp[w];
-            *c = s;
+        if (filter) {
+#pragma unroll
+            for (int j = 0; j < N; j++)
+                if ((filter >> ((id + STEP * j) & 63)) & 1)
+                    for (int k = 0; k < gone_n; k++)
+                        if (s_gone[k] == id + STEP * j) m[j] = 0.0;
         }
-        pg::cluster_sync();
-        double total = 0.0;
-        for (int k = 0; k < ranks; k++) total += vf::peek(c, k);
-        return total;
     };
 
-    // ---- the walk: one thread, until it ends or a test needs its row's sum in 64 bits
+    // ---- the walk by one thread, until it ends or a test needs its row's sum in 64 bits;
+    // that sum; the draw's.  One loop, so that the sums' code is there (and fetched) once.
+    enum { WALK, DRAW, DRAW_ALL } state = WALK;
     int known = -1;  // the node whose sum is known
-    double exact = 0.0;
-    for (;;) {
-        if (tid == 0) {
-            int at = s_at, count = s_count, gn = s_gone_n, rejected = s_rejected, i = s_next, ask = -1;
-            double gone = s_lost;  // the rejected siblings' weight
-            for (; i < n; i++) {
-                if (s_parent[i] != at) continue;
-                double mass = s_mass[i];
-                bool again = false;  // a sibling with this token was rejected
-                for (int k = 0; k < gn; k++) again |= s_gone[k] == s_token[i];
-                if (again) mass = 0.0;
-                const double total = known == at ? exact : s_total[i], weighed = a.probs ? total : total - gone;
-                const double held = s_limit[i] * weighed;
-                if (!greedy && known != at && mass > 0.0 &&
-                    (fabs(held - mass) <= VF_OFF * fabs(s_limit[i]) * total || heat < VF_COLD)) {
-                    ask = at;
-                    break;
+    double exact = 0.0, total = 0.0;
+    for (int turn = 0;; turn++) {
+        if (state == WALK) {
+            if (tid == 0) {
+                int at = s_at, count = s_count, gn = s_gone_n, rejected = s_rejected, i = s_next, ask = -1;
+                double gone = s_lost;  // the rejected siblings' weight
+                for (; i < n; i++) {
+                    if (s_parent[i] != at) continue;
+                    double mass = s_mass[i];
+                    bool again = false;  // a sibling with this token was rejected
+                    for (int k = 0; k < gn; k++) again |= s_gone[k] == s_token[i];
+                    if (again) mass = 0.0;
+                    const double sum = known == at ? exact : s_total[i], weighed = a.probs ? sum : sum - gone;
+                    const double held = s_limit[i] * weighed;
+                    if (!greedy && known != at && mass > 0.0 && (fabs(held - mass) <= VF_OFF * fabs(s_limit[i]) * sum || heat < VF_COLD)) {
+                        ask = at;
+                        break;
+                    }
+                    if (held < mass) {
+                        if (rank == 0) nodes[count] = i, tokens[count - 1] = s_token[i];
+                        at = i, count++;
+                        gone = 0.0, gn = 0, rejected = -1;
+                    } else {
+                        if (!again) gone += mass, s_gone[gn++] = s_token[i];
+                        rejected = i;
+                    }
                 }
-                if (held < mass) {
-                    if (rank == 0) nodes[count] = i, tokens[count - 1] = s_token[i];
-                    at = i, count++;
-                    gone = 0.0, gn = 0, rejected = -1;
-                } else {
-                    if (!again) gone += mass, s_gone[gn++] = s_token[i];
-                    rejected = i;
-                }
+                s_at = at, s_count = count, s_gone_n = gn, s_rejected = rejected, s_next = i, s_lost = gone, s_ask = ask;
             }
-            s_at = at, s_count = count, s_gone_n = gn, s_rejected = rejected, s_next = i, s_lost = gone, s_ask = ask;
+            __syncthreads();
         }
-        __syncthreads();
-        const int node = s_at, ask = s_ask;
+        const int node = s_at, rejected = s_rejected;
         const VerifyRow r = a.rows[first + node];
         p = logits + (first + node) * a.logits_row;
-        top = r.top;
-        if (ask < 0) {
+        at_heat.top32 = r.top, at_heat.top = vf::widen(r.top);
+        if (state == WALK && s_ask < 0) {
             if (greedy || !vf::proper(r.sum)) {  // the whole cluster
                 if (rank == 0 && tid == 0) {
                     tokens[s_count - 1] = vf::proper(r.sum) ? r.best : -1;
                     a.counts[b] = s_count;
                 }
-                // what others have of this CTA's sums they have read: nothing was summed, or a barrier follows
-                if (turn) pg::cluster_sync();
+                if (turn) pg::cluster_sync();  // this CTA's sums have been read
                 return;
             }
-            if (!(a.probs && s_rejected >= 0) || known == node) break;
+            if (!a.probs || rejected < 0 || known == node) state = DRAW;
         }
-        exact = sum_row();
-        known = node;
-        if (ask < 0) break;
+        if (state == DRAW) {
+            if (a.probs) {
+                if (rejected >= 0) q = a.probs + (first + rejected) * a.probs_row, scale = 1.0 / exact;
+            } else {
+                gone_n = s_gone_n;
+                for (int k = 0; k < gone_n; k++) filter |= 1ull << (s_gone[k] & 63);
+            }
+        }
+        // the row's sums
+        double all = 0.0;
+        for (int k = 0, p0 = w0; k < VW_PARTS && p0 < w1; k++, p0 += run) {
+            double sum = 0.0;
+            const int p1 = min(w1, p0 + run);
+            for (int id = p0; id < p1; id += VW_RUN) {
+                double m[VW_BATCH];
+                batch(id + lane, p1, m, std::integral_constant<int, 32>{});
+#pragma unroll
+                for (int j = 0; j < VW_BATCH; j++) sum += m[j];
+            }
+            sum = vf::warp_sum(sum);
+            if (lane == 0) s_part[warp * VW_PARTS + k] = sum;
+            all += sum;
+        }
+        if (lane == 0) s_warp[warp] = all;
+        __syncthreads();
+        sums = &c_sum[turn & 1];  // the other one may still be read
+        if (warp == 0) {
+            const double s = vf::warp_sum(lane < VW_WARPS ? s_warp[lane] : 0.0);
+            if (lane == 0) c_sum[turn & 1] = s;
+        }
+        pg::cluster_sync();
+        total = vf::warp_sum(lane < ranks ? vf::peek(sums, lane) : 0.0);
+        if (state == WALK) {
+            exact = total, known = node;
+        } else if (total > 0.0 || state == DRAW_ALL) {
+            break;
+        } else {  // nothing is left: the row as if nothing had been rejected
+            q = nullptr, filter = 0;
+            state = DRAW_ALL;
+        }
     }
-
-    // ---- the draw
     const int count = s_count;
-    if (a.probs) {
-        if (s_rejected >= 0) q = a.probs + (first + s_rejected) * a.probs_row, scale = 1.0 / exact;
-    } else {
-        gone_n = s_gone_n;
-        for (int k = 0; k < gone_n; k++) filter |= 1ull << (s_gone[k] & 63);
-    }
-    double total = sum_row();
-    if (!(total > 0.0)) {  // nothing is left: the row as if nothing had been rejected
-        q = nullptr, filter = 0;
-        total = sum_row();
-    }
     const double target = __ldg(a.uniforms + first) * total;
-    const double* sums = &c_sum[(turn - 1) & 1];
     if (warp == 0) {
         double passed = 0.0;
-        const int cta = vf::pick([&](int k) { return vf::peek(sums, k); }, ranks, target, passed);
+        const double mine = lane < ranks ? vf::peek(sums, lane) : 0.0;
+        const int cta = vf::pick([&](int) { return mine; }, ranks, target, passed);  // lane k has CTA k's
         if (cta == rank) {
             const int part = vf::pick([&](int k) { return s_part[k]; }, VW_WARPS * VW_PARTS, target, passed);
-            // ids of the part: a lane's are neighbours
+            // through the part's ids, of which a lane has neighbours
             const int c0 = rank * share + part / VW_PARTS * each;
             const int p0 = c0 + part % VW_PARTS * run, p1 = min(min(a.vocab, c0 + each), p0 + run);
             int token = -1;
-            for (int id = p0; id < p1; id += VW_RUN) {
+#pragma unroll 1
+            for (int id = p0 + lane * VW_BATCH; id - lane * VW_BATCH < p1; id += VW_RUN) {
                 double m[VW_BATCH], sum = 0.0;
-                batch(id + lane * VW_BATCH, 1, p1, m);
+                batch(id, p1, m, std::integral_constant<int, 1>{});
 #pragma unroll
                 for (int j = 0; j < VW_BATCH; j++) sum += m[j];
                 double up = sum;
@@ -461,16 +508,14 @@ __global__ void __launch_bounds__(VW_THREADS, 1) k_verify_walk(VerifyArgs a) {
                     const double v = __shfl_up_sync(0xffffffffu, up, o);
                     if (lane >= o) up += v;
                 }
-                const uint32_t over = __ballot_sync(0xffffffffu, sum > 0.0 && passed + up > target), any = __ballot_sync(0xffffffffu, sum > 0.0);
-                if (any) {
-                    const int chosen = over ? __ffs(over) - 1 : 31 - __clz(any);
-                    int mine = -1;
-                    double at = passed + (up - sum);
+                const uint32_t any = __ballot_sync(0xffffffffu, sum > 0.0), over = __ballot_sync(0xffffffffu, passed + up > target) & any;
+                // the first of the lane's ids that passes the target, or its last with a weight
+                int found = -1;
+                double at = passed + (up - sum);
 #pragma unroll
-                    for (int j = 0; j < VW_BATCH; j++)
-                        if (m[j] > 0.0 && (mine < 0 || !(at > target))) mine = id + lane * VW_BATCH + j, at += m[j];
-                    token = __shfl_sync(0xffffffffu, mine, chosen);
-                }
+                for (int j = 0; j < VW_BATCH; j++)
+                    if (m[j] > 0.0 && (found < 0 || !(at > target))) found = id + j, at += m[j];
+                if (any) token = __shfl_sync(0xffffffffu, found, over ? __ffs(over) - 1 : 31 - __clz(any));
                 if (over) break;
                 passed += __shfl_sync(0xffffffffu, up, 31);
             }
