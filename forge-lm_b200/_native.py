@@ -51,7 +51,7 @@ EXPORTED = [
     "fb2_kvq_sizes", "fb2_kvq_write", "fb2_kvq_read", "fb2_kvq_attend_workspace", "fb2_kvq_attend",
     "fb2_w4_sizes", "fb2_w4_pack", "fb2_w4_matvec_workspace", "fb2_w4_matvec", "fb2_logit_controls",
     "fb2_pages_check", "fb2_pages_extend", "fb2_pages_truncate", "fb2_residual_norm", "fb2_quantise_rows", "fb2_w8_check", "fb2_w8_pack",
-    "fb2_w8_matmul", "fb2_verify_workspace", "fb2_verify_drafts",
+    "fb2_w8_matmul", "fb2_w8_forward_workspace", "fb2_w8_forward", "fb2_verify_workspace", "fb2_verify_drafts",
 ]
 TEST_EXPORTED = ["fb2_test_expf", "fb2_test_expf_hash", "fb2_test_dotnet_random", "fb2_test_mk_trace",
                  "fb2_test_gemm_tc", "fb2_test_sha256", "fb2_test_mk_withhold", "fb2_test_fail_alloc", "fb2_test_mk_geometry",
@@ -166,6 +166,8 @@ def load(path: str | None = None):
     L.fb2_quantise_rows.argtypes = [i32, i32, vp, i32, i64, vp, i64, vp, vp]
     L.fb2_w8_pack.argtypes = [st, vp, i32, i64, vp]
     L.fb2_w8_matmul.argtypes = [st, i32, vp, i64, vp, vp, i64, i32, vp]
+    L.fb2_w8_forward_workspace.argtypes = [st, i32, i64p]
+    L.fb2_w8_forward.argtypes = [st, i32, vp, i64, vp, i64, i32, vp, i64, vp]
     L.fb2_verify_workspace.argtypes = [st, i64p]
     L.fb2_verify_drafts.argtypes = [st, vp]
     L.fb2_test_w8_withhold.argtypes = [i32, i64]

@@ -29,57 +29,68 @@ struct NormArgs {
 
 namespace nrm {
 
-// Sum (or, of bits, largest) over the G threads that share a row.
+// Sum (or, of bits, largest) over the G threads that share a row; `turn` counts the
+// calls: the place of the one before may still be read.
 template <int G>
-FB2_DEV float sum(float v, float* s) {
+FB2_DEV float sum(float v, float (*s)[32], int& turn) {
     v = warp_sum(v);
     if constexpr (G > 32) {
-        __syncthreads();  // s may still be read from the last time
-        if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+        float* to = s[turn++ & 1];
+        if ((threadIdx.x & 31) == 0) to[threadIdx.x >> 5] = v;
         __syncthreads();
         v = 0.f;
 #pragma unroll
-        for (int i = 0; i < G / 32; i++) v += s[i];
+        for (int i = 0; i < G / 32; i++) v += to[i];
     }
     return v;
 }
 template <int G>
-FB2_DEV uint32_t largest(uint32_t v, float* s) {
+FB2_DEV uint32_t largest(uint32_t v, float (*s)[32], int& turn) {
     v = __reduce_max_sync(0xffffffffu, v);
     if constexpr (G > 32) {
-        __syncthreads();
-        if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = __uint_as_float(v);
+        float* to = s[turn++ & 1];
+        if ((threadIdx.x & 31) == 0) to[threadIdx.x >> 5] = __uint_as_float(v);
         __syncthreads();
         v = 0;
 #pragma unroll
-        for (int i = 0; i < G / 32; i++) v = max(v, __float_as_uint(s[i]));
+        for (int i = 0; i < G / 32; i++) v = max(v, __float_as_uint(to[i]));
     }
     return v;
 }
 
-// 8 values of a row from `at` on; those past `n` are 0.
-template <class T, bool VEC>
-FB2_DEV void load(const T* row, int at, int n, float (&v)[NORM_E]) {
+// Value i of piece j of a thread's: eight neighbours where rows can be read sixteen
+// bytes at a time, else neighbouring threads have neighbouring values.
+template <int G, bool VEC>
+FB2_DEV int at(int tid, int j, int i) {
+    return VEC ? (tid + j * G) * NORM_E + i : tid + (j * NORM_E + i) * G;
+}
+// Those past `n` are 0.
+template <class T, int G, bool VEC>
+FB2_DEV void load(const T* row, int tid, int j, int n, float (&v)[NORM_E]) {
     if constexpr (VEC) {
-        if (at < n) {
-            load8(row + at, v);
+        if (at<G, VEC>(tid, j, 0) < n) {
+            load8(row + at<G, VEC>(tid, j, 0), v);
             return;
         }
-    }
 #pragma unroll
-    for (int i = 0; i < NORM_E; i++) v[i] = at + i < n ? Dense<T>::get(row[at + i]) : 0.f;
+        for (int i = 0; i < NORM_E; i++) v[i] = 0.f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < NORM_E; i++) v[i] = at<G, VEC>(tid, j, i) < n ? Dense<T>::get(row[at<G, VEC>(tid, j, i)]) : 0.f;
+    }
 }
-template <class T, bool VEC>
-FB2_DEV void store(T* row, int at, int n, const float (&v)[NORM_E]) {
+template <class T, int G, bool VEC>
+FB2_DEV void store(T* row, int tid, int j, int n, const float (&v)[NORM_E]) {
     if constexpr (VEC) {
-        if (at >= n) return;
+        T* to = row + at<G, VEC>(tid, j, 0);
+        if (at<G, VEC>(tid, j, 0) >= n) return;
         constexpr int N = 16 / sizeof(T);
 #pragma unroll
-        for (int i = 0; i < NORM_E; i += N) *reinterpret_cast<uint4*>(row + at + i) = pack16<T>(v + i);
+        for (int i = 0; i < NORM_E; i += N) *reinterpret_cast<uint4*>(to + i) = pack16<T>(v + i);
     } else {
 #pragma unroll
         for (int i = 0; i < NORM_E; i++)
-            if (at + i < n) row[at + i] = Dense<T>::put(v[i]);
+            if (at<G, VEC>(tid, j, i) < n) row[at<G, VEC>(tid, j, i)] = Dense<T>::put(v[i]);
     }
 }
 
@@ -101,34 +112,36 @@ FB2_DEV uint32_t code(float x, float inv) {
     // no code is past 127: x * inv is at most 127 and two roundings
     return inv == 0.f ? 0u : (uint32_t)__float2int_rn(x * inv) & 0xffu;
 }
-template <bool VEC>
-FB2_DEV void store_codes(signed char* row, int at, int n, const float (&v)[NORM_E], float inv) {
-    if (VEC || at + NORM_E <= n) {  // rows of codes begin on 16 bytes
-        if (at >= n) return;
+template <int G, bool VEC>
+FB2_DEV void store_codes(signed char* row, int tid, int j, int n, const float (&v)[NORM_E], float inv) {
+    if constexpr (VEC) {  // rows of codes begin on 16 bytes
+        if (at<G, VEC>(tid, j, 0) >= n) return;
         uint32_t w[2] = {0, 0};
 #pragma unroll
         for (int i = 0; i < NORM_E; i++) w[i / 4] |= code(v[i], inv) << (8 * (i & 3));
-        *reinterpret_cast<uint2*>(row + at) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint2*>(row + at<G, VEC>(tid, j, 0)) = make_uint2(w[0], w[1]);
     } else {
 #pragma unroll
         for (int i = 0; i < NORM_E; i++)
-            if (at + i < n) row[at + i] = (signed char)code(v[i], inv);
+            if (at<G, VEC>(tid, j, i) < n) row[at<G, VEC>(tid, j, i)] = (signed char)code(v[i], inv);
     }
 }
 
 }  // namespace nrm
 
 // T: h, gate and y; X: x and the sum.  G threads share a row and hold 8 * NJ of
-// its values each; blockDim: G, or rows / warp of 4 for G = 32.
+// its values each; blockDim: G, or four rows of a warp each for G = 32.
 template <class T, class X, int G, int NJ, bool VEC>
 __global__ void __launch_bounds__(G == 32 ? 128 : G) k_residual_norm(NormArgs a) {
-    __shared__ float s[32];
+    __shared__ float s[2][32];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // a product's launch; it waits for this grid's end
     const int tid = G == 32 ? threadIdx.x & 31 : threadIdx.x;
     const int row = G == 32 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
     if (row >= a.rows) return;
     const int n = a.dim;
     const float count = (float)n;
-    float v[NJ][NORM_E];
+    int turn = 0;
+    float v[NJ][NORM_E], xv[NJ][NORM_E];
     // (v - mean) / sqrt(var + eps), or v / sqrt(mean square + eps)
     auto normed = [&](const float* w, const float* b) {
         float mean = 0.f, part = 0.f;
@@ -137,7 +150,7 @@ __global__ void __launch_bounds__(G == 32 ? 128 : G) k_residual_norm(NormArgs a)
             for (int j = 0; j < NJ; j++)
 #pragma unroll
                 for (int i = 0; i < NORM_E; i++) part += v[j][i];
-            mean = nrm::sum<G>(part, s) / count;
+            mean = nrm::sum<G>(part, s, turn) / count;
         }
         part = 0.f;
 #pragma unroll
@@ -145,89 +158,112 @@ __global__ void __launch_bounds__(G == 32 ? 128 : G) k_residual_norm(NormArgs a)
 #pragma unroll
             for (int i = 0; i < NORM_E; i++) {
                 const float d = v[j][i] - mean;
-                if ((tid + j * G) * NORM_E + i < n) part += d * d;
+                if (nrm::at<G, VEC>(tid, j, i) < n) part += d * d;
             }
-        const float r = 1.f / sqrtf(nrm::sum<G>(part, s) / count + a.eps);
+        const float r = 1.f / sqrtf(nrm::sum<G>(part, s, turn) / count + a.eps);
 #pragma unroll
         for (int j = 0; j < NJ; j++) {
-            const int at = (tid + j * G) * NORM_E;
             float wv[NORM_E], bv[NORM_E];
-            nrm::load<float, VEC>(w, at, n, wv);
-            if (b) nrm::load<float, VEC>(b, at, n, bv);
+            nrm::load<float, G, VEC>(w, tid, j, n, wv);
+            if (b) nrm::load<float, G, VEC>(b, tid, j, n, bv);
 #pragma unroll
             for (int i = 0; i < NORM_E; i++) {
                 v[j][i] = (v[j][i] - mean) * r * wv[i];
                 if (b) v[j][i] += bv[i];
-                if constexpr (!VEC) v[j][i] = at + i < n ? v[j][i] : 0.f;
             }
         }
     };
+    // all of the row's loads at once
     const X* x = static_cast<const X*>(a.x) + row * a.x_row;
+#pragma unroll
+    for (int j = 0; j < NJ; j++) nrm::load<X, G, VEC>(x, tid, j, n, xv[j]);
     if (a.h) {
         const T* h = static_cast<const T*>(a.h) + row * a.h_row;
 #pragma unroll
-        for (int j = 0; j < NJ; j++) nrm::load<T, VEC>(h, (tid + j * G) * NORM_E, n, v[j]);
+        for (int j = 0; j < NJ; j++) nrm::load<T, G, VEC>(h, tid, j, n, v[j]);
         if (a.post) normed(a.post_w, a.post_b);
-        const T* gate = static_cast<const T*>(a.gate) + (a.gate ? row * a.gate_row : 0);
+        if (a.gate) {
+            const T* gate = static_cast<const T*>(a.gate) + row * a.gate_row;
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                float gv[NORM_E];
+                nrm::load<T, G, VEC>(gate, tid, j, n, gv);
+#pragma unroll
+                for (int i = 0; i < NORM_E; i++) v[j][i] *= gv[i];
+            }
+        }
         X* sum = static_cast<X*>(a.sum) + row * a.sum_row;
 #pragma unroll
         for (int j = 0; j < NJ; j++) {
-            const int at = (tid + j * G) * NORM_E;
-            float xv[NORM_E], gv[NORM_E];
-            nrm::load<X, VEC>(x, at, n, xv);
-            if (a.gate) nrm::load<T, VEC>(gate, at, n, gv);
 #pragma unroll
-            for (int i = 0; i < NORM_E; i++) {
-                if (a.gate) v[j][i] *= gv[i];
-                v[j][i] = xv[i] + a.scale * v[j][i];
-            }
-            nrm::store<X, VEC>(sum, at, n, v[j]);
+            for (int i = 0; i < NORM_E; i++) v[j][i] = xv[j][i] + a.scale * v[j][i];
+            nrm::store<X, G, VEC>(sum, tid, j, n, v[j]);
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < NJ; j++) nrm::load<X, VEC>(x, (tid + j * G) * NORM_E, n, v[j]);
+        for (int j = 0; j < NJ; j++)
+#pragma unroll
+            for (int i = 0; i < NORM_E; i++) v[j][i] = xv[j][i];
     }
     normed(a.w, a.b);
     if (!a.codes) {
         T* y = static_cast<T*>(a.y) + row * a.y_row;
 #pragma unroll
-        for (int j = 0; j < NJ; j++) nrm::store<T, VEC>(y, (tid + j * G) * NORM_E, n, v[j]);
+        for (int j = 0; j < NJ; j++) nrm::store<T, G, VEC>(y, tid, j, n, v[j]);
         return;
     }
     uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < NJ; j++)
 #pragma unroll
-        for (int i = 0; i < NORM_E; i++) top = max(top, __float_as_uint(v[j][i]) & 0x7fffffffu);
+        for (int i = 0; i < NORM_E; i++)
+            if (nrm::at<G, VEC>(tid, j, i) < n) top = max(top, __float_as_uint(v[j][i]) & 0x7fffffffu);
     float inv, scale;
-    nrm::code_scale(nrm::largest<G>(top, s), inv, scale);
+    nrm::code_scale(nrm::largest<G>(top, s, turn), inv, scale);
 #pragma unroll
-    for (int j = 0; j < NJ; j++) nrm::store_codes<VEC>(a.codes + row * a.code_row, (tid + j * G) * NORM_E, n, v[j], inv);
+    for (int j = 0; j < NJ; j++) nrm::store_codes<G, VEC>(a.codes + row * a.code_row, tid, j, n, v[j], inv);
     if (tid == 0) a.scales[row] = scale;
 }
 
-// Rows x [rows][n] as codes: a CTA of 256 threads takes a row, of any length.
-constexpr int QR_THREADS = 256;
-template <class T, bool VEC>
-__global__ void __launch_bounds__(QR_THREADS) k_quantise_rows(const T* x, long long x_row, int n, signed char* codes, long long code_row,
-                                                              float* scales) {
-    __shared__ float s[32];
+// Rows x [rows][n] as codes, 8 * NJ values to a thread; NJ = 0: of any length, read
+// twice.
+template <class T, int G, int NJ, bool VEC>
+__global__ void __launch_bounds__(G) k_quantise_rows(const T* x, long long x_row, int n, signed char* codes, long long code_row,
+                                                     float* scales) {
+    __shared__ float s[2][32];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int tid = threadIdx.x;
     const long long row = blockIdx.x;
     x += row * x_row;
     codes += row * code_row;
     uint32_t top = 0;
-    float v[NORM_E];
-    for (int at = tid * NORM_E; at < n; at += QR_THREADS * NORM_E) {
-        nrm::load<T, VEC>(x, at, n, v);
+    float v[NJ ? NJ : 1][NORM_E];
+    auto most = [&](const float (&p)[NORM_E]) {
 #pragma unroll
-        for (int i = 0; i < NORM_E; i++) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+        for (int i = 0; i < NORM_E; i++) top = max(top, __float_as_uint(p[i]) & 0x7fffffffu);
+    };
+    if constexpr (NJ > 0) {
+#pragma unroll
+        for (int j = 0; j < NJ; j++) nrm::load<T, G, VEC>(x, tid, j, n, v[j]);
+#pragma unroll
+        for (int j = 0; j < NJ; j++) most(v[j]);
+    } else {
+        for (int j = 0; j * G * NORM_E < n; j++) {
+            nrm::load<T, G, VEC>(x, tid, j, n, v[0]);
+            most(v[0]);
+        }
     }
     float inv, scale;
-    nrm::code_scale(nrm::largest<QR_THREADS>(top, s), inv, scale);
-    for (int at = tid * NORM_E; at < n; at += QR_THREADS * NORM_E) {
-        nrm::load<T, VEC>(x, at, n, v);
-        nrm::store_codes<VEC>(codes, at, n, v, inv);
+    int turn = 0;
+    nrm::code_scale(nrm::largest<G>(top, s, turn), inv, scale);
+    if constexpr (NJ > 0) {
+#pragma unroll
+        for (int j = 0; j < NJ; j++) nrm::store_codes<G, VEC>(codes, tid, j, n, v[j], inv);
+    } else {
+        for (int j = 0; j * G * NORM_E < n; j++) {
+            nrm::load<T, G, VEC>(x, tid, j, n, v[0]);
+            nrm::store_codes<G, VEC>(codes, tid, j, n, v[0], inv);
+        }
     }
     if (tid == 0) scales[row] = scale;
 }

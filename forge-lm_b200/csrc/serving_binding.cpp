@@ -735,15 +735,6 @@ PyObject* linear8_pack(PyObject*, PyObject* const* args, Py_ssize_t count) {
     });
 }
 
-// codes and scales of the rows of x
-void quantised(const at::Tensor& x, int64_t rows, int64_t dim, int index, at::Tensor& codes, at::Tensor& scales, void* stream) {
-    const int32_t code = code_of(x.scalar_type());
-    codes = empty_codes(rows, dim, index), scales = empty({rows}, at::kFloat, index);
-    if (rows)
-        status(fb2_quantise_rows(small(rows, "rows"), small(dim, "columns"), x.data_ptr(), code, x.stride(0), codes.data_ptr(), codes.stride(0),
-                                 static_cast<float*>(scales.data_ptr()), stream));
-}
-
 PyObject* quantise_rows(PyObject*, PyObject* const* args, Py_ssize_t count) {
     ARGS(1)  // x
     return guarded([&]() -> PyObject* {
@@ -751,8 +742,10 @@ PyObject* quantise_rows(PyObject*, PyObject* const* args, Py_ssize_t count) {
         need(x.dim() == 2 && x.is_cuda() && x.size(1) > 0, "x must be a CUDA tensor [rows, columns]");
         matrix(args[0], "x", x.size(0), x.size(1), x.get_device());
         OnDevice on(x.get_device());
-        at::Tensor codes, scales;
-        quantised(x, x.size(0), x.size(1), on.index, codes, scales, on.stream());
+        const int32_t code = code_of(x.scalar_type());
+        at::Tensor codes = empty_codes(x.size(0), x.size(1), on.index), scales = empty({x.size(0)}, at::kFloat, on.index);
+        status(fb2_quantise_rows(small(x.size(0), "rows"), small(x.size(1), "columns"), x.data_ptr(), code, x.stride(0), codes.data_ptr(),
+                                 codes.stride(0), static_cast<float*>(scales.data_ptr()), on.stream()));
         return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(codes)), result(std::move(scales), x, "quantise_rows"));
     });
 }
@@ -781,15 +774,29 @@ PyObject* linear8_call(PyObject*, PyObject* const* args, Py_ssize_t count) {
         shape.back() = n;
         const fb2_w8_linear l = h.now();
         OnDevice on(h.index);
-        at::Tensor codes, scales;
-        if (!coded)
-            quantised(flat, rows, k, h.index, codes, scales, on.stream());
-        else if (reinterpret_cast<uintptr_t>(flat.data_ptr()) % 16 || (rows > 1 && (flat.stride(0) % 16 || flat.stride(0) < k)))
-            codes = empty_codes(rows, k, h.index).copy_(flat);  // the kernels' copies begin on 16 bytes
-        const at::Tensor& c = codes.defined() ? codes : flat;
-        at::Tensor y = empty(shape, type, h.index);
-        status(fb2_w8_matmul(&l, small(rows, "rows"), c.data_ptr(), c.stride(0),
-                             static_cast<const float*>((coded ? *given_scales : scales).data_ptr()), y.data_ptr(), n, code, on.stream()));
+        at::Tensor y = empty(shape, type, h.index), other_codes, work;
+        const int32_t n_rows = small(rows, "rows");
+        if (coded) {
+            // the kernels' copies begin on 16 bytes
+            if (reinterpret_cast<uintptr_t>(flat.data_ptr()) % 16 || (rows > 1 && (flat.stride(0) % 16 || flat.stride(0) < k)))
+                other_codes = empty_codes(rows, k, h.index).copy_(flat);
+            const at::Tensor& c = other_codes.defined() ? other_codes : flat;
+            status(fb2_w8_matmul(&l, n_rows, c.data_ptr(), c.stride(0), data<float>(given_scales), y.data_ptr(), n, code, on.stream()));
+        } else {
+            int64_t size = 0;
+            status(fb2_w8_forward_workspace(&l, n_rows, &size));
+            if (size) work = empty({size}, at::kByte, h.index);
+            if (type == x.scalar_type()) {
+                status(fb2_w8_forward(&l, n_rows, flat.data_ptr(), flat.stride(0), y.data_ptr(), n, code, size ? work.data_ptr() : nullptr, size,
+                                      on.stream()));
+            } else {  // a result of another type: by the codes
+                at::Tensor codes = empty_codes(rows, k, h.index), scales = empty({rows}, at::kFloat, h.index);
+                status(fb2_quantise_rows(n_rows, (int32_t)k, flat.data_ptr(), code_of(x.scalar_type()), flat.stride(0), codes.data_ptr(),
+                                         codes.stride(0), static_cast<float*>(scales.data_ptr()), on.stream()));
+                status(fb2_w8_matmul(&l, n_rows, codes.data_ptr(), codes.stride(0), static_cast<const float*>(scales.data_ptr()), y.data_ptr(), n,
+                                     code, on.stream()));
+            }
+        }
         return result(std::move(y), {&x, given_scales, &h.scales, h.bias.defined() ? &h.bias : nullptr}, "W8Linear");
     });
 }

@@ -114,12 +114,20 @@ void launch_norm(const NormArgs& a, bool vec, cudaStream_t stream) {
 }
 template <class T, class X>
 void launch_norm(const NormArgs& a, bool vec, cudaStream_t stream) {
+    // threads of a row: few values each where rows are few, else up to 32
+    const bool few = a.rows <= 4 * 148;
     if (a.dim <= 256)
         launch_norm<T, X, 32, 1>(a, vec, stream);
+    else if (a.dim <= 1024 && few)
+        launch_norm<T, X, 128, 1>(a, vec, stream);
     else if (a.dim <= 1024)
         launch_norm<T, X, 32, 4>(a, vec, stream);
+    else if (a.dim <= 4096 && few)
+        launch_norm<T, X, 512, 1>(a, vec, stream);
     else if (a.dim <= 4096)
         launch_norm<T, X, 128, 4>(a, vec, stream);
+    else if (a.dim <= 8192)
+        launch_norm<T, X, 256, 4>(a, vec, stream);
     else if (a.dim <= 16384)
         launch_norm<T, X, 512, 4>(a, vec, stream);
     else
@@ -190,8 +198,17 @@ int32_t fb2_quantise_rows(int32_t n_rows, int32_t dim, const void* x, int32_t dt
         const bool vec = dim % NORM_E == 0 && aligned(x, 16) && (n_rows == 1 || x_row * es % 16 == 0);
         with_type(dtype, [&](auto t) {
             using T = decltype(t);
-            (vec ? k_quantise_rows<T, true> : k_quantise_rows<T, false>)<<<n_rows, QR_THREADS, 0, (cudaStream_t)stream>>>(
-                (const T*)x, x_row, dim, (signed char*)codes, code_row, scales);
+            auto launch = [&](auto kernel, int threads) {
+                kernel<<<n_rows, threads, 0, (cudaStream_t)stream>>>((const T*)x, x_row, dim, (signed char*)codes, code_row, scales);
+            };
+            if (dim <= 1024)
+                launch(vec ? k_quantise_rows<T, 128, 1, true> : k_quantise_rows<T, 128, 1, false>, 128);
+            else if (dim <= 4096)
+                launch(vec ? k_quantise_rows<T, 128, 4, true> : k_quantise_rows<T, 128, 4, false>, 128);
+            else if (dim <= 16384)
+                launch(vec ? k_quantise_rows<T, 512, 4, true> : k_quantise_rows<T, 512, 4, false>, 512);
+            else
+                launch(vec ? k_quantise_rows<T, 512, 0, true> : k_quantise_rows<T, 512, 0, false>, 512);
         });
         launched();
     });
@@ -243,8 +260,48 @@ template <class T, int BN>
 void launch_few(const CUtensorMap& mw, const CUtensorMap& mx, const W8Args& a, void* stream) {
     const int tiles = (a.out + 127) / 128, across = (a.rows + BN - 1) / BN, blocks = (a.in + W8_K - 1) / W8_K;
     int ranks = 1;
-    while (ranks < 8 && (int64_t)tiles * across * ranks * 2 <= 148 && ranks * 2 <= blocks) ranks *= 2;
+    while (ranks < 8 && (int64_t)tiles * across * ranks * 2 <= 2 * 148 && ranks * 2 <= blocks) ranks *= 2;
     launch_cluster(k_w8_few<T, BN>, dim3(tiles * ranks, across), W8_THREADS, W8Few<BN>::SMEM, ranks, true, stream, mw, mx, a, ranks);
+}
+
+// Few rows: pieces of a lane's inputs, warps that share an output's
+struct W8Rows {
+    int pieces, per_k;
+};
+constexpr int W8R_MOST = 4;
+bool w8_by_rows(int rows, int in) { return rows <= W8R_MOST && in <= 4 * W8R_WARPS * 512; }
+W8Rows w8_rows_plan(int in) {
+    W8Rows p{1, 1};
+    while (p.per_k < W8R_WARPS && p.per_k * 512 < in) p.per_k *= 2;
+    while (p.pieces * p.per_k * 512 < in) p.pieces *= 2;
+    return p;
+}
+template <class T, class X, int ROWS>
+void launch_rows(const fb2_w8_linear* w, const W8Args& a, const X* x, int64_t x_row, bool vec, bool early, void* stream) {
+    const W8Rows p = w8_rows_plan(a.in);
+    const int slots = W8R_WARPS / p.per_k;
+    // two CTAs on each SM, of at least an output for each slot, and what the sums have room for
+    int64_t grid = std::min<int64_t>(2 * 148, (a.out + slots - 1) / slots);
+    grid = std::max<int64_t>(grid, ((int64_t)a.out * ROWS + W8R_SUMS - ROWS - 1) / (W8R_SUMS - ROWS));
+    auto go = [&](auto kernel) {
+        launch_cluster(kernel, dim3((unsigned)grid), W8R_THREADS, 0, 1, early, stream, a, x, x_row, (const signed char*)w->device_codes,
+                       row_stride(a.out, w->code_row_stride, a.in), p.per_k, vec);
+    };
+    if (p.pieces == 1)
+        go(k_w8_rows<T, X, ROWS, 1>);
+    else if (p.pieces == 2)
+        go(k_w8_rows<T, X, ROWS, 2>);
+    else
+        go(k_w8_rows<T, X, ROWS, 4>);
+}
+template <class T, class X>
+void launch_rows(const fb2_w8_linear* w, const W8Args& a, const X* x, int64_t x_row, bool vec, bool early, void* stream) {
+    if (a.rows == 1)
+        launch_rows<T, X, 1>(w, a, x, x_row, vec, early, stream);
+    else if (a.rows == 2)
+        launch_rows<T, X, 2>(w, a, x, x_row, vec, early, stream);
+    else
+        launch_rows<T, X, 4>(w, a, x, x_row, vec, early, stream);
 }
 
 std::atomic<int> g_withhold_block{-1};
@@ -301,7 +358,9 @@ int32_t fb2_w8_matmul(const fb2_w8_linear* w, int32_t n_rows, const void* codes,
         auto w_map = [&](int box) { return byte_map(w->device_codes, a.in, a.out, row_stride(a.out, w->code_row_stride, a.in), box); };
         with_type(dtype, [&](auto t) {
             using T = decltype(t);
-            if (n_rows <= 16)
+            if (w8_by_rows(n_rows, a.in))
+                launch_rows<T>(w, a, (const signed char*)codes, code_row, true, true, stream);
+            else if (n_rows <= 16)
                 launch_few<T, 16>(w_map(128), x_map(16), a, stream);
             else if (n_rows <= 32)
                 launch_few<T, 32>(w_map(128), x_map(32), a, stream);
@@ -317,6 +376,46 @@ int32_t fb2_w8_matmul(const fb2_w8_linear* w, int32_t n_rows, const void* codes,
             }
         });
         launched();
+    });
+}
+
+int32_t fb2_w8_forward_workspace(const fb2_w8_linear* w, int32_t n_rows, int64_t* bytes) {
+    return guarded([&] {
+        check_w8(w);
+        need(n_rows >= 0, "n_rows must not be negative");
+        need(bytes, "bytes is NULL");
+        // codes on 16 bytes, and scales
+        *bytes = n_rows == 0 || w8_by_rows(n_rows, w->in_features) ? 0 : (int64_t)n_rows * (row_stride(1, 0, w->in_features) + 4);
+    });
+}
+
+int32_t fb2_w8_forward(const fb2_w8_linear* w, int32_t n_rows, const void* x, int64_t x_row, void* y, int64_t y_row, int32_t dtype,
+                       void* workspace, int64_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        check_w8(w);
+        check_dtype(dtype);
+        need(n_rows >= 0 && n_rows <= INT32_MAX - 255, "n_rows must be in 0..2^31 - 256");
+        if (n_rows == 0) return;
+        need(x && y, "NULL argument");
+        const size_t es = size_of(dtype);
+        need(aligned(x, es) && aligned(y, es), "a tensor is not aligned to its element size");
+        need(n_rows == 1 || y_row >= w->out_features, "y_row_stride must be at least out_features");
+        if (w8_by_rows(n_rows, w->in_features)) {
+            const W8Args a{nullptr, w->device_scales, w->device_bias, y, y_row, n_rows, w->in_features, w->out_features, false, -1, 0};
+            const bool vec = aligned(x, 16) && (n_rows == 1 || x_row * es % 16 == 0);
+            with_type(dtype, [&](auto t) {
+                using T = decltype(t);
+                launch_rows<T>(w, a, (const T*)x, x_row, vec, false, stream);
+            });
+            return;
+        }
+        const int64_t row = row_stride(1, 0, w->in_features), bytes = n_rows * (row + 4);
+        need(workspace && workspace_bytes >= bytes, "the workspace is too small");
+        need(aligned(workspace, 16), "the workspace must be 16-byte aligned");
+        float* scales = reinterpret_cast<float*>(static_cast<char*>(workspace) + n_rows * row);
+        int32_t s = fb2_quantise_rows(n_rows, w->in_features, x, dtype, x_row, workspace, row, scales, stream);
+        if (s == FB2_OK) s = fb2_w8_matmul(w, n_rows, workspace, row, scales, y, y_row, dtype, stream);
+        if (s != FB2_OK) fail(s, std::string(fb2_last_error()));
     });
 }
 

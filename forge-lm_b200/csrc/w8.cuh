@@ -8,6 +8,7 @@
 // no bit; only the epilogue rounds.  Both operands are K-major rows of bytes, TMA
 // boxes of 128 bytes x rows, 128-byte swizzled.
 //
+// k_w8_rows: up to 4 rows of x, on the warps' dot products, quantised on the way.
 // k_w8_few: up to 128 rows of x to a tile, as the N side of the tiles, the weights
 // as the M side: each weight is read once.  A cluster shares a tile's inputs where
 // there are fewer tiles than SMs.
@@ -57,12 +58,20 @@ FB2_DEV void ld16(uint32_t at, int (&v)[16]) {
         : "r"(at));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+FB2_DEV void prefetch(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory"); }
 FB2_DEV void arrive(uint64_t* b) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_addr(b)) : "memory"); }
 FB2_DEV int peek(uint32_t at, int rank) {
     uint32_t r;
     int v;
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
     asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(r) : "memory");
+    return v;
+}
+FB2_DEV int4 peek4(uint32_t at, int rank) {
+    uint32_t r;
+    int4 v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(r) : "memory");
     return v;
 }
 FB2_DEV float value(int sum, float w_scale, float x_scale, float bias) {
@@ -74,7 +83,7 @@ FB2_DEV float value(int sum, float w_scale, float x_scale, float bias) {
 template <int BN>
 struct W8Few {
     static constexpr int STAGE = W8_TILE + BN * W8_K;
-    static constexpr int STAGES = (200 * 1024) / STAGE > 8 ? 8 : (200 * 1024) / STAGE;
+    static constexpr int STAGES = (108 * 1024) / STAGE;  // two CTAs to an SM
     static constexpr int PART = BN * 128 * 4;  // sums of a tile
     static constexpr int SMEM = (STAGES * STAGE > PART ? STAGES * STAGE : PART) + 1024;
     static constexpr uint32_t COLS = BN < 32 ? 32 : BN;
@@ -83,7 +92,7 @@ struct W8Few {
 // blockIdx.x: tile of 128 outputs and, fastest, the CTA's rank in the cluster that
 // shares its inputs; blockIdx.y: tile of BN rows of x.
 template <class T, int BN>
-__global__ void __launch_bounds__(W8_THREADS, 1)
+__global__ void __launch_bounds__(W8_THREADS, 2)
     k_w8_few(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, W8Args a, int ranks) {
     using S = W8Few<BN>;
     extern __shared__ unsigned char w8_raw[];
@@ -96,6 +105,7 @@ __global__ void __launch_bounds__(W8_THREADS, 1)
     const int blocks = (a.in + W8_K - 1) / W8_K;
     const int k0 = (int)((long long)blocks * rank / ranks), nk = (int)((long long)blocks * (rank + 1) / ranks) - k0;
     if (tid == 0) {
+        w8::prefetch(&map_w), w8::prefetch(&map_x);
         s_abort = 0;
         for (int i = 0; i < S::STAGES; i++) {
             tc::bar_init(&full[i], 1);
@@ -199,17 +209,38 @@ __global__ void __launch_bounds__(W8_THREADS, 1)
             }
         }
         pg::cluster_sync();
-        // each CTA sums and writes some of the rows
-        if (warp < 4) {
-            bool bad = false;
-            for (int k = 0; k < ranks; k++) bad |= w8::peek(tc::smem_addr(&s_failed), k) != 0;
-            const int o = o0 + 32 * quarter + lane;
-            const float ws = o < a.out ? __ldg(a.w_scales + o) : 0.f, bias = a.bias && o < a.out ? __ldg(a.bias + o) : 0.f;
-            for (int c = rank; c < BN && r0 + c < a.rows; c += ranks) {
-                int sum = 0;
-                for (int k = 0; k < ranks; k++) sum += w8::peek(tc::smem_addr(part + c * 128 + 32 * quarter + lane), k);
-                const int r = r0 + c;
-                if (o < a.out) y[r * a.y_row + o] = Dense<T>::put(bad ? nan : w8::value(sum, ws, __ldg(a.x_scales + r), bias));
+        // each CTA sums and writes some of the rows: a warp a row, a lane four outputs
+        const bool bad = __any_sync(0xffffffffu, lane < ranks && w8::peek(tc::smem_addr(&s_failed), lane) != 0);
+        const int o = o0 + 4 * lane;
+        float ws[4], bias[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            ws[j] = o + j < a.out ? __ldg(a.w_scales + o + j) : 0.f;
+            bias[j] = a.bias && o + j < a.out ? __ldg(a.bias + o + j) : 0.f;
+        }
+        const bool whole = a.vec && o + 4 <= a.out && a.out % 4 == 0;
+        for (int c = rank + warp * ranks; c < BN && r0 + c < a.rows; c += ranks * (W8_THREADS / 32)) {
+            const int r = r0 + c;
+            const float xs = __ldg(a.x_scales + r);
+            int4 sum = make_int4(0, 0, 0, 0);
+            for (int k = 0; k < ranks; k++) {
+                const int4 v = w8::peek4(tc::smem_addr(part + c * 128 + 4 * lane), k);
+                sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+            }
+            const int s4[4] = {sum.x, sum.y, sum.z, sum.w};
+            T* to = y + r * a.y_row + o;
+            __align__(16) T out[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) out[j] = Dense<T>::put(bad ? nan : w8::value(s4[j], ws[j], xs, bias[j]));
+            if (whole) {
+                if constexpr (sizeof(T) == 4)
+                    *reinterpret_cast<uint4*>(to) = *reinterpret_cast<uint4*>(out);
+                else
+                    *reinterpret_cast<uint2*>(to) = *reinterpret_cast<uint2*>(out);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (o + j < a.out) to[j] = out[j];
             }
         }
         pg::cluster_sync();  // the others' shared memory stays until it is read
@@ -220,6 +251,158 @@ __global__ void __launch_bounds__(W8_THREADS, 1)
         tc::fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");
     }
+}
+
+// ---- up to four rows, on the integer dot products of the warps ---------------------------
+// One launch from x to y.  A lane keeps its inputs (16 bytes of codes for each row and
+// piece of 512 inputs of a warp) in registers and takes the weights of one output after
+// another against them, W8R_AHEAD pieces in flight; what a row's scale needs of all
+// inputs each CTA finds for itself.  `per_k` warps share an output's inputs, the sums
+// meet in shared memory as integers.  The weights' bytes bound it.
+constexpr int W8R_THREADS = 512, W8R_WARPS = W8R_THREADS / 32, W8R_AHEAD = 8;
+constexpr int W8R_SUMS = 6144;  // sums of a CTA: outputs times rows
+
+// T: type of y; X: of x, signed char for codes; PIECES: of a lane's inputs
+template <class T, class X, int ROWS, int PIECES>
+__global__ void __launch_bounds__(W8R_THREADS, PIECES * ROWS <= 4 ? 2 : 1)
+    k_w8_rows(W8Args a, const X* x, long long x_row, const signed char* w, long long w_row, int per_k, bool vec) {
+    constexpr bool CODES = sizeof(X) == 1;
+    constexpr int AHEAD = W8R_AHEAD / PIECES;  // outputs
+    __shared__ int s_sum[W8R_SUMS];
+    __shared__ uint32_t s_top[ROWS][W8R_WARPS];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int slots = W8R_WARPS / per_k, slot = warp / per_k, part = warp % per_k;
+    const int o0 = (int)((long long)a.out * blockIdx.x / gridDim.x), o1 = (int)((long long)a.out * (blockIdx.x + 1) / gridDim.x);
+    // piece p of the lane: inputs at(p) .. at(p) + 15
+    auto at = [&](int p) { return ((part + p * per_k) * 32 + lane) * 16; };
+    // 16 weights; what lies behind the row's end may be anything, as x is 0 there, but is
+    // not read past the piece that has the end
+    auto weights = [&](int o, int p) {
+        const signed char* from = w + o * w_row + at(p);
+        if (at(p) + 16 <= a.in) return __ldcs(reinterpret_cast<const int4*>(from));
+        int v[4] = {0, 0, 0, 0};
+        for (int i = 0; at(p) + i < a.in; i++) v[i >> 2] |= (from[i] & 0xff) << (8 * (i & 3));
+        return make_int4(v[0], v[1], v[2], v[3]);
+    };
+    int4 next[AHEAD][PIECES];
+    auto load = [&](int o) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++)
+#pragma unroll
+            for (int p = 0; p < PIECES; p++)
+                if (o + u * slots < o1) next[u][p] = weights(o + u * slots, p);
+    };
+    for (int i = tid; i < (o1 - o0) * ROWS; i += W8R_THREADS) s_sum[i] = 0;
+    pdl_wait();
+    load(o0 + slot);
+    int code[ROWS][PIECES][4];
+    float x_scale[ROWS];
+    if constexpr (CODES) {
+#pragma unroll
+        for (int r = 0; r < ROWS; r++) {
+            x_scale[r] = r < a.rows ? __ldg(a.x_scales + r) : 0.f;
+#pragma unroll
+            for (int p = 0; p < PIECES; p++) {
+                int4 v = make_int4(0, 0, 0, 0);
+                const signed char* from = x + r * x_row + at(p);
+                if (r < a.rows && at(p) + 16 <= a.in) {
+                    v = *reinterpret_cast<const int4*>(from);
+                } else if (r < a.rows) {
+                    int b[4] = {0, 0, 0, 0};
+                    for (int i = 0; at(p) + i < a.in; i++) b[i >> 2] |= (from[i] & 0xff) << (8 * (i & 3));
+                    v = make_int4(b[0], b[1], b[2], b[3]);
+                }
+                code[r][p][0] = v.x, code[r][p][1] = v.y, code[r][p][2] = v.z, code[r][p][3] = v.w;
+            }
+        }
+        __syncthreads();
+    } else {
+        // rows past the last are rows of zeros; a warp that repeats another's inputs does so
+        auto values = [&](int r, int p, float (&v)[16]) {
+            const X* from = x + r * x_row + at(p);
+            if (vec && at(p) + 16 <= a.in) {
+                constexpr int N = 16 / sizeof(X);
+#pragma unroll
+                for (int i = 0; i < 16; i += N) unpack16<X>(__ldg(reinterpret_cast<const uint4*>(from + i)), v + i);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; i++) v[i] = at(p) + i < a.in ? Dense<X>::get(from[i]) : 0.f;
+            }
+        };
+        float keep[ROWS * PIECES == 1 ? 16 : 1];
+#pragma unroll
+        for (int r = 0; r < ROWS; r++) {
+            uint32_t top = 0;
+            if (r < a.rows) {
+#pragma unroll
+                for (int p = 0; p < PIECES; p++) {
+                    float v[16];
+                    values(r, p, v);
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+                        if constexpr (ROWS * PIECES == 1) keep[i] = v[i];
+                    }
+                }
+            }
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0) s_top[r][warp] = top;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < ROWS; r++) {
+            float inv;
+            nrm::code_scale(__reduce_max_sync(0xffffffffu, s_top[r][lane % W8R_WARPS]), inv, x_scale[r]);
+#pragma unroll
+            for (int p = 0; p < PIECES; p++) {
+                float v[16];
+                if constexpr (ROWS * PIECES == 1) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) v[i] = keep[i];
+                } else if (r < a.rows) {
+                    values(r, p, v);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    code[r][p][j] = 0;
+                    if (r < a.rows)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) code[r][p][j] |= nrm::code(v[4 * j + i], inv) << (8 * i);
+                }
+            }
+        }
+    }
+    for (int o = o0 + slot; o < o1; o += AHEAD * slots) {
+        int4 now[AHEAD][PIECES];
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++)
+#pragma unroll
+            for (int p = 0; p < PIECES; p++) now[u][p] = next[u][p];
+        load(o + AHEAD * slots);
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+            if (o + u * slots >= o1) break;
+#pragma unroll
+            for (int r = 0; r < ROWS; r++) {
+                int sum = 0;
+#pragma unroll
+                for (int p = 0; p < PIECES; p++) {
+                    sum = __dp4a(now[u][p].x, code[r][p][0], sum);
+                    sum = __dp4a(now[u][p].y, code[r][p][1], sum);
+                    sum = __dp4a(now[u][p].z, code[r][p][2], sum);
+                    sum = __dp4a(now[u][p].w, code[r][p][3], sum);
+                }
+                sum = __reduce_add_sync(0xffffffffu, sum);
+                if (lane == 0) atomicAdd(&s_sum[(o + u * slots - o0) * ROWS + r], sum);
+            }
+        }
+    }
+    __syncthreads();
+    T* y = static_cast<T*>(a.y);
+#pragma unroll
+    for (int r = 0; r < ROWS; r++)
+        for (int i = tid; r < a.rows && i < o1 - o0; i += W8R_THREADS)
+            y[r * a.y_row + o0 + i] = Dense<T>::put(w8::value(s_sum[i * ROWS + r], __ldg(a.w_scales + o0 + i), x_scale[r], a.bias ? __ldg(a.bias + o0 + i) : 0.f));
 }
 
 // ---- many rows -------------------------------------------------------------------------
@@ -251,6 +434,7 @@ __global__ void __launch_bounds__(W8_THREADS, 1)
         o0 = within / high * W8M_N;
     };
     if (tid == 0) {
+        w8::prefetch(&map_w), w8::prefetch(&map_x);
         s_abort = 0;
         for (int i = 0; i < W8M_STAGES; i++) {
             tc::bar_init(&full[i], 1);

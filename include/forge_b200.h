@@ -549,6 +549,13 @@ int32_t fb2_w8_pack(const fb2_w8_linear* w, const void* device_w, int32_t dtype,
 int32_t fb2_w8_matmul(const fb2_w8_linear* w, int32_t n_rows, const void* device_codes, int64_t code_row_stride, const float* device_scales,
                       void* device_y, int64_t y_row_stride, int32_t dtype, void* cuda_stream);
 
+/* The same of rows of values x [n_rows][in] (dtype, x_row_stride elements apart), which are
+ * quantised as by fb2_quantise_rows on the way.  device_workspace: fb2_w8_forward_workspace
+ * bytes, 16-byte aligned. */
+int32_t fb2_w8_forward_workspace(const fb2_w8_linear* w, int32_t n_rows, int64_t* bytes);
+int32_t fb2_w8_forward(const fb2_w8_linear* w, int32_t n_rows, const void* device_x, int64_t x_row_stride, void* device_y,
+                       int64_t y_row_stride, int32_t dtype, void* device_workspace, int64_t workspace_bytes, void* cuda_stream);
+
 /* Drafted tokens against the target's probabilities.  Rows row_starts[b] ..
  * row_starts[b + 1] - 1 (ascending) are sequence b's nodes: the first its last
  * token, the others drafts below it, node i below node parents[i] < i (counted from the
