@@ -269,39 +269,39 @@ struct W8Rows {
     int pieces, per_k;
 };
 constexpr int W8R_MOST = 4;
-bool w8_by_rows(int rows, int in) { return rows <= W8R_MOST && in <= 4 * W8R_WARPS * 512; }
+bool w8_by_rows(int rows, int in) {
+    return rows <= W8R_MOST && in <= W8R_CODES && (rows > 2 ? 4 : rows) * ((in + 15) / 16 * 16) <= W8R_CODES;
+}
 W8Rows w8_rows_plan(int in) {
     W8Rows p{1, 1};
     while (p.per_k < W8R_WARPS && p.per_k * 512 < in) p.per_k *= 2;
     while (p.pieces * p.per_k * 512 < in) p.pieces *= 2;
     return p;
 }
-template <class T, class X, int ROWS>
-void launch_rows(const fb2_w8_linear* w, const W8Args& a, const X* x, int64_t x_row, bool vec, bool early, void* stream) {
-    const W8Rows p = w8_rows_plan(a.in);
-    const int slots = W8R_WARPS / p.per_k;
-    // two CTAs on each SM, of at least an output for each slot, and what the sums have room for
-    int64_t grid = std::min<int64_t>(2 * 148, (a.out + slots - 1) / slots);
+template <class T, class X, int ROWS, int PIECES>
+void launch_rows(const fb2_w8_linear* w, const W8Args& a, const X* x, int64_t x_row, bool vec, bool early, int per_k, void* stream) {
+    const int slots = W8R_WARPS / per_k, codes = sizeof(X) == 1 ? 0 : a.rows * (int)row_stride(1, 0, a.in);
+    // every SM full, an output at least for each slot, and what the sums have room for
+    int64_t grid = std::min<int64_t>(w8r_resident<X, ROWS, PIECES> * 148, (a.out + slots - 1) / slots);
     grid = std::max<int64_t>(grid, ((int64_t)a.out * ROWS + W8R_SUMS - ROWS - 1) / (W8R_SUMS - ROWS));
-    auto go = [&](auto kernel) {
-        launch_cluster(kernel, dim3((unsigned)grid), W8R_THREADS, 0, 1, early, stream, a, x, x_row, (const signed char*)w->device_codes,
-                       row_stride(a.out, w->code_row_stride, a.in), p.per_k, vec);
-    };
-    if (p.pieces == 1)
-        go(k_w8_rows<T, X, ROWS, 1>);
-    else if (p.pieces == 2)
-        go(k_w8_rows<T, X, ROWS, 2>);
-    else
-        go(k_w8_rows<T, X, ROWS, 4>);
+    launch_cluster(k_w8_rows<T, X, ROWS, PIECES>, dim3((unsigned)grid), W8R_THREADS, codes, 1, early, stream, a, x, x_row,
+                   (const signed char*)w->device_codes, row_stride(a.out, w->code_row_stride, a.in), per_k, vec);
 }
 template <class T, class X>
 void launch_rows(const fb2_w8_linear* w, const W8Args& a, const X* x, int64_t x_row, bool vec, bool early, void* stream) {
-    if (a.rows == 1)
-        launch_rows<T, X, 1>(w, a, x, x_row, vec, early, stream);
+    const W8Rows p = w8_rows_plan(a.in);  // rows (3 count as 4) times pieces: at most 4
+    auto go = [&](auto rows, auto pieces) {
+        launch_rows<T, X, decltype(rows)::value, decltype(pieces)::value>(w, a, x, x_row, vec, early, p.per_k, stream);
+    };
+    const std::integral_constant<int, 1> one;
+    const std::integral_constant<int, 2> two;
+    const std::integral_constant<int, 4> four;
+    if (a.rows > 2)
+        go(four, one);
     else if (a.rows == 2)
-        launch_rows<T, X, 2>(w, a, x, x_row, vec, early, stream);
+        p.pieces == 1 ? go(two, one) : go(two, two);
     else
-        launch_rows<T, X, 4>(w, a, x, x_row, vec, early, stream);
+        p.pieces == 1 ? go(one, one) : p.pieces == 2 ? go(one, two) : go(one, four);
 }
 
 std::atomic<int> g_withhold_block{-1};

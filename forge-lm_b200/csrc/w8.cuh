@@ -254,20 +254,25 @@ __global__ void __launch_bounds__(W8_THREADS, 2)
 }
 
 // ---- up to four rows, on the integer dot products of the warps ---------------------------
-// One launch from x to y.  A lane keeps its inputs (16 bytes of codes for each row and
-// piece of 512 inputs of a warp) in registers and takes the weights of one output after
-// another against them, W8R_AHEAD pieces in flight; what a row's scale needs of all
-// inputs each CTA finds for itself.  `per_k` warps share an output's inputs, the sums
-// meet in shared memory as integers.  The weights' bytes bound it.
+// One launch from x to y.  Each CTA makes the codes of x for itself, in shared memory; a
+// lane takes its inputs of them (16 bytes for each row and piece of 512 inputs of a warp)
+// into registers and the weights of one output after another against them, W8R_AHEAD
+// pieces in flight.  `per_k` warps share an output's inputs; the sums meet in shared
+// memory as integers.  The weights' bytes bound it.
 constexpr int W8R_THREADS = 512, W8R_WARPS = W8R_THREADS / 32, W8R_AHEAD = 8;
-constexpr int W8R_SUMS = 6144;  // sums of a CTA: outputs times rows
+constexpr int W8R_SUMS = 4096;       // sums of a CTA: outputs times rows
+constexpr int W8R_CODES = 32 * 1024;  // bytes of x's codes: what a lane's registers take of them
+template <class X, int ROWS, int PIECES>
+constexpr int w8r_resident = sizeof(X) > 1 && ROWS * PIECES == 1 ? 2 : 1;  // CTAs of an SM, by registers
 
-// T: type of y; X: of x, signed char for codes; PIECES: of a lane's inputs
+// T: type of y; X: of x, signed char for codes; PIECES: of a lane's inputs; `vec`: rows of
+// values can be read 16 bytes at a time
 template <class T, class X, int ROWS, int PIECES>
-__global__ void __launch_bounds__(W8R_THREADS, PIECES * ROWS <= 4 ? 2 : 1)
+__global__ void __launch_bounds__(W8R_THREADS, w8r_resident<X, ROWS, PIECES>)
     k_w8_rows(W8Args a, const X* x, long long x_row, const signed char* w, long long w_row, int per_k, bool vec) {
     constexpr bool CODES = sizeof(X) == 1;
     constexpr int AHEAD = W8R_AHEAD / PIECES;  // outputs
+    extern __shared__ __align__(16) signed char s_code[];  // [ROWS][in, rounded up to 16]
     __shared__ int s_sum[W8R_SUMS];
     __shared__ uint32_t s_top[ROWS][W8R_WARPS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -275,127 +280,123 @@ __global__ void __launch_bounds__(W8R_THREADS, PIECES * ROWS <= 4 ? 2 : 1)
     const int o0 = (int)((long long)a.out * blockIdx.x / gridDim.x), o1 = (int)((long long)a.out * (blockIdx.x + 1) / gridDim.x);
     // piece p of the lane: inputs at(p) .. at(p) + 15
     auto at = [&](int p) { return ((part + p * per_k) * 32 + lane) * 16; };
-    // 16 weights; what lies behind the row's end may be anything, as x is 0 there, but is
-    // not read past the piece that has the end
-    auto weights = [&](int o, int p) {
-        const signed char* from = w + o * w_row + at(p);
-        if (at(p) + 16 <= a.in) return __ldcs(reinterpret_cast<const int4*>(from));
-        int v[4] = {0, 0, 0, 0};
-        for (int i = 0; at(p) + i < a.in; i++) v[i >> 2] |= (from[i] & 0xff) << (8 * (i & 3));
-        return make_int4(v[0], v[1], v[2], v[3]);
-    };
-    int4 next[AHEAD][PIECES];
-    auto load = [&](int o) {
-#pragma unroll
-        for (int u = 0; u < AHEAD; u++)
-#pragma unroll
-            for (int p = 0; p < PIECES; p++)
-                if (o + u * slots < o1) next[u][p] = weights(o + u * slots, p);
+    const long long step = slots * w_row;
+    // the weights of a piece; those behind the row's end may be anything, as x is 0 there.
+    // What is behind the last row may not be memory: its last piece comes at the end.
+    auto weights = [&](int o, const signed char* row, int p) {
+        const bool there = at(p) < a.in && (o < a.out - 1 || at(p) + 16 <= a.in);
+        return there ? __ldcs(reinterpret_cast<const int4*>(row + at(p))) : make_int4(0, 0, 0, 0);
     };
     for (int i = tid; i < (o1 - o0) * ROWS; i += W8R_THREADS) s_sum[i] = 0;
     pdl_wait();
-    load(o0 + slot);
-    int code[ROWS][PIECES][4];
+    int4 held[AHEAD][PIECES];
+    const signed char* from = w + (o0 + slot) * w_row;
+#pragma unroll
+    for (int u = 0; u < AHEAD; u++)
+#pragma unroll
+        for (int p = 0; p < PIECES; p++)
+            if (o0 + slot + u * slots < o1) held[u][p] = weights(o0 + slot + u * slots, from + u * step, p);
+    int4 code[ROWS][PIECES];
     float x_scale[ROWS];
     if constexpr (CODES) {
+        __syncthreads();  // the sums are 0
 #pragma unroll
         for (int r = 0; r < ROWS; r++) {
             x_scale[r] = r < a.rows ? __ldg(a.x_scales + r) : 0.f;
 #pragma unroll
             for (int p = 0; p < PIECES; p++) {
-                int4 v = make_int4(0, 0, 0, 0);
-                const signed char* from = x + r * x_row + at(p);
+                code[r][p] = make_int4(0, 0, 0, 0);
+                const signed char* xr = (const signed char*)x + r * x_row + at(p);
                 if (r < a.rows && at(p) + 16 <= a.in) {
-                    v = *reinterpret_cast<const int4*>(from);
-                } else if (r < a.rows) {
-                    int b[4] = {0, 0, 0, 0};
-                    for (int i = 0; at(p) + i < a.in; i++) b[i >> 2] |= (from[i] & 0xff) << (8 * (i & 3));
-                    v = make_int4(b[0], b[1], b[2], b[3]);
+                    code[r][p] = __ldg(reinterpret_cast<const int4*>(xr));
+                } else if (r < a.rows && at(p) < a.in) {  // the row ends inside the piece
+                    int c[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int i = 0; i < 15; i++) c[i / 4] |= at(p) + i < a.in ? (xr[i] & 0xff) << (8 * (i & 3)) : 0;
+                    code[r][p] = make_int4(c[0], c[1], c[2], c[3]);
                 }
-                code[r][p][0] = v.x, code[r][p][1] = v.y, code[r][p][2] = v.z, code[r][p][3] = v.w;
             }
         }
-        __syncthreads();
     } else {
-        // rows past the last are rows of zeros; a warp that repeats another's inputs does so
-        auto values = [&](int r, int p, float (&v)[16]) {
-            const X* from = x + r * x_row + at(p);
-            if (vec && at(p) + 16 <= a.in) {
-                constexpr int N = 16 / sizeof(X);
-#pragma unroll
-                for (int i = 0; i < 16; i += N) unpack16<X>(__ldg(reinterpret_cast<const uint4*>(from + i)), v + i);
+        const int pad = (a.in + 15) & ~15;
+        auto values = [&](int r, int i, float (&v)[NORM_E]) {
+            const X* row = x + r * x_row;
+            if (vec && i + NORM_E <= a.in) {
+                load8(row + i, v);
             } else {
 #pragma unroll
-                for (int i = 0; i < 16; i++) v[i] = at(p) + i < a.in ? Dense<X>::get(from[i]) : 0.f;
+                for (int j = 0; j < NORM_E; j++) v[j] = i + j < a.in ? Dense<X>::get(row[i + j]) : 0.f;
             }
         };
-        float keep[ROWS * PIECES == 1 ? 16 : 1];
+        uint32_t top[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; r++) top[r] = 0;
+        for (int i = tid * NORM_E; i < a.in; i += W8R_THREADS * NORM_E)
+#pragma unroll
+            for (int r = 0; r < ROWS; r++)
+                if (r < a.rows) {
+                    float v[NORM_E];
+                    values(r, i, v);
+#pragma unroll
+                    for (int j = 0; j < NORM_E; j++) top[r] = max(top[r], __float_as_uint(v[j]) & 0x7fffffffu);
+                }
 #pragma unroll
         for (int r = 0; r < ROWS; r++) {
-            uint32_t top = 0;
-            if (r < a.rows) {
-#pragma unroll
-                for (int p = 0; p < PIECES; p++) {
-                    float v[16];
-                    values(r, p, v);
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-                        if constexpr (ROWS * PIECES == 1) keep[i] = v[i];
-                    }
-                }
-            }
-            top = __reduce_max_sync(0xffffffffu, top);
-            if (lane == 0) s_top[r][warp] = top;
+            top[r] = __reduce_max_sync(0xffffffffu, top[r]);
+            if (lane == 0) s_top[r][warp] = top[r];
         }
         __syncthreads();
+        float inv[ROWS];
 #pragma unroll
-        for (int r = 0; r < ROWS; r++) {
-            float inv;
-            nrm::code_scale(__reduce_max_sync(0xffffffffu, s_top[r][lane % W8R_WARPS]), inv, x_scale[r]);
+        for (int r = 0; r < ROWS; r++) nrm::code_scale(__reduce_max_sync(0xffffffffu, s_top[r][lane % W8R_WARPS]), inv[r], x_scale[r]);
+        for (int i = tid * NORM_E; i < pad; i += W8R_THREADS * NORM_E)
 #pragma unroll
-            for (int p = 0; p < PIECES; p++) {
-                float v[16];
-                if constexpr (ROWS * PIECES == 1) {
+            for (int r = 0; r < ROWS; r++)
+                if (r < a.rows) {
+                    float v[NORM_E];
+                    values(r, i, v);
+                    uint32_t c[2] = {0, 0};
 #pragma unroll
-                    for (int i = 0; i < 16; i++) v[i] = keep[i];
-                } else if (r < a.rows) {
-                    values(r, p, v);
+                    for (int j = 0; j < NORM_E; j++) c[j / 4] |= nrm::code(v[j], inv[r]) << (8 * (j & 3));
+                    *reinterpret_cast<uint2*>(s_code + r * pad + i) = make_uint2(c[0], c[1]);
                 }
+        __syncthreads();
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    code[r][p][j] = 0;
-                    if (r < a.rows)
+        for (int r = 0; r < ROWS; r++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) code[r][p][j] |= nrm::code(v[4 * j + i], inv) << (8 * i);
-                }
-            }
-        }
+            for (int p = 0; p < PIECES; p++)
+                code[r][p] = r < a.rows && at(p) < a.in ? *reinterpret_cast<const int4*>(s_code + r * pad + at(p)) : make_int4(0, 0, 0, 0);
     }
-    for (int o = o0 + slot; o < o1; o += AHEAD * slots) {
-        int4 now[AHEAD][PIECES];
-#pragma unroll
-        for (int u = 0; u < AHEAD; u++)
-#pragma unroll
-            for (int p = 0; p < PIECES; p++) now[u][p] = next[u][p];
-        load(o + AHEAD * slots);
+    for (int o = o0 + slot; o < o1; o += AHEAD * slots, from += AHEAD * step) {
 #pragma unroll
         for (int u = 0; u < AHEAD; u++) {
             if (o + u * slots >= o1) break;
+            int4 now[PIECES];
+#pragma unroll
+            for (int p = 0; p < PIECES; p++) {
+                now[p] = held[u][p];
+                const int next = o + (u + AHEAD) * slots;
+                if (next < o1) held[u][p] = weights(next, from + (u + AHEAD) * step, p);
+            }
 #pragma unroll
             for (int r = 0; r < ROWS; r++) {
                 int sum = 0;
 #pragma unroll
                 for (int p = 0; p < PIECES; p++) {
-                    sum = __dp4a(now[u][p].x, code[r][p][0], sum);
-                    sum = __dp4a(now[u][p].y, code[r][p][1], sum);
-                    sum = __dp4a(now[u][p].z, code[r][p][2], sum);
-                    sum = __dp4a(now[u][p].w, code[r][p][3], sum);
+                    sum = __dp4a(now[p].x, code[r][p].x, sum);
+                    sum = __dp4a(now[p].y, code[r][p].y, sum);
+                    sum = __dp4a(now[p].z, code[r][p].z, sum);
+                    sum = __dp4a(now[p].w, code[r][p].w, sum);
                 }
                 sum = __reduce_add_sync(0xffffffffu, sum);
                 if (lane == 0) atomicAdd(&s_sum[(o + u * slots - o0) * ROWS + r], sum);
             }
         }
+    }
+    if (o1 == a.out && warp < ROWS && warp < a.rows && lane < (a.in & 15)) {  // the last row's last piece
+        const int i = (a.in & ~15) + lane;
+        const int x_code = CODES ? ((const signed char*)x)[warp * x_row + i] : s_code[warp * ((a.in + 15) & ~15) + i];
+        atomicAdd(&s_sum[(o1 - 1 - o0) * ROWS + warp], x_code * w[(o1 - 1) * w_row + i]);
     }
     __syncthreads();
     T* y = static_cast<T*>(a.y);
