@@ -259,8 +259,11 @@ int64_t row_stride(int64_t rows, int64_t stride, int64_t inner) { return rows > 
 template <class T, int BN>
 void launch_few(const CUtensorMap& mw, const CUtensorMap& mx, const W8Args& a, void* stream) {
     const int tiles = (a.out + 127) / 128, across = (a.rows + BN - 1) / BN, blocks = (a.in + W8_K - 1) / W8_K;
+    // CTAs to a tile: of two blocks of inputs at least, up to one on each SM, two where
+    // they have 16 blocks each (us with up to 148 and up to 296 CTAs of any length: 61 x
+    // 1024 x 4096 6.3 and 8.8, 61 x 4096 x 4096 8.2 and 10.1, 16 x 8192 x 8192 17.0 and 16.0)
     int ranks = 1;
-    while (ranks < 8 && (int64_t)tiles * across * ranks * 2 <= 2 * 148 && ranks * 2 <= blocks) ranks *= 2;
+    while (ranks < 8 && ranks * 4 <= blocks && (int64_t)tiles * across * ranks * 2 <= (blocks >= ranks * 32 ? 2 : 1) * 148) ranks *= 2;
     launch_cluster(k_w8_few<T, BN>, dim3(tiles * ranks, across), W8_THREADS, W8Few<BN>::SMEM, ranks, true, stream, mw, mx, a, ranks);
 }
 
@@ -369,10 +372,10 @@ int32_t fb2_w8_matmul(const fb2_w8_linear* w, int32_t n_rows, const void* codes,
             else if (n_rows <= 128)
                 launch_few<T, 128>(w_map(128), x_map(128), a, stream);
             else {
-                const int64_t tiles = (int64_t)((a.rows + 127) / 128) * ((a.out + W8M_N - 1) / W8M_N);
+                const int64_t tiles = (int64_t)((a.rows + 255) / 256) * ((a.out + W8M_N - 1) / W8M_N);
                 need(tiles <= INT32_MAX - 65536, "too many rows for one call");
-                launch_cluster(k_w8_many<T>, dim3((unsigned)std::min<int64_t>(tiles, 148)), W8_THREADS, W8M_SMEM, 1, true, stream,
-                               w_map(W8M_N), x_map(128), a);
+                launch_cluster(k_w8_many<T>, dim3((unsigned)std::min<int64_t>(2 * tiles, 148)), W8_THREADS, W8M_SMEM, 2, true, stream,
+                               w_map(128), x_map(128), a);
             }
         });
         launched();

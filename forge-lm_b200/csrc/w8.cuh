@@ -12,7 +12,7 @@
 // k_w8_few: up to 128 rows of x to a tile, as the N side of the tiles, the weights
 // as the M side: each weight is read once.  A cluster shares a tile's inputs where
 // there are fewer tiles than SMs.
-// k_w8_many: 128 rows of x by 256 outputs, one CTA on each SM.
+// k_w8_many: 256 rows of x by 256 outputs, a pair of CTAs to a tile.
 // Every wait is bounded (2 s); on expiry a CTA stops, waits (bounded) for its
 // copies and MMAs in flight, frees its tensor memory, and its rows of y are NaN.
 #pragma once
@@ -59,7 +59,6 @@ FB2_DEV void ld16(uint32_t at, int (&v)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 FB2_DEV void prefetch(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory"); }
-FB2_DEV void arrive(uint64_t* b) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_addr(b)) : "memory"); }
 FB2_DEV int peek(uint32_t at, int rank) {
     uint32_t r;
     int v;
@@ -407,31 +406,69 @@ __global__ void __launch_bounds__(W8R_THREADS, w8r_resident<X, ROWS, PIECES>)
 }
 
 // ---- many rows -------------------------------------------------------------------------
-constexpr int W8M_N = 256, W8M_STAGE = W8_TILE + W8M_N * W8_K, W8M_STAGES = 4;
+// A pair of CTAs (on the two SMs of a TPC) takes a tile of 256 rows of x by 256 outputs:
+// one MMA of both, whose A and B tiles lie half in each one's shared memory, so that a
+// stage brings 32 KB to an SM for the products that cost one SM by itself 48 KB; what
+// crosses from L2 bounds these tiles.
+constexpr int W8M_N = 256, W8M_STAGE = 2 * W8_TILE, W8M_STAGES = 6;
 constexpr int W8M_SMEM = W8M_STAGES * W8M_STAGE + 1024;
-constexpr int W8M_GROUP = 16;  // tiles of rows that are walked together: what runs at a time shares operands in L2
+constexpr int W8M_GROUP = 8;  // tiles of rows that are walked together: what runs at a time shares operands in L2
 
-// One CTA on each SM walks the tiles.  Warp 0 copies, warp 1 issues the MMAs into
-// one of two accumulators, warps 2..5 bring the other one out: lane r of quarter q
-// is row 32 q + r of the tile, its columns are outputs.
+namespace w8 {
+FB2_DEV uint32_t at_leader(const void* p) {  // the same place in the pair's first CTA
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(tc::smem_addr(p)));
+    return r;
+}
+// A box into this CTA's memory, counted at the barrier `bar` of the pair's first CTA.
+FB2_DEV void load_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            tc::smem_addr(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+FB2_DEV void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+    asm volatile(
+        "{ .reg .pred p; setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p; }" ::"r"(d),
+        "l"(a), "l"(b), "r"(id), "r"(accumulate), "r"(0u)
+        : "memory");
+}
+// Arrives at the barrier at this place in both CTAs once the MMAs before are done.
+FB2_DEV void commit_pair(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(tc::smem_addr(bar)),
+                 "h"((uint16_t)3)
+                 : "memory");
+}
+FB2_DEV void arrive_at(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+}  // namespace w8
+
+// Pairs of CTAs walk the tiles.  Warp 0 of each copies its halves, warp 1 of the first
+// issues the MMAs into one of two accumulators, warps 2..5 of each bring its rows of the
+// other one out: lane r of quarter q is row 32 q + r, its columns are outputs.
 template <class T>
 __global__ void __launch_bounds__(W8_THREADS, 1)
     k_w8_many(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, W8Args a) {
     extern __shared__ unsigned char w8_raw[];
+    // full and taken: the first CTA's count for both
     __shared__ __align__(8) uint64_t full[W8M_STAGES], empty[W8M_STAGES], ready[2], taken[2], drain;
     __shared__ uint32_t tmem_base;
     __shared__ volatile int s_abort;
     __shared__ __align__(16) float s_scale[2][W8M_N], s_bias[2][W8M_N];
     unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(w8_raw) + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int tiles_r = (a.rows + 127) / 128, tiles_o = (a.out + W8M_N - 1) / W8M_N;
+    const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int tiles_r = (a.rows + 255) / 256, tiles_o = (a.out + W8M_N - 1) / W8M_N;
     const int tiles = tiles_r * tiles_o;
     const int nk = (a.in + W8_K - 1) / W8_K;
-    // groups of W8M_GROUP tiles of rows, through all outputs
+    // groups of W8M_GROUP tiles of rows, through all outputs; r0: this CTA's rows
     auto place = [&](int t, int& r0, int& o0) {
         const int group = t / (W8M_GROUP * tiles_o), within = t - group * W8M_GROUP * tiles_o;
         const int high = min(W8M_GROUP, tiles_r - group * W8M_GROUP);
-        r0 = (group * W8M_GROUP + within % high) * 128;
+        r0 = (group * W8M_GROUP + within % high) * 256 + 128 * rank;
         o0 = within / high * W8M_N;
     };
     if (tid == 0) {
@@ -443,18 +480,19 @@ __global__ void __launch_bounds__(W8_THREADS, 1)
         }
         for (int i = 0; i < 2; i++) {
             tc::bar_init(&ready[i], 1);
-            tc::bar_init(&taken[i], 4);
+            tc::bar_init(&taken[i], 8);
         }
         tc::bar_init(&drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_addr(&tmem_base)), "r"(512u)
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_addr(&tmem_base)), "r"(512u)
                      : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     tc::fence_before();
     __syncthreads();
+    pg::cluster_sync();  // both have their barriers and tensor memory
     tc::fence_after();
     const uint32_t tmem = tmem_base;
     pdl_wait();
@@ -462,7 +500,7 @@ __global__ void __launch_bounds__(W8_THREADS, 1)
     if (warp == 0 && lane == 0) {
         uint32_t it = 0;
         bool stop = false;
-        for (int t = blockIdx.x; t < tiles && !stop; t += gridDim.x) {
+        for (int t = pair; t < tiles && !stop; t += pairs) {
             int r0, o0;
             place(t, r0, o0);
             for (int i = 0; i < nk; i++, it++) {
@@ -472,26 +510,27 @@ __global__ void __launch_bounds__(W8_THREADS, 1)
                     break;
                 }
                 unsigned char* at = sm + st * W8M_STAGE;
-                tc::bar_expect_tx(&full[st], W8M_STAGE);
-                tc::tma_load_2d(at, &map_x, i * W8_K, r0, &full[st]);
+                const uint32_t bar = w8::at_leader(&full[st]);
+                if (rank == 0) tc::bar_expect_tx(&full[st], 2 * W8M_STAGE);
+                w8::load_pair(at, &map_x, i * W8_K, r0, bar);
                 if (blockIdx.x == 0 && (int)it == a.withhold) {
                     stop = true;
                     break;
                 }
-                tc::tma_load_2d(at + W8_TILE, &map_w, i * W8_K, o0, &full[st]);
+                w8::load_pair(at + W8_TILE, &map_w, i * W8_K, o0 + 128 * rank, bar);
             }
         }
-        // copies still landing (after an abort): each stage's latest fill
-        if (s_abort || stop) {
+        // after an abort, copies of both may still be landing, which the first CTA sees
+        if (rank == 0 && (s_abort || stop)) {
             const unsigned long long t0 = tc::now_ns();
-            for (uint32_t j = it > W8M_STAGES ? it - W8M_STAGES : 0; j < it; j++)
-                while (!tc::bar_try(&full[j % W8M_STAGES], (j / W8M_STAGES) & 1) && tc::now_ns() - t0 < kTcTimeoutNs) {
+            for (uint32_t j = it > W8M_STAGES ? it - W8M_STAGES : 0; j <= it; j++)
+                while (!tc::bar_try(&full[j % W8M_STAGES], (j / W8M_STAGES) & 1) && tc::now_ns() - t0 < a.wait_ns) {
                 }
         }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1 && lane == 0 && rank == 0) {
         uint32_t it = 0, local = 0;
         bool stop = false;
-        for (int t = blockIdx.x; t < tiles && !stop; t += gridDim.x, local++) {
+        for (int t = pair; t < tiles && !stop; t += pairs, local++) {
             const uint32_t acc = local & 1;
             if (local >= 2 && !tc::bar_wait(&taken[acc], (local / 2 - 1) & 1, &s_abort, a.wait_ns)) break;
             tc::fence_after();
@@ -506,13 +545,13 @@ __global__ void __launch_bounds__(W8_THREADS, 1)
                 const uint64_t x = tc::sw128_desc(at, 16, 1024), w = tc::sw128_desc(at + W8_TILE, 16, 1024);
 #pragma unroll
                 for (int k = 0; k < W8_K / 32; k++)
-                    w8::mma(tmem + acc * W8M_N, x + 2 * k, w + 2 * k, w8::idesc(128, W8M_N), (i | k) != 0);
-                tc::mma_commit(&empty[st]);
+                    w8::mma_pair(tmem + acc * W8M_N, x + 2 * k, w + 2 * k, w8::idesc(256, W8M_N), (i | k) != 0);
+                w8::commit_pair(&empty[st]);
             }
-            if (!stop) tc::mma_commit(&ready[acc]);
+            if (!stop) w8::commit_pair(&ready[acc]);
         }
         // every MMA issued completes before the accumulators are freed
-        tc::mma_commit(&drain);
+        w8::commit_pair(&drain);
         const unsigned long long t0 = tc::now_ns();
         while (!tc::bar_try(&drain, 0) && tc::now_ns() - t0 < kTcTimeoutNs) {
         }
@@ -522,7 +561,7 @@ __global__ void __launch_bounds__(W8_THREADS, 1)
         T* y = static_cast<T*>(a.y);
         uint32_t local = 0;
         bool failed = false;  // from the first tile that never came on: the rest is NaN
-        for (int t = blockIdx.x; t < tiles; t += gridDim.x, local++) {
+        for (int t = pair; t < tiles; t += pairs, local++) {
             const uint32_t acc = local & 1;
             int r0, o0;
             place(t, r0, o0);
@@ -569,15 +608,16 @@ __global__ void __launch_bounds__(W8_THREADS, 1)
             }
             tc::fence_before();
             __syncwarp();
-            if (lane == 0) w8::arrive(&taken[acc]);
+            if (lane == 0) w8::arrive_at(w8::at_leader(&taken[acc]));
         }
     }
     __syncwarp();
     tc::fence_before();
     __syncthreads();
+    pg::cluster_sync();  // neither ends or frees while the other's MMAs or copies go on
     if (warp == 0) {
         tc::fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
 }
 
