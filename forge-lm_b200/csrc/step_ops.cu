@@ -22,7 +22,8 @@ using namespace fb2;
 
 namespace {
 
-// A launch of clusters of `cluster` CTAs along x; `early`: it may begin before
+// A launch of clusters of `cluster` CTAs along x (`smem`: the same for every launch of a
+// kernel, or opted in for its most before); `early`: it may begin before
 // the launch before it has ended (the kernel waits in pdl_wait).
 template <class... P, class... A>
 void launch_cluster(void (*kernel)(P...), dim3 grid, int threads, int smem, int cluster, bool early, void* stream, A... args) {
@@ -79,6 +80,7 @@ int32_t fb2_pages_extend(const fb2_pages* p, const int32_t* counts, int32_t max_
              "a tensor is not aligned to its element size");
         const bool vec = aligned(slots, 16) && aligned(positions, 16);
         auto launch = [&](auto kernel, int threads, int ranks) {
+            opt_in_smem((const void*)kernel, 12 * PG_SEQS);
             launch_cluster(kernel, dim3(ranks), threads, 12 * v.n_seqs, ranks, false, stream, v, counts, max_rows, starts, prefix_lens, slots,
                            positions, vec);
         };
@@ -97,10 +99,14 @@ int32_t fb2_pages_truncate(const fb2_pages* p, const int32_t* lens, void* stream
         if (v.n_seqs == 0) return;
         need(lens, "NULL argument");
         need(aligned(lens, 4), "a tensor is not aligned to its element size");
+        auto launch = [&](auto kernel, int threads) {
+            opt_in_smem((const void*)kernel, 8 * PG_SEQS);
+            launch_cluster(kernel, dim3(1), threads, 8 * v.n_seqs, 1, false, stream, v, lens);
+        };
         if (v.n_seqs <= 256)
-            launch_cluster(k_pages_truncate<256>, dim3(1), 256, 8 * v.n_seqs, 1, false, stream, v, lens);
+            launch(k_pages_truncate<256>, 256);
         else
-            launch_cluster(k_pages_truncate<1024>, dim3(1), 1024, 8 * v.n_seqs, 1, false, stream, v, lens);
+            launch(k_pages_truncate<1024>, 1024);
     });
 }
 
@@ -307,6 +313,13 @@ void launch_rows(const fb2_w8_linear* w, const W8Args& a, const X* x, int64_t x_
         p.pieces == 1 ? go(one, one) : p.pieces == 2 ? go(one, two) : go(one, four);
 }
 
+// More than 128 rows: whether tiles of 128 x 128 whose inputs a cluster shares take less
+// than 256 x 256 by pairs of CTAs that leave most SMs without one (us, shared and not:
+// 256 x 1024 x 4096, 16 of the larger tiles, 9.6 and 9.5; 256 x 4096 x 4096, 16, 13.5 and
+// 17.4; 512 x 4096 x 4096, 32, 17.0 and 18.1; 512 x 1024 x 4096, 32, 13.6 and 9.7; 256 x 4096 x
+// 14336, 56, 26.9 and 20.6).
+bool w8_splits(int64_t tiles, int in) { return in >= 32 * W8_K ? tiles <= 37 : in >= 8 * W8_K && tiles <= 18; }
+
 std::atomic<int> g_withhold_block{-1};
 std::atomic<int64_t> g_withhold_wait_ns{0};
 }  // namespace
@@ -357,6 +370,7 @@ int32_t fb2_w8_matmul(const fb2_w8_linear* w, int32_t n_rows, const void* codes,
         W8Args a{scales, w->device_scales, w->device_bias, y, y_row, n_rows, w->in_features, w->out_features,
                  aligned(y, 16) && (n_rows == 1 || y_row * es % 16 == 0), g_withhold_block.exchange(-1), kTcTimeoutNs};
         if (a.withhold >= 0) a.wait_ns = (unsigned long long)g_withhold_wait_ns.load();
+        const int64_t tiles = (int64_t)((a.rows + 255) / 256) * ((a.out + W8M_N - 1) / W8M_N);  // of the largest kind
         auto x_map = [&](int box) { return byte_map(codes, a.in, a.rows, row_stride(a.rows, code_row, a.in), box); };
         auto w_map = [&](int box) { return byte_map(w->device_codes, a.in, a.out, row_stride(a.out, w->code_row_stride, a.in), box); };
         with_type(dtype, [&](auto t) {
@@ -369,10 +383,9 @@ int32_t fb2_w8_matmul(const fb2_w8_linear* w, int32_t n_rows, const void* codes,
                 launch_few<T, 32>(w_map(128), x_map(32), a, stream);
             else if (n_rows <= 64)
                 launch_few<T, 64>(w_map(128), x_map(64), a, stream);
-            else if (n_rows <= 128)
+            else if (n_rows <= 128 || w8_splits(tiles, a.in))
                 launch_few<T, 128>(w_map(128), x_map(128), a, stream);
             else {
-                const int64_t tiles = (int64_t)((a.rows + 255) / 256) * ((a.out + W8M_N - 1) / W8M_N);
                 need(tiles <= INT32_MAX - 65536, "too many rows for one call");
                 launch_cluster(k_w8_many<T>, dim3((unsigned)std::min<int64_t>(2 * tiles, 148)), W8_THREADS, W8M_SMEM, 2, true, stream,
                                w_map(128), x_map(128), a);

@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(W8_THREADS, 2)
 // pieces in flight.  `per_k` warps share an output's inputs; the sums meet in shared
 // memory as integers.  The weights' bytes bound it.
 constexpr int W8R_THREADS = 512, W8R_WARPS = W8R_THREADS / 32, W8R_AHEAD = 8;
-constexpr int W8R_SUMS = 4096;       // sums of a CTA: outputs times rows
+constexpr int W8R_SUMS = 3200;       // sums of a CTA: outputs times rows (with the codes below 48 KB)
 constexpr int W8R_CODES = 32 * 1024;  // bytes of x's codes: what a lane's registers take of them
 template <class X, int ROWS, int PIECES>
 constexpr int w8r_resident = sizeof(X) > 1 && ROWS * PIECES == 1 ? 2 : 1;  // CTAs of an SM, by registers

@@ -669,3 +669,478 @@ def test_accepted_tokens_are_distributed_as_the_target(pkg, drawn):
     tokens, _, _ = pkg.verify_drafts(logits, drafts, uniforms, starts=starts, draft_probs=probs, max_nodes=2)
     counts = torch.bincount(tokens[:, 0].long(), minlength=vocab).double()
     assert ((counts - n * p).abs() <= 6 * torch.sqrt(n * p * (1 - p))).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("heat", [0.0, 0.8])
+def test_verification_under_masks_of_the_lowest_value(pkg, dtype, heat):
+    """Masked by the type's lowest value, in part and in whole (then all are alike)."""
+    g, rng = gen(3), random.Random(3)
+    logits, drafts, uniforms, starts, parents, _ = verify_case(g, rng, [5, 9, 2], 3001, DTYPES[dtype], True)
+    low = torch.finfo(DTYPES[dtype]).min
+    logits[torch.rand(logits.shape, device="cuda", generator=g) < 0.6] = low
+    check_verify(pkg, logits, drafts, uniforms, starts, parents, heat=[heat] * 3)
+    logits[starts[1]:] = low
+    logits[starts[2], :7] = -math.inf
+    check_verify(pkg, logits, drafts, uniforms, starts, parents, heat=[heat] * 3)
+
+
+@gpu
+def test_verification_decides_close_tests_in_64_bits(pkg):
+    """Uniforms a part in 10^12 to either side of a draft's probability: sums from 32-bit
+    exponentials cannot tell them apart."""
+    g = gen(21)
+    vocab, n = 5000, 12
+    logits = normal(g, 2 * n, vocab)
+    drafts = torch.randint(0, vocab, (2 * n,), device="cuda", generator=g).to(torch.int32)
+    uniforms = torch.rand(2 * n, device="cuda", generator=g, dtype=torch.float64)
+    starts, heat = list(range(0, 2 * n + 1, 2)), [0.5 + 0.1 * i for i in range(n)]
+    p = torch.stack([torch.softmax(logits[2 * i].double() / float(torch.tensor(heat[i])), 0) for i in range(n)])
+    at = p[torch.arange(n), drafts[1::2].long()]
+    probs = torch.softmax(normal(g, 2 * n, vocab), 1)
+    q = probs[torch.arange(1, 2 * n, 2), drafts[1::2].long()].double()
+    for side, count in ((1 - 1e-12, 2), (1 + 1e-12, 1)):
+        uniforms[1::2] = at * side
+        _, _, counts = check_verify(pkg, logits, drafts, uniforms, starts, heat=heat)
+        assert counts.eq(count).all()
+        uniforms[1::2] = at / q * side  # (past 1 for some: as good a number to compare)
+        _, _, counts = check_verify(pkg, logits, drafts, uniforms, starts, heat=heat, probs=probs)
+        assert counts.eq(count).all()
+    # siblings: the second is held against what the first has left, and a chain goes on behind a close test
+    wide = logits[:1].expand(4, vocab).contiguous()
+    p = torch.softmax(wide[0].double(), 0)
+    a, b = int(p.argmax()), int(p.argmin())
+    for side, want in ((1 - 1e-12, 2), (1 + 1e-12, 1)):
+        u = torch.tensor([0.5, float(p[a]) * (1 + 1e-12), float(p[b] / (1 - p[a])) * side, 0.0], dtype=torch.float64, device="cuda")
+        _, _, counts = check_verify(pkg, wide, ints([0, a, b, 7]), u, [0, 4], parents=[0, 0, 0, 1])
+        assert counts.tolist() == [want]
+
+
+@gpu
+def test_verification_of_many_rows_and_far_ones(pkg):
+    """More rows than 16 bits count, and logits and probabilities past 2^32 bytes."""
+    g = gen(2)
+    n, vocab = 70000, 64
+    logits = normal(g, n, vocab, dtype=torch.bfloat16)
+    uniforms = torch.rand(n, device="cuda", generator=g, dtype=torch.float64)
+    starts = torch.arange(0, n + 1, 2, dtype=torch.int32, device="cuda")
+    drafts = torch.randint(0, vocab, (n,), device="cuda", generator=g).to(torch.int32)
+    tokens, nodes, counts = pkg.verify_drafts(logits, drafts, uniforms, starts=starts, max_nodes=2)
+    want = plain_verify(logits[-200:], drafts[-200:].tolist(), uniforms[-200:], list(range(0, 201, 2)), wide=2)
+    assert tokens[-100:].tolist() == want[0] and counts[-100:].tolist() == want[2]
+    rows, vocab = 3, 1 << 20
+    flat = torch.zeros(rows * 1200000000 // 2, dtype=torch.bfloat16, device="cuda")  # 3.6 GB
+    far = flat.as_strided((rows, vocab), (600000000, 1))
+    far.copy_(normal(g, rows, vocab))
+    q = torch.zeros(2 * 1200000000 // 2 + vocab, device="cuda").as_strided((rows, vocab), (600000000, 1))  # 4.8 GB
+    q.copy_(torch.softmax(normal(g, rows, vocab), 1))
+    drafts = torch.multinomial(q, 1, generator=g).squeeze(1).to(torch.int32)
+    uniforms = torch.rand(rows, device="cuda", generator=g, dtype=torch.float64)
+    check_verify(pkg, far, drafts, uniforms, [0, 3], probs=q)
+
+
+@gpu
+@pytest.mark.parametrize("rows,k", [(1, 32768), (1, 20000), (2, 16384), (2, 9000), (3, 8192), (4, 8192), (4, 8191), (3, 10000), (1, 32769)])
+def test_products_at_the_ends_of_few_rows(pkg, rows, k):
+    """The sizes at which lanes hold their last piece of inputs, and those past them."""
+    g = gen(k)
+    for n in (5, 1203):
+        linear = w8_case(pkg, g, k, n)
+        x = normal(g, rows, k, dtype=torch.bfloat16)
+        codes, scales = plain_codes(x)
+        check_w8(linear, codes, scales, linear(x))
+        check_w8(linear, codes, scales, linear(codes.to(torch.int8).cuda(), scales=scales.cuda()))
+
+
+@gpu
+def test_products_read_nothing_behind_the_last_row(pkg):
+    """Buffers that end with the last row's last code: what is behind is another tensor's NaN, and stays."""
+    g = gen(5)
+    for k, n, rows in ((77, 9, 2), (100, 40, 6), (1000, 130, 40), (300, 257, 200)):
+        row = -(-k // 16) * 16
+        flat = torch.randint(-127, 128, ((n - 1) * row + k,), device="cuda", generator=g).to(torch.int8)
+        linear = pkg.W8Linear(flat.as_strided((n, k), (row, 1)), torch.rand(n, device="cuda", generator=g) + 0.1)
+        x = torch.randint(-127, 128, ((rows - 1) * row + k,), device="cuda", generator=g).to(torch.int8).as_strided((rows, k), (row, 1))
+        scales = torch.rand(rows, device="cuda", generator=g)
+        check_w8(linear, x, scales, linear(x, scales=scales))
+
+
+@gpu
+def test_product_past_32_bit_offsets(pkg):
+    g = gen(6)
+    k, n = 48, 100_000_000  # 4.8 GB of codes
+    codes = torch.zeros((n, k), dtype=torch.int8, device="cuda")
+    codes[-1000:] = torch.randint(-127, 128, (1000, k), device="cuda", generator=g).to(torch.int8)
+    scales = torch.ones(n, device="cuda")
+    linear = pkg.W8Linear(codes, scales)
+    for rows in (1, 5, 130):
+        x = torch.randint(-127, 128, (rows, k), device="cuda", generator=g).to(torch.int8)
+        y = linear(x, scales=torch.ones(rows, device="cuda"), dtype=torch.bfloat16)
+        want = x.double() @ codes[-1000:].double().T
+        assert torch.equal(y[:, -1000:], want.to(torch.bfloat16)) and y[:, :-1000:4099].eq(0).all()
+
+
+@gpu
+def test_norm_of_rows_past_32_bit_offsets(pkg):
+    g = gen(7)
+    rows, dim = 600_000, 4096  # 4.9 GB of h
+    h = torch.zeros((rows, dim), dtype=torch.bfloat16, device="cuda")
+    h[-50:] = normal(g, 50, dim)
+    x = torch.zeros(1, dim, device="cuda").expand(rows, dim)  # one row for all
+    w = 1 + 0.1 * normal(g, dim)
+    s, codes, scales = pkg.residual_norm(h, x, w, quantise=True, kind="rms")
+    few = pkg.residual_norm(h[-50:], x[-50:], w, quantise=True, kind="rms")
+    assert torch.equal(s[-50:], few[0]) and torch.equal(scales[:-50], torch.zeros_like(scales[:-50]))
+    # (other threads hold a row's parts where rows are few: sums differ in their last bits)
+    assert (codes[-50:].int() - few[1].int()).abs().max() <= 1 and torch.allclose(scales[-50:], few[2], rtol=1e-5, atol=0)
+
+
+# ---- calls as a program makes them -----------------------------------------------------------
+
+@gpu
+def test_operators_on_another_stream(pkg):
+    g = gen(12)
+    x, w = normal(g, 40, 512, dtype=torch.bfloat16), normal(g, 512, 300)
+    linear, weight = pkg.W8Linear.pack(w), torch.ones(512, device="cuda")
+    logits, uniforms = normal(g, 6, 9000), torch.rand(6, device="cuda", generator=g, dtype=torch.float64)
+    drafts, starts = ints([1, 2, 3, 4, 5, 6]), ints([0, 3, 6])
+
+    def calls(x, logits):
+        s, codes, scales = pkg.residual_norm(x, x, weight, quantise=True)
+        return s, linear(codes, scales=scales), linear(x[:2]), *pkg.verify_drafts(logits, drafts, uniforms, starts=starts)
+
+    want = calls(x, logits)
+    side = torch.cuda.Stream()
+    busy = torch.zeros(1 << 28, device="cuda")
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(4):
+            busy.add_(1.0)
+        a, b = x * busy[0] / 4, logits * busy[0] / 4  # made behind the stream's long work
+        got = calls(a, b)
+    side.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(want, got))
+
+
+class Step:
+    """One layer of a decoder that drafts and verifies, on the operators."""
+
+    def __init__(self, pkg, g, seqs, dim, heads, vocab, drafts, page):
+        self.pkg, self.heads, self.dim, self.vocab, self.most = pkg, heads, dim, vocab, seqs * (drafts + 1)
+        self.pages = pkg.PageTable.empty(seqs, 6, seqs * 5, page)
+        self.cache = pkg.QuantKvCache.empty(seqs * 5, page, heads, dim // heads, "int8")
+        self.emb = normal(g, vocab, dim, dtype=torch.bfloat16)
+        self.qkv, self.out, self.head = (pkg.W8Linear.pack(normal(g, dim, n) / dim ** 0.5) for n in (3 * dim, dim, vocab))
+        self.w, self.b = 1 + 0.1 * normal(g, dim), 0.1 * normal(g, dim)
+
+    def run(self, tokens, counts, uniforms):
+        """tokens [most] of the served rows in order; returns everything that the step makes."""
+        pkg, n = self.pkg, self.most
+        starts, prefix, slots, positions = self.pages.extend(counts, n)
+        x = self.emb[tokens.long()] + 0.01 * positions[:, None]
+        _, codes, scales = pkg.residual_norm(None, x, self.w, self.b, quantise=True)
+        qkv = self.qkv(codes, scales=scales, dtype=torch.bfloat16).view(n, 3, self.heads, -1)
+        self.cache.write(qkv[:, 1], qkv[:, 2], slots)
+        a, _ = self.cache.attend(qkv[:, 0], self.pages.table, prefix, starts=starts, max_nodes=8)
+        x, h = pkg.residual_norm(self.out(a.reshape(n, -1)), x, self.w, self.b)
+        logits = pkg.logit_controls(self.head(h))
+        kept, nodes, gained = pkg.verify_drafts(logits, tokens, uniforms, starts=starts, max_nodes=8)
+        self.pages.truncate(prefix + gained)
+        return starts, prefix, slots, positions, logits, kept, nodes, gained, self.pages.lens.clone(), self.pages.table.clone()
+
+
+@gpu
+def test_a_step_of_all_operators(pkg):
+    """A sequence of steps: pages and verification as their rules say of what the step made, and the
+    logits as a plain computation of the same layer over everything kept so far."""
+    g = gen(31)
+    seqs, dim, heads, vocab, page = 5, 128, 4, 500, 8
+    step = Step(pkg, g, seqs, dim, heads, vocab, 5, page)
+    want = Pages(seqs, 6, seqs * 5, page)
+    text = [[] for _ in range(seqs)]  # tokens in the cache
+    rng = random.Random(4)
+    last = [rng.randrange(vocab) for _ in range(seqs)]
+    scale = [l.scales.double() for l in (step.qkv, step.out, step.head)]
+    dense = [(l.codes.double() * s[:, None]).T for l, s in zip((step.qkv, step.out, step.head), scale)]
+    for turn in range(5):
+        news = [[last[b]] + [rng.randrange(vocab) for _ in range(rng.randint(0, 5))] for b in range(seqs)]
+        counts = [len(t) for t in news]
+        tokens = [t for n in news for t in n]
+        uniforms = torch.rand(step.most, device="cuda", generator=g, dtype=torch.float64)
+        made = step.run(ints(tokens + [0] * (step.most - len(tokens))), ints(counts), uniforms)
+        starts, prefix, slots, positions, logits, kept, nodes, gained = made[:8]
+        assert [t.tolist() for t in made[:4]] == list(want.extend(counts, step.most))
+        plain = plain_verify(logits, tokens, uniforms, starts.tolist(), wide=8)
+        assert (kept.tolist(), nodes.tolist(), gained.tolist()) == plain
+        want.truncate([n + c for n, c in zip(prefix.tolist(), plain[2])])
+        assert want.same(step.pages)
+        for b in range(seqs):
+            ids = torch.tensor(text[b] + news[b], device="cuda")
+            x = step.emb[ids].double() + 0.01 * torch.arange(len(ids), device="cuda")[:, None]
+            qkv = (plain_norm(x, step.w, step.b, "layer", 1e-5) @ dense[0]).view(-1, 3, heads, dim // heads)
+            s = torch.einsum("qhd,khd->hqk", qkv[:, 0], qkv[:, 1]) / math.sqrt(dim // heads)
+            s = s.masked_fill(~torch.ones(len(ids), len(ids), device="cuda").tril().bool(), -math.inf)
+            a = torch.einsum("hqk,khd->qhd", torch.softmax(s, 2), qkv[:, 2]).flatten(1)
+            ref = plain_norm(x + a @ dense[1], step.w, step.b, "layer", 1e-5) @ dense[2]
+            got = logits[int(starts[b]):int(starts[b + 1])].double()
+            ref = ref[-len(news[b]):]
+            # three products of 8-bit rows (a row's half step is 1/254 of its largest, some 3 deviations: 1 % of a
+            # deviation, over sums of independent terms), an 8-bit cache as much, bf16 in between: 4 % at most
+            assert ((got - ref).square().mean() / ref.square().mean()).sqrt() < 0.04
+            text[b] += [news[b][i] for i in plain[1][b] if i >= 0]
+            last[b] = plain[0][b][plain[2][b] - 1]
+
+
+@gpu
+def test_a_step_in_a_graph(pkg):
+    """Captured once, replayed with other inputs in the same places: as without the graph."""
+    def steps(g):
+        return Step(pkg, g, 5, 128, 4, 500, 5, 8)
+    plain, own = steps(gen(8)), steps(gen(8))
+    g = gen(9)
+    tokens, counts = torch.zeros(own.most, dtype=torch.int32, device="cuda"), ints([0] * 5)
+    uniforms = torch.zeros(own.most, dtype=torch.float64, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        own.run(tokens, counts, uniforms)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = own.run(tokens, counts, uniforms)
+    torch.cuda.synchronize()
+    for turn in range(6):
+        tokens.copy_(torch.randint(0, 500, (own.most,), device="cuda", generator=g))
+        counts.copy_(torch.randint(0, 7, (5,), device="cuda", generator=g))
+        uniforms.copy_(torch.rand(own.most, device="cuda", generator=g, dtype=torch.float64))
+        graph.replay()
+        want = plain.run(tokens, counts, uniforms)
+        n = int(want[0][-1])
+        for i, (a, b) in enumerate(zip(got, want)):
+            assert torch.equal(a[:n] if i == 4 else a, b[:n] if i == 4 else b), i  # (logits of rows that are there)
+
+
+@gpu
+def test_two_calls_give_the_same_bits(pkg):
+    g = gen(17)
+    x = normal(g, 300, 1500, dtype=torch.bfloat16)
+    linear = pkg.W8Linear.pack(normal(g, 1500, 700))
+    logits, uniforms = normal(g, 30, 30000), torch.rand(30, device="cuda", generator=g, dtype=torch.float64)
+    probs = torch.softmax(normal(g, 30, 30000), 1)
+    drafts, starts = torch.multinomial(probs, 1, generator=g).squeeze(1).to(torch.int32), ints(list(range(0, 31, 6)))
+    calls = [lambda: pkg.residual_norm(x, x, torch.ones(1500, device="cuda")), lambda: (linear(x), linear(x[:3]), linear(x[:50])),
+             lambda: pkg.verify_drafts(logits, drafts, uniforms, starts=starts, draft_probs=probs)]
+    for call in calls:
+        first = call()
+        for _ in range(5):
+            assert all(torch.equal(a, b) for a, b in zip(first, call()))
+
+
+@gpu
+def test_step_operators_cut_no_gradient_in_silence(pkg):
+    x = torch.randn((3, 64), device="cuda", requires_grad=True)
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    linear = pkg.W8Linear.pack(torch.randn(64, 20, device="cuda"))
+    plain = x.detach()
+    results = [pkg.residual_norm(x, plain, w.detach())[0], pkg.residual_norm(plain, x, w.detach())[1],
+               pkg.residual_norm(plain, plain, w)[1], pkg.residual_norm(plain, plain, w, quantise=True)[2], linear(x),
+               pkg.quantise_rows(x)[1], linear(x, dtype=torch.bfloat16)]
+    for r in results:
+        assert r.requires_grad
+        with pytest.raises(RuntimeError, match="computes no gradient"):
+            r.sum().backward()
+    assert not pkg.residual_norm(plain, plain, w)[0].requires_grad  # the stream does not depend on the norm's weight
+    with torch.no_grad():
+        assert not linear(x).requires_grad
+
+
+@gpu
+def test_step_operators_count_what_they_change(pkg):
+    pages = pkg.PageTable.empty(2, 3, 6, 8)
+    before = [t._version for t in (pages.table, pages.lens, pages.free, pages.n_free)]
+    pages.extend(ints([3, 4]), 10)
+    after = [t._version for t in (pages.table, pages.lens, pages.free, pages.n_free)]
+    assert [b - a for a, b in zip(before, after)] == [1, 1, 0, 1]
+    pages.truncate(ints([0, 0]))
+    assert [t._version - a for t, a in zip((pages.table, pages.lens, pages.free, pages.n_free), after)] == [1, 1, 1, 1]
+
+
+@gpu
+def test_step_operators_refuse_replaced_buffers(pkg):
+    pages = pkg.PageTable.empty(2, 3, 6, 8)
+    pages.lens.resize_(3)
+    with pytest.raises(pkg.ArgumentError):
+        pages.extend(ints([1, 1]), 4)
+    linear = pkg.W8Linear.pack(torch.ones(32, 16, device="cuda"))
+    x = torch.ones((2, 32), device="cuda")
+    before = linear(x)
+    linear.codes.data = torch.zeros((16, 48), dtype=torch.int8, device="cuda")
+    with pytest.raises(pkg.ArgumentError):
+        linear(x)
+    linear.codes.data = torch.zeros((16, 32), dtype=torch.int8, device="cuda")
+    assert linear(x).eq(0).all() and before.gt(0).all()
+
+
+@gpu
+@pytest.mark.parametrize("rows,k,n,lost_rows,lost_outputs", [(40, 1024, 1024, 40, 128), (300, 1024, 1024, 128, 128), (300, 512, 9000, 256, 256)])
+def test_a_wait_of_the_products_that_runs_out(pkg, rows, k, n, lost_rows, lost_outputs):
+    """A copy that never comes: that block's rows are NaN, the call returns, the next one is right."""
+    from forge_lm_b200 import _native as N
+    g = gen(1)
+    linear = w8_case(pkg, g, k, n)
+    x = torch.randint(-127, 128, (rows, k), device="cuda", generator=g).to(torch.int8)
+    scales = torch.ones(rows, device="cuda")
+    want = linear(x, scales=scales)
+    N.check(N.load().fb2_test_w8_withhold(1, 200_000_000))
+    y = linear(x, scales=scales)
+    torch.cuda.synchronize()
+    lost = y.isnan()
+    assert lost[:lost_rows, :lost_outputs].all() and int(lost.sum()) == lost_rows * lost_outputs
+    assert torch.equal(y[~lost], want[~lost])
+    assert torch.equal(linear(x, scales=scales), want)
+
+
+@gpu
+def test_step_refusals_on_the_device(pkg):
+    E = pkg.ArgumentError
+    f, h = torch.ones((3, 64), device="cuda"), torch.ones((3, 64), device="cuda", dtype=torch.bfloat16)
+    w = torch.ones(64, device="cuda")
+    pages = pkg.PageTable.empty(2, 3, 6, 8)
+    linear = pkg.W8Linear.pack(torch.ones(64, 32, device="cuda"))
+    codes, scales = pkg.quantise_rows(f)
+    u = torch.zeros(3, device="cuda", dtype=torch.float64)
+    d = ints([0, 0, 0])
+    neg = torch.complex(f, f).conj().imag
+    for call in (
+            lambda: pages.extend(ints([1, 1, 1]), 4), lambda: pages.extend(ints([1, 1]).long(), 4), lambda: pages.extend(ints([1, 1]), -1),
+            lambda: pages.extend(ints([1, 1]).cpu(), 4), lambda: pages.extend(ints([1, 1]), 2 ** 31), lambda: pages.extend(None, 4),
+            lambda: pages.truncate(ints([1])), lambda: pages.truncate([1, 1]),
+            lambda: pkg.PageTable(pages.table, pages.lens, pages.free, pages.n_free, 12),
+            lambda: pkg.PageTable(pages.table.t(), pages.lens, pages.free, pages.n_free, 8),
+            lambda: pkg.PageTable(pages.table, pages.lens[:1], pages.free, pages.n_free, 8),
+            lambda: pkg.PageTable(pages.table, pages.lens, pages.free, pages.lens, 8),
+            lambda: pkg.PageTable(pages.table, pages.lens, None, pages.n_free, 8),
+            lambda: pkg.PageTable.empty(20000, 1, 1, 8),
+            lambda: pkg.residual_norm(f, h, w), lambda: pkg.residual_norm(f, f[:2], w), lambda: pkg.residual_norm(f, f, w[:5]),
+            lambda: pkg.residual_norm(f, f, w.half()), lambda: pkg.residual_norm(f, f, None), lambda: pkg.residual_norm(f, f.t(), w),
+            lambda: pkg.residual_norm(f.double(), f, w), lambda: pkg.residual_norm(f, f, w, kind="other"),
+            lambda: pkg.residual_norm(f, f, w, scale=math.inf), lambda: pkg.residual_norm(f, f, w, eps=-1.0),
+            lambda: pkg.residual_norm(None, f, w, gate=f), lambda: pkg.residual_norm(None, f, w, post_weight=w),
+            lambda: pkg.residual_norm(f, f, w, gate=h), lambda: pkg.residual_norm(f, f, w, gate=w[:3]),
+            lambda: pkg.residual_norm(f, f, w, post_bias=w), lambda: pkg.residual_norm(f, f.cpu(), w),
+            lambda: pkg.residual_norm(f, neg, w), lambda: pkg.residual_norm(f, f, w, dtype=torch.bfloat16),
+            lambda: pkg.residual_norm(torch.ones((1, 40000), device="cuda"), torch.ones((1, 40000), device="cuda"), torch.ones(40000, device="cuda")),
+            lambda: pkg.quantise_rows(f.t()), lambda: pkg.quantise_rows(f.double()), lambda: pkg.quantise_rows(f[0]), lambda: pkg.quantise_rows(f.cpu()),
+            lambda: linear(f[:, :63]), lambda: linear(f.cpu()), lambda: linear(f.double()), lambda: linear(codes), lambda: linear(f, scales=scales),
+            lambda: linear(codes, scales=scales[:2]), lambda: linear(codes, scales=scales.half()), lambda: linear(torch.ones((64, 3), device="cuda").t()),
+            lambda: linear(f, dtype=torch.float64), lambda: linear(neg),
+            lambda: pkg.W8Linear(codes.float(), scales), lambda: pkg.W8Linear(codes, scales[:2]), lambda: pkg.W8Linear(codes, scales, bias=scales[:1]),
+            lambda: pkg.W8Linear(codes[:, 1:], scales), lambda: pkg.W8Linear(codes[:1].expand(3, 64), scales),
+            lambda: pkg.W8Linear(torch.zeros((2, 131073 + 15), dtype=torch.int8, device="cuda")[:, :131073], scales[:2]),
+            lambda: pkg.W8Linear.pack(f.double()), lambda: pkg.W8Linear.pack(f.t()), lambda: pkg.W8Linear.pack(f[0]),
+            lambda: pkg.verify_drafts(f, d, u.float()), lambda: pkg.verify_drafts(f, d.long(), u), lambda: pkg.verify_drafts(f, d[:2], u),
+            lambda: pkg.verify_drafts(f.t(), d, u), lambda: pkg.verify_drafts(f.double(), d, u), lambda: pkg.verify_drafts(f, d, u[:2]),
+            lambda: pkg.verify_drafts(f, d, u, parents=d, draft_probs=f), lambda: pkg.verify_drafts(f, d, u, draft_probs=h),
+            lambda: pkg.verify_drafts(f, d, u, draft_probs=f[:2]), lambda: pkg.verify_drafts(f, d, u, max_nodes=0),
+            lambda: pkg.verify_drafts(f, d, u, max_nodes=1025), lambda: pkg.verify_drafts(f, d, u, temperature=w[:2]),
+            lambda: pkg.verify_drafts(f, d, u, starts=ints([])), lambda: pkg.verify_drafts(f, d, u, starts=ints([0, 3]), temperature=w[:2]),
+            lambda: pkg.verify_drafts(f[:, :0], d, u), lambda: pkg.verify_drafts(f.cpu(), d, u)):
+        with pytest.raises(E):
+            call()
+    many = torch.zeros((1025, 4), device="cuda")
+    with pytest.raises(E):  # a bound of a sequence's rows is needed
+        pkg.verify_drafts(many, ints([0] * 1025), torch.zeros(1025, device="cuda", dtype=torch.float64), starts=ints([0, 1025]))
+
+
+def test_step_refusals_of_the_c_entries(pkg):
+    """What the C entry points refuse before any device work."""
+    import ctypes as C
+    import struct
+    from forge_lm_b200 import _native as N
+    L = N.load()
+    bad, ok, p = N.FB2_INVALID_ARG, N.FB2_OK, 4096
+    pages = struct.Struct("=4Qq4i")
+    base = [p, p, p, p, 10, 4, 10, 100, 16]
+    assert L.fb2_pages_check(pages.pack(*base)) == ok
+    for where, value in ((0, 0), (1, 0), (2, 0), (3, 0), (0, 4098), (1, 4097), (2, 4098), (3, 4097), (4, 9), (5, -1), (5, 16385), (6, -1),
+                         (7, -1), (8, 12), (8, 4), (8, 2048), (7, 2 ** 31 - 1)):
+        wrong = list(base)
+        wrong[where] = value
+        s = pages.pack(*wrong)
+        assert L.fb2_pages_check(s) == bad, (where, value)
+        assert L.fb2_pages_extend(s, p, 10, p, p, p, p, None) == bad and L.fb2_pages_truncate(s, p, None) == bad
+    assert L.fb2_pages_check(None) == bad
+    good = pages.pack(*base)
+    for args in ((0, 10, p, p, p, p), (p, 10, 0, p, p, p), (p, 10, p, 0, p, p), (p, 10, p, p, 0, p), (p, 10, p, p, p, 0), (p, -1, p, p, p, p),
+                 (p, 2 ** 31 - 1, p, p, p, p), (4098, 10, p, p, p, p), (p, 10, p, p, 4097, p)):
+        assert L.fb2_pages_extend(good, *args, None) == bad, args
+    assert L.fb2_pages_truncate(good, None, None) == bad and L.fb2_pages_truncate(good, 4098, None) == bad
+
+    norm = struct.Struct("=11Q6q5i2fi")
+    base = [p, p, 0, p, 0, 0, 0, p, p, 0, 0] + [64] * 5 + [64] + [2, 64, 1, 1, 0, 1.0, 1e-5, 0]
+    for where, value in ((1, 0), (3, 0), (7, 0), (8, 0), (9, p), (10, p), (0, 4097), (1, 4097), (8, 4097), (3, 4098), (6, p), (14, 63), (15, 63),
+                         (17, -1), (18, 0), (18, 32769), (19, 3), (20, 2), (21, 2), (22, math.nan), (23, -1.0), (23, math.inf)):
+        wrong = list(base)
+        wrong[where] = value
+        assert L.fb2_residual_norm(norm.pack(*wrong), None) == bad, (where, value)
+    coded = list(base)
+    coded[8], coded[9], coded[10] = 0, p, p
+    for where, value in ((9, 4100), (16, 60), (16, 72), (10, 4098)):
+        wrong = list(coded)
+        wrong[where] = value
+        assert L.fb2_residual_norm(norm.pack(*wrong), None) == bad, (where, value)
+    alone = list(base)
+    alone[0], alone[2] = 0, p
+    assert L.fb2_residual_norm(norm.pack(*alone), None) == bad and L.fb2_residual_norm(None, None) == bad
+    base[17] = 0
+    assert L.fb2_residual_norm(norm.pack(*base), None) == ok
+
+    for args in ((-1, 8, p, 0, 8, p, 16, p), (1, 0, p, 0, 8, p, 16, p), (1, 8, 0, 0, 8, p, 16, p), (1, 8, p, 3, 8, p, 16, p), (1, 8, p, 0, 8, 4100, 16, p),
+                 (2, 8, p, 0, 8, p, 8, p), (2, 32, p, 0, 32, p, 16, p), (1, 8, 4098, 0, 8, p, 16, p), (1, 8, p, 0, 8, p, 16, 4098)):
+        assert L.fb2_quantise_rows(*args, None) == bad, args
+    assert L.fb2_quantise_rows(0, 8, None, 0, 8, None, 16, None, None) == ok
+
+    lin = struct.Struct("=QQQq2i")
+    base = [p, p, 0, 112, 100, 33]
+    n = C.c_int64()
+    for where, value in ((0, 0), (1, 0), (0, 4104), (1, 4098), (2, 4098), (3, 96), (3, 104), (4, 0), (4, 131073), (5, 0), (5, 2 ** 31 - 1)):
+        wrong = list(base)
+        wrong[where] = value
+        w = lin.pack(*wrong)
+        assert L.fb2_w8_check(w) == bad, (where, value)
+        assert L.fb2_w8_pack(w, p, 0, 33, None) == bad and L.fb2_w8_matmul(w, 1, p, 112, p, p, 33, 0, None) == bad
+        assert L.fb2_w8_forward(w, 1, p, 100, p, 33, 0, p, 1 << 20, None) == bad and L.fb2_w8_forward_workspace(w, 1, C.byref(n)) == bad
+    w = lin.pack(*base)
+    assert L.fb2_w8_check(w) == ok and L.fb2_w8_check(None) == bad
+    assert L.fb2_w8_pack(w, None, 0, 33, None) == bad and L.fb2_w8_pack(w, p, 0, 32, None) == bad and L.fb2_w8_pack(w, 4098, 0, 33, None) == bad
+    for args in ((-1, p, 112, p, p, 33, 0), (1, 0, 112, p, p, 33, 0), (1, p, 112, 0, p, 33, 0), (1, p, 112, p, 0, 33, 0), (1, p, 112, p, p, 33, 5),
+                 (1, 4104, 112, p, p, 33, 0), (2, p, 96, p, p, 33, 0), (2, p, 104, p, p, 33, 0), (2, p, 112, p, p, 32, 0), (1, p, 112, 4098, p, 33, 0),
+                 (1, p, 112, p, 4097, 33, 1)):
+        assert L.fb2_w8_matmul(w, *args, None) == bad, args
+    assert L.fb2_w8_matmul(w, 0, None, 0, None, None, 0, 0, None) == ok
+    assert L.fb2_w8_forward_workspace(w, 9, C.byref(n)) == ok and n.value == 9 * (112 + 4)
+    assert L.fb2_w8_forward_workspace(w, -1, C.byref(n)) == bad and L.fb2_w8_forward_workspace(w, 9, None) == bad
+    for args in ((9, p, 100, p, 33, 0, p, 9 * 116 - 1), (9, p, 100, p, 33, 0, 0, 0), (9, p, 100, p, 33, 0, 4100, 9 * 116), (9, 0, 100, p, 33, 0, p, 9 * 116),
+                 (9, p, 100, p, 32, 0, p, 9 * 116), (9, 4098, 100, p, 33, 0, p, 9 * 116), (-1, p, 100, p, 33, 0, p, 9 * 116)):
+        assert L.fb2_w8_forward(w, *args, None) == bad, args
+    assert L.fb2_w8_forward(w, 0, None, 0, None, 0, 0, None, 0, None) == ok
+
+    ver = struct.Struct("=11Q3q6i")
+    base = [p, 0, p, p, 0, p, 0, p, p, p, p] + [6 * 16, 50, 50] + [2, 6, 50, 0, 4, 0]
+    assert L.fb2_verify_workspace(ver.pack(*base), C.byref(n)) == ok and n.value == 6 * 16
+    for where, value in ((0, 0), (2, 0), (5, 0), (7, 0), (8, 0), (9, 0), (10, 0), (0, 4098), (1, 4098), (2, 4097), (3, 4097), (4, 4097), (5, 4100), (6, 4097),
+                         (7, 4097), (8, 4098), (9, 4098), (10, 4104), (11, 95), (14, -1), (15, -1), (16, 0), (16, 2 ** 31 - 1), (17, 4), (18, 0), (18, 1025)):
+        wrong = list(base)
+        wrong[where] = value
+        assert L.fb2_verify_drafts(ver.pack(*wrong), None) == bad, (where, value)
+    chain = list(base)
+    chain[1] = chain[4] = p
+    assert L.fb2_verify_drafts(ver.pack(*chain), None) == bad
+    alone = list(base)
+    alone[3] = 0
+    assert L.fb2_verify_drafts(ver.pack(*alone), None) == bad  # 6 rows, 2 sequences
+    base[14] = 0
+    assert L.fb2_verify_drafts(ver.pack(*base), None) == ok
+    assert L.fb2_verify_drafts(None, None) == bad and L.fb2_verify_workspace(ver.pack(*base), None) == bad
+    assert L.fb2_test_w8_withhold(-1, 5) == bad and L.fb2_test_w8_withhold(0, 0) == bad and L.fb2_test_w8_withhold(0, 3_000_000_000) == bad
+    assert L.fb2_last_error() != b""
