@@ -193,28 +193,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_pages_truncate(PagesView p, cons
     const int total = (int)min(all.a, (long long)INT32_MAX);
     if (tid == 0) *p.n_free = (int)min((long long)n_free + total, (long long)p.n_pages);
     // the first page dropped ends up last on the list: the next to be taken
-    for (int j0 = tid * PG_RUN; j0 < total; j0 += THREADS * PG_RUN) {
-        int* entry[PG_RUN];
-        int page[PG_RUN], b = -1, end = j0;
-#pragma unroll
-        for (int i = 0; i < PG_RUN; i++) {
-            const int j = j0 + i;
-            if (j >= total) break;
-            if (j >= end) {
-                b = pg::owner(s_at, p.n_seqs, j);
-                end = b + 1 < p.n_seqs ? s_at[b + 1] : total;
-            }
-            entry[i] = p.table + b * p.stride + s_keep[b] + (j - s_at[b]);
-            page[i] = *entry[i];
-        }
-#pragma unroll
-        for (int i = 0; i < PG_RUN; i++) {
-            const int j = j0 + i;
-            if (j >= total) break;
-            const long long to_place = (long long)n_free + total - 1 - j;
-            if (to_place < p.n_pages) p.free[to_place] = page[i];
-            *entry[i] = -1;
-        }
+    for (int j = tid; j < total; j += THREADS) {
+        const int b = pg::owner(s_at, p.n_seqs, j);
+        int* entry = p.table + b * p.stride + s_keep[b] + (j - s_at[b]);
+        const long long i = (long long)n_free + total - 1 - j;
+        if (i < p.n_pages) p.free[i] = *entry;
+        *entry = -1;
     }
 }
 

@@ -437,6 +437,15 @@ int32_t fb2_w8_forward(const fb2_w8_linear* w, int32_t n_rows, const void* x, in
 
 // ---- verification of drafts -----------------------------------------------------------
 namespace {
+// CTAs to a row: of at least 2048 ids each where rows leave SMs free, else of 32768
+// and up to 8 on each SM.
+int verify_ranks(int vocab, int rows) {
+    int ranks = 1;
+    while (ranks < VF_RANKS && vocab > 2048 * ranks &&
+           ((int64_t)rows * ranks * 2 <= 2 * 148 || (vocab > 32768 * ranks && (int64_t)rows * ranks * 2 <= 8 * 148)))
+        ranks *= 2;
+    return ranks;
+}
 VerifyArgs verify_args(const fb2_verify* v) {
     need(v, "verify arguments are NULL");
     check_dtype(v->dtype);
@@ -463,24 +472,17 @@ VerifyArgs verify_args(const fb2_verify* v) {
     a.n_rows = v->n_rows;
     a.vocab = v->vocab;
     a.max_nodes = v->max_nodes;
+    a.parts = verify_ranks(a.vocab, a.n_rows);
+    a.ranks = verify_ranks(a.vocab, a.n_seqs);
     return a;
-}
-// CTAs to a row: of at least 2048 ids each where rows leave SMs free, else of 16384
-// and up to 8 on each SM (161 rows x 131071 bf16, all of a call: 53 us with 4, 57 with
-// 2, 64 with 1; 289 x 50257 fp16: 35 with 2, 37 with 4, 41 with 8).
-int verify_ranks(int vocab, int rows) {
-    int ranks = 1;
-    while (ranks < VF_RANKS && vocab > 2048 * ranks &&
-           ((int64_t)rows * ranks * 2 <= 2 * 148 || (vocab > 16384 * ranks && (int64_t)rows * ranks * 2 <= 8 * 148)))
-        ranks *= 2;
-    return ranks;
 }
 }  // namespace
 
 int32_t fb2_verify_workspace(const fb2_verify* v, int64_t* bytes) {
     return guarded([&] {
         need(bytes, "bytes is NULL");
-        *bytes = (int64_t)verify_args(v).n_rows * sizeof(VerifyRow);
+        const VerifyArgs a = verify_args(v);
+        *bytes = (int64_t)a.n_rows * a.parts * (int64_t)sizeof(VerifyRow);
     });
 }
 
@@ -494,16 +496,16 @@ int32_t fb2_verify_drafts(const fb2_verify* v, void* stream) {
                  aligned(a.parents, 4) && aligned(a.uniforms, 8) && aligned(a.temperature, 4) && aligned(a.tokens, 4) &&
                  aligned(a.nodes, 4) && aligned(a.counts, 4),
              "a tensor is not aligned to its element size");
-        need(a.n_rows == 0 || (v->device_workspace && v->workspace_bytes >= (int64_t)a.n_rows * (int64_t)sizeof(VerifyRow)),
+        need(a.n_rows == 0 || (v->device_workspace && v->workspace_bytes >= (int64_t)a.n_rows * a.parts * (int64_t)sizeof(VerifyRow)),
              "the workspace is too small");
         need(aligned(v->device_workspace, 16), "the workspace must be 16-byte aligned");
         a.rows = static_cast<VerifyRow*>(v->device_workspace);
         with_type(v->dtype, [&](auto t) {
             using T = decltype(t);
-            a.ranks = verify_ranks(a.vocab, a.n_rows);
-            if (a.n_rows) launch_cluster(k_verify_rows<T>, dim3(a.n_rows * a.ranks), VF_THREADS, 0, a.ranks, false, stream, a);
-            a.ranks = verify_ranks(a.vocab, a.n_seqs);
-            launch_cluster(k_verify_walk<T>, dim3(a.n_seqs * a.ranks), VW_THREADS, 0, a.ranks, a.n_rows > 0, stream, a);
+            if (a.n_rows) k_verify_rows<T><<<a.n_rows * a.parts, VF_THREADS, 0, (cudaStream_t)stream>>>(a);
+            launched();
+            opt_in_smem((const void*)k_verify_walk<T>, VF_NODES * VW_NODE);
+            launch_cluster(k_verify_walk<T>, dim3(a.n_seqs * a.ranks), VW_THREADS, a.max_nodes * VW_NODE, a.ranks, a.n_rows > 0, stream, a);
         });
     });
 }

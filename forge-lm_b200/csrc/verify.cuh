@@ -2,10 +2,10 @@
 // that follows the accepted ones (include/forge_b200.h, fb2_verify_drafts, has
 // the rules).
 //
-// Two kernels.  k_verify_rows reads every row of logits once: its largest and
-// sum of exp((l - largest) / T), or where it is largest for T <= 0.
-// k_verify_walk takes a sequence: the drafts' probabilities are looked up at once
-// and walked down by one thread; then the row at which the walk ended is weighed
+// Two kernels.  k_verify_rows reads every row of logits once, some CTAs to a row:
+// the largest and the sum of exp((l - largest) / T) of their parts, and where the
+// largest is for T <= 0.  k_verify_walk takes a sequence: the drafts' probabilities
+// are looked up at once and walked down by one warp; then the row at which the walk ended is weighed
 // (without rejected tokens, or less the draft's probabilities), its sums over
 // parts in the order of ids say in which part the draw falls, and that part is
 // looked through.
@@ -28,6 +28,7 @@ constexpr int VW_THREADS = 512, VW_WARPS = VW_THREADS / 32;
 constexpr int VW_BATCH = 4;                 // loads of a lane that are in flight at once
 constexpr int VW_RUN = 32 * VW_BATCH;       // ids of a warp's batch
 constexpr int VW_PARTS = 16;                // of a warp's ids, each with its own sum
+constexpr int VW_NODE = 44;                 // bytes of shared memory for a node
 // How far a sum of k_verify_rows may be off, relative.  An exponent (l - top) * log2(e) / T
 // has three roundings, and the exponents' mean under p is at most log2(vocab) <= 31: 31 *
 // 3 * 2^-24 * ln 2; ex2.approx 2^-22; a sum of 8 in fp32, the rest in fp64: 2^-21.
@@ -38,7 +39,7 @@ constexpr float VF_COLD = 1e-30f;  // a T below is not divided by in 32 bits: al
 struct VerifyRow {
     double sum;  // of exp((l - top) / T), to VF_OFF; not positive and finite where the row has no probabilities
     float top;
-    int best;  // the lowest id of the largest logit (T <= 0)
+    int best;  // the lowest id of the largest logit (T <= 0; -1: none)
 };
 struct VerifyArgs {
     const void* logits;
@@ -47,9 +48,10 @@ struct VerifyArgs {
     const double* uniforms;
     const float* temperature;
     int *tokens, *nodes, *counts;
-    VerifyRow* rows;
+    VerifyRow* rows;  // [n_rows][parts]: of a part of a row each
     long long logits_row, probs_row;
-    int n_seqs, n_rows, vocab, max_nodes, ranks;  // ranks: CTAs of a cluster, a power of two
+    int n_seqs, n_rows, vocab, max_nodes;
+    int parts, ranks;  // CTAs of a row, and of a sequence's cluster: at most VF_RANKS
     // the rows of sequence b
     FB2_DEV void rows_of(int b, int& first, int& last) const {
         if (!starts) {
@@ -170,6 +172,21 @@ FB2_DEV int pick(F part, int n, double target, double& passed) {
     passed = __shfl_sync(0xffffffffu, before, chosen);
     return __shfl_sync(0xffffffffu, at, chosen);
 }
+// log2(e) / T, T > 0; not 0 for T = inf, as -inf times it has to be -inf
+FB2_DEV float near_of(float heat) { return fmaxf(1.44269504088896341f / fmaxf(heat, VF_COLD), 1e-44f); }
+// The whole row's of its parts
+FB2_DEV VerifyRow joined(const VerifyRow* parts, int n, float near) {
+    VerifyRow all = parts[0];
+#pragma unroll 1
+    for (int k = 1; k < n; k++) {
+        const VerifyRow r = parts[k];
+        if (r.best >= 0 && (all.best < 0 || r.top > all.top || (r.top == all.top && r.best < all.best))) all.best = r.best;
+        const float top = fmaxf(all.top, r.top);
+        all.sum = all.sum * (double)ex2((all.top - top) * near) + r.sum * (double)ex2((r.top - top) * near);
+        all.top = top;
+    }
+    return all;
+}
 // The sequence of a row: the last b with starts[b] <= row, by all lanes.
 FB2_DEV int owner(const int* starts, int n, int row) {
     int lo = 0, hi = n;  // starts[lo] <= row (or lo = 0), starts[hi] > row (or hi = n)
@@ -186,51 +203,53 @@ FB2_DEV bool proper(double sum) { return sum > 0.0 && sum < INFINITY; }
 
 }  // namespace vf
 
-// A cluster to a row; its CTAs each take a part of it.
+// a.parts CTAs to a row.
 template <class T>
 __global__ void __launch_bounds__(VF_THREADS) k_verify_rows(VerifyArgs a) {
-    __shared__ double s_sum[VF_WARPS], c_sum;
-    __shared__ float s_top[VF_WARPS], c_top;
-    __shared__ int s_best[VF_WARPS], c_best;
+    __shared__ double s_sum[VF_WARPS];
+    __shared__ float s_top[VF_WARPS];
+    __shared__ int s_best[VF_WARPS];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the walk's launch; it waits for this grid's end
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int ranks = a.ranks, rank = blockIdx.x % ranks, row = blockIdx.x / ranks;
+    const int part = blockIdx.x % a.parts, row = blockIdx.x / a.parts;
     const int b = a.starts ? vf::owner(a.starts, a.n_seqs, row) : row;
     int first, last;
     a.rows_of(b, first, last);
-    if (row < first || row >= last) {  // the whole cluster
-        if (rank == 0 && tid == 0) a.rows[row] = {0.0, -INFINITY, -1};
+    if (row < first || row >= last) {
+        if (tid == 0) a.rows[blockIdx.x] = {0.0, -INFINITY, -1};
         return;
     }
     const float heat = a.heat(b);
     const bool greedy = !(heat > 0.f);
-    // (not 0 for T = inf: -inf times it is -inf)
-    const float cold = fmaxf(1.44269504088896341f / (greedy ? 1.f : fmaxf(heat, VF_COLD)), 1e-44f);
+    const float cold = vf::near_of(greedy ? 1.f : heat);
     const T* p = (const T*)a.logits + row * a.logits_row;
     constexpr int N = 16 / sizeof(T);
     // ids before the first 16-byte boundary, pieces of 16 bytes, the rest
     const int head = min(a.vocab, (int)(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T)));
-    const int pieces = (a.vocab - head) / N, per = (pieces + ranks - 1) / ranks;
-    const int p0 = min(rank * per, pieces), p1 = min(p0 + per, pieces);
-    float top = -3.402823466e38f;  // (finite: -inf less this is -inf)
+    const int pieces = (a.vocab - head) / N, per = (pieces + a.parts - 1) / a.parts;
+    const int p0 = min(part * per, pieces), p1 = min(p0 + per, pieces);
+    // The terms are relative to `base`, which follows the largest logit when that is 2^8
+    // of a term away: a sum that was rescaled weighs a 256th, and its roundings with it.
+    float top = -3.402823466e38f, base = top;  // (finite: -inf less this is -inf)
     double sum = 0.0;
     int best = -1;
-    auto raise = [&](float to) {
-        if (to > top) {
-            sum *= (double)vf::ex2((top - to) * cold);
-            top = to;
+    auto raise = [&](float most) {
+        top = fmaxf(top, most);
+        if ((most - base) * cold > 8.f) {
+            sum *= (double)vf::ex2((base - most) * cold);
+            base = most;
         }
     };
-    // sum of exp2((v - top) * cold) of a piece (NaN for NaN, and for all where one is inf), two values to an instruction
-    auto terms = [&](const float (&v)[16 / sizeof(T)]) {
-        const float2 up = make_float2(-top, -top), by = make_float2(cold, cold);
-        float2 part = make_float2(0.f, 0.f);
+    // sum of exp2((v - base) * cold) of a piece (NaN for NaN, and for all where one is inf), two values to an instruction
+    auto terms = [&](const float (&v)[N]) {
+        const float2 up = make_float2(-base, -base), by = make_float2(cold, cold);
+        float2 s = make_float2(0.f, 0.f);
 #pragma unroll
         for (int j = 0; j < N; j += 2) {
             const float2 x = vf::mul2(vf::add2(make_float2(v[j], v[j + 1]), up), by);
-            part = vf::add2(part, make_float2(vf::ex2(x.x), vf::ex2(x.y)));
+            s = vf::add2(s, make_float2(vf::ex2(x.x), vf::ex2(x.y)));
         }
-        return part.x + part.y;
+        return s.x + s.y;
     };
     const uint4* body = reinterpret_cast<const uint4*>(p + head);
     constexpr int M = 4;  // loads in flight
@@ -259,50 +278,40 @@ __global__ void __launch_bounds__(VF_THREADS) k_verify_rows(VerifyArgs a) {
         const float v = Dense<T>::get(p[id]);
         if (v > top || (v == top && (best < 0 || id < best))) best = id;
         raise(v);
-        sum += (double)vf::ex2((v - top) * cold);
+        sum += (double)vf::ex2((v - base) * cold);
     };
-    if (rank == 0 && tid < head) edge(tid);
-    if (rank == ranks - 1 && head + pieces * N + tid < a.vocab) edge(head + pieces * N + tid);
-    // the lanes' parts: in every lane the largest, the sum below it, the first id that has it
+    if (part == 0 && tid < head) edge(tid);
+    if (part == a.parts - 1 && head + pieces * N + tid < a.vocab) edge(head + pieces * N + tid);
+    // in every lane the lanes' largest, the sum below it, the first id that has it
     auto join = [&]() {
         const float most = warp_max(top);
         if (greedy) best = (int)__reduce_min_sync(0xffffffffu, top == most ? (uint32_t)best : 0xffffffffu);  // -1: none
-        sum = vf::warp_sum(sum * (double)vf::ex2((top - most) * cold));
-        top = most;
+        sum = vf::warp_sum(sum * (double)vf::ex2((base - most) * cold));
+        top = base = most;
     };
-    auto none = [&]() { top = -3.402823466e38f, sum = 0.0, best = -1; };
     join();
     if (lane == 0) s_top[warp] = top, s_sum[warp] = sum, s_best[warp] = best;
     __syncthreads();
-    if (warp == 0) {  // the warps' parts, then the cluster's
-        if (lane < VF_WARPS)
-            top = s_top[lane], sum = s_sum[lane], best = s_best[lane];
-        else
-            none();
+    if (warp == 0) {
+        const bool one = lane < VF_WARPS;
+        top = base = one ? s_top[lane] : -3.402823466e38f, sum = one ? s_sum[lane] : 0.0, best = one ? s_best[lane] : -1;
         join();
-        if (lane == 0) c_top = top, c_sum = sum, c_best = best;
+        if (lane == 0) a.rows[blockIdx.x] = {sum, top, best};
     }
-    if (ranks > 1) pg::cluster_sync();
-    if (rank == 0 && warp == 0) {
-        if (ranks > 1) {
-            if (lane < ranks)
-                top = vf::peek(&c_top, lane), sum = vf::peek(&c_sum, lane), best = vf::peek(&c_best, lane);
-            else
-                none();
-            join();
-        }
-        if (lane == 0) a.rows[row] = {sum, top, best};
-    }
-    if (ranks > 1) pg::cluster_sync();  // the others' shared memory stays until it is read
 }
 
 // A cluster to a sequence; its CTAs share the draw's row.
 template <class T>
 __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
-    __shared__ double s_mass[VF_NODES], s_limit[VF_NODES], s_total[VF_NODES];
-    __shared__ int s_parent[VF_NODES], s_token[VF_NODES], s_gone[VF_NODES];
+    // of the nodes: their rows' sums; the drafts' weights at their parents, what they are held
+    // against, their parents, their tokens; the tokens of rejected ones
+    extern __shared__ __align__(16) unsigned char vw_smem[];
+    VerifyRow* s_row = reinterpret_cast<VerifyRow*>(vw_smem);
+    double *s_mass = reinterpret_cast<double*>(s_row + a.max_nodes), *s_limit = s_mass + a.max_nodes;
+    int *s_parent = reinterpret_cast<int*>(s_limit + a.max_nodes), *s_token = s_parent + a.max_nodes, *s_gone = s_token + a.max_nodes;
     __shared__ double s_powers[1024], s_factors[64], s_part[VW_WARPS * VW_PARTS], s_warp[VW_WARPS], c_sum[2];
     __shared__ double s_lost;
+    __shared__ unsigned char s_hit[VW_WARPS * VW_PARTS];  // parts that have a rejected token
     __shared__ int s_at, s_count, s_gone_n, s_rejected, s_next, s_ask;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int ranks = a.ranks, rank = blockIdx.x % ranks, b = blockIdx.x / ranks;
@@ -317,6 +326,7 @@ __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
     vf::Heat at_heat;
     at_heat.cold = greedy ? 0.0 : 1024 * 1.4426950408889634074 / (double)heat;
     at_heat.near = fmaxf((float)(at_heat.cold / 1024), 1e-44f);
+    const float near = vf::near_of(greedy ? 1.f : heat);
     const T* logits = (const T*)a.logits;
     pdl_wait();  // the rows' sums, and the outputs' memory
     if (rank == 0)
@@ -325,19 +335,20 @@ __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
         if (rank == 0 && tid == 0) a.counts[b] = 0;
         return;
     }
-    __syncthreads();  // the table
+    for (int i = tid; i < n; i += VW_THREADS) s_row[i] = vf::joined(a.rows + (long long)(first + i) * a.parts, a.parts, near);
+    __syncthreads();  // they and the table
     // a draft's weight at its parent, and what it is held against
     for (int i = 1 + tid; i < n; i += VW_THREADS) {
         int parent = a.parents ? __ldg(a.parents + first + i) : i - 1;
         const int token = __ldg(a.drafts + first + i);
-        double mass = 0.0, total = 1.0, limit = __ldg(a.uniforms + first + i);
+        double mass = 0.0, limit = __ldg(a.uniforms + first + i);
         if (parent < 0 || parent >= i) {
             parent = -1;
         } else {
             const bool known = (unsigned)token < (unsigned)a.vocab;
             const float l = known ? Dense<T>::get(logits[(first + parent) * a.logits_row + token]) : -INFINITY;
             const double q = a.probs && known ? (double)a.probs[(first + i) * a.probs_row + token] : NAN;
-            const VerifyRow r = a.rows[first + parent];
+            const VerifyRow r = s_row[parent];
             if (!vf::proper(r.sum))
                 mass = NAN;  // nothing is accepted
             else if (greedy)
@@ -347,15 +358,14 @@ __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
                 h.top32 = r.top, h.top = vf::widen(r.top);
                 mass = h.weight(l, s_powers);
             }
-            if (!greedy) total = r.sum;
             if (a.probs) limit *= q;
         }
         s_parent[i] = parent, s_token[i] = token;
-        s_mass[i] = mass, s_limit[i] = limit, s_total[i] = total;
+        s_mass[i] = mass, s_limit[i] = limit;
     }
     if (tid == 0) s_at = 0, s_count = 1, s_gone_n = 0, s_rejected = -1, s_next = 1, s_lost = 0.0;
     if (tid == 0 && rank == 0) nodes[0] = 0;
-    for (int i = tid; i < VW_WARPS * VW_PARTS; i += VW_THREADS) s_part[i] = 0.0;  // parts behind the row's end stay so
+    for (int i = tid; i < VW_WARPS * VW_PARTS; i += VW_THREADS) s_part[i] = 0.0, s_hit[i] = 0;  // parts behind the row's end stay so
     __syncthreads();
 
     // ---- sums over a row, in parts in the order of ids: a CTA's, a warp's, a batch's
@@ -367,9 +377,8 @@ __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
     double scale = 1.0;                  // with q: 1 / the row's sum
     const double* sums = nullptr;        // of the CTAs
     int gone_n = 0;                      // rejected tokens that count as nothing
-    unsigned long long filter = 0;       // their low bits
     // weights of VW_BATCH ids from `id` on, STEP apart, up to `end`
-    auto batch = [&](int id, int end, double (&m)[VW_BATCH], auto step) {
+    auto batch = [&](int id, int end, double (&m)[VW_BATCH], auto step, bool hit) {
         constexpr int N = VW_BATCH, STEP = decltype(step)::value;
         float l[N], qv[N];
 #pragma unroll
@@ -384,52 +393,70 @@ __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
 #pragma unroll
             for (int j = 0; j < N; j++) m[j] = vf::positive(fma(m[j], scale, -vf::widen(qv[j])));
         }
-        if (filter) {
+        if (hit)
+            for (int k = 0; k < gone_n; k++)
 #pragma unroll
-            for (int j = 0; j < N; j++)
-                if ((filter >> ((id + STEP * j) & 63)) & 1)
-                    for (int k = 0; k < gone_n; k++)
-                        if (s_gone[k] == id + STEP * j) m[j] = 0.0;
-        }
+                for (int j = 0; j < N; j++)
+                    if (s_gone[k] == id + STEP * j) m[j] = 0.0;
     };
 
-    // ---- the walk by one thread, until it ends or a test needs its row's sum in 64 bits;
+    // ---- the walk by one warp, until it ends or a test needs its row's sum in 64 bits;
     // that sum; the draw's.  One loop, so that the sums' code is there (and fetched) once.
     enum { WALK, DRAW, DRAW_ALL } state = WALK;
     int known = -1;  // the node whose sum is known
     double exact = 0.0, total = 0.0;
     for (int turn = 0;; turn++) {
         if (state == WALK) {
-            if (tid == 0) {
-                int at = s_at, count = s_count, gn = s_gone_n, rejected = s_rejected, i = s_next, ask = -1;
+            if (warp == 0) {
+                int at = s_at, count = s_count, gn = s_gone_n, rejected = s_rejected, ask = -1;
                 double gone = s_lost;  // the rejected siblings' weight
-                for (; i < n; i++) {
-                    if (s_parent[i] != at) continue;
+                for (int i = s_next;;) {
+                    // the node's next child
+                    uint32_t kids = 0;
+                    int i0 = i;
+                    for (; i0 < n; i0 += 32) {
+                        kids = __ballot_sync(0xffffffffu, i0 + lane < n && s_parent[i0 + lane] == at);
+                        if (kids) break;
+                    }
+                    if (!kids) {
+                        s_next = n;
+                        break;
+                    }
+                    i = i0 + __ffs(kids) - 1;
+                    const int token = s_token[i];
                     double mass = s_mass[i];
                     bool again = false;  // a sibling with this token was rejected
-                    for (int k = 0; k < gn; k++) again |= s_gone[k] == s_token[i];
+                    for (int k = lane; k < gn; k += 32) again |= s_gone[k] == token;
+                    again = __any_sync(0xffffffffu, again);
                     if (again) mass = 0.0;
-                    const double sum = known == at ? exact : s_total[i], weighed = a.probs ? sum : sum - gone;
+                    const double sum = greedy ? 1.0 : known == at ? exact : s_row[at].sum, weighed = a.probs ? sum : sum - gone;
                     const double held = s_limit[i] * weighed;
                     if (!greedy && known != at && mass > 0.0 && (fabs(held - mass) <= VF_OFF * fabs(s_limit[i]) * sum || heat < VF_COLD)) {
                         ask = at;
+                        s_next = i;
                         break;
                     }
                     if (held < mass) {
-                        if (rank == 0) nodes[count] = i, tokens[count - 1] = s_token[i];
+                        if (rank == 0 && lane == 0) nodes[count] = i, tokens[count - 1] = token;
                         at = i, count++;
                         gone = 0.0, gn = 0, rejected = -1;
                     } else {
-                        if (!again) gone += mass, s_gone[gn++] = s_token[i];
+                        if (!again) {
+                            gone += mass;
+                            if (lane == 0) s_gone[gn] = token;
+                            gn++;
+                        }
                         rejected = i;
                     }
+                    __syncwarp();
+                    i++;
                 }
-                s_at = at, s_count = count, s_gone_n = gn, s_rejected = rejected, s_next = i, s_lost = gone, s_ask = ask;
+                if (lane == 0) s_at = at, s_count = count, s_gone_n = gn, s_rejected = rejected, s_lost = gone, s_ask = ask;
             }
             __syncthreads();
         }
         const int node = s_at, rejected = s_rejected;
-        const VerifyRow r = a.rows[first + node];
+        const VerifyRow r = s_row[node];
         p = logits + (first + node) * a.logits_row;
         at_heat.top32 = r.top, at_heat.top = vf::widen(r.top);
         if (state == WALK && s_ask < 0) {
@@ -448,7 +475,11 @@ __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
                 if (rejected >= 0) q = a.probs + (first + rejected) * a.probs_row, scale = 1.0 / exact;
             } else {
                 gone_n = s_gone_n;
-                for (int k = 0; k < gone_n; k++) filter |= 1ull << (s_gone[k] & 63);
+                for (int k = tid; k < gone_n; k += VW_THREADS) {
+                    const int at = s_gone[k] - rank * share;
+                    if (at >= 0 && at < share) s_hit[at / each * VW_PARTS + at % each / run] = 1;
+                }
+                __syncthreads();
             }
         }
         // the row's sums
@@ -456,9 +487,10 @@ __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
         for (int k = 0, p0 = w0; k < VW_PARTS && p0 < w1; k++, p0 += run) {
             double sum = 0.0;
             const int p1 = min(w1, p0 + run);
+            const bool hit = gone_n && s_hit[warp * VW_PARTS + k];
             for (int id = p0; id < p1; id += VW_RUN) {
                 double m[VW_BATCH];
-                batch(id + lane, p1, m, std::integral_constant<int, 32>{});
+                batch(id + lane, p1, m, std::integral_constant<int, 32>{}, hit);
 #pragma unroll
                 for (int j = 0; j < VW_BATCH; j++) sum += m[j];
             }
@@ -480,7 +512,7 @@ __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
         } else if (total > 0.0 || state == DRAW_ALL) {
             break;
         } else {  // nothing is left: the row as if nothing had been rejected
-            q = nullptr, filter = 0;
+            q = nullptr, gone_n = 0;
             state = DRAW_ALL;
         }
     }
@@ -499,7 +531,7 @@ __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
 #pragma unroll 1
             for (int id = p0 + lane * VW_BATCH; id - lane * VW_BATCH < p1; id += VW_RUN) {
                 double m[VW_BATCH], sum = 0.0;
-                batch(id, p1, m, std::integral_constant<int, 1>{});
+                batch(id, p1, m, std::integral_constant<int, 1>{}, gone_n && s_hit[part]);
 #pragma unroll
                 for (int j = 0; j < VW_BATCH; j++) sum += m[j];
                 double up = sum;

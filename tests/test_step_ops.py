@@ -598,7 +598,7 @@ def test_verification_of_rows_without_probabilities(pkg):
     drafts[0] = -1
     drafts = drafts.roll(1)
     uniforms = torch.rand(12, device="cuda", generator=g, dtype=torch.float64)
-    for heat in ([1.0] * 6, [0.0] * 6, [-1.0] * 6, [math.inf] * 6, [1e-30] * 6):
+    for heat in ([1.0] * 6, [0.0] * 6, [-1.0] * 6, [math.inf] * 6, [1e-30] * 6, [1e-38] * 6, [3e38] * 6):
         check_verify(pkg, logits, drafts, uniforms, list(range(0, 13, 2)), heat=heat)
         check_verify(pkg, logits, drafts, uniforms * 0, [0, 4, 8, 12], heat=heat[:3])
 
