@@ -17,7 +17,6 @@
 namespace fb2 {
 
 constexpr int PG_SEQS = 16384;  // sequences: three words each in shared memory
-constexpr int PG_RUN = 4;       // neighbouring rows of a thread: one search, one store
 
 struct PagesView {
     int* table;  // [n_seqs], rows `stride` apart
@@ -76,8 +75,10 @@ FB2_DEV void cluster_sync() {
 
 }  // namespace pg
 
-// gridDim.x: the CTAs of the one cluster; `vec`: slots and positions begin on 16 bytes
-template <int THREADS>
+// gridDim.x: the CTAs of the one cluster; RUN: neighbouring rows of a thread, 1 or 4 (one
+// search, one store where there are many rows; where there are few, a thread's rows would
+// be of different sequences); `vec`: slots and positions begin on 16 bytes
+template <int THREADS, int RUN>
 __global__ void __launch_bounds__(THREADS, 1)
     k_pages_extend(PagesView p, const int* counts, int max_rows, int* starts, int* prefix, int* slots, int* positions, bool vec) {
     extern __shared__ int pg_smem[];
@@ -128,11 +129,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
     }
     const int mask = (1 << p.shift) - 1;
-    for (int r0 = (rank * THREADS + tid) * PG_RUN; r0 < max_rows; r0 += ranks * THREADS * PG_RUN) {
-        int slot[PG_RUN], pos[PG_RUN];
+    for (int r0 = (rank * THREADS + tid) * RUN; r0 < max_rows; r0 += ranks * THREADS * RUN) {
+        int slot[RUN], pos[RUN];
         int b = -1, end = r0, last = -1, page = -1;  // the sequence of the row before, where it ends; its last page
 #pragma unroll
-        for (int i = 0; i < PG_RUN; i++) {
+        for (int i = 0; i < RUN; i++) {
             const int r = r0 + i;
             slot[i] = -1, pos[i] = 0;
             if (r >= total) continue;
@@ -156,13 +157,16 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
             if ((unsigned)page < (unsigned)p.n_pages) slot[i] = (page << p.shift) + within;
         }
-        if (vec && r0 + PG_RUN <= max_rows) {
-            *reinterpret_cast<int4*>(slots + r0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
-            *reinterpret_cast<int4*>(positions + r0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
-        } else {
-            for (int i = 0; i < PG_RUN; i++)
-                if (r0 + i < max_rows) slots[r0 + i] = slot[i], positions[r0 + i] = pos[i];
+        if constexpr (RUN == 4) {
+            if (vec && r0 + 4 <= max_rows) {
+                *reinterpret_cast<int4*>(slots + r0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+                *reinterpret_cast<int4*>(positions + r0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+                continue;
+            }
         }
+#pragma unroll
+        for (int i = 0; i < RUN; i++)
+            if (r0 + i < max_rows) slots[r0 + i] = slot[i], positions[r0 + i] = pos[i];
     }
 }
 

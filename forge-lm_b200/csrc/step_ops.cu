@@ -85,11 +85,11 @@ int32_t fb2_pages_extend(const fb2_pages* p, const int32_t* counts, int32_t max_
                            positions, vec);
         };
         int ranks = 1;
-        while (ranks < 8 && max_rows > 1024 * PG_RUN * ranks) ranks *= 2;
-        if (v.n_seqs <= 256 && max_rows <= 256 * PG_RUN)
-            launch(k_pages_extend<256>, 256, 1);
+        while (ranks < 8 && max_rows > 1024 * 4 * ranks) ranks *= 2;
+        if (v.n_seqs <= 256 && max_rows <= 1024)
+            launch(k_pages_extend<256, 1>, 256, 1);
         else
-            launch(k_pages_extend<1024>, 1024, ranks);
+            launch(k_pages_extend<1024, 4>, 1024, ranks);
     });
 }
 
