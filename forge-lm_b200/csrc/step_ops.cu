@@ -81,11 +81,12 @@ int32_t fb2_pages_extend(const fb2_pages* p, const int32_t* counts, int32_t max_
         const bool vec = aligned(slots, 16) && aligned(positions, 16);
         auto launch = [&](auto kernel, int threads, int ranks) {
             opt_in_smem((const void*)kernel, 12 * PG_SEQS);
+            if (ranks > 8) CK(cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
             launch_cluster(kernel, dim3(ranks), threads, 12 * v.n_seqs, ranks, false, stream, v, counts, max_rows, starts, prefix_lens, slots,
                            positions, vec);
         };
         int ranks = 1;
-        while (ranks < 8 && max_rows > 1024 * 4 * ranks) ranks *= 2;
+        while (ranks < 16 && max_rows > 1024 * 4 * ranks) ranks *= 2;
         if (v.n_seqs <= 256 && max_rows <= 1024)
             launch(k_pages_extend<256, 1>, 256, 1);
         else

@@ -123,13 +123,18 @@ FB2_DEV double widen(float v) {
 // series to t^3 (t^4 / 24 < 2^-50).  0 where it falls below 2^-1000.
 struct Heat {
     double cold;  // 1024 log2(e) / T
-    float near;   // log2(e) / T, not 0
     double top;
-    float top32;
+    float cut;  // below: 0
+    FB2_DEV void at(float t) {
+        top = widen(t);
+        cut = fmaxf(t - (float)(1000.0 * 1024 / cold), -3.402823466e38f);  // (-inf is below)
+    }
+    // BITS: of a logit's type; 16-bit ones leave the low half of a double 0
+    template <int BITS>
     FB2_DEV double weight(float l, const double* powers) const {
-        const bool none = (l - top32) * near < -1000.f;  // (-inf too)
+        const bool none = l < cut;
         const double magic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the nearest whole number
-        const double d = widen(l) - top, high = fma(d, cold, magic), t = fma(d, cold, magic - high);
+        const double wide = widen(l), d = (BITS == 32 ? wide : __hiloint2double(__double2hiint(wide), 0)) - top, high = fma(d, cold, magic), t = fma(d, cold, magic - high);
         const int n = __double2loint(high);
         constexpr double u = 6.7690154351557159e-4;  // ln 2 / 1024
         double e = fma(t, u * u * u / 6, u * u / 2);
@@ -174,18 +179,17 @@ FB2_DEV int pick(F part, int n, double target, double& passed) {
 }
 // log2(e) / T, T > 0; not 0 for T = inf, as -inf times it has to be -inf
 FB2_DEV float near_of(float heat) { return fmaxf(1.44269504088896341f / fmaxf(heat, VF_COLD), 1e-44f); }
-// The whole row's of its parts
-FB2_DEV VerifyRow joined(const VerifyRow* parts, int n, float near) {
-    VerifyRow all = parts[0];
-#pragma unroll 1
-    for (int k = 1; k < n; k++) {
-        const VerifyRow r = parts[k];
-        if (r.best >= 0 && (all.best < 0 || r.top > all.top || (r.top == all.top && r.best < all.best))) all.best = r.best;
-        const float top = fmaxf(all.top, r.top);
-        all.sum = all.sum * (double)ex2((all.top - top) * near) + r.sum * (double)ex2((r.top - top) * near);
-        all.top = top;
+// The whole row's of its parts, which VF_RANKS neighbouring lanes have one each of
+FB2_DEV VerifyRow joined(VerifyRow r, float near) {
+#pragma unroll
+    for (int o = 1; o < VF_RANKS; o *= 2) {
+        const VerifyRow s{__shfl_xor_sync(0xffffffffu, r.sum, o), __shfl_xor_sync(0xffffffffu, r.top, o), __shfl_xor_sync(0xffffffffu, r.best, o)};
+        if (s.best >= 0 && (r.best < 0 || s.top > r.top || (s.top == r.top && s.best < r.best))) r.best = s.best;
+        const float top = fmaxf(r.top, s.top);
+        r.sum = r.sum * (double)ex2((r.top - top) * near) + s.sum * (double)ex2((s.top - top) * near);
+        r.top = top;
     }
-    return all;
+    return r;
 }
 // The sequence of a row: the last b with starts[b] <= row, by all lanes.
 FB2_DEV int owner(const int* starts, int n, int row) {
@@ -325,7 +329,6 @@ __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
     const bool greedy = !(heat > 0.f);
     vf::Heat at_heat;
     at_heat.cold = greedy ? 0.0 : 1024 * 1.4426950408889634074 / (double)heat;
-    at_heat.near = fmaxf((float)(at_heat.cold / 1024), 1e-44f);
     const float near = vf::near_of(greedy ? 1.f : heat);
     const T* logits = (const T*)a.logits;
     pdl_wait();  // the rows' sums, and the outputs' memory
@@ -335,7 +338,13 @@ __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
         if (rank == 0 && tid == 0) a.counts[b] = 0;
         return;
     }
-    for (int i = tid; i < n; i += VW_THREADS) s_row[i] = vf::joined(a.rows + (long long)(first + i) * a.parts, a.parts, near);
+    for (int i0 = 0; i0 < n; i0 += VW_THREADS / VF_RANKS) {
+        const int i = i0 + tid / VF_RANKS, k = tid % VF_RANKS;
+        VerifyRow r{0.0, -3.402823466e38f, -1};
+        if (i < n && k < a.parts) r = a.rows[(long long)(first + i) * a.parts + k];
+        r = vf::joined(r, near);
+        if (i < n && k == 0) s_row[i] = r;
+    }
     __syncthreads();  // they and the table
     // a draft's weight at its parent, and what it is held against
     for (int i = 1 + tid; i < n; i += VW_THREADS) {
@@ -355,8 +364,8 @@ __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
                 mass = token == r.best;
             else {
                 vf::Heat h = at_heat;
-                h.top32 = r.top, h.top = vf::widen(r.top);
-                mass = h.weight(l, s_powers);
+                h.at(r.top);
+                mass = h.template weight<8 * sizeof(T)>(l, s_powers);
             }
             if (a.probs) limit *= q;
         }
@@ -388,7 +397,7 @@ __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
             for (int j = 0; j < N; j++) qv[j] = id + STEP * j < end ? __ldg(q + id + STEP * j) : 0.f;
         }
 #pragma unroll
-        for (int j = 0; j < N; j++) m[j] = at_heat.weight(l[j], s_powers);
+        for (int j = 0; j < N; j++) m[j] = at_heat.template weight<8 * sizeof(T)>(l[j], s_powers);
         if (q) {
 #pragma unroll
             for (int j = 0; j < N; j++) m[j] = vf::positive(fma(m[j], scale, -vf::widen(qv[j])));
@@ -458,7 +467,7 @@ __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
         const int node = s_at, rejected = s_rejected;
         const VerifyRow r = s_row[node];
         p = logits + (first + node) * a.logits_row;
-        at_heat.top32 = r.top, at_heat.top = vf::widen(r.top);
+        at_heat.at(r.top);
         if (state == WALK && s_ask < 0) {
             if (greedy || !vf::proper(r.sum)) {  // the whole cluster
                 if (rank == 0 && tid == 0) {
@@ -509,6 +518,7 @@ __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
         total = vf::warp_sum(lane < ranks ? vf::peek(sums, lane) : 0.0);
         if (state == WALK) {
             exact = total, known = node;
+            if (s_ask < 0) state = DRAW;
         } else if (total > 0.0 || state == DRAW_ALL) {
             break;
         } else {  // nothing is left: the row as if nothing had been rejected
