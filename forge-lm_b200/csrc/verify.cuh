@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(VF_THREADS) k_verify_rows(VerifyArgs a) {
         return s.x + s.y;
     };
     const uint4* body = reinterpret_cast<const uint4*>(p + head);
-    constexpr int M = 4;  // loads in flight
+    constexpr int M = 2;  // loads in flight (4: 2 us more for 289 rows x 50257, fp16)
     for (int i0 = p0 + tid; i0 < p1; i0 += M * VF_THREADS) {
         uint4 w[M];
 #pragma unroll
