@@ -34,13 +34,18 @@ void launch_cluster(void (*kernel)(P...), dim3 grid, int threads, int smem, int 
     cfg.dynamicSmemBytes = smem;
     cfg.stream = (cudaStream_t)stream;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = early ? 2 : 1;
+    if (cluster > 1) {
+        cudaLaunchAttribute& a = attr[cfg.numAttrs++];
+        a.id = cudaLaunchAttributeClusterDimension;
+        a.val.clusterDim.x = cluster;
+        a.val.clusterDim.y = a.val.clusterDim.z = 1;
+    }
+    if (early) {
+        cudaLaunchAttribute& a = attr[cfg.numAttrs++];
+        a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        a.val.programmaticStreamSerializationAllowed = 1;
+    }
     CK(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
 }
 
@@ -123,19 +128,22 @@ template <class T, class X>
 void launch_norm(const NormArgs& a, bool vec, cudaStream_t stream) {
     // threads of a row: few values each where rows are few, else up to 32
     const bool few = a.rows <= 4 * 148;
-    if (a.dim <= 256)
+    const int dim = a.dim;
+    if (dim <= 256)
         launch_norm<T, X, 32, 1>(a, vec, stream);
-    else if (a.dim <= 1024 && few)
+    else if (dim <= 1024 && few)
         launch_norm<T, X, 128, 1>(a, vec, stream);
-    else if (a.dim <= 1024)
+    else if (dim <= 1024)
         launch_norm<T, X, 32, 4>(a, vec, stream);
-    else if (a.dim <= 4096 && few)
+    else if (dim <= 4096 && few)
         launch_norm<T, X, 512, 1>(a, vec, stream);
-    else if (a.dim <= 4096)
+    else if (dim <= 2048)
+        launch_norm<T, X, 64, 4>(a, vec, stream);
+    else if (dim <= 4096)
         launch_norm<T, X, 128, 4>(a, vec, stream);
-    else if (a.dim <= 8192)
+    else if (dim <= 8192)
         launch_norm<T, X, 256, 4>(a, vec, stream);
-    else if (a.dim <= 16384)
+    else if (dim <= 16384)
         launch_norm<T, X, 512, 4>(a, vec, stream);
     else
         launch_norm<T, X, 1024, 4>(a, vec, stream);
@@ -167,7 +175,7 @@ int32_t fb2_residual_norm(const fb2_norm* n, void* stream) {
              "sum_row_stride and y_row_stride must be at least dim");
         need(!n->device_codes || (aligned(n->device_codes, 16) && (!many || (n->code_row_stride >= n->dim && n->code_row_stride % 16 == 0))),
              "rows of codes must begin on 16 bytes and not overlap");
-        bool vec = n->dim % NORM_E == 0;
+        bool vec = n->dim % NORM_E == 0;  // rows that begin on 16 bytes throughout
         auto runs = [&](const void* p, int64_t row, size_t size) {
             if (p && (!aligned(p, 16) || (many && row * (int64_t)size % 16))) vec = false;
         };
@@ -202,20 +210,32 @@ int32_t fb2_quantise_rows(int32_t n_rows, int32_t dim, const void* x, int32_t dt
         need(aligned(x, es) && aligned(scales, 4), "a tensor is not aligned to its element size");
         need(aligned(codes, 16) && (n_rows == 1 || (code_row >= dim && code_row % 16 == 0)),
              "rows of codes must begin on 16 bytes and not overlap");
-        const bool vec = dim % NORM_E == 0 && aligned(x, 16) && (n_rows == 1 || x_row * es % 16 == 0);
+        const bool vec = aligned(x, 16) && dim % NORM_E == 0 && (n_rows == 1 || x_row * es % 16 == 0);
         with_type(dtype, [&](auto t) {
             using T = decltype(t);
-            auto launch = [&](auto kernel, int threads) {
-                kernel<<<n_rows, threads, 0, (cudaStream_t)stream>>>((const T*)x, x_row, dim, (signed char*)codes, code_row, scales);
+            auto launch = [&](auto threads, auto pieces) {
+                constexpr int G = decltype(threads)::value, NJ = decltype(pieces)::value, rows = G == 32 ? 4 : 1;
+                auto kernel = vec ? k_quantise_rows<T, G, NJ, true> : k_quantise_rows<T, G, NJ, false>;
+                kernel<<<(unsigned)(((int64_t)n_rows + rows - 1) / rows), G == 32 ? 128 : G, 0, (cudaStream_t)stream>>>(
+                    (const T*)x, x_row, n_rows, dim, (signed char*)codes, code_row, scales);
             };
-            if (dim <= 1024)
-                launch(vec ? k_quantise_rows<T, 128, 1, true> : k_quantise_rows<T, 128, 1, false>, 128);
+            const bool few = n_rows <= 4 * 148;
+            if (dim <= 256)
+                launch(std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{});
+            else if (dim <= 1024 && !few)
+                launch(std::integral_constant<int, 32>{}, std::integral_constant<int, 4>{});
+            else if (dim <= 1024)
+                launch(std::integral_constant<int, 128>{}, std::integral_constant<int, 1>{});
+            else if (dim <= 2048)
+                launch(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
             else if (dim <= 4096)
-                launch(vec ? k_quantise_rows<T, 128, 4, true> : k_quantise_rows<T, 128, 4, false>, 128);
+                launch(std::integral_constant<int, 128>{}, std::integral_constant<int, 4>{});
+            else if (dim <= 8192)
+                launch(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
             else if (dim <= 16384)
-                launch(vec ? k_quantise_rows<T, 512, 4, true> : k_quantise_rows<T, 512, 4, false>, 512);
+                launch(std::integral_constant<int, 512>{}, std::integral_constant<int, 4>{});
             else
-                launch(vec ? k_quantise_rows<T, 512, 0, true> : k_quantise_rows<T, 512, 0, false>, 512);
+                launch(std::integral_constant<int, 512>{}, std::integral_constant<int, 0>{});
         });
         launched();
     });

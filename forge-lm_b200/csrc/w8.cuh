@@ -11,7 +11,8 @@
 // k_w8_rows: up to 4 rows of x, on the warps' dot products, quantised on the way.
 // k_w8_few: up to 128 rows of x to a tile, as the N side of the tiles, the weights
 // as the M side: each weight is read once.  A cluster shares a tile's inputs where
-// there are fewer tiles than SMs.
+// there are fewer tiles than SMs.  64 x 8192 x 28672 46 us (5.1 TB/s of weights), 61 x 1024 x
+// 4096 6.3 us, of which the products are a small part.
 // k_w8_many: 256 rows of x by 256 outputs, a pair of CTAs to a tile.
 // Every wait is bounded (2 s); on expiry a CTA stops, waits (bounded) for its
 // copies and MMAs in flight, frees its tensor memory, and its rows of y are NaN.
@@ -257,7 +258,9 @@ __global__ void __launch_bounds__(W8_THREADS, 2)
 // lane takes its inputs of them (16 bytes for each row and piece of 512 inputs of a warp)
 // into registers and the weights of one output after another against them, W8R_AHEAD
 // pieces in flight.  `per_k` warps share an output's inputs; the sums meet in shared
-// memory as integers.  The weights' bytes bound it.
+// memory as integers.  The weights' bytes bound it: 1 x 8192 x 28672, bf16, 41 us, 5.7 TB/s
+// (on tcgen05 tiles after a launch for the codes 53); 1 x 768 x 2304, fp32, 4.1 us, a
+// launch and a chain of loads (7.1).
 constexpr int W8R_THREADS = 512, W8R_WARPS = W8R_THREADS / 32, W8R_AHEAD = 8;
 constexpr int W8R_SUMS = 3200;       // sums of a CTA: outputs times rows (with the codes below 48 KB)
 constexpr int W8R_CODES = 32 * 1024;  // bytes of x's codes: what a lane's registers take of them
@@ -408,8 +411,10 @@ __global__ void __launch_bounds__(W8R_THREADS, w8r_resident<X, ROWS, PIECES>)
 // ---- many rows -------------------------------------------------------------------------
 // A pair of CTAs (on the two SMs of a TPC) takes a tile of 256 rows of x by 256 outputs:
 // one MMA of both, whose A and B tiles lie half in each one's shared memory, so that a
-// stage brings 32 KB to an SM for the products that cost one SM by itself 48 KB; what
-// crosses from L2 bounds these tiles.
+// stage brings 32 KB to an SM for the products that cost one SM by itself 48 KB.  8192 x
+// 4096 x 14336 takes 336 us, 2.87 POP/s (354 with tiles of one CTA): the tensor pipe is
+// active for 77 % of the cycles, at the 1.64 GHz that the power limit leaves; the
+// operands, 64 bytes a cycle and SM at the pipe's full rate, are what it waits for.
 constexpr int W8M_N = 256, W8M_STAGE = 2 * W8_TILE, W8M_STAGES = 6;
 constexpr int W8M_SMEM = W8M_STAGES * W8M_STAGE + 1024;
 constexpr int W8M_GROUP = 8;  // tiles of rows that are walked together: what runs at a time shares operands in L2
