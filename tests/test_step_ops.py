@@ -92,7 +92,8 @@ class Pages:
 
 @gpu
 @pytest.mark.parametrize("seqs,width,pages,page,most", [(1, 1, 1, 8, 8), (1, 40, 50, 16, 300), (3, 7, 12, 8, 40), (33, 5, 100, 16, 200),
-                                                         (1024, 3, 2000, 8, 9000), (1500, 2, 900, 32, 4000), (16384, 1, 9000, 8, 30000)])
+                                                         (1024, 3, 2000, 8, 9000), (1500, 2, 900, 32, 4000), (16384, 1, 9000, 8, 30000), (40, 400, 12000, 8, 90000),
+                                                         (2, 9000, 17000, 8, 140001)])
 def test_pages_come_and_go(pkg, seqs, width, pages, page, most):
     rng = random.Random(seqs)
     own, want = pkg.PageTable.empty(seqs, width, pages, page), Pages(seqs, width, pages, page)
@@ -1144,3 +1145,48 @@ def test_step_refusals_of_the_c_entries(pkg):
     assert L.fb2_verify_drafts(None, None) == bad and L.fb2_verify_workspace(ver.pack(*base), None) == bad
     assert L.fb2_test_w8_withhold(-1, 5) == bad and L.fb2_test_w8_withhold(0, 0) == bad and L.fb2_test_w8_withhold(0, 3_000_000_000) == bad
     assert L.fb2_last_error() != b""
+
+
+@gpu
+def test_calls_of_two_streams_at_once(pkg):
+    """Nothing that one call writes is another's: the same calls on two streams, begun together again and again."""
+    g = gen(14)
+    linear = pkg.W8Linear.pack(normal(g, 700, 900))
+    weight = torch.ones(700, device="cuda")
+    logits, probs = normal(g, 40, 20000, dtype=torch.bfloat16), torch.softmax(normal(g, 40, 20000), 1)
+    drafts = torch.multinomial(probs, 1, generator=g).squeeze(1).to(torch.int32)
+    starts, uniforms = ints(list(range(0, 41, 5))), torch.rand(40, device="cuda", generator=g, dtype=torch.float64)
+    xs = [normal(g, n, 700, dtype=torch.float16) for n in (2, 60, 700)]
+
+    def calls():
+        made = []
+        for x in xs:
+            s, codes, scales = pkg.residual_norm(x, x, weight, quantise=True)
+            made += [s, linear(codes, scales=scales, dtype=torch.float16), linear(x)]
+        return made + list(pkg.verify_drafts(logits, drafts, uniforms, starts=starts, draft_probs=probs, max_nodes=5))
+
+    want = calls()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(calls())
+    torch.cuda.synchronize()
+    for rounds in got:
+        for made in rounds:
+            assert all(torch.equal(a, b) for a, b in zip(want, made))
+
+
+@gpu
+@pytest.mark.parametrize("vocab", [300001, 3000000])
+def test_verification_over_very_large_vocabularies(pkg, vocab):
+    """More ids than the parts of one pass have batches for, in rows of every alignment."""
+    g = gen(vocab)
+    logits = normal(g, 6, vocab + 7, dtype=torch.bfloat16)[:, 3:3 + vocab]
+    probs = torch.softmax(logits.float().roll(1, 0) + 0.5 * normal(g, 6, vocab), 1)
+    drafts = torch.multinomial(probs, 1, generator=g).squeeze(1).to(torch.int32)
+    uniforms = torch.rand(6, device="cuda", generator=g, dtype=torch.float64)
+    check_verify(pkg, logits, drafts, uniforms, [0, 3, 6], probs=probs, heat=[1.0, 0.7])
+    check_verify(pkg, logits, drafts, uniforms, [0, 3, 6], parents=[0, 0, 0, 0, 0, 1], heat=[1.5, 0.7])
