@@ -221,7 +221,7 @@ def check_norm(c, got, scale, kind, eps):
 @gpu
 @pytest.mark.parametrize("dtype,stream", [("fp32", "fp32"), ("bf16", "bf16"), ("bf16", "fp32"), ("fp16", "fp16"), ("fp16", "fp32")])
 @pytest.mark.parametrize("kind", ["layer", "rms"])
-@pytest.mark.parametrize("rows,dim", [(1, 768), (5, 64), (3, 1), (7, 257), (9, 1000), (2, 1025), (4, 4096), (3, 5001), (2, 16384), (2, 32767)])
+@pytest.mark.parametrize("rows,dim", [(1, 768), (5, 64), (3, 1), (7, 257), (9, 1000), (2, 1025), (4, 4096), (3, 5001), (2, 16384), (2, 32767), (2, 32768)])
 def test_residual_and_norm(pkg, dtype, stream, kind, rows, dim):
     g = gen(rows * dim)
     for post, gate, strided in ((False, None, False), (True, "rows", False), (True, "all", True), (False, "rows", True)):
