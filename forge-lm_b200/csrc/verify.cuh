@@ -19,7 +19,7 @@
 // read at the cost of 32-bit exponentials.
 //
 // 161 rows x 131071, bf16, of 32 sequences with draft probabilities: 47 us, 16 of them for
-// the rows (2.6 TB/s; some 12 instructions a logit bound it), the rest for the draws: two
+// the rows (2.6 TB/s; 10 instructions a logit and the waits between them), the rest for the draws: two
 // passes of some 35 instructions a logit where a draft was rejected (fp64 arithmetic
 // itself goes at 64 lanes a cycle and is a quarter of them).  Exponentials of CUDA's exp()
 // in fp64 for all rows: 184.  289 rows x 50257, fp16, 8 trees: 22 us (89); 5 rows x 16384: 12
