@@ -145,6 +145,42 @@ at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, int index) {
     return at::detail::empty_cuda(shape, type, c10::Device(c10::kCUDA, index), std::nullopt);
 }
 
+// A call's results.  Small ones come from one allocation (each takes the allocator half a
+// microsecond, a quarter of what a launch takes); large ones from their own, so that a
+// result that is dropped frees its memory.
+struct Results {
+    static constexpr int64_t kSmall = 64 * 1024, kAlign = 256;
+    struct Piece {
+        at::Tensor* to;
+        c10::SmallVector<int64_t, 2> shape;
+        at::ScalarType type;
+    };
+    c10::SmallVector<Piece, 4> pieces;
+    void add(at::Tensor& to, std::initializer_list<int64_t> shape, at::ScalarType type) { pieces.push_back({&to, shape, type}); }
+    void make(int index) {
+        int64_t all = 0;
+        auto bytes = [](const Piece& p) {
+            int64_t n = (int64_t)c10::elementSize(p.type);
+            for (int64_t s : p.shape) n *= s;
+            return (n + kAlign - 1) / kAlign * kAlign;
+        };
+        for (const Piece& p : pieces) all += bytes(p);
+        if (all > kSmall || pieces.size() == 1) {
+            for (const Piece& p : pieces) *p.to = empty(p.shape, p.type, index);
+            return;
+        }
+        const at::Tensor base = empty({all}, at::kByte, index);
+        int64_t offset = 0;
+        for (const Piece& p : pieces) {
+            at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), c10::scalarTypeToTypeMeta(p.type));
+            t.unsafeGetTensorImpl()->set_sizes_contiguous(p.shape);
+            t.unsafeGetTensorImpl()->set_storage_offset(offset / (int64_t)c10::elementSize(p.type));
+            *p.to = std::move(t);
+            offset += bytes(p);
+        }
+    }
+};
+
 template <class H>
 void destroy(PyObject* capsule) {
     delete static_cast<H*>(PyCapsule_GetPointer(capsule, H::kName));
@@ -553,8 +589,11 @@ PyObject* pages_extend(PyObject*, PyObject* const* args, Py_ssize_t count) {
         need(rows >= 0, "max_rows must not be negative");
         const fb2_pages p = h.now();
         OnDevice on(h.index);
-        at::Tensor starts = empty({(int64_t)p.n_seqs + 1}, at::kInt, h.index), prefix = empty({p.n_seqs}, at::kInt, h.index);
-        at::Tensor slots = empty({rows}, at::kInt, h.index), positions = empty({rows}, at::kInt, h.index);
+        at::Tensor starts, prefix, slots, positions;
+        Results made;
+        made.add(starts, {(int64_t)p.n_seqs + 1}, at::kInt), made.add(prefix, {p.n_seqs}, at::kInt);
+        made.add(slots, {rows}, at::kInt), made.add(positions, {rows}, at::kInt);
+        made.make(h.index);
         status(fb2_pages_extend(&p, data<int32_t>(counts), rows, data<int32_t>(&starts), data<int32_t>(&prefix), data<int32_t>(&slots),
                                 data<int32_t>(&positions), on.stream()));
         changed(h.table), changed(h.lens), changed(h.n_free);
@@ -588,8 +627,10 @@ const at::Tensor& matrix(PyObject* o, const char* name, int64_t rows, int64_t di
     return t;
 }
 // rows of codes that begin on 16 bytes
+int64_t padded(int64_t dim) { return (dim + 15) / 16 * 16; }
 at::Tensor empty_codes(int64_t rows, int64_t dim, int index) {
-    return empty({rows, (dim + 15) / 16 * 16}, at::kChar, index).narrow(1, 0, dim);
+    at::Tensor t = empty({rows, padded(dim)}, at::kChar, index);
+    return padded(dim) == dim ? t : t.narrow(1, 0, dim);
 }
 
 PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t count) {
@@ -640,11 +681,14 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t count) {
         if (quantise < 0) throw Raised{};
         OnDevice on(index);
         at::Tensor sum, y, codes, scales;
-        if (h) sum = empty({rows, dim}, x.scalar_type(), index);
+        Results made;
+        if (h) made.add(sum, {rows, dim}, x.scalar_type());
         if (quantise)
-            codes = empty_codes(rows, dim, index), scales = empty({rows}, at::kFloat, index);
+            made.add(codes, {rows, padded(dim)}, at::kChar), made.add(scales, {rows}, at::kFloat);
         else
-            y = empty({rows, dim}, type, index);
+            made.add(y, {rows, dim}, type);
+        made.make(index);
+        if (quantise && padded(dim) != dim) codes = codes.narrow(1, 0, dim);
         n.device_h = data<void>(h);
         n.device_x = x.data_ptr();
         n.device_gate = data<void>(gate);
@@ -659,7 +703,7 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t count) {
         n.h_row_stride = h ? h->stride(0) : 0;
         n.x_row_stride = x.stride(0);
         n.sum_row_stride = n.y_row_stride = dim;
-        n.code_row_stride = (dim + 15) / 16 * 16;
+        n.code_row_stride = padded(dim);
         n.n_rows = small(rows, "rows");
         n.dim = small(dim, "dim");
         if (rows) status(fb2_residual_norm(&n, on.stream()));
@@ -844,8 +888,10 @@ PyObject* verify(PyObject*, PyObject* const* args, Py_ssize_t count) {
         v.vocab = small(vocab, "vocab");
         v.max_nodes = (int32_t)nodes;
         OnDevice on(index);
-        at::Tensor tokens = empty({seqs, nodes}, at::kInt, index), path = empty({seqs, nodes}, at::kInt, index),
-                   counts = empty({seqs}, at::kInt, index), work;
+        at::Tensor tokens, path, counts, work;
+        Results made;
+        made.add(tokens, {seqs, nodes}, at::kInt), made.add(path, {seqs, nodes}, at::kInt), made.add(counts, {seqs}, at::kInt);
+        made.make(index);
         status(fb2_verify_workspace(&v, &v.workspace_bytes));
         if (v.workspace_bytes) work = empty({v.workspace_bytes}, at::kByte, index);
         v.device_workspace = v.workspace_bytes ? work.data_ptr() : nullptr;

@@ -1190,3 +1190,24 @@ def test_verification_over_very_large_vocabularies(pkg, vocab):
     uniforms = torch.rand(6, device="cuda", generator=g, dtype=torch.float64)
     check_verify(pkg, logits, drafts, uniforms, [0, 3, 6], probs=probs, heat=[1.0, 0.7])
     check_verify(pkg, logits, drafts, uniforms, [0, 3, 6], parents=[0, 0, 0, 0, 0, 1], heat=[1.5, 0.7])
+
+
+@gpu
+def test_results_are_apart(pkg):
+    """Small results come from one allocation: none overlaps another, and what is written into one
+    changes nothing else and only its own version."""
+    g = gen(3)
+    x, w = normal(g, 3, 100, dtype=torch.bfloat16), torch.ones(100, device="cuda")
+    pages = pkg.PageTable.empty(3, 4, 12, 8)
+    u = torch.rand(3, device="cuda", generator=g, dtype=torch.float64)
+    made = [pkg.residual_norm(x, x, w), pkg.residual_norm(x, x, w, quantise=True), pages.extend(ints([3, 9, 1]), 20),
+            pkg.verify_drafts(normal(g, 3, 500), ints([1, 2, 3]), u, starts=ints([0, 2, 3]))]
+    for results in made:
+        before = [t.clone() for t in results]
+        spans = sorted((t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * t.stride(0) + t[0].numel()) * t.element_size()) for t in results)
+        assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:])) and all(t.data_ptr() % 16 == 0 for t in results)
+        for i, t in enumerate(results):
+            versions = [r._version for r in results]
+            t.add_(1)
+            assert [r._version - v for r, v in zip(results, versions)] == [int(i == k) for k in range(len(results))]
+            assert all(torch.equal(r, b) for k, (r, b) in enumerate(zip(results, before)) if k > i)
