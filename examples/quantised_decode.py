@@ -1,14 +1,17 @@
-"""Greedy generation with the serving operators: 4-bit projections, a paged
-K/V cache that is quantised as it is written, attention of drafted trees over
-it, and penalties and a grammar's mask on the logits.
+"""Greedy generation with the serving operators: projections with 4-bit weights
+or in 8-bit integers, a paged K/V cache that is quantised as it is written,
+attention of drafted trees over it, and penalties and a grammar's mask on the
+logits.
 
     python examples/quantised_decode.py [--cache int4] [--draft 0] ...
 
 Weights are the seeded initialisation of a GPT of the given size.  Each step
 runs the last token of every sequence and two drafted continuations, taken
 from where the sequence had the same token before; the greedy path through
-them is kept.  torch computes the embeddings, norms and GELU around the
-operators.
+them is kept.  torch computes the embeddings and GELU around the operators, and
+with 4-bit weights the norms; products in 8-bit integers take their rows from
+residual_norm, which adds a block's output to the stream and norms it for the
+next.
 """
 from __future__ import annotations
 
@@ -30,18 +33,23 @@ def _ints(values):
 
 
 class QuantisedGpt:
-    """The GPT of a ModelConfig with W4Linear projections and one QuantKvCache
-    per layer; sequence s owns pages s * pages_per_seq onwards."""
+    """The GPT of a ModelConfig with W4Linear or W8Linear projections and one
+    QuantKvCache per layer; sequence s owns pages s * pages_per_seq onwards."""
 
     def __init__(self, cfg, params, seqs: int, cache: str = "int8", group: int = 64, page: int = 32,
-                 dtype=torch.bfloat16, spare: int = 16):
-        self.cfg, self.dtype, self.page = cfg, dtype, page
+                 dtype=torch.bfloat16, spare: int = 16, products: str = "int4"):
+        self.cfg, self.dtype, self.page, self.products = cfg, dtype, page, products
         p = {n: torch.from_numpy(a).cuda() for n, a in zip(forge.param_names(cfg), params)}
-        self.norms = {n: t.to(dtype) for n, t in p.items() if ".ln" in n or n.startswith("ln_f")}
+        eight = products == "int8"
+
+        def pack(w, bias=None):
+            return forge.W8Linear.pack(w, bias) if eight else forge.W4Linear.pack(w, group, bias)
+
+        self.norms = {n: t if eight else t.to(dtype) for n, t in p.items() if ".ln" in n or n.startswith("ln_f")}
         self.tok, self.pos = p["tok_emb"].to(dtype), p["pos_emb"].to(dtype)
-        self.layers = [{n: forge.W4Linear.pack(p[f"blocks.{i}.{n}.w"], group, p[f"blocks.{i}.{n}.b"])
+        self.layers = [{n: pack(p[f"blocks.{i}.{n}.w"], p[f"blocks.{i}.{n}.b"])
                         for n in ("attn.qkv", "attn.proj", "mlp.fc", "mlp.proj")} for i in range(cfg.n_layers)]
-        self.head = forge.W4Linear.pack(p["tok_emb"].t().contiguous(), group)
+        self.head = pack(p["tok_emb"].t().contiguous())
         pages = -(-(cfg.context_length + spare) // page)  # a step's drafted rows may pass the last position
         self.table = torch.arange(seqs * pages, dtype=torch.int32, device="cuda").view(seqs, pages)
         self.caches = [forge.QuantKvCache.empty(seqs * pages, page, cfg.n_heads, cfg.head_dim, cache)
@@ -60,6 +68,8 @@ class QuantisedGpt:
         cfg, rows = self.cfg, len(tokens)
         slots, prefix, starts = _ints(slots), _ints(prefix), _ints(starts)
         x = self.tok[_ints(tokens).long()] + self.pos[_ints(positions).long()]
+        if self.products == "int8":
+            return self._logits8(x, slots, prefix, starts, mask, max_nodes)
         for i, layer in enumerate(self.layers):
             qkv = layer["attn.qkv"](self._norm(x, f"blocks.{i}.ln1")).view(rows, 3, cfg.n_heads, cfg.head_dim)
             self.caches[i].write(qkv[:, 1], qkv[:, 2], slots)
@@ -68,6 +78,25 @@ class QuantisedGpt:
             h = layer["mlp.fc"](self._norm(x, f"blocks.{i}.ln2"))
             x = x + layer["mlp.proj"](torch.nn.functional.gelu(h, approximate="tanh"))
         return self.head(self._norm(x, "ln_f"))
+
+    def _logits8(self, x, slots, prefix, starts, mask, max_nodes):
+        """The blocks in 8-bit integers: each residual_norm adds the output h of
+        the block before to the stream and makes the next product's rows."""
+        cfg, h = self.cfg, None
+
+        def enter(linear, name):
+            nonlocal x
+            x, codes, scales = forge.residual_norm(h, x, self.norms[name + ".w"], self.norms[name + ".b"], quantise=True)
+            return linear(codes, scales=scales, dtype=self.dtype)
+
+        for i, layer in enumerate(self.layers):
+            qkv = enter(layer["attn.qkv"], f"blocks.{i}.ln1").view(len(x), 3, cfg.n_heads, cfg.head_dim)
+            self.caches[i].write(qkv[:, 1], qkv[:, 2], slots)
+            out, _ = self.caches[i].attend(qkv[:, 0], self.table, prefix, starts=starts, mask=mask, max_nodes=max_nodes)
+            h = layer["attn.proj"](out.reshape(len(x), -1))
+            f = enter(layer["mlp.fc"], f"blocks.{i}.ln2")
+            h = layer["mlp.proj"](torch.nn.functional.gelu(f, approximate="tanh"))
+        return enter(self.head, "ln_f")
 
     def move(self, seq: int, sources: list[int], targets: list[int]) -> None:
         """Copies cache rows as they are (the kept drafted rows to their places)."""
@@ -170,6 +199,7 @@ def main(argv=None):
     ap.add_argument("--vocab", type=int, default=16384)
     ap.add_argument("--context", type=int, default=1024)
     ap.add_argument("--cache", choices=("int8", "int4"), default="int8")
+    ap.add_argument("--products", choices=("int4", "int8"), default="int4", help="4-bit weights, or 8-bit integers throughout")
     ap.add_argument("--group", type=int, choices=(32, 64, 128), default=64)
     ap.add_argument("--seqs", type=int, default=4)
     ap.add_argument("--prompt", type=int, default=64, help="tokens of a prompt")
@@ -180,7 +210,7 @@ def main(argv=None):
     if not 0 <= args.draft <= 7:
         ap.error("--draft must be 0 to 7")
     cfg = forge.ModelConfig(args.vocab, args.context, args.d_model, args.layers, args.heads)
-    model = QuantisedGpt(cfg, forge.init_params(cfg, args.seed), args.seqs, args.cache, args.group)
+    model = QuantisedGpt(cfg, forge.init_params(cfg, args.seed), args.seqs, args.cache, args.group, products=args.products)
     gen = torch.Generator().manual_seed(args.seed)
     prompts = torch.randint(0, args.vocab, (args.seqs, args.prompt), generator=gen).tolist()
     out, steps = generate(model, prompts, args.new, args.draft)

@@ -1211,3 +1211,31 @@ def test_results_are_apart(pkg):
             t.add_(1)
             assert [r._version - v for r, v in zip(results, versions)] == [int(i == k) for k in range(len(results))]
             assert all(torch.equal(r, b) for k, (r, b) in enumerate(zip(results, before)) if k > i)
+
+
+@gpu
+@pytest.mark.parametrize("cache", ["int8", "int4"])
+def test_example_of_a_decoder_in_8_bit_integers(pkg, cache):
+    """It runs, keeps to the grammar, and its logits are finite and do not hang on rows of other sequences."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "quantised_decode.py")
+    spec = importlib.util.spec_from_file_location("quantised_decode", path)
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    cfg = pkg.ModelConfig(512, 128, 128, 3, 4)
+    params = pkg.init_params(cfg, 5)
+
+    def model():
+        return ex.QuantisedGpt(cfg, params, 3, cache, products="int8")
+
+    words = torch.full((1, 16), -1, dtype=torch.int32, device="cuda")
+    words[0, 1] = 0  # not 32..63
+    out, steps = ex.generate(model(), [[1, 2, 3, 1, 2, 3], [7], [9, 8] * 20], 20, draft=4, allowed=words)
+    assert [len(t) for t in out] == [20] * 3 and 1 <= steps <= 20
+    assert all(0 <= x < 512 and not 32 <= x < 64 for t in out for x in t)
+    both, one = model(), model()
+    tokens = [5, 6, 7, 8, 9, 10]
+    logits = both.logits(tokens, [0, 1, 2, 0, 1, 2], both.slots(0, range(3)) + both.slots(1, range(3)), [0, 0, 0], [0, 3, 6, 6], max_nodes=3)
+    first = one.logits(tokens[:3], [0, 1, 2], one.slots(0, range(3)), [0, 0, 0], [0, 3, 3, 3], max_nodes=3)
+    assert logits.isfinite().all() and torch.equal(logits[:3], first)
