@@ -471,11 +471,12 @@ __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
             }
             __syncthreads();
         }
-        const int node = s_at, rejected = s_rejected;
+        // (here, behind the barrier: warp 0 writes them again in its next turn)
+        const int node = s_at, rejected = s_rejected, ask = s_ask;
         const VerifyRow r = s_row[node];
         p = logits + (first + node) * a.logits_row;
         at_heat.at(r.top);
-        if (state == WALK && s_ask < 0) {
+        if (state == WALK && ask < 0) {
             if (greedy || !vf::proper(r.sum)) {  // the whole cluster
                 if (rank == 0 && tid == 0) {
                     tokens[s_count - 1] = vf::proper(r.sum) ? r.best : -1;
@@ -525,7 +526,7 @@ __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
         total = vf::warp_sum(lane < ranks ? vf::peek(sums, lane) : 0.0);
         if (state == WALK) {
             exact = total, known = node;
-            if (s_ask < 0) state = DRAW;
+            if (ask < 0) state = DRAW;
         } else if (total > 0.0 || state == DRAW_ALL) {
             break;
         } else {  // nothing is left: the row as if nothing had been rejected

@@ -1239,3 +1239,47 @@ def test_example_of_a_decoder_in_8_bit_integers(pkg, cache):
     logits = both.logits(tokens, [0, 1, 2, 0, 1, 2], both.slots(0, range(3)) + both.slots(1, range(3)), [0, 0, 0], [0, 3, 6, 6], max_nodes=3)
     first = one.logits(tokens[:3], [0, 1, 2], one.slots(0, range(3)), [0, 0, 0], [0, 3, 3, 3], max_nodes=3)
     assert logits.isfinite().all() and torch.equal(logits[:3], first)
+
+
+@gpu
+@pytest.mark.parametrize("drawn", [False, True])
+def test_verification_asks_for_sums_all_along_a_path(pkg, drawn):
+    """Chains whose every test is next to equal, so that the walk goes on after each row's sum of 64 bits: to the
+    last node, or to a rejected one; in clusters of every size, with more CTAs than the GPU holds at once."""
+    g = gen(31)
+    for vocab, n, seqs in ((1000, 6, 300), (6000, 5, 40), (40000, 4, 12)):
+        logits = normal(g, seqs * n, vocab, dtype=torch.bfloat16)
+        drafts = torch.randint(0, vocab, (seqs * n,), device="cuda", generator=g).to(torch.int32)
+        p = torch.softmax(logits.double(), 1)
+        at = p[:-1].gather(1, drafts[1:].long().unsqueeze(1)).squeeze(1)
+        probs = None
+        if drawn:
+            probs = torch.softmax(normal(g, seqs * n, vocab), 1)
+            at = at / probs[1:].gather(1, drafts[1:].long().unsqueeze(1)).squeeze(1).double()
+        side = torch.full((seqs, n), 1 - 1e-12, dtype=torch.float64, device="cuda")
+        want = [n if b % 3 == 0 else 1 + b % (n - 1) for b in range(seqs)]  # tokens of each sequence
+        for b, w in enumerate(want):
+            if w < n:
+                side[b, w] = 1 + 1e-12
+        uniforms = torch.rand(seqs * n, device="cuda", generator=g, dtype=torch.float64)
+        uniforms[1:] = torch.where(torch.arange(1, seqs * n, device="cuda") % n == 0, uniforms[1:], at * side.flatten()[1:])
+        args = dict(starts=ints(list(range(0, seqs * n + 1, n))), draft_probs=probs, max_nodes=n)
+        first = pkg.verify_drafts(logits, drafts, uniforms, **args)
+        assert first[2].tolist() == want
+        some = 4 * n
+        check_verify(pkg, logits[:some], drafts[:some], uniforms[:some], list(range(0, some + 1, n)),
+                     probs=None if probs is None else probs[:some])
+        for _ in range(20):
+            assert all(torch.equal(a, b) for a, b in zip(first, pkg.verify_drafts(logits, drafts, uniforms, **args)))
+
+
+@gpu
+def test_verification_asks_for_sums_at_the_lowest_temperatures(pkg):
+    """Below 1e-30 every test asks for its row's sum: p is shared by the largest logits."""
+    g, rng = gen(32), random.Random(32)
+    logits, drafts, uniforms, starts, parents, _ = verify_case(g, rng, [9, 1, 17, 6], 5000, torch.float32, True)
+    logits = (logits * 0.5).round()
+    drafts = ints([int(r[0]) for r in logits.topk(1, 1).indices[[max(p, 0) + starts[sum(s <= i for s in starts) - 1] for i, p in enumerate(parents)]]])
+    for heat in (1e-31, 1e-36):
+        check_verify(pkg, logits, drafts, uniforms, starts, parents, heat=[heat] * 4)
+        check_verify(pkg, logits, drafts, uniforms, starts, heat=[heat] * 4)
