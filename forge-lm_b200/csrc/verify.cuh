@@ -127,14 +127,16 @@ FB2_DEV double widen(float v) {
 // exp((l - top) / T), l <= top, by a table and a polynomial (P. T. P. Tang,
 // Table-driven implementation of the exponential function, ACM TOMS 15, 1989):
 // 2^(n / 1024) from the table and the exponent, exp(t), |t| <= ln 2 / 2048, from its
-// series to t^3 (t^4 / 24 < 2^-50).  0 where it falls below 2^-1000.
+// series to t^3 (t^4 / 24 < 2^-50).  0 where it falls below 2^-1000: the first logit that does
+// not is found in 64 bits and rounded up (a limit rounded to nearest lets in logits whose
+// exponent is far below where T is less than the step between logits).
 struct Heat {
     double cold;  // 1024 log2(e) / T
     double top;
     float cut;  // below: 0
     FB2_DEV void at(float t) {
         top = widen(t);
-        cut = fmaxf(t - (float)(1000.0 * 1024 / cold), -3.402823466e38f);  // (-inf is below)
+        cut = fmaxf(__double2float_ru((double)t - 1000.0 * 1024 / cold), -3.402823466e38f);  // (-inf is below)
     }
     // BITS: of a logit's type; 16-bit ones leave the low half of a double 0
     template <int BITS>

@@ -1283,3 +1283,33 @@ def test_verification_asks_for_sums_at_the_lowest_temperatures(pkg):
     for heat in (1e-31, 1e-36):
         check_verify(pkg, logits, drafts, uniforms, starts, parents, heat=[heat] * 4)
         check_verify(pkg, logits, drafts, uniforms, starts, heat=[heat] * 4)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "fp16"])
+def test_verification_of_temperatures_next_to_a_logits_step(pkg, dtype):
+    """Temperatures down to far below the step between neighbouring logits: weights fall from 1 to
+    nothing (below 2^-1000) within a few steps, and none lies beyond."""
+    g, rng = gen(33), random.Random(33)
+    vocab, nodes, cases = 2500, 3, []
+    steps = torch.finfo(DTYPES[dtype]).eps
+    for top in (1500.0, 30.0, 10.0, 1.0, -40.0):
+        for heat in (1e-3, 1e-5, 1e-6, 1e-7, 1e-8, 1e-9, 3e-12):
+            cases.append((top, heat))
+    rows = nodes * len(cases)
+    logits = torch.empty((rows, vocab), dtype=torch.float64, device="cuda")
+    for i, (top, _) in enumerate(cases):
+        step = 2.0 ** math.floor(math.log2(abs(top))) * steps  # of the type at the largest logit
+        down = torch.randint(0, 13, (nodes, vocab), device="cuda", generator=g)
+        logits[nodes * i:nodes * (i + 1)] = top - step * down
+    logits = logits.to(DTYPES[dtype])
+    drafts = torch.randint(0, vocab, (rows,), device="cuda", generator=g).to(torch.int32)
+    drafts[1:] = torch.where(torch.rand(rows - 1, device="cuda", generator=g) < 0.7, logits[:-1].argmax(1), drafts[1:]).to(torch.int32)
+    starts, heats = list(range(0, rows + 1, nodes)), [h for _, h in cases]
+    parents = [i - 1 if rng.random() < 0.5 else 0 for _ in cases for i in range(nodes)]
+    for _ in range(3):
+        uniforms = torch.rand(rows, device="cuda", generator=g, dtype=torch.float64)
+        check_verify(pkg, logits, drafts, uniforms, starts, heat=heats)
+        check_verify(pkg, logits, drafts, uniforms, starts, parents=parents, heat=heats)
+        probs = torch.softmax(normal(g, rows, vocab), 1)
+        check_verify(pkg, logits, drafts, uniforms, starts, probs=probs, heat=heats)
