@@ -131,14 +131,22 @@ FB2_DEV double widen(float v) {
 // not is found in 64 bits and rounded up (a limit rounded to nearest lets in logits whose
 // exponent is far below where T is less than the step between logits).
 struct Heat {
-    double cold;  // 1024 log2(e) / T
+    double cold;  // 1024 log2(e) / T, of logits as `weight` takes them
     double top;
-    float cut;  // below: 0
-    FB2_DEV void at(float t) {
+    float cut;   // below: 0
+    bool small;  // logits are taken 2^100 times as large
+    FB2_DEV void at(float t, float heat) {
+        // T below 2^-70 and a top as small as what `widen` is off by may be next to it: logits go
+        // up, those that overflow are far below.  (Below a larger top every other logit is.)
+        small = heat < 0x1p-70f && fabsf(t) < 0x1p-20f;
+        const double by = small ? heat * 0x1p100 : (double)heat;
+        cold = 1024 * 1.4426950408889634074 / by;
+        t = scaled(t);
         top = widen(t);
-        cut = fmaxf(__double2float_ru((double)t - 1000.0 * 1024 / cold), -3.402823466e38f);  // (-inf is below)
+        cut = fmaxf(__double2float_ru((double)t - 1000 * 0.69314718055994530942 * by), -3.402823466e38f);  // (-inf is below)
     }
-    // BITS: of a logit's type; 16-bit ones leave the low half of a double 0
+    FB2_DEV float scaled(float l) const { return small ? l * 0x1p100f : l; }
+    // l: scaled; BITS: of a logit's type; 16-bit ones leave the low half of a double 0
     template <int BITS>
     FB2_DEV double weight(float l, const double* powers) const {
         const bool none = l < cut;
@@ -337,7 +345,6 @@ __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
     const float heat = a.heat(b);
     const bool greedy = !(heat > 0.f);
     vf::Heat at_heat;
-    at_heat.cold = greedy ? 0.0 : 1024 * 1.4426950408889634074 / (double)heat;
     const float near = vf::near_of(greedy ? 1.f : heat);
     const T* logits = (const T*)a.logits;
     pdl_wait();  // the rows' sums, and the outputs' memory
@@ -372,9 +379,9 @@ __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
             else if (greedy)
                 mass = token == r.best;
             else {
-                vf::Heat h = at_heat;
-                h.at(r.top);
-                mass = h.template weight<8 * sizeof(T)>(l, s_powers);
+                vf::Heat h;
+                h.at(r.top, heat);
+                mass = h.template weight<8 * sizeof(T)>(h.scaled(l), s_powers);
             }
             if (a.probs) limit *= q;
         }
@@ -404,6 +411,10 @@ __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
         if (q) {
 #pragma unroll
             for (int j = 0; j < N; j++) qv[j] = id + STEP * j < end ? __ldg(q + id + STEP * j) : 0.f;
+        }
+        if (at_heat.small) {
+#pragma unroll
+            for (int j = 0; j < N; j++) l[j] = at_heat.scaled(l[j]);
         }
 #pragma unroll
         for (int j = 0; j < N; j++) m[j] = at_heat.template weight<8 * sizeof(T)>(l[j], s_powers);
@@ -477,7 +488,7 @@ __global__ void __launch_bounds__(VW_THREADS, 2) k_verify_walk(VerifyArgs a) {
         const int node = s_at, rejected = s_rejected, ask = s_ask;
         const VerifyRow r = s_row[node];
         p = logits + (first + node) * a.logits_row;
-        at_heat.at(r.top);
+        at_heat.at(r.top, heat);
         if (state == WALK && ask < 0) {
             if (greedy || !vf::proper(r.sum)) {  // the whole cluster
                 if (rank == 0 && tid == 0) {

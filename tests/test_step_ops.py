@@ -1313,3 +1313,26 @@ def test_verification_of_temperatures_next_to_a_logits_step(pkg, dtype):
         check_verify(pkg, logits, drafts, uniforms, starts, parents=parents, heat=heats)
         probs = torch.softmax(normal(g, rows, vocab), 1)
         check_verify(pkg, logits, drafts, uniforms, starts, probs=probs, heat=heats)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_verification_of_tiny_logits_at_tiny_temperatures(pkg, dtype):
+    """Zeros of both signs and logits below the normal numbers, at temperatures about as small: as in fp64."""
+    g = gen(34)
+    vocab, nodes = 1500, 3
+    least = 2.0 ** -149 if dtype == "fp32" else 2.0 ** -133  # of the type
+    heats = [least, 3 * least, 1e-38, 3e-37, 1e-31, 1e-24, 1e-21, 1e-3]
+    rows = nodes * len(heats)
+    for step in (least, 1e-38, 1e-24):
+        logits = -step * torch.randint(0, 9, (rows, vocab), device="cuda", generator=g).double()
+        logits = logits.to(DTYPES[dtype])  # -0 among them
+        logits[:, ::7] = logits[:, ::7].abs() * 0
+        logits[:, 5::11] = -1e30
+        drafts = logits.argmax(1).roll(1).to(torch.int32)
+        for _ in range(3):
+            uniforms = torch.rand(rows, device="cuda", generator=g, dtype=torch.float64)
+            check_verify(pkg, logits, drafts, uniforms, list(range(0, rows + 1, nodes)), heat=heats)
+            check_verify(pkg, logits, drafts, uniforms, list(range(0, rows + 1, nodes)), parents=[-1, 0, 0] * len(heats), heat=heats)
+            check_verify(pkg, logits, drafts, uniforms, list(range(0, rows + 1, nodes)), heat=heats,
+                         probs=torch.softmax(normal(g, rows, vocab), 1))
