@@ -14,6 +14,9 @@
 // there are fewer tiles than SMs.  64 x 8192 x 28672 46 us (5.1 TB/s of weights), 61 x 1024 x
 // 4096 6.3 us, of which the products are a small part.
 // k_w8_many: 256 rows of x by 256 outputs, a pair of CTAs to a tile.
+// All of them may begin while the launch before still writes what they read: rows' codes and
+// scales come by TMA or past L1 (__ldcg), behind pdl_wait, and so do the weights' scales and
+// the bias; __ldg would say that they do not change while the kernel runs.
 // Every wait is bounded (2 s); on expiry a CTA stops, waits (bounded) for its
 // copies and MMAs in flight, frees its tensor memory, and its rows of y are NaN.
 #pragma once
@@ -181,7 +184,7 @@ __global__ void __launch_bounds__(W8_THREADS, 2)
     if (ranks == 1) {
         if (warp < 4) {
             const int o = o0 + 32 * quarter + lane;
-            const float ws = o < a.out ? __ldg(a.w_scales + o) : 0.f, bias = a.bias && o < a.out ? __ldg(a.bias + o) : 0.f;
+            const float ws = o < a.out ? __ldcg(a.w_scales + o) : 0.f, bias = a.bias && o < a.out ? __ldcg(a.bias + o) : 0.f;
 #pragma unroll 1
             for (int c = 0; c < BN; c += 16) {
                 if (r0 + c >= a.rows) break;
@@ -191,7 +194,7 @@ __global__ void __launch_bounds__(W8_THREADS, 2)
                 for (int i = 0; i < 16; i++) {
                     const int r = r0 + c + i;
                     if (r < a.rows && o < a.out)
-                        y[r * a.y_row + o] = Dense<T>::put(failed ? nan : w8::value(v[i], ws, __ldg(a.x_scales + r), bias));
+                        y[r * a.y_row + o] = Dense<T>::put(failed ? nan : w8::value(v[i], ws, __ldcg(a.x_scales + r), bias));
                 }
             }
         }
@@ -215,13 +218,13 @@ __global__ void __launch_bounds__(W8_THREADS, 2)
         float ws[4], bias[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            ws[j] = o + j < a.out ? __ldg(a.w_scales + o + j) : 0.f;
-            bias[j] = a.bias && o + j < a.out ? __ldg(a.bias + o + j) : 0.f;
+            ws[j] = o + j < a.out ? __ldcg(a.w_scales + o + j) : 0.f;
+            bias[j] = a.bias && o + j < a.out ? __ldcg(a.bias + o + j) : 0.f;
         }
         const bool whole = a.vec && o + 4 <= a.out && a.out % 4 == 0;
         for (int c = rank + warp * ranks; c < BN && r0 + c < a.rows; c += ranks * (W8_THREADS / 32)) {
             const int r = r0 + c;
-            const float xs = __ldg(a.x_scales + r);
+            const float xs = __ldcg(a.x_scales + r);
             int4 sum = make_int4(0, 0, 0, 0);
             for (int k = 0; k < ranks; k++) {
                 const int4 v = w8::peek4(tc::smem_addr(part + c * 128 + 4 * lane), k);
@@ -304,13 +307,13 @@ __global__ void __launch_bounds__(W8R_THREADS, w8r_resident<X, ROWS, PIECES>)
         __syncthreads();  // the sums are 0
 #pragma unroll
         for (int r = 0; r < ROWS; r++) {
-            x_scale[r] = r < a.rows ? __ldg(a.x_scales + r) : 0.f;
+            x_scale[r] = r < a.rows ? __ldcg(a.x_scales + r) : 0.f;
 #pragma unroll
             for (int p = 0; p < PIECES; p++) {
                 code[r][p] = make_int4(0, 0, 0, 0);
                 const signed char* xr = (const signed char*)x + r * x_row + at(p);
                 if (r < a.rows && at(p) + 16 <= a.in) {
-                    code[r][p] = __ldg(reinterpret_cast<const int4*>(xr));
+                    code[r][p] = __ldcg(reinterpret_cast<const int4*>(xr));
                 } else if (r < a.rows && at(p) < a.in) {  // the row ends inside the piece
                     int c[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -405,7 +408,7 @@ __global__ void __launch_bounds__(W8R_THREADS, w8r_resident<X, ROWS, PIECES>)
 #pragma unroll
     for (int r = 0; r < ROWS; r++)
         for (int i = tid; r < a.rows && i < o1 - o0; i += W8R_THREADS)
-            y[r * a.y_row + o0 + i] = Dense<T>::put(w8::value(s_sum[i * ROWS + r], __ldg(a.w_scales + o0 + i), x_scale[r], a.bias ? __ldg(a.bias + o0 + i) : 0.f));
+            y[r * a.y_row + o0 + i] = Dense<T>::put(w8::value(s_sum[i * ROWS + r], __ldcg(a.w_scales + o0 + i), x_scale[r], a.bias ? __ldcg(a.bias + o0 + i) : 0.f));
 }
 
 // ---- many rows -------------------------------------------------------------------------
@@ -574,15 +577,15 @@ __global__ void __launch_bounds__(W8_THREADS, 1)
             asm volatile("bar.sync 1, 128;" ::: "memory");
             for (int i = thread; i < W8M_N; i += 128) {
                 const int o = o0 + i;
-                s_scale[acc][i] = o < a.out ? __ldg(a.w_scales + o) : 0.f;
-                s_bias[acc][i] = a.bias && o < a.out ? __ldg(a.bias + o) : 0.f;
+                s_scale[acc][i] = o < a.out ? __ldcg(a.w_scales + o) : 0.f;
+                s_bias[acc][i] = a.bias && o < a.out ? __ldcg(a.bias + o) : 0.f;
             }
             asm volatile("bar.sync 1, 128;" ::: "memory");
             const bool ok = !failed && tc::bar_wait(&ready[acc], (local / 2) & 1, &s_abort, 2 * a.wait_ns);
             failed = !__all_sync(0xffffffffu, ok);
             tc::fence_after();
             const int r = r0 + 32 * quarter + lane;
-            const float xs = r < a.rows ? __ldg(a.x_scales + r) : 0.f;
+            const float xs = r < a.rows ? __ldcg(a.x_scales + r) : 0.f;
             T* to = y + r * a.y_row + o0;
 #pragma unroll 1
             for (int c = 0; c < W8M_N; c += 16) {

@@ -1336,3 +1336,36 @@ def test_verification_of_tiny_logits_at_tiny_temperatures(pkg, dtype):
             check_verify(pkg, logits, drafts, uniforms, list(range(0, rows + 1, nodes)), parents=[-1, 0, 0] * len(heats), heat=heats)
             check_verify(pkg, logits, drafts, uniforms, list(range(0, rows + 1, nodes)), heat=heats,
                          probs=torch.softmax(normal(g, rows, vocab), 1))
+
+
+@gpu
+def test_products_read_what_the_launch_before_has_just_written(pkg):
+    """Rows and weights that are made again and again in the same memory by the launch before a product,
+    which begins under it: nothing of the round before is read."""
+    g = gen(35)
+    k, n = 1040, 600
+    weight = torch.ones(k, device="cuda")
+    sources = [normal(g, n, k), 3 * normal(g, n, k)]
+
+    def round_of(x, w):
+        codes, scales = pkg.quantise_rows(w)
+        linear = pkg.W8Linear(codes, scales)
+        y = linear(x)  # begins under the rows' codes
+        _, c, s = pkg.residual_norm(x, x, weight, quantise=True)
+        made = [y, linear(c, scales=s)]
+        codes.copy_(pkg.quantise_rows(-w)[0])  # the same memory, for a product right behind
+        return made + [pkg.W8Linear(*pkg.quantise_rows(w[:, :256]))(c[:, :256], scales=s), linear(c, scales=s)]
+
+    for rows in (1, 2, 4, 40, 100, 300, 600):
+        xs = [normal(g, rows, k, dtype=torch.bfloat16), 5 * normal(g, rows, k, dtype=torch.bfloat16)]
+        want = []
+        for x, w in zip(xs, sources):
+            want.append([t.clone() for t in round_of(x, w)])
+            torch.cuda.synchronize()
+        got = [round_of(xs[i % 2], sources[i % 2]) for i in range(12)]
+        for i, made in enumerate(got):
+            assert all(torch.equal(a, b) for a, b in zip(want[i % 2], made))
+        for i in range(12):  # memory of the round before, freed
+            made = round_of(xs[i % 2], sources[i % 2])
+            assert all(torch.equal(a, b) for a, b in zip(want[i % 2], made))
+            del made
