@@ -52,6 +52,11 @@ void changed(const at::Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// Forward-mode derivatives are not computed either; a result could not say so later.
+void no_tangent(std::initializer_list<const at::Tensor*> from, const char* call) {
+    for (const at::Tensor* t : from)
+        if (t && t->_fw_grad(0).defined()) refuse(std::string(call) + " computes no gradient: an input has a tangent");
+}
 bool needs_gradient(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 // A result of `from` (null: not given): no gradient is computed, and a backward
 // pass that comes to it says so instead of stopping there.
@@ -311,6 +316,7 @@ PyObject* cache_attend(PyObject*, PyObject* const* args, Py_ssize_t count) {
         need(any.dim() == 3, "q must be [rows, heads, head_dim]");
         const int64_t rows = any.size(0), heads = any.size(1);
         const at::Tensor& q = rows_of(h, args[1], "q", rows, heads);
+        no_tangent({&q}, "QuantKvCache.attend");
         fb2_kvq_attention a{};
         a.dtype = code_of(q.scalar_type());
         const at::Tensor& table = tensor(args[2], "page_table");
@@ -439,6 +445,7 @@ PyObject* linear_call(PyObject*, PyObject* const* args, Py_ssize_t count) {
         const int64_t k = h.w.in_features, n = h.w.out_features;
         if (x.dim() == 0 || x.size(-1) != k || !x.is_cuda() || x.get_device() != h.index)
             refuse("x must be [..., " + std::to_string(k) + "] on cuda:" + std::to_string(h.index));
+        no_tangent({&x, h.bias.defined() ? &h.bias : nullptr}, "W4Linear");
         const int32_t code = code_of(x.scalar_type());
         at::Tensor other;
         if (x.dim() != 2) other = x.reshape({-1, k});
@@ -502,6 +509,7 @@ PyObject* controls(PyObject*, PyObject* const* args, Py_ssize_t count) {
         OnDevice on(index);
         at::Tensor fresh;
         const at::Tensor* out = args[11] == Py_None ? nullptr : &tensor(args[11], "out");
+        no_tangent({&logits, repetition, presence, frequency, values, out}, "logit_controls");
         need(!out || !(needs_gradient(logits) || needs_gradient(*out)), "out= goes without gradients: detach() or no_grad()");
         if (out)
             need(out->sizes() == logits.sizes() && out->scalar_type() == logits.scalar_type() && out->is_cuda() &&
@@ -672,6 +680,7 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t count) {
                 n.gate_row_stride = gate->stride(0);
             }
         }
+        no_tangent({h, &x, gate, w[0], w[1], w[2], w[3]}, "residual_norm");
         n.scale = (float)PyFloat_AsDouble(args[7]);
         if (PyErr_Occurred()) throw Raised{};
         n.kind = (int32_t)integer(args[8], "kind");
@@ -785,6 +794,7 @@ PyObject* quantise_rows(PyObject*, PyObject* const* args, Py_ssize_t count) {
         const at::Tensor& x = tensor(args[0], "x");
         need(x.dim() == 2 && x.is_cuda() && x.size(1) > 0, "x must be a CUDA tensor [rows, columns]");
         matrix(args[0], "x", x.size(0), x.size(1), x.get_device());
+        no_tangent({&x}, "quantise_rows");
         OnDevice on(x.get_device());
         const int32_t code = code_of(x.scalar_type());
         at::Tensor codes = empty_codes(x.size(0), x.size(1), on.index), scales = empty({x.size(0)}, at::kFloat, on.index);
@@ -814,6 +824,7 @@ PyObject* linear8_call(PyObject*, PyObject* const* args, Py_ssize_t count) {
         const int64_t rows = flat.size(0);
         const at::Tensor* given_scales = coded ? given(plain(args[2], "scales", at::kFloat, h.index), "scales") : nullptr;
         need(!coded || given_scales->numel() == rows, "scales must have one entry per row");
+        no_tangent({&x, given_scales, &h.scales, h.bias.defined() ? &h.bias : nullptr}, "W8Linear");
         c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
         shape.back() = n;
         const fb2_w8_linear l = h.now();

@@ -6,11 +6,13 @@ biases and grammar masks on logits, and the verification of drafted tokens.
 
 Every call runs the library's kernels on torch's current stream of the
 tensors' device and returns without waiting.  Results and workspaces come from
-torch's allocator (small results of one call may share an allocation).  Nothing here computes gradients: a backward pass that comes
-to the result of an input that requires one raises (out= refuses such inputs;
-what is written to a cache or packed is its values).  Wrong shapes, types or
-devices raise ArgumentError before anything is launched.  The checks and calls
-are compiled (csrc/serving_binding.cpp).
+torch's allocator (small results of one call may share an allocation).
+Nothing here computes gradients: a backward pass that comes to the result of an
+input that requires one raises (out= refuses such inputs), an input with a
+forward-mode tangent is refused; what is written to a cache or packed, and
+whole-number results, are of the values.  Wrong shapes, types or devices raise
+ArgumentError before anything is launched.  The checks and calls are compiled
+(csrc/serving_binding.cpp).
 """
 from __future__ import annotations
 

@@ -1369,3 +1369,36 @@ def test_products_read_what_the_launch_before_has_just_written(pkg):
             made = round_of(xs[i % 2], sources[i % 2])
             assert all(torch.equal(a, b) for a, b in zip(want[i % 2], made))
             del made
+
+
+@gpu
+def test_serving_operators_refuse_tangents(pkg):
+    """Forward-mode derivatives are not computed either, and do not vanish in silence."""
+    from torch.autograd import forward_ad
+    w = torch.ones(64, device="cuda")
+    plain = torch.randn((3, 64), device="cuda")
+    linear, four = pkg.W8Linear.pack(torch.randn(64, 20, device="cuda")), pkg.W4Linear.pack(torch.randn(64, 20, device="cuda"))
+    cache = pkg.QuantKvCache.empty(2, 16, 1, 64)
+    table, lens = ints([[0], [1], [1]]), ints([0, 0, 0])
+    codes, scales = pkg.quantise_rows(plain)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        x = dual(plain)
+        calls = [lambda: pkg.residual_norm(x, plain, w), lambda: pkg.residual_norm(plain, x, w), lambda: pkg.residual_norm(None, x, w),
+                 lambda: pkg.residual_norm(plain, plain, dual(w), quantise=True), lambda: pkg.residual_norm(plain, plain, w, dual(w)),
+                 lambda: pkg.residual_norm(plain, plain, w, gate=x), lambda: pkg.residual_norm(plain, plain, w, post_weight=dual(w)),
+                 lambda: linear(x), lambda: linear(codes, scales=dual(scales)),
+                 lambda: pkg.W8Linear(linear.codes, dual(linear.scales))(plain),
+                 lambda: pkg.W8Linear(linear.codes, linear.scales, dual(w[:20]))(plain), lambda: pkg.quantise_rows(x),
+                 lambda: four(x), lambda: pkg.logit_controls(x), lambda: pkg.logit_controls(x, out=plain.clone()),
+                 lambda: pkg.logit_controls(plain, out=dual(plain.clone())),
+                 lambda: cache.attend(x.view(3, 1, 64), table, lens)]
+        for call in calls:
+            with torch.no_grad(), pytest.raises(pkg.ArgumentError, match="computes no gradient"):
+                call()
+            with pytest.raises(pkg.ArgumentError, match="computes no gradient"):
+                call()
+        assert pkg.residual_norm(plain, plain, w)[1].shape == plain.shape  # none here
+        cache.write(x.view(3, 1, 64), x.view(3, 1, 64), ints([0, 1, 2]))  # (its values)
