@@ -1402,3 +1402,25 @@ def test_serving_operators_refuse_tangents(pkg):
                 call()
         assert pkg.residual_norm(plain, plain, w)[1].shape == plain.shape  # none here
         cache.write(x.view(3, 1, 64), x.view(3, 1, 64), ints([0, 1, 2]))  # (its values)
+
+
+@gpu
+def test_verification_over_the_largest_vocabulary(pkg):
+    """2^31 - 65537 ids: ends of parts come near 2^31.  Four of them have a weight, in the first and last parts."""
+    vocab = 2**31 - 1 - 65536
+    ids = [5, vocab // 2, vocab - 200000, vocab - 1]
+    row = torch.full((1, vocab), -math.inf, dtype=torch.bfloat16, device="cuda")
+    row[0, ids] = 0.0
+    with pytest.raises(pkg.ArgumentError):
+        pkg.verify_drafts(torch.empty((1, vocab + 1), dtype=torch.bfloat16, device="cuda"), ints([0]),
+                          torch.zeros(1, dtype=torch.float64, device="cuda"))
+    uniforms = torch.tensor([0.1, 0.3, 0.6, 0.9], dtype=torch.float64, device="cuda")
+    for heat in (None, torch.full((4,), 1e-20, device="cuda")):
+        tokens, _, counts = pkg.verify_drafts(row.expand(4, vocab), ints([0] * 4), uniforms, temperature=heat)
+        assert tokens.flatten().tolist() == ids and counts.eq(1).all()
+    tokens, _, _ = pkg.verify_drafts(row, ints([0]), uniforms[:1], temperature=torch.zeros(1, device="cuda"))
+    assert tokens.tolist() == [[5]]
+    drafts, starts = ints([0, ids[3], 0, ids[2]]), ints([0, 2, 4])
+    uniforms = torch.tensor([0.9, 0.2, 0.7, 0.3], dtype=torch.float64, device="cuda")
+    tokens, nodes, counts = pkg.verify_drafts(row.expand(4, vocab), drafts, uniforms, starts=starts, max_nodes=2)
+    assert counts.tolist() == [2, 1] and tokens.tolist() == [[ids[3], ids[3]], [ids[3], -1]] and nodes.tolist() == [[0, 1], [0, -1]]
