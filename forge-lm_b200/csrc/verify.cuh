@@ -84,12 +84,6 @@ FB2_DEV double peek(const double* p, int rank) {
     asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(cluster_map((uint32_t)__cvta_generic_to_shared(p), rank)) : "memory");
     return v;
 }
-FB2_DEV int peek(const int* p, int rank) {
-    int v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_map((uint32_t)__cvta_generic_to_shared(p), rank)) : "memory");
-    return v;
-}
-FB2_DEV float peek(const float* p, int rank) { return __int_as_float(peek(reinterpret_cast<const int*>(p), rank)); }
 FB2_DEV double warp_sum(double v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
