@@ -2,15 +2,19 @@
 // next block, in one pass, and rows as 8-bit codes (include/forge_b200.h,
 // fb2_residual_norm and fb2_quantise_rows, has the formulas).
 //
-// A row is held in the registers of the threads that share it, as fp32, from the
-// first load to the last store: h and x are read once, the stream and the normed
+// A row is held by the threads that share it, as fp32, from the first load to the last
+// store, in registers up to 16384 values (beyond, 1024 threads have 64 registers each for 64
+// values, and some are spilled: 2000 x 32768 bf16 172 us, fp32 228, with both norms 231 and 340,
+// where x 16384 takes 75, 100, 96 and 132): h and x are read once, the stream and the normed
 // row written once, and means and variances are taken of values at hand (the
 // variance of differences from the mean, not of squares).  All of a row's loads go out
 // before the first sum (with x behind the norm of h: 226 us instead of 137 for 16383 x
 // 4096, h bf16, x fp32, both norms).  What bounds it is HBM where there are rows enough:
 // that case moves 805 MB at 5.9 TB/s, 30000 x 1999 in fp32 6.6 TB/s; rows of 16-bit values
 // that do not begin on 16 bytes go by accesses of two bytes a lane (30000 x 1999 bf16 174
-// us, x 2000 87).  One row takes as long as a launch, its loads and its sums: 2.3 us (768),
+// us, x 2000 87).  Rows of up to 256 have a warp each, whatever their length, and are
+// bound by its instructions: 100 thousand x 256 bf16 50 us where the bytes take 31, 200 thousand x
+// 128 85, 400 thousand x 64 162, x 70 180 (their codes 27, 53, 105 and 105; bytes 12).  One row takes as long as a launch, its loads and its sums: 2.3 us (768),
 // 4.2 (8192).
 #pragma once
 #include "kvq.cuh"

@@ -343,10 +343,16 @@ void launch_rows(const fb2_w8_linear* w, const W8Args& a, const X* x, int64_t x_
 }
 
 // More than 128 rows: whether tiles of 128 x 128 whose inputs a cluster shares take less
-// than 256 x 256 by pairs of CTAs that leave most SMs without one (us, shared and not:
-// 256 x 1024 x 4096, 16 of the larger tiles, 9.6 and 9.5; 256 x 4096 x 4096, 16, 13.5 and
-// 17.4; 512 x 4096 x 4096, 32, 17.0 and 18.1; 512 x 1024 x 4096, 32, 13.6 and 9.7; 256 x 4096 x
-// 14336, 56, 26.9 and 20.6).
+// than 256 x 256 by pairs of CTAs that leave most SMs without one.  us, shared and not, of
+// rows x inputs x outputs with so many of the larger tiles:
+//   below 1024 inputs   256 x 512 x 1024, 4, 8.9 and 8.0; x 4096, 16, 9.3 and 8.3 (x 4608, 18, 9.3
+//                       and 9.8)
+//   1024 to 4095        256 x 1024 x 1024, 4, 7.6 and 9.5; x 4096, 16, 9.9 and 9.7; x 4608, 18, 9.9 and
+//                       11.3; 256 x 2048 x 4096, 16, 11.2 and 12.2; x 6144, 24, 32 and 13.3 (2048 to
+//                       4096 rows x 1024, 16: up to 10 % the other way)
+//   4096 on             256 x 4096 x 4096, 16, 13.8 and 17.4; x 9472, 37, 19.7 and 20.2; x 11008, 43, 42 and
+//                       21; 256 x 16384 x 8192, 32, 41 and 50 (256 x 5000 x 8192, 32, 29 and 22; 2048 x 4096 x
+//                       1152, 40, 17.5 and 19.2)
 bool w8_splits(int64_t tiles, int in) { return in >= 32 * W8_K ? tiles <= 37 : in >= 8 * W8_K && tiles <= 18; }
 
 std::atomic<int> g_withhold_block{-1};

@@ -17,8 +17,9 @@
 // All of them may begin while the launch before still writes what they read: rows' codes and
 // scales come by TMA or past L1 (__ldcg), behind pdl_wait, and so do the weights' scales and
 // the bias; __ldg would say that they do not change while the kernel runs.
-// Every wait is bounded (2 s); on expiry a CTA stops, waits (bounded) for its
-// copies and MMAs in flight, frees its tensor memory, and its rows of y are NaN.
+// Every wait is bounded: 2 s for a stage or an accumulator, 4 for a tile's sums (which come
+// after those); on expiry a CTA stops, waits up to 2 s more for its copies and MMAs in
+// flight, frees its tensor memory, and its rows of y are NaN.
 #pragma once
 #include <type_traits>
 
@@ -154,8 +155,9 @@ __global__ void __launch_bounds__(W8_THREADS, 2)
         tc::mma_commit(&done);
     }
     __syncwarp();
-    // all MMAs have completed, with all copies that they read; after an abort the
-    // copies in flight land before the ring is used again
+    // all MMAs have completed, with all copies that they read (warp 1 says so after its own
+    // waits, whose limit is half of this one's); after an abort the copies in flight land
+    // before the ring is used again
     bool ok = tc::bar_try(&done, 0);
     if (!ok) {
         const unsigned long long t0 = tc::now_ns();
@@ -631,7 +633,9 @@ __global__ void __launch_bounds__(W8_THREADS, 1)
 
 // W [in][out] as codes [out][in] with a scale for each output: a warp's lanes take 32
 // neighbouring outputs, 8 warps the inputs in turns; codes go through shared memory,
-// so that both sides are read and written in runs.
+// so that both sides are read and written in runs.  Once for a model's weights, and far from
+// the bytes' time, as few CTAs read W twice with a load at a time: 4096 x 14336 fp32 306 us
+// (bytes 45), bf16 355, 8192 x 28672 714 and 788.
 constexpr int W8P_THREADS = 256;
 template <class T>
 __global__ void __launch_bounds__(W8P_THREADS) k_w8_pack(const T* w, long long w_row, int in, int out, signed char* codes, long long code_row,

@@ -227,7 +227,9 @@ class PageTable:
 
     def truncate(self, lens) -> None:
         """Shortens the sequences to lens [sequences] int32 tokens (one that is
-        not longer stays as it is); pages that they no longer need are free."""
+        not longer stays as it is); pages that they no longer need are free.
+        A sequence's first tokens stay: the rows of others that are to stay (a
+        tree's accepted ones) have to be moved in the cache first."""
         self._calls.pages_truncate(self._handle, lens)
 
 
@@ -242,7 +244,8 @@ def residual_norm(h, x, weight, bias=None, *, post_weight=None, post_bias=None, 
     float32 [dim].  post_weight norms h first; gate [dim] or [rows, dim] has h's
     dtype.  x, the stream, has h's dtype or is float32.  h None: s is x, and y
     has x's dtype or `dtype`.  Computed in fp32, y from s before s is rounded; s
-    has x's dtype, y has h's."""
+    has x's dtype, y has h's.  A row's sums may be in another order in a call of
+    more (over 592) or fewer rows: the last bit, or a code, may differ."""
     _need(kind in _NORMS, "kind must be 'layer' or 'rms'")
     return (_calls or _load()).norm(h, x, weight, bias, post_weight, post_bias, gate, scale, _NORMS[kind], eps, quantise, dtype)
 
@@ -304,7 +307,10 @@ def verify_drafts(logits, drafts, uniforms, *, starts=None, parents=None, draft_
     counts [sequences] int32: tokens gained, accepted ones and the last; tokens
     [sequences, max_nodes] int32: these; nodes [sequences, max_nodes] int32: the
     row, counted from the sequence's first, that each of them follows, so the rows
-    that stay in the cache; -1 behind them.  max_nodes (up to 1024) is a host bound
-    of a sequence's rows; later ones are not looked at.  A row of logits with a NaN, a +inf
-    or nothing above -inf accepts nothing and draws -1."""
+    that stay in the cache; -1 behind them.  Of a chain these are the first rows, and
+    PageTable.truncate(prefix_lens + counts) drops the others; of a tree they may lie
+    apart, and the cache's rows nodes[b, j] have to be moved to places j before.
+    max_nodes (up to 1024) is a host bound of a sequence's rows; later ones are not looked
+    at.  A row of logits with a NaN, a +inf or nothing above -inf accepts nothing and
+    draws -1."""
     return (_calls or _load()).verify(logits, drafts, uniforms, starts, parents, draft_probs, temperature, max_nodes)

@@ -475,7 +475,9 @@ int32_t fb2_pages_extend(const fb2_pages* p, const int32_t* device_counts, int32
 /* Shortens every sequence b to lens[b] tokens (below 0: 0; a sequence that is not
  * longer stays as it is).  Pages that it no longer needs go to the end of the list,
  * the first of them last: an extend that asks for them again gets the same ones.
- * Their table entries become -1.  device_lens here may not be the pages' own. */
+ * Their table entries become -1.  device_lens here may not be the pages' own.  What stays
+ * are a sequence's first tokens: where others were accepted (of a tree), the caller moves
+ * their rows of the cache to the first places before. */
 int32_t fb2_pages_truncate(const fb2_pages* p, const int32_t* device_lens, void* cuda_stream);
 
 /* A block's output h onto the residual stream x, and the norm before what follows:
@@ -486,7 +488,11 @@ int32_t fb2_pages_truncate(const fb2_pages* p, const int32_t* device_lens, void*
  * the biases 0 where NULL.  Without h: s = x, which is not written.  In fp32 from
  * the inputs on (y is the norm of s before s is rounded); sum has x's type, y h's.
  * The result is y, or codes and scales as fb2_quantise_rows makes them of y before
- * it is rounded.  Squares of differences from the mean have to be finite in fp32.
+ * it is rounded.  Squares of differences from the mean have to be finite in fp32.  A row's
+ * result does not depend on the other rows, but the order of its sums does on how many
+ * there are (from 593 on it is another in 257 to 4096 columns) and on whether rows begin on 16
+ * bytes, which may show in the last bit or in a code: rows taken in parts need not give
+ * the bits of all at once.
  * sum, y, codes and scales share nothing with the inputs. */
 typedef enum { FB2_NORM_LAYER = 0, FB2_NORM_RMS = 1 } fb2_norm_kind;
 typedef struct {
@@ -544,8 +550,9 @@ int32_t fb2_w8_check(const fb2_w8_linear* w); /* whether the calls below take it
 int32_t fb2_w8_pack(const fb2_w8_linear* w, const void* device_w, int32_t dtype, int64_t w_row_stride, void* cuda_stream);
 /* y[r][o] = (sum_i codes[r][i] * W codes[o][i]) * W scale[o] * scales[r] + bias[o]: the sum
  * is exact, the products with the scales and the bias are fp32, rounded once to dtype.
- * codes int8 [n_rows][in] as fb2_quantise_rows writes them.  Waits inside a kernel are
- * bounded as in fb2_kvq_attend. */
+ * codes int8 [n_rows][in] as fb2_quantise_rows writes them (-128 is none of them: 128 *
+ * 127 * 131072 < 2^31).  Waits inside a kernel are bounded as in fb2_kvq_attend (4 s for a
+ * tile's sums, which come after its other waits). */
 int32_t fb2_w8_matmul(const fb2_w8_linear* w, int32_t n_rows, const void* device_codes, int64_t code_row_stride, const float* device_scales,
                       void* device_y, int64_t y_row_stride, int32_t dtype, void* cuda_stream);
 
@@ -576,7 +583,9 @@ int32_t fb2_w8_forward(const fb2_w8_linear* w, int32_t n_rows, const void* devic
  * Sums and exponentials are fp64.
  *   counts[b]: tokens that sequence b gains, accepted ones and the last (0: no rows);
  *   tokens[b][0 .. counts[b] - 1]: these; nodes[b][j]: the node that tokens[b][j] follows (nodes
- *   that stay in the cache); -1 behind them.  Nodes past max_nodes are not looked at. */
+ *   that stay in the cache); -1 behind them.  Nodes past max_nodes are not looked at.
+ * Of a chain the nodes that stay are the first counts[b]; of a tree they may lie apart, and
+ * the cache's row of node nodes[b][j] belongs in place j of the sequence's rows. */
 typedef struct {
     const void* device_logits;        /* [n_rows][vocab], rows logits_row_stride apart */
     const float* device_draft_probs;  /* [n_rows][vocab], rows probs_row_stride apart, or NULL */
