@@ -14,7 +14,8 @@
 // that do not begin on 16 bytes go by accesses of two bytes a lane (30000 x 1999 bf16 174
 // us, x 2000 87).  Rows of up to 256 have a warp each, whatever their length, and are
 // bound by its instructions: 100 thousand x 256 bf16 50 us where the bytes take 31, 200 thousand x
-// 128 85, 400 thousand x 64 162, x 70 180 (their codes 27, 53, 105 and 105; bytes 12).  One row takes as long as a launch, its loads and its sums: 2.3 us (768),
+// 128 85, 400 thousand x 64 162, x 70 180 (their codes 27, 53, 105 and 105; bytes 12).  One row
+// takes as long as a launch, its loads and its sums: 2.3 us (768),
 // 4.2 (8192).
 #pragma once
 #include "kvq.cuh"
