@@ -14,9 +14,9 @@
 // there are fewer tiles than SMs.  64 x 8192 x 28672 46 us (5.1 TB/s of weights), 61 x 1024 x
 // 4096 6.3 us, of which the products are a small part.
 // k_w8_many: 256 rows of x by 256 outputs, a pair of CTAs to a tile.
-// All of them may begin while the launch before still writes what they read: rows' codes and
-// scales come by TMA or past L1 (__ldcg), behind pdl_wait, and so do the weights' scales and
-// the bias; __ldg would say that they do not change while the kernel runs.
+// All of them may begin while the launch before still writes what they read, weights among it
+// (quantise_rows makes them too): all of it comes by TMA or by w8::late and w8::stream, which
+// stay behind pdl_wait; __ldg would say that it does not change while the kernel runs.
 // Every wait is bounded: 2 s for a stage or an accumulator, 4 for a tile's sums (which come
 // after those); on expiry a CTA stops, waits up to 2 s more for its copies and MMAs in
 // flight, frees its tensor memory, and its rows of y are NaN.
@@ -64,6 +64,22 @@ FB2_DEV void ld16(uint32_t at, int (&v)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 FB2_DEV void prefetch(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory"); }
+// Loads that no compiler moves over pdl_wait, as both are volatile: past L1; of what is read once.
+FB2_DEV float late(const float* p) {
+    float v;
+    asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p));
+    return v;
+}
+FB2_DEV int4 late(const int4* p) {
+    int4 v;
+    asm volatile("ld.global.cg.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+FB2_DEV int4 stream(const int4* p) {
+    int4 v;
+    asm volatile("ld.global.cs.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
 FB2_DEV int peek(uint32_t at, int rank) {
     uint32_t r;
     int v;
@@ -186,7 +202,7 @@ __global__ void __launch_bounds__(W8_THREADS, 2)
     if (ranks == 1) {
         if (warp < 4) {
             const int o = o0 + 32 * quarter + lane;
-            const float ws = o < a.out ? __ldcg(a.w_scales + o) : 0.f, bias = a.bias && o < a.out ? __ldcg(a.bias + o) : 0.f;
+            const float ws = o < a.out ? w8::late(a.w_scales + o) : 0.f, bias = a.bias && o < a.out ? w8::late(a.bias + o) : 0.f;
 #pragma unroll 1
             for (int c = 0; c < BN; c += 16) {
                 if (r0 + c >= a.rows) break;
@@ -196,7 +212,7 @@ __global__ void __launch_bounds__(W8_THREADS, 2)
                 for (int i = 0; i < 16; i++) {
                     const int r = r0 + c + i;
                     if (r < a.rows && o < a.out)
-                        y[r * a.y_row + o] = Dense<T>::put(failed ? nan : w8::value(v[i], ws, __ldcg(a.x_scales + r), bias));
+                        y[r * a.y_row + o] = Dense<T>::put(failed ? nan : w8::value(v[i], ws, w8::late(a.x_scales + r), bias));
                 }
             }
         }
@@ -220,13 +236,13 @@ __global__ void __launch_bounds__(W8_THREADS, 2)
         float ws[4], bias[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            ws[j] = o + j < a.out ? __ldcg(a.w_scales + o + j) : 0.f;
-            bias[j] = a.bias && o + j < a.out ? __ldcg(a.bias + o + j) : 0.f;
+            ws[j] = o + j < a.out ? w8::late(a.w_scales + o + j) : 0.f;
+            bias[j] = a.bias && o + j < a.out ? w8::late(a.bias + o + j) : 0.f;
         }
         const bool whole = a.vec && o + 4 <= a.out && a.out % 4 == 0;
         for (int c = rank + warp * ranks; c < BN && r0 + c < a.rows; c += ranks * (W8_THREADS / 32)) {
             const int r = r0 + c;
-            const float xs = __ldcg(a.x_scales + r);
+            const float xs = w8::late(a.x_scales + r);
             int4 sum = make_int4(0, 0, 0, 0);
             for (int k = 0; k < ranks; k++) {
                 const int4 v = w8::peek4(tc::smem_addr(part + c * 128 + 4 * lane), k);
@@ -292,7 +308,7 @@ __global__ void __launch_bounds__(W8R_THREADS, w8r_resident<X, ROWS, PIECES>)
     // What is behind the last row may not be memory: its last piece comes at the end.
     auto weights = [&](int o, const signed char* row, int p) {
         const bool there = at(p) < a.in && (o < a.out - 1 || at(p) + 16 <= a.in);
-        return there ? __ldcs(reinterpret_cast<const int4*>(row + at(p))) : make_int4(0, 0, 0, 0);
+        return there ? w8::stream(reinterpret_cast<const int4*>(row + at(p))) : make_int4(0, 0, 0, 0);
     };
     for (int i = tid; i < (o1 - o0) * ROWS; i += W8R_THREADS) s_sum[i] = 0;
     pdl_wait();
@@ -309,13 +325,13 @@ __global__ void __launch_bounds__(W8R_THREADS, w8r_resident<X, ROWS, PIECES>)
         __syncthreads();  // the sums are 0
 #pragma unroll
         for (int r = 0; r < ROWS; r++) {
-            x_scale[r] = r < a.rows ? __ldcg(a.x_scales + r) : 0.f;
+            x_scale[r] = r < a.rows ? w8::late(a.x_scales + r) : 0.f;
 #pragma unroll
             for (int p = 0; p < PIECES; p++) {
                 code[r][p] = make_int4(0, 0, 0, 0);
                 const signed char* xr = (const signed char*)x + r * x_row + at(p);
                 if (r < a.rows && at(p) + 16 <= a.in) {
-                    code[r][p] = __ldcg(reinterpret_cast<const int4*>(xr));
+                    code[r][p] = w8::late(reinterpret_cast<const int4*>(xr));
                 } else if (r < a.rows && at(p) < a.in) {  // the row ends inside the piece
                     int c[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -410,7 +426,7 @@ __global__ void __launch_bounds__(W8R_THREADS, w8r_resident<X, ROWS, PIECES>)
 #pragma unroll
     for (int r = 0; r < ROWS; r++)
         for (int i = tid; r < a.rows && i < o1 - o0; i += W8R_THREADS)
-            y[r * a.y_row + o0 + i] = Dense<T>::put(w8::value(s_sum[i * ROWS + r], __ldcg(a.w_scales + o0 + i), x_scale[r], a.bias ? __ldcg(a.bias + o0 + i) : 0.f));
+            y[r * a.y_row + o0 + i] = Dense<T>::put(w8::value(s_sum[i * ROWS + r], w8::late(a.w_scales + o0 + i), x_scale[r], a.bias ? w8::late(a.bias + o0 + i) : 0.f));
 }
 
 // ---- many rows -------------------------------------------------------------------------
@@ -579,15 +595,15 @@ __global__ void __launch_bounds__(W8_THREADS, 1)
             asm volatile("bar.sync 1, 128;" ::: "memory");
             for (int i = thread; i < W8M_N; i += 128) {
                 const int o = o0 + i;
-                s_scale[acc][i] = o < a.out ? __ldcg(a.w_scales + o) : 0.f;
-                s_bias[acc][i] = a.bias && o < a.out ? __ldcg(a.bias + o) : 0.f;
+                s_scale[acc][i] = o < a.out ? w8::late(a.w_scales + o) : 0.f;
+                s_bias[acc][i] = a.bias && o < a.out ? w8::late(a.bias + o) : 0.f;
             }
             asm volatile("bar.sync 1, 128;" ::: "memory");
             const bool ok = !failed && tc::bar_wait(&ready[acc], (local / 2) & 1, &s_abort, 2 * a.wait_ns);
             failed = !__all_sync(0xffffffffu, ok);
             tc::fence_after();
             const int r = r0 + 32 * quarter + lane;
-            const float xs = r < a.rows ? __ldcg(a.x_scales + r) : 0.f;
+            const float xs = r < a.rows ? w8::late(a.x_scales + r) : 0.f;
             T* to = y + r * a.y_row + o0;
 #pragma unroll 1
             for (int c = 0; c < W8M_N; c += 16) {
